@@ -169,6 +169,36 @@ int lrq_fp8_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t 
                    int bias_dtype, void* out, lrq_stream_t stream);
 
 /*
+ * FP8 products on a weight in 128x128 tiles, the layout lrq_fp8_block_quant
+ * writes with 128 x 128 blocks (vLLM's weight_scale_inv):
+ *   out[m, n] = sum_b (xs[m, b] * ws[n / 128, b]) sum_{k in block b} xc[m, k] wc[n, k] + bias[n],
+ * sums and the scales' product in float32, one rounding to out's type.  No
+ * counterpart in the reference, which leaves these products to vLLM / ATOM.
+ *   lrq_fp8_matmul: x as e4m3 codes [rows, k] (row stride ld >= k) with float32
+ *     scales [rows, ceil(k/128)], dense; out of out_dtype (bf16, fp16 or fp32).
+ *   lrq_fp8_block_linear: x of x_dtype (bf16, fp16 or fp32; row stride ld),
+ *     quantized as lrq_fp8_block_quant does with 1 x 128 blocks (float32
+ *     arithmetic); out of x's type.  `workspace`: device memory, 256-byte
+ *     aligned, of lrq_fp8_block_linear_workspace(rows, k) bytes (0 for few
+ *     tokens, which are quantized within the product), overwritten.
+ *   codes  : [n, k] e4m3 bytes, dense;  scales : [ceil(n/128), ceil(k/128)]
+ *            float32, dense;  bias : [n] of bias_dtype, or null;
+ *   out    : [rows, n], dense.
+ * Any extents and element alignment; rows of codes that are 16-byte aligned are
+ * moved fastest.  k and ld at most 2^22; rows at most 2^28, n 2^26 and rows * n
+ * 2^33.  A pair of scales whose product leaves float32's normal range loses
+ * bits, as the product does.
+ */
+int lrq_fp8_matmul(const uint8_t* x_codes, const float* x_scales, int64_t rows, int64_t k, int64_t ld,
+                   const uint8_t* codes, const float* scales, int64_t n, const void* bias, int bias_dtype,
+                   void* out, int out_dtype, lrq_stream_t stream);
+int64_t lrq_fp8_block_linear_workspace(int64_t rows, int64_t k);
+int lrq_fp8_block_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t ld,
+                         const uint8_t* codes, const float* scales, int64_t n, const void* bias,
+                         int bias_dtype, void* out, void* workspace, int64_t workspace_bytes,
+                         lrq_stream_t stream);
+
+/*
  * Unscaled cast of n contiguous elements to float8_e4m3fn, as torch's
  * `tensor.to(torch.float8_e4m3fn)`: round to nearest even, |x| rounding past
  * 448, +-inf and NaN -> NaN (0x7F | sign).  Replaces the FP8 path of

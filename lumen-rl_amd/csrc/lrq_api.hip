@@ -682,6 +682,64 @@ int lrq_fp8_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t 
   return check_hip(lrq::launch_linear(a, x_dtype, (hipStream_t)stream), "kernel launch");
 }
 
+namespace {
+// what both FP8 products on 128x128-tile weights ask of their arguments; > 0: nothing to do
+int check_matmul(const char* what, int64_t rows, int64_t k, int64_t ld, const uint8_t* codes, const float* scales, int64_t n,
+                 const void* bias, int bias_dtype, const void* x, const void* out, int out_dtype) {
+  if (!valid_dtype(out_dtype)) return fail(LRQ_ERR_ARG, "%s: bad result dtype %d", what, out_dtype);
+  if (bias && !valid_dtype(bias_dtype)) return fail(LRQ_ERR_ARG, "%s: bad bias dtype %d", what, bias_dtype);
+  if (rows < 0 || n < 0 || k < 0) return fail(LRQ_ERR_ARG, "%s: negative extent", what);
+  if (rows > lrq::kMmRowsMax || n > lrq::kMmOutMax || k > lrq::kMmPitchMax || ld > lrq::kMmPitchMax ||
+      rows * n > lrq::kMmCellsMax)
+    return fail(LRQ_ERR_ARG, "%s of %lld x %lld x %lld (pitch %lld) is too large", what, (long long)rows, (long long)n,
+                (long long)k, (long long)ld);
+  if (rows == 0 || n == 0) return 1;
+  if (k == 0 || ld < k) return fail(LRQ_ERR_ARG, "%s: ld < k, or k is 0", what);
+  if (!x || !codes || !scales || !out) return fail(LRQ_ERR_ARG, "%s: null pointer", what);
+  if (!aligned(scales, 4) || !aligned(out, (uintptr_t)esize(out_dtype)) ||
+      (bias && !aligned(bias, (uintptr_t)esize(bias_dtype))))
+    return fail(LRQ_ERR_ALIGN, "%s: scales, bias and result must be element-aligned", what);
+  return 0;
+}
+}  // namespace
+
+int lrq_fp8_matmul(const uint8_t* x_codes, const float* x_scales, int64_t rows, int64_t k, int64_t ld,
+                   const uint8_t* codes, const float* scales, int64_t n, const void* bias, int bias_dtype, void* out,
+                   int out_dtype, lrq_stream_t stream) {
+  g_err.clear();
+  const int rc = check_matmul("fp8_matmul", rows, k, ld, codes, scales, n, bias, bias_dtype, x_codes, out, out_dtype);
+  if (rc) return rc > 0 ? 0 : rc;
+  if (!x_scales) return fail(LRQ_ERR_ARG, "fp8_matmul: null pointer");
+  if (!aligned(x_scales, 4)) return fail(LRQ_ERR_ALIGN, "fp8_matmul: scales must be element-aligned");
+  const lrq::MatmulArgs a{x_codes, x_scales, codes, scales, bias, out, ld, rows, n, k, (k + 127) / 128, bias_dtype, out_dtype};
+  return check_hip(lrq::launch_matmul(a, -1, (hipStream_t)stream), "kernel launch");
+}
+
+int64_t lrq_fp8_block_linear_workspace(int64_t rows, int64_t k) {
+  if (rows <= 0 || k <= 0 || rows > lrq::kMmRowsMax || k > lrq::kMmPitchMax || lrq::matmul_quantizes(rows, k)) return 0;
+  return (rows * k + 255) / 256 * 256 + 4 * rows * ((k + 127) / 128);
+}
+
+int lrq_fp8_block_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t ld, const uint8_t* codes,
+                         const float* scales, int64_t n, const void* bias, int bias_dtype, void* out, void* workspace,
+                         int64_t workspace_bytes, lrq_stream_t stream) {
+  g_err.clear();
+  const int rc = check_matmul("fp8_block_linear", rows, k, ld, codes, scales, n, bias, bias_dtype, x, out, x_dtype);
+  if (rc) return rc > 0 ? 0 : rc;
+  if (!aligned(x, (uintptr_t)esize(x_dtype))) return fail(LRQ_ERR_ALIGN, "fp8_block_linear: x must be element-aligned");
+  lrq::MatmulArgs a{x, nullptr, codes, scales, bias, out, ld, rows, n, k, (k + 127) / 128, bias_dtype, x_dtype};
+  if (lrq::matmul_quantizes(rows, k)) return check_hip(lrq::launch_matmul(a, x_dtype, (hipStream_t)stream), "kernel launch");
+  if (workspace_bytes < lrq_fp8_block_linear_workspace(rows, k) || !workspace)
+    return fail(LRQ_ERR_CAPACITY, "fp8_block_linear: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                (long long)lrq_fp8_block_linear_workspace(rows, k));
+  if (!aligned(workspace, 256)) return fail(LRQ_ERR_ALIGN, "fp8_block_linear: workspace must be 256-byte aligned");
+  uint8_t* const x_codes = static_cast<uint8_t*>(workspace);
+  float* const x_scales = reinterpret_cast<float*>(x_codes + (rows * k + 255) / 256 * 256);
+  if (int q = lrq_fp8_block_quant(x, x_dtype, 1, rows, k, ld, rows * ld, 1, 128, x_codes, x_scales, 0, stream)) return q;
+  a.x = x_codes, a.sx = x_scales, a.ldx = k;
+  return check_hip(lrq::launch_matmul(a, -1, (hipStream_t)stream), "kernel launch");
+}
+
 int lrq_cast_e4m3(const void* in, int in_dtype, int64_t n, uint8_t* out, lrq_stream_t stream) {
   g_err.clear();
   lrq_tensor t{in, out, nullptr, 1, 1, n, n, n};

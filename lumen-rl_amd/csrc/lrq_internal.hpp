@@ -264,6 +264,27 @@ struct LinearArgs {
 };
 hipError_t launch_linear(const LinearArgs& a, int dtype, hipStream_t stream);
 
+// FP8 products on 128x128-tile weights: y [m, n] = x [m, k] w [n, k]^T + bias.
+// x: codes (row pitch ldx) with scales sx [m, kb], or, for few tokens, values of
+// a type (pitch ldx elements) that the kernel quantizes; w: dense codes with
+// scales sw [ceil(n / 128), kb]; kb = ceil(k / 128).
+constexpr int64_t kMmPitchMax = 1 << 22;  // 32-bit byte offsets within a tile of 256 rows
+constexpr int64_t kMmRowsMax = 1 << 28, kMmOutMax = 1 << 26, kMmCellsMax = int64_t(1) << 33;
+struct MatmulArgs {
+  const void* x;
+  const float* sx;
+  const uint8_t* w;
+  const float* sw;
+  const void* bias;  // null: none
+  void* y;
+  int64_t ldx, m, n, k, kb;
+  int bias_dtype, out_dtype;
+};
+// true: launch_matmul takes values of x, whatever n is
+bool matmul_quantizes(int64_t m, int64_t k);
+// x_dtype: the type of x's values, or -1: codes
+hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, hipStream_t stream);
+
 // Diagnostics: element encoders applied to raw inputs.
 hipError_t launch_diag_e4m3_bits(uint32_t start, int64_t n, uint8_t* out, hipStream_t stream);
 hipError_t launch_diag_bf16_bits(uint32_t start, int64_t n, uint16_t* out, hipStream_t stream);

@@ -8,6 +8,7 @@ from lumenrl_amd.quantization.fp8_config import (
     TrainingQuantConfig,
 )
 from lumenrl_amd.quantization.fp8_kv_cache import FP8KVCacheQuantizer
+from lumenrl_amd.quantization.fp8_product import fp8_block_linear, fp8_matmul
 from lumenrl_amd.quantization.fp8_rollout import FP8RolloutQuantizer
 from lumenrl_amd.quantization.ops import (
     CopyPlan,
@@ -38,8 +39,10 @@ __all__ = [
     "act_qdq",
     "fp8_block_dequant",
     "fp8_block_quant",
+    "fp8_block_linear",
     "fp8_e4m3_max",
     "fp8_linear",
+    "fp8_matmul",
     "quantize_fp8_blockwise",
     "quantize_mxfp4",
     "quantize_mxfp8",

@@ -1,0 +1,129 @@
+"""FP8 products on weights in 128x128 tiles.
+
+``quantize_fp8_blockwise`` writes a weight as e4m3 codes [N, K] with one float32
+scale per 128x128 tile, the layout vLLM and ATOM load as ``weight_scale_inv``.
+These are the products that consume it on this side: with activations that were
+quantized earlier (``fp8_matmul``), or quantized on the way in
+(``fp8_block_linear``).  Both return without synchronizing, on the current
+stream of the operands' device.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from lumenrl_amd import _lib
+from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _dense, _on, _prod, _stream
+
+_BLOCK = 128
+
+
+def check_tiles(what: str, codes: Tensor, scales: Tensor, device: torch.device) -> tuple[Tensor, Tensor]:
+    """``codes`` [..., N, K] and their scales [..., ceil(N/128), ceil(K/128)], both dense on ``device``."""
+    if not isinstance(codes, Tensor) or not isinstance(scales, Tensor):
+        raise TypeError(f"{what}: codes and scales must be tensors")
+    if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        raise TypeError(f"{what}: codes must be float8_e4m3fn with float32 scales, got {codes.dtype} and {scales.dtype}")
+    if codes.dim() < 2:
+        raise ValueError(f"{what}: codes must have rows and columns, got {tuple(codes.shape)}")
+    *lead, n, k = codes.shape
+    if scales.shape != (*lead, -(-n // _BLOCK), -(-k // _BLOCK)):
+        raise ValueError(f"{what}: scales {tuple(scales.shape)} are not those of 128x128 tiles of {tuple(codes.shape)}")
+    if codes.device != device or scales.device != device:
+        raise ValueError(f"{what}: codes and scales must be on {device}")
+    return (codes if codes.is_contiguous() else codes.contiguous(),
+            scales if scales.is_contiguous() else scales.contiguous())
+
+
+def _check_bias(what: str, bias: Optional[Tensor], n: int, device: torch.device) -> tuple[Optional[int], int]:
+    if bias is None:
+        return None, 0
+    if bias.shape != (n,) or bias.dtype not in _IN_DTYPES or bias.device != device or not bias.is_contiguous():
+        raise ValueError(f"{what}: bias must be a contiguous [{n}] bf16, fp16 or fp32 tensor on {device}")
+    return bias.data_ptr(), _IN_DTYPES[bias.dtype]
+
+
+def _empty_sum(rows: int, n: int, bias: Optional[Tensor], dtype: torch.dtype, device: torch.device) -> Tensor:
+    y = torch.zeros((rows, n), dtype=torch.float32, device=device)
+    return (y if bias is None else y + bias).to(dtype)
+
+
+def fp8_matmul(x_codes: Tensor, x_scales: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Tensor] = None, *,
+               out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """``x`` [M, K] times the transpose of a weight [N, K], both e4m3.
+
+    ``x_codes`` [M, K] with float32 ``x_scales`` [M, ceil(K/128)] (as
+    ``fp8_block_quant(x, (1, 128))`` gives them; rows may be a view's),
+    ``codes`` [N, K] with float32 ``scales`` [ceil(N/128), ceil(K/128)] ->
+    [M, N] of ``out_dtype`` (bfloat16, float16 or float32), sums in float32.
+    """
+    if not isinstance(x_codes, Tensor) or not x_codes.is_cuda:
+        raise ValueError("fp8_matmul: expected codes on a HIP device")
+    if x_codes.dtype != torch.float8_e4m3fn or x_scales.dtype != torch.float32:
+        raise TypeError(f"fp8_matmul: x must be float8_e4m3fn with float32 scales, got {x_codes.dtype} and {x_scales.dtype}")
+    if out_dtype not in _IN_DTYPES:
+        raise ValueError(f"fp8_matmul: out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
+    dev = x_codes.device
+    codes, scales = check_tiles("fp8_matmul", codes, scales, dev)
+    if x_codes.dim() != 2 or codes.dim() != 2 or x_codes.shape[1] != codes.shape[1]:
+        raise ValueError(f"fp8_matmul: x {tuple(x_codes.shape)} and codes {tuple(codes.shape)} do not fit")
+    m, k = x_codes.shape
+    n = codes.shape[0]
+    if x_scales.shape != (m, -(-k // _BLOCK)) or x_scales.device != dev:
+        raise ValueError(f"fp8_matmul: x's scales must be {(m, -(-k // _BLOCK))} on {dev}, got {tuple(x_scales.shape)}")
+    bias_ptr, bias_dtype = _check_bias("fp8_matmul", bias, n, dev)
+    if k == 0:
+        return _empty_sum(m, n, bias, out_dtype, dev)
+    ld = x_codes.stride(0) if m > 1 else k
+    if (k > 1 and x_codes.stride(1) != 1) or ld < k:
+        x_codes, ld = x_codes.contiguous(), k
+    if not x_scales.is_contiguous():
+        x_scales = x_scales.contiguous()
+    out = _dense((m, n), out_dtype, dev)
+    with _on(dev):
+        rc = _lib.lib().lrq_fp8_matmul(x_codes.data_ptr(), x_scales.data_ptr(), m, k, ld, codes.data_ptr(), scales.data_ptr(),
+                                       n, bias_ptr, bias_dtype, out.data_ptr(), _IN_DTYPES[out_dtype], _stream(dev))
+    if rc:
+        _lib.check(rc, "lrq_fp8_matmul")
+    return out
+
+
+def fp8_block_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Tensor] = None) -> Tensor:
+    """A linear layer in FP8: ``x`` [..., K] is quantized to e4m3 in 1x128 blocks
+    (as ``fp8_block_quant(x, (1, 128))``) and multiplied with ``codes`` [N, K]
+    and float32 ``scales`` [ceil(N/128), ceil(K/128)] -> [..., N] in x's dtype.
+
+    Up to 16 tokens take one launch, more take two.
+    """
+    _check_input(x, "fp8_block_linear")
+    dev = x.device
+    codes, scales = check_tiles("fp8_block_linear", codes, scales, dev)
+    if x.dim() < 1 or codes.dim() != 2 or x.shape[-1] != codes.shape[1]:
+        raise ValueError(f"fp8_block_linear: x {tuple(x.shape)} and codes {tuple(codes.shape)} do not fit")
+    n, k = codes.shape
+    lead = x.shape[:-1]
+    bias_ptr, bias_dtype = _check_bias("fp8_block_linear", bias, n, dev)
+    if k == 0:
+        return _empty_sum(_prod(lead), n, bias, x.dtype, dev).view(*lead, n)
+    if x.dim() == 2 and x.is_contiguous():
+        rows, ld = x.shape[0], k
+    else:
+        rows = x.numel() // k
+        x = x.reshape(rows, k)
+        ld = x.stride(0) if rows > 1 else k
+        if (k > 1 and x.stride(1) != 1) or ld < k:
+            x, ld = x.contiguous(), k
+    out = _dense((*lead, n), x.dtype, dev)
+    L = _lib.lib()
+    need = L.lrq_fp8_block_linear_workspace(rows, k)
+    work = _dense((need,), torch.uint8, dev) if need else None
+    with _on(dev):
+        rc = L.lrq_fp8_block_linear(x.data_ptr(), _IN_DTYPES[x.dtype], rows, k, ld, codes.data_ptr(), scales.data_ptr(), n,
+                                    bias_ptr, bias_dtype, out.data_ptr(), work.data_ptr() if need else None, need,
+                                    _stream(dev))
+    if rc:
+        _lib.check(rc, "lrq_fp8_block_linear")
+    return out

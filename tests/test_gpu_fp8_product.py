@@ -1,0 +1,157 @@
+"""``fp8_matmul`` and ``fp8_block_linear`` against float64 products of the same codes and scales."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from lumenrl_amd.quantization import fp8_block_linear, fp8_block_quant, fp8_matmul, quantize_fp8_blockwise
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def weight(n, k, seed=0):
+    """Every code but the NaNs, scales over two binades."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    codes = torch.randint(0, 256, (n, k), generator=g, device=DEV, dtype=torch.uint8)
+    codes[(codes & 0x7F) == 0x7F] = 0x30
+    scales = (torch.rand(-(-n // 128), -(-k // 128), generator=g, device=DEV) * 3 + 1) * 1e-4
+    return codes.view(torch.float8_e4m3fn), scales
+
+
+def acts(m, k, dtype, seed=1):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(m, k, generator=g, device=DEV)
+    x[:, k // 3] *= 40.0
+    return x.to(dtype)
+
+
+def spread(scales, rows, cols, block=(128, 128)):
+    s = scales.double()
+    return s.repeat_interleave(block[0], 0)[:rows].repeat_interleave(block[1], 1)[:, :cols]
+
+
+def check(y, x_codes, x_scales, codes, scales, bias=None):
+    """|y - exact| within the result's rounding and the sums' own bound.
+
+    A block sums 128 exact products in float32, K/128 blocks and 8 waves' parts follow, each step off by at most
+    2^-23 of the terms' magnitude, and the product of the two scales by 2^-24.  16-bit results of more than 64
+    tokens come from matrix instructions that drop what is 2^-13 below the block's largest product: 128 times
+    that for each block."""
+    (m, k), n = x_codes.shape, codes.shape[0]
+    xd = x_codes.double() * spread(x_scales, m, k, (1, 128))
+    wd = codes.double() * spread(scales, n, k)
+    want, size = xd @ wd.T, xd.abs() @ wd.abs().T
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    half = torch.finfo(y.dtype).eps / 2
+    least = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24, torch.float32: 2.0 ** -149}[y.dtype]
+    bound = half * want.abs() * 1.01 + (128 + k // 128 + 12) * 2.0 ** -23 * size + least
+    if m > 64 and y.dtype != torch.float32:
+        for b in range(0, k, 128):
+            top = xd[:, b: b + 128].abs().amax(1)[:, None] * wd[:, b: b + 128].abs().amax(1)[None]
+            bound += 128 * 2.0 ** -13 * top
+    off = (y.double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())
+
+
+# tokens of each kernel (few: up to 16, 32, 64; tiles of three sizes), weights cut in every way
+SHAPES = [(1, 1, 1), (1, 4096, 4096), (3, 200, 130), (16, 130, 1104), (16, 64, 12288), (17, 129, 384), (33, 1, 1100), (64, 300, 272),
+          (65, 127, 15), (65, 128, 128), (100, 130, 144), (777, 1500, 1100), (2000, 2040, 1040), (1999, 2041, 1041), (4100, 3850, 272)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_matmul_vs_float64(m, n, k, dtype):
+    x_codes, x_scales = fp8_block_quant(acts(m, k, torch.bfloat16, m), (1, 128))
+    codes, scales = weight(n, k, n + k)
+    bias = torch.randn(n, device=DEV).to(TYPES[n % 3]) if m % 2 else None
+    y = fp8_matmul(x_codes, x_scales, codes, scales, bias, out_dtype=dtype)
+    assert y.shape == (m, n) and y.dtype == dtype
+    check(y, x_codes, x_scales, codes, scales, bias)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_linear_is_the_product_of_the_quantized_activations(m, n, k, dtype):
+    x = acts(m, k, dtype, m + 7)
+    codes, scales = weight(n, k, n + k + 1)
+    y = fp8_block_linear(x, codes, scales)
+    x_codes, x_scales = fp8_block_quant(x, (1, 128))
+    check(y, x_codes, x_scales, codes, scales)
+
+
+def test_weights_as_the_framework_quantizes_them():
+    w = torch.randn(520, 1000, device=DEV, dtype=torch.bfloat16) * 0.02
+    codes, scales = quantize_fp8_blockwise(w)
+    x = acts(40, 1000, torch.bfloat16)
+    check(fp8_block_linear(x, codes, scales), *fp8_block_quant(x, (1, 128)), codes, scales)
+
+
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_strides_leading_dims_and_alignment(m):
+    n, k = 270, 400
+    codes, scales = weight(n, k)
+    big = acts(m, 3 * k + 7, torch.bfloat16)
+    for x in (big[:, 5: 5 + k], big[:, 16: 16 + k], big[:, : 2 * k: 2], big.t()[:k].t()):
+        check(fp8_block_linear(x, codes, scales), *fp8_block_quant(x, (1, 128)), codes, scales)
+    x = acts(2 * m, k, torch.float16).view(2, m, k)
+    y = fp8_block_linear(x, codes, scales)
+    assert y.shape == (2, m, n)
+    check(y.view(-1, n), *fp8_block_quant(x.view(-1, k), (1, 128)), codes, scales)
+    # codes whose rows are a view's, off their 16-byte boundaries, and a weight that is a transpose
+    xc, xs = fp8_block_quant(acts(m, k, torch.bfloat16), (1, 128))
+    wide = torch.zeros(m, 3 * k + 5, dtype=torch.uint8, device=DEV)
+    for at in (0, 3, 16):
+        wide[:, at: at + k] = xc.view(torch.uint8)
+        view = wide.view(torch.float8_e4m3fn)[:, at: at + k]
+        check(fp8_matmul(view, xs, codes, scales, out_dtype=torch.float32), xc, xs, codes, scales)
+    turned = codes.view(torch.uint8).t().contiguous().t().view(torch.float8_e4m3fn)
+    check(fp8_matmul(xc, xs, turned, scales, out_dtype=torch.float32), xc, xs, codes, scales)
+    shifted = torch.zeros(n * k + 1, dtype=torch.uint8, device=DEV)[1:].view(n, k).copy_(codes.view(torch.uint8))
+    check(fp8_matmul(xc, xs, shifted.view(torch.float8_e4m3fn), scales, out_dtype=torch.float32), xc, xs, codes, scales)
+
+
+@pytest.mark.parametrize("m", [4, 30, 200])
+def test_nan_inf_and_zero_rows_stay_in_their_rows(m):
+    n, k = 150, 300
+    codes, scales = weight(n, k)
+    x = acts(m, k, torch.bfloat16)
+    x[0, 7], x[1, 290], x[2] = float("nan"), float("-inf"), 0.0
+    y = fp8_block_linear(x, codes, scales)
+    assert bool(y[:2].isnan().all()) and bool((y[2] == 0).all())
+    rest = x[3:]
+    check(y[3:], *fp8_block_quant(rest, (1, 128)), codes, scales)
+
+
+def test_empty_extents():
+    codes, scales = weight(64, 256)
+    assert fp8_block_linear(torch.zeros(0, 256, device=DEV), codes, scales).shape == (0, 64)
+    assert fp8_block_linear(torch.zeros(2, 0, 256, device=DEV), codes, scales).shape == (2, 0, 64)
+    assert fp8_block_linear(torch.zeros(5, 256, device=DEV), codes[:0], scales[:0]).shape == (5, 0)
+    none = torch.empty(64, 0, dtype=torch.float8_e4m3fn, device=DEV)
+    b = torch.randn(64, device=DEV)
+    y = fp8_block_linear(torch.zeros(3, 0, device=DEV), none, torch.empty(1, 0, device=DEV), b)
+    assert torch.equal(y, b.expand(3, 64))
+
+
+def test_other_stream_and_graph():
+    codes, scales = weight(512, 640)
+    for m in (3, 50, 500):
+        x = acts(m, 640, torch.bfloat16)
+        want = fp8_block_linear(x, codes, scales)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = fp8_block_linear(x, codes, scales)
+        side.synchronize()
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = fp8_block_linear(x, codes, scales)
+        for seed in range(3):
+            x.copy_(acts(m, 640, torch.bfloat16, seed))
+            graph.replay()
+            assert torch.equal(y, fp8_block_linear(x, codes, scales))
