@@ -199,6 +199,28 @@ int lrq_fp8_block_linear(const void* x, int x_dtype, int64_t rows, int64_t k, in
                          lrq_stream_t stream);
 
 /*
+ * Routing to experts: each token's top_k of `experts` (1..512), and their weights.
+ *   score = softmax or sigmoid of the logits; pick = score + bias (bias: [experts]
+ *   float32 or null); with groups > 1 (at most 16 equal runs of experts) only the
+ *   top_groups groups with the highest sum of their group_top (1 or 2) highest
+ *   picks are open.  ids: the top_k (at most 64) highest picks, highest first, ties
+ *   to the lowest index, as exact arithmetic orders them; NaN counts as highest.
+ *   weights: scale * score[id], divided by the chosen scores' sum (plus 1e-20 for
+ *   sigmoid) if `renormalize`.  float32 [tokens, top_k] and int32 [tokens, top_k].
+ * lrq_route_grad: out = the logits' gradient [tokens, experts], of their type, from
+ *   the weights' gradient `grad` [tokens, top_k] and the ids that lrq_route gave.
+ * No counterpart in the reference, which leaves routing to vLLM / ATOM and the
+ * trainer's model code.
+ */
+enum { LRQ_SCORE_SOFTMAX = 0, LRQ_SCORE_SIGMOID = 1 };
+int lrq_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, const float* bias,
+              int top_k, int score, int groups, int top_groups, int group_top, int renormalize, float scale,
+              float* weights, int32_t* ids, lrq_stream_t stream);
+int lrq_route_grad(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, const int32_t* ids,
+                   const float* grad, int top_k, int score, int renormalize, float scale, void* out,
+                   lrq_stream_t stream);
+
+/*
  * Unscaled cast of n contiguous elements to float8_e4m3fn, as torch's
  * `tensor.to(torch.float8_e4m3fn)`: round to nearest even, |x| rounding past
  * 448, +-inf and NaN -> NaN (0x7F | sign).  Replaces the FP8 path of

@@ -740,6 +740,59 @@ int lrq_fp8_block_linear(const void* x, int x_dtype, int64_t rows, int64_t k, in
   return check_hip(lrq::launch_matmul(a, -1, (hipStream_t)stream), "kernel launch");
 }
 
+namespace {
+int check_route(const char* what, int dtype, int64_t tokens, int64_t experts, int64_t ld, const void* logits, int top_k, int score,
+                const void* ids) {
+  if (!valid_dtype(dtype)) return fail(LRQ_ERR_ARG, "%s: bad logits dtype %d", what, dtype);
+  if (score != LRQ_SCORE_SOFTMAX && score != LRQ_SCORE_SIGMOID) return fail(LRQ_ERR_ARG, "%s: bad score %d", what, score);
+  if (experts < 1 || experts > lrq::kRouteExpertsMax)
+    return fail(LRQ_ERR_ARG, "%s: %lld experts, 1 to %d are routed to", what, (long long)experts, lrq::kRouteExpertsMax);
+  if (top_k < 1 || top_k > lrq::kRouteMost || top_k > experts)
+    return fail(LRQ_ERR_ARG, "%s: top_k %d of %lld experts (%d at most)", what, top_k, (long long)experts, lrq::kRouteMost);
+  if (tokens < 0 || tokens > int64_t(1) << 31 || ld > int64_t(1) << 31)
+    return fail(LRQ_ERR_ARG, "%s of %lld tokens (pitch %lld)", what, (long long)tokens, (long long)ld);
+  if (tokens == 0) return 1;
+  if (ld < experts) return fail(LRQ_ERR_ARG, "%s: ld < experts", what);
+  if (!logits || !ids) return fail(LRQ_ERR_ARG, "%s: null pointer", what);
+  if (!aligned(logits, (uintptr_t)esize(dtype)) || !aligned(ids, 4))
+    return fail(LRQ_ERR_ALIGN, "%s: operands must be element-aligned", what);
+  return 0;
+}
+}  // namespace
+
+int lrq_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, const float* bias, int top_k, int score,
+              int groups, int top_groups, int group_top, int renormalize, float scale, float* weights, int32_t* ids,
+              lrq_stream_t stream) {
+  g_err.clear();
+  const int rc = check_route("route", dtype, tokens, experts, ld, logits, top_k, score, ids);
+  if (rc < 0) return rc;
+  if (groups < 1 || groups > lrq::kRouteGroupsMax || experts % groups != 0)
+    return fail(LRQ_ERR_ARG, "route: %d groups of %lld experts (they divide them, %d at most)", groups, (long long)experts,
+                lrq::kRouteGroupsMax);
+  if (top_groups < 1 || top_groups > groups || top_k > experts / groups * top_groups)
+    return fail(LRQ_ERR_ARG, "route: top_k %d from %d of %d groups", top_k, top_groups, groups);
+  if (group_top != 1 && group_top != 2) return fail(LRQ_ERR_ARG, "route: group_top must be 1 or 2, got %d", group_top);
+  if (rc > 0) return 0;
+  if (!weights) return fail(LRQ_ERR_ARG, "route: null pointer");
+  if (!aligned(weights, 4) || !aligned(bias, 4)) return fail(LRQ_ERR_ALIGN, "route: operands must be element-aligned");
+  const lrq::RouteArgs a{logits, bias, weights, ids, tokens, ld, (int)experts, top_k, groups, top_groups, group_top,
+                         score == LRQ_SCORE_SIGMOID, renormalize != 0, scale};
+  return check_hip(lrq::launch_route(a, dtype, nullptr, nullptr, (hipStream_t)stream), "kernel launch");
+}
+
+int lrq_route_grad(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, const int32_t* ids,
+                   const float* grad, int top_k, int score, int renormalize, float scale, void* out, lrq_stream_t stream) {
+  g_err.clear();
+  const int rc = check_route("route_grad", dtype, tokens, experts, ld, logits, top_k, score, ids);
+  if (rc) return rc > 0 ? 0 : rc;
+  if (!grad || !out) return fail(LRQ_ERR_ARG, "route_grad: null pointer");
+  if (!aligned(grad, 4) || !aligned(out, (uintptr_t)esize(dtype)))
+    return fail(LRQ_ERR_ALIGN, "route_grad: operands must be element-aligned");
+  const lrq::RouteArgs a{logits, nullptr, nullptr, const_cast<int32_t*>(ids), tokens, ld, (int)experts, top_k, 1, 1, 1,
+                         score == LRQ_SCORE_SIGMOID, renormalize != 0, scale};
+  return check_hip(lrq::launch_route(a, dtype, grad, out, (hipStream_t)stream), "kernel launch");
+}
+
 int lrq_cast_e4m3(const void* in, int in_dtype, int64_t n, uint8_t* out, lrq_stream_t stream) {
   g_err.clear();
   lrq_tensor t{in, out, nullptr, 1, 1, n, n, n};

@@ -285,6 +285,25 @@ bool matmul_quantizes(int64_t m, int64_t k);
 // x_dtype: the type of x's values, or -1: codes
 hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, hipStream_t stream);
 
+// Routing to experts (lrq_route.hip).
+constexpr int kRouteExpertsMax = 512, kRouteGroupsMax = 16;  // one lane of 16 looks through a group
+constexpr int kRouteMost = 64;       // top_k: four a lane
+constexpr int kRoutePitch = kRouteMost + 2;
+constexpr float kRouteTol = 0x1p-18f;  // picks nearer than this (relative to 1 + |pick|) are compared in float64: four
+                                       // times what float32 scores and sums are off by at most
+struct RouteArgs {
+  const void* logits;  // [tokens, experts], row pitch ld
+  const float* bias;   // null: none
+  float* weights;      // [tokens, top_k]
+  int32_t* ids;
+  int64_t tokens, ld;
+  int experts, top_k, groups, top_groups, group_top;
+  bool sigmoid, renormalize;
+  float scale;
+};
+// out null: the choice and its weights; otherwise the logits' gradient, from ids and the weights' gradient
+hipError_t launch_route(const RouteArgs& a, int dtype, const float* grad, void* out, hipStream_t stream);
+
 // Diagnostics: element encoders applied to raw inputs.
 hipError_t launch_diag_e4m3_bits(uint32_t start, int64_t n, uint8_t* out, hipStream_t stream);
 hipError_t launch_diag_bf16_bits(uint32_t start, int64_t n, uint16_t* out, hipStream_t stream);

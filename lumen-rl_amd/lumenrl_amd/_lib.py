@@ -17,6 +17,7 @@ DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_F64 = 0, 1, 2, 3
 FLAG_POW2_SCALE, FLAG_NATIVE_ARITH, FLAG_SCALE_BF16, FLAG_OUT_BF16 = 1, 2, 4, 8
 FMT_FP8_BLOCK, FMT_MXFP8, FMT_MXFP4, FMT_FP8_DEQUANT, FMT_TENSOR_SCALE, FMT_COPY = 0, 1, 2, 3, 4, 5
 FMT_CAST_E4M3, FMT_MXFP8_DEQUANT, FMT_MXFP4_DEQUANT = 6, 7, 8
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 ERR_ARG, ERR_ALIGN, ERR_CAPACITY, ERR_TABLE = -1, -2, -3, -4
 STATIC_WORKSPACE_BYTES = 4 << 20  # LRQ_STATIC_WORKSPACE_BYTES
 UPLOAD_TENSORS = 32  # LRQ_UPLOAD_TENSORS
@@ -53,6 +54,8 @@ SIGNATURES = {
     "lrq_fp8_matmul": (_CI, [_VP, _VP, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _CI, _VP, _CI, _VP]),
     "lrq_fp8_block_linear_workspace": (_I64, [_I64, _I64]),
     "lrq_fp8_block_linear": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _CI, _VP, _VP, _I64, _VP]),
+    "lrq_route": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _CI, _CI, _CI, _CI, _CI, _CI, ctypes.c_float, _VP, _VP, _VP]),
+    "lrq_route_grad": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _CI, _CI, _CI, ctypes.c_float, _VP, _VP]),
     "lrq_cast_e4m3": (_CI, [_VP, _CI, _I64, _VP, _VP]),
     "lrq_mx_dequant": (_CI, [_CI, _VP, _VP, _I64, _I64, _VP, _CI, _VP]),
     "lrq_group_table_bytes": (_I64, [_CI, ctypes.POINTER(LrqTensor), _I64, _CI, _I64, _I64, _CU]),

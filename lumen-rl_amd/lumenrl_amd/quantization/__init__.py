@@ -1,6 +1,7 @@
 """Weight quantization for trainer -> rollout weight sync (lumenrl/quantization mirror)."""
 
 from lumenrl_amd.quantization.bucket import QuantizedBucketWriter, encode_bucket
+from lumenrl_amd.quantization.experts import route_experts
 from lumenrl_amd.quantization.fp8_config import (
     FP8Config,
     QuantizationConfig,
@@ -46,4 +47,5 @@ __all__ = [
     "quantize_fp8_blockwise",
     "quantize_mxfp4",
     "quantize_mxfp8",
+    "route_experts",
 ]

@@ -1,0 +1,113 @@
+"""Mixture-of-experts operators: the router, and the experts on FP8 weights.
+
+``route_experts`` turns a router's logits into each token's experts and their
+weights, with the gradient of the logits.  Every function launches on the
+current stream of its operands' device and returns without synchronizing.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from lumenrl_amd import _lib
+from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _dense, _on, _stream
+
+_SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+
+
+def _rows(x: Tensor) -> tuple[Tensor, int, int]:
+    """``x`` [..., E] as rows of unit stride: (tensor, rows, row pitch); a copy only where it has to be."""
+    e = x.shape[-1]
+    if x.is_contiguous():
+        return x, x.numel() // e, e
+    rows = x.numel() // e
+    x = x.reshape(rows, e)
+    ld = x.stride(0) if rows > 1 else e
+    if (e > 1 and x.stride(1) != 1) or ld < e:
+        return x.contiguous(), rows, e
+    return x, rows, ld
+
+
+def _route(logits: Tensor, bias: Optional[Tensor], cfg: tuple) -> tuple[Tensor, Tensor]:
+    top_k, score, groups, top_groups, group_top, renormalize, scale = cfg
+    dev = logits.device
+    shape = (*logits.shape[:-1], top_k)
+    e = logits.shape[-1]
+    x, rows, ld = _rows(logits)
+    weights, ids = _dense(shape, torch.float32, dev), _dense(shape, torch.int32, dev)
+    with _on(dev):
+        rc = _lib.lib().lrq_route(x.data_ptr(), _IN_DTYPES[x.dtype], rows, e, ld, bias.data_ptr() if bias is not None else None,
+                                  top_k, score, groups, top_groups, group_top, renormalize, scale, weights.data_ptr(),
+                                  ids.data_ptr(), _stream(dev))
+    if rc:
+        _lib.check(rc, "lrq_route")
+    return weights, ids
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, cfg):
+        weights, ids = _route(logits, bias, cfg)
+        ctx.save_for_backward(logits, ids)
+        ctx.cfg = cfg
+        ctx.mark_non_differentiable(ids)
+        return weights, ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        logits, ids = ctx.saved_tensors
+        top_k, score, _groups, _top_groups, _group_top, renormalize, scale = ctx.cfg
+        dev = logits.device
+        grad = grad.contiguous()
+        x, rows, ld = _rows(logits)
+        out = _dense(tuple(logits.shape), logits.dtype, dev)
+        with _on(dev):
+            rc = _lib.lib().lrq_route_grad(x.data_ptr(), _IN_DTYPES[x.dtype], rows, logits.shape[-1], ld, ids.data_ptr(),
+                                           grad.data_ptr(), top_k, score, renormalize, scale, out.data_ptr(), _stream(dev))
+        if rc:
+            _lib.check(rc, "lrq_route_grad")
+        return out, None, None
+
+
+def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Optional[Tensor] = None, groups: int = 1,
+                  top_groups: int = 1, group_top: int = 1, renormalize: bool = True, scale: float = 1.0
+                  ) -> tuple[Tensor, Tensor]:
+    """Each token's experts: ``logits`` [..., E] -> (weights float32 [..., top_k], ids int32 [..., top_k]).
+
+    Experts are chosen by their score (``"softmax"`` or ``"sigmoid"`` of the logits)
+    plus ``bias`` [E] (float32; for balance: it moves the choice, not the weights,
+    and takes no gradient), highest first, ties to the lowest index.  With
+    ``groups`` > 1 only the ``top_groups`` runs of E / groups experts with the highest
+    sum of their ``group_top`` (1 or 2) best are open.  Weights are the scores times
+    ``scale``, divided by the chosen scores' sum if ``renormalize``.
+
+    The choice is that of exact arithmetic; a NaN counts as the highest.  E is at
+    most 512, ``top_k`` 64, ``groups`` 16.  The weights carry the gradient of the
+    logits (once; not its own gradient).
+    """
+    _check_input(logits, "route_experts")
+    if score not in _SCORES:
+        raise ValueError(f"route_experts: score must be 'softmax' or 'sigmoid', got {score!r}")
+    if logits.dim() < 1:
+        raise ValueError("route_experts: logits must have a dimension of experts")
+    e = logits.shape[-1]
+    if bias is not None:
+        if not isinstance(bias, Tensor) or bias.dtype != torch.float32:
+            raise TypeError("route_experts: bias must be a float32 tensor")
+        if bias.shape != (e,) or bias.device != logits.device:
+            raise ValueError(f"route_experts: bias must be [{e}] on {logits.device}, got {tuple(bias.shape)} on {bias.device}")
+        bias = bias.detach().contiguous()
+    if not 1 <= e <= 512 or not 1 <= top_k <= min(e, 64):
+        raise ValueError(f"route_experts: top_k {top_k} of {e} experts (at most 64 of 512)")
+    if not 1 <= groups <= 16 or e % groups or not 1 <= top_groups <= groups or top_k > e // groups * top_groups:
+        raise ValueError(f"route_experts: top_k {top_k} of {e} experts in {top_groups} of {groups} groups (at most 16)")
+    if group_top not in (1, 2):
+        raise ValueError(f"route_experts: group_top must be 1 or 2, got {group_top}")
+    cfg = (top_k, _SCORES[score], groups, top_groups, group_top, int(renormalize), scale)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Route.apply(logits, bias, cfg)
+    return _route(logits, bias, cfg)
