@@ -221,6 +221,27 @@ int lrq_route_grad(const void* logits, int dtype, int64_t tokens, int64_t expert
                    lrq_stream_t stream);
 
 /*
+ * The chosen experts' SwiGLU MLPs on weights in 128x128 tiles, and their sum:
+ *   out[t] = sum_j weights[t, j] * down_e(silu(gate_e(x_t)) * up_e(x_t)), e = ids[t, j],
+ * x and the hidden values quantized to e4m3 in 1x128 blocks (as lrq_fp8_block_quant
+ * with float32 arithmetic), everything else float32, one rounding to x's type (bf16
+ * or fp16).  A pair whose id is outside 0 .. experts - 1 is left out.
+ *   x : [tokens, hidden], row stride ld;  ids, weights : [tokens, top_k], dense;
+ *   gate_up : [experts, 2 inter, hidden] codes, gate's rows first, with float32
+ *   scales [experts, ceil(2 inter / 128), ceil(hidden / 128)];
+ *   down : [experts, hidden, inter], scales [experts, ceil(hidden / 128), ceil(inter / 128)];
+ *   out : [tokens, hidden], dense.  Codes and out 16-byte aligned.
+ * hidden and inter: multiples of 16, 2 hidden inter < 2^31; experts at most 1024,
+ * top_k 64.  `workspace`: lrq_fp8_experts_workspace bytes of device memory, 256-byte
+ * aligned, overwritten.  No counterpart in the reference (vLLM / ATOM run these).
+ */
+int64_t lrq_fp8_experts_workspace(int64_t tokens, int64_t hidden, int64_t inter, int64_t experts, int64_t top_k);
+int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, int64_t ld, const int32_t* ids,
+                    const float* weights, int64_t top_k, const uint8_t* gate_up, const float* gate_up_scales,
+                    const uint8_t* down, const float* down_scales, int64_t experts, int64_t inter, void* out,
+                    void* workspace, int64_t workspace_bytes, lrq_stream_t stream);
+
+/*
  * Unscaled cast of n contiguous elements to float8_e4m3fn, as torch's
  * `tensor.to(torch.float8_e4m3fn)`: round to nearest even, |x| rounding past
  * 448, +-inf and NaN -> NaN (0x7F | sign).  Replaces the FP8 path of

@@ -793,6 +793,62 @@ int lrq_route_grad(const void* logits, int dtype, int64_t tokens, int64_t expert
   return check_hip(lrq::launch_route(a, dtype, grad, out, (hipStream_t)stream), "kernel launch");
 }
 
+namespace {
+// the sizes of an expert MLP; > 0: nothing to do
+int check_experts(int64_t tokens, int64_t hidden, int64_t inter, int64_t experts, int64_t top_k) {
+  if (tokens < 0 || tokens > int64_t(1) << 28) return fail(LRQ_ERR_ARG, "fp8_experts of %lld tokens", (long long)tokens);
+  if (experts < 1 || experts > lrq::kExpertsMax)
+    return fail(LRQ_ERR_ARG, "fp8_experts: %lld experts (1 to %d)", (long long)experts, lrq::kExpertsMax);
+  if (top_k < 1 || top_k > lrq::kRouteMost)
+    return fail(LRQ_ERR_ARG, "fp8_experts: top_k %lld (1 to %d)", (long long)top_k, lrq::kRouteMost);
+  if (hidden < 16 || inter < 16 || hidden % 16 || inter % 16 || hidden > 1 << 16 || inter > 1 << 16 ||
+      2 * hidden * inter >= int64_t(1) << 31)
+    return fail(LRQ_ERR_ARG, "fp8_experts: hidden %lld and intermediate %lld must be multiples of 16, 2 x hidden x intermediate below 2^31",
+                (long long)hidden, (long long)inter);
+  return tokens == 0;
+}
+lrq::ExpertArgs expert_sizes(int64_t hidden, int64_t inter, int64_t experts, int64_t top_k) {
+  lrq::ExpertArgs a{};
+  a.experts = (int)experts, a.hidden = (int)hidden, a.inter = (int)inter, a.top_k = (int)top_k;
+  a.kb = (int)(hidden + 127) / 128, a.ib = (int)(inter + 127) / 128, a.gb = (int)(2 * inter + 127) / 128;
+  return a;
+}
+hipError_t quantize_tokens(const lrq::ExpertArgs& a, int dtype, hipStream_t stream) {
+  return lrq_fp8_block_quant(a.x, dtype, 1, a.tokens, a.hidden, a.ldx, a.tokens * a.ldx, 1, 128, a.xq, a.xs, 0, stream)
+             ? hipErrorInvalidValue
+             : hipSuccess;
+}
+}  // namespace
+
+int64_t lrq_fp8_experts_workspace(int64_t tokens, int64_t hidden, int64_t inter, int64_t experts, int64_t top_k) {
+  if (check_experts(tokens, hidden, inter, experts, top_k)) return 0;
+  return lrq::experts_workspace(tokens, expert_sizes(hidden, inter, experts, top_k));
+}
+
+int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, int64_t ld, const int32_t* ids,
+                    const float* weights, int64_t top_k, const uint8_t* gate_up, const float* gate_up_scales,
+                    const uint8_t* down, const float* down_scales, int64_t experts, int64_t inter, void* out,
+                    void* workspace, int64_t workspace_bytes, lrq_stream_t stream) {
+  g_err.clear();
+  if (x_dtype != lrq::kBF16 && x_dtype != lrq::kF16) return fail(LRQ_ERR_ARG, "fp8_experts: bad activation dtype %d", x_dtype);
+  const int rc = check_experts(tokens, hidden, inter, experts, top_k);
+  if (rc) return rc > 0 ? 0 : rc;
+  if (ld < hidden || ld > int64_t(1) << 31) return fail(LRQ_ERR_ARG, "fp8_experts: ld < hidden, or too large");
+  if (!x || !ids || !weights || !gate_up || !gate_up_scales || !down || !down_scales || !out)
+    return fail(LRQ_ERR_ARG, "fp8_experts: null pointer");
+  if (!aligned(x, 2) || !aligned(ids, 4) || !aligned(weights, 4) || !aligned(gate_up_scales, 4) || !aligned(down_scales, 4) ||
+      !aligned(gate_up, 16) || !aligned(down, 16) || !aligned(out, 16))
+    return fail(LRQ_ERR_ALIGN, "fp8_experts: operands must be element-aligned, codes and result 16-byte aligned");
+  lrq::ExpertArgs a = expert_sizes(hidden, inter, experts, top_k);
+  const int64_t need = lrq::experts_workspace(tokens, a);
+  if (!workspace || workspace_bytes < need)
+    return fail(LRQ_ERR_CAPACITY, "fp8_experts: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  if (!aligned(workspace, 256)) return fail(LRQ_ERR_ALIGN, "fp8_experts: workspace must be 256-byte aligned");
+  a.x = x, a.ldx = ld, a.ids = ids, a.weights = weights, a.gu = gate_up, a.gus = gate_up_scales, a.dn = down, a.dns = down_scales;
+  a.out = out;
+  return check_hip(lrq::launch_experts(a, x_dtype, tokens, workspace, quantize_tokens, (hipStream_t)stream), "kernel launch");
+}
+
 int lrq_cast_e4m3(const void* in, int in_dtype, int64_t n, uint8_t* out, lrq_stream_t stream) {
   g_err.clear();
   lrq_tensor t{in, out, nullptr, 1, 1, n, n, n};

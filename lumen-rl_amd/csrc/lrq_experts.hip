@@ -1,0 +1,518 @@
+// The experts' MLPs on FP8 weights in 128x128 tiles.  For a pair of a token t and
+// one of its experts e,
+//   g, u = x_q Wgu[e]^T (two halves), h = g / (1 + exp(-g)) u, y = h_q Wd[e]^T,
+//   out[t] = sum over the token's pairs of weight y,
+// with x and h quantized to e4m3 in 1x128 blocks.  Everything between is float32;
+// out is rounded once.  lrq_mma8.hpp has the products' mathematics.
+//
+// Few pairs: two launches, a pair by itself (its expert's weights are all that
+// moves).  More: pairs are sorted by expert, and an expert's rows go through tiles
+// whose gate and up rows meet in one wave; h leaves the first product quantized.
+#include "lrq.h"
+#include "lrq_device.hpp"
+#include "lrq_internal.hpp"
+#include "lrq_mma8.hpp"
+
+namespace lrq {
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+// ---------------------------------------------------------------------------
+// Pairs sorted by expert
+// ---------------------------------------------------------------------------
+// One work-group: counts, the experts' runs and their tiles of `bm` rows, then each
+// pair's place.  Pairs of an expert come in any order, which no result depends on.
+// Ids outside 0 .. experts - 1 have no place.
+constexpr int kSortThreads = 1024;
+__global__ __launch_bounds__(kSortThreads) void k_ex_sort(const int32_t* ids, int pairs, int experts, int bm, ExpertTile* tiles,
+                                                          int32_t* total, int32_t* order) {
+  __shared__ int32_t count[kExpertsMax], start[kExpertsMax + 1], part[2][kSortThreads];
+  const int tid = threadIdx.x;
+  for (int e = tid; e < experts; e += kSortThreads) count[e] = 0;
+  __syncthreads();
+  for (int p = tid; p < pairs; p += kSortThreads) {
+    const uint32_t e = (uint32_t)gld<int32_t>(ids + p);
+    if (e < (uint32_t)experts) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  // one expert a thread: sums of rows and of tiles before it
+  const int mine = tid < experts ? count[tid] : 0, my_tiles = (mine + bm - 1) / bm;
+  part[0][tid] = mine, part[1][tid] = my_tiles;
+  __syncthreads();
+  for (int off = 1; off < kSortThreads; off *= 2) {
+    const int a = tid >= off ? part[0][tid - off] : 0, b = tid >= off ? part[1][tid - off] : 0;
+    __syncthreads();
+    part[0][tid] += a, part[1][tid] += b;
+    __syncthreads();
+  }
+  const int first = part[0][tid] - mine, tile = part[1][tid] - my_tiles;
+  if (tid < experts) start[tid] = first;
+  if (tid == kSortThreads - 1) gst<int32_t>(total, part[1][tid]);
+  for (int i = 0; i < my_tiles; ++i) {
+    const int rows = mine - i * bm < bm ? mine - i * bm : bm;
+    tiles[tile + i] = ExpertTile{tid, first + i * bm, rows, 0};
+  }
+  __syncthreads();
+  for (int p = tid; p < pairs; p += kSortThreads) {
+    const uint32_t e = (uint32_t)gld<int32_t>(ids + p);
+    if (e < (uint32_t)experts) gst<int32_t>(order + atomicAdd(&start[e], 1), p);
+  }
+}
+
+// Work-group wg of a grid for `total` tiles by nb: each XCD (wg % 8) takes one run,
+// a tile's nb pieces after one another, so that it reads an expert's weights once.
+__device__ __forceinline__ bool expert_piece(int wg, int total, int nb, int& tile, int& n) {
+  const int all = total * nb, per = (all + 7) >> 3;
+  const int t = (wg & 7) * per + (wg >> 3);
+  if ((wg >> 3) >= per || t >= all) return false;
+  tile = t / nb, n = t % nb;
+  return true;
+}
+
+// h [rows, 128] of a work-group whose WN waves hold 16 NS columns each: lane (c, g)
+// has columns 16 i + 4 g .. + 3 of rows 16 j + c.  Quantized and stored.
+template <int NS, int FM, int WN>
+__device__ __forceinline__ void store_hidden(const ExpertArgs& a, f32x4 (&h)[NS][FM], int first, int row0, int rows, int block, int wn,
+                                             uint32_t* amax, int bm) {
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t v = f2u(h[i][j][r]) & 0x7FFFFFFFu;
+        m = v > m ? v : m;
+      }
+    uint32_t o = (uint32_t)__shfl_xor((int)m, 16, 64);
+    m = o > m ? o : m;
+    o = (uint32_t)__shfl_xor((int)m, 32, 64);
+    m = o > m ? o : m;
+    if (g == 0) amax[wn * bm + row0 + 16 * j + c] = m;
+  }
+  lds_barrier8();
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    const int row = row0 + 16 * j + c;
+    uint32_t m = amax[row];
+#pragma unroll
+    for (int w = 1; w < WN; ++w) {
+      const uint32_t o = amax[w * bm + row];
+      m = o > m ? o : m;
+    }
+    const BlockScale b = block_scale<kF32>(m, false);
+    if (row >= rows) continue;
+    const int64_t at = first + row;
+    if (wn == 0 && g == 0) gst<float>(a.hs + at * a.ib + block, b.s);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int n = 128 * block + 16 * (NS * wn + i) + 4 * g;
+      if (n >= a.inter) continue;
+      uint32_t q;
+      if (b.kind >= kScaleInf) {
+        q = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) q |= special_code<kF32>(h[i][j][r], b) << (8 * r);
+      } else {
+        q = cvt_e4m3x4(block_quot<kF32>(h[i][j][0], b), block_quot<kF32>(h[i][j][1], b), block_quot<kF32>(h[i][j][2], b),
+                       block_quot<kF32>(h[i][j][3], b));
+      }
+      gst<uint32_t>(a.hq + at * a.inter + n, q);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Some rows an expert: weights from memory into registers
+// ---------------------------------------------------------------------------
+// A work-group of 8 waves takes a tile of 16 MT pairs and 128 columns of h (or of
+// out), a wave 16 of them over the whole of K.
+struct UpRows {
+  const ExpertArgs& a;
+  const ExpertTile& t;
+  int n, c;
+  const uint8_t* wb;
+  const float* sb;
+  __device__ int row(int j) const { const int r = 16 * j + c; return r < t.rows ? r : t.rows - 1; }
+  __device__ int64_t token(int j) const { return gld<int32_t>(a.order + t.first + row(j)) / a.top_k; }
+  __device__ const uint8_t* w(int i) const { return wb + (int64_t)(i * a.inter + n + c) * a.hidden; }
+  __device__ const float* sw(int i) const { return sb + (int64_t)((i * a.inter + n) / kBlk) * a.kb; }
+  __device__ const uint8_t* x(int j) const { return a.xq + token(j) * a.hidden; }
+  __device__ const float* sx(int j) const { return a.xs + token(j) * a.kb; }
+};
+
+template <int MT>
+__global__ __launch_bounds__(512) void k_ex_up_rows(ExpertArgs a) {
+  __shared__ uint32_t amax[8 * 16 * MT];
+  int tile, block;
+  if (!expert_piece(blockIdx.x, gld<int32_t>(a.total), a.ib, tile, block)) return;
+  const ExpertTile t = a.tiles[tile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = 128 * block + 16 * wave;
+  f32x4 h[1][MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) h[0][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (n < a.inter) {
+    const UpRows src{a, t, n, lane & 15, a.gu + (int64_t)t.expert * 2 * a.inter * a.hidden, a.gus + (int64_t)t.expert * a.gb * a.kb};
+    f32x4 acc[2][MT];
+    row_sums<2, MT, 2, false, true>(src, 0, a.kb, a.hidden, acc, [] {});
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) h[0][j][r] = silu_mul(acc[0][j][r], acc[1][j][r]);
+  }
+  store_hidden<1, MT, 8>(a, h, t.first, 0, t.rows, block, wave, amax, 16 * MT);
+}
+
+struct DownRows {
+  const ExpertArgs& a;
+  const ExpertTile& t;
+  int n, c;
+  const uint8_t* wb;
+  const float* sb;
+  __device__ int row(int j) const { const int r = 16 * j + c; return r < t.rows ? r : t.rows - 1; }
+  __device__ const uint8_t* w(int) const { return wb + (int64_t)(n + c) * a.inter; }
+  __device__ const float* sw(int) const { return sb + (int64_t)(n / kBlk) * a.ib; }
+  __device__ const uint8_t* x(int j) const { return a.hq + (int64_t)(t.first + row(j)) * a.inter; }
+  __device__ const float* sx(int j) const { return a.hs + (int64_t)(t.first + row(j)) * a.ib; }
+};
+
+template <int MT>
+__global__ __launch_bounds__(512) void k_ex_down_rows(ExpertArgs a) {
+  int tile, block;
+  if (!expert_piece(blockIdx.x, gld<int32_t>(a.total), a.kb, tile, block)) return;
+  const ExpertTile t = a.tiles[tile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4, n = 128 * block + 16 * wave;
+  if (n >= a.hidden) return;
+  const DownRows src{a, t, n, c, a.dn + (int64_t)t.expert * a.hidden * a.inter, a.dns + (int64_t)t.expert * a.kb * a.ib};
+  f32x4 acc[1][MT];
+  row_sums<1, MT, 2, false, true>(src, 0, a.ib, a.inter, acc, [] {});
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    if (16 * j + c >= t.rows) continue;
+    const int pair = gld<int32_t>(a.order + t.first + 16 * j + c);
+    const float w = gld<float>(a.weights + pair);
+    gst<f32x4>(a.y + (int64_t)pair * a.hidden + n + 4 * g, f32x4{acc[0][j][0] * w, acc[0][j][1] * w, acc[0][j][2] * w, acc[0][j][3] * w});
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows an expert: tiles through LDS
+// ---------------------------------------------------------------------------
+// Weight rows of a tile: 16 of gate, the same 16 of up, and so on.
+struct UpTile {
+  const ExpertArgs& a;
+  const ExpertTile& t;
+  int block, wn;  // wn: the wave's first tile row
+  __device__ const uint8_t* w() const { return a.gu + (int64_t)t.expert * 2 * a.inter * a.hidden; }
+  __device__ const uint8_t* x() const { return a.xq; }
+  __device__ uint32_t w_bytes() const { return (uint32_t)(2 * a.inter * a.hidden); }
+  __device__ uint32_t x_bytes() const { return (uint32_t)(a.tokens * a.hidden); }
+  __device__ int column(int r) const { return 128 * block + 16 * (r >> 5) + (r & 15); }
+  __device__ uint32_t w_off(int r) const {
+    const int n = column(r);
+    return n < a.inter ? (uint32_t)((r >> 4 & 1 ? a.inter : 0) + n) * (uint32_t)a.hidden : kNoRow;
+  }
+  __device__ int token(int r) const { return gld<int32_t>(a.order + t.first + (r < t.rows ? r : t.rows - 1)) / a.top_k; }
+  __device__ uint32_t x_off(int r) const { return r < t.rows ? (uint32_t)token(r) * (uint32_t)a.hidden : kNoRow; }
+  __device__ const float* sx(int r) const { return a.xs + (int64_t)token(r) * a.kb; }
+  __device__ const float* sw(int i) const {
+    const int r = wn + 16 * i, n = column(r) < a.inter ? column(r) : a.inter - 1;
+    return a.gus + ((int64_t)t.expert * a.gb + ((r >> 4 & 1 ? a.inter : 0) + n) / kBlk) * a.kb;
+  }
+};
+
+template <int FN, int FM, int WN, int WM>
+__global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
+  static_assert(16 * FN * WN == 256, "128 columns of h");
+  constexpr int BM = 16 * FM * WM;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kTileStage<FN, FM, WN, WM>];
+  int tile, block;
+  if (!expert_piece(blockIdx.x, gld<int32_t>(a.total), a.ib, tile, block)) return;
+  const ExpertTile t = a.tiles[tile];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const UpTile src{a, t, block, wave / WM * 16 * FN};
+  f32x4 acc[FN][FM], h[FN / 2][FM];
+  tile_sums<FN, FM, WN, WM, true, true, false>(src, a.hidden, lds, acc);
+#pragma unroll
+  for (int i = 0; i < FN / 2; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) h[i][j][r] = silu_mul(acc[2 * i][j][r], acc[2 * i + 1][j][r]);
+  store_hidden<FN / 2, FM, WN>(a, h, t.first, wave % WM * 16 * FM, t.rows, block, wave / WM, reinterpret_cast<uint32_t*>(lds), BM);
+}
+
+struct DownTile {
+  const ExpertArgs& a;
+  const ExpertTile& t;
+  int n0, wn;
+  __device__ const uint8_t* w() const { return a.dn + (int64_t)t.expert * a.hidden * a.inter; }
+  __device__ const uint8_t* x() const { return a.hq + (int64_t)t.first * a.inter; }
+  __device__ uint32_t w_bytes() const { return (uint32_t)(a.hidden * a.inter); }
+  __device__ uint32_t x_bytes() const { return (uint32_t)(t.rows * a.inter); }
+  __device__ uint32_t w_off(int r) const { return n0 + r < a.hidden ? (uint32_t)(n0 + r) * (uint32_t)a.inter : kNoRow; }
+  __device__ uint32_t x_off(int r) const { return r < t.rows ? (uint32_t)r * (uint32_t)a.inter : kNoRow; }
+  __device__ const float* sx(int r) const { return a.hs + (int64_t)(t.first + (r < t.rows ? r : t.rows - 1)) * a.ib; }
+  __device__ const float* sw(int) const {
+    const int n = n0 + wn < a.hidden ? n0 + wn : a.hidden - 1;
+    return a.dns + ((int64_t)t.expert * a.kb + n / kBlk) * a.ib;
+  }
+};
+
+template <int FN, int FM, int WN, int WM>
+__global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_down_tiles(ExpertArgs a) {
+  constexpr int BN = 16 * FN * WN;
+  static_assert(16 * FN <= kBlk, "one scale for a wave's rows");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kTileStage<FN, FM, WN, WM>];
+  int tile, block;
+  if (!expert_piece(blockIdx.x, gld<int32_t>(a.total), (a.hidden + BN - 1) / BN, tile, block)) return;
+  const ExpertTile t = a.tiles[tile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4, wn = wave / WM * 16 * FN, wm = wave % WM * 16 * FM;
+  const DownTile src{a, t, block * BN, wn};
+  f32x4 acc[FN][FM];
+  tile_sums<FN, FM, WN, WM, true, false, false>(src, a.inter, lds, acc);
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    const int row = wm + 16 * j + c;
+    if (row >= t.rows) continue;
+    const int pair = gld<int32_t>(a.order + t.first + row);
+    const float w = gld<float>(a.weights + pair);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const int n = src.n0 + wn + 16 * i + 4 * g;
+      if (n < a.hidden)
+        gst<f32x4>(a.y + (int64_t)pair * a.hidden + n, f32x4{acc[i][j][0] * w, acc[i][j][1] * w, acc[i][j][2] * w, acc[i][j][3] * w});
+    }
+  }
+}
+
+// out[t] = the sum of the token's rows of y, in the order of its pairs.
+template <int DT>
+__global__ __launch_bounds__(256) void k_ex_sum(ExpertArgs a) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (at >= a.tokens * a.hidden) return;
+  const int64_t t = at / a.hidden, n = at % a.hidden;
+  float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int j = 0; j < a.top_k; ++j) {
+    if ((uint32_t)gld<int32_t>(a.ids + t * a.top_k + j) >= (uint32_t)a.experts) continue;
+    const float* y = a.y + (t * a.top_k + j) * a.hidden + n;
+    const f32x4 lo = gld<f32x4>(y), hi = gld<f32x4>(y + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] += lo[i], s[4 + i] += hi[i];
+  }
+  uint32_t b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i] = bits16<DT>(s[i]);
+  *(LRQ_GLOBAL v4u_any*)(static_cast<uint16_t*>(a.out) + at) = v4u{b[0] | b[1] << 16, b[2] | b[3] << 16, b[4] | b[5] << 16, b[6] | b[7] << 16};
+}
+
+// ---------------------------------------------------------------------------
+// Few pairs
+// ---------------------------------------------------------------------------
+// h of a pair and 16 columns: x is quantized by every work-group, K is split over
+// its 8 waves.
+struct OneRow {
+  const uint8_t* w0;   // lane's row of weight strip 0
+  int64_t w_step;      // bytes to strip 1's
+  const float *s0, *s1;
+  const uint8_t* codes;
+  const float* scales;
+  int at;
+  __device__ const uint8_t* w(int i) const { return w0 + i * w_step; }
+  __device__ const float* sw(int i) const { return i ? s1 : s0; }
+  __device__ const uint8_t* x(int) const { return nullptr; }
+  __device__ const float* sx(int) const { return nullptr; }
+  __device__ Codes32 block(int, int kb) const {
+    const uint8_t* p = codes + kb * kBlk + at;
+    return {*reinterpret_cast<const v4u*>(p), *reinterpret_cast<const v4u*>(p + 64)};
+  }
+  __device__ float scale(int, int kb) const { return scales[kb]; }
+};
+
+template <int DT>
+__global__ __launch_bounds__(512) void k_ex_up_few(ExpertArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int pair = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int expert = gld<int32_t>(a.ids + pair);
+  if ((uint32_t)expert >= (uint32_t)a.experts) return;
+  const int c = lane & 15, g = lane >> 4, n = 16 * blockIdx.x;
+  uint8_t* const codes = lds;
+  float* const scales = reinterpret_cast<float*>(lds + a.kb * kBlk);
+  const uint8_t* const gu = a.gu + (int64_t)expert * 2 * a.inter * a.hidden;
+  const float* const gus = a.gus + (int64_t)expert * a.gb * a.kb;
+  const OneRow src{gu + (int64_t)(n + c) * a.hidden, (int64_t)a.inter * a.hidden, gus + (int64_t)(n / kBlk) * a.kb,
+                   gus + (int64_t)((a.inter + n) / kBlk) * a.kb, codes, scales, 16 * g};
+  const int steps = (a.kb + 7) / 8, kb0 = wave * steps, kb1 = kb0 + steps < a.kb ? kb0 + steps : a.kb;
+  f32x4 acc[2][1];
+  row_sums<2, 1, 2, true, true>(src, kb0, kb1, a.hidden, acc, [&] {
+    const void* const x = static_cast<const uint8_t*>(a.x) + (int64_t)(pair / a.top_k) * a.ldx * 2;
+    for (int b = tid >> 4; b < a.kb; b += 32) {
+      float v[8], s;
+      load_acts<DT>(x, b * kBlk + 8 * (tid & 15), a.hidden, v);
+      *reinterpret_cast<v2u*>(codes + b * kBlk + 8 * (tid & 15)) = quant8(v, s);
+      if ((tid & 15) == 0) scales[b] = s;
+    }
+    lds_barrier8();
+  });
+  lds_barrier8();
+  float* const red = reinterpret_cast<float*>(lds);  // [wave][gate, up][row]
+  if (c == 0) {
+    *reinterpret_cast<f32x4*>(red + wave * 32 + 4 * g) = acc[0][0];
+    *reinterpret_cast<f32x4*>(red + wave * 32 + 16 + 4 * g) = acc[1][0];
+  }
+  lds_barrier8();
+  if (tid < 16) {
+    float gate = 0.0f, up = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) gate += red[w * 32 + tid], up += red[w * 32 + 16 + tid];
+    gst<float>(a.y + (int64_t)pair * a.inter + n + tid, silu_mul(gate, up));
+  }
+}
+
+// 16 columns of a token's output: its pairs' h are quantized by every work-group;
+// its 8 waves take the pairs, or parts of their K.
+template <int DT>
+__global__ __launch_bounds__(512) void k_ex_down_few(ExpertArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int t = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4, n = 16 * blockIdx.x, blocks = a.top_k * a.ib;
+  uint8_t* const codes = lds;
+  float* const scales = reinterpret_cast<float*>(lds + blocks * kBlk);
+  for (int b = tid >> 4; b < blocks; b += 32) {
+    float v[8], s;
+    const int j = b / a.ib, kb = b % a.ib;
+    load_acts<kF32>(a.y + ((int64_t)t * a.top_k + j) * a.inter, kb * kBlk + 8 * (tid & 15), a.inter, v);
+    *reinterpret_cast<v2u*>(codes + b * kBlk + 8 * (tid & 15)) = quant8(v, s);
+    if ((tid & 15) == 0) scales[b] = s;
+  }
+  lds_barrier8();
+  const int parts = a.top_k >= 8 ? 1 : 8 / a.top_k, step = (a.ib + parts - 1) / parts;
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int u = wave; u < a.top_k * parts; u += 8) {
+    const int j = u / parts, kb0 = u % parts * step, kb1 = kb0 + step < a.ib ? kb0 + step : a.ib;
+    const int expert = gld<int32_t>(a.ids + (int64_t)t * a.top_k + j);
+    if ((uint32_t)expert >= (uint32_t)a.experts || kb0 >= kb1) continue;
+    const float* const s = a.dns + ((int64_t)expert * a.kb + n / kBlk) * a.ib;
+    const OneRow src{a.dn + ((int64_t)expert * a.hidden + n + c) * a.inter, 0, s, s, codes + j * a.ib * kBlk, scales + j * a.ib, 16 * g};
+    f32x4 acc[1][1];
+    row_sums<1, 1, 4, true, true>(src, kb0, kb1, a.inter, acc, [] {});
+    const float w = gld<float>(a.weights + (int64_t)t * a.top_k + j);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum[r] = __builtin_fmaf(acc[0][0][r], w, sum[r]);
+  }
+  lds_barrier8();
+  float* const red = reinterpret_cast<float*>(lds);
+  if (c == 0) *reinterpret_cast<f32x4*>(red + wave * 16 + 4 * g) = sum;
+  lds_barrier8();
+  if (tid < 16) {
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += red[w * 16 + tid];
+    gst<uint16_t>(static_cast<uint16_t*>(a.out) + (int64_t)t * a.hidden + n + tid, bits16<DT>(v));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Which kernels, and their memory
+// ---------------------------------------------------------------------------
+static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// Rows of a tile: 0 for few pairs.
+static int expert_rows(int64_t tokens, const ExpertArgs& a) {
+  const int64_t pairs = tokens * a.top_k, few_lds = (int64_t)a.top_k * a.ib * (kBlk + 4);
+  if (pairs <= 64 && pairs <= a.experts && few_lds <= 48 * 1024 && a.kb * (kBlk + 4) <= 48 * 1024) return 0;
+  const int64_t each = pairs / a.experts;
+  return each < 16 ? 16 : each < 48 ? 32 : 128;
+}
+// Tokens of a pass: 32-bit offsets into the codes of x, and 1 GiB of y.
+static int64_t expert_pass(int64_t tokens, const ExpertArgs& a) {
+  int64_t most = (int64_t(1) << 28) / ((int64_t)a.top_k * a.hidden);
+  most = most < 1 ? 1 : most;
+  return tokens < most ? tokens : most;
+}
+static int64_t tile_bound(int64_t pairs, int bm, int experts) {
+  return (pairs + bm - 1) / bm + (pairs < experts ? pairs : experts);
+}
+
+static int64_t expert_layout(int64_t tokens, int bm, ExpertArgs& a, uint8_t* base) {
+  const int64_t pairs = tokens * a.top_k;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) { uint8_t* p = base + at; at += up256(bytes); return p; };
+  if (bm == 0) {
+    a.y = reinterpret_cast<float*>(take(4 * pairs * a.inter));
+    return at;
+  }
+  a.xq = take(tokens * a.hidden);
+  a.xs = reinterpret_cast<float*>(take(4 * tokens * a.kb));
+  a.order = reinterpret_cast<int32_t*>(take(4 * pairs));
+  a.total = reinterpret_cast<int32_t*>(take(4));
+  a.tiles = reinterpret_cast<ExpertTile*>(take((int64_t)sizeof(ExpertTile) * tile_bound(pairs, bm, a.experts)));
+  a.hq = take(pairs * a.inter);
+  a.hs = reinterpret_cast<float*>(take(4 * pairs * a.ib));
+  a.y = reinterpret_cast<float*>(take(4 * pairs * a.hidden));
+  return at;
+}
+
+int64_t experts_workspace(int64_t tokens, ExpertArgs a) {
+  const int64_t pass = expert_pass(tokens, a);
+  int64_t most = expert_layout(pass, expert_rows(pass, a), a, nullptr);
+  if (tokens % pass) {  // the last pass can be laid out otherwise
+    const int64_t last = expert_layout(tokens % pass, expert_rows(tokens % pass, a), a, nullptr);
+    most = last > most ? last : most;
+  }
+  return most;
+}
+
+template <int DT>
+static hipError_t few(const ExpertArgs& a, hipStream_t stream) {
+  const unsigned up = (unsigned)(a.kb * (kBlk + 4)), down = (unsigned)(a.top_k * a.ib * (kBlk + 4));
+  hipLaunchKernelGGL((k_ex_up_few<DT>), dim3((unsigned)(a.inter / 16), (unsigned)(a.tokens * a.top_k)), dim3(512), up < 1024 ? 1024 : up, stream, a);
+  hipLaunchKernelGGL((k_ex_down_few<DT>), dim3((unsigned)(a.hidden / 16), (unsigned)a.tokens), dim3(512), down < 512 ? 512 : down, stream, a);
+  return hipGetLastError();
+}
+
+template <int MT>
+static void by_rows(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
+  hipLaunchKernelGGL((k_ex_up_rows<MT>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(512), 0, stream, a);
+  hipLaunchKernelGGL((k_ex_down_rows<MT>), dim3((unsigned)((tiles * a.kb + 7) / 8 * 8)), dim3(512), 0, stream, a);
+}
+
+hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspace, ExpertQuant quant, hipStream_t stream) {
+  const int64_t pass = expert_pass(tokens, a);
+  const uint8_t* const x = static_cast<const uint8_t*>(a.x);
+  const int32_t* const ids = a.ids;
+  const float* const weights = a.weights;
+  uint8_t* const out = static_cast<uint8_t*>(a.out);
+  for (int64_t t0 = 0; t0 < tokens; t0 += pass) {
+    a.tokens = tokens - t0 < pass ? tokens - t0 : pass;
+    a.x = x + 2 * t0 * a.ldx, a.ids = ids + t0 * a.top_k, a.weights = weights + t0 * a.top_k, a.out = out + 2 * t0 * a.hidden;
+    const int bm = expert_rows(a.tokens, a);
+    expert_layout(a.tokens, bm, a, static_cast<uint8_t*>(workspace));
+    if (bm == 0) {
+      if (hipError_t e = dtype == kBF16 ? few<kBF16>(a, stream) : few<kF16>(a, stream)) return e;
+      continue;
+    }
+    const int64_t pairs = a.tokens * a.top_k, tiles = tile_bound(pairs, bm, a.experts);
+    if (hipError_t e = quant(a, dtype, stream)) return e;
+    hipLaunchKernelGGL(k_ex_sort, dim3(1), dim3(kSortThreads), 0, stream, a.ids, (int)pairs, a.experts, bm, a.tiles, a.total, a.order);
+    if (bm == 16) {
+      by_rows<1>(a, tiles, stream);
+    } else if (bm == 32) {
+      by_rows<2>(a, tiles, stream);
+    } else {
+      hipLaunchKernelGGL((k_ex_up_tiles<4, 4, 4, 2>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(512), 0, stream, a);
+      hipLaunchKernelGGL((k_ex_down_tiles<4, 4, 2, 2>), dim3((unsigned)((tiles * ((a.hidden + 127) / 128) + 7) / 8 * 8)), dim3(256), 0, stream, a);
+    }
+    const dim3 sum((unsigned)((a.tokens * a.hidden / 8 + 255) / 256));
+    if (dtype == kBF16) hipLaunchKernelGGL((k_ex_sum<kBF16>), sum, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((k_ex_sum<kF16>), sum, dim3(256), 0, stream, a);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace lrq

@@ -304,6 +304,31 @@ struct RouteArgs {
 // out null: the choice and its weights; otherwise the logits' gradient, from ids and the weights' gradient
 hipError_t launch_route(const RouteArgs& a, int dtype, const float* grad, void* out, hipStream_t stream);
 
+// The experts' MLPs on FP8 weights (lrq_experts.hip).
+constexpr int kExpertsMax = 1024;  // one thread of the sort each
+struct ExpertTile {
+  int32_t expert, first, rows, unused;  // rows of the sorted pairs from `first` on
+};
+struct ExpertArgs {
+  const void* x;  // [tokens, hidden], row pitch ldx
+  const int32_t* ids;
+  const float* weights;  // [tokens, top_k]
+  const uint8_t *gu, *dn;   // [experts, 2 inter, hidden], [experts, hidden, inter]
+  const float *gus, *dns;   // [experts, gb, kb], [experts, kb, ib]
+  void* out;
+  int64_t ldx, tokens;
+  int experts, hidden, inter, top_k;
+  int kb, ib, gb;  // ceil(hidden / 128), ceil(inter / 128), ceil(2 inter / 128)
+  // workspace: x and h in codes, the pairs' order, tiles of it and their number, and the pairs' results
+  uint8_t *xq, *hq;
+  float *xs, *hs, *y;
+  int32_t *order, *total;
+  ExpertTile* tiles;
+};
+typedef hipError_t (*ExpertQuant)(const ExpertArgs& a, int dtype, hipStream_t stream);  // x -> xq, xs
+int64_t experts_workspace(int64_t tokens, ExpertArgs a);
+hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspace, ExpertQuant quant, hipStream_t stream);
+
 // Diagnostics: element encoders applied to raw inputs.
 hipError_t launch_diag_e4m3_bits(uint32_t start, int64_t n, uint8_t* out, hipStream_t stream);
 hipError_t launch_diag_bf16_bits(uint32_t start, int64_t n, uint16_t* out, hipStream_t stream);

@@ -56,6 +56,8 @@ SIGNATURES = {
     "lrq_fp8_block_linear": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _CI, _VP, _VP, _I64, _VP]),
     "lrq_route": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _CI, _CI, _CI, _CI, _CI, _CI, ctypes.c_float, _VP, _VP, _VP]),
     "lrq_route_grad": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _CI, _CI, _CI, ctypes.c_float, _VP, _VP]),
+    "lrq_fp8_experts_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64]),
+    "lrq_fp8_experts": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _VP, _VP, _VP, _I64, _I64, _VP, _VP, _I64, _VP]),
     "lrq_cast_e4m3": (_CI, [_VP, _CI, _I64, _VP, _VP]),
     "lrq_mx_dequant": (_CI, [_CI, _VP, _VP, _I64, _I64, _VP, _CI, _VP]),
     "lrq_group_table_bytes": (_I64, [_CI, ctypes.POINTER(LrqTensor), _I64, _CI, _I64, _I64, _CU]),

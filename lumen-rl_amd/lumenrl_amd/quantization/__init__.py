@@ -1,7 +1,7 @@
 """Weight quantization for trainer -> rollout weight sync (lumenrl/quantization mirror)."""
 
 from lumenrl_amd.quantization.bucket import QuantizedBucketWriter, encode_bucket
-from lumenrl_amd.quantization.experts import route_experts
+from lumenrl_amd.quantization.experts import fp8_experts, route_experts
 from lumenrl_amd.quantization.fp8_config import (
     FP8Config,
     QuantizationConfig,
@@ -42,6 +42,7 @@ __all__ = [
     "fp8_block_quant",
     "fp8_block_linear",
     "fp8_e4m3_max",
+    "fp8_experts",
     "fp8_linear",
     "fp8_matmul",
     "quantize_fp8_blockwise",

@@ -1,7 +1,8 @@
 """Mixture-of-experts operators: the router, and the experts on FP8 weights.
 
 ``route_experts`` turns a router's logits into each token's experts and their
-weights, with the gradient of the logits.  Every function launches on the
+weights, with the gradient of the logits; ``fp8_experts`` runs those experts' MLPs
+on the stacks that ``quantize_fp8_blockwise`` writes.  Every function launches on the
 current stream of its operands' device and returns without synchronizing.
 """
 
@@ -13,6 +14,7 @@ import torch
 from torch import Tensor
 
 from lumenrl_amd import _lib
+from lumenrl_amd.quantization.fp8_product import check_tiles
 from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _dense, _on, _stream
 
 _SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
@@ -111,3 +113,58 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: O
     if logits.requires_grad and torch.is_grad_enabled():
         return _Route.apply(logits, bias, cfg)
     return _route(logits, bias, cfg)
+
+
+def fp8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_up_scales: Tensor, down: Tensor,
+                down_scales: Tensor) -> Tensor:
+    """The chosen experts' SwiGLU MLPs in FP8, and their weighted sum.
+
+    ``x`` [..., H] (bf16 or fp16) with ``ids`` and float32 ``weights`` [..., k] (as
+    ``route_experts`` gives them; int32, int64 ids are narrowed) -> [..., H] in x's
+    dtype.  ``gate_up`` [E, 2 I, H] (gate's rows first) and ``down`` [E, H, I] are
+    e4m3 codes with float32 scales of 128x128 tiles, as ``quantize_fp8_blockwise``
+    writes them; H and I are multiples of 16.  x and the hidden values are quantized
+    in 1x128 blocks; all else is float32.  A pair whose id is not one of 0 .. E - 1
+    is left out (a shard's other experts, say).
+    """
+    what = "fp8_experts"
+    _check_input(x, what)
+    dev = x.device
+    if x.dtype == torch.float32:
+        raise TypeError(f"{what}: x must be bf16 or fp16")
+    if not isinstance(ids, Tensor) or not isinstance(weights, Tensor):
+        raise TypeError(f"{what}: ids and weights must be tensors")
+    if ids.dtype not in (torch.int32, torch.int64) or weights.dtype != torch.float32:
+        raise TypeError(f"{what}: ids must be int32 or int64 and weights float32, got {ids.dtype} and {weights.dtype}")
+    gate_up, gate_up_scales = check_tiles(what, gate_up, gate_up_scales, dev)
+    down, down_scales = check_tiles(what, down, down_scales, dev)
+    if x.dim() < 1 or gate_up.dim() != 3 or down.dim() != 3:
+        raise ValueError(f"{what}: x {tuple(x.shape)}, gate_up {tuple(gate_up.shape)} and down {tuple(down.shape)} do not fit")
+    e, h, i = down.shape
+    if gate_up.shape != (e, 2 * i, h) or x.shape[-1] != h:
+        raise ValueError(f"{what}: x {tuple(x.shape)}, gate_up {tuple(gate_up.shape)} and down {tuple(down.shape)} do not fit")
+    lead = x.shape[:-1]
+    if ids.dim() != x.dim() or ids.shape[:-1] != lead or weights.shape != ids.shape:
+        raise ValueError(f"{what}: ids {tuple(ids.shape)} and weights {tuple(weights.shape)} must be {(*lead, 'k')}")
+    if ids.device != dev or weights.device != dev:
+        raise ValueError(f"{what}: ids and weights must be on {dev}")
+    k = ids.shape[-1]
+    if not 1 <= e <= 1024 or not 1 <= k <= 64 or h % 16 or i % 16 or not h or not i or 2 * h * i >= 1 << 31:
+        raise ValueError(f"{what}: {e} experts (at most 1024), top {k} (at most 64), H {h} and I {i} (multiples of 16, "
+                         "2 H I below 2^31)")
+    if ids.dtype == torch.int64:
+        ids = ids.clamp(-1, e).to(torch.int32)
+    x, rows, ld = _rows(x)
+    gate_up, down = (w if w.data_ptr() % 16 == 0 else w.clone() for w in (gate_up, down))
+    ids, weights = ids.contiguous(), weights.contiguous()
+    out = _dense((*lead, h), x.dtype, dev)
+    L = _lib.lib()
+    need = L.lrq_fp8_experts_workspace(rows, h, i, e, k)
+    work = _dense((need,), torch.uint8, dev)
+    with _on(dev):
+        rc = L.lrq_fp8_experts(x.data_ptr(), _IN_DTYPES[x.dtype], rows, h, ld, ids.data_ptr(), weights.data_ptr(), k,
+                               gate_up.data_ptr(), gate_up_scales.data_ptr(), down.data_ptr(), down_scales.data_ptr(), e, i,
+                               out.data_ptr(), work.data_ptr(), need, _stream(dev))
+    if rc:
+        _lib.check(rc, "lrq_fp8_experts")
+    return out

@@ -1,0 +1,237 @@
+"""``fp8_experts`` against its definition in float64, pair by pair."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from lumenrl_amd.quantization import fp8_block_quant, fp8_experts, quantize_fp8_blockwise, route_experts
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+E4M3 = torch.float8_e4m3fn
+
+
+def spread(s, rows, cols, br=128, bc=128):
+    return s.double().repeat_interleave(br, 0)[:rows].repeat_interleave(bc, 1)[:, :cols]
+
+
+def grid(v):
+    """float64 -> the nearest e4m3 value, ties to even."""
+    exponent = torch.frexp(v).exponent
+    step = torch.ldexp(torch.ones_like(v), (exponent - 4).clamp_min(-9))
+    return torch.round(v / step) * step
+
+
+def image(h, scale):
+    return (grid((h / scale).clamp(-448, 448)) * scale).float().double()
+
+
+def hidden_scale(h):
+    pad = torch.zeros(h.shape[0], -(-h.shape[1] // 128) * 128, dtype=h.dtype, device=h.device)
+    pad[:, : h.shape[1]] = h
+    s = (pad.view(h.shape[0], -1, 128).abs().amax(-1) / 448).clamp_min(2.0 ** -126)
+    return s.repeat_interleave(128, 1)[:, : h.shape[1]]
+
+
+def product_bound(xd, wd, trunc=True):
+    """Sums of K/128 blocks: float32's own errors, and the f8f6f4 instructions', which drop what is 2^-13 below a block's
+    largest product, 128 products a block."""
+    k = xd.shape[1]
+    bound = (128 + k // 128 + 16) * 2.0 ** -23 * (xd.abs() @ wd.abs().T)
+    if trunc:
+        for b in range(0, k, 128):
+            bound += 2.0 ** -6 * xd[:, b: b + 128].abs().amax(1)[:, None] * wd[:, b: b + 128].abs().amax(1)[None]
+    return bound
+
+
+def reference(x, ids, weights, gu, gus, dn, dns, exact_sums=False):
+    """out and how far a right kernel may be from it, [T, H] float64.
+
+    gate and up are off by product_bound (nothing but float32's roundings if the products are small whole numbers), h by that
+    through silu (slope at most 1.1) and 8 roundings; a hidden value whose quotient comes within that of a border may be
+    quantized to the neighbour (both images are tried), and scales move by as much."""
+    t, k = ids.shape
+    inter, hidden = dn.shape[2], dn.shape[1]
+    xc, xs = fp8_block_quant(x, (1, 128))
+    xd = xc.double() * spread(xs, t, hidden, 1)
+    out = torch.zeros(t, hidden, dtype=torch.float64, device=DEV)
+    slack = torch.zeros_like(out)
+    for e in range(gu.shape[0]):
+        hit = ids == e
+        tok = hit.any(1).nonzero()[:, 0]
+        if not len(tok):
+            continue
+        wgu = gu[e].double() * spread(gus[e], 2 * inter, hidden)
+        wd = dn[e].double() * spread(dns[e], hidden, inter)
+        a = xd[tok] @ wgu.T
+        da = product_bound(xd[tok], wgu, not exact_sums)
+        g, u, dg, du = a[:, :inter], a[:, inter:], da[:, :inter], da[:, inter:]
+        h = g * torch.sigmoid(g) * u
+        dh = 1.1 * dg * (u.abs() + du) + (g * torch.sigmoid(g)).abs() * du + 8 * 2.0 ** -23 * h.abs() + 2.0 ** -140
+        s, s_lo, s_hi = hidden_scale(h), hidden_scale((h.abs() - dh).clamp_min(0)), hidden_scale(h.abs() + dh)
+        q = image(h, s)
+        moved = torch.zeros_like(q)
+        for v in (h - dh, h + dh):
+            for sc in (s_lo, s, s_hi):
+                moved = torch.maximum(moved, (image(v, sc) - q).abs())
+        w = (weights.double() * hit).sum(1)[tok][:, None]
+        out[tok] += (q @ wd.T) * w
+        slack[tok] += (moved @ wd.abs().T + product_bound(q, wd) + 2.0 ** -22 * (q.abs() @ wd.abs().T)) * w.abs()
+        slack[tok] += k * 2.0 ** -23 * ((q @ wd.T) * w).abs()
+    return out, slack
+
+
+def check(y, want, slack):
+    half = torch.finfo(y.dtype).eps / 2
+    off = (y.double() - want).abs()
+    bound = slack + half * (want.abs() + slack) + (2.0 ** -24 if y.dtype == torch.float16 else 2.0 ** -133)
+    assert bool((off <= bound).all()), float((off / bound).nan_to_num(9e9).max())
+
+
+def whole_weights(e, n, k, gen):
+    """Codes of 0, +-1, +-2 and scales that are powers of two: the first product's block sums are whole numbers."""
+    codes = torch.randint(-2, 3, (e, n, k), generator=gen, device=DEV).float().to(E4M3)
+    scales = torch.pow(2.0, torch.randint(-8, -5, (e, -(-n // 128), -(-k // 128)), generator=gen, device=DEV).float())
+    return codes, scales
+
+
+def make(t, e, h, i, k, dtype=torch.bfloat16, seed=0, whole=True):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    if whole:
+        x = torch.randint(-2, 3, (t, h), generator=gen, device=DEV).to(dtype)
+        x[:, ::16] = 2.0
+        gu, gus = whole_weights(e, 2 * i, h, gen)
+        dn, dns = whole_weights(e, h, i, gen)
+    else:
+        x = torch.randn(t, h, generator=gen, device=DEV).to(dtype)
+        gu, gus = quantize_fp8_blockwise(torch.randn(e, 2 * i, h, generator=gen, device=DEV) * 0.05)
+        dn, dns = quantize_fp8_blockwise(torch.randn(e, h, i, generator=gen, device=DEV) * 0.05)
+    top = torch.topk(torch.randn(t, e, generator=gen, device=DEV) + torch.randn(e, generator=gen, device=DEV), k)
+    return x, top.indices.to(torch.int32), torch.softmax(top.values, -1), gu, gus, dn, dns
+
+
+# few pairs, rows of 16 and 32, tiles; hidden and intermediate sizes cut every way, more experts than pairs and fewer
+SHAPES = [(1, 8, 256, 128, 2), (1, 128, 2048, 768, 8), (3, 40, 144, 80, 8), (5, 16, 1040, 208, 3), (7, 64, 272, 1040, 9),
+          (60, 8, 512, 192, 2), (200, 64, 528, 192, 8), (40, 4, 384, 96, 3), (170, 6, 272, 336, 1), (33, 1, 256, 256, 1),
+          (700, 4, 512, 192, 2), (1111, 8, 400, 272, 4), (2000, 3, 1040, 144, 2), (500, 5, 128, 16, 2), (300, 2, 16, 640, 2)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,e,h,i,k", SHAPES)
+def test_whole_numbers(t, e, h, i, k, dtype):
+    args = make(t, e, h, i, k, dtype, t + h)
+    y = fp8_experts(*args)
+    assert y.shape == (t, h) and y.dtype == dtype
+    check(y, *reference(*args, exact_sums=True))
+
+
+@pytest.mark.parametrize("t,e,h,i,k", SHAPES)
+def test_random_weights(t, e, h, i, k):
+    args = make(t, e, h, i, k, torch.bfloat16, t + i, whole=False)
+    y = fp8_experts(*args)
+    want, slack = reference(*args)
+    check(y, want, slack)
+    # most of the slack is for codes that flip, which are few and of either sign: the whole is nearer than that
+    off = (y.double() - want).norm() / want.norm()
+    assert float(off) < 2.0 ** -6, float(off)
+
+
+@pytest.mark.parametrize("t", [2, 90, 900])
+def test_pairs_left_out(t):
+    x, ids, weights, *w = make(t, 12, 256, 160, 3)
+    ids[0] = torch.tensor([-1, 12, 1 << 30], device=DEV, dtype=torch.int32)  # nothing left: zeros
+    ids[1, 1] = -7
+    y = fp8_experts(x, ids, weights, *w)
+    assert bool((y[0] == 0).all())
+    check(y, *reference(x, ids, weights, *w, exact_sums=True))
+    assert torch.equal(y, fp8_experts(x, ids.long(), weights, *w))
+    ids[:] = 99
+    assert bool((fp8_experts(x, ids, weights, *w) == 0).all())
+
+
+@pytest.mark.parametrize("t", [4, 100, 600])
+def test_one_expert_takes_all_and_the_same_expert_twice(t):
+    x, ids, weights, *w = make(t, 9, 256, 128, 2)
+    ids[:] = 4
+    y = fp8_experts(x, ids, weights, *w)
+    once = reference(x, ids[:, :1], weights.sum(1, keepdim=True), *w, exact_sums=True)
+    check(y, once[0], 2 * once[1])
+
+
+@pytest.mark.parametrize("t", [3, 80, 500])
+def test_strides_and_leading_dims(t):
+    x, ids, weights, *w = make(t, 6, 272, 144, 2)
+    want = fp8_experts(x, ids, weights, *w)
+    wide = torch.zeros(t, 3 * 272 + 3, device=DEV, dtype=x.dtype)
+    wide[:, 5:277] = x
+    assert torch.equal(fp8_experts(wide[:, 5:277], ids, weights, *w), want)
+    assert torch.equal(fp8_experts(x.t().contiguous().t(), ids.t().contiguous().t(), weights.t().contiguous().t(), *w), want)
+    y = fp8_experts(x[None], ids[None], weights[None], *w)
+    assert y.shape == (1, t, 272) and torch.equal(y[0], want)
+    gu, gus, dn, dns = w
+    moved = torch.zeros(gu.numel() + 1, dtype=torch.uint8, device=DEV)[1:].view(gu.shape).copy_(gu.view(torch.uint8)).view(E4M3)
+    assert torch.equal(fp8_experts(x, ids, weights, moved, gus, dn, dns), want)
+    one = fp8_experts(x[0], ids[0], weights[0], *w)
+    assert one.shape == (272,)
+    check(one[None], *reference(x[:1], ids[:1], weights[:1], *w, exact_sums=True))
+
+
+@pytest.mark.parametrize("t", [3, 80, 700])
+def test_nan_and_inf_stay_in_their_rows(t):
+    x, ids, weights, *w = make(t, 6, 256, 128, 2)
+    x[0, 9], x[1, 200], x[2] = float("nan"), float("inf"), 0.0
+    y = fp8_experts(x, ids, weights, *w)
+    assert bool(y[:2].isnan().all()) and bool((y[2] == 0).all())
+    check(y[3:], *reference(x[3:], ids[3:], weights[3:], *w, exact_sums=True))
+
+
+def test_empty():
+    x, ids, weights, *w = make(2, 4, 128, 64, 2)
+    assert fp8_experts(x[:0], ids[:0], weights[:0], *w).shape == (0, 128)
+
+
+@pytest.mark.parametrize("t", [2, 70, 800])
+def test_other_stream_graph_and_repeats(t):
+    x, ids, weights, *w = make(t, 10, 272, 192, 3)
+    want = fp8_experts(x, ids, weights, *w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = fp8_experts(x, ids, weights, *w)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fp8_experts(x, ids, weights, *w)
+    for seed in range(4):
+        nx, nids, nweights, *_ = make(t, 10, 272, 192, 3, seed=seed)
+        x.copy_(nx), ids.copy_(nids), weights.copy_(nweights)
+        graph.replay()
+        assert torch.equal(y, fp8_experts(x, ids, weights, *w))
+
+
+def test_router_and_experts_as_a_layer():
+    torch.manual_seed(0)
+    e, h, i, k = 16, 256, 128, 4
+    x, _, _, gu, gus, dn, dns = make(50, e, h, i, k)
+    weights, ids = route_experts(x.float() @ torch.randn(h, e, device=DEV), k)
+    check(fp8_experts(x, ids, weights, gu, gus, dn, dns), *reference(x, ids, weights, gu, gus, dn, dns, exact_sums=True))
+
+
+def test_refusals():
+    x, ids, weights, gu, gus, dn, dns = make(4, 4, 128, 64, 2)
+    bad = [(TypeError, dict(x=x.float())), (TypeError, dict(weights=weights.half())), (TypeError, dict(ids=ids.to(torch.int16))),
+           (ValueError, dict(ids=ids[:3])), (ValueError, dict(weights=weights[:, :1])), (ValueError, dict(x=x[:, :64])),
+           (ValueError, dict(gus=gus[:, :, :0])), (ValueError, dict(gu=gu[:3])), (ValueError, dict(dn=dn[0], dns=dns[0])),
+           (TypeError, dict(gu=gu.view(torch.uint8))), (ValueError, dict(ids=ids.cpu())), (ValueError, dict(x=x.cpu())),
+           (TypeError, dict(dns=dns.double())), (ValueError, dict(ids=ids[:, :0], weights=weights[:, :0]))]
+    for err, kw in bad:
+        a = dict(x=x, ids=ids, weights=weights, gu=gu, gus=gus, dn=dn, dns=dns)
+        a.update(kw)
+        with pytest.raises(err, match="fp8_experts"):
+            fp8_experts(*a.values())
+    odd = [torch.zeros(2, 80, 40, dtype=torch.uint8, device=DEV).view(E4M3), torch.ones(2, 1, 1, device=DEV),
+           torch.zeros(2, 40, 40, dtype=torch.uint8, device=DEV).view(E4M3), torch.ones(2, 1, 1, device=DEV)]
+    with pytest.raises(ValueError, match="multiples of 16"):
+        fp8_experts(x[:, :40], ids, weights, *odd)
