@@ -203,9 +203,10 @@ __global__ __launch_bounds__(512) void k_ex_down_rows(ExpertArgs a) {
 // ---------------------------------------------------------------------------
 // Weight rows of a tile: 16 of gate, the same 16 of up, and so on.
 struct UpTile {
+  static constexpr bool kCut = false;
   const ExpertArgs& a;
   const ExpertTile& t;
-  int block, wn;  // wn: the wave's first tile row
+  int block;
   __device__ const uint8_t* w() const { return a.gu + (int64_t)t.expert * 2 * a.inter * a.hidden; }
   __device__ const uint8_t* x() const { return a.xq; }
   __device__ uint32_t w_bytes() const { return (uint32_t)(2 * a.inter * a.hidden); }
@@ -217,25 +218,29 @@ struct UpTile {
   }
   __device__ int token(int r) const { return gld<int32_t>(a.order + t.first + (r < t.rows ? r : t.rows - 1)) / a.top_k; }
   __device__ uint32_t x_off(int r) const { return r < t.rows ? (uint32_t)token(r) * (uint32_t)a.hidden : kNoRow; }
-  __device__ const float* sx(int r) const { return a.xs + (int64_t)token(r) * a.kb; }
-  __device__ const float* sw(int i) const {
-    const int r = wn + 16 * i, n = column(r) < a.inter ? column(r) : a.inter - 1;
-    return a.gus + ((int64_t)t.expert * a.gb + ((r >> 4 & 1 ? a.inter : 0) + n) / kBlk) * a.kb;
+  __device__ const float* sx() const { return a.xs; }
+  __device__ const float* sw() const { return a.gus + (int64_t)t.expert * a.gb * a.kb; }
+  __device__ uint32_t sx_bytes() const { return (uint32_t)(4 * a.tokens * a.kb); }
+  __device__ uint32_t sw_bytes() const { return (uint32_t)(4 * a.gb * a.kb); }
+  __device__ uint32_t sx_off(int r) const { return 4 * (uint32_t)token(r) * (uint32_t)a.kb; }
+  __device__ uint32_t sw_off(int s) const {
+    const int n = column(16 * s) < a.inter ? column(16 * s) : a.inter - 1;
+    return (uint32_t)(4 * (((s & 1 ? a.inter : 0) + n) / kBlk) * a.kb);
   }
 };
 
-template <int FN, int FM, int WN, int WM>
+template <int FN, int FM, int WN, int WM, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
   static_assert(16 * FN * WN == 256, "128 columns of h");
   constexpr int BM = 16 * FM * WM;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kTileStage<FN, FM, WN, WM>];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<FN, FM, WN, WM, STAGES>];
   int tile, block;
   if (!expert_piece(blockIdx.x, gld<int32_t>(a.total), a.ib, tile, block)) return;
   const ExpertTile t = a.tiles[tile];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const UpTile src{a, t, block, wave / WM * 16 * FN};
+  const UpTile src{a, t, block};
   f32x4 acc[FN][FM], h[FN / 2][FM];
-  tile_sums<FN, FM, WN, WM, true, true, false>(src, a.hidden, lds, acc);
+  tile_sums<FN, FM, WN, WM, STAGES, true, true, false>(src, a.hidden, lds, acc);
 #pragma unroll
   for (int i = 0; i < FN / 2; ++i)
 #pragma unroll
@@ -246,35 +251,40 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
 }
 
 struct DownTile {
+  static constexpr bool kCut = false;
   const ExpertArgs& a;
   const ExpertTile& t;
-  int n0, wn;
+  int n0;
   __device__ const uint8_t* w() const { return a.dn + (int64_t)t.expert * a.hidden * a.inter; }
   __device__ const uint8_t* x() const { return a.hq + (int64_t)t.first * a.inter; }
   __device__ uint32_t w_bytes() const { return (uint32_t)(a.hidden * a.inter); }
   __device__ uint32_t x_bytes() const { return (uint32_t)(t.rows * a.inter); }
   __device__ uint32_t w_off(int r) const { return n0 + r < a.hidden ? (uint32_t)(n0 + r) * (uint32_t)a.inter : kNoRow; }
   __device__ uint32_t x_off(int r) const { return r < t.rows ? (uint32_t)r * (uint32_t)a.inter : kNoRow; }
-  __device__ const float* sx(int r) const { return a.hs + (int64_t)(t.first + (r < t.rows ? r : t.rows - 1)) * a.ib; }
-  __device__ const float* sw(int) const {
-    const int n = n0 + wn < a.hidden ? n0 + wn : a.hidden - 1;
-    return a.dns + ((int64_t)t.expert * a.kb + n / kBlk) * a.ib;
+  __device__ const float* sx() const { return a.hs + (int64_t)t.first * a.ib; }
+  __device__ const float* sw() const { return a.dns + (int64_t)t.expert * a.kb * a.ib; }
+  __device__ uint32_t sx_bytes() const { return (uint32_t)(4 * t.rows * a.ib); }
+  __device__ uint32_t sw_bytes() const { return (uint32_t)(4 * a.kb * a.ib); }
+  __device__ uint32_t sx_off(int r) const { return (uint32_t)(4 * (r < t.rows ? r : t.rows - 1) * a.ib); }
+  __device__ uint32_t sw_off(int s) const {
+    const int n = n0 + 16 * s < a.hidden ? n0 + 16 * s : a.hidden - 1;
+    return (uint32_t)(4 * (n / kBlk) * a.ib);
   }
 };
 
-template <int FN, int FM, int WN, int WM>
+template <int FN, int FM, int WN, int WM, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_down_tiles(ExpertArgs a) {
   constexpr int BN = 16 * FN * WN;
   static_assert(16 * FN <= kBlk, "one scale for a wave's rows");
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kTileStage<FN, FM, WN, WM>];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<FN, FM, WN, WM, STAGES>];
   int tile, block;
   if (!expert_piece(blockIdx.x, gld<int32_t>(a.total), (a.hidden + BN - 1) / BN, tile, block)) return;
   const ExpertTile t = a.tiles[tile];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4, wn = wave / WM * 16 * FN, wm = wave % WM * 16 * FM;
-  const DownTile src{a, t, block * BN, wn};
+  const DownTile src{a, t, block * BN};
   f32x4 acc[FN][FM];
-  tile_sums<FN, FM, WN, WM, true, false, false>(src, a.inter, lds, acc);
+  tile_sums<FN, FM, WN, WM, STAGES, true, false, false>(src, a.inter, lds, acc);
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
     const int row = wm + 16 * j + c;
@@ -504,8 +514,8 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
     } else if (bm == 32) {
       by_rows<2>(a, tiles, stream);
     } else {
-      hipLaunchKernelGGL((k_ex_up_tiles<4, 4, 4, 2>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(512), 0, stream, a);
-      hipLaunchKernelGGL((k_ex_down_tiles<4, 4, 2, 2>), dim3((unsigned)((tiles * ((a.hidden + 127) / 128) + 7) / 8 * 8)), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((k_ex_up_tiles<4, 4, 4, 2, 3>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(512), 0, stream, a);
+      hipLaunchKernelGGL((k_ex_down_tiles<4, 4, 2, 2, 4>), dim3((unsigned)((tiles * ((a.hidden + 127) / 128) + 7) / 8 * 8)), dim3(256), 0, stream, a);
     }
     const dim3 sum((unsigned)((a.tokens * a.hidden / 8 + 255) / 256));
     if (dtype == kBF16) hipLaunchKernelGGL((k_ex_sum<kBF16>), sum, dim3(256), 0, stream, a);

@@ -106,8 +106,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_mm8_rows(MatmulArgs a) {
 // Many tokens
 // ---------------------------------------------------------------------------
 struct DenseTile {
+  static constexpr bool kCut = true;
   const MatmulArgs& a;
-  int n0, m0, wn, n_last, m_last;  // n_last, m_last: within the tile
+  int n0, m0, n_last, m_last;  // n_last, m_last: within the tile
   bool dma;
   __device__ const uint8_t* w() const { return a.w + (int64_t)n0 * a.k; }
   __device__ const uint8_t* x() const { return static_cast<const uint8_t*>(a.x) + (int64_t)m0 * a.ldx; }
@@ -115,8 +116,15 @@ struct DenseTile {
   __device__ uint32_t x_bytes() const { return (uint32_t)((m_last < 255 ? m_last : 255) * a.ldx + a.k); }
   __device__ uint32_t w_off(int r) const { return r <= n_last ? (uint32_t)(r * a.k) : dma ? kNoRow : (uint32_t)(n_last * a.k); }
   __device__ uint32_t x_off(int r) const { return r <= m_last ? (uint32_t)(r * a.ldx) : dma ? kNoRow : (uint32_t)(m_last * a.ldx); }
-  __device__ const float* sx(int r) const { return a.sx + (int64_t)(m0 + (r < m_last ? r : m_last)) * a.kb; }
-  __device__ const float* sw(int i) const { return a.sw + (int64_t)((n0 + (wn < n_last ? wn : n_last)) / kBlk) * a.kb; }
+  __device__ const float* sx() const { return a.sx + (int64_t)m0 * a.kb; }
+  __device__ const float* sw() const { return a.sw + (int64_t)(n0 / kBlk) * a.kb; }
+  __device__ uint32_t sx_bytes() const { return (uint32_t)(4 * ((m_last < 255 ? m_last : 255) + 1) * a.kb); }
+  __device__ uint32_t sw_bytes() const { return (uint32_t)(4 * ((n_last < 255 ? n_last : 255) / kBlk + 1) * a.kb); }
+  __device__ uint32_t sx_off(int r) const { return (uint32_t)(4 * (r < m_last ? r : m_last) * a.kb); }
+  __device__ uint32_t sw_off(int s) const {
+    const int r = (n0 & (kBlk - 1)) + (16 * s < n_last ? 16 * s : n_last);
+    return (uint32_t)(4 * (r / kBlk) * a.kb);
+  }
 };
 
 template <int ODT, int FN, int FM>
@@ -167,18 +175,18 @@ __device__ __forceinline__ void store_tile(const MatmulArgs& a, f32x4 (&acc)[FN]
   }
 }
 
-template <int FN, int FM, int WN, int WM, bool DMA, bool EXACT>
+template <int FN, int FM, int WN, int WM, int STAGES, bool DMA, bool EXACT>
 __global__ __launch_bounds__(64 * WN * WM, 1) void k_mm8_tiles(MatmulArgs a, int tiles_m, int tiles_n) {
-  constexpr int BN = 16 * FN * WN, BM = 16 * FM * WM, kStages = 2 * kTileStage<FN, FM, WN, WM>;
-  static_assert(WN * WM * 16 * (64 * FN + 16) <= kStages, "results pass through the stages");
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kStages];
+  constexpr int BN = 16 * FN * WN, BM = 16 * FM * WM, kLds = kTileLds<FN, FM, WN, WM, STAGES>;
+  static_assert(WN * WM * 16 * (64 * FN + 16) <= kLds, "results pass through the stages");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = (wave / WM) * 16 * FN, wm = (wave % WM) * 16 * FM;
-  const DenseTile src{a, tn * BN, tm * BM, wn, (int)a.n - 1 - tn * BN, (int)a.m - 1 - tm * BM, DMA};
+  const DenseTile src{a, tn * BN, tm * BM, (int)a.n - 1 - tn * BN, (int)a.m - 1 - tm * BM, DMA};
   f32x4 acc[FN][FM];
-  tile_sums<FN, FM, WN, WM, DMA, false, EXACT>(src, (int)a.k, lds, acc);
+  tile_sums<FN, FM, WN, WM, STAGES, DMA, false, EXACT>(src, (int)a.k, lds, acc);
   if constexpr (EXACT) return store_tile<kF32>(a, acc, src.n0 + wn, src.m0 + wm, lds);
   else if (a.out_dtype == kBF16) return store_tile<kBF16>(a, acc, src.n0 + wn, src.m0 + wm, lds);
   else return store_tile<kF16>(a, acc, src.n0 + wn, src.m0 + wm, lds);
@@ -189,13 +197,13 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_mm8_tiles(MatmulArgs a, int
 // ---------------------------------------------------------------------------
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static bool dma_ok(const MatmulArgs& a) {
-  return a.k % 16 == 0 && a.ldx % 16 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
+  return a.k % 4 == 0 && a.ldx % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 4 == 0 && reinterpret_cast<uintptr_t>(a.w) % 4 == 0;
 }
 
-template <int FN, int FM, int WN, int WM, bool DMA, bool EXACT>
+template <int FN, int FM, int WN, int WM, int STAGES, bool DMA, bool EXACT>
 static void launch_tiles(const MatmulArgs& a, hipStream_t stream) {
   const int tiles_m = (int)ceil_div(a.m, 16 * FM * WM), tiles_n = (int)ceil_div(a.n, 16 * FN * WN);
-  hipLaunchKernelGGL((k_mm8_tiles<FN, FM, WN, WM, DMA, EXACT>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * WN * WM), 0, stream, a,
+  hipLaunchKernelGGL((k_mm8_tiles<FN, FM, WN, WM, STAGES, DMA, EXACT>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * WN * WM), 0, stream, a,
                      tiles_m, tiles_n);
 }
 template <int XDT, int NT, int MT, int D>
@@ -208,9 +216,9 @@ static void launch_rows(const MatmulArgs& a, int64_t x_lds, hipStream_t stream) 
 template <bool DMA, bool EXACT>
 static void launch_tiles_of(const MatmulArgs& a, hipStream_t stream) {
   if constexpr (DMA && !EXACT)
-    if (ceil_div(a.m, 256) * ceil_div(a.n, 256) >= 200) return launch_tiles<8, 4, 2, 4, DMA, EXACT>(a, stream);
-  if (ceil_div(a.m, 128) * ceil_div(a.n, 128) >= 200) return launch_tiles<4, 4, 2, 2, DMA, EXACT>(a, stream);
-  launch_tiles<2, 2, 2, 2, DMA, EXACT>(a, stream);
+    if (ceil_div(a.m, 256) * ceil_div(a.n, 256) >= 200) return launch_tiles<8, 4, 2, 4, 2, DMA, EXACT>(a, stream);
+  if (ceil_div(a.m, 128) * ceil_div(a.n, 128) >= 200) return launch_tiles<4, 4, 2, 2, DMA ? 4 : 2, DMA, EXACT>(a, stream);
+  launch_tiles<2, 2, 2, 2, DMA ? 4 : 2, DMA, EXACT>(a, stream);
 }
 
 bool matmul_quantizes(int64_t m, int64_t k) {

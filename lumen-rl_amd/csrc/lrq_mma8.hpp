@@ -107,7 +107,7 @@ __device__ __forceinline__ void lds_barrier8() {
 // ---------------------------------------------------------------------------
 // 16 bytes a lane, at `off` from the descriptor's base (zeros if off + 16 passes
 // its size), to 16 l + `lds`.  In assembly because the compiler, which cannot
-// tell the two stages of a tile apart, waits for every such load before the
+// tell a tile's stages apart, waits for every such load before the
 // next read of LDS; dma_wait() is the wait, before the barrier that hands the
 // stage over.  The instruction has no register output.
 typedef uint32_t Rsrc __attribute__((ext_vector_type(4)));
@@ -121,7 +121,9 @@ __device__ __forceinline__ void dma16(Rsrc r, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(lds), "v"(off), "s"(r) : "memory");
 }
-__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Until at most N of the wave's loads are on their way: they arrive in order.
+template <int N>
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 constexpr uint32_t kNoRow = 0x80000000u;  // an offset past every descriptor's size
 constexpr int64_t kDmaBytes = 0x7FFFFF00ll;  // so a descriptor holds at most this
 
@@ -185,32 +187,42 @@ __device__ __forceinline__ v2u quant8(const float* v, float& scale) {
 // Many tokens: tiles through LDS
 // ---------------------------------------------------------------------------
 // The sums of a tile of BM = 16 FM WM tokens and BN = 16 FN WN weight rows by
-// WN x WM waves, each its 16 FN x 16 FM of it.  K goes block by block through
-// two stages of LDS, codes of both operands in rows of 128 bytes whose 16-byte
-// pieces stand at places (piece ^ row / 2): reads of one piece from 16 rows
-// then fall into all 64 banks.  A wave keeps the block of its tokens in
-// registers and takes the weight 16 rows at a time: FM matrix instructions,
-// whose results the scales multiply into the sums one step later, between the
-// next step's matrix instructions.
+// WN x WM waves, each its 16 FN x 16 FM of it.  K goes block by block through a
+// ring of STAGES in LDS: codes of both operands in rows of 128 bytes whose
+// 16-byte pieces stand at places (piece ^ row / 2), so that reads of one piece
+// from 16 rows fall into all 64 banks.  Behind the ring stand the scales of four
+// blocks at a time, and of the next four.  A wave keeps the block of its tokens in
+// registers and takes the weight 16 rows at a time; a result is scaled into the
+// sums three matrix instructions after its own, which the compiler, left to
+// itself, does at once, and waits (2534 instead of 3000 TFLOP/s without any loads).
 //
-// DMA: codes go from memory straight into LDS; rows are 16-byte aligned.
-// Otherwise any address: through registers, which costs 32 of them.
+// DMA (rows are 4-byte aligned): codes and scales go from memory straight into
+// LDS, STAGES - 1 blocks ahead, each wave waiting only for its own part of the
+// oldest.  Otherwise (any address): through registers, kTileSets blocks ahead.
 //
-// Src gives: w_bytes(), x_bytes() and the operands' bases w(), x();
+// Src gives: w_bytes(), x_bytes(), sw_bytes(), sx_bytes() and the operands'
+// bases w(), x(), sw(), sx();
 //   w_off(r), x_off(r): the byte offset of a tile row, kNoRow for none (its sums
 //   are not stored; without DMA some row that is there instead);
-//   sx(r): the scales of tile row r of the tokens (of some token, if none);
-//   sw(i): the scales of the wave's weight rows 16 i .. (one scale for 16 rows).
-// EACH: sw(i) differ; otherwise sw(0) is for all of a wave's rows.
+//   sx_off(r): of the scales of tile row r of the tokens, sw_off(s) of those of
+//   weight rows 16 s .. (one scale for 16 rows); of some row that is there, if none.
+//   kCut: k may be no multiple of 16.
+// EACH: the scales of a wave's weight rows differ; otherwise the first is for all.
+constexpr int kTileSets = 2;
 template <int FN, int FM, int WN, int WM>
 constexpr int kTileStage = 16 * (FN * WN + FM * WM) * kBlk;
+template <int FN, int FM, int WN, int WM>
+constexpr int kTileScales = 16 * 64 * WN * WM;  // of four blocks: a place for every thread
+template <int FN, int FM, int WN, int WM, int STAGES>
+constexpr int kTileLds = STAGES * kTileStage<FN, FM, WN, WM> + 2 * kTileScales<FN, FM, WN, WM>;
 
-template <int FN, int FM, int WN, int WM, bool DMA, bool EACH, bool EXACT, class Src>
+template <int FN, int FM, int WN, int WM, int STAGES, bool DMA, bool EACH, bool EXACT, class Src>
 __device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f32x4 (&acc)[FN][FM]) {
-  constexpr int T = 64 * WN * WM, BN = 16 * FN * WN, BM = 16 * FM * WM;
-  constexpr int PW = BN * 8 / T, PX = BM * 8 / T;  // 16-byte pieces a thread moves per block
-  constexpr int kStage = kTileStage<FN, FM, WN, WM>, SW = EACH ? FN : 1;
-  static_assert(PW * T == BN * 8 && PX * T == BM * 8 && T % 128 == 0, "");
+  constexpr int T = 64 * WN * WM, BN = 16 * FN * WN, BM = 16 * FM * WM, TILES = FN * FM, LAG = TILES > 4 ? 3 : 1;
+  constexpr int PW = BN * 8 / T, PX = BM * 8 / T;  // 16-byte pieces a thread moves per block, and one scale
+  constexpr int kStage = kTileStage<FN, FM, WN, WM>, kScales = kTileScales<FN, FM, WN, WM>;
+  static_assert(PW * T == BN * 8 && PX * T == BM * 8 && T % 128 == 0 && BM % 64 == 0 && BM + BN / 16 <= T, "");
+  static_assert(STAGES >= 2 && STAGES <= 5, "the next four blocks' scales arrive before them");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int wn = (wave / WM) * 16 * FN, wm = (wave % WM) * 16 * FM;
@@ -221,93 +233,42 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f
   for (int p = 0; p < PW; ++p) wo[p] = src.w_off((T / 8) * p + (tid >> 3)) + 16 * piece;
 #pragma unroll
   for (int p = 0; p < PX; ++p) xo[p] = src.x_off((T / 8) * p + (tid >> 3)) + 16 * piece;
-  // DMA: offsets past the row's end in the last block read as zeros
-  Rsrc rw, rx;
-  uint32_t to = 0;
-  if constexpr (DMA) {
-    rw = make_rsrc(src.w(), src.w_bytes());
-    rx = make_rsrc(src.x(), src.x_bytes());
-    to = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds) + 1024 * wave;
-  }
-  v4u gw[DMA ? 1 : PW], gx[DMA ? 1 : PX];
-  auto fetch = [&](int kb, int stage) {
-    const uint32_t at = (uint32_t)(kb * kBlk);
-    if constexpr (DMA) {
-      const uint32_t past = (int)at + 16 * piece < k ? 0 : kNoRow;
+  // the thread's scales: tokens first, then one for every 16 weight rows
+  const bool tokens = wave < BM / 64;
+  const uint32_t so = tokens ? src.sx_off(tid) : tid < BM + BN / 16 ? src.sw_off(tid - BM) : kNoRow;
+  uint8_t* const scales = lds + STAGES * kStage;
 #pragma unroll
-      for (int p = 0; p < PW; ++p) dma16(rw, (wo[p] + at) | past, to + stage * kStage + 128 * (T / 8) * p);
+  for (int i = 0; i < FN; ++i)
 #pragma unroll
-      for (int p = 0; p < PX; ++p) dma16(rx, (xo[p] + at) | past, to + stage * kStage + 128 * (BN + (T / 8) * p));
-    } else if ((int)at + kBlk <= k) {
-#pragma unroll
-      for (int p = 0; p < PW; ++p) gw[p] = load_codes((GlobalCodes)src.w() + (wo[p] + at));
-#pragma unroll
-      for (int p = 0; p < PX; ++p) gx[p] = load_codes((GlobalCodes)src.x() + (xo[p] + at));
-    } else {
-#pragma unroll
-      for (int p = 0; p < PW; ++p) gw[p] = load_codes_cut((GlobalCodes)src.w() + (wo[p] - 16 * piece), (int)at + 16 * piece, k);
-#pragma unroll
-      for (int p = 0; p < PX; ++p) gx[p] = load_codes_cut((GlobalCodes)src.x() + (xo[p] - 16 * piece), (int)at + 16 * piece, k);
-    }
-  };
-  auto put = [&](int stage) {
-    if constexpr (!DMA) {
-      uint8_t* const s = lds + stage * kStage + 16 * tid;
-#pragma unroll
-      for (int p = 0; p < PW; ++p) *reinterpret_cast<v4u*>(s + 128 * (T / 8) * p) = gw[p];
-#pragma unroll
-      for (int p = 0; p < PX; ++p) *reinterpret_cast<v4u*>(s + 128 * (BN + (T / 8) * p)) = gx[p];
-    } else {
-      dma_wait();
-    }
-  };
-  const float* sxp[FM];
-#pragma unroll
-  for (int j = 0; j < FM; ++j) sxp[j] = src.sx(wm + 16 * j + c);
-  const float* swp[SW];
-#pragma unroll
-  for (int i = 0; i < SW; ++i) swp[i] = src.sw(i);
-  float sx[FM], sw[SW];
-  auto scales = [&](int kb) {
-#pragma unroll
-    for (int j = 0; j < FM; ++j) sx[j] = gld<float>(sxp[j] + kb);
-#pragma unroll
-    for (int i = 0; i < SW; ++i) sw[i] = gld<float>(swp[i] + kb);
-  };
-  f32x4 p[FM], pp[FM];
-  float sp[FM];
-#pragma unroll
-  for (int j = 0; j < FM; ++j) {
-    pp[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    sp[j] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < FN; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  fetch(0, 0);
-  scales(0);
-  put(0);
-  lds_barrier8();
+    for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
   const int at0 = 16 * (g ^ (c >> 1)), at1 = 16 * ((g + 4) ^ (c >> 1));
-  for (int kb = 0; kb < kb_n; ++kb) {
-    const uint8_t* const cw = lds + (kb & 1) * kStage + 128 * (wn + c);
-    const uint8_t* const cx = lds + (kb & 1) * kStage + 128 * (BN + wm + c);
-    if (kb + 1 < kb_n) fetch(kb + 1, (kb + 1) & 1);
-    float s[FM], si[SW];
+  auto multiply = [&](const uint8_t* stage, int kb) {
+    const uint8_t* const cw = stage + 128 * (wn + c);
+    const uint8_t* const cx = stage + 128 * (BN + wm + c);
+    const float* const sc = reinterpret_cast<const float*>(scales + (kb >> 2 & 1) * kScales) + (kb & 3);
+    float s[FM], si[EACH ? FN : 1];
 #pragma unroll
-    for (int j = 0; j < FM; ++j) s[j] = sx[j];
+    for (int j = 0; j < FM; ++j) s[j] = sc[4 * (wm + 16 * j + c)];
 #pragma unroll
-    for (int i = 0; i < SW; ++i) si[i] = sw[i];
+    for (int i = 0; i < (EACH ? FN : 1); ++i) si[i] = sc[4 * (BM + wn / 16 + i)];
+    decltype(operand<EXACT>(Codes32{})) x[FM];
+    Codes32 w[2];
+    w[0] = {*reinterpret_cast<const v4u*>(cw + at0), *reinterpret_cast<const v4u*>(cw + at1)};
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+      x[j] = operand<EXACT>({*reinterpret_cast<const v4u*>(cx + 2048 * j + at0), *reinterpret_cast<const v4u*>(cx + 2048 * j + at1)});
     if constexpr (!EACH) {
 #pragma unroll
       for (int j = 0; j < FM; ++j) s[j] *= si[0];
     }
-    if (kb + 1 < kb_n) scales(kb + 1);
-    decltype(operand<EXACT>(Codes32{})) x[FM];
-    Codes32 w[2];
+    f32x4 p[LAG + 1];
+    auto scale = [&](int t) {
+      const int i = t / FM, j = t % FM;
+      const float f = EACH ? s[j] * si[EACH ? i : 0] : s[j];
 #pragma unroll
-    for (int j = 0; j < FM; ++j)
-      x[j] = operand<EXACT>({*reinterpret_cast<const v4u*>(cx + 2048 * j + at0), *reinterpret_cast<const v4u*>(cx + 2048 * j + at1)});
-    w[0] = {*reinterpret_cast<const v4u*>(cw + at0), *reinterpret_cast<const v4u*>(cw + at1)};
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(p[t % (LAG + 1)][r], f, acc[i][j][r]);
+    };
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
       if (i + 1 < FN)
@@ -316,24 +277,113 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f
       const auto wi = operand<EXACT>(w[i & 1]);
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
-        p[j] = mma8(wi, x[j]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[(i + FN - 1) % FN][j][r] = __builtin_fmaf(pp[j][r], sp[j], acc[(i + FN - 1) % FN][j][r]);
+        const int t = i * FM + j;
+        p[t % (LAG + 1)] = mma8(wi, x[j]);
+        if (t >= LAG) scale(t - LAG);
+        __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int j = 0; j < FM; ++j) {
-        pp[j] = p[j];
-        sp[j] = EACH ? s[j] * si[EACH ? i : 0] : s[j];
-      }
-      __builtin_amdgcn_sched_barrier(0);  // or every strip's codes are read at once, into registers there are not
     }
-    if (kb + 1 < kb_n) put((kb + 1) & 1);
-    lds_barrier8();  // every read of this stage is done, and the next is whole
+#pragma unroll
+    for (int t = TILES - LAG; t < TILES; ++t) scale(t);
+  };
+
+  if constexpr (DMA) {
+    const Rsrc rw = make_rsrc(src.w(), src.w_bytes()), rx = make_rsrc(src.x(), src.x_bytes());
+    const Rsrc rs = tokens ? make_rsrc(src.sx(), src.sx_bytes()) : make_rsrc(src.sw(), src.sw_bytes());
+    const uint32_t to = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds) + 1024 * wave;
+    auto fetch = [&](int kb, int stage) {
+      // blocks past the last are asked for, so that every wait counts the same, and read as zeros
+      const uint32_t at = (uint32_t)(kb * kBlk), past = (int)at + 16 * piece < k ? 0 : kNoRow;
+      const uint32_t here = to + (uint32_t)(stage * kStage);
+#pragma unroll
+      for (int p = 0; p < PW; ++p) dma16(rw, (wo[p] + at) | past, here + 128 * (T / 8) * p);
+#pragma unroll
+      for (int p = 0; p < PX; ++p) dma16(rx, (xo[p] + at) | past, here + 128 * (BN + (T / 8) * p));
+    };
+    auto fetch_scales = [&](int kb) {  // of blocks kb .. kb + 3; those past a row's end are the next row's, and not used
+      dma16(rs, (so + 4 * kb) | (kb < kb_n ? 0 : kNoRow), to + (uint32_t)(STAGES * kStage + (kb >> 2 & 1) * kScales));
+    };
+    // a row's last codes, where 16 bytes would reach past its end: one row a thread
+    const bool cut = Src::kCut && k % 16 != 0;
+    v4u last = {0, 0, 0, 0};
+    if (cut && tid < BN + BM) {
+      const uint32_t off = tid < BN ? src.w_off(tid) : src.x_off(tid - BN);
+      const GlobalCodes row = (GlobalCodes)(tid < BN ? src.w() : src.x()) + (off + (k & ~15));
+      if (off != kNoRow) {
+        last.x = gld<uint32_t>((const void*)row);
+        if (k % 16 > 4) last.y = gld<uint32_t>((const void*)(row + 4));
+        if (k % 16 > 8) last.z = gld<uint32_t>((const void*)(row + 8));
+      }
+    }
+    fetch_scales(0);
+#pragma unroll
+    for (int s = 0; s + 1 < STAGES; ++s) fetch(s, s);
+    int stage = 0, free = STAGES - 1;
+    for (int kb = 0; kb < kb_n; kb += 4) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (kb + r >= kb_n) break;
+        // on their way since this block's codes were asked for: the blocks between, and scales
+        if (r >= 1 && r <= STAGES - 2) dma_wait<(STAGES - 2) * (PW + PX) + 1>();
+        else dma_wait<(STAGES - 2) * (PW + PX)>();
+        lds_barrier8();  // every wave's part of this block is there, and every read of the last is done
+        if (r == 0) fetch_scales(kb + 4);
+        fetch(kb + r + STAGES - 1, free);
+        if (cut && kb + r == kb_n - 1) {
+          static_assert(BN + BM <= T || !Src::kCut, "");
+          if (tid < BN + BM) *reinterpret_cast<v4u*>(lds + stage * kStage + 128 * tid + 16 * ((k % kBlk / 16) ^ (tid >> 1 & 7))) = last;
+          lds_barrier8();
+        }
+        multiply(lds + stage * kStage, kb + r);
+        free = stage;
+        stage = stage + 1 < STAGES ? stage + 1 : 0;
+      }
+    }
+    dma_wait<0>();
+    lds_barrier8();
+  } else {
+    v4u gw[kTileSets][PW], gx[kTileSets][PX];
+    float gs[kTileSets];
+    const uint8_t* const sb = reinterpret_cast<const uint8_t*>(tokens ? src.sx() : src.sw());
+    auto fetch = [&](int kb, int set) {
+      const int at = kb * kBlk;
+      if (at + kBlk <= k) {
+#pragma unroll
+        for (int p = 0; p < PW; ++p) gw[set][p] = load_codes((GlobalCodes)src.w() + (wo[p] + at));
+#pragma unroll
+        for (int p = 0; p < PX; ++p) gx[set][p] = load_codes((GlobalCodes)src.x() + (xo[p] + at));
+      } else {
+#pragma unroll
+        for (int p = 0; p < PW; ++p) gw[set][p] = load_codes_cut((GlobalCodes)src.w() + (wo[p] - 16 * piece), at + 16 * piece, k);
+#pragma unroll
+        for (int p = 0; p < PX; ++p) gx[set][p] = load_codes_cut((GlobalCodes)src.x() + (xo[p] - 16 * piece), at + 16 * piece, k);
+      }
+      gs[set] = so != kNoRow && kb < kb_n ? gld<float>(sb + (so + 4 * kb)) : 0.0f;
+    };
+    auto put = [&](int set, int kb) {
+      uint8_t* const s = lds + (kb & 1) * kStage + 16 * tid;
+#pragma unroll
+      for (int p = 0; p < PW; ++p) *reinterpret_cast<v4u*>(s + 128 * (T / 8) * p) = gw[set][p];
+#pragma unroll
+      for (int p = 0; p < PX; ++p) *reinterpret_cast<v4u*>(s + 128 * (BN + (T / 8) * p)) = gx[set][p];
+      reinterpret_cast<float*>(scales + (kb >> 2 & 1) * kScales)[4 * tid + (kb & 3)] = gs[set];
+    };
+#pragma unroll
+    for (int s = 0; s < kTileSets; ++s) fetch(s, s);
+    put(0, 0);
+    fetch(kTileSets, 0);
+    for (int kb = 0; kb < kb_n; kb += 2 * kTileSets) {
+#pragma unroll
+      for (int r = 0; r < 2 * kTileSets; ++r) {
+        if (kb + r >= kb_n) break;
+        lds_barrier8();
+        put((r + 1) % kTileSets, kb + r + 1);
+        fetch(kb + r + 1 + kTileSets, (r + 1) % kTileSets);
+        multiply(lds + (r & 1) * kStage, kb + r);
+      }
+    }
+    lds_barrier8();
   }
-#pragma unroll
-  for (int j = 0; j < FM; ++j)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) acc[FN - 1][j][r] = __builtin_fmaf(pp[j][r], sp[j], acc[FN - 1][j][r]);
 }
 
 // ---------------------------------------------------------------------------
