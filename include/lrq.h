@@ -176,23 +176,27 @@ int lrq_fp8_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t 
  * counterpart in the reference, which leaves these products to vLLM / ATOM.
  *   lrq_fp8_matmul: x as e4m3 codes [rows, k] (row stride ld >= k) with float32
  *     scales [rows, ceil(k/128)], dense; out of out_dtype (bf16, fp16 or fp32).
+ *     `workspace`: lrq_fp8_matmul_workspace(rows, k, n) bytes, 0 but for some tens
+ *     of tokens, whose K is split.
  *   lrq_fp8_block_linear: x of x_dtype (bf16, fp16 or fp32; row stride ld),
  *     quantized as lrq_fp8_block_quant does with 1 x 128 blocks (float32
- *     arithmetic); out of x's type.  `workspace`: device memory, 256-byte
- *     aligned, of lrq_fp8_block_linear_workspace(rows, k) bytes (0 for few
- *     tokens, which are quantized within the product), overwritten.
+ *     arithmetic); out of x's type.  `workspace`: likewise of
+ *     lrq_fp8_block_linear_workspace(rows, k, n) bytes, 0 for a few tokens, which are
+ *     quantized within the product.  Workspaces are device memory, 256-byte aligned,
+ *     and overwritten.
  *   codes  : [n, k] e4m3 bytes, dense;  scales : [ceil(n/128), ceil(k/128)]
  *            float32, dense;  bias : [n] of bias_dtype, or null;
  *   out    : [rows, n], dense.
- * Any extents and element alignment; rows of codes that are 16-byte aligned are
+ * Any extents and element alignment; rows of codes that are 4-byte aligned are
  * moved fastest.  k and ld at most 2^22; rows at most 2^28, n 2^26 and rows * n
  * 2^33.  A pair of scales whose product leaves float32's normal range loses
  * bits, as the product does.
  */
 int lrq_fp8_matmul(const uint8_t* x_codes, const float* x_scales, int64_t rows, int64_t k, int64_t ld,
                    const uint8_t* codes, const float* scales, int64_t n, const void* bias, int bias_dtype,
-                   void* out, int out_dtype, lrq_stream_t stream);
-int64_t lrq_fp8_block_linear_workspace(int64_t rows, int64_t k);
+                   void* out, int out_dtype, void* workspace, int64_t workspace_bytes, lrq_stream_t stream);
+int64_t lrq_fp8_matmul_workspace(int64_t rows, int64_t k, int64_t n);
+int64_t lrq_fp8_block_linear_workspace(int64_t rows, int64_t k, int64_t n);
 int lrq_fp8_block_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t ld,
                          const uint8_t* codes, const float* scales, int64_t n, const void* bias,
                          int bias_dtype, void* out, void* workspace, int64_t workspace_bytes,

@@ -703,21 +703,39 @@ int check_matmul(const char* what, int64_t rows, int64_t k, int64_t ld, const ui
 }
 }  // namespace
 
+int64_t lrq_fp8_matmul_workspace(int64_t rows, int64_t k, int64_t n) {
+  if (rows <= 0 || k <= 0 || n <= 0 || rows > lrq::kMmRowsMax || k > lrq::kMmPitchMax || n > lrq::kMmOutMax) return 0;
+  return lrq::matmul_workspace(rows, n, k);
+}
+
+namespace {
+int check_workspace(const char* what, const void* workspace, int64_t bytes, int64_t need) {
+  if (need && (!workspace || bytes < need))
+    return fail(LRQ_ERR_CAPACITY, "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)need);
+  if (need && !aligned(workspace, 256)) return fail(LRQ_ERR_ALIGN, "%s: workspace must be 256-byte aligned", what);
+  return 0;
+}
+int64_t quantized_bytes(int64_t rows, int64_t k) { return (rows * k + 255) / 256 * 256 + (4 * rows * ((k + 127) / 128) + 255) / 256 * 256; }
+}  // namespace
+
 int lrq_fp8_matmul(const uint8_t* x_codes, const float* x_scales, int64_t rows, int64_t k, int64_t ld,
                    const uint8_t* codes, const float* scales, int64_t n, const void* bias, int bias_dtype, void* out,
-                   int out_dtype, lrq_stream_t stream) {
+                   int out_dtype, void* workspace, int64_t workspace_bytes, lrq_stream_t stream) {
   g_err.clear();
   const int rc = check_matmul("fp8_matmul", rows, k, ld, codes, scales, n, bias, bias_dtype, x_codes, out, out_dtype);
   if (rc) return rc > 0 ? 0 : rc;
   if (!x_scales) return fail(LRQ_ERR_ARG, "fp8_matmul: null pointer");
   if (!aligned(x_scales, 4)) return fail(LRQ_ERR_ALIGN, "fp8_matmul: scales must be element-aligned");
+  if (int w = check_workspace("fp8_matmul", workspace, workspace_bytes, lrq_fp8_matmul_workspace(rows, k, n))) return w;
   const lrq::MatmulArgs a{x_codes, x_scales, codes, scales, bias, out, ld, rows, n, k, (k + 127) / 128, bias_dtype, out_dtype};
-  return check_hip(lrq::launch_matmul(a, -1, (hipStream_t)stream), "kernel launch");
+  return check_hip(lrq::launch_matmul(a, -1, workspace, (hipStream_t)stream), "kernel launch");
 }
 
-int64_t lrq_fp8_block_linear_workspace(int64_t rows, int64_t k) {
-  if (rows <= 0 || k <= 0 || rows > lrq::kMmRowsMax || k > lrq::kMmPitchMax || lrq::matmul_quantizes(rows, k)) return 0;
-  return (rows * k + 255) / 256 * 256 + 4 * rows * ((k + 127) / 128);
+int64_t lrq_fp8_block_linear_workspace(int64_t rows, int64_t k, int64_t n) {
+  if (rows <= 0 || k <= 0 || n <= 0 || rows > lrq::kMmRowsMax || k > lrq::kMmPitchMax || n > lrq::kMmOutMax ||
+      lrq::matmul_quantizes(rows, k))
+    return 0;
+  return quantized_bytes(rows, k) + lrq::matmul_workspace(rows, n, k);
 }
 
 int lrq_fp8_block_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t ld, const uint8_t* codes,
@@ -727,17 +745,15 @@ int lrq_fp8_block_linear(const void* x, int x_dtype, int64_t rows, int64_t k, in
   const int rc = check_matmul("fp8_block_linear", rows, k, ld, codes, scales, n, bias, bias_dtype, x, out, x_dtype);
   if (rc) return rc > 0 ? 0 : rc;
   if (!aligned(x, (uintptr_t)esize(x_dtype))) return fail(LRQ_ERR_ALIGN, "fp8_block_linear: x must be element-aligned");
+  if (int w = check_workspace("fp8_block_linear", workspace, workspace_bytes, lrq_fp8_block_linear_workspace(rows, k, n))) return w;
   lrq::MatmulArgs a{x, nullptr, codes, scales, bias, out, ld, rows, n, k, (k + 127) / 128, bias_dtype, x_dtype};
-  if (lrq::matmul_quantizes(rows, k)) return check_hip(lrq::launch_matmul(a, x_dtype, (hipStream_t)stream), "kernel launch");
-  if (workspace_bytes < lrq_fp8_block_linear_workspace(rows, k) || !workspace)
-    return fail(LRQ_ERR_CAPACITY, "fp8_block_linear: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-                (long long)lrq_fp8_block_linear_workspace(rows, k));
-  if (!aligned(workspace, 256)) return fail(LRQ_ERR_ALIGN, "fp8_block_linear: workspace must be 256-byte aligned");
+  if (lrq::matmul_quantizes(rows, k))
+    return check_hip(lrq::launch_matmul(a, x_dtype, nullptr, (hipStream_t)stream), "kernel launch");
   uint8_t* const x_codes = static_cast<uint8_t*>(workspace);
   float* const x_scales = reinterpret_cast<float*>(x_codes + (rows * k + 255) / 256 * 256);
   if (int q = lrq_fp8_block_quant(x, x_dtype, 1, rows, k, ld, rows * ld, 1, 128, x_codes, x_scales, 0, stream)) return q;
   a.x = x_codes, a.sx = x_scales, a.ldx = k;
-  return check_hip(lrq::launch_matmul(a, -1, (hipStream_t)stream), "kernel launch");
+  return check_hip(lrq::launch_matmul(a, -1, x_codes + quantized_bytes(rows, k), (hipStream_t)stream), "kernel launch");
 }
 
 namespace {

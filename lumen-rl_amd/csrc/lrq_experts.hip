@@ -124,82 +124,7 @@ __device__ __forceinline__ void store_hidden(const ExpertArgs& a, f32x4 (&h)[NS]
 }
 
 // ---------------------------------------------------------------------------
-// Some rows an expert: weights from memory into registers
-// ---------------------------------------------------------------------------
-// A work-group of 8 waves takes a tile of 16 MT pairs and 128 columns of h (or of
-// out), a wave 16 of them over the whole of K.
-struct UpRows {
-  const ExpertArgs& a;
-  const ExpertTile& t;
-  int n, c;
-  const uint8_t* wb;
-  const float* sb;
-  __device__ int row(int j) const { const int r = 16 * j + c; return r < t.rows ? r : t.rows - 1; }
-  __device__ int64_t token(int j) const { return gld<int32_t>(a.order + t.first + row(j)) / a.top_k; }
-  __device__ const uint8_t* w(int i) const { return wb + (int64_t)(i * a.inter + n + c) * a.hidden; }
-  __device__ const float* sw(int i) const { return sb + (int64_t)((i * a.inter + n) / kBlk) * a.kb; }
-  __device__ const uint8_t* x(int j) const { return a.xq + token(j) * a.hidden; }
-  __device__ const float* sx(int j) const { return a.xs + token(j) * a.kb; }
-};
-
-template <int MT>
-__global__ __launch_bounds__(512) void k_ex_up_rows(ExpertArgs a) {
-  __shared__ uint32_t amax[8 * 16 * MT];
-  int tile, block;
-  if (!expert_piece(blockIdx.x, gld<int32_t>(a.total), a.ib, tile, block)) return;
-  const ExpertTile t = a.tiles[tile];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = 128 * block + 16 * wave;
-  f32x4 h[1][MT];
-#pragma unroll
-  for (int j = 0; j < MT; ++j) h[0][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  if (n < a.inter) {
-    const UpRows src{a, t, n, lane & 15, a.gu + (int64_t)t.expert * 2 * a.inter * a.hidden, a.gus + (int64_t)t.expert * a.gb * a.kb};
-    f32x4 acc[2][MT];
-    row_sums<2, MT, 2, false, true>(src, 0, a.kb, a.hidden, acc, [] {});
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) h[0][j][r] = silu_mul(acc[0][j][r], acc[1][j][r]);
-  }
-  store_hidden<1, MT, 8>(a, h, t.first, 0, t.rows, block, wave, amax, 16 * MT);
-}
-
-struct DownRows {
-  const ExpertArgs& a;
-  const ExpertTile& t;
-  int n, c;
-  const uint8_t* wb;
-  const float* sb;
-  __device__ int row(int j) const { const int r = 16 * j + c; return r < t.rows ? r : t.rows - 1; }
-  __device__ const uint8_t* w(int) const { return wb + (int64_t)(n + c) * a.inter; }
-  __device__ const float* sw(int) const { return sb + (int64_t)(n / kBlk) * a.ib; }
-  __device__ const uint8_t* x(int j) const { return a.hq + (int64_t)(t.first + row(j)) * a.inter; }
-  __device__ const float* sx(int j) const { return a.hs + (int64_t)(t.first + row(j)) * a.ib; }
-};
-
-template <int MT>
-__global__ __launch_bounds__(512) void k_ex_down_rows(ExpertArgs a) {
-  int tile, block;
-  if (!expert_piece(blockIdx.x, gld<int32_t>(a.total), a.kb, tile, block)) return;
-  const ExpertTile t = a.tiles[tile];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4, n = 128 * block + 16 * wave;
-  if (n >= a.hidden) return;
-  const DownRows src{a, t, n, c, a.dn + (int64_t)t.expert * a.hidden * a.inter, a.dns + (int64_t)t.expert * a.kb * a.ib};
-  f32x4 acc[1][MT];
-  row_sums<1, MT, 2, false, true>(src, 0, a.ib, a.inter, acc, [] {});
-#pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    if (16 * j + c >= t.rows) continue;
-    const int pair = gld<int32_t>(a.order + t.first + 16 * j + c);
-    const float w = gld<float>(a.weights + pair);
-    gst<f32x4>(a.y + (int64_t)pair * a.hidden + n + 4 * g, f32x4{acc[0][j][0] * w, acc[0][j][1] * w, acc[0][j][2] * w, acc[0][j][3] * w});
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Many rows an expert: tiles through LDS
+// An expert's rows in tiles
 // ---------------------------------------------------------------------------
 // Weight rows of a tile: 16 of gate, the same 16 of up, and so on.
 struct UpTile {
@@ -229,7 +154,7 @@ struct UpTile {
   }
 };
 
-template <int FN, int FM, int WN, int WM, int STAGES>
+template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
 __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
   static_assert(16 * FN * WN == 256, "128 columns of h");
   constexpr int BM = 16 * FM * WM;
@@ -240,7 +165,7 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const UpTile src{a, t, block};
   f32x4 acc[FN][FM], h[FN / 2][FM];
-  tile_sums<FN, FM, WN, WM, STAGES, true, true, false>(src, a.hidden, lds, acc);
+  tile_sums<FN, FM, WN, WM, STAGES, true, true, EXACT>(src, a.hidden, 0, a.kb, lds, acc);
 #pragma unroll
   for (int i = 0; i < FN / 2; ++i)
 #pragma unroll
@@ -272,7 +197,7 @@ struct DownTile {
   }
 };
 
-template <int FN, int FM, int WN, int WM, int STAGES>
+template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
 __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_down_tiles(ExpertArgs a) {
   constexpr int BN = 16 * FN * WN;
   static_assert(16 * FN <= kBlk, "one scale for a wave's rows");
@@ -284,7 +209,7 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_down_tiles(ExpertArgs a)
   const int c = lane & 15, g = lane >> 4, wn = wave / WM * 16 * FN, wm = wave % WM * 16 * FM;
   const DownTile src{a, t, block * BN};
   f32x4 acc[FN][FM];
-  tile_sums<FN, FM, WN, WM, STAGES, true, false, false>(src, a.inter, lds, acc);
+  tile_sums<FN, FM, WN, WM, STAGES, true, false, EXACT>(src, a.inter, 0, a.ib, lds, acc);
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
     const int row = wm + 16 * j + c;
@@ -323,107 +248,106 @@ __global__ __launch_bounds__(256) void k_ex_sum(ExpertArgs a) {
 // ---------------------------------------------------------------------------
 // Few pairs
 // ---------------------------------------------------------------------------
-// h of a pair and 16 columns: x is quantized by every work-group, K is split over
-// its 8 waves.
-struct OneRow {
-  const uint8_t* w0;   // lane's row of weight strip 0
-  int64_t w_step;      // bytes to strip 1's
-  const float *s0, *s1;
-  const uint8_t* codes;
-  const float* scales;
-  int at;
-  __device__ const uint8_t* w(int i) const { return w0 + i * w_step; }
-  __device__ const float* sw(int i) const { return i ? s1 : s0; }
-  __device__ const uint8_t* x(int) const { return nullptr; }
-  __device__ const float* sx(int) const { return nullptr; }
-  __device__ Codes32 block(int, int kb) const {
-    const uint8_t* p = codes + kb * kBlk + at;
-    return {*reinterpret_cast<const v4u*>(p), *reinterpret_cast<const v4u*>(p + 64)};
-  }
-  __device__ float scale(int, int kb) const { return scales[kb]; }
-};
-
+// h of a pair: a wave makes one column, from its rows of gate and up; x is
+// quantized by every work-group while the first weights are on their way.
 template <int DT>
 __global__ __launch_bounds__(512) void k_ex_up_few(ExpertArgs a) {
+  constexpr int D = 4;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int pair = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int pair = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int expert = gld<int32_t>(a.ids + pair);
   if ((uint32_t)expert >= (uint32_t)a.experts) return;
-  const int c = lane & 15, g = lane >> 4, n = 16 * blockIdx.x;
-  uint8_t* const codes = lds;
-  float* const scales = reinterpret_cast<float*>(lds + a.kb * kBlk);
-  const uint8_t* const gu = a.gu + (int64_t)expert * 2 * a.inter * a.hidden;
-  const float* const gus = a.gus + (int64_t)expert * a.gb * a.kb;
-  const OneRow src{gu + (int64_t)(n + c) * a.hidden, (int64_t)a.inter * a.hidden, gus + (int64_t)(n / kBlk) * a.kb,
-                   gus + (int64_t)((a.inter + n) / kBlk) * a.kb, codes, scales, 16 * g};
-  const int steps = (a.kb + 7) / 8, kb0 = wave * steps, kb1 = kb0 + steps < a.kb ? kb0 + steps : a.kb;
-  f32x4 acc[2][1];
-  row_sums<2, 1, 2, true, true>(src, kb0, kb1, a.hidden, acc, [&] {
-    const void* const x = static_cast<const uint8_t*>(a.x) + (int64_t)(pair / a.top_k) * a.ldx * 2;
-    for (int b = tid >> 4; b < a.kb; b += 32) {
-      float v[8], s;
-      load_acts<DT>(x, b * kBlk + 8 * (tid & 15), a.hidden, v);
-      *reinterpret_cast<v2u*>(codes + b * kBlk + 8 * (tid & 15)) = quant8(v, s);
-      if ((tid & 15) == 0) scales[b] = s;
-    }
-    lds_barrier8();
-  });
-  lds_barrier8();
-  float* const red = reinterpret_cast<float*>(lds);  // [wave][gate, up][row]
-  if (c == 0) {
-    *reinterpret_cast<f32x4*>(red + wave * 32 + 4 * g) = acc[0][0];
-    *reinterpret_cast<f32x4*>(red + wave * 32 + 16 + 4 * g) = acc[1][0];
-  }
-  lds_barrier8();
-  if (tid < 16) {
-    float gate = 0.0f, up = 0.0f;
+  const int n = 8 * blockIdx.x + wave, chunks = (a.hidden + 1023) / 1024, pitch = a.kb * kBlk;
+  float* const scales = reinterpret_cast<float*>(lds + pitch);
+  const GlobalCodes w[2] = {(GlobalCodes)a.gu + ((int64_t)expert * 2 * a.inter + n) * a.hidden,
+                            (GlobalCodes)a.gu + ((int64_t)expert * 2 * a.inter + a.inter + n) * a.hidden};
+  const float* const sw[2] = {a.gus + ((int64_t)expert * a.gb + n / kBlk) * a.kb,
+                              a.gus + ((int64_t)expert * a.gb + (a.inter + n) / kBlk) * a.kb};
+  struct Chunk {
+    v4u w[2];
+    float s[2];
+  } st[D];
+  auto load = [&](Chunk& c, int i) {
+    if (i >= chunks) return;
+    const int at = 1024 * i + 16 * lane, kb = at < a.hidden ? at / kBlk : 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) gate += red[w * 32 + tid], up += red[w * 32 + 16 + tid];
-    gst<float>(a.y + (int64_t)pair * a.inter + n + tid, silu_mul(gate, up));
+    for (int r = 0; r < 2; ++r) {
+      c.w[r] = at < a.hidden ? load_codes_nt(w[r] + at) : v4u{0, 0, 0, 0};
+      c.s[r] = gld<float>(sw[r] + kb);
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) load(st[d], d);
+  quant_row<DT, 512>(static_cast<const uint8_t*>(a.x) + (int64_t)(pair / a.top_k) * a.ldx * 2, a.hidden, a.kb, lds, scales);
+  lds_barrier8();
+  float acc[2] = {0.0f, 0.0f};
+  for (int i0 = 0; i0 < chunks; i0 += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (i0 + d >= chunks) break;
+      const int at = 1024 * (i0 + d) + 16 * lane, x_at = at < a.hidden ? at : 0;
+      const Floats16 x = codes_to_f32(*reinterpret_cast<const v4u*>(lds + x_at));
+      const float s = scales[x_at / kBlk];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float p = dot16(codes_to_f32(st[d].w[r]), x);
+        acc[r] = at < a.hidden ? __builtin_fmaf(p, s * st[d].s[r], acc[r]) : acc[r];
+      }
+      load(st[d], i0 + d + D);
+    }
   }
+  const float g = lanes_sum(acc[0]), u = lanes_sum(acc[1]);
+  if (lane == 0) gst<float>(a.y + (int64_t)pair * a.inter + n, silu_mul(g, u));
 }
 
-// 16 columns of a token's output: its pairs' h are quantized by every work-group;
-// its 8 waves take the pairs, or parts of their K.
+// A token's output: a wave makes one column of all its pairs, whose h every
+// work-group quantizes; the pairs' K stand one after another.
 template <int DT>
 __global__ __launch_bounds__(512) void k_ex_down_few(ExpertArgs a) {
+  constexpr int D = 6;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int t = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 15, g = lane >> 4, n = 16 * blockIdx.x, blocks = a.top_k * a.ib;
-  uint8_t* const codes = lds;
-  float* const scales = reinterpret_cast<float*>(lds + blocks * kBlk);
-  for (int b = tid >> 4; b < blocks; b += 32) {
-    float v[8], s;
-    const int j = b / a.ib, kb = b % a.ib;
-    load_acts<kF32>(a.y + ((int64_t)t * a.top_k + j) * a.inter, kb * kBlk + 8 * (tid & 15), a.inter, v);
-    *reinterpret_cast<v2u*>(codes + b * kBlk + 8 * (tid & 15)) = quant8(v, s);
-    if ((tid & 15) == 0) scales[b] = s;
-  }
-  lds_barrier8();
-  const int parts = a.top_k >= 8 ? 1 : 8 / a.top_k, step = (a.ib + parts - 1) / parts;
-  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int u = wave; u < a.top_k * parts; u += 8) {
-    const int j = u / parts, kb0 = u % parts * step, kb1 = kb0 + step < a.ib ? kb0 + step : a.ib;
-    const int expert = gld<int32_t>(a.ids + (int64_t)t * a.top_k + j);
-    if ((uint32_t)expert >= (uint32_t)a.experts || kb0 >= kb1) continue;
-    const float* const s = a.dns + ((int64_t)expert * a.kb + n / kBlk) * a.ib;
-    const OneRow src{a.dn + ((int64_t)expert * a.hidden + n + c) * a.inter, 0, s, s, codes + j * a.ib * kBlk, scales + j * a.ib, 16 * g};
-    f32x4 acc[1][1];
-    row_sums<1, 1, 4, true, true>(src, kb0, kb1, a.inter, acc, [] {});
-    const float w = gld<float>(a.weights + (int64_t)t * a.top_k + j);
+  const int t = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = 8 * blockIdx.x + wave, each = a.inter / 16, pieces = a.top_k * each, chunks = (pieces + 63) / 64;
+  const int pitch = a.ib * kBlk;
+  float* const scales = reinterpret_cast<float*>(lds + a.top_k * pitch);
+  // lane j holds pair j's expert and weight
+  const int64_t first = (int64_t)t * a.top_k;
+  const int id = lane < a.top_k ? gld<int32_t>(a.ids + first + lane) : -1;
+  const float weight = lane < a.top_k ? gld<float>(a.weights + first + lane) : 0.0f;
+  struct Chunk {
+    v4u w;
+    float s;
+    int at;  // of the piece in LDS, -1: none
+  } st[D];
+  auto load = [&](Chunk& c, int i) {
+    if (i >= chunks) return;
+    const int p = 64 * i + lane, j = p < pieces ? p / each : 0, k = 16 * (p - j * each);
+    const int expert = __shfl(id, j, 64);
+    const float f = __shfl(weight, j, 64);
+    c.at = p < pieces && (uint32_t)expert < (uint32_t)a.experts ? j * pitch + k : -1;
+    c.w = v4u{0, 0, 0, 0}, c.s = 0.0f;
+    if (c.at < 0) return;
+    c.w = load_codes_nt((GlobalCodes)a.dn + (((int64_t)expert * a.hidden + n) * a.inter + k));
+    c.s = f * gld<float>(a.dns + ((int64_t)expert * a.kb + n / kBlk) * a.ib + k / kBlk);
+  };
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sum[r] = __builtin_fmaf(acc[0][0][r], w, sum[r]);
-  }
+  for (int d = 0; d < D; ++d) load(st[d], d);
+  for (int j = 0; j < a.top_k; ++j)
+    quant_row<kF32, 512>(a.y + (first + j) * a.inter, a.inter, a.ib, lds + j * pitch, scales + j * a.ib);
   lds_barrier8();
-  float* const red = reinterpret_cast<float*>(lds);
-  if (c == 0) *reinterpret_cast<f32x4*>(red + wave * 16 + 4 * g) = sum;
-  lds_barrier8();
-  if (tid < 16) {
-    float v = 0.0f;
+  float acc = 0.0f;
+  for (int i0 = 0; i0 < chunks; i0 += D) {
 #pragma unroll
-    for (int w = 0; w < 8; ++w) v += red[w * 16 + tid];
-    gst<uint16_t>(static_cast<uint16_t*>(a.out) + (int64_t)t * a.hidden + n + tid, bits16<DT>(v));
+    for (int d = 0; d < D; ++d) {
+      if (i0 + d >= chunks) break;
+      const int at = st[d].at < 0 ? 0 : st[d].at;
+      const float p = dot16(codes_to_f32(st[d].w), codes_to_f32(*reinterpret_cast<const v4u*>(lds + at)));
+      acc = st[d].at < 0 ? acc : __builtin_fmaf(p, scales[at / kBlk] * st[d].s, acc);
+      load(st[d], i0 + d + D);
+    }
   }
+  acc = lanes_sum(acc);
+  if (lane == 0) gst<uint16_t>(static_cast<uint16_t*>(a.out) + (int64_t)t * a.hidden + n, bits16<DT>(acc));
 }
 
 // ---------------------------------------------------------------------------
@@ -480,15 +404,21 @@ int64_t experts_workspace(int64_t tokens, ExpertArgs a) {
 template <int DT>
 static hipError_t few(const ExpertArgs& a, hipStream_t stream) {
   const unsigned up = (unsigned)(a.kb * (kBlk + 4)), down = (unsigned)(a.top_k * a.ib * (kBlk + 4));
-  hipLaunchKernelGGL((k_ex_up_few<DT>), dim3((unsigned)(a.inter / 16), (unsigned)(a.tokens * a.top_k)), dim3(512), up < 1024 ? 1024 : up, stream, a);
-  hipLaunchKernelGGL((k_ex_down_few<DT>), dim3((unsigned)(a.hidden / 16), (unsigned)a.tokens), dim3(512), down < 512 ? 512 : down, stream, a);
+  hipLaunchKernelGGL((k_ex_up_few<DT>), dim3((unsigned)(a.inter / 8), (unsigned)(a.tokens * a.top_k)), dim3(512), up, stream, a);
+  hipLaunchKernelGGL((k_ex_down_few<DT>), dim3((unsigned)(a.hidden / 8), (unsigned)a.tokens), dim3(512), down, stream, a);
   return hipGetLastError();
 }
 
-template <int MT>
-static void by_rows(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
-  hipLaunchKernelGGL((k_ex_up_rows<MT>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(512), 0, stream, a);
-  hipLaunchKernelGGL((k_ex_down_rows<MT>), dim3((unsigned)((tiles * a.kb + 7) / 8 * 8)), dim3(512), 0, stream, a);
+template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
+static void up(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
+  hipLaunchKernelGGL((k_ex_up_tiles<FN, FM, WN, WM, STAGES, EXACT>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(64 * WN * WM), 0,
+                     stream, a);
+}
+template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
+static void down(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
+  constexpr int BN = 16 * FN * WN;
+  hipLaunchKernelGGL((k_ex_down_tiles<FN, FM, WN, WM, STAGES, EXACT>), dim3((unsigned)((tiles * ((a.hidden + BN - 1) / BN) + 7) / 8 * 8)),
+                     dim3(64 * WN * WM), 0, stream, a);
 }
 
 hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspace, ExpertQuant quant, hipStream_t stream) {
@@ -510,12 +440,14 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
     if (hipError_t e = quant(a, dtype, stream)) return e;
     hipLaunchKernelGGL(k_ex_sort, dim3(1), dim3(kSortThreads), 0, stream, a.ids, (int)pairs, a.experts, bm, a.tiles, a.total, a.order);
     if (bm == 16) {
-      by_rows<1>(a, tiles, stream);
+      up<2, 1, 8, 1, 2, true>(a, tiles, stream);
+      down<1, 1, 8, 1, 3, true>(a, tiles, stream);
     } else if (bm == 32) {
-      by_rows<2>(a, tiles, stream);
+      up<2, 2, 8, 1, 2, true>(a, tiles, stream);
+      down<1, 2, 8, 1, 3, true>(a, tiles, stream);
     } else {
-      hipLaunchKernelGGL((k_ex_up_tiles<4, 4, 4, 2, 3>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(512), 0, stream, a);
-      hipLaunchKernelGGL((k_ex_down_tiles<4, 4, 2, 2, 4>), dim3((unsigned)((tiles * ((a.hidden + 127) / 128) + 7) / 8 * 8)), dim3(256), 0, stream, a);
+      up<4, 4, 4, 2, 3, false>(a, tiles, stream);
+      down<4, 4, 2, 2, 4, false>(a, tiles, stream);
     }
     const dim3 sum((unsigned)((a.tokens * a.hidden / 8 + 255) / 256));
     if (dtype == kBF16) hipLaunchKernelGGL((k_ex_sum<kBF16>), sum, dim3(256), 0, stream, a);

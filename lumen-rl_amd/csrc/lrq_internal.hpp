@@ -282,8 +282,10 @@ struct MatmulArgs {
 };
 // true: launch_matmul takes values of x, whatever n is
 bool matmul_quantizes(int64_t m, int64_t k);
+// device memory that launch_matmul needs for the sums of parts of K
+int64_t matmul_workspace(int64_t m, int64_t n, int64_t k);
 // x_dtype: the type of x's values, or -1: codes
-hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, hipStream_t stream);
+hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, void* workspace, hipStream_t stream);
 
 // Routing to experts (lrq_route.hip).
 constexpr int kRouteExpertsMax = 512, kRouteGroupsMax = 16;  // one lane of 16 looks through a group

@@ -14,96 +14,97 @@ __device__ __forceinline__ void store_y(const MatmulArgs& a, int64_t at, float v
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens
+// Up to four tokens
 // ---------------------------------------------------------------------------
-// A work-group of KW waves makes 16 NT weight rows x 16 MT tokens; each wave
-// takes a run of K blocks, and their sums meet in LDS.
-struct RowsFromCodes {
-  const MatmulArgs& a;
-  int n0, m0, c;
-  __device__ int row(int i) const { const int n = n0 + 16 * i + c; return n < a.n ? n : (int)a.n - 1; }
-  __device__ int64_t token(int j) const { const int64_t m = (int64_t)m0 + 16 * j + c; return m < a.m ? m : a.m - 1; }
-  __device__ const uint8_t* w(int i) const { return a.w + (int64_t)row(i) * a.k; }
-  __device__ const float* sw(int i) const {
-    const int n = n0 + 16 * i;
-    return a.sw + (int64_t)((n < a.n ? n : (int)a.n - 1) / kBlk) * a.kb;
-  }
-  __device__ const uint8_t* x(int j) const { return static_cast<const uint8_t*>(a.x) + token(j) * a.ldx; }
-  __device__ const float* sx(int j) const { return a.sx + token(j) * a.kb; }
-};
-
-// Tokens quantized by the work-group itself into LDS: rows of `pitch` bytes,
-// their scales behind them.
-struct RowsFromLds : RowsFromCodes {
-  const uint8_t* codes;
-  const float* scales;
-  int pitch;
-  __device__ int mine(int j) const { const int m = 16 * j + c; return m < a.m ? m : (int)a.m - 1; }
-  __device__ Codes32 block(int j, int kb) const {
-    const uint8_t* p = codes + mine(j) * pitch + kb * kBlk + 16 * ((threadIdx.x & 63) >> 4);
-    return {*reinterpret_cast<const v4u*>(p), *reinterpret_cast<const v4u*>(p + 64)};
-  }
-  __device__ float scale(int j, int kb) const { return scales[mine(j) * (int)a.kb + kb]; }
-};
-
-template <int DT, int T>
-__device__ __forceinline__ void quant_to_lds(const MatmulArgs& a, uint8_t* codes, float* scales, int pitch) {
-  const int groups = (int)(a.m * a.kb);  // 16 lanes each
-  for (int e = threadIdx.x >> 4; e < groups; e += T / 16) {
-    const int m = e / (int)a.kb, kb = e % (int)a.kb, at = kb * kBlk + 8 * (threadIdx.x & 15);
-    float v[8], s;
-    load_acts<DT>(static_cast<const uint8_t*>(a.x) + (int64_t)m * a.ldx * (DT == kF32 ? 4 : 2), at, (int)a.k, v);
-    *reinterpret_cast<v2u*>(codes + m * pitch + at) = quant8(v, s);
-    if ((threadIdx.x & 15) == 0) scales[e] = s;
-  }
-}
-
-constexpr int kRowWaves = 8;
-// XDT: the type of x, or -1: codes and scales
-template <int XDT, int NT, int MT, int D>
-__global__ __launch_bounds__(64 * kRowWaves) void k_mm8_rows(MatmulArgs a) {
-  constexpr int KW = kRowWaves, CELLS = 256 * NT * MT;
+// A wave makes R rows of up to M tokens, 1024 k at a time.  XDT: the type of x,
+// which the work-group quantizes into LDS while the first weights are on their
+// way, or -1: codes and scales.
+template <int XDT, int M, int R>
+__global__ __launch_bounds__(512) void k_mm8_dot(MatmulArgs a) {
+  constexpr int D = 8 / R;  // chunks ahead
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
-  const int steps = (int)((a.kb + KW - 1) / KW);
-  const int kb0 = wave * steps, kb1 = kb0 + steps < a.kb ? kb0 + steps : (int)a.kb;
-  f32x4 acc[NT][MT];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int k = (int)a.k, kb_n = (int)a.kb, m_n = (int)a.m, chunks = (k + 1023) / 1024;
+  const int64_t n0 = ((int64_t)blockIdx.x * 8 + wave) * R;
+  const int64_t first = n0 < a.n ? n0 : a.n - 1;
+  GlobalCodes w[R], x[M];
+#pragma unroll
+  for (int r = 0; r < R; ++r) w[r] = (GlobalCodes)a.w + (n0 + r < a.n ? n0 + r : a.n - 1) * a.k;
+#pragma unroll
+  for (int m = 0; m < M; ++m) x[m] = (GlobalCodes)a.x + (m < m_n ? m : m_n - 1) * a.ldx;
+  const float* const sw = a.sw + first / kBlk * a.kb;
+  const int pitch = kb_n * kBlk;
+  const float* const sx = XDT >= 0 ? reinterpret_cast<const float*>(lds + m_n * pitch) : a.sx;
+  struct Chunk {
+    v4u w[R], x[XDT >= 0 ? 1 : M];
+    float s;
+  } st[D];
+  auto load = [&](Chunk& c, int i) {
+    if (i >= chunks) return;
+    const int at = 1024 * i + 16 * lane;
+    if (1024 * i + 1024 <= k) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) c.w[r] = load_codes_nt(w[r] + at);
+      if constexpr (XDT < 0)
+#pragma unroll
+        for (int m = 0; m < M; ++m) c.x[m] = load_codes(x[m] + at);
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) c.w[r] = load_codes_cut(w[r], at, k);
+      if constexpr (XDT < 0)
+#pragma unroll
+        for (int m = 0; m < M; ++m) c.x[m] = load_codes_cut(x[m], at, k);
+    }
+    c.s = gld<float>(sw + (at / kBlk < kb_n ? at / kBlk : kb_n - 1));
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) load(st[d], d);
   if constexpr (XDT >= 0) {
-    const int pitch = (int)a.kb * kBlk + 16;
-    float* const scales = reinterpret_cast<float*>(lds + a.m * pitch);
-    const RowsFromLds src{{a, n0, m0, c}, lds, scales, pitch};
-    row_sums<NT, MT, D, true, true>(src, kb0, kb1, (int)a.k, acc, [&] {
-      quant_to_lds<XDT, 64 * KW>(a, lds, scales, pitch);
-      lds_barrier8();
-    });
+    for (int m = 0; m < m_n; ++m)
+      quant_row<XDT, 512>(static_cast<const uint8_t*>(a.x) + m * a.ldx * (XDT == kF32 ? 4 : 2), k, kb_n, lds + m * pitch,
+                          const_cast<float*>(sx) + m * kb_n);
     lds_barrier8();
-  } else {
-    const RowsFromCodes src{a, n0, m0, c};
-    row_sums<NT, MT, D, false, true>(src, kb0, kb1, (int)a.k, acc, [] {});
   }
-  float* const red = reinterpret_cast<float*>(lds);  // [wave][token][row]
+  float acc[R][M];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int j = 0; j < MT; ++j)
-      *reinterpret_cast<f32x4*>(red + wave * CELLS + (16 * j + c) * 16 * NT + 16 * i + 4 * g) = acc[i][j];
-  lds_barrier8();
-  for (int e = tid; e < CELLS; e += 64 * KW) {
-    const int64_t m = (int64_t)m0 + e / (16 * NT);
-    const int n = n0 + e % (16 * NT);
-    if (m >= a.m || n >= a.n) continue;
-    float sum = red[e];
+    for (int m = 0; m < M; ++m) acc[r][m] = 0.0f;
+  for (int i0 = 0; i0 < chunks; i0 += D) {
 #pragma unroll
-    for (int w = 1; w < KW; ++w) sum += red[w * CELLS + e];
-    if (a.bias != nullptr) sum += load_as_f32(a.bias, a.bias_dtype, n);
-    store_y(a, m * a.n + n, sum);
+    for (int d = 0; d < D; ++d) {
+      if (i0 + d >= chunks) break;
+      const int at = 1024 * (i0 + d) + 16 * lane, kb = at / kBlk < kb_n ? at / kBlk : kb_n - 1;
+      Floats16 wf[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) wf[r] = codes_to_f32(st[d].w[r]);
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const int mm = m < m_n ? m : m_n - 1;
+        Floats16 xf;  // past the row's end w is 0 and x any
+        if constexpr (XDT >= 0) xf = codes_to_f32(*reinterpret_cast<const v4u*>(lds + mm * pitch + (at < pitch ? at : pitch - 16)));
+        else xf = codes_to_f32(st[d].x[m]);
+        const float s = (XDT >= 0 ? sx[mm * kb_n + kb] : gld<float>(sx + mm * a.kb + kb)) * st[d].s;
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r][m] = __builtin_fmaf(dot16(wf[r], xf), s, acc[r][m]);
+      }
+      load(st[d], i0 + d + D);
+    }
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      float sum = lanes_sum(acc[r][m]);
+      const int64_t n = n0 + r;
+      if (lane != 0 || m >= m_n || n >= a.n) continue;
+      if (a.bias != nullptr) sum += load_as_f32(a.bias, a.bias_dtype, n);
+      store_y(a, m * a.n + n, sum);
+    }
 }
 
 // ---------------------------------------------------------------------------
-// Many tokens
+// More: tiles
 // ---------------------------------------------------------------------------
 struct DenseTile {
   static constexpr bool kCut = true;
@@ -175,8 +176,9 @@ __device__ __forceinline__ void store_tile(const MatmulArgs& a, f32x4 (&acc)[FN]
   }
 }
 
-template <int FN, int FM, int WN, int WM, int STAGES, bool DMA, bool EXACT>
-__global__ __launch_bounds__(64 * WN * WM, 1) void k_mm8_tiles(MatmulArgs a, int tiles_m, int tiles_n) {
+// SPLIT: K in gridDim.y parts, whose sums go to `parts` [part][token][row] in float32.
+template <int FN, int FM, int WN, int WM, int STAGES, bool DMA, bool EXACT, bool SPLIT>
+__global__ __launch_bounds__(64 * WN * WM, 1) void k_mm8_tiles(MatmulArgs a, int tiles_m, int tiles_n, float* parts) {
   constexpr int BN = 16 * FN * WN, BM = 16 * FM * WM, kLds = kTileLds<FN, FM, WN, WM, STAGES>;
   static_assert(WN * WM * 16 * (64 * FN + 16) <= kLds, "results pass through the stages");
   __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
@@ -186,10 +188,28 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_mm8_tiles(MatmulArgs a, int
   const int wn = (wave / WM) * 16 * FN, wm = (wave % WM) * 16 * FM;
   const DenseTile src{a, tn * BN, tm * BM, (int)a.n - 1 - tn * BN, (int)a.m - 1 - tm * BM, DMA};
   f32x4 acc[FN][FM];
-  tile_sums<FN, FM, WN, WM, STAGES, DMA, false, EXACT>(src, (int)a.k, lds, acc);
-  if constexpr (EXACT) return store_tile<kF32>(a, acc, src.n0 + wn, src.m0 + wm, lds);
-  else if (a.out_dtype == kBF16) return store_tile<kBF16>(a, acc, src.n0 + wn, src.m0 + wm, lds);
-  else return store_tile<kF16>(a, acc, src.n0 + wn, src.m0 + wm, lds);
+  if constexpr (SPLIT) {
+    const int steps = ((int)a.kb + gridDim.y - 1) / gridDim.y, kb0 = steps * blockIdx.y;
+    tile_sums<FN, FM, WN, WM, STAGES, DMA, false, EXACT>(src, (int)a.k, kb0, kb0 + steps < a.kb ? kb0 + steps : (int)a.kb, lds, acc);
+    MatmulArgs part = a;
+    part.bias = nullptr, part.y = parts + blockIdx.y * a.m * a.n;
+    store_tile<kF32>(part, acc, src.n0 + wn, src.m0 + wm, lds);
+  } else {
+    tile_sums<FN, FM, WN, WM, STAGES, DMA, false, EXACT>(src, (int)a.k, 0, (int)a.kb, lds, acc);
+    if (EXACT && a.out_dtype == kF32) return store_tile<kF32>(a, acc, src.n0 + wn, src.m0 + wm, lds);
+    if (a.out_dtype == kBF16) return store_tile<kBF16>(a, acc, src.n0 + wn, src.m0 + wm, lds);
+    else return store_tile<kF16>(a, acc, src.n0 + wn, src.m0 + wm, lds);
+  }
+}
+
+// The parts' sum, in their order.
+__global__ __launch_bounds__(256) void k_mm8_join(MatmulArgs a, const float* parts, int count) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, cells = a.m * a.n;
+  if (at >= cells) return;
+  float sum = gld<float>(parts + at);
+  for (int p = 1; p < count; ++p) sum += gld<float>(parts + p * cells + at);
+  if (a.bias != nullptr) sum += load_as_f32(a.bias, a.bias_dtype, at % a.n);
+  store_y(a, at, sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -200,46 +220,64 @@ static bool dma_ok(const MatmulArgs& a) {
   return a.k % 4 == 0 && a.ldx % 4 == 0 && reinterpret_cast<uintptr_t>(a.x) % 4 == 0 && reinterpret_cast<uintptr_t>(a.w) % 4 == 0;
 }
 
-template <int FN, int FM, int WN, int WM, int STAGES, bool DMA, bool EXACT>
-static void launch_tiles(const MatmulArgs& a, hipStream_t stream) {
+template <int FN, int FM, int WN, int WM, int STAGES, bool DMA, bool EXACT, bool SPLIT = false>
+static void launch_tiles(const MatmulArgs& a, hipStream_t stream, float* parts = nullptr, int count = 1) {
   const int tiles_m = (int)ceil_div(a.m, 16 * FM * WM), tiles_n = (int)ceil_div(a.n, 16 * FN * WN);
-  hipLaunchKernelGGL((k_mm8_tiles<FN, FM, WN, WM, STAGES, DMA, EXACT>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64 * WN * WM), 0, stream, a,
-                     tiles_m, tiles_n);
+  hipLaunchKernelGGL((k_mm8_tiles<FN, FM, WN, WM, STAGES, DMA, EXACT, SPLIT>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)count),
+                     dim3(64 * WN * WM), 0, stream, a, tiles_m, tiles_n, parts);
 }
-template <int XDT, int NT, int MT, int D>
-static void launch_rows(const MatmulArgs& a, int64_t x_lds, hipStream_t stream) {
-  const int64_t sums = 4 * 256 * NT * MT * kRowWaves;
-  const dim3 grid((unsigned)ceil_div(a.n, 16 * NT), (unsigned)ceil_div(a.m, 16 * MT));
-  hipLaunchKernelGGL((k_mm8_rows<XDT, NT, MT, D>), grid, dim3(64 * kRowWaves), (unsigned)(sums > x_lds ? sums : x_lds), stream, a);
+template <int XDT, int M, int R>
+static void launch_dot(const MatmulArgs& a, hipStream_t stream) {
+  const unsigned lds = XDT >= 0 ? (unsigned)(a.m * a.kb * (kBlk + 4)) : 0;
+  hipLaunchKernelGGL((k_mm8_dot<XDT, M, R>), dim3((unsigned)ceil_div(a.n, 8 * R)), dim3(512), lds, stream, a);
+}
+template <int XDT>
+static void launch_dots(const MatmulArgs& a, hipStream_t stream) {
+  if (a.m == 1) a.n >= 4096 ? launch_dot<XDT, 1, 2>(a, stream) : launch_dot<XDT, 1, 1>(a, stream);
+  else if (a.m == 2) a.n >= 4096 ? launch_dot<XDT, 2, 2>(a, stream) : launch_dot<XDT, 2, 1>(a, stream);
+  else a.n >= 4096 ? launch_dot<XDT, 4, 2>(a, stream) : launch_dot<XDT, 4, 1>(a, stream);
 }
 
 template <bool DMA, bool EXACT>
 static void launch_tiles_of(const MatmulArgs& a, hipStream_t stream) {
-  if constexpr (DMA && !EXACT)
+  if constexpr (DMA && !EXACT) {
     if (ceil_div(a.m, 256) * ceil_div(a.n, 256) >= 200) return launch_tiles<8, 4, 2, 4, 2, DMA, EXACT>(a, stream);
+    if (ceil_div(a.m, 128) * ceil_div(a.n, 256) >= 200) return launch_tiles<4, 4, 4, 2, 3, DMA, EXACT>(a, stream);
+  }
   if (ceil_div(a.m, 128) * ceil_div(a.n, 128) >= 200) return launch_tiles<4, 4, 2, 2, DMA ? 4 : 2, DMA, EXACT>(a, stream);
   launch_tiles<2, 2, 2, 2, DMA ? 4 : 2, DMA, EXACT>(a, stream);
 }
 
-bool matmul_quantizes(int64_t m, int64_t k) {
-  return m <= 16 && m * (ceil_div(k, kBlk) * kBlk + 16 + 4 * ceil_div(k, kBlk)) <= 32768;
+constexpr int64_t kDots = 4, kSplitRows = 64;
+bool matmul_quantizes(int64_t m, int64_t k) { return m <= kDots && m * ceil_div(k, kBlk) * (kBlk + 4) <= 65536; }
+
+// Parts of K: a work-group for every CU, of 4 blocks at least.
+static int64_t split_parts(int64_t m, int64_t n, int64_t k) {
+  if (m <= kDots || m > kSplitRows) return 1;
+  const int64_t tiles = ceil_div(n, 64), kb = ceil_div(k, kBlk);
+  int64_t parts = 512 / tiles < kb / 4 ? 512 / tiles : kb / 4;
+  if (parts < 2) return 1;
+  return ceil_div(kb, ceil_div(kb, parts));  // none of them empty
+}
+int64_t matmul_workspace(int64_t m, int64_t n, int64_t k) {
+  const int64_t parts = split_parts(m, n, k);
+  return parts > 1 ? 4 * parts * m * n : 0;
 }
 
-hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, hipStream_t stream) {
-  if (x_dtype >= 0) {
-    const int64_t x_lds = a.m * (a.kb * kBlk + 16 + 4 * a.kb);
-    if (x_dtype == kBF16) launch_rows<kBF16, 1, 1, 4>(a, x_lds, stream);
-    else if (x_dtype == kF16) launch_rows<kF16, 1, 1, 4>(a, x_lds, stream);
-    else launch_rows<kF32, 1, 1, 4>(a, x_lds, stream);
-  } else if (a.m <= 16) {
-    launch_rows<-1, 1, 1, 4>(a, 0, stream);
-  } else if (a.m <= 32) {
-    launch_rows<-1, 1, 2, 2>(a, 0, stream);
-  } else if (a.m <= 64) {
-    launch_rows<-1, 1, 4, 2>(a, 0, stream);
-  } else if (a.out_dtype == kF32) {
-    if (dma_ok(a)) launch_tiles_of<true, true>(a, stream);
-    else launch_tiles_of<false, true>(a, stream);
+hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, void* workspace, hipStream_t stream) {
+  if (a.m <= kDots) {
+    if (x_dtype == kBF16) launch_dots<kBF16>(a, stream);
+    else if (x_dtype == kF16) launch_dots<kF16>(a, stream);
+    else if (x_dtype == kF32) launch_dots<kF32>(a, stream);
+    else launch_dots<-1>(a, stream);
+  } else if (const int64_t parts = split_parts(a.m, a.n, a.k); parts > 1) {
+    float* const sums = static_cast<float*>(workspace);
+    if (dma_ok(a)) launch_tiles<1, 4, 4, 1, 4, true, true, true>(a, stream, sums, (int)parts);
+    else launch_tiles<1, 4, 4, 1, 2, false, true, true>(a, stream, sums, (int)parts);
+    hipLaunchKernelGGL(k_mm8_join, dim3((unsigned)ceil_div(a.m * a.n, 256)), dim3(256), 0, stream, a, sums, (int)parts);
+  } else if (a.m <= kSplitRows || a.out_dtype == kF32) {
+    if (a.m > kSplitRows) dma_ok(a) ? launch_tiles_of<true, true>(a, stream) : launch_tiles_of<false, true>(a, stream);
+    else dma_ok(a) ? launch_tiles<1, 4, 4, 1, 4, true, true>(a, stream) : launch_tiles<1, 4, 4, 1, 2, false, true>(a, stream);
   } else {
     if (dma_ok(a)) launch_tiles_of<true, false>(a, stream);
     else launch_tiles_of<false, false>(a, stream);

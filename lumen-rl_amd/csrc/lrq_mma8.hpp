@@ -14,7 +14,8 @@
 //     own rounding is a hundred times that; or
 //   * EXACT: four bf16 instructions on the same codes, which are exact in bf16, as
 //     are their products; sums are float32.  Half the rate, and conversions.  Taken
-//     for float32 results, and wherever memory is the bound anyway (few tokens).
+//     for float32 results, and wherever memory is the bound anyway (few tokens); or
+//   * for up to four tokens, float32 multiply-adds.
 #pragma once
 
 #include "lrq_device.hpp"
@@ -212,30 +213,36 @@ constexpr int kTileSets = 2;
 template <int FN, int FM, int WN, int WM>
 constexpr int kTileStage = 16 * (FN * WN + FM * WM) * kBlk;
 template <int FN, int FM, int WN, int WM>
-constexpr int kTileScales = 16 * 64 * WN * WM;  // of four blocks: a place for every thread
+constexpr int kTileScaleWaves = (16 * FM * WM + 63) / 64 + (FN * WN + 63) / 64;  // a thread for every 16 bytes of scales
+template <int FN, int FM, int WN, int WM>
+constexpr int kTileScales = 1024 * kTileScaleWaves<FN, FM, WN, WM>;  // of four blocks
 template <int FN, int FM, int WN, int WM, int STAGES>
 constexpr int kTileLds = STAGES * kTileStage<FN, FM, WN, WM> + 2 * kTileScales<FN, FM, WN, WM>;
 
+// Blocks [kb0, kb1) of K.
 template <int FN, int FM, int WN, int WM, int STAGES, bool DMA, bool EACH, bool EXACT, class Src>
-__device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f32x4 (&acc)[FN][FM]) {
-  constexpr int T = 64 * WN * WM, BN = 16 * FN * WN, BM = 16 * FM * WM, TILES = FN * FM, LAG = TILES > 4 ? 3 : 1;
-  constexpr int PW = BN * 8 / T, PX = BM * 8 / T;  // 16-byte pieces a thread moves per block, and one scale
+__device__ __forceinline__ void tile_sums(const Src& src, int k, int kb0, int kb1, uint8_t* lds, f32x4 (&acc)[FN][FM]) {
+  constexpr int T = 64 * WN * WM, BN = 16 * FN * WN, BM = 16 * FM * WM, TILES = FN * FM, LAG = TILES > 4 ? 3 : TILES > 1 ? 1 : 0;
+  // 16-byte pieces a thread moves per block; of few tokens the first waves' threads alone
+  constexpr int PW = BN * 8 / T, PX = BM * 8 / T > 0 ? BM * 8 / T : 1, XWAVES = BM * 8 / 64 / PX;
+  constexpr int SW = (BM + 63) / 64 * 64, SWAVES = kTileScaleWaves<FN, FM, WN, WM>;  // scales: tokens' threads, then weights'
   constexpr int kStage = kTileStage<FN, FM, WN, WM>, kScales = kTileScales<FN, FM, WN, WM>;
-  static_assert(PW * T == BN * 8 && PX * T == BM * 8 && T % 128 == 0 && BM % 64 == 0 && BM + BN / 16 <= T, "");
+  static_assert(PW * T == BN * 8 && PX * XWAVES * 64 == BM * 8 && T % 128 == 0 && SWAVES <= WN * WM, "");
+  static_assert(XWAVES == WN * WM || DMA, "");
   static_assert(STAGES >= 2 && STAGES <= 5, "the next four blocks' scales arrive before them");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int wn = (wave / WM) * 16 * FN, wm = (wave % WM) * 16 * FM;
-  const int kb_n = (k + kBlk - 1) / kBlk;
+  const int kb_n = kb1 - kb0;
   const int piece = (tid & 7) ^ ((tid >> 4) & 7);  // of tile rows (T / 8) p + tid / 8
   uint32_t wo[PW], xo[PX];
 #pragma unroll
   for (int p = 0; p < PW; ++p) wo[p] = src.w_off((T / 8) * p + (tid >> 3)) + 16 * piece;
 #pragma unroll
-  for (int p = 0; p < PX; ++p) xo[p] = src.x_off((T / 8) * p + (tid >> 3)) + 16 * piece;
-  // the thread's scales: tokens first, then one for every 16 weight rows
-  const bool tokens = wave < BM / 64;
-  const uint32_t so = tokens ? src.sx_off(tid) : tid < BM + BN / 16 ? src.sw_off(tid - BM) : kNoRow;
+  for (int p = 0; p < PX; ++p) xo[p] = (wave < XWAVES ? src.x_off((T / 8) * p + (tid >> 3)) : 0) + 16 * piece;
+  // the thread's scales: of a token, or of 16 weight rows
+  const bool tokens = wave < SW / 64;
+  const uint32_t so = (tokens ? tid < BM ? src.sx_off(tid) : kNoRow : tid < SW + BN / 16 ? src.sw_off(tid - SW) : kNoRow) + 4 * kb0;
   uint8_t* const scales = lds + STAGES * kStage;
 #pragma unroll
   for (int i = 0; i < FN; ++i)
@@ -251,7 +258,7 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f
 #pragma unroll
     for (int j = 0; j < FM; ++j) s[j] = sc[4 * (wm + 16 * j + c)];
 #pragma unroll
-    for (int i = 0; i < (EACH ? FN : 1); ++i) si[i] = sc[4 * (BM + wn / 16 + i)];
+    for (int i = 0; i < (EACH ? FN : 1); ++i) si[i] = sc[4 * (SW + wn / 16 + i)];
     decltype(operand<EXACT>(Codes32{})) x[FM];
     Codes32 w[2];
     w[0] = {*reinterpret_cast<const v4u*>(cw + at0), *reinterpret_cast<const v4u*>(cw + at1)};
@@ -293,18 +300,19 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f
     const uint32_t to = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds) + 1024 * wave;
     auto fetch = [&](int kb, int stage) {
       // blocks past the last are asked for, so that every wait counts the same, and read as zeros
-      const uint32_t at = (uint32_t)(kb * kBlk), past = (int)at + 16 * piece < k ? 0 : kNoRow;
+      const uint32_t at = (uint32_t)((kb0 + kb) * kBlk), past = kb < kb_n && (int)at + 16 * piece < k ? 0 : kNoRow;
       const uint32_t here = to + (uint32_t)(stage * kStage);
 #pragma unroll
       for (int p = 0; p < PW; ++p) dma16(rw, (wo[p] + at) | past, here + 128 * (T / 8) * p);
+      if (wave < XWAVES)
 #pragma unroll
-      for (int p = 0; p < PX; ++p) dma16(rx, (xo[p] + at) | past, here + 128 * (BN + (T / 8) * p));
+        for (int p = 0; p < PX; ++p) dma16(rx, (xo[p] + at) | past, here + 128 * (BN + (T / 8) * p));
     };
     auto fetch_scales = [&](int kb) {  // of blocks kb .. kb + 3; those past a row's end are the next row's, and not used
-      dma16(rs, (so + 4 * kb) | (kb < kb_n ? 0 : kNoRow), to + (uint32_t)(STAGES * kStage + (kb >> 2 & 1) * kScales));
+      if (wave < SWAVES) dma16(rs, (so + 4 * kb) | (kb < kb_n ? 0 : kNoRow), to + (uint32_t)(STAGES * kStage + (kb >> 2 & 1) * kScales));
     };
     // a row's last codes, where 16 bytes would reach past its end: one row a thread
-    const bool cut = Src::kCut && k % 16 != 0;
+    const bool cut = Src::kCut && k % 16 != 0 && kb1 * kBlk >= k;
     v4u last = {0, 0, 0, 0};
     if (cut && tid < BN + BM) {
       const uint32_t off = tid < BN ? src.w_off(tid) : src.x_off(tid - BN);
@@ -324,8 +332,10 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f
       for (int r = 0; r < 4; ++r) {
         if (kb + r >= kb_n) break;
         // on their way since this block's codes were asked for: the blocks between, and scales
-        if (r >= 1 && r <= STAGES - 2) dma_wait<(STAGES - 2) * (PW + PX) + 1>();
-        else dma_wait<(STAGES - 2) * (PW + PX)>();
+        constexpr int kPer = STAGES - 2;
+        const bool more = r >= 1 && r <= STAGES - 2 && wave < SWAVES;
+        if (wave < XWAVES) more ? dma_wait<kPer * (PW + PX) + 1>() : dma_wait<kPer * (PW + PX)>();
+        else more ? dma_wait<kPer * PW + 1>() : dma_wait<kPer * PW>();
         lds_barrier8();  // every wave's part of this block is there, and every read of the last is done
         if (r == 0) fetch_scales(kb + 4);
         fetch(kb + r + STAGES - 1, free);
@@ -346,7 +356,7 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f
     float gs[kTileSets];
     const uint8_t* const sb = reinterpret_cast<const uint8_t*>(tokens ? src.sx() : src.sw());
     auto fetch = [&](int kb, int set) {
-      const int at = kb * kBlk;
+      const int at = kb < kb_n ? (kb0 + kb) * kBlk : k;
       if (at + kBlk <= k) {
 #pragma unroll
         for (int p = 0; p < PW; ++p) gw[set][p] = load_codes((GlobalCodes)src.w() + (wo[p] + at));
@@ -358,7 +368,7 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f
 #pragma unroll
         for (int p = 0; p < PX; ++p) gx[set][p] = load_codes_cut((GlobalCodes)src.x() + (xo[p] - 16 * piece), at + 16 * piece, k);
       }
-      gs[set] = so != kNoRow && kb < kb_n ? gld<float>(sb + (so + 4 * kb)) : 0.0f;
+      gs[set] = so < kNoRow && kb < kb_n ? gld<float>(sb + (so + 4 * kb)) : 0.0f;
     };
     auto put = [&](int set, int kb) {
       uint8_t* const s = lds + (kb & 1) * kStage + 16 * tid;
@@ -366,7 +376,7 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f
       for (int p = 0; p < PW; ++p) *reinterpret_cast<v4u*>(s + 128 * (T / 8) * p) = gw[set][p];
 #pragma unroll
       for (int p = 0; p < PX; ++p) *reinterpret_cast<v4u*>(s + 128 * (BN + (T / 8) * p)) = gx[set][p];
-      reinterpret_cast<float*>(scales + (kb >> 2 & 1) * kScales)[4 * tid + (kb & 3)] = gs[set];
+      if (wave < SWAVES) reinterpret_cast<float*>(scales + (kb >> 2 & 1) * kScales)[4 * tid + (kb & 3)] = gs[set];
     };
 #pragma unroll
     for (int s = 0; s < kTileSets; ++s) fetch(s, s);
@@ -387,101 +397,52 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, uint8_t* lds, f
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens: weights from memory into registers
+// A few tokens: dot products
 // ---------------------------------------------------------------------------
-// A wave's sums of 16 NT weight rows and 16 MT tokens over blocks [kb0, kb1).
-// Bound by the weight's bytes, each read once: a lane loads its own 32 codes of
-// a row, D blocks ahead, and nothing passes through LDS.
-// Src gives: w(i), x(j): the lane's row (l % 16) of weight rows 16 i .. and of
-// tokens 16 j ..; sx(j): its token's scales; sw(i): the weight rows' scales;
-// block(j, kb): the lane's codes of its token, where XOWN.
-// XOWN: tokens come from block(), and their scales from scale(j, kb).
-// `between` runs once the first loads are on their way.
-template <int NT, int MT>
-struct RowStage {
-  Codes32 w[NT], x[MT];
-  float sw[NT], sx[MT];
+// Up to four tokens are bound by the weight's bytes and by latency.  A wave takes
+// whole rows, 16 codes a lane and 1 KiB an instruction, several of them ahead; 24
+// vector instructions for 16 codes of a token keep up with memory, and nothing has
+// to be turned round for matrix instructions.
+struct Floats16 {
+  float v[16];
 };
-
-template <int NT, int MT, int D, bool XOWN, bool ONCE, class Src, class Between>
-__device__ __forceinline__ void row_sums(const Src& src, int kb0, int kb1, int k, f32x4 (&acc)[NT][MT], Between between) {
-  const int g = (threadIdx.x & 63) >> 4;
+__device__ __forceinline__ Floats16 codes_to_f32(v4u c) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  Floats16 r;
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  GlobalCodes wp[NT], xp[MT];
-  const float *swp[NT], *sxp[MT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) wp[i] = (GlobalCodes)src.w(i), swp[i] = src.sw(i);
-#pragma unroll
-  for (int j = 0; j < MT; ++j)
-    if constexpr (!XOWN) xp[j] = (GlobalCodes)src.x(j), sxp[j] = src.sx(j);
-  const int whole = k / kBlk < kb1 ? k / kBlk : kb1;  // blocks before a cut one
-  RowStage<NT, MT> st[D];
-  auto load = [&](RowStage<NT, MT>& a, int kb) {
-    kb = kb < whole ? kb : whole - 1;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const GlobalCodes q = wp[i] + (kb * kBlk + 16 * g);
-      a.w[i] = ONCE ? Codes32{load_codes_nt(q), load_codes_nt(q + 64)} : Codes32{load_codes(q), load_codes(q + 64)};
-      a.sw[i] = gld<float>(swp[i] + kb);
-    }
-    if constexpr (!XOWN) {
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const GlobalCodes q = xp[j] + (kb * kBlk + 16 * g);
-        a.x[j] = {load_codes(q), load_codes(q + 64)};
-        a.sx[j] = gld<float>(sxp[j] + kb);
-      }
-    }
-  };
-  auto multiply = [&](RowStage<NT, MT>& a, int kb) {
-    if constexpr (XOWN) {
-#pragma unroll
-      for (int j = 0; j < MT; ++j) a.x[j] = src.block(j, kb), a.sx[j] = src.scale(j, kb);
-    }
-    Wide32 x[MT];
-#pragma unroll
-    for (int j = 0; j < MT; ++j) x[j] = widen(a.x[j]);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const Wide32 w = widen(a.w[i]);
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const f32x4 p = mma8(w, x[j]);
-        const float s = a.sx[j] * a.sw[i];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(p[r], s, acc[i][j][r]);
-      }
-    }
-  };
-  if (kb0 < whole) {
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(st[d], kb0 + d);
+  for (int i = 0; i < 4; ++i) {
+    const f32x2 lo = e4m3x2_to_f32<false>(w[i]), hi = e4m3x2_to_f32<true>(w[i]);
+    r.v[4 * i] = lo.x, r.v[4 * i + 1] = lo.y, r.v[4 * i + 2] = hi.x, r.v[4 * i + 3] = hi.y;
   }
-  between();
-  int kb = kb0;
-  for (; kb + D <= whole; kb += D) {
+  return r;
+}
+__device__ __forceinline__ float dot16(const Floats16& a, const Floats16& b) {
+  float s = a.v[0] * b.v[0];
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      multiply(st[d], kb + d);
-      load(st[d], kb + d + D);
-    }
-  }
-#pragma unroll
-  for (int d = 0; d < D; ++d)
-    if (kb + d < whole) multiply(st[d], kb + d);
-  if (kb0 < kb1 && whole < kb1) {  // the last block of K, cut
-    RowStage<NT, MT>& a = st[0];
-    const int at = whole * kBlk + 16 * g;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) a.w[i] = {load_codes_cut(wp[i], at, k), load_codes_cut(wp[i], at + 64, k)}, a.sw[i] = gld<float>(swp[i] + whole);
-    if constexpr (!XOWN) {
-#pragma unroll
-      for (int j = 0; j < MT; ++j) a.x[j] = {load_codes_cut(xp[j], at, k), load_codes_cut(xp[j], at + 64, k)}, a.sx[j] = gld<float>(sxp[j] + whole);
-    }
-    multiply(a, whole);
+  for (int i = 1; i < 16; ++i) s = __builtin_fmaf(a.v[i], b.v[i], s);
+  return s;
+}
+// Over the wave; every lane is active.
+__device__ __forceinline__ float lanes_sum(float v) {
+#define LRQ_ADD_DPP(ctrl) v += u2f((uint32_t)__builtin_amdgcn_mov_dpp((int)f2u(v), ctrl, 0xF, 0xF, false))
+  LRQ_ADD_DPP(0xB1);
+  LRQ_ADD_DPP(0x4E);
+  LRQ_ADD_DPP(0x141);
+  LRQ_ADD_DPP(0x140);
+#undef LRQ_ADD_DPP
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+// The codes of `blocks` 1x128 blocks of a row of k values into LDS, and their
+// scales: 16 lanes a block, T threads.
+template <int DT, int T>
+__device__ __forceinline__ void quant_row(const void* row, int k, int blocks, uint8_t* codes, float* scales) {
+  const int l = threadIdx.x & 15;
+  for (int b = threadIdx.x >> 4; b < blocks; b += T / 16) {
+    float v[8], s;
+    load_acts<DT>(row, b * kBlk + 8 * l, k, v);
+    *reinterpret_cast<v2u*>(codes + b * kBlk + 8 * l) = quant8(v, s);
+    if (l == 0) scales[b] = s;
   }
 }
 

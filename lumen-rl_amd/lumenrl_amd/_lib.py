@@ -51,8 +51,9 @@ SIGNATURES = {
     "lrq_mxfp4_quant": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _VP]),
     "lrq_act_qdq": (_CI, [_VP, _CI, _I64, _I64, _I64, _I64, _CU, _VP, _VP]),
     "lrq_fp8_linear": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _CI, _VP, _VP]),
-    "lrq_fp8_matmul": (_CI, [_VP, _VP, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _CI, _VP, _CI, _VP]),
-    "lrq_fp8_block_linear_workspace": (_I64, [_I64, _I64]),
+    "lrq_fp8_matmul": (_CI, [_VP, _VP, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _CI, _VP, _CI, _VP, _I64, _VP]),
+    "lrq_fp8_matmul_workspace": (_I64, [_I64, _I64, _I64]),
+    "lrq_fp8_block_linear_workspace": (_I64, [_I64, _I64, _I64]),
     "lrq_fp8_block_linear": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _CI, _VP, _VP, _I64, _VP]),
     "lrq_route": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _CI, _CI, _CI, _CI, _CI, _CI, ctypes.c_float, _VP, _VP, _VP]),
     "lrq_route_grad": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _CI, _CI, _CI, ctypes.c_float, _VP, _VP]),

@@ -83,9 +83,13 @@ def fp8_matmul(x_codes: Tensor, x_scales: Tensor, codes: Tensor, scales: Tensor,
     if not x_scales.is_contiguous():
         x_scales = x_scales.contiguous()
     out = _dense((m, n), out_dtype, dev)
+    L = _lib.lib()
+    need = L.lrq_fp8_matmul_workspace(m, k, n)
+    work = _dense((need,), torch.uint8, dev) if need else None
     with _on(dev):
-        rc = _lib.lib().lrq_fp8_matmul(x_codes.data_ptr(), x_scales.data_ptr(), m, k, ld, codes.data_ptr(), scales.data_ptr(),
-                                       n, bias_ptr, bias_dtype, out.data_ptr(), _IN_DTYPES[out_dtype], _stream(dev))
+        rc = L.lrq_fp8_matmul(x_codes.data_ptr(), x_scales.data_ptr(), m, k, ld, codes.data_ptr(), scales.data_ptr(), n,
+                              bias_ptr, bias_dtype, out.data_ptr(), _IN_DTYPES[out_dtype],
+                              work.data_ptr() if need else None, need, _stream(dev))
     if rc:
         _lib.check(rc, "lrq_fp8_matmul")
     return out
@@ -96,7 +100,7 @@ def fp8_block_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Te
     (as ``fp8_block_quant(x, (1, 128))``) and multiplied with ``codes`` [N, K]
     and float32 ``scales`` [ceil(N/128), ceil(K/128)] -> [..., N] in x's dtype.
 
-    Up to 16 tokens take one launch, more take two.
+    Up to four tokens take one launch, more take two or three.
     """
     _check_input(x, "fp8_block_linear")
     dev = x.device
@@ -118,7 +122,7 @@ def fp8_block_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Te
             x, ld = x.contiguous(), k
     out = _dense((*lead, n), x.dtype, dev)
     L = _lib.lib()
-    need = L.lrq_fp8_block_linear_workspace(rows, k)
+    need = L.lrq_fp8_block_linear_workspace(rows, k, n)
     work = _dense((need,), torch.uint8, dev) if need else None
     with _on(dev):
         rc = L.lrq_fp8_block_linear(x.data_ptr(), _IN_DTYPES[x.dtype], rows, k, ld, codes.data_ptr(), scales.data_ptr(), n,
