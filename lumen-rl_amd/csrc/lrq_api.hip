@@ -829,11 +829,6 @@ lrq::ExpertArgs expert_sizes(int64_t hidden, int64_t inter, int64_t experts, int
   a.kb = (int)(hidden + 127) / 128, a.ib = (int)(inter + 127) / 128, a.gb = (int)(2 * inter + 127) / 128;
   return a;
 }
-hipError_t quantize_tokens(const lrq::ExpertArgs& a, int dtype, hipStream_t stream) {
-  return lrq_fp8_block_quant(a.x, dtype, 1, a.tokens, a.hidden, a.ldx, a.tokens * a.ldx, 1, 128, a.xq, a.xs, 0, stream)
-             ? hipErrorInvalidValue
-             : hipSuccess;
-}
 }  // namespace
 
 int64_t lrq_fp8_experts_workspace(int64_t tokens, int64_t hidden, int64_t inter, int64_t experts, int64_t top_k) {
@@ -862,7 +857,7 @@ int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, 
   if (!aligned(workspace, 256)) return fail(LRQ_ERR_ALIGN, "fp8_experts: workspace must be 256-byte aligned");
   a.x = x, a.ldx = ld, a.ids = ids, a.weights = weights, a.gu = gate_up, a.gus = gate_up_scales, a.dn = down, a.dns = down_scales;
   a.out = out;
-  return check_hip(lrq::launch_experts(a, x_dtype, tokens, workspace, quantize_tokens, (hipStream_t)stream), "kernel launch");
+  return check_hip(lrq::launch_experts(a, x_dtype, tokens, workspace, (hipStream_t)stream), "kernel launch");
 }
 
 int lrq_cast_e4m3(const void* in, int in_dtype, int64_t n, uint8_t* out, lrq_stream_t stream) {

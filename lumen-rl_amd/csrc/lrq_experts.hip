@@ -18,44 +18,76 @@ namespace lrq {
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
 // ---------------------------------------------------------------------------
-// Pairs sorted by expert
+// Tokens quantized, pairs sorted by expert
 // ---------------------------------------------------------------------------
-// One work-group: counts, the experts' runs and their tiles of `bm` rows, then each
-// pair's place.  Pairs of an expert come in any order, which no result depends on.
-// Ids outside 0 .. experts - 1 have no place.
-constexpr int kSortThreads = 1024;
-__global__ __launch_bounds__(kSortThreads) void k_ex_sort(const int32_t* ids, int pairs, int experts, int bm, ExpertTile* tiles,
-                                                          int32_t* total, int32_t* order) {
-  __shared__ int32_t count[kExpertsMax], start[kExpertsMax + 1], part[2][kSortThreads];
+// The first work-group sorts: counts (which give each pair its rank), the experts'
+// runs and their tiles of `bm` rows, then each pair's place.  Pairs of an expert
+// come in any order, which no result depends on.  Ids outside 0 .. experts - 1 have
+// no place.  The others meanwhile quantize x, 64 blocks each.
+constexpr int kSortThreads = 1024, kSortAhead = 8;
+template <int DT>
+__global__ __launch_bounds__(kSortThreads) void k_ex_prepare(ExpertArgs a, int bm) {
+  __shared__ int32_t count[kExpertsMax], start[kExpertsMax], part[2][kSortThreads];
   const int tid = threadIdx.x;
-  for (int e = tid; e < experts; e += kSortThreads) count[e] = 0;
+  if (blockIdx.x > 0) {
+    const int64_t b = (int64_t)(blockIdx.x - 1) * (kSortThreads / 16) + (tid >> 4);
+    const int64_t t = b / a.kb;
+    if (t >= a.tokens) return;  // 16 lanes at once
+    const int kb = (int)(b - t * a.kb), at = kb * kBlk + 8 * (tid & 15);
+    float v[8], s;
+    load_acts<DT>(static_cast<const uint8_t*>(a.x) + t * a.ldx * 2, at, a.hidden, v);
+    const v2u q = quant8(v, s);
+    if (at < a.hidden) *(LRQ_GLOBAL v2u_out*)(a.xq + t * a.hidden + at) = q;
+    if ((tid & 15) == 0) gst<float>(a.xs + b, s);
+    return;
+  }
+  const int pairs = (int)(a.tokens * a.top_k);
+  const uint32_t none = (uint32_t)a.experts;
+  for (int e = tid; e < a.experts; e += kSortThreads) count[e] = 0;
   __syncthreads();
-  for (int p = tid; p < pairs; p += kSortThreads) {
-    const uint32_t e = (uint32_t)gld<int32_t>(ids + p);
-    if (e < (uint32_t)experts) atomicAdd(&count[e], 1);
+  for (int p0 = tid; p0 < pairs; p0 += kSortThreads * kSortAhead) {
+    uint32_t e[kSortAhead];
+    int rank[kSortAhead];
+#pragma unroll
+    for (int i = 0; i < kSortAhead; ++i)
+      e[i] = p0 + kSortThreads * i < pairs ? (uint32_t)gld<int32_t>(a.ids + p0 + kSortThreads * i) : none;
+#pragma unroll
+    for (int i = 0; i < kSortAhead; ++i) rank[i] = e[i] < none ? atomicAdd(&count[e[i]], 1) : 0;
+#pragma unroll
+    for (int i = 0; i < kSortAhead; ++i)
+      if (e[i] < none) gst<int32_t>(a.rank + p0 + kSortThreads * i, rank[i]);
   }
   __syncthreads();
   // one expert a thread: sums of rows and of tiles before it
-  const int mine = tid < experts ? count[tid] : 0, my_tiles = (mine + bm - 1) / bm;
+  const int mine = tid < a.experts ? count[tid] : 0, my_tiles = (mine + bm - 1) / bm;
   part[0][tid] = mine, part[1][tid] = my_tiles;
   __syncthreads();
   for (int off = 1; off < kSortThreads; off *= 2) {
-    const int a = tid >= off ? part[0][tid - off] : 0, b = tid >= off ? part[1][tid - off] : 0;
+    const int m = tid >= off ? part[0][tid - off] : 0, n = tid >= off ? part[1][tid - off] : 0;
     __syncthreads();
-    part[0][tid] += a, part[1][tid] += b;
+    part[0][tid] += m, part[1][tid] += n;
     __syncthreads();
   }
   const int first = part[0][tid] - mine, tile = part[1][tid] - my_tiles;
-  if (tid < experts) start[tid] = first;
-  if (tid == kSortThreads - 1) gst<int32_t>(total, part[1][tid]);
+  if (tid < a.experts) start[tid] = first;
+  if (tid == kSortThreads - 1) gst<int32_t>(a.total, part[1][tid]);
   for (int i = 0; i < my_tiles; ++i) {
     const int rows = mine - i * bm < bm ? mine - i * bm : bm;
-    tiles[tile + i] = ExpertTile{tid, first + i * bm, rows, 0};
+    a.tiles[tile + i] = ExpertTile{tid, first + i * bm, rows, 0};
   }
   __syncthreads();
-  for (int p = tid; p < pairs; p += kSortThreads) {
-    const uint32_t e = (uint32_t)gld<int32_t>(ids + p);
-    if (e < (uint32_t)experts) gst<int32_t>(order + atomicAdd(&start[e], 1), p);
+  for (int p0 = tid; p0 < pairs; p0 += kSortThreads * kSortAhead) {
+    uint32_t e[kSortAhead];
+    int rank[kSortAhead];
+#pragma unroll
+    for (int i = 0; i < kSortAhead; ++i) {
+      const int p = p0 + kSortThreads * i < pairs ? p0 + kSortThreads * i : tid;
+      e[i] = (uint32_t)gld<int32_t>(a.ids + p), rank[i] = gld<int32_t>(a.rank + p);  // this thread's own writes
+      if (p0 + kSortThreads * i >= pairs) e[i] = none;
+    }
+#pragma unroll
+    for (int i = 0; i < kSortAhead; ++i)
+      if (e[i] < none) gst<int32_t>(a.order + start[e[i]] + rank[i], p0 + kSortThreads * i);
   }
 }
 
@@ -332,8 +364,13 @@ __global__ __launch_bounds__(512) void k_ex_down_few(ExpertArgs a) {
   };
 #pragma unroll
   for (int d = 0; d < D; ++d) load(st[d], d);
-  for (int j = 0; j < a.top_k; ++j)
-    quant_row<kF32, 512>(a.y + (first + j) * a.inter, a.inter, a.ib, lds + j * pitch, scales + j * a.ib);
+  for (int b = threadIdx.x >> 4; b < a.top_k * a.ib; b += 32) {
+    const int j = b / a.ib, at = (b - j * a.ib) * kBlk + 8 * (threadIdx.x & 15);
+    float v[8], q;
+    load_acts<kF32>(a.y + (first + j) * a.inter, at, a.inter, v);
+    *reinterpret_cast<v2u*>(lds + j * pitch + at) = quant8(v, q);
+    if ((threadIdx.x & 15) == 0) scales[b] = q;
+  }
   lds_barrier8();
   float acc = 0.0f;
   for (int i0 = 0; i0 < chunks; i0 += D) {
@@ -383,6 +420,7 @@ static int64_t expert_layout(int64_t tokens, int bm, ExpertArgs& a, uint8_t* bas
   a.xq = take(tokens * a.hidden);
   a.xs = reinterpret_cast<float*>(take(4 * tokens * a.kb));
   a.order = reinterpret_cast<int32_t*>(take(4 * pairs));
+  a.rank = reinterpret_cast<int32_t*>(take(4 * pairs));
   a.total = reinterpret_cast<int32_t*>(take(4));
   a.tiles = reinterpret_cast<ExpertTile*>(take((int64_t)sizeof(ExpertTile) * tile_bound(pairs, bm, a.experts)));
   a.hq = take(pairs * a.inter);
@@ -421,7 +459,7 @@ static void down(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
                      dim3(64 * WN * WM), 0, stream, a);
 }
 
-hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspace, ExpertQuant quant, hipStream_t stream) {
+hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspace, hipStream_t stream) {
   const int64_t pass = expert_pass(tokens, a);
   const uint8_t* const x = static_cast<const uint8_t*>(a.x);
   const int32_t* const ids = a.ids;
@@ -437,17 +475,18 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
       continue;
     }
     const int64_t pairs = a.tokens * a.top_k, tiles = tile_bound(pairs, bm, a.experts);
-    if (hipError_t e = quant(a, dtype, stream)) return e;
-    hipLaunchKernelGGL(k_ex_sort, dim3(1), dim3(kSortThreads), 0, stream, a.ids, (int)pairs, a.experts, bm, a.tiles, a.total, a.order);
+    const dim3 prepare((unsigned)(1 + (a.tokens * a.kb + kSortThreads / 16 - 1) / (kSortThreads / 16)));
+    if (dtype == kBF16) hipLaunchKernelGGL((k_ex_prepare<kBF16>), prepare, dim3(kSortThreads), 0, stream, a, bm);
+    else hipLaunchKernelGGL((k_ex_prepare<kF16>), prepare, dim3(kSortThreads), 0, stream, a, bm);
     if (bm == 16) {
       up<2, 1, 8, 1, 2, true>(a, tiles, stream);
-      down<1, 1, 8, 1, 3, true>(a, tiles, stream);
+      down<1, 1, 8, 1, 2, true>(a, tiles, stream);
     } else if (bm == 32) {
       up<2, 2, 8, 1, 2, true>(a, tiles, stream);
-      down<1, 2, 8, 1, 3, true>(a, tiles, stream);
+      down<1, 2, 8, 1, 2, true>(a, tiles, stream);
     } else {
       up<4, 4, 4, 2, 3, false>(a, tiles, stream);
-      down<4, 4, 2, 2, 4, false>(a, tiles, stream);
+      down<4, 4, 2, 2, 2, false>(a, tiles, stream);
     }
     const dim3 sum((unsigned)((a.tokens * a.hidden / 8 + 255) / 256));
     if (dtype == kBF16) hipLaunchKernelGGL((k_ex_sum<kBF16>), sum, dim3(256), 0, stream, a);

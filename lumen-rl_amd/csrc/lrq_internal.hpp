@@ -324,12 +324,11 @@ struct ExpertArgs {
   // workspace: x and h in codes, the pairs' order, tiles of it and their number, and the pairs' results
   uint8_t *xq, *hq;
   float *xs, *hs, *y;
-  int32_t *order, *total;
+  int32_t *order, *rank, *total;
   ExpertTile* tiles;
 };
-typedef hipError_t (*ExpertQuant)(const ExpertArgs& a, int dtype, hipStream_t stream);  // x -> xq, xs
 int64_t experts_workspace(int64_t tokens, ExpertArgs a);
-hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspace, ExpertQuant quant, hipStream_t stream);
+hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspace, hipStream_t stream);
 
 // Diagnostics: element encoders applied to raw inputs.
 hipError_t launch_diag_e4m3_bits(uint32_t start, int64_t n, uint8_t* out, hipStream_t stream);

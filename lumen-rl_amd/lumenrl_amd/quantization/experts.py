@@ -33,46 +33,53 @@ def _rows(x: Tensor) -> tuple[Tensor, int, int]:
     return x, rows, ld
 
 
-def _route(logits: Tensor, bias: Optional[Tensor], cfg: tuple) -> tuple[Tensor, Tensor]:
+def _route(logits: Tensor, ids: Tensor, bias: Optional[Tensor], cfg: tuple) -> Tensor:
     top_k, score, groups, top_groups, group_top, renormalize, scale = cfg
     dev = logits.device
-    shape = (*logits.shape[:-1], top_k)
-    e = logits.shape[-1]
     x, rows, ld = _rows(logits)
-    weights, ids = _dense(shape, torch.float32, dev), _dense(shape, torch.int32, dev)
+    weights = _dense(ids.shape, torch.float32, dev)
     with _on(dev):
-        rc = _lib.lib().lrq_route(x.data_ptr(), _IN_DTYPES[x.dtype], rows, e, ld, bias.data_ptr() if bias is not None else None,
-                                  top_k, score, groups, top_groups, group_top, renormalize, scale, weights.data_ptr(),
-                                  ids.data_ptr(), _stream(dev))
+        rc = _lib.lib().lrq_route(x.data_ptr(), _IN_DTYPES[x.dtype], rows, logits.shape[-1], ld,
+                                  bias.data_ptr() if bias is not None else None, top_k, score, groups, top_groups, group_top,
+                                  renormalize, scale, weights.data_ptr(), ids.data_ptr(), _stream(dev))
     if rc:
         _lib.check(rc, "lrq_route")
-    return weights, ids
+    return weights
+
+
+def _route_grad(ctx, grad: Tensor, *_):
+    logits, ids = ctx.saved_tensors
+    top_k, score, _, _, _, renormalize, scale = ctx.cfg
+    dev = logits.device
+    grad = grad.contiguous()
+    x, rows, ld = _rows(logits)
+    out = _dense(logits.shape, logits.dtype, dev)
+    with _on(dev):
+        rc = _lib.lib().lrq_route_grad(x.data_ptr(), _IN_DTYPES[x.dtype], rows, logits.shape[-1], ld, ids.data_ptr(),
+                                       grad.data_ptr(), top_k, score, renormalize, scale, out.data_ptr(), _stream(dev))
+    if rc:
+        _lib.check(rc, "lrq_route_grad")
+    return out, None, None, None
 
 
 class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, bias, cfg):
-        weights, ids = _route(logits, bias, cfg)
-        ctx.save_for_backward(logits, ids)
-        ctx.cfg = cfg
-        ctx.mark_non_differentiable(ids)
-        return weights, ids
+    """Weights of ``logits``; ``ids`` is filled on the way (as an input it costs autograd nothing)."""
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad, _):
-        logits, ids = ctx.saved_tensors
-        top_k, score, _groups, _top_groups, _group_top, renormalize, scale = ctx.cfg
-        dev = logits.device
-        grad = grad.contiguous()
-        x, rows, ld = _rows(logits)
-        out = _dense(tuple(logits.shape), logits.dtype, dev)
-        with _on(dev):
-            rc = _lib.lib().lrq_route_grad(x.data_ptr(), _IN_DTYPES[x.dtype], rows, logits.shape[-1], ld, ids.data_ptr(),
-                                           grad.data_ptr(), top_k, score, renormalize, scale, out.data_ptr(), _stream(dev))
-        if rc:
-            _lib.check(rc, "lrq_route_grad")
-        return out, None, None
+    def forward(ctx, logits, ids, bias, cfg):
+        ctx.save_for_backward(logits, ids)
+        ctx.cfg = cfg
+        return _route(logits, ids, bias, cfg)
+
+    # the wrapper refuses a second derivative, also that by way of the logits; only for
+    # backward passes that record one
+    _recorded = staticmethod(torch.autograd.function.once_differentiable(_route_grad))
+
+    @staticmethod
+    def backward(ctx, grad):
+        if torch.is_grad_enabled():
+            return _Route._recorded(ctx, grad, ctx.saved_tensors[0])
+        return _route_grad(ctx, grad)
 
 
 def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Optional[Tensor] = None, groups: int = 1,
@@ -110,9 +117,10 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: O
     if group_top not in (1, 2):
         raise ValueError(f"route_experts: group_top must be 1 or 2, got {group_top}")
     cfg = (top_k, _SCORES[score], groups, top_groups, group_top, int(renormalize), scale)
+    ids = _dense((*logits.shape[:-1], top_k), torch.int32, logits.device)
     if logits.requires_grad and torch.is_grad_enabled():
-        return _Route.apply(logits, bias, cfg)
-    return _route(logits, bias, cfg)
+        return _Route.apply(logits, ids, bias, cfg), ids
+    return _route(logits, ids, bias, cfg), ids
 
 
 def fp8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_up_scales: Tensor, down: Tensor,

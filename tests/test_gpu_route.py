@@ -266,6 +266,11 @@ def test_the_choice_takes_no_gradient_and_no_graph_without_one():
         assert not route_experts(x, 3)[0].requires_grad
     y = x * 1.0
     w, _ = route_experts(y, 3)
+    (g,) = torch.autograd.grad(w[:, 0].sum(), x, create_graph=True)
+    assert g.requires_grad
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    w, _ = route_experts(y, 3)
     y.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         w.sum().backward()
