@@ -20,17 +20,67 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f +
 // ---------------------------------------------------------------------------
 // Tokens quantized, pairs sorted by expert
 // ---------------------------------------------------------------------------
-// The first work-group sorts: counts (which give each pair its rank), the experts'
-// runs and their tiles of `bm` rows, then each pair's place.  Pairs of an expert
-// come in any order, which no result depends on.  Ids outside 0 .. experts - 1 have
-// no place.  The others meanwhile quantize x, 64 blocks each.
-constexpr int kSortThreads = 1024, kSortAhead = 8;
-template <int DT>
-__global__ __launch_bounds__(kSortThreads) void k_ex_prepare(ExpertArgs a, int bm) {
-  __shared__ int32_t count[kExpertsMax], start[kExpertsMax], part[2][kSortThreads];
+// The first work-groups sort, kSortPairs pairs each (or a kSortMost-th of them): they
+// count their pairs of each expert, which gives each pair its rank.  The experts'
+// runs, the tiles of `bm` rows and each pair's place follow at once if there is one
+// such work-group, in a launch of their own if there are more: atomics on a few
+// words are slow, 32768 pairs take 42 us in one work-group, 14 in four.  Pairs of an
+// expert come in any order, which no result depends on.  Ids outside 0 .. experts -
+// 1 have no place.  The other work-groups meanwhile quantize x, 64 blocks each.
+constexpr int kSortThreads = 1024, kSortAhead = 8, kSortPairs = 8192, kSortMost = 64;
+
+__device__ __forceinline__ void place_pairs(const ExpertArgs& a, int bm, int p0, int p1, int group, int groups, int32_t* start,
+                                            int32_t (*part)[kSortThreads]) {
   const int tid = threadIdx.x;
-  if (blockIdx.x > 0) {
-    const int64_t b = (int64_t)(blockIdx.x - 1) * (kSortThreads / 16) + (tid >> 4);
+  const uint32_t none = (uint32_t)a.experts;
+  // one expert a thread: sums of rows and of tiles before it
+  int mine = 0, before = 0;
+  if (tid < a.experts)
+    for (int g = 0; g < groups; ++g) {
+      const int n = gld<int32_t>(a.counts + g * a.experts + tid);
+      mine += n, before += g < group ? n : 0;
+    }
+  const int my_tiles = (mine + bm - 1) / bm;
+  part[0][tid] = mine, part[1][tid] = my_tiles;
+  __syncthreads();
+  for (int off = 1; off < kSortThreads; off *= 2) {
+    const int m = tid >= off ? part[0][tid - off] : 0, n = tid >= off ? part[1][tid - off] : 0;
+    __syncthreads();
+    part[0][tid] += m, part[1][tid] += n;
+    __syncthreads();
+  }
+  const int first = part[0][tid] - mine, tile = part[1][tid] - my_tiles;
+  if (tid < a.experts) start[tid] = first + before;
+  if (group == 0) {
+    if (tid == kSortThreads - 1) gst<int32_t>(a.total, part[1][tid]);
+    for (int i = 0; i < my_tiles; ++i) {
+      const int rows = mine - i * bm < bm ? mine - i * bm : bm;
+      a.tiles[tile + i] = ExpertTile{tid, first + i * bm, rows, 0};
+    }
+  }
+  __syncthreads();
+  for (int p = p0 + tid; p < p1; p += kSortThreads * kSortAhead) {
+    uint32_t e[kSortAhead];
+    int rank[kSortAhead];
+#pragma unroll
+    for (int i = 0; i < kSortAhead; ++i) {
+      const bool has = p + kSortThreads * i < p1;
+      const int q = has ? p + kSortThreads * i : p;
+      e[i] = (uint32_t)gld<int32_t>(a.ids + q), rank[i] = gld<int32_t>(a.rank + q);
+      if (!has) e[i] = none;
+    }
+#pragma unroll
+    for (int i = 0; i < kSortAhead; ++i)
+      if (e[i] < none) gst<int32_t>(a.order + start[e[i]] + rank[i], p + kSortThreads * i);
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kSortThreads) void k_ex_prepare(ExpertArgs a, int bm, int groups, int each) {
+  __shared__ int32_t count[kExpertsMax], part[2][kSortThreads];
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x >= groups) {
+    const int64_t b = (int64_t)(blockIdx.x - groups) * (kSortThreads / 16) + (tid >> 4);
     const int64_t t = b / a.kb;
     if (t >= a.tokens) return;  // 16 lanes at once
     const int kb = (int)(b - t * a.kb), at = kb * kBlk + 8 * (tid & 15);
@@ -41,54 +91,31 @@ __global__ __launch_bounds__(kSortThreads) void k_ex_prepare(ExpertArgs a, int b
     if ((tid & 15) == 0) gst<float>(a.xs + b, s);
     return;
   }
-  const int pairs = (int)(a.tokens * a.top_k);
+  const int pairs = (int)(a.tokens * a.top_k), group = blockIdx.x;
+  const int p0 = group * each, p1 = p0 + each < pairs ? p0 + each : pairs;
   const uint32_t none = (uint32_t)a.experts;
   for (int e = tid; e < a.experts; e += kSortThreads) count[e] = 0;
   __syncthreads();
-  for (int p0 = tid; p0 < pairs; p0 += kSortThreads * kSortAhead) {
+  for (int p = p0 + tid; p < p1; p += kSortThreads * kSortAhead) {
     uint32_t e[kSortAhead];
     int rank[kSortAhead];
 #pragma unroll
-    for (int i = 0; i < kSortAhead; ++i)
-      e[i] = p0 + kSortThreads * i < pairs ? (uint32_t)gld<int32_t>(a.ids + p0 + kSortThreads * i) : none;
+    for (int i = 0; i < kSortAhead; ++i) e[i] = p + kSortThreads * i < p1 ? (uint32_t)gld<int32_t>(a.ids + p + kSortThreads * i) : none;
 #pragma unroll
     for (int i = 0; i < kSortAhead; ++i) rank[i] = e[i] < none ? atomicAdd(&count[e[i]], 1) : 0;
 #pragma unroll
     for (int i = 0; i < kSortAhead; ++i)
-      if (e[i] < none) gst<int32_t>(a.rank + p0 + kSortThreads * i, rank[i]);
+      if (e[i] < none) gst<int32_t>(a.rank + p + kSortThreads * i, rank[i]);
   }
   __syncthreads();
-  // one expert a thread: sums of rows and of tiles before it
-  const int mine = tid < a.experts ? count[tid] : 0, my_tiles = (mine + bm - 1) / bm;
-  part[0][tid] = mine, part[1][tid] = my_tiles;
-  __syncthreads();
-  for (int off = 1; off < kSortThreads; off *= 2) {
-    const int m = tid >= off ? part[0][tid - off] : 0, n = tid >= off ? part[1][tid - off] : 0;
-    __syncthreads();
-    part[0][tid] += m, part[1][tid] += n;
-    __syncthreads();
-  }
-  const int first = part[0][tid] - mine, tile = part[1][tid] - my_tiles;
-  if (tid < a.experts) start[tid] = first;
-  if (tid == kSortThreads - 1) gst<int32_t>(a.total, part[1][tid]);
-  for (int i = 0; i < my_tiles; ++i) {
-    const int rows = mine - i * bm < bm ? mine - i * bm : bm;
-    a.tiles[tile + i] = ExpertTile{tid, first + i * bm, rows, 0};
-  }
-  __syncthreads();
-  for (int p0 = tid; p0 < pairs; p0 += kSortThreads * kSortAhead) {
-    uint32_t e[kSortAhead];
-    int rank[kSortAhead];
-#pragma unroll
-    for (int i = 0; i < kSortAhead; ++i) {
-      const int p = p0 + kSortThreads * i < pairs ? p0 + kSortThreads * i : tid;
-      e[i] = (uint32_t)gld<int32_t>(a.ids + p), rank[i] = gld<int32_t>(a.rank + p);  // this thread's own writes
-      if (p0 + kSortThreads * i >= pairs) e[i] = none;
-    }
-#pragma unroll
-    for (int i = 0; i < kSortAhead; ++i)
-      if (e[i] < none) gst<int32_t>(a.order + start[e[i]] + rank[i], p0 + kSortThreads * i);
-  }
+  if (tid < a.experts) gst<int32_t>(a.counts + group * a.experts + tid, count[tid]);  // read by this thread, or the next launch
+  if (groups == 1) place_pairs(a, bm, p0, p1, 0, 1, count, part);
+}
+
+__global__ __launch_bounds__(kSortThreads) void k_ex_place(ExpertArgs a, int bm, int groups, int each) {
+  __shared__ int32_t start[kExpertsMax], part[2][kSortThreads];
+  const int pairs = (int)(a.tokens * a.top_k), p0 = (int)blockIdx.x * each;
+  place_pairs(a, bm, p0, p0 + each < pairs ? p0 + each : pairs, (int)blockIdx.x, groups, start, part);
 }
 
 // Work-group wg of a grid for `total` tiles by nb: each XCD (wg % 8) takes one run,
@@ -160,7 +187,7 @@ __device__ __forceinline__ void store_hidden(const ExpertArgs& a, f32x4 (&h)[NS]
 // ---------------------------------------------------------------------------
 // Weight rows of a tile: 16 of gate, the same 16 of up, and so on.
 struct UpTile {
-  static constexpr bool kCut = false;
+  static constexpr bool kCut = false, kSkip = true;
   const ExpertArgs& a;
   const ExpertTile& t;
   int block;
@@ -175,6 +202,7 @@ struct UpTile {
   }
   __device__ int token(int r) const { return gld<int32_t>(a.order + t.first + (r < t.rows ? r : t.rows - 1)) / a.top_k; }
   __device__ uint32_t x_off(int r) const { return r < t.rows ? (uint32_t)token(r) * (uint32_t)a.hidden : kNoRow; }
+  __device__ int tokens() const { return t.rows; }
   __device__ const float* sx() const { return a.xs; }
   __device__ const float* sw() const { return a.gus + (int64_t)t.expert * a.gb * a.kb; }
   __device__ uint32_t sx_bytes() const { return (uint32_t)(4 * a.tokens * a.kb); }
@@ -208,7 +236,7 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
 }
 
 struct DownTile {
-  static constexpr bool kCut = false;
+  static constexpr bool kCut = false, kSkip = true;
   const ExpertArgs& a;
   const ExpertTile& t;
   int n0;
@@ -218,6 +246,7 @@ struct DownTile {
   __device__ uint32_t x_bytes() const { return (uint32_t)(t.rows * a.inter); }
   __device__ uint32_t w_off(int r) const { return n0 + r < a.hidden ? (uint32_t)(n0 + r) * (uint32_t)a.inter : kNoRow; }
   __device__ uint32_t x_off(int r) const { return r < t.rows ? (uint32_t)r * (uint32_t)a.inter : kNoRow; }
+  __device__ int tokens() const { return t.rows; }
   __device__ const float* sx() const { return a.hs + (int64_t)t.first * a.ib; }
   __device__ const float* sw() const { return a.dns + (int64_t)t.expert * a.kb * a.ib; }
   __device__ uint32_t sx_bytes() const { return (uint32_t)(4 * t.rows * a.ib); }
@@ -421,6 +450,7 @@ static int64_t expert_layout(int64_t tokens, int bm, ExpertArgs& a, uint8_t* bas
   a.xs = reinterpret_cast<float*>(take(4 * tokens * a.kb));
   a.order = reinterpret_cast<int32_t*>(take(4 * pairs));
   a.rank = reinterpret_cast<int32_t*>(take(4 * pairs));
+  a.counts = reinterpret_cast<int32_t*>(take(4 * kSortMost * (int64_t)a.experts));
   a.total = reinterpret_cast<int32_t*>(take(4));
   a.tiles = reinterpret_cast<ExpertTile*>(take((int64_t)sizeof(ExpertTile) * tile_bound(pairs, bm, a.experts)));
   a.hq = take(pairs * a.inter);
@@ -475,9 +505,13 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
       continue;
     }
     const int64_t pairs = a.tokens * a.top_k, tiles = tile_bound(pairs, bm, a.experts);
-    const dim3 prepare((unsigned)(1 + (a.tokens * a.kb + kSortThreads / 16 - 1) / (kSortThreads / 16)));
-    if (dtype == kBF16) hipLaunchKernelGGL((k_ex_prepare<kBF16>), prepare, dim3(kSortThreads), 0, stream, a, bm);
-    else hipLaunchKernelGGL((k_ex_prepare<kF16>), prepare, dim3(kSortThreads), 0, stream, a, bm);
+    int64_t each = (pairs + kSortMost - 1) / kSortMost;
+    each = each < kSortPairs ? kSortPairs : each;
+    const int groups = (int)((pairs + each - 1) / each);
+    const dim3 prepare((unsigned)(groups + (a.tokens * a.kb + kSortThreads / 16 - 1) / (kSortThreads / 16)));
+    if (dtype == kBF16) hipLaunchKernelGGL((k_ex_prepare<kBF16>), prepare, dim3(kSortThreads), 0, stream, a, bm, groups, (int)each);
+    else hipLaunchKernelGGL((k_ex_prepare<kF16>), prepare, dim3(kSortThreads), 0, stream, a, bm, groups, (int)each);
+    if (groups > 1) hipLaunchKernelGGL(k_ex_place, dim3((unsigned)groups), dim3(kSortThreads), 0, stream, a, bm, groups, (int)each);
     if (bm == 16) {
       up<2, 1, 8, 1, 2, true>(a, tiles, stream);
       down<1, 1, 8, 1, 2, true>(a, tiles, stream);
@@ -486,7 +520,7 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
       down<1, 2, 8, 1, 2, true>(a, tiles, stream);
     } else {
       up<4, 4, 4, 2, 3, false>(a, tiles, stream);
-      down<4, 4, 2, 2, 2, false>(a, tiles, stream);
+      down<4, 4, 4, 2, 3, false>(a, tiles, stream);
     }
     const dim3 sum((unsigned)((a.tokens * a.hidden / 8 + 255) / 256));
     if (dtype == kBF16) hipLaunchKernelGGL((k_ex_sum<kBF16>), sum, dim3(256), 0, stream, a);

@@ -324,7 +324,7 @@ struct ExpertArgs {
   // workspace: x and h in codes, the pairs' order, tiles of it and their number, and the pairs' results
   uint8_t *xq, *hq;
   float *xs, *hs, *y;
-  int32_t *order, *rank, *total;
+  int32_t *order, *rank, *counts, *total;
   ExpertTile* tiles;
 };
 int64_t experts_workspace(int64_t tokens, ExpertArgs a);

@@ -107,7 +107,7 @@ __global__ __launch_bounds__(512) void k_mm8_dot(MatmulArgs a) {
 // More: tiles
 // ---------------------------------------------------------------------------
 struct DenseTile {
-  static constexpr bool kCut = true;
+  static constexpr bool kCut = true, kSkip = false;  // (the branch costs 256 x 256 tiles their registers)
   const MatmulArgs& a;
   int n0, m0, n_last, m_last;  // n_last, m_last: within the tile
   bool dma;
@@ -117,6 +117,7 @@ struct DenseTile {
   __device__ uint32_t x_bytes() const { return (uint32_t)((m_last < 255 ? m_last : 255) * a.ldx + a.k); }
   __device__ uint32_t w_off(int r) const { return r <= n_last ? (uint32_t)(r * a.k) : dma ? kNoRow : (uint32_t)(n_last * a.k); }
   __device__ uint32_t x_off(int r) const { return r <= m_last ? (uint32_t)(r * a.ldx) : dma ? kNoRow : (uint32_t)(m_last * a.ldx); }
+  __device__ int tokens() const { return m_last + 1; }
   __device__ const float* sx() const { return a.sx + (int64_t)m0 * a.kb; }
   __device__ const float* sw() const { return a.sw + (int64_t)(n0 / kBlk) * a.kb; }
   __device__ uint32_t sx_bytes() const { return (uint32_t)(4 * ((m_last < 255 ? m_last : 255) + 1) * a.kb); }
@@ -238,14 +239,32 @@ static void launch_dots(const MatmulArgs& a, hipStream_t stream) {
   else a.n >= 4096 ? launch_dot<XDT, 4, 2>(a, stream) : launch_dot<XDT, 4, 1>(a, stream);
 }
 
+// Tiles, by what a round of them over the chip takes (us for K = 4096, measured one
+// shape at a time): `one` with at most a work-group on each CU, `full` with as many
+// as LDS allows (one of 256 x 256 and of 128 tokens x 256, two of the others).
+// bf16: 1024 tokens x [12288, 4096] 56 us in 256 x 256, 64 in 128 x 256, 92 in 64 x
+// 64; 1536 x [4096, 4096] 51, 34 and 46; 256 x [12288, 4096] 49, 32, 23 in 64 x 128,
+// 29.  128 x 128 wins nowhere (1024 x [4096, 4096] 25, as 64 x 128), but for float32
+// results, whose conversions take the registers of the larger ones: 3000 x [4096,
+// 4096] 91 us, 105 in 64 x 128, 110 in 128 x 256.  So do loads by way of registers.
 template <bool DMA, bool EXACT>
 static void launch_tiles_of(const MatmulArgs& a, hipStream_t stream) {
-  if constexpr (DMA && !EXACT) {
-    if (ceil_div(a.m, 256) * ceil_div(a.n, 256) >= 200) return launch_tiles<8, 4, 2, 4, 2, DMA, EXACT>(a, stream);
-    if (ceil_div(a.m, 128) * ceil_div(a.n, 256) >= 200) return launch_tiles<4, 4, 4, 2, 3, DMA, EXACT>(a, stream);
+  auto whole = [&](int64_t bm, int64_t bn, double full) { return (double)ceil_div(ceil_div(a.m, bm) * ceil_div(a.n, bn), 256) * full; };
+  auto pairs = [&](int64_t bm, int64_t bn, double one, double full) {
+    const int64_t tiles = ceil_div(a.m, bm) * ceil_div(a.n, bn);
+    return tiles <= 256 ? one : tiles <= 512 ? one + (full - one) * (double)(tiles - 256) / 256 : full * (double)tiles / 512;
+  };
+  const double s = EXACT ? pairs(64, 64, 18, 26.5) : pairs(64, 64, 14.5, 18);
+  const double u = EXACT ? pairs(64, 128, 26, 40) : pairs(64, 128, 16, 24.5);
+  if constexpr (DMA && EXACT) {
+    if (const double d = pairs(128, 128, 36, 62); d <= s && d <= u) return launch_tiles<4, 4, 2, 2, 2, DMA, EXACT>(a, stream);
+  } else if constexpr (DMA) {
+    const double b = whole(128, 256, 31), l = whole(256, 256, 49);
+    if (l <= s && l <= u && l <= b) return launch_tiles<8, 4, 2, 4, 2, DMA, EXACT>(a, stream);
+    if (b <= s && b <= u) return launch_tiles<4, 4, 4, 2, 3, DMA, EXACT>(a, stream);
   }
-  if (ceil_div(a.m, 128) * ceil_div(a.n, 128) >= 200) return launch_tiles<4, 4, 2, 2, DMA ? 4 : 2, DMA, EXACT>(a, stream);
-  launch_tiles<2, 2, 2, 2, DMA ? 4 : 2, DMA, EXACT>(a, stream);
+  if (u <= s) return launch_tiles<4, 2, 2, 2, DMA ? 3 : 2, DMA, EXACT>(a, stream);
+  launch_tiles<2, 2, 2, 2, DMA && !EXACT ? 4 : 2, DMA, EXACT>(a, stream);
 }
 
 constexpr int64_t kDots = 4, kSplitRows = 64;

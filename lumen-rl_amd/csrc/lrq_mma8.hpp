@@ -207,6 +207,7 @@ __device__ __forceinline__ v2u quant8(const float* v, float& scale) {
 //   are not stored; without DMA some row that is there instead);
 //   sx_off(r): of the scales of tile row r of the tokens, sw_off(s) of those of
 //   weight rows 16 s .. (one scale for 16 rows); of some row that is there, if none.
+//   kSkip: waves without a token, of the tokens() that are there, multiply nothing;
 //   kCut: k may be no multiple of 16.
 // EACH: the scales of a wave's weight rows differ; otherwise the first is for all.
 constexpr int kTileSets = 2;
@@ -235,11 +236,12 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, int kb0, int kb
   const int wn = (wave / WM) * 16 * FN, wm = (wave % WM) * 16 * FM;
   const int kb_n = kb1 - kb0;
   const int piece = (tid & 7) ^ ((tid >> 4) & 7);  // of tile rows (T / 8) p + tid / 8
+  const bool moves_x = XWAVES == WN * WM || wave < XWAVES, moves_s = SWAVES == WN * WM || wave < SWAVES;
   uint32_t wo[PW], xo[PX];
 #pragma unroll
   for (int p = 0; p < PW; ++p) wo[p] = src.w_off((T / 8) * p + (tid >> 3)) + 16 * piece;
 #pragma unroll
-  for (int p = 0; p < PX; ++p) xo[p] = (wave < XWAVES ? src.x_off((T / 8) * p + (tid >> 3)) : 0) + 16 * piece;
+  for (int p = 0; p < PX; ++p) xo[p] = (moves_x ? src.x_off((T / 8) * p + (tid >> 3)) : 0) + 16 * piece;
   // the thread's scales: of a token, or of 16 weight rows
   const bool tokens = wave < SW / 64;
   const uint32_t so = (tokens ? tid < BM ? src.sx_off(tid) : kNoRow : tid < SW + BN / 16 ? src.sw_off(tid - SW) : kNoRow) + 4 * kb0;
@@ -250,7 +252,8 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, int kb0, int kb
     for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int at0 = 16 * (g ^ (c >> 1)), at1 = 16 * ((g + 4) ^ (c >> 1));
-  auto multiply = [&](const uint8_t* stage, int kb) {
+  // `between(t)` runs after the block's matrix instruction t
+  auto multiply = [&](const uint8_t* stage, int kb, auto between) {
     const uint8_t* const cw = stage + 128 * (wn + c);
     const uint8_t* const cx = stage + 128 * (BN + wm + c);
     const float* const sc = reinterpret_cast<const float*>(scales + (kb >> 2 & 1) * kScales) + (kb & 3);
@@ -287,6 +290,7 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, int kb0, int kb
         const int t = i * FM + j;
         p[t % (LAG + 1)] = mma8(wi, x[j]);
         if (t >= LAG) scale(t - LAG);
+        between(t);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -298,18 +302,20 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, int kb0, int kb
     const Rsrc rw = make_rsrc(src.w(), src.w_bytes()), rx = make_rsrc(src.x(), src.x_bytes());
     const Rsrc rs = tokens ? make_rsrc(src.sx(), src.sx_bytes()) : make_rsrc(src.sw(), src.sw_bytes());
     const uint32_t to = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds) + 1024 * wave;
-    auto fetch = [&](int kb, int stage) {
-      // blocks past the last are asked for, so that every wait counts the same, and read as zeros
+    // pieces [p0, p1) of a block; blocks past the last are asked for too, so that every
+    // wait counts the same, and read as zeros
+    auto fetch = [&](int kb, int stage, int p0, int p1) {
       const uint32_t at = (uint32_t)((kb0 + kb) * kBlk), past = kb < kb_n && (int)at + 16 * piece < k ? 0 : kNoRow;
       const uint32_t here = to + (uint32_t)(stage * kStage);
 #pragma unroll
-      for (int p = 0; p < PW; ++p) dma16(rw, (wo[p] + at) | past, here + 128 * (T / 8) * p);
-      if (wave < XWAVES)
-#pragma unroll
-        for (int p = 0; p < PX; ++p) dma16(rx, (xo[p] + at) | past, here + 128 * (BN + (T / 8) * p));
+      for (int p = 0; p < PW + PX; ++p) {
+        if (p < p0 || p >= p1) continue;
+        if (p < PW) dma16(rw, (wo[p < PW ? p : 0] + at) | past, here + 128 * (T / 8) * p);
+        else if (moves_x) dma16(rx, (xo[p < PW ? 0 : p - PW] + at) | past, here + 128 * (BN + (T / 8) * (p - PW)));
+      }
     };
     auto fetch_scales = [&](int kb) {  // of blocks kb .. kb + 3; those past a row's end are the next row's, and not used
-      if (wave < SWAVES) dma16(rs, (so + 4 * kb) | (kb < kb_n ? 0 : kNoRow), to + (uint32_t)(STAGES * kStage + (kb >> 2 & 1) * kScales));
+      if (moves_s) dma16(rs, (so + 4 * kb) | (kb < kb_n ? 0 : kNoRow), to + (uint32_t)(STAGES * kStage + (kb >> 2 & 1) * kScales));
     };
     // a row's last codes, where 16 bytes would reach past its end: one row a thread
     const bool cut = Src::kCut && k % 16 != 0 && kb1 * kBlk >= k;
@@ -325,7 +331,7 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, int kb0, int kb
     }
     fetch_scales(0);
 #pragma unroll
-    for (int s = 0; s + 1 < STAGES; ++s) fetch(s, s);
+    for (int s = 0; s + 1 < STAGES; ++s) fetch(s, s, 0, PW + PX);
     int stage = 0, free = STAGES - 1;
     for (int kb = 0; kb < kb_n; kb += 4) {
 #pragma unroll
@@ -333,18 +339,28 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, int kb0, int kb
         if (kb + r >= kb_n) break;
         // on their way since this block's codes were asked for: the blocks between, and scales
         constexpr int kPer = STAGES - 2;
-        const bool more = r >= 1 && r <= STAGES - 2 && wave < SWAVES;
-        if (wave < XWAVES) more ? dma_wait<kPer * (PW + PX) + 1>() : dma_wait<kPer * (PW + PX)>();
+        const bool more = r >= 1 && r <= STAGES - 2 && moves_s;
+        if (moves_x) more ? dma_wait<kPer * (PW + PX) + 1>() : dma_wait<kPer * (PW + PX)>();
         else more ? dma_wait<kPer * PW + 1>() : dma_wait<kPer * PW>();
         lds_barrier8();  // every wave's part of this block is there, and every read of the last is done
-        if (r == 0) fetch_scales(kb + 4);
-        fetch(kb + r + STAGES - 1, free);
         if (cut && kb + r == kb_n - 1) {
           static_assert(BN + BM <= T || !Src::kCut, "");
           if (tid < BN + BM) *reinterpret_cast<v4u*>(lds + stage * kStage + 128 * tid + 16 * ((k % kBlk / 16) ^ (tid >> 1 & 7))) = last;
           lds_barrier8();
         }
-        multiply(lds + stage * kStage, kb + r);
+        // the next loads go out among the first half of the matrix instructions: all at
+        // once they would hold up the wave, whose reads of LDS stand behind them
+        constexpr int H = TILES >= 2 ? TILES / 2 : 1, N = PW + PX;
+        auto next = [&](int t) {
+          if (t == 0 && r == 0) fetch_scales(kb + 4);
+          if (t < H) fetch(kb + r + STAGES - 1, free, t * N / H, (t + 1) * N / H);
+        };
+        if (!Src::kSkip || wm < src.tokens()) {
+          multiply(lds + stage * kStage, kb + r, next);
+        } else {
+#pragma unroll
+          for (int t = 0; t < H; ++t) next(t);
+        }
         free = stage;
         stage = stage + 1 < STAGES ? stage + 1 : 0;
       }
@@ -376,7 +392,7 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, int kb0, int kb
       for (int p = 0; p < PW; ++p) *reinterpret_cast<v4u*>(s + 128 * (T / 8) * p) = gw[set][p];
 #pragma unroll
       for (int p = 0; p < PX; ++p) *reinterpret_cast<v4u*>(s + 128 * (BN + (T / 8) * p)) = gx[set][p];
-      if (wave < SWAVES) reinterpret_cast<float*>(scales + (kb >> 2 & 1) * kScales)[4 * tid + (kb & 3)] = gs[set];
+      if (moves_s) reinterpret_cast<float*>(scales + (kb >> 2 & 1) * kScales)[4 * tid + (kb & 3)] = gs[set];
     };
 #pragma unroll
     for (int s = 0; s < kTileSets; ++s) fetch(s, s);
@@ -389,7 +405,7 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, int kb0, int kb
         lds_barrier8();
         put((r + 1) % kTileSets, kb + r + 1);
         fetch(kb + r + 1 + kTileSets, (r + 1) % kTileSets);
-        multiply(lds + (r & 1) * kStage, kb + r);
+        multiply(lds + (r & 1) * kStage, kb + r, [](int) {});
       }
     }
     lds_barrier8();

@@ -114,7 +114,8 @@ def make(t, e, h, i, k, dtype=torch.bfloat16, seed=0, whole=True):
 # few pairs, rows of 16 and 32, tiles; hidden and intermediate sizes cut every way, more experts than pairs and fewer
 SHAPES = [(1, 8, 256, 128, 2), (1, 128, 2048, 768, 8), (3, 40, 144, 80, 8), (5, 16, 1040, 208, 3), (7, 64, 272, 1040, 9),
           (60, 8, 512, 192, 2), (200, 64, 528, 192, 8), (40, 4, 384, 96, 3), (170, 6, 272, 336, 1), (33, 1, 256, 256, 1),
-          (700, 4, 512, 192, 2), (1111, 8, 400, 272, 4), (2000, 3, 1040, 144, 2), (500, 5, 128, 16, 2), (300, 2, 16, 640, 2)]
+          (700, 4, 512, 192, 2), (1111, 8, 400, 272, 4), (2000, 3, 1040, 144, 2), (500, 5, 128, 16, 2), (300, 2, 16, 640, 2), (5000, 70, 64, 32, 2),
+          (3000, 20, 128, 64, 8)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
