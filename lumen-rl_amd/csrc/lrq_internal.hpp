@@ -290,9 +290,9 @@ hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, void* workspace, hipS
 // Routing to experts (lrq_route.hip).
 constexpr int kRouteExpertsMax = 512, kRouteGroupsMax = 16;  // one lane of 16 looks through a group
 constexpr int kRouteMost = 64;       // top_k: four a lane
-constexpr int kRoutePitch = kRouteMost + 2;
-constexpr float kRouteTol = 0x1p-18f;  // picks nearer than this (relative to 1 + |pick|) are compared in float64: four
-                                       // times what float32 scores and sums are off by at most
+constexpr int kRoutePitch = kRouteMost + 2, kRouteWords = 2 * kRoutePitch + kRouteGroupsMax;
+constexpr float kRouteTol = 0x1p-18f;  // picks nearer than this (relative to 1 + |pick|) are compared in float64: at
+                                       // least twice what float32 scores, sums and fixed-point values are off by
 struct RouteArgs {
   const void* logits;  // [tokens, experts], row pitch ld
   const float* bias;   // null: none

@@ -197,8 +197,8 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_mm8_tiles(MatmulArgs a, int
     store_tile<kF32>(part, acc, src.n0 + wn, src.m0 + wm, lds);
   } else {
     tile_sums<FN, FM, WN, WM, STAGES, DMA, false, EXACT>(src, (int)a.k, 0, (int)a.kb, lds, acc);
-    if (EXACT && a.out_dtype == kF32) return store_tile<kF32>(a, acc, src.n0 + wn, src.m0 + wm, lds);
-    if (a.out_dtype == kBF16) return store_tile<kBF16>(a, acc, src.n0 + wn, src.m0 + wm, lds);
+    if constexpr (EXACT) return store_tile<kF32>(a, acc, src.n0 + wn, src.m0 + wm, lds);
+    else if (a.out_dtype == kBF16) return store_tile<kBF16>(a, acc, src.n0 + wn, src.m0 + wm, lds);
     else return store_tile<kF16>(a, acc, src.n0 + wn, src.m0 + wm, lds);
   }
 }
@@ -270,11 +270,13 @@ static void launch_tiles_of(const MatmulArgs& a, hipStream_t stream) {
 constexpr int64_t kDots = 4, kSplitRows = 64;
 bool matmul_quantizes(int64_t m, int64_t k) { return m <= kDots && m * ceil_div(k, kBlk) * (kBlk + 4) <= 65536; }
 
-// Parts of K: a work-group for every CU, of 4 blocks at least.
+// Parts of K: a work-group for every CU, of 3 blocks at least.  48 tokens x [4096,
+// 12288] in 4 parts of 24 blocks 16.5 us, 18.4 in 8, 28 in one; 64-row tiles, as 128-row
+// ones are two times fewer (19 us).
 static int64_t split_parts(int64_t m, int64_t n, int64_t k) {
   if (m <= kDots || m > kSplitRows) return 1;
   const int64_t tiles = ceil_div(n, 64), kb = ceil_div(k, kBlk);
-  int64_t parts = 512 / tiles < kb / 4 ? 512 / tiles : kb / 4;
+  int64_t parts = 256 / tiles < kb / 3 ? 256 / tiles : kb / 3;
   if (parts < 2) return 1;
   return ceil_div(kb, ceil_div(kb, parts));  // none of them empty
 }
@@ -283,20 +285,32 @@ int64_t matmul_workspace(int64_t m, int64_t n, int64_t k) {
   return parts > 1 ? 4 * parts * m * n : 0;
 }
 
+template <bool EXACT>
+static void launch_few(const MatmulArgs& a, float* sums, hipStream_t stream) {
+  const int64_t parts = split_parts(a.m, a.n, a.k);
+  if (parts > 1) {
+    if (dma_ok(a)) launch_tiles<1, 4, 4, 1, 4, true, EXACT, true>(a, stream, sums, (int)parts);
+    else launch_tiles<1, 4, 4, 1, 2, false, EXACT, true>(a, stream, sums, (int)parts);
+    hipLaunchKernelGGL(k_mm8_join, dim3((unsigned)ceil_div(a.m * a.n, 256)), dim3(256), 0, stream, a, sums, (int)parts);
+  } else if (dma_ok(a)) {
+    launch_tiles<1, 4, 4, 1, 4, true, EXACT>(a, stream);
+  } else {
+    launch_tiles<1, 4, 4, 1, 2, false, EXACT>(a, stream);
+  }
+}
+
 hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, void* workspace, hipStream_t stream) {
   if (a.m <= kDots) {
     if (x_dtype == kBF16) launch_dots<kBF16>(a, stream);
     else if (x_dtype == kF16) launch_dots<kF16>(a, stream);
     else if (x_dtype == kF32) launch_dots<kF32>(a, stream);
     else launch_dots<-1>(a, stream);
-  } else if (const int64_t parts = split_parts(a.m, a.n, a.k); parts > 1) {
-    float* const sums = static_cast<float*>(workspace);
-    if (dma_ok(a)) launch_tiles<1, 4, 4, 1, 4, true, true, true>(a, stream, sums, (int)parts);
-    else launch_tiles<1, 4, 4, 1, 2, false, true, true>(a, stream, sums, (int)parts);
-    hipLaunchKernelGGL(k_mm8_join, dim3((unsigned)ceil_div(a.m * a.n, 256)), dim3(256), 0, stream, a, sums, (int)parts);
-  } else if (a.m <= kSplitRows || a.out_dtype == kF32) {
-    if (a.m > kSplitRows) dma_ok(a) ? launch_tiles_of<true, true>(a, stream) : launch_tiles_of<false, true>(a, stream);
-    else dma_ok(a) ? launch_tiles<1, 4, 4, 1, 4, true, true>(a, stream) : launch_tiles<1, 4, 4, 1, 2, false, true>(a, stream);
+  } else if (a.m <= kSplitRows) {
+    if (a.out_dtype == kF32) launch_few<true>(a, static_cast<float*>(workspace), stream);
+    else launch_few<false>(a, static_cast<float*>(workspace), stream);
+  } else if (a.out_dtype == kF32) {
+    if (dma_ok(a)) launch_tiles_of<true, true>(a, stream);
+    else launch_tiles_of<false, true>(a, stream);
   } else {
     if (dma_ok(a)) launch_tiles_of<true, false>(a, stream);
     else launch_tiles_of<false, false>(a, stream);

@@ -7,16 +7,19 @@
 //        lowest index; weights: scale score_id, over sum score_id if renormalized.
 //
 // The choice is that of exact arithmetic, up to 64-bit rounding.  Without a bias
-// both scores rise with the logit, so logits are compared, as they are.  Picks and
-// sums of two scores are computed in float32; a token with two neighbours in the
-// order (or two groups) nearer to each other than float32 can tell is chosen again
-// by its whole wave in float64, unless the two have the same logit and bias and so
-// are a tie.  With random biases that happens to some 0.1 % of tokens, and costs
-// nothing to the rest.
+// both scores rise with the logit, so logits are compared.  Picks, and sums of two
+// scores, are computed in float32.  What is compared becomes one word of an expert:
+// the order of a 16-bit logit above the index, or a fixed-point value (23 to 25 bits
+// of the 4 below a token's highest pick, of the 64 below its highest logit) above
+// it; so a round of the choice is one maximum, and ties go to the lowest index.  A
+// token with two neighbours in that order (or two groups) nearer to each other than
+// the words can tell is chosen again by its whole wave in float64, unless the two
+// have the same logit and bias and so are a tie.  With random biases that happens to
+// some 0.1 % of tokens, and costs the rest nothing.
 //
-// Moves little: 2 or 4 bytes an expert.  What it spends is instructions, some 4 an
-// expert for each of the top_k rounds; so 16 lanes take a token, four tokens a
-// wave, whose maxima go through DPP rows without LDS.
+// Moves little: 2 or 4 bytes an expert.  What it spends is instructions, 1.5 an
+// expert for each of the top_k rounds and some 15 before; so 16 lanes take a token,
+// four tokens a wave, whose maxima go through DPP rows without LDS.
 #include "lrq.h"
 #include "lrq_device.hpp"
 #include "lrq_internal.hpp"
@@ -34,9 +37,6 @@ __device__ __forceinline__ uint32_t order32(float v) {
   const uint32_t b = f2u(v + 0.0f);
   return v != v ? 0xFFFFFFFFu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float order32_value(uint32_t k) {
-  return u2f(k ^ (k & 0x80000000u ? 0x80000000u : 0xFFFFFFFFu));
-}
 __device__ __forceinline__ uint64_t order64(double v) {
   const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
   return v != v ? ~0ull : b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
@@ -52,9 +52,6 @@ __device__ __forceinline__ uint32_t row16(uint32_t v, F f) {
   v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));
   v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));
   return f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, false));
-}
-__device__ __forceinline__ uint32_t row_min(uint32_t v) {
-  return row16(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
 }
 __device__ __forceinline__ uint32_t row_max(uint32_t v) {
   return row16(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
@@ -203,7 +200,7 @@ __device__ __forceinline__ void choose_wide(const RouteArgs& a, int64_t token, u
     wave_fence8();
 #pragma unroll
     for (int j = 0; j < J; ++j)
-      if (lane + 64 * j < a.experts) stage[lane + 64 * j] = order64(p[j]);
+      if (lane + 64 * j < a.experts) stage[lane + 64 * j] = order64(by_logit && a.group_top == 1 ? (double)x[j] : p[j]);
     wave_fence8();
     uint64_t value = 0;
     if (lane < a.groups) {
@@ -248,46 +245,75 @@ __device__ __forceinline__ void choose_wide(const RouteArgs& a, int64_t token, u
 // ---------------------------------------------------------------------------
 // the router
 // ---------------------------------------------------------------------------
-// What keys hold: bf16 logits have 16 bits of order, so the index goes below them
-// and one maximum gives both; other logits, and picks, take a second look for the
-// lowest index that has the maximum.
-enum RouteKeys { kKeysPacked, kKeysLogit, kKeysPick };
+enum RouteKeys { kKeysLogit16, kKeysLogit32, kKeysPick };
+
+__device__ __forceinline__ void top_two(float& first, float& second, float a, float b) {  // a >= b
+  second = fmaxf(fmaxf(second, b), fminf(first, a));
+  first = fmaxf(first, a);
+}
 
 template <int DT, int CHUNKS, int KEYS>
 __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
   constexpr int S = 8 * CHUNKS;
-  // words of LDS: each token's choice and its keys, then (with groups) its picks
+  constexpr int BITS = KEYS == kKeysLogit16 ? 16 : CHUNKS == 1 ? 7 : CHUNKS == 2 ? 8 : 9;  // of the index
+  constexpr uint32_t kIndex = (1u << BITS) - 1;
+  constexpr float kWindow = KEYS == kKeysPick ? 4.0f : 64.0f, kMost = (float)((1ull << (32 - BITS)) - 16);
+  // words of LDS: each token's choice and its keys, its groups' values, then (with
+  // groups) its picks
   extern __shared__ __attribute__((aligned(16))) uint32_t lds_route[];
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, row = tid >> 4;
   const int64_t token = (int64_t)blockIdx.x * kRouteTokens + row;
   const int64_t mine = token < a.tokens ? token : a.tokens - 1;
   const uint8_t* const logits = static_cast<const uint8_t*>(a.logits) + mine * a.ld * (DT == kF32 ? 4 : 2);
-  uint32_t* const ids = lds_route + row * 2 * kRoutePitch;
+  uint32_t* const ids = lds_route + row * kRouteWords;
   uint32_t* const keys = ids + kRoutePitch;
-  uint32_t* const waves = lds_route + 2 * kRoutePitch * kRouteTokens + (tid >> 6) * 4 * a.experts;  // the wave's stage
-  uint32_t* const stage = waves + (row & 3) * a.experts;
+  float* const values = reinterpret_cast<float*>(keys + kRoutePitch);
+  uint32_t* const waves = lds_route + kRouteWords * kRouteTokens + (tid >> 6) * 4 * a.experts;  // the wave's stage
+  float* const stage = reinterpret_cast<float*>(waves + (row & 3) * a.experts);
 
-  float x[S];
+  float x[S], v[S];  // v: what orders experts
   load_row<DT, CHUNKS>(logits, a.experts, l, x);
-  uint32_t key[S];
   bool unsure = false;
   float poison = 0.0f;  // NaN where a logit that need not be chosen makes every softmax score NaN
+#pragma unroll
+  for (int s = 0; s < S; s += 2) unsure |= __builtin_isunordered(x[s], x[s + 1]);  // past the last expert they are 0
   if constexpr (KEYS == kKeysPick) {
-    float p[S];
-    quick_scores<CHUNKS>(a, x, l, true, p);
-    if (!a.sigmoid) poison = 0.0f * p[0];
+    quick_scores<CHUNKS>(a, x, l, true, v);
+    if (!a.sigmoid) poison = 0.0f * v[0];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       float b[8];
       load_acts<kF32>(a.bias, 128 * c + 8 * l, a.experts, b);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) key[8 * c + i] = order32(p[8 * c + i] + b[i]);
+      for (int i = 0; i < 8; ++i) v[8 * c + i] += b[i];
     }
+#pragma unroll
+    for (int s = 0; s < S; s += 2) unsure |= __builtin_isunordered(v[s], v[s + 1]);
   } else {
 #pragma unroll
+    for (int s = 0; s < S; ++s) v[s] = x[s];
+  }
+
+  uint32_t key[S];
+  float low = 0.0f;
+  if constexpr (KEYS == kKeysLogit16) {
+#pragma unroll
     for (int s = 0; s < S; ++s) {
-      key[s] = order32(x[s]);
-      if (KEYS == kKeysPacked) key[s] = (key[s] & 0xFFFF0000u) | (uint32_t)(0xFFFF - expert_of(s, l));
+      const uint32_t b = DT == kBF16 ? f2u(x[s] + 0.0f) >> 16 : f16_bits(x[s] + 0.0f);
+      const uint32_t order = b & 0x8000u ? 0xFFFFu ^ b : 0x8000u | b;
+      key[s] = order << 16 | (kIndex - (uint32_t)expert_of(s, l));
+    }
+  } else {
+    float top = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < S; ++s) top = fmaxf(top, expert_of(s, l) < a.experts ? v[s] : -INFINITY);
+    top = row_fmax(top);
+    unsure |= fabsf(top) == INFINITY;
+    low = top - kWindow;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const float q = fmaxf((v[s] - low) * (kMost / kWindow), 1.0f);  // rises with v; NaN and below the window: 1
+      key[s] = (uint32_t)q << BITS | (kIndex - (uint32_t)expert_of(s, l));
     }
   }
 #pragma unroll
@@ -296,81 +322,95 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
 
   if (a.groups > 1) {
     const int size = a.experts / a.groups;
-    const bool sums = KEYS == kKeysPick || a.group_top == 2;
-    if (KEYS != kKeysPick && a.group_top == 2) {
-      float p[S];
-      quick_scores<CHUNKS>(a, x, l, false, p);
+    const bool sums = KEYS == kKeysPick || a.group_top == 2;  // otherwise logits, which are exact
+    if (KEYS != kKeysPick && a.group_top == 2) quick_scores<CHUNKS>(a, x, l, false, v);
+    float first = -INFINITY, second = -INFINITY;  // lane g: of group g
+    if (size % 8 == 0) {  // a lane's 8 experts are in one group
 #pragma unroll
-      for (int s = 0; s < S; ++s)
-        if (expert_of(s, l) < a.experts) stage[expert_of(s, l)] = order32(p[s]);
+      for (int c = 0; c < CHUNKS; ++c) {
+        float one = v[8 * c], two = -INFINITY;
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top_two(one, two, v[8 * c + i], -INFINITY);
+        if (128 * c + 8 * l < a.experts) {
+          stage[2 * (16 * c + l)] = one;
+          stage[2 * (16 * c + l) + 1] = two;
+        }
+      }
+      wave_fence8();
+      if (l < a.groups)
+        for (int i = 0; i < size / 8; ++i) {
+          const float* const p = stage + 2 * (l * (size / 8) + i);
+          top_two(first, second, p[0], p[1]);
+        }
     } else {
 #pragma unroll
       for (int s = 0; s < S; ++s)
-        if (expert_of(s, l) < a.experts) stage[expert_of(s, l)] = key[s];
-    }
-    wave_fence8();
-    // lane g looks through group g, each from another place: no bank conflicts
-    uint32_t first = 0, second = 0;
-    if (l < a.groups) {
-      int at = l % size;
-      for (int i = 0; i < size; ++i) {
-        const uint32_t k = stage[l * size + at];
-        const uint32_t low = k < first ? k : first;
-        second = second > low ? second : low;
-        first = first > k ? first : k;
-        at = at + 1 < size ? at + 1 : 0;
+        if (expert_of(s, l) < a.experts) stage[expert_of(s, l)] = v[s];
+      wave_fence8();
+      if (l < a.groups) {
+        int at = l % size;  // each lane from another place: no bank conflicts
+        for (int i = 0; i < size; ++i) {
+          top_two(first, second, stage[l * size + at], -INFINITY);
+          at = at + 1 < size ? at + 1 : 0;
+        }
       }
     }
-    float value = order32_value(first);
-    if (a.group_top == 2 && size > 1) value += order32_value(second);
-    const uint32_t rank = sums ? order32(value) : first;
+    const float value = a.group_top == 2 && size > 1 ? first + second : first;
+    values[l] = l < a.groups ? value : -INFINITY;
+    wave_fence8();
     int before = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const uint32_t o = (uint32_t)__shfl((int)rank, g, 16);
-      before += o > rank || (o == rank && g < l) ? 1 : 0;
-      if (sums && g != l && !(fabsf(order32_value(o) - value) > kRouteTol * (2.0f + fabsf(value)))) unsure = true;
+#pragma unroll
+    for (int g = 0; g < kRouteGroupsMax; ++g) {
+      const float o = values[g];
+      before += g < a.groups && (o > value || (o == value && g < l)) ? 1 : 0;
+      unsure |= sums && l < a.groups && g < a.groups && g != l && !(fabsf(o - value) > kRouteTol * (2.0f + fabsf(value)));
     }
-    unsure = unsure && l < a.groups;
     const uint64_t all = __ballot(l < a.groups && before < a.top_groups);
     const uint32_t allowed = (uint32_t)(all >> (lane & 48)) & 0xFFFFu;
     const uint32_t recip = group_recip(size);
+    if (size % 8 == 0) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const uint32_t g = (uint32_t)expert_of(s, l) * recip >> 20;
-      if (!(allowed >> (g & 31) & 1)) key[s] = 0;
+      for (int c = 0; c < CHUNKS; ++c) {
+        const uint32_t g = (uint32_t)(128 * c + 8 * l) * recip >> 20;
+        const bool open = allowed >> (g & 31) & 1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) key[8 * c + i] = open ? key[8 * c + i] : 0;
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const uint32_t g = (uint32_t)expert_of(s, l) * recip >> 20;
+        if (!(allowed >> (g & 31) & 1)) key[s] = 0;
+      }
     }
   }
 
+  // Rounds: the highest key below the last one.  key - last wraps round for the keys
+  // below it, which so come above all others, in their order.
   const int left = a.groups > 1 ? a.experts / a.groups * a.top_groups : a.experts;
-  const int rounds = KEYS == kKeysPick && left > a.top_k ? a.top_k + 1 : a.top_k;
+  const int rounds = KEYS != kKeysLogit16 && left > a.top_k ? a.top_k + 1 : a.top_k;
+  uint32_t last = 0;
   for (int i = 0; i < rounds; ++i) {
     uint32_t best = 0;
 #pragma unroll
-    for (int s = 0; s < S; ++s) best = key[s] > best ? key[s] : best;
-    best = row_max(best);
-    uint32_t e;
-    if constexpr (KEYS == kKeysPacked) {
-      e = 0xFFFFu - (best & 0xFFFFu);
-#pragma unroll
-      for (int s = 0; s < S; ++s) key[s] = key[s] == best ? 0 : key[s];
-    } else {
-      e = 0xFFFFu;
-#pragma unroll
-      for (int s = S - 1; s >= 0; --s) e = key[s] == best ? (uint32_t)expert_of(s, l) : e;
-      e = row_min(e);
-#pragma unroll
-      for (int s = 0; s < S; ++s) key[s] = e == (uint32_t)expert_of(s, l) ? 0 : key[s];
+    for (int s = 0; s < S; ++s) {
+      const uint32_t k = key[s] - last;
+      best = k > best ? k : best;
     }
-    if (l == 0) ids[i] = e, keys[i] = best;
+    last += row_max(best);
+    if (l == 0) ids[i] = kIndex - (last & kIndex), keys[i] = last >> BITS;
   }
   wave_fence8();
-  if constexpr (KEYS == kKeysPick) {
+  if constexpr (KEYS != kKeysLogit16) {
     for (int i = l; i + 1 < rounds; i += 16) {
-      const float here = order32_value(keys[i]), next = order32_value(keys[i + 1]);
-      if (fabsf(here - next) > kRouteTol * (1.0f + fabsf(here))) continue;
+      const float here = (float)keys[i], next = (float)keys[i + 1];
+      if (KEYS == kKeysPick ? (here - next) * (kWindow / kMost) > kRouteTol * (1.0f + fabsf(low) + kWindow) : here != next) continue;
       const uint32_t e = ids[i], f = ids[i + 1];
-      const float xe = load_as_f32(logits, DT, e), xf = load_as_f32(logits, DT, f);
-      unsure = unsure || !(xe == xf && gld<float>(a.bias + e) == gld<float>(a.bias + f));
+      const float xe = load_as_f32(logits, DT, e < (uint32_t)a.experts ? e : 0), xf = load_as_f32(logits, DT, f < (uint32_t)a.experts ? f : 0);
+      bool tie = xe == xf;
+      if (KEYS == kKeysPick)
+        tie &= gld<float>(a.bias + (e < (uint32_t)a.experts ? e : 0)) == gld<float>(a.bias + (f < (uint32_t)a.experts ? f : 0));
+      unsure |= !tie;
     }
   }
   uint64_t again = __ballot(unsure);
@@ -380,7 +420,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
     const int64_t t = (int64_t)blockIdx.x * kRouteTokens + (row & ~3) + r;
     wave_fence8();
     choose_wide<DT, CHUNKS>(a, t < a.tokens ? t : a.tokens - 1, reinterpret_cast<uint64_t*>(waves),
-                            lds_route + ((row & ~3) + r) * 2 * kRoutePitch);
+                            lds_route + ((row & ~3) + r) * kRouteWords);
   }
   wave_fence8();
 
@@ -509,9 +549,9 @@ static void launch(const RouteArgs& a, const float* grad, void* out, hipStream_t
     hipLaunchKernelGGL((k_route_grad<DT, CHUNKS>), grid, dim3(256), 0, stream, a, grad, out);
     return;
   }
-  const unsigned lds = 4 * kRouteTokens * (2 * kRoutePitch + (a.groups > 1 ? a.experts : 0));
+  const unsigned lds = 4 * kRouteTokens * (kRouteWords + (a.groups > 1 ? a.experts : 0));
   if (a.bias != nullptr) hipLaunchKernelGGL((k_route<DT, CHUNKS, kKeysPick>), grid, dim3(256), lds, stream, a);
-  else hipLaunchKernelGGL((k_route<DT, CHUNKS, DT == kBF16 ? kKeysPacked : kKeysLogit>), grid, dim3(256), lds, stream, a);
+  else hipLaunchKernelGGL((k_route<DT, CHUNKS, DT == kF32 ? kKeysLogit32 : kKeysLogit16>), grid, dim3(256), lds, stream, a);
 }
 template <int DT>
 static void launch_of(const RouteArgs& a, const float* grad, void* out, hipStream_t stream) {

@@ -8,6 +8,7 @@ current stream of its operands' device and returns without synchronizing.
 
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -123,6 +124,11 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: O
     return _route(logits, ids, bias, cfg), ids
 
 
+@functools.lru_cache(maxsize=4096)
+def _experts_workspace(rows: int, hidden: int, inter: int, experts: int, top_k: int) -> int:
+    return _lib.lib().lrq_fp8_experts_workspace(rows, hidden, inter, experts, top_k)
+
+
 def fp8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_up_scales: Tensor, down: Tensor,
                 down_scales: Tensor) -> Tensor:
     """The chosen experts' SwiGLU MLPs in FP8, and their weighted sum.
@@ -166,13 +172,12 @@ def fp8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_u
     gate_up, down = (w if w.data_ptr() % 16 == 0 else w.clone() for w in (gate_up, down))
     ids, weights = ids.contiguous(), weights.contiguous()
     out = _dense((*lead, h), x.dtype, dev)
-    L = _lib.lib()
-    need = L.lrq_fp8_experts_workspace(rows, h, i, e, k)
+    need = _experts_workspace(rows, h, i, e, k)
     work = _dense((need,), torch.uint8, dev)
     with _on(dev):
-        rc = L.lrq_fp8_experts(x.data_ptr(), _IN_DTYPES[x.dtype], rows, h, ld, ids.data_ptr(), weights.data_ptr(), k,
-                               gate_up.data_ptr(), gate_up_scales.data_ptr(), down.data_ptr(), down_scales.data_ptr(), e, i,
-                               out.data_ptr(), work.data_ptr(), need, _stream(dev))
+        rc = _lib.lib().lrq_fp8_experts(x.data_ptr(), _IN_DTYPES[x.dtype], rows, h, ld, ids.data_ptr(), weights.data_ptr(), k,
+                                        gate_up.data_ptr(), gate_up_scales.data_ptr(), down.data_ptr(), down_scales.data_ptr(),
+                                        e, i, out.data_ptr(), work.data_ptr(), need, _stream(dev))
     if rc:
         _lib.check(rc, "lrq_fp8_experts")
     return out

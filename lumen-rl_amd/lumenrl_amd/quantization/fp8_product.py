@@ -10,6 +10,7 @@ stream of the operands' device.
 
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -27,11 +28,11 @@ def check_tiles(what: str, codes: Tensor, scales: Tensor, device: torch.device) 
         raise TypeError(f"{what}: codes and scales must be tensors")
     if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
         raise TypeError(f"{what}: codes must be float8_e4m3fn with float32 scales, got {codes.dtype} and {scales.dtype}")
-    if codes.dim() < 2:
-        raise ValueError(f"{what}: codes must have rows and columns, got {tuple(codes.shape)}")
-    *lead, n, k = codes.shape
-    if scales.shape != (*lead, -(-n // _BLOCK), -(-k // _BLOCK)):
-        raise ValueError(f"{what}: scales {tuple(scales.shape)} are not those of 128x128 tiles of {tuple(codes.shape)}")
+    shape = codes.shape
+    if len(shape) < 2:
+        raise ValueError(f"{what}: codes must have rows and columns, got {tuple(shape)}")
+    if scales.shape != (*shape[:-2], -(-shape[-2] // _BLOCK), -(-shape[-1] // _BLOCK)):
+        raise ValueError(f"{what}: scales {tuple(scales.shape)} are not those of 128x128 tiles of {tuple(shape)}")
     if codes.device != device or scales.device != device:
         raise ValueError(f"{what}: codes and scales must be on {device}")
     return (codes if codes.is_contiguous() else codes.contiguous(),
@@ -49,6 +50,11 @@ def _check_bias(what: str, bias: Optional[Tensor], n: int, device: torch.device)
 def _empty_sum(rows: int, n: int, bias: Optional[Tensor], dtype: torch.dtype, device: torch.device) -> Tensor:
     y = torch.zeros((rows, n), dtype=torch.float32, device=device)
     return (y if bias is None else y + bias).to(dtype)
+
+
+@functools.lru_cache(maxsize=4096)
+def _matmul_workspace(rows: int, k: int, n: int) -> int:
+    return _lib.lib().lrq_fp8_matmul_workspace(rows, k, n)
 
 
 def fp8_matmul(x_codes: Tensor, x_scales: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Tensor] = None, *,
@@ -83,16 +89,20 @@ def fp8_matmul(x_codes: Tensor, x_scales: Tensor, codes: Tensor, scales: Tensor,
     if not x_scales.is_contiguous():
         x_scales = x_scales.contiguous()
     out = _dense((m, n), out_dtype, dev)
-    L = _lib.lib()
-    need = L.lrq_fp8_matmul_workspace(m, k, n)
+    need = _matmul_workspace(m, k, n)
     work = _dense((need,), torch.uint8, dev) if need else None
     with _on(dev):
-        rc = L.lrq_fp8_matmul(x_codes.data_ptr(), x_scales.data_ptr(), m, k, ld, codes.data_ptr(), scales.data_ptr(), n,
-                              bias_ptr, bias_dtype, out.data_ptr(), _IN_DTYPES[out_dtype],
-                              work.data_ptr() if need else None, need, _stream(dev))
+        rc = _lib.lib().lrq_fp8_matmul(x_codes.data_ptr(), x_scales.data_ptr(), m, k, ld, codes.data_ptr(), scales.data_ptr(), n,
+                                       bias_ptr, bias_dtype, out.data_ptr(), _IN_DTYPES[out_dtype],
+                                       work.data_ptr() if need else None, need, _stream(dev))
     if rc:
         _lib.check(rc, "lrq_fp8_matmul")
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_workspace(rows: int, k: int, n: int) -> int:
+    return _lib.lib().lrq_fp8_block_linear_workspace(rows, k, n)
 
 
 def fp8_block_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Tensor] = None) -> Tensor:
@@ -105,29 +115,28 @@ def fp8_block_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Te
     _check_input(x, "fp8_block_linear")
     dev = x.device
     codes, scales = check_tiles("fp8_block_linear", codes, scales, dev)
-    if x.dim() < 1 or codes.dim() != 2 or x.shape[-1] != codes.shape[1]:
-        raise ValueError(f"fp8_block_linear: x {tuple(x.shape)} and codes {tuple(codes.shape)} do not fit")
+    shape = x.shape
+    if not shape or codes.dim() != 2 or shape[-1] != codes.shape[1]:
+        raise ValueError(f"fp8_block_linear: x {tuple(shape)} and codes {tuple(codes.shape)} do not fit")
     n, k = codes.shape
-    lead = x.shape[:-1]
-    bias_ptr, bias_dtype = _check_bias("fp8_block_linear", bias, n, dev)
+    bias_ptr, bias_dtype = (None, 0) if bias is None else _check_bias("fp8_block_linear", bias, n, dev)
     if k == 0:
-        return _empty_sum(_prod(lead), n, bias, x.dtype, dev).view(*lead, n)
-    if x.dim() == 2 and x.is_contiguous():
-        rows, ld = x.shape[0], k
+        return _empty_sum(_prod(shape[:-1]), n, bias, x.dtype, dev).view(*shape[:-1], n)
+    if x.is_contiguous():
+        rows, ld = x.numel() // k, k
     else:
         rows = x.numel() // k
         x = x.reshape(rows, k)
         ld = x.stride(0) if rows > 1 else k
         if (k > 1 and x.stride(1) != 1) or ld < k:
             x, ld = x.contiguous(), k
-    out = _dense((*lead, n), x.dtype, dev)
-    L = _lib.lib()
-    need = L.lrq_fp8_block_linear_workspace(rows, k, n)
+    out = _dense((*shape[:-1], n), x.dtype, dev)
+    need = _linear_workspace(rows, k, n)
     work = _dense((need,), torch.uint8, dev) if need else None
+    dtype = _IN_DTYPES[x.dtype]
     with _on(dev):
-        rc = L.lrq_fp8_block_linear(x.data_ptr(), _IN_DTYPES[x.dtype], rows, k, ld, codes.data_ptr(), scales.data_ptr(), n,
-                                    bias_ptr, bias_dtype, out.data_ptr(), work.data_ptr() if need else None, need,
-                                    _stream(dev))
+        rc = _lib.lib().lrq_fp8_block_linear(x.data_ptr(), dtype, rows, k, ld, codes.data_ptr(), scales.data_ptr(), n, bias_ptr,
+                                             bias_dtype, out.data_ptr(), work.data_ptr() if need else None, need, _stream(dev))
     if rc:
         _lib.check(rc, "lrq_fp8_block_linear")
     return out

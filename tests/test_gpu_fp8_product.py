@@ -37,8 +37,8 @@ def check(y, x_codes, x_scales, codes, scales, bias=None):
     """|y - exact| within the result's rounding and the sums' own bound.
 
     A block sums 128 exact products in float32, K/128 blocks and 8 waves' parts follow, each step off by at most
-    2^-23 of the terms' magnitude, and the product of the two scales by 2^-24.  16-bit results of more than 64
-    tokens come from matrix instructions that drop what is 2^-13 below the block's largest product: 128 times
+    2^-23 of the terms' magnitude, and the product of the two scales by 2^-24.  16-bit results of more than
+    four tokens come from matrix instructions that drop what is 2^-13 below the block's largest product: 128 times
     that for each block."""
     (m, k), n = x_codes.shape, codes.shape[0]
     xd = x_codes.double() * spread(x_scales, m, k, (1, 128))
@@ -49,7 +49,7 @@ def check(y, x_codes, x_scales, codes, scales, bias=None):
     half = torch.finfo(y.dtype).eps / 2
     least = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24, torch.float32: 2.0 ** -149}[y.dtype]
     bound = half * want.abs() * 1.01 + (128 + k // 128 + 12) * 2.0 ** -23 * size + least
-    if m > 64 and y.dtype != torch.float32:
+    if m > 4 and y.dtype != torch.float32:
         for b in range(0, k, 128):
             top = xd[:, b: b + 128].abs().amax(1)[:, None] * wd[:, b: b + 128].abs().amax(1)[None]
             bound += 128 * 2.0 ** -13 * top
@@ -57,8 +57,8 @@ def check(y, x_codes, x_scales, codes, scales, bias=None):
     assert bool((off <= bound).all()), float((off / bound).max())
 
 
-# tokens of each kernel (few: up to 16, 32, 64; tiles of three sizes), weights cut in every way
-SHAPES = [(1, 1, 1), (1, 4096, 4096), (3, 200, 130), (16, 130, 1104), (16, 64, 12288), (17, 129, 384), (33, 1, 1100), (64, 300, 272),
+# tokens of each kernel (up to four: dot products; up to 64: K in parts; tiles of four sizes), weights cut in every way
+SHAPES = [(1, 1, 1), (2, 77, 2100), (4, 4100, 515), (1, 5000, 1032), (1, 4096, 4096), (3, 200, 130), (16, 130, 1104), (16, 64, 12288), (17, 129, 384), (33, 1, 1100), (64, 300, 272),
           (65, 127, 15), (65, 128, 128), (100, 130, 144), (777, 1500, 1100), (2000, 2040, 1040), (1999, 2041, 1041), (4100, 3850, 272),
           (130, 190, 1036), (300, 129, 1164), (2000, 2040, 1048), (4100, 3850, 268), (70, 65, 4), (400, 12300, 128), (1100, 6200, 144)]
 
