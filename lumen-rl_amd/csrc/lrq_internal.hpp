@@ -291,8 +291,12 @@ hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, void* workspace, hipS
 constexpr int kRouteExpertsMax = 512, kRouteGroupsMax = 16;  // one lane of 16 looks through a group
 constexpr int kRouteMost = 64;       // top_k: four a lane
 constexpr int kRoutePitch = kRouteMost + 2, kRouteWords = 2 * kRoutePitch + kRouteGroupsMax;
-constexpr float kRouteTol = 0x1p-18f;  // picks nearer than this (relative to 1 + |pick|) are compared in float64: at
-                                       // least twice what float32 scores, sums and fixed-point values are off by
+// Picks nearer than this (relative to 1 + |pick|, twice it for softmax) are compared
+// in float64.  Two picks are off by 2^-22 each for their scores (softmax, whose sum is
+// too, by 2^-20), 2^-24 |pick| for the bias, 2^-24 of the window of 4 for its
+// difference and as much for its product, and 2^-21 together for whole numbers:
+// 2^-19 (2^-18.2) at most.  Sums of two picks have no whole numbers.
+constexpr float kRouteTol = 0x1p-19f;
 struct RouteArgs {
   const void* logits;  // [tokens, experts], row pitch ld
   const float* bias;   // null: none

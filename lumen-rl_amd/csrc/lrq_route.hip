@@ -138,26 +138,32 @@ __device__ __forceinline__ void quick_scores(const RouteArgs& a, const float* x,
 // ---------------------------------------------------------------------------
 // one token's choice in float64, by a whole wave
 // ---------------------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ uint64_t moved64(uint64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)v, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(v >> 32), CTRL, 0xF, 0xF, false);
+  return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+// Over the wave, in DPP rows and then from one lane of each.
+template <class F>
+__device__ __forceinline__ uint64_t wave64(uint64_t v, F f) {
+  v = f(v, moved64<0xB1>(v));
+  v = f(v, moved64<0x4E>(v));
+  v = f(v, moved64<0x141>(v));
+  v = f(v, moved64<0x140>(v));
+  return f(f(lane64(v, 0), lane64(v, 16)), f(lane64(v, 32), lane64(v, 48)));
+}
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    const uint64_t o = (uint64_t)__shfl_xor((unsigned long long)v, off, 64);
-    v = v > o ? v : o;
-  }
-  return v;
+  return wave64(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
 }
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
-}
-__device__ __forceinline__ uint32_t wave_min32(uint32_t v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)v, off, 64);
-    v = v < o ? v : o;
-  }
-  return v;
+  return __longlong_as_double((long long)wave64((uint64_t)__double_as_longlong(v), [](uint64_t a, uint64_t b) {
+    return (uint64_t)__double_as_longlong(__longlong_as_double((long long)a) + __longlong_as_double((long long)b));
+  }));
 }
 
 template <int DT, int CHUNKS>
@@ -178,8 +184,9 @@ __device__ __forceinline__ void choose_wide(const RouteArgs& a, int64_t token, u
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < J; ++j) top = fmaxf(top, x[j]);
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    top = row_fmax(top);
+    auto row = [&](int lane) { return u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(top), lane)); };
+    top = fmaxf(fmaxf(row(0), row(16)), fmaxf(row(32), row(48)));
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -205,6 +212,7 @@ __device__ __forceinline__ void choose_wide(const RouteArgs& a, int64_t token, u
     uint64_t value = 0;
     if (lane < a.groups) {
       uint64_t first = 0, second = 0;
+#pragma unroll 8
       for (int i = 0; i < size; ++i) {
         const uint64_t k = stage[lane * size + i];
         second = k > first ? first : k > second ? k : second;
@@ -214,7 +222,7 @@ __device__ __forceinline__ void choose_wide(const RouteArgs& a, int64_t token, u
     }
     int before = 0;
     for (int g = 0; g < a.groups; ++g) {
-      const uint64_t o = (uint64_t)__shfl((unsigned long long)value, g, 64);
+      const uint64_t o = lane64(value, g);
       before += o > value || (o == value && g < lane) ? 1 : 0;
     }
     allowed = __ballot(lane < a.groups && before < a.top_groups);
@@ -232,10 +240,12 @@ __device__ __forceinline__ void choose_wide(const RouteArgs& a, int64_t token, u
 #pragma unroll
     for (int j = 0; j < J; ++j) best = key[j] > best ? key[j] : best;
     best = wave_max64(best);
-    uint32_t e = ~0u;
+    uint32_t e = 0;
 #pragma unroll
-    for (int j = J - 1; j >= 0; --j) e = key[j] == best ? (uint32_t)(lane + 64 * j) : e;
-    e = wave_min32(e);
+    for (int j = J - 1; j >= 0; --j) {
+      const uint64_t has = __ballot(key[j] == best);
+      e = has ? 64 * j + (uint32_t)__builtin_ctzll(has) : e;
+    }
 #pragma unroll
     for (int j = 0; j < J; ++j) key[j] = e == (uint32_t)(lane + 64 * j) ? 0 : key[j];
     if (lane == 0) ids[i] = e;
@@ -295,6 +305,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
   }
 
   uint32_t key[S];
+  const float tol = a.sigmoid ? kRouteTol : 2.0f * kRouteTol;
   float low = 0.0f;
   if constexpr (KEYS == kKeysLogit16) {
 #pragma unroll
@@ -363,7 +374,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
     for (int g = 0; g < kRouteGroupsMax; ++g) {
       const float o = values[g];
       before += g < a.groups && (o > value || (o == value && g < l)) ? 1 : 0;
-      unsure |= sums && l < a.groups && g < a.groups && g != l && !(fabsf(o - value) > kRouteTol * (2.0f + fabsf(value)));
+      unsure |= sums && l < a.groups && g < a.groups && g != l && !(fabsf(o - value) > tol * (1.0f + fabsf(value)));
     }
     const uint64_t all = __ballot(l < a.groups && before < a.top_groups);
     const uint32_t allowed = (uint32_t)(all >> (lane & 48)) & 0xFFFFu;
@@ -403,8 +414,8 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
   wave_fence8();
   if constexpr (KEYS != kKeysLogit16) {
     for (int i = l; i + 1 < rounds; i += 16) {
-      const float here = (float)keys[i], next = (float)keys[i + 1];
-      if (KEYS == kKeysPick ? (here - next) * (kWindow / kMost) > kRouteTol * (1.0f + fabsf(low) + kWindow) : here != next) continue;
+      const float here = (float)keys[i] * (kWindow / kMost), next = (float)keys[i + 1] * (kWindow / kMost);
+      if (KEYS == kKeysPick ? here - next > tol * (1.0f + fabsf(low + here)) : keys[i] != keys[i + 1]) continue;
       const uint32_t e = ids[i], f = ids[i + 1];
       const float xe = load_as_f32(logits, DT, e < (uint32_t)a.experts ? e : 0), xf = load_as_f32(logits, DT, f < (uint32_t)a.experts ? f : 0);
       bool tie = xe == xf;
