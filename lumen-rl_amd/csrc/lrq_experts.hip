@@ -214,7 +214,7 @@ struct UpTile {
   }
 };
 
-template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
+template <int FN, int FM, int WN, int WM, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
   static_assert(16 * FN * WN == 256, "128 columns of h");
   constexpr int BM = 16 * FM * WM;
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const UpTile src{a, t, block};
   f32x4 acc[FN][FM], h[FN / 2][FM];
-  tile_sums<FN, FM, WN, WM, STAGES, true, true, EXACT>(src, a.hidden, 0, a.kb, lds, acc);
+  tile_sums<FN, FM, WN, WM, STAGES, true, true, false>(src, a.hidden, 0, a.kb, lds, acc);
 #pragma unroll
   for (int i = 0; i < FN / 2; ++i)
 #pragma unroll
@@ -258,7 +258,7 @@ struct DownTile {
   }
 };
 
-template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
+template <int FN, int FM, int WN, int WM, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_down_tiles(ExpertArgs a) {
   constexpr int BN = 16 * FN * WN;
   static_assert(16 * FN <= kBlk, "one scale for a wave's rows");
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_down_tiles(ExpertArgs a)
   const int c = lane & 15, g = lane >> 4, wn = wave / WM * 16 * FN, wm = wave % WM * 16 * FM;
   const DownTile src{a, t, block * BN};
   f32x4 acc[FN][FM];
-  tile_sums<FN, FM, WN, WM, STAGES, true, false, EXACT>(src, a.inter, 0, a.ib, lds, acc);
+  tile_sums<FN, FM, WN, WM, STAGES, true, false, false>(src, a.inter, 0, a.ib, lds, acc);
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
     const int row = wm + 16 * j + c;
@@ -421,12 +421,15 @@ __global__ __launch_bounds__(512) void k_ex_down_few(ExpertArgs a) {
 // ---------------------------------------------------------------------------
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// Rows of a tile: 0 for few pairs.
+// Rows of a tile, by the pairs an expert has on average; 0 for few pairs.  With 128
+// experts of 2048 x 192, us in tiles of 16, 64 and 128 rows: 32 tokens of 8 pairs 41,
+// 40, 51; 400 tokens 57, 67, 67; 800 tokens 86, 77, 97.  Of 2048 x 768: 512 tokens
+// 199, 161, 169; 2048 tokens -, 277, 276; 4096 tokens -, 451, 433.  32 rows win nowhere.
 static int expert_rows(int64_t tokens, const ExpertArgs& a) {
   const int64_t pairs = tokens * a.top_k, few_lds = (int64_t)a.top_k * a.ib * (kBlk + 4);
   if (pairs <= 64 && pairs <= a.experts && few_lds <= 48 * 1024 && a.kb * (kBlk + 4) <= 48 * 1024) return 0;
   const int64_t each = pairs / a.experts;
-  return each < 16 ? 16 : each < 48 ? 32 : 128;
+  return each < 16 ? 16 : each < 128 ? 64 : 128;
 }
 // Tokens of a pass: 32-bit offsets into the codes of x, and 1 GiB of y.
 static int64_t expert_pass(int64_t tokens, const ExpertArgs& a) {
@@ -477,15 +480,15 @@ static hipError_t few(const ExpertArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
+template <int FN, int FM, int WN, int WM, int STAGES>
 static void up(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
-  hipLaunchKernelGGL((k_ex_up_tiles<FN, FM, WN, WM, STAGES, EXACT>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(64 * WN * WM), 0,
+  hipLaunchKernelGGL((k_ex_up_tiles<FN, FM, WN, WM, STAGES>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(64 * WN * WM), 0,
                      stream, a);
 }
-template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
+template <int FN, int FM, int WN, int WM, int STAGES>
 static void down(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
   constexpr int BN = 16 * FN * WN;
-  hipLaunchKernelGGL((k_ex_down_tiles<FN, FM, WN, WM, STAGES, EXACT>), dim3((unsigned)((tiles * ((a.hidden + BN - 1) / BN) + 7) / 8 * 8)),
+  hipLaunchKernelGGL((k_ex_down_tiles<FN, FM, WN, WM, STAGES>), dim3((unsigned)((tiles * ((a.hidden + BN - 1) / BN) + 7) / 8 * 8)),
                      dim3(64 * WN * WM), 0, stream, a);
 }
 
@@ -513,14 +516,14 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
     else hipLaunchKernelGGL((k_ex_prepare<kF16>), prepare, dim3(kSortThreads), 0, stream, a, bm, groups, (int)each);
     if (groups > 1) hipLaunchKernelGGL(k_ex_place, dim3((unsigned)groups), dim3(kSortThreads), 0, stream, a, bm, groups, (int)each);
     if (bm == 16) {
-      up<2, 1, 8, 1, 2, true>(a, tiles, stream);
-      down<1, 1, 8, 1, 2, true>(a, tiles, stream);
-    } else if (bm == 32) {
-      up<2, 2, 8, 1, 2, true>(a, tiles, stream);
-      down<1, 2, 8, 1, 2, true>(a, tiles, stream);
+      up<2, 1, 8, 1, 2>(a, tiles, stream);
+      down<1, 1, 8, 1, 2>(a, tiles, stream);
+    } else if (bm == 64) {
+      up<4, 2, 4, 2, 3>(a, tiles, stream);
+      down<4, 2, 2, 2, 2>(a, tiles, stream);
     } else {
-      up<4, 4, 4, 2, 3, false>(a, tiles, stream);
-      down<4, 4, 4, 2, 3, false>(a, tiles, stream);
+      up<4, 4, 4, 2, 3>(a, tiles, stream);
+      down<4, 4, 4, 2, 3>(a, tiles, stream);
     }
     const dim3 sum((unsigned)((a.tokens * a.hidden / 8 + 255) / 256));
     if (dtype == kBF16) hipLaunchKernelGGL((k_ex_sum<kBF16>), sum, dim3(256), 0, stream, a);
