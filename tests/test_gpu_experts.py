@@ -236,3 +236,23 @@ def test_refusals():
            torch.zeros(2, 40, 40, dtype=torch.uint8, device=DEV).view(E4M3), torch.ones(2, 1, 1, device=DEV)]
     with pytest.raises(ValueError, match="multiples of 16"):
         fp8_experts(x[:, :40], ids, weights, *odd)
+
+
+@pytest.mark.parametrize("tokens", [1, 64, 700])
+def test_the_example_layer(tokens):
+    """Its products are those of the bf16 weights up to the rounding of both operands to e4m3: 2^-4 each at most, relative to
+    an element, 2^-4 / sqrt(3) in the mean over a code's step, and independent from element to element; the experts quantize
+    three times."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples", "fp8_moe_layer.py")
+    spec = importlib.util.spec_from_file_location("fp8_moe_layer", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    errors = module.main(tokens)
+    one = 2.0 ** -4 / 3 ** 0.5
+    for name in "qkvo":
+        assert errors[name] < 2 ** 0.5 * one, errors
+    assert errors["experts"] < 5 ** 0.5 * one, errors  # x and its two weights' halves, h and down
+    assert errors["router gradient finite"]
