@@ -214,7 +214,11 @@ struct UpTile {
   }
 };
 
-template <int FN, int FM, int WN, int WM, int STAGES>
+// EXACT: float32 sums (lrq_mma8.hpp).  The f8f6f4 instructions' sums are off by 1.5e-5
+// of their norm, which is little beside h's 4 bits, but moves one code in some 3000 to
+// its neighbour: 2e-3 of the norm of out.  bf16 results' own rounding is 1.7e-3, and
+// with it 2.6e-3; fp16's is 2e-4, so they take exact sums.
+template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
 __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
   static_assert(16 * FN * WN == 256, "128 columns of h");
   constexpr int BM = 16 * FM * WM;
@@ -225,7 +229,7 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const UpTile src{a, t, block};
   f32x4 acc[FN][FM], h[FN / 2][FM];
-  tile_sums<FN, FM, WN, WM, STAGES, true, true, false>(src, a.hidden, 0, a.kb, lds, acc);
+  tile_sums<FN, FM, WN, WM, STAGES, true, true, EXACT>(src, a.hidden, 0, a.kb, lds, acc);
 #pragma unroll
   for (int i = 0; i < FN / 2; ++i)
 #pragma unroll
@@ -481,9 +485,10 @@ static hipError_t few(const ExpertArgs& a, hipStream_t stream) {
 }
 
 template <int FN, int FM, int WN, int WM, int STAGES>
-static void up(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
-  hipLaunchKernelGGL((k_ex_up_tiles<FN, FM, WN, WM, STAGES>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(64 * WN * WM), 0,
-                     stream, a);
+static void up(const ExpertArgs& a, int dtype, int64_t tiles, hipStream_t stream) {
+  const dim3 grid((unsigned)((tiles * a.ib + 7) / 8 * 8)), block(64 * WN * WM);
+  if (dtype == kBF16) hipLaunchKernelGGL((k_ex_up_tiles<FN, FM, WN, WM, STAGES, false>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((k_ex_up_tiles<FN, FM, WN, WM, STAGES, true>), grid, block, 0, stream, a);
 }
 template <int FN, int FM, int WN, int WM, int STAGES>
 static void down(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
@@ -516,13 +521,13 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
     else hipLaunchKernelGGL((k_ex_prepare<kF16>), prepare, dim3(kSortThreads), 0, stream, a, bm, groups, (int)each);
     if (groups > 1) hipLaunchKernelGGL(k_ex_place, dim3((unsigned)groups), dim3(kSortThreads), 0, stream, a, bm, groups, (int)each);
     if (bm == 16) {
-      up<2, 1, 8, 1, 2>(a, tiles, stream);
+      up<2, 1, 8, 1, 2>(a, dtype, tiles, stream);
       down<1, 1, 8, 1, 2>(a, tiles, stream);
     } else if (bm == 64) {
-      up<4, 2, 4, 2, 3>(a, tiles, stream);
+      up<4, 2, 4, 2, 3>(a, dtype, tiles, stream);
       down<4, 2, 2, 2, 2>(a, tiles, stream);
     } else {
-      up<4, 4, 4, 2, 3>(a, tiles, stream);
+      up<4, 4, 4, 2, 3>(a, dtype, tiles, stream);
       down<4, 4, 4, 2, 3>(a, tiles, stream);
     }
     const dim3 sum((unsigned)((a.tokens * a.hidden / 8 + 255) / 256));

@@ -14,7 +14,8 @@
 //     own rounding is a hundred times that; or
 //   * EXACT: four bf16 instructions on the same codes, which are exact in bf16, as
 //     are their products; sums are float32.  Half the rate, and conversions: 48 tokens
-//     x [4096, 12288] 20.8 us instead of 16.5.  Taken for float32 results; or
+//     x [4096, 12288] 20.8 us instead of 16.5.  Taken for float32 results and for
+//     what fp16 experts quantize; or
 //   * for up to four tokens, float32 multiply-adds.
 #pragma once
 

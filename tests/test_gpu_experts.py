@@ -138,6 +138,18 @@ def test_random_weights(t, e, h, i, k):
     assert float(off) < 2.0 ** -6, float(off)
 
 
+@pytest.mark.parametrize("t,e,h,i,k", SHAPES)
+def test_fp16_hidden_values_are_those_of_float32_sums(t, e, h, i, k):
+    """The first product of fp16 experts is summed in float32: few hidden values come near enough to a border of the codes to
+    move, so the whole is as near as fp16's own rounding, 2^-11 at most an element, the second product's sums (2^-13 of a block's
+    largest product at most, 128 products that are off one way or the other: 2^-13 128^-1/2 8 of the norm, the largest being some
+    4 times the norm's share of an operand) and one code in 2^17 that moves by 2^-3 at most allow."""
+    args = make(t, e, h, i, k, torch.float16, t + h + i, whole=False)
+    want, _ = reference(*args)
+    off = (fp8_experts(*args).double() - want).norm() / want.norm()
+    assert float(off) < 2.0 ** -11 + 2.0 ** -13.5 + 2.0 ** -8.5 * 2.0 ** -3, float(off)
+
+
 @pytest.mark.parametrize("t", [2, 90, 900])
 def test_pairs_left_out(t):
     x, ids, weights, *w = make(t, 12, 256, 160, 3)
