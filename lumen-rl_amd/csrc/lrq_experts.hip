@@ -37,9 +37,11 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 // words are slow, 32768 pairs take 42 us in one work-group, 14 in four.  Pairs of an
 // expert come in any order, which no result depends on.  Ids outside 0 .. experts -
 // 1 have no place.  The other work-groups meanwhile quantize x, 64 blocks each.
-constexpr int kSortThreads = 1024, kSortAhead = 8, kSortPairs = 8192, kSortMost = 64;
+constexpr int kSortThreads = 1024, kSortAhead = 8, kSortPairs = 8192, kSortMost = 64, kBigRows = 256;
 
-__device__ __forceinline__ void place_pairs(const ExpertArgs& a, int bm, int p0, int p1, int group, int groups, int32_t* start,
+// An expert's rows are cut into tiles of kBigRows, if BIG, as long as more than bm are
+// left, and of bm; big tiles come first in the table.
+__device__ __forceinline__ void place_pairs(const ExpertArgs& a, int bm, bool big, int p0, int p1, int group, int groups, int32_t* start,
                                             int32_t (*part)[kSortThreads]) {
   const int tid = threadIdx.x;
   const uint32_t none = (uint32_t)a.experts;
@@ -50,22 +52,31 @@ __device__ __forceinline__ void place_pairs(const ExpertArgs& a, int bm, int p0,
       const int n = gld<int32_t>(a.counts + g * a.experts + tid);
       mine += n, before += g < group ? n : 0;
     }
-  const int my_tiles = (mine + bm - 1) / bm;
-  part[0][tid] = mine, part[1][tid] = my_tiles;
+  const int my_big = big ? (mine + kBigRows - 1 - bm) / kBigRows : 0;
+  const int rest = mine - my_big * kBigRows, my_tiles = rest > 0 ? (rest + bm - 1) / bm : 0;
+  part[0][tid] = mine, part[1][tid] = my_big, part[2][tid] = my_tiles;
   __syncthreads();
   for (int off = 1; off < kSortThreads; off *= 2) {
-    const int m = tid >= off ? part[0][tid - off] : 0, n = tid >= off ? part[1][tid - off] : 0;
+    int v[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) v[i] = tid >= off ? part[i][tid - off] : 0;
     __syncthreads();
-    part[0][tid] += m, part[1][tid] += n;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) part[i][tid] += v[i];
     __syncthreads();
   }
-  const int first = part[0][tid] - mine, tile = part[1][tid] - my_tiles;
+  const int first = part[0][tid] - mine, all_big = part[1][kSortThreads - 1];
+  const int tile_big = part[1][tid] - my_big, tile = all_big + part[2][tid] - my_tiles;
   if (tid < a.experts) start[tid] = first + before;
   if (group == 0) {
-    if (tid == kSortThreads - 1) gst<int32_t>(a.total, part[1][tid]);
+    if (tid == kSortThreads - 1) gst<int32_t>(a.total, all_big), gst<int32_t>(a.total + 1, part[2][tid]);
+    for (int i = 0; i < my_big; ++i) {
+      const int rows = mine - i * kBigRows < kBigRows ? mine - i * kBigRows : kBigRows;
+      a.tiles[tile_big + i] = ExpertTile{tid, first + i * kBigRows, rows, 0};
+    }
     for (int i = 0; i < my_tiles; ++i) {
-      const int rows = mine - i * bm < bm ? mine - i * bm : bm;
-      a.tiles[tile + i] = ExpertTile{tid, first + i * bm, rows, 0};
+      const int rows = rest - i * bm < bm ? rest - i * bm : bm;
+      a.tiles[tile + i] = ExpertTile{tid, first + my_big * kBigRows + i * bm, rows, 0};
     }
   }
   __syncthreads();
@@ -86,8 +97,8 @@ __device__ __forceinline__ void place_pairs(const ExpertArgs& a, int bm, int p0,
 }
 
 template <int DT>
-__global__ __launch_bounds__(kSortThreads) void k_ex_prepare(ExpertArgs a, int bm, int groups, int each) {
-  __shared__ int32_t count[kExpertsMax], part[2][kSortThreads];
+__global__ __launch_bounds__(kSortThreads) void k_ex_prepare(ExpertArgs a, int bm, bool big, int groups, int each) {
+  __shared__ int32_t count[kExpertsMax], part[3][kSortThreads];
   const int tid = threadIdx.x;
   if ((int)blockIdx.x >= groups) {
     const int64_t b = (int64_t)(blockIdx.x - groups) * (kSortThreads / 16) + (tid >> 4);
@@ -119,22 +130,25 @@ __global__ __launch_bounds__(kSortThreads) void k_ex_prepare(ExpertArgs a, int b
   }
   __syncthreads();
   if (tid < a.experts) gst<int32_t>(a.counts + group * a.experts + tid, count[tid]);  // read by this thread, or the next launch
-  if (groups == 1) place_pairs(a, bm, p0, p1, 0, 1, count, part);
+  if (groups == 1) place_pairs(a, bm, big, p0, p1, 0, 1, count, part);
 }
 
-__global__ __launch_bounds__(kSortThreads) void k_ex_place(ExpertArgs a, int bm, int groups, int each) {
-  __shared__ int32_t start[kExpertsMax], part[2][kSortThreads];
+__global__ __launch_bounds__(kSortThreads) void k_ex_place(ExpertArgs a, int bm, bool big, int groups, int each) {
+  __shared__ int32_t start[kExpertsMax], part[3][kSortThreads];
   const int pairs = (int)(a.tokens * a.top_k), p0 = (int)blockIdx.x * each;
-  place_pairs(a, bm, p0, p0 + each < pairs ? p0 + each : pairs, (int)blockIdx.x, groups, start, part);
+  place_pairs(a, bm, big, p0, p0 + each < pairs ? p0 + each : pairs, (int)blockIdx.x, groups, start, part);
 }
 
-// Work-group wg of a grid for `total` tiles by nb: each XCD (wg % 8) takes one run,
-// a tile's nb pieces after one another, so that it reads an expert's weights once.
-__device__ __forceinline__ bool expert_piece(int wg, int total, int nb, int& tile, int& n) {
-  const int all = total * nb, per = (all + 7) >> 3;
-  const int t = (wg & 7) * per + (wg >> 3);
-  if ((wg >> 3) >= per || t >= all) return false;
-  tile = t / nb, n = t % nb;
+// Work-group wg's tile and its piece of nb: each XCD (wg % 8) takes one run of the big
+// tiles and one of the others, a tile's pieces after one another, so that it reads an
+// expert's weights once, and the longest work comes first.
+__device__ __forceinline__ bool expert_piece(const ExpertArgs& a, int wg, int nb, int& tile, int& n) {
+  const int big = gld<int32_t>(a.total), rest = gld<int32_t>(a.total + 1);
+  const int per_big = (big * nb + 7) >> 3, per = (rest * nb + 7) >> 3, i = wg >> 3, x = wg & 7;
+  const bool is_big = i < per_big;
+  const int t = is_big ? x * per_big + i : x * per + i - per_big;
+  if (t >= (is_big ? big : rest) * nb || i - per_big >= per) return false;
+  tile = t / nb + (is_big ? 0 : big), n = t % nb;
   return true;
 }
 
@@ -196,8 +210,9 @@ __device__ __forceinline__ void store_hidden(const ExpertArgs& a, f32x4 (&h)[NS]
 // An expert's rows in tiles
 // ---------------------------------------------------------------------------
 // Weight rows of a tile: 16 of gate, the same 16 of up, and so on.
+template <bool SKIP>
 struct UpTile {
-  static constexpr bool kCut = false, kSkip = true;
+  static constexpr bool kCut = false, kSkip = SKIP;
   const ExpertArgs& a;
   const ExpertTile& t;
   int block;
@@ -228,16 +243,11 @@ struct UpTile {
 // of their norm, which is little beside h's 4 bits, but moves one code in some 3000 to
 // its neighbour: 2e-3 of the norm of out.  bf16 results' own rounding is 1.7e-3, and
 // with it 2.6e-3; fp16's is 2e-4, so they take exact sums.
-template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
-__global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
+template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT, bool SKIP = true>
+__device__ __forceinline__ void up_tile(const ExpertArgs& a, const ExpertTile& t, int block, uint8_t* lds) {
   static_assert(16 * FN * WN == 256, "128 columns of h");
-  constexpr int BM = 16 * FM * WM;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<FN, FM, WN, WM, STAGES>];
-  int tile, block;
-  if (!expert_piece(blockIdx.x, gld<int32_t>(a.total), a.ib, tile, block)) return;
-  const ExpertTile t = a.tiles[tile];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const UpTile src{a, t, block};
+  const UpTile<SKIP> src{a, t, block};
   f32x4 acc[FN][FM], h[FN / 2][FM];
   tile_sums<FN, FM, WN, WM, STAGES, true, true, EXACT>(src, a.hidden, 0, a.kb, lds, acc);
 #pragma unroll
@@ -246,11 +256,36 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
     for (int j = 0; j < FM; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) h[i][j][r] = silu_mul(acc[2 * i][j][r], acc[2 * i + 1][j][r]);
-  store_hidden<FN / 2, FM, WN>(a, h, t.first, wave % WM * 16 * FM, t.rows, block, wave / WM, reinterpret_cast<uint32_t*>(lds), BM);
+  store_hidden<FN / 2, FM, WN>(a, h, t.first, wave % WM * 16 * FM, t.rows, block, wave / WM, reinterpret_cast<uint32_t*>(lds),
+                               16 * FM * WM);
 }
 
+template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
+__global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<FN, FM, WN, WM, STAGES>];
+  int tile, block;
+  if (!expert_piece(a, blockIdx.x, a.ib, tile, block)) return;
+  const ExpertTile t = a.tiles[tile];
+  up_tile<FN, FM, WN, WM, STAGES, EXACT>(a, t, block, lds);
+}
+
+// Tiles of 256 and of up to 128 rows in one launch: the large ones take 49 us a round
+// over the chip, of 4096 k, and the others 31 (and cut experts' rows with less left
+// over: 32768 pairs of 128 experts in 27 % more rows than there are, 256 rows alone in
+// 55 %).
+constexpr int kMixedLds = kTileLds<4, 4, 4, 2, 3> > kTileLds<8, 4, 2, 4, 2> ? kTileLds<4, 4, 4, 2, 3> : kTileLds<8, 4, 2, 4, 2>;
+__global__ __launch_bounds__(512, 1) void k_ex_up_mixed(ExpertArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kMixedLds];
+  int tile, block;
+  if (!expert_piece(a, blockIdx.x, a.ib, tile, block)) return;
+  const ExpertTile t = a.tiles[tile];
+  if (t.rows > 128) up_tile<8, 4, 2, 4, 2, false, false>(a, t, block, lds);
+  else up_tile<4, 4, 4, 2, 3, false>(a, t, block, lds);
+}
+
+template <bool SKIP>
 struct DownTile {
-  static constexpr bool kCut = false, kSkip = true;
+  static constexpr bool kCut = false, kSkip = SKIP;
   const ExpertArgs& a;
   const ExpertTile& t;
   int n0;
@@ -272,17 +307,12 @@ struct DownTile {
   }
 };
 
-template <int FN, int FM, int WN, int WM, int STAGES>
-__global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_down_tiles(ExpertArgs a) {
-  constexpr int BN = 16 * FN * WN;
+template <int FN, int FM, int WN, int WM, int STAGES, bool SKIP = true>
+__device__ __forceinline__ void down_tile(const ExpertArgs& a, const ExpertTile& t, int block, uint8_t* lds) {
   static_assert(16 * FN <= kBlk, "one scale for a wave's rows");
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<FN, FM, WN, WM, STAGES>];
-  int tile, block;
-  if (!expert_piece(blockIdx.x, gld<int32_t>(a.total), (a.hidden + BN - 1) / BN, tile, block)) return;
-  const ExpertTile t = a.tiles[tile];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4, wn = wave / WM * 16 * FN, wm = wave % WM * 16 * FM;
-  const DownTile src{a, t, block * BN};
+  const DownTile<SKIP> src{a, t, block * 16 * FN * WN};
   f32x4 acc[FN][FM];
   tile_sums<FN, FM, WN, WM, STAGES, true, false, false>(src, a.inter, 0, a.ib, lds, acc);
 #pragma unroll
@@ -298,6 +328,24 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_down_tiles(ExpertArgs a)
         gst<f32x4>(a.y + (int64_t)pair * a.hidden + n, f32x4{acc[i][j][0] * w, acc[i][j][1] * w, acc[i][j][2] * w, acc[i][j][3] * w});
     }
   }
+}
+
+template <int FN, int FM, int WN, int WM, int STAGES>
+__global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_down_tiles(ExpertArgs a) {
+  constexpr int BN = 16 * FN * WN;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<FN, FM, WN, WM, STAGES>];
+  int tile, block;
+  if (!expert_piece(a, blockIdx.x, (a.hidden + BN - 1) / BN, tile, block)) return;
+  const ExpertTile t = a.tiles[tile];
+  down_tile<FN, FM, WN, WM, STAGES>(a, t, block, lds);
+}
+__global__ __launch_bounds__(512, 1) void k_ex_down_mixed(ExpertArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kMixedLds];
+  int tile, block;
+  if (!expert_piece(a, blockIdx.x, (a.hidden + 255) / 256, tile, block)) return;
+  const ExpertTile t = a.tiles[tile];
+  if (t.rows > 128) down_tile<8, 4, 2, 4, 2, false>(a, t, block, lds);
+  else down_tile<4, 4, 4, 2, 3>(a, t, block, lds);
 }
 
 // out[t] = the sum of the token's rows of y, in the order of its pairs.
@@ -479,7 +527,7 @@ static int64_t expert_layout(int64_t tokens, int bm, ExpertArgs& a, uint8_t* bas
   a.order = reinterpret_cast<int32_t*>(take(4 * pairs));
   a.rank = reinterpret_cast<int32_t*>(take(4 * pairs));
   a.counts = reinterpret_cast<int32_t*>(take(4 * kSortMost * (int64_t)a.experts));
-  a.total = reinterpret_cast<int32_t*>(take(4));
+  a.total = reinterpret_cast<int32_t*>(take(8));
   a.tiles = reinterpret_cast<ExpertTile*>(take((int64_t)sizeof(ExpertTile) * tile_bound(pairs, bm, a.experts)));
   a.hq = take(pairs * a.inter);
   a.hs = reinterpret_cast<float*>(take(4 * pairs * a.ib));
@@ -534,19 +582,24 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
       continue;
     }
     const int64_t pairs = a.tokens * a.top_k, tiles = tile_bound(pairs, bm, a.experts);
+    const bool big = bm == 128 && dtype == kBF16;  // conversions to bf16 take the registers of 256 rows
     int64_t each = (pairs + kSortMost - 1) / kSortMost;
     each = each < kSortPairs ? kSortPairs : each;
     const int groups = (int)((pairs + each - 1) / each);
     const dim3 prepare((unsigned)(groups + (a.tokens * a.kb + kSortThreads / 16 - 1) / (kSortThreads / 16)));
-    if (dtype == kBF16) hipLaunchKernelGGL((k_ex_prepare<kBF16>), prepare, dim3(kSortThreads), 0, stream, a, bm, groups, (int)each);
-    else hipLaunchKernelGGL((k_ex_prepare<kF16>), prepare, dim3(kSortThreads), 0, stream, a, bm, groups, (int)each);
-    if (groups > 1) hipLaunchKernelGGL(k_ex_place, dim3((unsigned)groups), dim3(kSortThreads), 0, stream, a, bm, groups, (int)each);
+    if (dtype == kBF16) hipLaunchKernelGGL((k_ex_prepare<kBF16>), prepare, dim3(kSortThreads), 0, stream, a, bm, big, groups, (int)each);
+    else hipLaunchKernelGGL((k_ex_prepare<kF16>), prepare, dim3(kSortThreads), 0, stream, a, bm, big, groups, (int)each);
+    if (groups > 1) hipLaunchKernelGGL(k_ex_place, dim3((unsigned)groups), dim3(kSortThreads), 0, stream, a, bm, big, groups, (int)each);
     if (bm == 16) {
       up<2, 1, 8, 1, 2>(a, dtype, tiles, stream);
       down<1, 1, 4, 1, 2>(a, tiles, stream);
     } else if (bm == 64) {
       up<4, 2, 4, 2, 3>(a, dtype, tiles, stream);
       down<4, 2, 2, 2, 2>(a, tiles, stream);
+    } else if (big) {
+      const unsigned pieces = (unsigned)tiles + 16;  // each kind's runs are rounded up to 8 pieces
+      hipLaunchKernelGGL(k_ex_up_mixed, dim3(pieces * (unsigned)a.ib), dim3(512), 0, stream, a);
+      hipLaunchKernelGGL(k_ex_down_mixed, dim3(pieces * (unsigned)((a.hidden + 255) / 256)), dim3(512), 0, stream, a);
     } else {
       up<4, 4, 4, 2, 3>(a, dtype, tiles, stream);
       down<4, 4, 4, 2, 3>(a, tiles, stream);
