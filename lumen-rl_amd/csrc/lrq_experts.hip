@@ -241,8 +241,12 @@ struct UpTile {
 
 // EXACT: float32 sums (lrq_mma8.hpp).  The f8f6f4 instructions' sums are off by 1.5e-5
 // of their norm, which is little beside h's 4 bits, but moves one code in some 3000 to
-// its neighbour: 2e-3 of the norm of out.  bf16 results' own rounding is 1.7e-3, and
-// with it 2.6e-3; fp16's is 2e-4, so they take exact sums.
+// its neighbour: 2e-3 of the norm of out, 3e-3 where a few activations are forty times
+// as large as the rest.  bf16 results' own rounding is 1.7e-3, so both together are
+// 1.2 to 1.6 times it for experts with 128 rows or more (2.3 times in the worst of 14
+// drawn sizes, with fewer rows); fp16's is 2e-4.  So only bf16 experts with many rows
+// take them: 4096 tokens of 8 pairs 417 us, 542 in exact sums; 512 tokens 160 and 173,
+// 200 on a quarter 51 and 54, where memory bounds both and sums are exact.
 template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT, bool SKIP = true>
 __device__ __forceinline__ void up_tile(const ExpertArgs& a, const ExpertTile& t, int block, uint8_t* lds) {
   static_assert(16 * FN * WN == 256, "128 columns of h");
@@ -260,13 +264,13 @@ __device__ __forceinline__ void up_tile(const ExpertArgs& a, const ExpertTile& t
                                16 * FM * WM);
 }
 
-template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT>
+template <int FN, int FM, int WN, int WM, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<FN, FM, WN, WM, STAGES>];
   int tile, block;
   if (!expert_piece(a, blockIdx.x, a.ib, tile, block)) return;
   const ExpertTile t = a.tiles[tile];
-  up_tile<FN, FM, WN, WM, STAGES, EXACT>(a, t, block, lds);
+  up_tile<FN, FM, WN, WM, STAGES, true>(a, t, block, lds);
 }
 
 // Tiles of 256 and of up to 128 rows in one launch: the large ones take 49 us a round
@@ -497,7 +501,8 @@ static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 // Rows of a tile, by the pairs an expert has on average; 0 for few pairs.  With 128
 // experts of 2048 x 192, us in tiles of 16, 64 and 128 rows: 32 tokens of 8 pairs 41,
 // 40, 51; 400 tokens 57, 67, 67; 800 tokens 86, 77, 97.  Of 2048 x 768: 512 tokens
-// 199, 161, 169; 2048 tokens -, 277, 276; 4096 tokens -, 451, 433.  32 rows win nowhere.
+// 199, 161, 169; 2048 tokens -, 277, 276; 4096 tokens -, 451, 433.  32 rows win
+// nowhere.  (All of them before 256 rows joined 128, and 64 rows took exact sums.)
 static int expert_rows(int64_t tokens, const ExpertArgs& a) {
   const int64_t pairs = tokens * a.top_k, few_lds = (int64_t)a.top_k * a.ib * (kBlk + 4);
   if (pairs <= 64 && pairs <= a.experts && few_lds <= 48 * 1024 && a.kb * (kBlk + 4) <= 48 * 1024) return 0;
@@ -554,10 +559,9 @@ static hipError_t few(const ExpertArgs& a, hipStream_t stream) {
 }
 
 template <int FN, int FM, int WN, int WM, int STAGES>
-static void up(const ExpertArgs& a, int dtype, int64_t tiles, hipStream_t stream) {
-  const dim3 grid((unsigned)((tiles * a.ib + 7) / 8 * 8)), block(64 * WN * WM);
-  if (dtype == kBF16) hipLaunchKernelGGL((k_ex_up_tiles<FN, FM, WN, WM, STAGES, false>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((k_ex_up_tiles<FN, FM, WN, WM, STAGES, true>), grid, block, 0, stream, a);
+static void up(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
+  hipLaunchKernelGGL((k_ex_up_tiles<FN, FM, WN, WM, STAGES>), dim3((unsigned)((tiles * a.ib + 7) / 8 * 8)), dim3(64 * WN * WM), 0,
+                     stream, a);
 }
 template <int FN, int FM, int WN, int WM, int STAGES>
 static void down(const ExpertArgs& a, int64_t tiles, hipStream_t stream) {
@@ -591,17 +595,17 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
     else hipLaunchKernelGGL((k_ex_prepare<kF16>), prepare, dim3(kSortThreads), 0, stream, a, bm, big, groups, (int)each);
     if (groups > 1) hipLaunchKernelGGL(k_ex_place, dim3((unsigned)groups), dim3(kSortThreads), 0, stream, a, bm, big, groups, (int)each);
     if (bm == 16) {
-      up<2, 1, 8, 1, 2>(a, dtype, tiles, stream);
+      up<2, 1, 8, 1, 2>(a, tiles, stream);
       down<1, 1, 4, 1, 2>(a, tiles, stream);
     } else if (bm == 64) {
-      up<4, 2, 4, 2, 3>(a, dtype, tiles, stream);
+      up<4, 2, 4, 2, 3>(a, tiles, stream);
       down<4, 2, 2, 2, 2>(a, tiles, stream);
     } else if (big) {
       const unsigned pieces = (unsigned)tiles + 16;  // each kind's runs are rounded up to 8 pieces
       hipLaunchKernelGGL(k_ex_up_mixed, dim3(pieces * (unsigned)a.ib), dim3(512), 0, stream, a);
       hipLaunchKernelGGL(k_ex_down_mixed, dim3(pieces * (unsigned)((a.hidden + 255) / 256)), dim3(512), 0, stream, a);
     } else {
-      up<4, 4, 4, 2, 3>(a, dtype, tiles, stream);
+      up<4, 4, 4, 2, 3>(a, tiles, stream);
       down<4, 4, 4, 2, 3>(a, tiles, stream);
     }
     const dim3 sum((unsigned)((a.tokens * a.hidden / 8 + 255) / 256));

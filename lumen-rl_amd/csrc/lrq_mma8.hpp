@@ -15,7 +15,7 @@
 //   * EXACT: four bf16 instructions on the same codes, which are exact in bf16, as
 //     are their products; sums are float32.  Half the rate, and conversions: 48 tokens
 //     x [4096, 12288] 20.8 us instead of 16.5.  Taken for float32 results and for
-//     what fp16 experts quantize; or
+//     most of what experts quantize again; or
 //   * for up to four tokens, float32 multiply-adds.
 #pragma once
 
@@ -53,21 +53,16 @@ template <bool HI>
 __device__ __forceinline__ uint32_t codes2_to_bf16(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
-__device__ __forceinline__ Wide32 widen(const Codes32& a) {
+__device__ __forceinline__ v4u widen_piece(const Codes32& a, int q) {
   const uint32_t w[8] = {a.lo.x, a.lo.y, a.lo.z, a.lo.w, a.hi.x, a.hi.y, a.hi.z, a.hi.w};
-  Wide32 r;
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    r.q[q] = v4u{codes2_to_bf16<false>(w[2 * q]), codes2_to_bf16<true>(w[2 * q]), codes2_to_bf16<false>(w[2 * q + 1]),
-                 codes2_to_bf16<true>(w[2 * q + 1])};
-  return r;
+  return v4u{codes2_to_bf16<false>(w[2 * q]), codes2_to_bf16<true>(w[2 * q]), codes2_to_bf16<false>(w[2 * q + 1]),
+             codes2_to_bf16<true>(w[2 * q + 1])};
 }
-__device__ __forceinline__ f32x4 mma8(const Wide32& w, const Wide32& a) {
-  f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, w.q[q]), __builtin_bit_cast(bf16x8v, a.q[q]), d, 0, 0, 0);
-  return d;
+__device__ __forceinline__ Wide32 widen(const Codes32& a) {
+  return Wide32{{widen_piece(a, 0), widen_piece(a, 1), widen_piece(a, 2), widen_piece(a, 3)}};
+}
+__device__ __forceinline__ f32x4 mma16(v4u w, v4u a, f32x4 d) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, w), __builtin_bit_cast(bf16x8v, a), d, 0, 0, 0);
 }
 template <bool EXACT>
 __device__ __forceinline__ auto operand(const Codes32& a) {
@@ -273,30 +268,57 @@ __device__ __forceinline__ void tile_sums(const Src& src, int k, int kb0, int kb
 #pragma unroll
       for (int j = 0; j < FM; ++j) s[j] *= si[0];
     }
-    f32x4 p[LAG + 1];
-    auto scale = [&](int t) {
-      const int i = t / FM, j = t % FM;
+    auto scale = [&](int i, int j, const f32x4& p) {
       const float f = EACH ? s[j] * si[EACH ? i : 0] : s[j];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(p[t % (LAG + 1)][r], f, acc[i][j][r]);
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(p[r], f, acc[i][j][r]);
     };
+    if constexpr (EXACT) {
+      // a strip's FM chains of four instructions side by side; between them the strip
+      // before is scaled and the next one's codes widened
+      f32x4 p[2][FM];
+      Wide32 wide[2];
+      wide[0] = widen(w[0]);
 #pragma unroll
-    for (int i = 0; i < FN; ++i) {
-      if (i + 1 < FN)
-        w[(i + 1) & 1] = {*reinterpret_cast<const v4u*>(cw + 2048 * (i + 1) + at0),
-                          *reinterpret_cast<const v4u*>(cw + 2048 * (i + 1) + at1)};
-      const auto wi = operand<EXACT>(w[i & 1]);
+      for (int i = 0; i < FN; ++i) {
+        if (i + 1 < FN)
+          w[(i + 1) & 1] = {*reinterpret_cast<const v4u*>(cw + 2048 * (i + 1) + at0),
+                            *reinterpret_cast<const v4u*>(cw + 2048 * (i + 1) + at1)};
 #pragma unroll
-      for (int j = 0; j < FM; ++j) {
-        const int t = i * FM + j;
-        p[t % (LAG + 1)] = mma8(wi, x[j]);
-        if (t >= LAG) scale(t - LAG);
-        between(t);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+          for (int j = 0; j < FM; ++j)
+            p[i & 1][j] = mma16(wide[i & 1].q[q], x[j].q[q], q == 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : p[i & 1][j]);
+#pragma unroll
+          for (int j = q * FM / 4; j < (q + 1) * FM / 4; ++j) {
+            if (i > 0) scale(i - 1, j, p[(i + 1) & 1][j]);
+            between(i * FM + j);
+          }
+          if (i + 1 < FN) wide[(i + 1) & 1].q[q] = widen_piece(w[(i + 1) & 1], q);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-    }
 #pragma unroll
-    for (int t = TILES - LAG; t < TILES; ++t) scale(t);
+      for (int j = 0; j < FM; ++j) scale(FN - 1, j, p[(FN - 1) & 1][j]);
+    } else {
+      f32x4 p[LAG + 1];
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        if (i + 1 < FN)
+          w[(i + 1) & 1] = {*reinterpret_cast<const v4u*>(cw + 2048 * (i + 1) + at0),
+                            *reinterpret_cast<const v4u*>(cw + 2048 * (i + 1) + at1)};
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+          const int t = i * FM + j;
+          p[t % (LAG + 1)] = mma8(w[i & 1], x[j]);
+          if (t >= LAG) scale((t - LAG) / FM, (t - LAG) % FM, p[(t - LAG) % (LAG + 1)]);
+          between(t);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+      for (int t = TILES - LAG; t < TILES; ++t) scale(t / FM, t % FM, p[t % (LAG + 1)]);
+    }
   };
 
   if constexpr (DMA) {

@@ -138,16 +138,19 @@ def test_random_weights(t, e, h, i, k):
     assert float(off) < 2.0 ** -6, float(off)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("t,e,h,i,k", SHAPES)
-def test_fp16_hidden_values_are_those_of_float32_sums(t, e, h, i, k):
-    """The first product of fp16 experts is summed in float32: few hidden values come near enough to a border of the codes to
-    move, so the whole is as near as fp16's own rounding, 2^-11 at most an element, the second product's sums (2^-13 of a block's
-    largest product at most, 128 products that are off one way or the other: 2^-13 128^-1/2 8 of the norm, the largest being some
-    4 times the norm's share of an operand) and one code in 2^17 that moves by 2^-3 at most allow."""
-    args = make(t, e, h, i, k, torch.float16, t + h + i, whole=False)
+def test_hidden_values_are_those_of_float32_sums(t, e, h, i, k, dtype):
+    """The first product is summed in float32, but for bf16 experts with 128 rows or more: few hidden values come near enough to a
+    border of the codes to move, so the whole is as near as the result's own rounding, half a step at most an element, the second
+    product's sums (2^-13 of a block's largest product at most, 128 products that are off one way or the other: 2^-13 128^-1/2 8 of
+    the norm, the largest being some 4 times the norm's share of an operand) and one code in 2^17 that moves by 2^-3 at most allow."""
+    if dtype == torch.bfloat16 and t * k >= 128 * e:
+        pytest.skip("f8f6f4 sums")
+    args = make(t, e, h, i, k, dtype, t + h + i, whole=False)
     want, _ = reference(*args)
     off = (fp8_experts(*args).double() - want).norm() / want.norm()
-    assert float(off) < 2.0 ** -11 + 2.0 ** -13.5 + 2.0 ** -8.5 * 2.0 ** -3, float(off)
+    assert float(off) < torch.finfo(dtype).eps / 2 + 2.0 ** -13.5 + 2.0 ** -8.5 * 2.0 ** -3, float(off)
 
 
 @pytest.mark.parametrize("t", [2, 90, 900])
