@@ -121,8 +121,7 @@ __device__ __forceinline__ void dma16(Rsrc r, uint32_t off, uint32_t lds) {
 // Until at most N of the wave's loads are on their way: they arrive in order.
 template <int N>
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
-constexpr uint32_t kNoRow = 0x80000000u;  // an offset past every descriptor's size
-constexpr int64_t kDmaBytes = 0x7FFFFF00ll;  // so a descriptor holds at most this
+constexpr uint32_t kNoRow = 0x80000000u;  // an offset past every descriptor's size (below 2^31)
 
 // ---------------------------------------------------------------------------
 // Quantizing activations (1 x 128 blocks, weight_quantizer.py:59-71 in float32)
@@ -191,7 +190,7 @@ __device__ __forceinline__ v2u quant8(const float* v, float& scale) {
 // blocks at a time, and of the next four.  A wave keeps the block of its tokens in
 // registers and takes the weight 16 rows at a time; a result is scaled into the
 // sums three matrix instructions after its own, which the compiler, left to
-// itself, does at once, and waits (2534 instead of 3000 TFLOP/s without any loads).
+// itself, does at once, and waits (8192^3 without any loads 374 us, 334 as here).
 //
 // DMA (rows are 4-byte aligned): codes and scales go from memory straight into
 // LDS, STAGES - 1 blocks ahead, each wave waiting only for its own part of the

@@ -33,7 +33,7 @@ def spread(scales, rows, cols, block=(128, 128)):
     return s.repeat_interleave(block[0], 0)[:rows].repeat_interleave(block[1], 1)[:, :cols]
 
 
-def check(y, x_codes, x_scales, codes, scales, bias=None):
+def check(y, x_codes, x_scales, codes, scales, bias=None, many=False):
     """|y - exact| within the result's rounding and the sums' own bound.
 
     A block sums 128 exact products in float32, K/128 blocks and 8 waves' parts follow, each step off by at most
@@ -49,7 +49,7 @@ def check(y, x_codes, x_scales, codes, scales, bias=None):
     half = torch.finfo(y.dtype).eps / 2
     least = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24, torch.float32: 2.0 ** -149}[y.dtype]
     bound = half * want.abs() * 1.01 + (128 + k // 128 + 12) * 2.0 ** -23 * size + least
-    if m > 4 and y.dtype != torch.float32:
+    if (m > 4 or many) and y.dtype != torch.float32:
         for b in range(0, k, 128):
             top = xd[:, b: b + 128].abs().amax(1)[:, None] * wd[:, b: b + 128].abs().amax(1)[None]
             bound += 128 * 2.0 ** -13 * top
@@ -156,3 +156,23 @@ def test_other_stream_and_graph():
             x.copy_(acts(m, 640, torch.bfloat16, seed))
             graph.replay()
             assert torch.equal(y, fp8_block_linear(x, codes, scales))
+
+
+@pytest.mark.parametrize("m", [3, 50, 130])
+def test_rows_far_apart_and_results_past_32_bits(m):
+    """Codes of x whose rows lie 2^22 bytes apart, at the end of them."""
+    pitch, k, n = 1 << 22, 256, 192
+    wide = torch.zeros((m, pitch), dtype=torch.uint8, device=DEV)
+    xc, xs = fp8_block_quant(acts(m, k, torch.bfloat16), (1, 128))
+    codes, scales = weight(n, k)
+    for at in (0, pitch - k):
+        wide[:, at: at + k] = xc.view(torch.uint8)
+        check(fp8_matmul(wide.view(torch.float8_e4m3fn)[:, at: at + k], xs, codes, scales), xc, xs, codes, scales)
+
+
+def test_a_result_of_more_than_2_31_cells():
+    codes, scales = weight(65536, 128)
+    x = acts(40000, 128, torch.bfloat16)
+    y = fp8_block_linear(x, codes, scales)
+    for rows in (slice(0, 3), slice(39997, 40000)):
+        check(y[rows], *fp8_block_quant(x[rows], (1, 128)), codes, scales, many=True)

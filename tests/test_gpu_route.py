@@ -311,3 +311,38 @@ def test_refusals():
         route_experts(x.double(), 4)
     with pytest.raises(ValueError):
         route_experts(torch.zeros(4, 32), 4)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(renormalize=False), dict(score="sigmoid")])
+def test_forward_and_gradient_in_a_graph(kw):
+    """Captured on leaves that no eager graph holds (torch ties a leaf's gradient to the stream of the graph that lives)."""
+    x = torch.randn(40, 64, device=DEV, requires_grad=True)
+    c = torch.randn(40, 4, device=DEV)
+
+    def step():
+        w, ids = route_experts(x, 4, **kw)
+        return w.detach(), ids, torch.autograd.grad(w, x, c)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in range(3):
+        x.data.copy_(torch.randn(40, 64, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+
+
+def test_far_rows_and_wide_pitches():
+    """Rows past 2^31 elements of the logits' storage."""
+    big = torch.zeros((1 << 31) + 4096, dtype=torch.bfloat16, device=DEV)
+    view = big.as_strided((5, 64), (1 << 29, 1))
+    view.copy_(torch.randn(5, 64, device=DEV))
+    check(view, 6)
+    check_grad(view, 6, renormalize=False)
