@@ -177,7 +177,8 @@ int lrq_fp8_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t 
  *   lrq_fp8_matmul: x as e4m3 codes [rows, k] (row stride ld >= k) with float32
  *     scales [rows, ceil(k/128)], dense; out of out_dtype (bf16, fp16 or fp32).
  *     `workspace`: lrq_fp8_matmul_workspace(rows, k, n) bytes, 0 but for some tens
- *     of tokens, whose K is split.
+ *     of tokens, whose K is split, and for many of a k that 4 does not divide, which
+ *     are copied to aligned rows.
  *   lrq_fp8_block_linear: x of x_dtype (bf16, fp16 or fp32; row stride ld),
  *     quantized as lrq_fp8_block_quant does with 1 x 128 blocks (float32
  *     arithmetic); out of x's type.  `workspace`: likewise of

@@ -282,10 +282,14 @@ struct MatmulArgs {
 };
 // true: launch_matmul takes values of x, whatever n is
 bool matmul_quantizes(int64_t m, int64_t k);
-// device memory that launch_matmul needs for the sums of parts of K
-int64_t matmul_workspace(int64_t m, int64_t n, int64_t k);
+// true: the operands are copied to rows of 16 ceil(k / 16) bytes first
+bool matmul_repacks(int64_t m, int64_t n, int64_t k);
+// device memory that launch_matmul needs for such rows, or for the sums of parts of K
+// x_packed: x has such rows already (launch_matmul_quant writes them)
+int64_t matmul_workspace(int64_t m, int64_t n, int64_t k, bool x_packed);
+hipError_t launch_matmul_quant(const void* x, int dtype, int64_t ld, int64_t m, int64_t k, uint8_t* codes, float* scales, hipStream_t stream);
 // x_dtype: the type of x's values, or -1: codes
-hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, void* workspace, hipStream_t stream);
+hipError_t launch_matmul(MatmulArgs a, int x_dtype, void* workspace, bool x_packed, hipStream_t stream);
 
 // Routing to experts (lrq_route.hip).
 constexpr int kRouteExpertsMax = 512, kRouteGroupsMax = 16;  // one lane of 16 looks through a group

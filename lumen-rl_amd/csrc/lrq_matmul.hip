@@ -214,6 +214,32 @@ __global__ __launch_bounds__(256) void k_mm8_join(MatmulArgs a, const float* par
 }
 
 // ---------------------------------------------------------------------------
+// Rows at a pitch of 16 bytes
+// ---------------------------------------------------------------------------
+// Codes whose rows are not 4-byte aligned go through registers, at less than half the
+// speed; with many tokens they are copied to rows of kp = 16 ceil(k / 16) first, zeros
+// at the end, and x is quantized into such rows.  8192 tokens x [12288, 4097] 448 us,
+// 1000 as they are; 4096 x [4096, 4097] 89 and 192; 1024 tokens 51 and 54, 512 36 and 31.
+__global__ __launch_bounds__(256) void k_mm8_pad(const uint8_t* from, int64_t ld, uint32_t pieces, int k, uint32_t per, uint8_t* to) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= pieces) return;
+  const uint32_t row = i / per, at = 16 * (i - row * per);
+  *(LRQ_GLOBAL v4u*)(to + 16 * (int64_t)i) = load_codes_cut((GlobalCodes)from + row * ld, (int)at, k);
+}
+template <int DT>
+__global__ __launch_bounds__(256) void k_mm8_quant(const void* x, int64_t ld, uint32_t blocks, int k, uint32_t kb, int64_t kp, uint8_t* codes,
+                                                   float* scales) {
+  const uint32_t b = blockIdx.x * 16u + (threadIdx.x >> 4);
+  if (b >= blocks) return;  // 16 lanes at once
+  const uint32_t row = b / kb, at = (b - row * kb) * kBlk + 8 * (threadIdx.x & 15);
+  float v[8], s;
+  load_acts<DT>(static_cast<const uint8_t*>(x) + row * ld * (DT == kF32 ? 4 : 2), (int)at, k, v);
+  const v2u q = quant8(v, s);
+  if (at < kp) *(LRQ_GLOBAL v2u*)(codes + row * kp + at) = q;
+  if ((threadIdx.x & 15) == 0) gst<float>(scales + b, s);
+}
+
+// ---------------------------------------------------------------------------
 // Which kernel
 // ---------------------------------------------------------------------------
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -280,9 +306,30 @@ static int64_t split_parts(int64_t m, int64_t n, int64_t k) {
   if (parts < 2) return 1;
   return ceil_div(kb, ceil_div(kb, parts));  // none of them empty
 }
-int64_t matmul_workspace(int64_t m, int64_t n, int64_t k) {
+static int64_t pitch16(int64_t k) { return (k + 15) / 16 * 16; }
+static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+bool matmul_repacks(int64_t m, int64_t n, int64_t k) {
+  return k % 4 != 0 && m >= 1536 && n * pitch16(k) < int64_t(1) << 31 && m * pitch16(k) < int64_t(1) << 35;
+}
+int64_t matmul_workspace(int64_t m, int64_t n, int64_t k, bool x_packed) {
+  if (matmul_repacks(m, n, k)) return up256(n * pitch16(k)) + (x_packed ? 0 : up256(m * pitch16(k)));
   const int64_t parts = split_parts(m, n, k);
   return parts > 1 ? 4 * parts * m * n : 0;
+}
+
+hipError_t launch_matmul_quant(const void* x, int dtype, int64_t ld, int64_t m, int64_t k, uint8_t* codes, float* scales, hipStream_t stream) {
+  const int64_t kb = ceil_div(k, kBlk);
+  const dim3 grid((unsigned)ceil_div(m * kb, 16)), block(256);
+  const uint32_t blocks = (uint32_t)(m * kb);
+  if (dtype == kBF16) hipLaunchKernelGGL((k_mm8_quant<kBF16>), grid, block, 0, stream, x, ld, blocks, (int)k, (uint32_t)kb, pitch16(k), codes, scales);
+  else if (dtype == kF16) hipLaunchKernelGGL((k_mm8_quant<kF16>), grid, block, 0, stream, x, ld, blocks, (int)k, (uint32_t)kb, pitch16(k), codes, scales);
+  else hipLaunchKernelGGL((k_mm8_quant<kF32>), grid, block, 0, stream, x, ld, blocks, (int)k, (uint32_t)kb, pitch16(k), codes, scales);
+  return hipGetLastError();
+}
+
+static void pad_rows(const uint8_t* from, int64_t ld, int64_t rows, int64_t k, uint8_t* to, hipStream_t stream) {
+  const int64_t per = pitch16(k) / 16, pieces = rows * per;
+  hipLaunchKernelGGL(k_mm8_pad, dim3((unsigned)ceil_div(pieces, 256)), dim3(256), 0, stream, from, ld, (uint32_t)pieces, (int)k, (uint32_t)per, to);
 }
 
 template <bool EXACT>
@@ -299,7 +346,18 @@ static void launch_few(const MatmulArgs& a, float* sums, hipStream_t stream) {
   }
 }
 
-hipError_t launch_matmul(const MatmulArgs& a, int x_dtype, void* workspace, hipStream_t stream) {
+hipError_t launch_matmul(MatmulArgs a, int x_dtype, void* workspace, bool x_packed, hipStream_t stream) {
+  if (matmul_repacks(a.m, a.n, a.k)) {
+    const int64_t kp = pitch16(a.k);
+    uint8_t* const w = static_cast<uint8_t*>(workspace);
+    pad_rows(a.w, a.k, a.n, a.k, w, stream);
+    if (!x_packed) {
+      uint8_t* const x = w + up256(a.n * kp);
+      pad_rows(static_cast<const uint8_t*>(a.x), a.ldx, a.m, a.k, x, stream);
+      a.x = x, a.ldx = kp;
+    }
+    a.w = w, a.k = kp;
+  }
   if (a.m <= kDots) {
     if (x_dtype == kBF16) launch_dots<kBF16>(a, stream);
     else if (x_dtype == kF16) launch_dots<kF16>(a, stream);

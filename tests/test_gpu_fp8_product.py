@@ -60,7 +60,8 @@ def check(y, x_codes, x_scales, codes, scales, bias=None, many=False):
 # tokens of each kernel (up to four: dot products; up to 64: K in parts; tiles of four sizes), weights cut in every way
 SHAPES = [(1, 1, 1), (2, 77, 2100), (4, 4100, 515), (1, 5000, 1032), (1, 4096, 4096), (3, 200, 130), (16, 130, 1104), (16, 64, 12288), (17, 129, 384), (33, 1, 1100), (64, 300, 272),
           (65, 127, 15), (65, 128, 128), (100, 130, 144), (777, 1500, 1100), (2000, 2040, 1040), (1999, 2041, 1041), (4100, 3850, 272),
-          (130, 190, 1036), (300, 129, 1164), (2000, 2040, 1048), (4100, 3850, 268), (70, 65, 4), (400, 12300, 128), (1100, 6200, 144)]
+          (130, 190, 1036), (300, 129, 1164), (2000, 2040, 1048), (4100, 3850, 268), (70, 65, 4), (400, 12300, 128), (1100, 6200, 144),
+          (1536, 300, 1041), (1600, 513, 129), (1536, 4000, 7), (1540, 130, 2046)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

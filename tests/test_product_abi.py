@@ -44,6 +44,14 @@ def test_parts_of_k_are_some_and_never_empty(rows, k, n, parts):
         assert (parts - 1) * -(-blocks // parts) < blocks
 
 
+def test_rows_that_are_not_aligned_are_copied_for_many_tokens():
+    up = lambda v: -(-v // 256) * 256  # noqa: E731
+    assert L().lrq_fp8_matmul_workspace(1536, 1041, 300) == up(300 * 1056) + up(1536 * 1056)
+    assert L().lrq_fp8_matmul_workspace(1535, 1041, 300) == 0 and L().lrq_fp8_matmul_workspace(1536, 1044, 300) == 0
+    assert L().lrq_fp8_block_linear_workspace(1536, 1041, 300) == up(1536 * 1056) + up(1536 * 9 * 4) + up(300 * 1056)
+    assert L().lrq_fp8_matmul_workspace(1536, (1 << 22) - 1, 1 << 12) == 0  # more than 2 GiB of weight: as they are
+
+
 def test_fp8_block_linear():
     def call(x=FAKE, dt=0, rows=70, k=300, ld=300, codes=FAKE, scales=FAKE, n=64, bias=None, bdt=0, out=FAKE, ws=FAKE, wb=1 << 30):
         return L().lrq_fp8_block_linear(x, dt, rows, k, ld, codes, scales, n, bias, bdt, out, ws, wb, None)
