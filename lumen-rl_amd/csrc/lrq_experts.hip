@@ -34,71 +34,68 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 // count their pairs of each expert, which gives each pair its rank.  The experts'
 // runs, the tiles of `bm` rows and each pair's place follow at once if there is one
 // such work-group, in a launch of their own if there are more: atomics on a few
-// words are slow, 32768 pairs take 42 us in one work-group, 14 in four.  Pairs of an
+// words are slow, 32768 pairs take 42 us in one work-group, 19 in two launches of four.  Pairs of an
 // expert come in any order, which no result depends on.  Ids outside 0 .. experts -
 // 1 have no place.  The other work-groups meanwhile quantize x, 64 blocks each.
 constexpr int kSortThreads = 1024, kSortAhead = 8, kSortPairs = 8192, kSortMost = 64, kBigRows = 256;
 
-// An expert's rows are cut into tiles of kBigRows, if BIG, as long as more than bm are
-// left, and of bm; big tiles come first in the table.
-__device__ __forceinline__ void place_pairs(const ExpertArgs& a, int bm, bool big, int p0, int p1, int group, int groups, int32_t* start,
-                                            int32_t (*part)[kSortThreads]) {
-  const int tid = threadIdx.x;
-  const uint32_t none = (uint32_t)a.experts;
-  // one expert a thread: sums of rows and of tiles before it
-  int mine = 0, before = 0;
-  if (tid < a.experts)
-    for (int g = 0; g < groups; ++g) {
-      const int n = gld<int32_t>(a.counts + g * a.experts + tid);
-      mine += n, before += g < group ? n : 0;
+// Sums over the threads before this one, and over all.
+template <int N>
+__device__ __forceinline__ void sums_before(int (&v)[N], int (&all)[N], int32_t (*part)[kSortThreads / 64]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int own[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) own[i] = v[i];
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int o = __shfl_up(v[i], off, 64);
+      v[i] += lane >= off ? o : 0;
     }
+  if (lane == 63)
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i][wave] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    all[i] = 0, v[i] -= own[i];
+#pragma unroll
+    for (int w = 0; w < kSortThreads / 64; ++w) {
+      const int o = part[i][w];
+      all[i] += o, v[i] += w < wave ? o : 0;
+    }
+  }
+}
+
+// From the pairs of each expert, one expert a thread: their runs' starts, where
+// `before` of them belong to other work-groups, and (by the first) the tiles.  An
+// expert's rows are cut into tiles of kBigRows, if `big`, as long as more than bm are
+// left, and of bm; big tiles come first in the table.
+__device__ __forceinline__ void lay_out(const ExpertArgs& a, int bm, bool big, int mine, int before, bool writes, int32_t* start,
+                                        int32_t (*part)[kSortThreads / 64]) {
+  const int tid = threadIdx.x;
   const int my_big = big ? (mine + kBigRows - 1 - bm) / kBigRows : 0;
   const int rest = mine - my_big * kBigRows, my_tiles = rest > 0 ? (rest + bm - 1) / bm : 0;
-  part[0][tid] = mine, part[1][tid] = my_big, part[2][tid] = my_tiles;
-  __syncthreads();
-  for (int off = 1; off < kSortThreads; off *= 2) {
-    int v[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) v[i] = tid >= off ? part[i][tid - off] : 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 3; ++i) part[i][tid] += v[i];
-    __syncthreads();
-  }
-  const int first = part[0][tid] - mine, all_big = part[1][kSortThreads - 1];
-  const int tile_big = part[1][tid] - my_big, tile = all_big + part[2][tid] - my_tiles;
+  int v[3] = {mine, my_big, my_tiles}, all[3];
+  sums_before(v, all, part);
+  const int first = v[0], tile_big = v[1], tile = all[1] + v[2];
   if (tid < a.experts) start[tid] = first + before;
-  if (group == 0) {
-    if (tid == kSortThreads - 1) gst<int32_t>(a.total, all_big), gst<int32_t>(a.total + 1, part[2][tid]);
-    for (int i = 0; i < my_big; ++i) {
-      const int rows = mine - i * kBigRows < kBigRows ? mine - i * kBigRows : kBigRows;
-      a.tiles[tile_big + i] = ExpertTile{tid, first + i * kBigRows, rows, 0};
-    }
-    for (int i = 0; i < my_tiles; ++i) {
-      const int rows = rest - i * bm < bm ? rest - i * bm : bm;
-      a.tiles[tile + i] = ExpertTile{tid, first + my_big * kBigRows + i * bm, rows, 0};
-    }
+  if (!writes) return;
+  if (tid == 0) gst<int32_t>(a.total, all[1]), gst<int32_t>(a.total + 1, all[2]);
+  for (int i = 0; i < my_big; ++i) {
+    const int rows = mine - i * kBigRows < kBigRows ? mine - i * kBigRows : kBigRows;
+    a.tiles[tile_big + i] = ExpertTile{tid, first + i * kBigRows, rows, 0};
   }
-  __syncthreads();
-  for (int p = p0 + tid; p < p1; p += kSortThreads * kSortAhead) {
-    uint32_t e[kSortAhead];
-    int rank[kSortAhead];
-#pragma unroll
-    for (int i = 0; i < kSortAhead; ++i) {
-      const bool has = p + kSortThreads * i < p1;
-      const int q = has ? p + kSortThreads * i : p;
-      e[i] = (uint32_t)gld<int32_t>(a.ids + q), rank[i] = gld<int32_t>(a.rank + q);
-      if (!has) e[i] = none;
-    }
-#pragma unroll
-    for (int i = 0; i < kSortAhead; ++i)
-      if (e[i] < none) gst<int32_t>(a.order + start[e[i]] + rank[i], p + kSortThreads * i);
+  for (int i = 0; i < my_tiles; ++i) {
+    const int rows = rest - i * bm < bm ? rest - i * bm : bm;
+    a.tiles[tile + i] = ExpertTile{tid, first + my_big * kBigRows + i * bm, rows, 0};
   }
 }
 
 template <int DT>
 __global__ __launch_bounds__(kSortThreads) void k_ex_prepare(ExpertArgs a, int bm, bool big, int groups, int each) {
-  __shared__ int32_t count[kExpertsMax], part[3][kSortThreads];
+  __shared__ int32_t count[kExpertsMax], part[3][kSortThreads / 64];
   const int tid = threadIdx.x;
   if ((int)blockIdx.x >= groups) {
     const int64_t b = (int64_t)(blockIdx.x - groups) * (kSortThreads / 16) + (tid >> 4);
@@ -117,27 +114,62 @@ __global__ __launch_bounds__(kSortThreads) void k_ex_prepare(ExpertArgs a, int b
   const uint32_t none = (uint32_t)a.experts;
   for (int e = tid; e < a.experts; e += kSortThreads) count[e] = 0;
   __syncthreads();
+  uint32_t e[kSortAhead];
+  int rank[kSortAhead];
   for (int p = p0 + tid; p < p1; p += kSortThreads * kSortAhead) {
-    uint32_t e[kSortAhead];
-    int rank[kSortAhead];
 #pragma unroll
     for (int i = 0; i < kSortAhead; ++i) e[i] = p + kSortThreads * i < p1 ? (uint32_t)gld<int32_t>(a.ids + p + kSortThreads * i) : none;
 #pragma unroll
     for (int i = 0; i < kSortAhead; ++i) rank[i] = e[i] < none ? atomicAdd(&count[e[i]], 1) : 0;
+    if (groups > 1)
 #pragma unroll
-    for (int i = 0; i < kSortAhead; ++i)
-      if (e[i] < none) gst<int32_t>(a.rank + p + kSortThreads * i, rank[i]);
+      for (int i = 0; i < kSortAhead; ++i)
+        if (e[i] < none) gst<int32_t>(a.rank + p + kSortThreads * i, rank[i]);
   }
   __syncthreads();
-  if (tid < a.experts) gst<int32_t>(a.counts + group * a.experts + tid, count[tid]);  // read by this thread, or the next launch
-  if (groups == 1) place_pairs(a, bm, big, p0, p1, 0, 1, count, part);
+  const int mine = tid < a.experts ? count[tid] : 0;
+  if (groups > 1) {
+    if (tid < a.experts) gst<int32_t>(a.counts + group * a.experts + tid, mine);
+    return;
+  }
+  // one group has kSortPairs at most: the thread's pairs are still in its registers
+  lay_out(a, bm, big, mine, 0, true, count, part);
+  __syncthreads();
+  if (p0 + tid >= p1) return;
+#pragma unroll
+  for (int i = 0; i < kSortAhead; ++i)
+    if (e[i] < none) gst<int32_t>(a.order + count[e[i]] + rank[i], p0 + tid + kSortThreads * i);
 }
 
 __global__ __launch_bounds__(kSortThreads) void k_ex_place(ExpertArgs a, int bm, bool big, int groups, int each) {
-  __shared__ int32_t start[kExpertsMax], part[3][kSortThreads];
-  const int pairs = (int)(a.tokens * a.top_k), p0 = (int)blockIdx.x * each;
-  place_pairs(a, bm, big, p0, p0 + each < pairs ? p0 + each : pairs, (int)blockIdx.x, groups, start, part);
+  __shared__ int32_t start[kExpertsMax], part[3][kSortThreads / 64];
+  const int tid = threadIdx.x, group = blockIdx.x, pairs = (int)(a.tokens * a.top_k);
+  const int p0 = group * each, p1 = p0 + each < pairs ? p0 + each : pairs;
+  const uint32_t none = (uint32_t)a.experts;
+  int mine = 0, before = 0;
+  if (tid < a.experts)
+    for (int g = 0; g < groups; ++g) {
+      const int n = gld<int32_t>(a.counts + g * a.experts + tid);
+      mine += n, before += g < group ? n : 0;
+    }
+  lay_out(a, bm, big, mine, before, group == 0, start, part);
+  __syncthreads();
+  for (int p = p0 + tid; p < p1; p += kSortThreads * kSortAhead) {
+    uint32_t e[kSortAhead];
+    int rank[kSortAhead];
+#pragma unroll
+    for (int i = 0; i < kSortAhead; ++i) {
+      const bool has = p + kSortThreads * i < p1;
+      const int q = has ? p + kSortThreads * i : p;
+      e[i] = (uint32_t)gld<int32_t>(a.ids + q), rank[i] = gld<int32_t>(a.rank + q);
+      if (!has) e[i] = none;
+    }
+#pragma unroll
+    for (int i = 0; i < kSortAhead; ++i)
+      if (e[i] < none) gst<int32_t>(a.order + start[e[i]] + rank[i], p + kSortThreads * i);
+  }
 }
+static_assert(kSortPairs == kSortThreads * kSortAhead, "");
 
 // Work-group wg's tile and its piece of nb: each XCD (wg % 8) takes one run of the big
 // tiles and one of the others, a tile's pieces after one another, so that it reads an
