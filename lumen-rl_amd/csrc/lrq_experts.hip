@@ -399,7 +399,7 @@ __global__ __launch_bounds__(256) void k_ex_sum(ExpertArgs a) {
     for (int j = 0; j < AHEAD; ++j) {
       const int64_t pair = t * a.top_k + (j0 + j < a.top_k ? j0 + j : 0);
       has[j] = j0 + j < a.top_k && (uint32_t)gld<int32_t>(a.ids + pair) < (uint32_t)a.experts;
-      lo[j] = gld<f32x4>(a.y + pair * a.hidden + n), hi[j] = gld<f32x4>(a.y + pair * a.hidden + n + 4);
+      lo[j] = gld_nt<f32x4>(a.y + pair * a.hidden + n), hi[j] = gld_nt<f32x4>(a.y + pair * a.hidden + n + 4);
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)

@@ -102,8 +102,8 @@ __device__ __forceinline__ void lds_barrier8() {
 // ---------------------------------------------------------------------------
 // Memory straight into LDS
 // ---------------------------------------------------------------------------
-// 16 bytes a lane, at `off` from the descriptor's base (zeros if off + 16 passes
-// its size), to 16 l + `lds`.  In assembly because the compiler, which cannot
+// 16 bytes a lane, at `off` from the descriptor's base (words past its
+// size read as zeros), to 16 l + `lds`.  In assembly because the compiler, which cannot
 // tell a tile's stages apart, waits for every such load before the
 // next read of LDS; dma_wait() is the wait, before the barrier that hands the
 // stage over.  The instruction has no register output.
