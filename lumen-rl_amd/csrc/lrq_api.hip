@@ -716,9 +716,9 @@ int check_workspace(const char* what, const void* workspace, int64_t bytes, int6
   return 0;
 }
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
-// the codes of x, at a pitch of 16 bytes where the product wants that, and their scales
-int64_t code_bytes(int64_t rows, int64_t k, int64_t n) { return up256(rows * (lrq::matmul_repacks(rows, n, k) ? (k + 15) / 16 * 16 : k)); }
-int64_t quantized_bytes(int64_t rows, int64_t k, int64_t n) { return code_bytes(rows, k, n) + up256(4 * rows * ((k + 127) / 128)); }
+// the codes of x in rows of 16 ceil(k / 16) bytes, and their scales
+int64_t code_bytes(int64_t rows, int64_t k) { return up256(rows * ((k + 15) / 16 * 16)); }
+int64_t quantized_bytes(int64_t rows, int64_t k) { return code_bytes(rows, k) + up256(4 * rows * ((k + 127) / 128)); }
 }  // namespace
 
 int lrq_fp8_matmul(const uint8_t* x_codes, const float* x_scales, int64_t rows, int64_t k, int64_t ld,
@@ -738,7 +738,7 @@ int64_t lrq_fp8_block_linear_workspace(int64_t rows, int64_t k, int64_t n) {
   if (rows <= 0 || k <= 0 || n <= 0 || rows > lrq::kMmRowsMax || k > lrq::kMmPitchMax || n > lrq::kMmOutMax ||
       lrq::matmul_quantizes(rows, k))
     return 0;
-  return quantized_bytes(rows, k, n) + lrq::matmul_workspace(rows, n, k, true);
+  return quantized_bytes(rows, k) + lrq::matmul_workspace(rows, n, k, true);
 }
 
 int lrq_fp8_block_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t ld, const uint8_t* codes,
@@ -748,20 +748,16 @@ int lrq_fp8_block_linear(const void* x, int x_dtype, int64_t rows, int64_t k, in
   const int rc = check_matmul("fp8_block_linear", rows, k, ld, codes, scales, n, bias, bias_dtype, x, out, x_dtype);
   if (rc) return rc > 0 ? 0 : rc;
   if (!aligned(x, (uintptr_t)esize(x_dtype))) return fail(LRQ_ERR_ALIGN, "fp8_block_linear: x must be element-aligned");
+  if (rows * ((k + 127) / 128) >= int64_t(1) << 31) return fail(LRQ_ERR_ARG, "fp8_block_linear: x has 2^31 blocks or more");
   if (int w = check_workspace("fp8_block_linear", workspace, workspace_bytes, lrq_fp8_block_linear_workspace(rows, k, n))) return w;
   lrq::MatmulArgs a{x, nullptr, codes, scales, bias, out, ld, rows, n, k, (k + 127) / 128, bias_dtype, x_dtype};
   if (lrq::matmul_quantizes(rows, k))
     return check_hip(lrq::launch_matmul(a, x_dtype, nullptr, false, (hipStream_t)stream), "kernel launch");
   uint8_t* const x_codes = static_cast<uint8_t*>(workspace);
-  float* const x_scales = reinterpret_cast<float*>(x_codes + code_bytes(rows, k, n));
-  const bool packed = lrq::matmul_repacks(rows, n, k);
-  if (packed) {
-    if (int q = check_hip(lrq::launch_matmul_quant(x, x_dtype, ld, rows, k, x_codes, x_scales, (hipStream_t)stream), "kernel launch")) return q;
-  } else if (int q = lrq_fp8_block_quant(x, x_dtype, 1, rows, k, ld, rows * ld, 1, 128, x_codes, x_scales, 0, stream)) {
-    return q;
-  }
-  a.x = x_codes, a.sx = x_scales, a.ldx = packed ? (k + 15) / 16 * 16 : k;
-  return check_hip(lrq::launch_matmul(a, -1, x_codes + quantized_bytes(rows, k, n), packed, (hipStream_t)stream), "kernel launch");
+  float* const x_scales = reinterpret_cast<float*>(x_codes + code_bytes(rows, k));
+  if (int q = check_hip(lrq::launch_matmul_quant(x, x_dtype, ld, rows, k, x_codes, x_scales, (hipStream_t)stream), "kernel launch")) return q;
+  a.x = x_codes, a.sx = x_scales, a.ldx = (k + 15) / 16 * 16;
+  return check_hip(lrq::launch_matmul(a, -1, x_codes + quantized_bytes(rows, k), true, (hipStream_t)stream), "kernel launch");
 }
 
 namespace {

@@ -218,7 +218,9 @@ __global__ __launch_bounds__(256) void k_mm8_join(MatmulArgs a, const float* par
 // ---------------------------------------------------------------------------
 // Codes whose rows are not 4-byte aligned go through registers, at less than half the
 // speed; with many tokens they are copied to rows of kp = 16 ceil(k / 16) first, zeros
-// at the end, and x is quantized into such rows.  8192 tokens x [12288, 4097] 448 us,
+// at the end.  fp8_block_linear quantizes x into such rows anyway, through the caches,
+// where the product finds them: 48 tokens x [4096, 12288] 18.5 us, 19.7 by k_row, which
+// stores past them; 1024 x [4096, 4096] 31 and 35, 8192 tokens 151 and 155.  8192 tokens x [12288, 4097] 448 us,
 // 1000 as they are; 4096 x [4096, 4097] 89 and 192; 1024 tokens 51 and 54, 512 36 and 31.
 __global__ __launch_bounds__(256) void k_mm8_pad(const uint8_t* from, int64_t ld, uint32_t pieces, int k, uint32_t per, uint8_t* to) {
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;

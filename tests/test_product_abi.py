@@ -57,13 +57,13 @@ def test_fp8_block_linear():
         return L().lrq_fp8_block_linear(x, dt, rows, k, ld, codes, scales, n, bias, bdt, out, ws, wb, None)
 
     assert call(rows=0) == 0 and call(n=0) == 0
-    for bad in ({"dt": 3}, {"k": 0}, {"ld": 299}, {"rows": -1}, {"x": None}, {"codes": None}, {"scales": None}, {"out": None},
+    for bad in ({"dt": 3}, {"k": 0}, {"ld": 299}, {"rows": 1 << 27, "n": 1, "k": 2048, "ld": 2048}, {"rows": -1}, {"x": None}, {"codes": None}, {"scales": None}, {"out": None},
                 {"bias": FAKE, "bdt": -1}, {"ld": (1 << 22) + 1}):
         assert call(**bad) == _lib.ERR_ARG, bad
     for bad in ({"x": ODD}, {"scales": ODD}, {"out": ODD}, {"bias": ODD}, {"ws": OFF4}):
         assert call(**bad) == _lib.ERR_ALIGN, bad
     need = L().lrq_fp8_block_linear_workspace(70, 300, 64)
-    assert need == 70 * 300 // 256 * 256 + 256 + (70 * 3 * 4 + 255) // 256 * 256
+    assert need == (70 * 304 + 255) // 256 * 256 + (70 * 3 * 4 + 255) // 256 * 256
     assert call(ws=None) == _lib.ERR_CAPACITY and call(wb=need - 1) == _lib.ERR_CAPACITY
     assert L().lrq_fp8_block_linear_workspace(4, 4096, 64) == 0 and L().lrq_fp8_block_linear_workspace(4, 1 << 20, 64) > 0
 
