@@ -15,17 +15,23 @@
 
 namespace lrq {
 
-// g / (1 + exp(-g)) u within some 2^-22: exp(-g) = 2^hi (1 + lo ln 2), where hi + lo is
-// -g log2(e) to twice float32's bits, by the hardware's 2^x and 1 / x (1 ulp each).
-// 4096 tokens of 8 pairs x 768: 450 us in all, 460 by expf and division.
+// g / (1 + exp(-g)) u within some (|g| + 8) 2^-23 of itself for normal g above -131, and
+// 0 below, where silu is under 1e-55.  With t = exp(-|g|), which cannot overflow, it is
+// g u / (1 + t), times t for g < 0.  t = 2^hi (1 + lo ln 2), where hi + lo is -|g|
+// log2(e) to twice float32's bits, by the hardware's 2^x and 1 / x (1 ulp each).  2^x
+// has no results below 2^-126: below g = -70 it makes 2^64 t (hi + 64 is exact), and the
+// factor goes out last, so that h leaves float32's range no sooner than it has to.
 __device__ __forceinline__ float silu_mul(float g, float u) {
   constexpr float kHi = 1.44269502162933349609375f, kLo = 1.92596299112661746887e-8f;  // log2(e)
-  const float hi = -g * kHi;
-  const float lo = __builtin_fabsf(hi) < 256.0f ? __builtin_fmaf(-g, kLo, __builtin_fmaf(-g, kHi, -hi)) : 0.0f;
-  const float e = __builtin_amdgcn_exp2f(hi);
-  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e, lo * 0.693147182f, e)) * u;
+  const float a = fminf(__builtin_fabsf(g), 1000.0f), hi = -a * kHi;  // (exp(-1000) is 0; of a NaN, n stays one)
+  const float lo = __builtin_fmaf(-a, kLo, __builtin_fmaf(-a, kHi, -hi));
+  const bool deep = g < -70.0f;
+  const float unit = deep ? 0x1p-64f : 1.0f;
+  const float e = __builtin_amdgcn_exp2f(deep ? hi + 64.0f : hi);
+  const float t = __builtin_fmaf(e, lo * 0.693147182f, e);
+  const float n = g < 0.0f ? g * t : g;
+  return n * __builtin_amdgcn_rcpf(__builtin_fmaf(t, unit, 1.0f)) * u * unit;
 }
-
 
 // ---------------------------------------------------------------------------
 // Tokens quantized, pairs sorted by expert

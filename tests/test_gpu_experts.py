@@ -283,3 +283,45 @@ def test_the_example_layer(tokens):
         assert errors[name] < 2 ** 0.5 * one, errors
     assert errors["experts"] < 5 ** 0.5 * one, errors  # x and its two weights' halves, h and down
     assert errors["router gradient finite"]
+
+
+GATES = [-1e4, -200.0, -178.0, -177.0, -150.0, -104.0, -103.0, -100.0, -95.0, -90.0, -89.0, -88.75, -88.5, -88.0, -87.5, -87.0, -80.0,
+         -70.5, -69.5, -30.0, -1.0, -0.015625, 0.0, 0.015625, 1.0, 30.0, 70.0, 88.0, 89.0, 100.0, 178.0, 1e4]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("spread_gates", [False, True])
+@pytest.mark.parametrize("repeats,e", [(1, 64), (1, 8), (20, 8), (66, 8)])  # few pairs; rows of 16, 64, 128 and up
+def test_gates_of_any_size(repeats, e, spread_gates, dtype):
+    """Gates far beyond exp's range, alone in their 1x128 block or beside others of either sign.
+
+    x is constant in a row, gate's codes are powers of two and up's are 1, so that block sums are exact in every kernel; down is
+    the identity, so a result is its weight (a power of two that brings the row's largest near 1) times the hidden value's image.
+    gate and up carry two roundings each, which silu stretches by 1 + |g| at most, h eight more; its image is within 2^-4 of it, or
+    half the smallest step, 2^-10 scales."""
+    gen = torch.Generator(device=DEV).manual_seed(repeats)
+    n = 128
+    x = torch.tensor(GATES, device=DEV).repeat(repeats)[:, None].expand(-1, n).to(dtype).contiguous()
+    t = x.shape[0]
+    codes = torch.ones(e, 2 * n, n, device=DEV)
+    if spread_gates:
+        codes[:, :n] = (torch.pow(2.0, torch.randint(-2, 2, (e, n, 1), generator=gen, device=DEV).float())
+                        * (1 - 2 * torch.randint(0, 2, (e, n, 1), generator=gen, device=DEV)))
+    gu, gus = codes.to(E4M3), torch.full((e, 2, 1), 2.0 ** -7, device=DEV)
+    dn, dns = torch.eye(n, device=DEV).repeat(e, 1, 1).to(E4M3), torch.ones(e, 1, 1, device=DEV)
+    # popular and unpopular experts: tiles of every height
+    ids = torch.randint(0, e, (t, 2), generator=gen, device=DEV).amin(1, keepdim=True).to(torch.int32)
+    xc, xs = fp8_block_quant(x, (1, 128))
+    xd = xc.double() * xs.double()
+    gate = (xd[:, None] * codes.double()[ids[:, 0].long(), :n]).sum(-1) * 2.0 ** -7
+    up = xd.sum(-1, keepdim=True) * 2.0 ** -7
+    h = gate * torch.sigmoid(gate) * up
+    top = h.abs().amax(1, keepdim=True)
+    weights = torch.pow(2.0, -torch.floor(torch.log2(top.clamp_min(2.0 ** -120)))).float()
+    y = fp8_experts(x, ids, weights, gu, gus, dn, dns)
+    assert bool(y.isfinite().all())
+    want = h * weights.double()
+    scale = (top / 448).clamp_min(2.0 ** -126)
+    off_h = (2.0 ** -4 + (gate.abs() + 12) * 2.0 ** -22) * h.abs() + 2.0 ** -9.9 * scale
+    slack = off_h * weights.double()
+    check(y, want, slack)
