@@ -14,8 +14,9 @@
 // it; so a round of the choice is one maximum, and ties go to the lowest index.  A
 // token with two neighbours in that order (or two groups) nearer to each other than
 // the words can tell is chosen again by its whole wave in float64, unless the two
-// have the same logit and bias and so are a tie.  With random biases that happens to
-// some 0.1 % of tokens, and costs the rest nothing.
+// have the same logit and bias and so are a tie.  A tie of the last one chosen with the
+// next counts only if all open experts behind them that are as near are their equals.
+// With random biases a token in a thousand is chosen again, and costs the rest nothing.
 //
 // Moves little: 2 or 4 bytes an expert.  What it spends is instructions, 1.5 an
 // expert for each of the top_k rounds and some 15 before; so 16 lanes take a token,
@@ -413,15 +414,28 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
   }
   wave_fence8();
   if constexpr (KEYS != kKeysLogit16) {
-    for (int i = l; i + 1 < rounds; i += 16) {
-      const float here = (float)keys[i] * (kWindow / kMost), next = (float)keys[i + 1] * (kWindow / kMost);
-      if (KEYS == kKeysPick ? here - next > tol * (1.0f + fabsf(low + here)) : keys[i] != keys[i + 1]) continue;
-      const uint32_t e = ids[i], f = ids[i + 1];
-      const float xe = load_as_f32(logits, DT, e < (uint32_t)a.experts ? e : 0), xf = load_as_f32(logits, DT, f < (uint32_t)a.experts ? f : 0);
-      bool tie = xe == xf;
-      if (KEYS == kKeysPick)
-        tie &= gld<float>(a.bias + (e < (uint32_t)a.experts ? e : 0)) == gld<float>(a.bias + (f < (uint32_t)a.experts ? f : 0));
-      unsure |= !tie;
+    // words that cannot tell which is higher, `next` being no higher than `word`
+    auto near = [&](uint32_t word, uint32_t next) {
+      const float here = (float)word * (kWindow / kMost), there = (float)next * (kWindow / kMost);
+      return KEYS == kKeysPick ? !(here - there > tol * (1.0f + fabsf(low + here))) : word == next;
+    };
+    auto expert = [&](int i) { return ids[i] < (uint32_t)a.experts ? ids[i] : 0u; };
+    auto bias_of = [&](uint32_t e) { return KEYS == kKeysPick ? gld<float>(a.bias + e) : 0.0f; };
+    auto equal = [&](uint32_t e, uint32_t f) {
+      return load_as_f32(logits, DT, e) == load_as_f32(logits, DT, f) && bias_of(e) == bias_of(f);
+    };
+    for (int i = l; i + 1 < rounds; i += 16)
+      if (near(keys[i], keys[i + 1])) unsure |= !equal(expert(i), expert(i + 1));
+    // A tie of the last one and the next does not settle the choice: any open expert
+    // behind them, as near to them but not their equal, may be higher.
+    const int k = a.top_k - 1;
+    if (rounds > a.top_k && near(keys[k], keys[k + 1]) && equal(expert(k), expert(k + 1))) {
+      const uint32_t e = expert(k), last_key = keys[k] << BITS | (kIndex - ids[k]);
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (key[s] != 0 && key[s] < last_key && near(keys[k], key[s] >> BITS)) {
+          if (!equal(e, (uint32_t)expert_of(s, l))) unsure = true;
+        }
     }
   }
   uint64_t again = __ballot(unsure);

@@ -346,3 +346,51 @@ def test_far_rows_and_wide_pitches():
     view.copy_(torch.randn(5, 64, device=DEV))
     check(view, 6)
     check_grad(view, 6, renormalize=False)
+
+
+INF = float("inf")
+
+
+@pytest.mark.parametrize("logits,bias,top_k", [
+    ([0.0, -100.0, -100.0, -90.0], None, 2), ([0.0, -1e4, -1e4, -70.0], None, 2), ([0.0, -INF, -INF, -70.0], None, 2),
+    ([1e-4, 1e-4, 1.01e-4], None, 1), ([0.0] * 100 + [1e-6] + [0.0] * 27, None, 1), ([5.0, -INF, -INF, -INF, -200.0, -INF], None, 2),
+    ([3e38, 1.0, 1.0, 2.0], None, 2), ([0.0] * 300 + [2e-7, 1e-7], None, 2),
+    ([0.0, 0.0, 0.0, 0.0], [0.0, -10.0, -10.0, -9.0], 2), ([0.0] * 4, [0.0, -INF, -INF, -9.0], 2),
+    ([1.0] * 6, [0.5, 0.5, 0.5, 0.5 + 2.0 ** -24, 0.5, 0.5 + 2.0 ** -24], 1), ([20.0, 1.0, 1.0, 1.5, 1.0], [0.0] * 5, 2),
+    ([20.0, -1.0, -1.0, -1.0, 2.0, 2.0, 2.5], [0.0] * 7, 3)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_a_tie_at_the_border_does_not_settle_it(logits, bias, top_k, score):
+    """The last chosen and the next one are equal, and a higher one stands behind them, too near to them, or too far below the
+    highest, for the words that order experts to tell."""
+    x = torch.tensor([logits] * 3, device=DEV)
+    kw = {"score": score}
+    if bias is not None:
+        kw["bias"] = torch.tensor(bias, device=DEV)
+    _, ids = route_experts(x, top_k, **kw)
+    assert torch.equal(ids.long().cpu(), choose(x, top_k, **kw))
+
+
+@pytest.mark.parametrize("groups", [1, 4])
+@pytest.mark.parametrize("kw", [dict(), dict(bias=0.0), dict(bias=1.0), dict(bias=30.0), dict(score="sigmoid", bias=0.0),
+                                dict(score="sigmoid", bias=1.0), dict(score="sigmoid", bias=30.0)], ids=str)
+@pytest.mark.parametrize("e,top_k", [(64, 2), (128, 8), (256, 8), (512, 20)])
+def test_ties_among_near_neighbours(e, top_k, kw, groups):
+    """Few distinct logits and biases, near one another or far below the highest, in every order: bf16 logits of a small spread
+    widened to float32, confident experts above a crowd, masks of -inf and of large negative values with live experts below them."""
+    g = torch.Generator(device=DEV).manual_seed(e + top_k)
+
+    def some(values):
+        return torch.tensor(values, device=DEV)[torch.randint(0, len(values), (64, e), generator=g, device=DEV)]
+
+    rows = [(torch.randn(64, e, generator=g, device=DEV) * 1e-4).bfloat16().float(), some([1.0, 1.0 + 2.0 ** -22, 1.0 + 2.0 ** -23]),
+            (torch.randn(64, e, generator=g, device=DEV) * 2).bfloat16().float(), some([-100.0, -90.0, -70.0, -1e4, -INF]),
+            some([-100.0, -90.0, -70.0]), some([0.0, 1e-7, 2e-7, -1e-7])]
+    for r in (2, 3, 4):  # confident experts above
+        rows[r][torch.arange(64, device=DEV), torch.randint(0, e, (64,), generator=g, device=DEV)] = 20.0
+    x = torch.cat(rows)
+    kw = dict(kw, groups=groups, top_groups=(groups + 1) // 2, group_top=2 if groups > 1 else 1)
+    if "bias" in kw:
+        few = torch.tensor([0.0, -1.0, -1.0 + 2.0 ** -23, -0.5], device=DEV)
+        kw["bias"] = few[torch.randint(0, 4, (e,), generator=g, device=DEV)] * kw["bias"]
+    _, ids = route_experts(x, top_k, **kw)
+    assert torch.equal(ids.long().cpu(), choose(x, top_k, **kw))
