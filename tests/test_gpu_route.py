@@ -394,3 +394,26 @@ def test_ties_among_near_neighbours(e, top_k, kw, groups):
         kw["bias"] = few[torch.randint(0, 4, (e,), generator=g, device=DEV)] * kw["bias"]
     _, ids = route_experts(x, top_k, **kw)
     assert torch.equal(ids.long().cpu(), choose(x, top_k, **kw))
+
+
+@pytest.mark.parametrize("kw", [k for k in CONFIGS if k.get("groups", 1) > 1], ids=str)
+@pytest.mark.parametrize("zero", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_groups_with_nan_infinite_and_masked_logits(dtype, zero, kw):
+    """Every row against the definition: a group with a NaN is the highest, groups that are masked as a whole rank by their biases."""
+    x, kw = inputs(12, 64, dtype, kw, 9)
+    if zero and kw.get("bias") is not None:
+        kw["bias"] = torch.zeros(64, device=DEV)
+    x[0, 5] = float("nan")
+    x[1] = -INF
+    x[2, 3:] = -INF
+    x[3, 40] = INF
+    x[4, [1, 63]] = float("nan")
+    x[5] = torch.finfo(dtype).min
+    x[6] = torch.finfo(dtype).max
+    x[7, 10:] = torch.finfo(dtype).min
+    x[8, [3, 17, 33]] = INF
+    x[9, 8:56] = -INF
+    x[10, ::2] = torch.finfo(dtype).min
+    _, ids = route_experts(x, 4, **kw)
+    assert torch.equal(ids.long().cpu(), choose(x, 4, **kw))
