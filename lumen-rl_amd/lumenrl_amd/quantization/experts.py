@@ -18,6 +18,7 @@ from lumenrl_amd import _lib
 from lumenrl_amd.quantization.fp8_product import check_tiles
 from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _dense, _on, _stream
 
+_PITCH_MAX = 1 << 31  # rows further apart are copied
 _SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
 
 
@@ -29,7 +30,7 @@ def _rows(x: Tensor) -> tuple[Tensor, int, int]:
     rows = x.numel() // e
     x = x.reshape(rows, e)
     ld = x.stride(0) if rows > 1 else e
-    if (e > 1 and x.stride(1) != 1) or ld < e:
+    if (e > 1 and x.stride(1) != 1) or not e <= ld <= _PITCH_MAX:
         return x.contiguous(), rows, e
     return x, rows, ld
 

@@ -20,6 +20,7 @@ from lumenrl_amd import _lib
 from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _dense, _on, _prod, _stream
 
 _BLOCK = 128
+_PITCH_MAX = 1 << 22  # of the kernels' 32-bit offsets; rows further apart are copied
 
 
 def check_tiles(what: str, codes: Tensor, scales: Tensor, device: torch.device) -> tuple[Tensor, Tensor]:
@@ -84,7 +85,7 @@ def fp8_matmul(x_codes: Tensor, x_scales: Tensor, codes: Tensor, scales: Tensor,
     if k == 0:
         return _empty_sum(m, n, bias, out_dtype, dev)
     ld = x_codes.stride(0) if m > 1 else k
-    if (k > 1 and x_codes.stride(1) != 1) or ld < k:
+    if (k > 1 and x_codes.stride(1) != 1) or not k <= ld <= _PITCH_MAX:
         x_codes, ld = x_codes.contiguous(), k
     if not x_scales.is_contiguous():
         x_scales = x_scales.contiguous()
@@ -128,7 +129,7 @@ def fp8_block_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Te
         rows = x.numel() // k
         x = x.reshape(rows, k)
         ld = x.stride(0) if rows > 1 else k
-        if (k > 1 and x.stride(1) != 1) or ld < k:
+        if (k > 1 and x.stride(1) != 1) or not k <= ld <= _PITCH_MAX:
             x, ld = x.contiguous(), k
     out = _dense((*shape[:-1], n), x.dtype, dev)
     need = _linear_workspace(rows, k, n)

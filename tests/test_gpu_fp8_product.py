@@ -177,3 +177,16 @@ def test_a_result_of_more_than_2_31_cells():
     y = fp8_block_linear(x, codes, scales)
     for rows in (slice(0, 3), slice(39997, 40000)):
         check(y[rows], *fp8_block_quant(x[rows], (1, 128)), codes, scales, many=True)
+
+
+@pytest.mark.parametrize("m", [3, 8, 100])
+def test_rows_further_apart_than_offsets_reach(m):
+    """The last token of each sequence, [m, 2048, 4096][:, -1]: a pitch of 2^23."""
+    codes, scales = weight(150, 4096)
+    hidden = torch.zeros(m, 2048, 4096, dtype=torch.bfloat16, device=DEV)
+    hidden[:, -1] = acts(m, 4096, torch.bfloat16)
+    xc, xs = fp8_block_quant(hidden[:, -1].contiguous(), (1, 128))
+    check(fp8_block_linear(hidden[:, -1], codes, scales), xc, xs, codes, scales)
+    wide = torch.zeros(m, (1 << 22) + 16, dtype=torch.uint8, device=DEV)
+    wide[:, 16: 16 + 4096] = xc.view(torch.uint8)
+    check(fp8_matmul(wide.view(torch.float8_e4m3fn)[:, 16: 16 + 4096], xs, codes, scales), xc, xs, codes, scales)

@@ -417,3 +417,11 @@ def test_groups_with_nan_infinite_and_masked_logits(dtype, zero, kw):
     x[10, ::2] = torch.finfo(dtype).min
     _, ids = route_experts(x, 4, **kw)
     assert torch.equal(ids.long().cpu(), choose(x, 4, **kw))
+
+
+def test_rows_more_than_2_31_elements_apart():
+    big = torch.zeros(2 * ((1 << 31) + 8) + 64, dtype=torch.bfloat16, device=DEV)
+    view = big.as_strided((3, 64), ((1 << 31) + 8, 1))
+    view.copy_(torch.randn(3, 64, device=DEV))
+    check(view, 6)
+    check_grad(view, 6)
