@@ -13,9 +13,10 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from lumenrl_amd import _lib
-from lumenrl_amd.quantization.fp8_product import check_tiles
+from lumenrl_amd.quantization.fp8_product import NoGradient, check_tiles
 from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _dense, _on, _stream
 
 _PITCH_MAX = 1 << 31  # rows further apart are copied
@@ -83,6 +84,10 @@ class _Route(torch.autograd.Function):
             return _Route._recorded(ctx, grad, ctx.saved_tensors[0])
         return _route_grad(ctx, grad)
 
+    @staticmethod
+    def jvp(ctx, *_):
+        raise RuntimeError("route_experts has no forward-mode derivative")
+
 
 def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Optional[Tensor] = None, groups: int = 1,
                   top_groups: int = 1, group_top: int = 1, renormalize: bool = True, scale: float = 1.0
@@ -120,7 +125,7 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: O
         raise ValueError(f"route_experts: group_top must be 1 or 2, got {group_top}")
     cfg = (top_k, _SCORES[score], groups, top_groups, group_top, int(renormalize), scale)
     ids = _dense((*logits.shape[:-1], top_k), torch.int32, logits.device)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if (logits.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0:
         return _Route.apply(logits, ids, bias, cfg), ids
     return _route(logits, ids, bias, cfg), ids
 
@@ -140,7 +145,8 @@ def fp8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_u
     e4m3 codes with float32 scales of 128x128 tiles, as ``quantize_fp8_blockwise``
     writes them; H and I are multiples of 16.  x and the hidden values are quantized
     in 1x128 blocks; all else is float32.  A pair whose id is not one of 0 .. E - 1
-    is left out (a shard's other experts, say).
+    is left out (a shard's other experts, say).  No gradient: a backward pass through
+    the result raises.
     """
     what = "fp8_experts"
     _check_input(x, what)
@@ -167,6 +173,17 @@ def fp8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_u
     if not 1 <= e <= 1024 or not 1 <= k <= 64 or h % 16 or i % 16 or not h or not i or 2 * h * i >= 1 << 31:
         raise ValueError(f"{what}: {e} experts (at most 1024), top {k} (at most 64), H {h} and I {i} (multiples of 16, "
                          "2 H I below 2^31)")
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
+            x.requires_grad or weights.requires_grad or gate_up.requires_grad or gate_up_scales.requires_grad
+            or down.requires_grad or down_scales.requires_grad):
+        return NoGradient.apply(what, _experts, x, ids, weights, gate_up, gate_up_scales, down, down_scales)
+    return _experts(x, ids, weights, gate_up, gate_up_scales, down, down_scales)
+
+
+def _experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_up_scales: Tensor, down: Tensor,
+             down_scales: Tensor) -> Tensor:
+    dev, lead, k = x.device, x.shape[:-1], ids.shape[-1]
+    e, h, i = down.shape
     if ids.dtype == torch.int64:
         ids = ids.clamp(-1, e).to(torch.int32)
     x, rows, ld = _rows(x)

@@ -15,6 +15,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from lumenrl_amd import _lib
 from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _dense, _on, _prod, _stream
@@ -40,17 +41,31 @@ def check_tiles(what: str, codes: Tensor, scales: Tensor, device: torch.device) 
             scales if scales.is_contiguous() else scales.contiguous())
 
 
-def _check_bias(what: str, bias: Optional[Tensor], n: int, device: torch.device) -> tuple[Optional[int], int]:
-    if bias is None:
-        return None, 0
+def _check_bias(what: str, bias: Tensor, n: int, device: torch.device) -> None:
     if bias.shape != (n,) or bias.dtype not in _IN_DTYPES or bias.device != device or not bias.is_contiguous():
         raise ValueError(f"{what}: bias must be a contiguous [{n}] bf16, fp16 or fp32 tensor on {device}")
-    return bias.data_ptr(), _IN_DTYPES[bias.dtype]
 
 
 def _empty_sum(rows: int, n: int, bias: Optional[Tensor], dtype: torch.dtype, device: torch.device) -> Tensor:
     y = torch.zeros((rows, n), dtype=torch.float32, device=device)
     return (y if bias is None else y + bias).to(dtype)
+
+
+class NoGradient(torch.autograd.Function):
+    """An operator without a gradient, on inputs that want one: whoever asks for it is told, and not left without."""
+
+    @staticmethod
+    def forward(ctx, what, call, *args):
+        ctx.what = what
+        return call(*args)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.what} has no gradient")
+
+    @staticmethod
+    def jvp(ctx, *_):
+        raise RuntimeError(f"{ctx.what} has no forward-mode derivative")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -66,6 +81,7 @@ def fp8_matmul(x_codes: Tensor, x_scales: Tensor, codes: Tensor, scales: Tensor,
     ``fp8_block_quant(x, (1, 128))`` gives them; rows may be a view's),
     ``codes`` [N, K] with float32 ``scales`` [ceil(N/128), ceil(K/128)] ->
     [M, N] of ``out_dtype`` (bfloat16, float16 or float32), sums in float32.
+    No gradient: a backward pass through the result raises.
     """
     if not isinstance(x_codes, Tensor) or not x_codes.is_cuda:
         raise ValueError("fp8_matmul: expected codes on a HIP device")
@@ -81,9 +97,22 @@ def fp8_matmul(x_codes: Tensor, x_scales: Tensor, codes: Tensor, scales: Tensor,
     n = codes.shape[0]
     if x_scales.shape != (m, -(-k // _BLOCK)) or x_scales.device != dev:
         raise ValueError(f"fp8_matmul: x's scales must be {(m, -(-k // _BLOCK))} on {dev}, got {tuple(x_scales.shape)}")
-    bias_ptr, bias_dtype = _check_bias("fp8_matmul", bias, n, dev)
+    if bias is not None:
+        _check_bias("fp8_matmul", bias, n, dev)
     if k == 0:
         return _empty_sum(m, n, bias, out_dtype, dev)
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
+            x_codes.requires_grad or x_scales.requires_grad or codes.requires_grad or scales.requires_grad
+            or (bias is not None and bias.requires_grad)):
+        return NoGradient.apply("fp8_matmul", _matmul, x_codes, x_scales, codes, scales, bias, out_dtype)
+    return _matmul(x_codes, x_scales, codes, scales, bias, out_dtype)
+
+
+def _matmul(x_codes: Tensor, x_scales: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Tensor],
+            out_dtype: torch.dtype) -> Tensor:
+    dev = x_codes.device
+    (m, k), n = x_codes.shape, codes.shape[0]
+    bias_ptr, bias_dtype = (None, 0) if bias is None else (bias.data_ptr(), _IN_DTYPES[bias.dtype])
     ld = x_codes.stride(0) if m > 1 else k
     if (k > 1 and x_codes.stride(1) != 1) or not k <= ld <= _PITCH_MAX:
         x_codes, ld = x_codes.contiguous(), k
@@ -111,7 +140,8 @@ def fp8_block_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Te
     (as ``fp8_block_quant(x, (1, 128))``) and multiplied with ``codes`` [N, K]
     and float32 ``scales`` [ceil(N/128), ceil(K/128)] -> [..., N] in x's dtype.
 
-    Up to four tokens take one launch, more take two or three.
+    Up to four tokens take one launch, more take two or three.  No gradient: a backward
+    pass through the result raises.
     """
     _check_input(x, "fp8_block_linear")
     dev = x.device
@@ -120,9 +150,20 @@ def fp8_block_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Te
     if not shape or codes.dim() != 2 or shape[-1] != codes.shape[1]:
         raise ValueError(f"fp8_block_linear: x {tuple(shape)} and codes {tuple(codes.shape)} do not fit")
     n, k = codes.shape
-    bias_ptr, bias_dtype = (None, 0) if bias is None else _check_bias("fp8_block_linear", bias, n, dev)
+    if bias is not None:
+        _check_bias("fp8_block_linear", bias, n, dev)
     if k == 0:
         return _empty_sum(_prod(shape[:-1]), n, bias, x.dtype, dev).view(*shape[:-1], n)
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
+            x.requires_grad or codes.requires_grad or scales.requires_grad or (bias is not None and bias.requires_grad)):
+        return NoGradient.apply("fp8_block_linear", _block_linear, x, codes, scales, bias)
+    return _block_linear(x, codes, scales, bias)
+
+
+def _block_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Tensor]) -> Tensor:
+    dev, shape = x.device, x.shape
+    n, k = codes.shape
+    bias_ptr, bias_dtype = (None, 0) if bias is None else (bias.data_ptr(), _IN_DTYPES[bias.dtype])
     if x.is_contiguous():
         rows, ld = x.numel() // k, k
     else:

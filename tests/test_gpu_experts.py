@@ -4,8 +4,9 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from lumenrl_amd.quantization import fp8_block_quant, fp8_experts, quantize_fp8_blockwise, route_experts
+from lumenrl_amd.quantization import fp8_block_linear, fp8_block_quant, fp8_experts, fp8_matmul, quantize_fp8_blockwise, route_experts
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -325,3 +326,48 @@ def test_gates_of_any_size(repeats, e, spread_gates, dtype):
     off_h = (2.0 ** -4 + (gate.abs() + 12) * 2.0 ** -22) * h.abs() + 2.0 ** -9.9 * scale
     slack = off_h * weights.double()
     check(y, want, slack)
+
+
+def operators():
+    """name -> (call of the operator on its first wants-a-gradient input, that input)."""
+    x, ids, weights, *w = make(6, 4, 128, 64, 2)
+    codes, scales = w[2][0], w[3][0]
+    xc, xs = fp8_block_quant(x[:, :64].contiguous(), (1, 128))
+    bias = torch.randn(128, device=DEV)
+    return {"fp8_experts x": (lambda v: fp8_experts(v, ids, weights, *w), x),
+            "fp8_experts weights": (lambda v: fp8_experts(x, ids, v, *w), weights),
+            "fp8_block_linear x": (lambda v: fp8_block_linear(v, codes, scales), x[:, :64]),
+            "fp8_block_linear bias": (lambda v: fp8_block_linear(x[:, :64], codes, scales, v), bias),
+            "fp8_matmul x_scales": (lambda v: fp8_matmul(xc, v, codes, scales), xs),
+            "fp8_matmul bias": (lambda v: fp8_matmul(xc, xs, codes, scales, v), bias)}
+
+
+@pytest.mark.parametrize("name", ["fp8_experts x", "fp8_experts weights", "fp8_block_linear x", "fp8_block_linear bias",
+                                  "fp8_matmul x_scales", "fp8_matmul bias"])
+def test_a_gradient_that_is_not_there_is_not_lost_silently(name):
+    call, value = operators()[name]
+    want = call(value)
+    assert not want.requires_grad
+    leaf = value.detach().clone().requires_grad_()
+    with torch.no_grad():
+        assert not call(leaf).requires_grad
+    y = call(leaf)
+    assert torch.equal(y, want) and y.requires_grad
+    with pytest.raises(RuntimeError, match=f"{name.split()[0]} has no gradient"):
+        y.float().sum().backward()
+    with forward_ad.dual_level():
+        assert torch.equal(call(value), want)
+        with pytest.raises(RuntimeError, match=f"{name.split()[0]} has no forward-mode derivative"):
+            call(forward_ad.make_dual(value, torch.ones_like(value)))
+
+
+def test_the_routers_gradient_does_not_end_in_the_experts():
+    x, _, _, *w = make(6, 4, 128, 64, 2)
+    logits = torch.randn(6, 4, device=DEV, requires_grad=True)
+    weights, ids = route_experts(logits, 2)
+    with pytest.raises(RuntimeError, match="fp8_experts has no gradient"):
+        fp8_experts(x, ids, weights, *w).float().sum().backward()
+    with forward_ad.dual_level():
+        assert torch.equal(route_experts(logits.detach(), 2)[0], weights)
+        with pytest.raises(RuntimeError, match="route_experts has no forward-mode derivative"):
+            route_experts(forward_ad.make_dual(logits.detach(), torch.ones_like(logits)), 2)
