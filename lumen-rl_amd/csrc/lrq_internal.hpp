@@ -312,7 +312,7 @@ struct RouteArgs {
   float scale;
 };
 // out null: the choice and its weights; otherwise the logits' gradient, from ids and the weights' gradient
-hipError_t launch_route(const RouteArgs& a, int dtype, const float* grad, void* out, hipStream_t stream);
+hipError_t launch_route(RouteArgs a, int dtype, const float* grad, void* out, hipStream_t stream);
 
 // The experts' MLPs on FP8 weights (lrq_experts.hip).
 constexpr int kExpertsMax = 1024;  // one thread of the sort each

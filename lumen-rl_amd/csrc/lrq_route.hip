@@ -584,11 +584,22 @@ static void launch_of(const RouteArgs& a, const float* grad, void* out, hipStrea
   else if (a.experts <= 256) launch<DT, 2>(a, grad, out, stream);
   else launch<DT, 4>(a, grad, out, stream);
 }
-hipError_t launch_route(const RouteArgs& a, int dtype, const float* grad, void* out, hipStream_t stream) {
-  if (dtype == kBF16) launch_of<kBF16>(a, grad, out, stream);
-  else if (dtype == kF16) launch_of<kF16>(a, grad, out, stream);
-  else launch_of<kF32>(a, grad, out, stream);
-  return hipGetLastError();
+// A launch has fewer than 2^32 threads, 16 of them a token.
+constexpr int64_t kRouteLaunch = int64_t(1) << 27;
+hipError_t launch_route(RouteArgs a, int dtype, const float* grad, void* out, hipStream_t stream) {
+  const int64_t es = dtype == kF32 ? 4 : 2, tokens = a.tokens;
+  for (int64_t t0 = 0; t0 < tokens; t0 += kRouteLaunch) {
+    a.tokens = tokens - t0 < kRouteLaunch ? tokens - t0 : kRouteLaunch;
+    if (dtype == kBF16) launch_of<kBF16>(a, grad, out, stream);
+    else if (dtype == kF16) launch_of<kF16>(a, grad, out, stream);
+    else launch_of<kF32>(a, grad, out, stream);
+    if (hipError_t e = hipGetLastError()) return e;
+    a.logits = static_cast<const uint8_t*>(a.logits) + kRouteLaunch * a.ld * es;
+    a.ids += kRouteLaunch * a.top_k;
+    if (out != nullptr) grad += kRouteLaunch * a.top_k, out = static_cast<uint8_t*>(out) + kRouteLaunch * a.experts * es;
+    else a.weights += kRouteLaunch * a.top_k;
+  }
+  return hipSuccess;
 }
 
 }  // namespace lrq

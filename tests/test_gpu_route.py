@@ -425,3 +425,18 @@ def test_rows_more_than_2_31_elements_apart():
     view.copy_(torch.randn(3, 64, device=DEV))
     check(view, 6)
     check_grad(view, 6)
+
+
+def test_more_tokens_than_a_launch_takes():
+    """2^28 + 5 tokens of two experts; with 16 threads a token more than the 2^32 of one launch."""
+    t = (1 << 28) + 5
+    x = torch.randn(t, 2, dtype=torch.bfloat16, device=DEV).requires_grad_()
+    w, ids = route_experts(x, 1, score="sigmoid", renormalize=False)
+    second = x.detach()[:, 1] > x.detach()[:, 0]
+    assert torch.equal(ids[:, 0] == 1, second)
+    (g,) = torch.autograd.grad(w, x, torch.ones(1, 1, device=DEV).expand(t, 1))
+    for rows in (slice(0, 1000), slice((1 << 27) - 500, (1 << 27) + 500), slice((1 << 28) - 995, None)):
+        s = torch.sigmoid(x.detach()[rows].double()).gather(1, ids[rows].long())
+        assert bool(((w[rows].double() - s).abs() <= 40 * 2.0 ** -24 * s).all())
+        want = torch.zeros(len(s), 2, dtype=torch.float64, device=DEV).scatter(1, ids[rows].long(), s * (1 - s))
+        assert bool(((g[rows].double() - want).abs() <= 1.01 * 2.0 ** -8 * want).all())
