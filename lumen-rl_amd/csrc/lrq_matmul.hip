@@ -320,13 +320,21 @@ int64_t matmul_workspace(int64_t m, int64_t n, int64_t k, bool x_packed) {
 }
 
 hipError_t launch_matmul_quant(const void* x, int dtype, int64_t ld, int64_t m, int64_t k, uint8_t* codes, float* scales, hipStream_t stream) {
-  const int64_t kb = ceil_div(k, kBlk);
-  const dim3 grid((unsigned)ceil_div(m * kb, 16)), block(256);
-  const uint32_t blocks = (uint32_t)(m * kb);
-  if (dtype == kBF16) hipLaunchKernelGGL((k_mm8_quant<kBF16>), grid, block, 0, stream, x, ld, blocks, (int)k, (uint32_t)kb, pitch16(k), codes, scales);
-  else if (dtype == kF16) hipLaunchKernelGGL((k_mm8_quant<kF16>), grid, block, 0, stream, x, ld, blocks, (int)k, (uint32_t)kb, pitch16(k), codes, scales);
-  else hipLaunchKernelGGL((k_mm8_quant<kF32>), grid, block, 0, stream, x, ld, blocks, (int)k, (uint32_t)kb, pitch16(k), codes, scales);
-  return hipGetLastError();
+  const int64_t kb = ceil_div(k, kBlk), kp = pitch16(k), es = dtype == kF32 ? 4 : 2;
+  const int64_t most = (int64_t(1) << 27) / kb;  // rows of a launch, which has fewer than 2^32 threads, 16 of them a block
+  for (int64_t r0 = 0; r0 < m; r0 += most) {
+    const int64_t rows = m - r0 < most ? m - r0 : most;
+    const dim3 grid((unsigned)ceil_div(rows * kb, 16)), block(256);
+    const uint32_t blocks = (uint32_t)(rows * kb);
+    const void* const from = static_cast<const uint8_t*>(x) + r0 * ld * es;
+    uint8_t* const to = codes + r0 * kp;
+    float* const s = scales + r0 * kb;
+    if (dtype == kBF16) hipLaunchKernelGGL((k_mm8_quant<kBF16>), grid, block, 0, stream, from, ld, blocks, (int)k, (uint32_t)kb, kp, to, s);
+    else if (dtype == kF16) hipLaunchKernelGGL((k_mm8_quant<kF16>), grid, block, 0, stream, from, ld, blocks, (int)k, (uint32_t)kb, kp, to, s);
+    else hipLaunchKernelGGL((k_mm8_quant<kF32>), grid, block, 0, stream, from, ld, blocks, (int)k, (uint32_t)kb, kp, to, s);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 static void pad_rows(const uint8_t* from, int64_t ld, int64_t rows, int64_t k, uint8_t* to, hipStream_t stream) {

@@ -190,3 +190,12 @@ def test_rows_further_apart_than_offsets_reach(m):
     wide = torch.zeros(m, (1 << 22) + 16, dtype=torch.uint8, device=DEV)
     wide[:, 16: 16 + 4096] = xc.view(torch.uint8)
     check(fp8_matmul(wide.view(torch.float8_e4m3fn)[:, 16: 16 + 4096], xs, codes, scales), xc, xs, codes, scales)
+
+
+def test_more_rows_than_a_launch_takes():
+    """2^28 rows of one value: as many blocks, and with 16 threads each the 2^32 of one launch.  A lone value's scale and
+    quotient are off by 2^-24 each, its code is 448, and the result rounds once."""
+    x = torch.randn(1 << 28, 1, dtype=torch.bfloat16, device=DEV)
+    codes = torch.full((1, 1), 2.0, device=DEV).to(torch.float8_e4m3fn)
+    y = fp8_block_linear(x, codes, torch.ones(1, 1, device=DEV))
+    assert bool(((y.float() - 2 * x.float()).abs() <= (2.0 ** -8 + 2.0 ** -22) * 2 * x.float().abs()).all())
