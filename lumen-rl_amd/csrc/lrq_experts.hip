@@ -547,9 +547,10 @@ static int expert_rows(int64_t tokens, const ExpertArgs& a) {
   const int64_t each = pairs / a.experts;
   return each < 16 ? 16 : each < 128 ? 64 : 128;
 }
-// Tokens of a pass: 32-bit offsets into the codes of x, and 1 GiB of y.
+// Tokens of a pass: 32-bit offsets into the codes of x, 1 GiB of y and 1 GiB of h's codes.
 static int64_t expert_pass(int64_t tokens, const ExpertArgs& a) {
-  int64_t most = (int64_t(1) << 28) / ((int64_t)a.top_k * a.hidden);
+  const int64_t y = (int64_t(1) << 28) / ((int64_t)a.top_k * a.hidden), h = (int64_t(1) << 30) / ((int64_t)a.top_k * a.inter);
+  int64_t most = y < h ? y : h;
   most = most < 1 ? 1 : most;
   return tokens < most ? tokens : most;
 }

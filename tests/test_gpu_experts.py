@@ -371,3 +371,11 @@ def test_the_routers_gradient_does_not_end_in_the_experts():
         assert torch.equal(route_experts(logits.detach(), 2)[0], weights)
         with pytest.raises(RuntimeError, match="route_experts has no forward-mode derivative"):
             route_experts(forward_ad.make_dual(logits.detach(), torch.ones_like(logits)), 2)
+
+
+def test_hidden_values_that_fill_a_pass():
+    """8192 tokens of 2 pairs and 65536 hidden values fill the 1 GiB of codes of a pass; 16 columns are 1 MiB of results."""
+    x, ids, weights, *w = make(8200, 3, 16, 65536, 2)
+    y = fp8_experts(x, ids, weights, *w)
+    for rows in (slice(0, 4), slice(8189, 8200)):
+        check(y[rows], *reference(x[rows], ids[rows], weights[rows], *w, exact_sums=True))

@@ -127,3 +127,21 @@ def test_host_tensors_are_refused():
                  lambda: fp8_experts(x, torch.zeros(4, 2, dtype=torch.int32), torch.ones(4, 2), w[None], s[None], w[None], s[None])):
         with pytest.raises(ValueError, match="HIP device"):
             call()
+
+
+@pytest.mark.parametrize("hidden,inter", [(16, 65536), (64, 16384), (256, 4096), (4096, 14336), (65536, 16)])
+def test_experts_workspace_is_bounded_for_any_sizes(hidden, inter):
+    """A pass holds at most 1 GiB of results and 1 GiB of hidden codes; their scales, x in codes and the pairs' order are no larger
+    than those (a token's row of x is at most its pairs' results, blocks of 16 columns at least a quarter of their scale)."""
+    ws = L().lrq_fp8_experts_workspace
+    for tokens in (1 << 12, 1 << 16, 1 << 20, 1 << 28):
+        assert 0 < ws(tokens, hidden, inter, 8, 2) < 4 << 30
+
+
+def test_a_pass_of_the_experts_is_no_shorter_for_ordinary_sizes():
+    """Up to an intermediate size of four times the hidden one, results alone bound it: 1 GiB of them."""
+    ws = L().lrq_fp8_experts_workspace
+    for hidden, inter in ((2048, 768), (4096, 14336), (2048, 8192)):
+        tokens = (1 << 28) // (2 * hidden)
+        assert ws(tokens, hidden, inter, 8, 2) > 1 << 30
+        assert ws(4 * tokens, hidden, inter, 8, 2) == ws(tokens, hidden, inter, 8, 2)
