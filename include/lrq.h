@@ -236,7 +236,7 @@ int lrq_route_grad(const void* logits, int dtype, int64_t tokens, int64_t expert
  *   scales [experts, ceil(2 inter / 128), ceil(hidden / 128)];
  *   down : [experts, hidden, inter], scales [experts, ceil(hidden / 128), ceil(inter / 128)];
  *   out : [tokens, hidden], dense.  Codes and out 16-byte aligned.
- * hidden and inter: multiples of 16, 2 hidden inter < 2^31; experts at most 1024,
+ * hidden and inter: multiples of 16 up to 65536, 2 hidden inter < 2^31; experts at most 1024,
  * top_k 64.  `workspace`: lrq_fp8_experts_workspace bytes of device memory, 256-byte
  * aligned, overwritten.  No counterpart in the reference (vLLM / ATOM run these).
  */

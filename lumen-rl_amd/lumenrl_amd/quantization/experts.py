@@ -143,7 +143,7 @@ def fp8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_u
     ``route_experts`` gives them; int32, int64 ids are narrowed) -> [..., H] in x's
     dtype.  ``gate_up`` [E, 2 I, H] (gate's rows first) and ``down`` [E, H, I] are
     e4m3 codes with float32 scales of 128x128 tiles, as ``quantize_fp8_blockwise``
-    writes them; H and I are multiples of 16.  x and the hidden values are quantized
+    writes them; H and I are multiples of 16 up to 65536.  x and the hidden values are quantized
     in 1x128 blocks; all else is float32.  A pair whose id is not one of 0 .. E - 1
     is left out (a shard's other experts, say).  No gradient: a backward pass through
     the result raises.
@@ -170,9 +170,10 @@ def fp8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_u
     if ids.device != dev or weights.device != dev:
         raise ValueError(f"{what}: ids and weights must be on {dev}")
     k = ids.shape[-1]
-    if not 1 <= e <= 1024 or not 1 <= k <= 64 or h % 16 or i % 16 or not h or not i or 2 * h * i >= 1 << 31:
-        raise ValueError(f"{what}: {e} experts (at most 1024), top {k} (at most 64), H {h} and I {i} (multiples of 16, "
-                         "2 H I below 2^31)")
+    if (not 1 <= e <= 1024 or not 1 <= k <= 64 or h % 16 or i % 16 or not 0 < h <= 65536 or not 0 < i <= 65536
+            or 2 * h * i >= 1 << 31):
+        raise ValueError(f"{what}: {e} experts (at most 1024), top {k} (at most 64), H {h} and I {i} (multiples of 16 up to "
+                         "65536, 2 H I below 2^31)")
     if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
             x.requires_grad or weights.requires_grad or gate_up.requires_grad or gate_up_scales.requires_grad
             or down.requires_grad or down_scales.requires_grad):

@@ -379,3 +379,12 @@ def test_hidden_values_that_fill_a_pass():
     y = fp8_experts(x, ids, weights, *w)
     for rows in (slice(0, 4), slice(8189, 8200)):
         check(y[rows], *reference(x[rows], ids[rows], weights[rows], *w, exact_sums=True))
+
+
+@pytest.mark.parametrize("h,i", [(1 << 17, 16), (16, 1 << 17)])
+def test_sizes_above_65536_are_refused_by_name(h, i):
+    gu, gus = torch.zeros(1, 2 * i, h, dtype=torch.uint8, device=DEV).view(E4M3), torch.ones(1, -(-2 * i // 128), -(-h // 128), device=DEV)
+    dn, dns = torch.zeros(1, h, i, dtype=torch.uint8, device=DEV).view(E4M3), torch.ones(1, -(-h // 128), -(-i // 128), device=DEV)
+    with pytest.raises(ValueError, match="fp8_experts: .*65536"):
+        fp8_experts(torch.zeros(2, h, dtype=torch.bfloat16, device=DEV), torch.zeros(2, 1, dtype=torch.int32, device=DEV),
+                    torch.ones(2, 1, device=DEV), gu, gus, dn, dns)
