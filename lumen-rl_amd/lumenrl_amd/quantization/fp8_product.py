@@ -42,6 +42,8 @@ def check_tiles(what: str, codes: Tensor, scales: Tensor, device: torch.device) 
 
 
 def _check_bias(what: str, bias: Tensor, n: int, device: torch.device) -> None:
+    if not isinstance(bias, Tensor):
+        raise TypeError(f"{what}: bias must be a tensor, got {type(bias)!r}")
     if bias.shape != (n,) or bias.dtype not in _IN_DTYPES or bias.device != device or not bias.is_contiguous():
         raise ValueError(f"{what}: bias must be a contiguous [{n}] bf16, fp16 or fp32 tensor on {device}")
 
@@ -85,6 +87,8 @@ def fp8_matmul(x_codes: Tensor, x_scales: Tensor, codes: Tensor, scales: Tensor,
     """
     if not isinstance(x_codes, Tensor) or not x_codes.is_cuda:
         raise ValueError("fp8_matmul: expected codes on a HIP device")
+    if not isinstance(x_scales, Tensor):
+        raise TypeError(f"fp8_matmul: x's scales must be a tensor, got {type(x_scales)!r}")
     if x_codes.dtype != torch.float8_e4m3fn or x_scales.dtype != torch.float32:
         raise TypeError(f"fp8_matmul: x must be float8_e4m3fn with float32 scales, got {x_codes.dtype} and {x_scales.dtype}")
     if out_dtype not in _IN_DTYPES:

@@ -199,3 +199,13 @@ def test_more_rows_than_a_launch_takes():
     codes = torch.full((1, 1), 2.0, device=DEV).to(torch.float8_e4m3fn)
     y = fp8_block_linear(x, codes, torch.ones(1, 1, device=DEV))
     assert bool(((y.float() - 2 * x.float()).abs() <= (2.0 ** -8 + 2.0 ** -22) * 2 * x.float().abs()).all())
+
+
+def test_operands_that_are_no_tensors_are_refused_by_name():
+    codes, scales = weight(64, 256)
+    x = acts(4, 256, torch.bfloat16)
+    xc, xs = fp8_block_quant(x, (1, 128))
+    for call in (lambda: fp8_matmul(xc, None, codes, scales), lambda: fp8_matmul(xc, xs, codes, scales, 1.0),
+                 lambda: fp8_block_linear(x, codes, scales, [0.0] * 64), lambda: fp8_block_linear(x, codes, None)):
+        with pytest.raises(TypeError, match="fp8_(matmul|block_linear): "):
+            call()
