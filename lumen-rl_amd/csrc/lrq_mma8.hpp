@@ -116,7 +116,7 @@ __device__ __forceinline__ Rsrc make_rsrc(const void* base, uint32_t bytes) {
 }
 __device__ __forceinline__ void dma16(Rsrc r, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :: "s"(lds), "v"(off), "s"(r) : "memory");
+               :: "s"(lds), "v"(off), "s"(r) : "memory", "m0");
 }
 // Until at most N of the wave's loads are on their way: they arrive in order.
 template <int N>
