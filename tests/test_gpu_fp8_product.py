@@ -209,3 +209,40 @@ def test_operands_that_are_no_tensors_are_refused_by_name():
                  lambda: fp8_block_linear(x, codes, scales, [0.0] * 64), lambda: fp8_block_linear(x, codes, None)):
         with pytest.raises(TypeError, match="fp8_(matmul|block_linear): "):
             call()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_whole_numbers_are_exact(m, n, k, dtype):
+    """Codes of 0, 1 and 2 either way and scales of 1 to 8: every product, block's sum and sum of blocks is a whole number below
+    2^24 (k x 4 x 64), which no instruction drops bits of, in any order.  So a result is the exact one, rounded once; a code that
+    is lost, misplaced or read twice shows."""
+    g = torch.Generator(device=DEV).manual_seed(m + n + k)
+
+    def codes(rows):
+        return torch.randint(-2, 3, (rows, k), generator=g, device=DEV).float().to(torch.float8_e4m3fn)
+
+    def scales(rows):
+        return torch.pow(2.0, torch.randint(0, 4, (rows, -(-k // 128)), generator=g, device=DEV).float())
+
+    xc, xs, wc, ws = codes(m), scales(m), codes(n), scales(-(-n // 128))
+    want = ((xc.double() * spread(xs, m, k, (1, 128))) @ (wc.double() * spread(ws, n, k)).T).to(dtype)
+    assert torch.equal(fp8_matmul(xc, xs, wc, ws, out_dtype=dtype), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [s for s in SHAPES if s[2] >= 128])
+def test_the_whole_is_as_near_as_the_results_own_rounding(m, n, k, dtype):
+    """Normal activations and weights, no channel above the rest: half a step at most an element, and what the instructions drop.
+
+    That is below 2^-13 of a block's largest product, some 4 x 4 times the norm's share of both operands, each product's one way
+    or the other: 2^-13 x 16 / sqrt(128), over the blocks as over their sum; none of it for float32 results or up to four tokens,
+    whose sums are off by (128 + k / 128 + 12) 2^-23 at most if all terms had one sign, and by that of their norm here."""
+    g = torch.Generator(device=DEV).manual_seed(m + 2 * n + k)
+    x = torch.randn(m, k, generator=g, device=DEV).to(dtype)
+    codes, scales = quantize_fp8_blockwise(torch.randn(n, k, generator=g, device=DEV) * 0.02)
+    xc, xs = fp8_block_quant(x, (1, 128))
+    want = (xc.double() * spread(xs, m, k, (1, 128))) @ (codes.double() * spread(scales, n, k)).T
+    off = float((fp8_block_linear(x, codes, scales).double() - want).norm() / want.norm())
+    drop = 2.0 ** -13 * 16 / 128 ** 0.5 if m > 4 and dtype != torch.float32 else 0.0
+    assert off < torch.finfo(dtype).eps / 2 + drop + (128 + k // 128 + 12) * 2.0 ** -23, off
