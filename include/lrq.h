@@ -172,8 +172,12 @@ int lrq_fp8_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t 
  * FP8 products on a weight in 128x128 tiles, the layout lrq_fp8_block_quant
  * writes with 128 x 128 blocks (vLLM's weight_scale_inv):
  *   out[m, n] = sum_b (xs[m, b] * ws[n / 128, b]) sum_{k in block b} xc[m, k] wc[n, k] + bias[n],
- * sums and the scales' product in float32, one rounding to out's type.  No
- * counterpart in the reference, which leaves these products to vLLM / ATOM.
+ * sums over blocks and the scales' product in float32, one rounding to out's type.
+ * A block's own sum is float32 too for float32 results and for up to four rows of x.
+ * 16-bit results of more rows take the f8f6f4 matrix instructions' sums, which drop
+ * what is below 2^-13 of the block's largest product: at most 128 times that a block,
+ * 1.5e-5 of the result's norm with normal codes.  No counterpart in the reference,
+ * which leaves these products to vLLM / ATOM.
  *   lrq_fp8_matmul: x as e4m3 codes [rows, k] (row stride ld >= k) with float32
  *     scales [rows, ceil(k/128)], dense; out of out_dtype (bf16, fp16 or fp32).
  *     `workspace`: lrq_fp8_matmul_workspace(rows, k, n) bytes, 0 but for some tens
@@ -229,8 +233,14 @@ int lrq_route_grad(const void* logits, int dtype, int64_t tokens, int64_t expert
  * The chosen experts' SwiGLU MLPs on weights in 128x128 tiles, and their sum:
  *   out[t] = sum_j weights[t, j] * down_e(silu(gate_e(x_t)) * up_e(x_t)), e = ids[t, j],
  * x and the hidden values quantized to e4m3 in 1x128 blocks (as lrq_fp8_block_quant
- * with float32 arithmetic), everything else float32, one rounding to x's type (bf16
- * or fp16).  A pair whose id is outside 0 .. experts - 1 is left out.
+ * with float32 arithmetic), one rounding to x's type (bf16 or fp16), everything
+ * between in float32 but for a block's own sum in two cases, which is f8f6f4's (above):
+ *   in the second product (down), beyond some 64 pairs;
+ *   in the first, for bf16 with 128 pairs (those left out counted) or more an expert:
+ *   one hidden code in some 3000 then is its neighbour, and the result's error, with its
+ *   rounding, 1.2 to 1.6 times that of float32 sums (2.3 at most measured with few rows,
+ *   as when most pairs are left out).
+ * A pair whose id is outside 0 .. experts - 1 is left out.
  *   x : [tokens, hidden], row stride ld;  ids, weights : [tokens, top_k], dense;
  *   gate_up : [experts, 2 inter, hidden] codes, gate's rows first, with float32
  *   scales [experts, ceil(2 inter / 128), ceil(hidden / 128)];

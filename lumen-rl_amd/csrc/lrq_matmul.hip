@@ -218,10 +218,14 @@ __global__ __launch_bounds__(256) void k_mm8_join(MatmulArgs a, const float* par
 // ---------------------------------------------------------------------------
 // Codes whose rows are not 4-byte aligned go through registers, at less than half the
 // speed; with many tokens they are copied to rows of kp = 16 ceil(k / 16) first, zeros
-// at the end.  fp8_block_linear quantizes x into such rows anyway, through the caches,
-// where the product finds them: 48 tokens x [4096, 12288] 18.5 us, 19.7 by k_row, which
-// stores past them; 1024 x [4096, 4096] 31 and 35, 8192 tokens 151 and 155.  8192 tokens x [12288, 4097] 448 us,
-// 1000 as they are; 4096 x [4096, 4097] 89 and 192; 1024 tokens 51 and 54, 512 36 and 31.
+// at the end (8192 tokens x [12288, 4097] 448 us, 1000 as they are; 4096 x [4096, 4097]
+// 89 and 192; 1024 tokens 51 and 54, 512 36 and 31).  Codes at odd addresses, or rows at
+// an odd pitch, of a k that 4 divides are left as they are.
+//
+// fp8_block_linear quantizes x into rows at such a pitch anyway, through the caches, where
+// the product finds them: with weights from memory, all launches of a call together, 48
+// tokens x [4096, 12288] 21.0 us and 8192 x [4096, 4096] 149, by k_row, which stores past
+// the caches, 21.9 and 151; 1024 x [4096, 4096] 36 by both.
 __global__ __launch_bounds__(256) void k_mm8_pad(const uint8_t* from, int64_t ld, uint32_t pieces, int k, uint32_t per, uint8_t* to) {
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   if (i >= pieces) return;
@@ -260,6 +264,11 @@ static void launch_dot(const MatmulArgs& a, hipStream_t stream) {
   const unsigned lds = XDT >= 0 ? (unsigned)(a.m * a.kb * (kBlk + 4)) : 0;
   hipLaunchKernelGGL((k_mm8_dot<XDT, M, R>), dim3((unsigned)ceil_div(a.n, 8 * R)), dim3(512), lds, stream, a);
 }
+// Two rows a wave from 4096 rows on, so that a token's codes are widened for both; with
+// fewer rows, twice the waves.  us by one and by two, weights from memory: one token x
+// [2048, 4096] 5.0 and 5.8, [4096, 4096] 7.1 and 6.9, [12288, 4096] 13.6 and 13.2; four
+// tokens 9.0 and 11.2, 12.7 and 12.3, 32 and 25.  (Of a K of 1024 one row stays ahead
+// up to 6144 rows, by 0.6 us at most; of 12288 two are ahead from 3000 on.)
 template <int XDT>
 static void launch_dots(const MatmulArgs& a, hipStream_t stream) {
   if (a.m == 1) a.n >= 4096 ? launch_dot<XDT, 1, 2>(a, stream) : launch_dot<XDT, 1, 1>(a, stream);
@@ -299,8 +308,9 @@ constexpr int64_t kDots = 4, kSplitRows = 64;
 bool matmul_quantizes(int64_t m, int64_t k) { return m <= kDots && m * ceil_div(k, kBlk) * (kBlk + 4) <= 65536; }
 
 // Parts of K: a work-group for every CU, of 3 blocks at least.  48 tokens x [4096,
-// 12288] in 4 parts of 24 blocks 16.5 us, 18.4 in 8, 28 in one; 64-row tiles, as 128-row
-// ones are two times fewer (19 us).
+// 12288], the product and its join with weights from memory: in 4 parts of 24 blocks
+// 16.8 us, 18.5 in 8, 23 in 2, 36 in one; 64-row tiles, as 128-row ones are two times
+// fewer.
 static int64_t split_parts(int64_t m, int64_t n, int64_t k) {
   if (m <= kDots || m > kSplitRows) return 1;
   const int64_t tiles = ceil_div(n, 64), kb = ceil_div(k, kBlk);

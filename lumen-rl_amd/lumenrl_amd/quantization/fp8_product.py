@@ -82,8 +82,11 @@ def fp8_matmul(x_codes: Tensor, x_scales: Tensor, codes: Tensor, scales: Tensor,
     ``x_codes`` [M, K] with float32 ``x_scales`` [M, ceil(K/128)] (as
     ``fp8_block_quant(x, (1, 128))`` gives them; rows may be a view's),
     ``codes`` [N, K] with float32 ``scales`` [ceil(N/128), ceil(K/128)] ->
-    [M, N] of ``out_dtype`` (bfloat16, float16 or float32), sums in float32.
-    No gradient: a backward pass through the result raises.
+    [M, N] of ``out_dtype`` (bfloat16, float16 or float32).  Sums are float32; within
+    a block of 128, 16-bit results of more than four rows take the matrix
+    instructions' own, which drop what is below 2^-13 of the block's largest product
+    (1.5e-5 of the result's norm with normal codes).  No gradient: a backward pass
+    through the result raises.
     """
     if not isinstance(x_codes, Tensor) or not x_codes.is_cuda:
         raise ValueError("fp8_matmul: expected codes on a HIP device")
@@ -144,8 +147,8 @@ def fp8_block_linear(x: Tensor, codes: Tensor, scales: Tensor, bias: Optional[Te
     (as ``fp8_block_quant(x, (1, 128))``) and multiplied with ``codes`` [N, K]
     and float32 ``scales`` [ceil(N/128), ceil(K/128)] -> [..., N] in x's dtype.
 
-    Up to four tokens take one launch, more take two or three.  No gradient: a backward
-    pass through the result raises.
+    Sums are ``fp8_matmul``'s.  Up to four tokens take one launch, more take two or
+    three.  No gradient: a backward pass through the result raises.
     """
     _check_input(x, "fp8_block_linear")
     dev = x.device
