@@ -233,13 +233,9 @@ int lrq_route_grad(const void* logits, int dtype, int64_t tokens, int64_t expert
  * The chosen experts' SwiGLU MLPs on weights in 128x128 tiles, and their sum:
  *   out[t] = sum_j weights[t, j] * down_e(silu(gate_e(x_t)) * up_e(x_t)), e = ids[t, j],
  * x and the hidden values quantized to e4m3 in 1x128 blocks (as lrq_fp8_block_quant
- * with float32 arithmetic), one rounding to x's type (bf16 or fp16), everything
- * between in float32 but for a block's own sum in two cases, which is f8f6f4's (above):
- *   in the second product (down), beyond some 64 pairs;
- *   in the first, for bf16 with 128 pairs (those left out counted) or more an expert:
- *   one hidden code in some 3000 then is its neighbour, and the result's error, with its
- *   rounding, 1.2 to 1.6 times that of float32 sums (2.3 at most measured with few rows,
- *   as when most pairs are left out).
+ * with float32 arithmetic), one rounding to x's type (bf16 or fp16), everything else
+ * float32, but that beyond some 64 pairs the second product's blocks are summed by the
+ * f8f6f4 instructions (above).
  * A pair whose id is outside 0 .. experts - 1 is left out.
  *   x : [tokens, hidden], row stride ld;  ids, weights : [tokens, top_k], dense;
  *   gate_up : [experts, 2 inter, hidden] codes, gate's rows first, with float32

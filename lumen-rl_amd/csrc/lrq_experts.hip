@@ -177,17 +177,20 @@ __global__ __launch_bounds__(kSortThreads) void k_ex_place(ExpertArgs a, int bm,
 }
 static_assert(kSortPairs == kSortThreads * kSortAhead, "");
 
-// Work-group wg's tile and its piece of nb: each XCD (wg % 8) takes one run of the big
-// tiles and one of the others, a tile's pieces after one another, so that it reads an
-// expert's weights once, and the longest work comes first.
-__device__ __forceinline__ bool expert_piece(const ExpertArgs& a, int wg, int nb, int& tile, int& n) {
+// Work-group wg's tile and its piece of nb, or of nb_big if the tile is a big one: each
+// XCD (wg % 8) takes one run of the big tiles and one of the others, a tile's pieces after
+// one another, so that it reads an expert's weights once, and the longest work comes first.
+struct ExpertPiece {
+  int tile, n;  // tile < 0: none is left
+  bool big;
+};
+__device__ __forceinline__ ExpertPiece expert_piece(const ExpertArgs& a, int wg, int nb_big, int nb) {
   const int big = gld<int32_t>(a.total), rest = gld<int32_t>(a.total + 1);
-  const int per_big = (big * nb + 7) >> 3, per = (rest * nb + 7) >> 3, i = wg >> 3, x = wg & 7;
+  const int per_big = (big * nb_big + 7) >> 3, per = (rest * nb + 7) >> 3, i = wg >> 3, x = wg & 7;
   const bool is_big = i < per_big;
-  const int t = is_big ? x * per_big + i : x * per + i - per_big;
-  if (t >= (is_big ? big : rest) * nb || i - per_big >= per) return false;
-  tile = t / nb + (is_big ? 0 : big), n = t % nb;
-  return true;
+  const int t = is_big ? x * per_big + i : x * per + i - per_big, pieces = is_big ? nb_big : nb;
+  if (t >= (is_big ? big : rest) * pieces || i - per_big >= per) return {-1, 0, false};
+  return {t / pieces + (is_big ? 0 : big), t % pieces, is_big};
 }
 
 // h [rows, 128] of a work-group whose WN waves hold 16 NS columns each: lane (c, g)
@@ -248,9 +251,8 @@ __device__ __forceinline__ void store_hidden(const ExpertArgs& a, f32x4 (&h)[NS]
 // An expert's rows in tiles
 // ---------------------------------------------------------------------------
 // Weight rows of a tile: 16 of gate, the same 16 of up, and so on.
-template <bool SKIP>
 struct UpTile {
-  static constexpr bool kCut = false, kSkip = SKIP;
+  static constexpr bool kCut = false, kSkip = true;
   const ExpertArgs& a;
   const ExpertTile& t;
   int block;
@@ -277,52 +279,36 @@ struct UpTile {
   }
 };
 
-// EXACT: float32 sums (lrq_mma8.hpp).  The f8f6f4 instructions' sums are off by 1.5e-5
-// of their norm, which is little beside h's 4 bits, but moves one code in some 3000 to
-// its neighbour: 2e-3 of the norm of out, 3e-3 where a few activations are forty times
-// as large as the rest.  bf16 results' own rounding is 1.7e-3, so both together are
-// 1.2 to 1.6 times it for experts with 128 rows or more (2.3 times in the worst of 14
-// drawn sizes, with fewer rows); fp16's is 2e-4.  So only bf16 experts with many rows
-// take them: 4096 tokens of 8 pairs 417 us, 542 in exact sums; 512 tokens 160 and 173,
-// 200 on a quarter 51 and 54, where memory bounds both and sums are exact.
-template <int FN, int FM, int WN, int WM, int STAGES, bool EXACT, bool SKIP = true>
-__device__ __forceinline__ void up_tile(const ExpertArgs& a, const ExpertTile& t, int block, uint8_t* lds) {
+// h comes from float32 sums (lrq_mma8.hpp), in whatever tile, so that a token's hidden
+// codes do not depend on the tokens beside it.  The f8f6f4 instructions' sums are off by
+// 1.5e-5 of their norm, which is little beside h's 4 bits, but moves one code in some
+// 3000 to its neighbour: 2e-3 of the norm of out, as much as a bf16 result's rounding
+// (0.0026 against 64 bits, 0.0018 as here).  4096 tokens of 8 pairs x 768 take 520 us,
+// 400 with them; 200 on a quarter, where memory bounds both, 54 and 51.
+// Big tiles are taken in parts of BM rows, side by side: conversions to bf16 take the
+// registers of 256.
+template <int FN, int FM, int WN, int WM, int STAGES>
+__global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
   static_assert(16 * FN * WN == 256, "128 columns of h");
+  constexpr int BM = 16 * FM * WM, PARTS = kBigRows / BM;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<FN, FM, WN, WM, STAGES>];
+  const ExpertPiece p = expert_piece(a, blockIdx.x, PARTS * a.ib, a.ib);
+  if (p.tile < 0) return;
+  ExpertTile t = a.tiles[p.tile];
+  const int block = p.big ? p.n / PARTS : p.n, part = p.big ? p.n % PARTS : 0;
+  t.first += BM * part, t.rows -= BM * part;
+  if (t.rows <= 0) return;
+  t.rows = t.rows < BM ? t.rows : BM;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const UpTile<SKIP> src{a, t, block};
   f32x4 acc[FN][FM], h[FN / 2][FM];
-  tile_sums<FN, FM, WN, WM, STAGES, true, true, EXACT>(src, a.hidden, 0, a.kb, lds, acc);
+  tile_sums<FN, FM, WN, WM, STAGES, true, true, true>(UpTile{a, t, block}, a.hidden, 0, a.kb, lds, acc);
 #pragma unroll
   for (int i = 0; i < FN / 2; ++i)
 #pragma unroll
     for (int j = 0; j < FM; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) h[i][j][r] = silu_mul(acc[2 * i][j][r], acc[2 * i + 1][j][r]);
-  store_hidden<FN / 2, FM, WN>(a, h, t.first, wave % WM * 16 * FM, t.rows, block, wave / WM, reinterpret_cast<uint32_t*>(lds),
-                               16 * FM * WM);
-}
-
-template <int FN, int FM, int WN, int WM, int STAGES>
-__global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_up_tiles(ExpertArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<FN, FM, WN, WM, STAGES>];
-  int tile, block;
-  if (!expert_piece(a, blockIdx.x, a.ib, tile, block)) return;
-  const ExpertTile t = a.tiles[tile];
-  up_tile<FN, FM, WN, WM, STAGES, true>(a, t, block, lds);
-}
-
-// Tiles of 256 and of up to 128 rows in one launch: the large ones take 49 us a round
-// over the chip, of 4096 k, and the others 31 (and cut experts' rows with less left
-// over: 32768 pairs of 128 experts in 27 % more rows than there are, 256 rows alone in
-// 55 %).
-constexpr int kMixedLds = kTileLds<4, 4, 4, 2, 3> > kTileLds<8, 4, 2, 4, 2> ? kTileLds<4, 4, 4, 2, 3> : kTileLds<8, 4, 2, 4, 2>;
-__global__ __launch_bounds__(512, 1) void k_ex_up_mixed(ExpertArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kMixedLds];
-  int tile, block;
-  if (!expert_piece(a, blockIdx.x, a.ib, tile, block)) return;
-  const ExpertTile t = a.tiles[tile];
-  if (t.rows > 128) up_tile<8, 4, 2, 4, 2, false, false>(a, t, block, lds);
-  else up_tile<4, 4, 4, 2, 3, false>(a, t, block, lds);
+  store_hidden<FN / 2, FM, WN>(a, h, t.first, wave % WM * 16 * FM, t.rows, block, wave / WM, reinterpret_cast<uint32_t*>(lds), BM);
 }
 
 template <bool SKIP>
@@ -376,18 +362,25 @@ template <int FN, int FM, int WN, int WM, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM, 1) void k_ex_down_tiles(ExpertArgs a) {
   constexpr int BN = 16 * FN * WN;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<FN, FM, WN, WM, STAGES>];
-  int tile, block;
-  if (!expert_piece(a, blockIdx.x, (a.hidden + BN - 1) / BN, tile, block)) return;
-  const ExpertTile t = a.tiles[tile];
-  down_tile<FN, FM, WN, WM, STAGES>(a, t, block, lds);
+  const int nb = (a.hidden + BN - 1) / BN;
+  const ExpertPiece p = expert_piece(a, blockIdx.x, nb, nb);
+  if (p.tile < 0) return;
+  const ExpertTile t = a.tiles[p.tile];
+  down_tile<FN, FM, WN, WM, STAGES>(a, t, p.n, lds);
 }
+// Tiles of 256 and of up to 128 rows in one launch: the large ones take 49 us a round
+// over the chip, of 4096 k, and the others 31 (and cut experts' rows with less left
+// over: 32768 pairs of 128 experts in 27 % more rows than there are, 256 rows alone in
+// 55 %).  4096 tokens of 8 pairs: 144 us, 171 in tiles of 128.
+constexpr int kMixedLds = kTileLds<4, 4, 4, 2, 3> > kTileLds<8, 4, 2, 4, 2> ? kTileLds<4, 4, 4, 2, 3> : kTileLds<8, 4, 2, 4, 2>;
 __global__ __launch_bounds__(512, 1) void k_ex_down_mixed(ExpertArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[kMixedLds];
-  int tile, block;
-  if (!expert_piece(a, blockIdx.x, (a.hidden + 255) / 256, tile, block)) return;
-  const ExpertTile t = a.tiles[tile];
-  if (t.rows > 128) down_tile<8, 4, 2, 4, 2, false>(a, t, block, lds);
-  else down_tile<4, 4, 4, 2, 3>(a, t, block, lds);
+  const int nb = (a.hidden + 255) / 256;
+  const ExpertPiece p = expert_piece(a, blockIdx.x, nb, nb);
+  if (p.tile < 0) return;
+  const ExpertTile t = a.tiles[p.tile];
+  if (t.rows > 128) down_tile<8, 4, 2, 4, 2, false>(a, t, p.n, lds);
+  else down_tile<4, 4, 4, 2, 3>(a, t, p.n, lds);
 }
 
 // out[t] = the sum of the token's rows of y, in the order of its pairs.
@@ -536,11 +529,12 @@ __global__ __launch_bounds__(512) void k_ex_down_few(ExpertArgs a) {
 // ---------------------------------------------------------------------------
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// Rows of a tile, by the pairs an expert has on average; 0 for few pairs.  With 128
-// experts of 2048 x 192, us in tiles of 16, 64 and 128 rows: 32 tokens of 8 pairs 41,
-// 40, 51; 400 tokens 57, 67, 67; 800 tokens 86, 77, 97.  Of 2048 x 768: 512 tokens
-// 199, 161, 169; 2048 tokens -, 277, 276; 4096 tokens -, 451, 433.  32 rows win
-// nowhere.  (All of them before 256 rows joined 128, and 64 rows took exact sums.)
+// Rows of a tile, by the pairs an expert has on average; 0 for few pairs.  us in tiles
+// of 16, 64 and 128 rows (256 and 128 in the second product): with 128 experts of 2048 x
+// 192, 100 tokens of 8 pairs 49, 51, 67; 200 tokens 57, 55, 72; 800 tokens 110, 95, 127;
+// 2048 tokens -, 168, 173; 4096 tokens -, 281, 267.  Of 2048 x 768: 200 tokens 130, 137,
+// 164; 512 tokens 192, 164, 190; 2048 tokens -, 330, 322; 4096 tokens -, 551, 511.  32
+// rows win nowhere.
 static int expert_rows(int64_t tokens, const ExpertArgs& a) {
   const int64_t pairs = tokens * a.top_k, few_lds = (int64_t)a.top_k * a.ib * (kBlk + 4);
   if (pairs <= 64 && pairs <= a.experts && few_lds <= 48 * 1024 && a.kb * (kBlk + 4) <= 48 * 1024) return 0;
@@ -625,7 +619,7 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
       continue;
     }
     const int64_t pairs = a.tokens * a.top_k, tiles = tile_bound(pairs, bm, a.experts);
-    const bool big = bm == 128 && dtype == kBF16;  // conversions to bf16 take the registers of 256 rows
+    const bool big = bm == 128;
     int64_t each = (pairs + kSortMost - 1) / kSortMost;
     each = each < kSortPairs ? kSortPairs : each;
     const int groups = (int)((pairs + each - 1) / each);
@@ -639,13 +633,10 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
     } else if (bm == 64) {
       up<4, 2, 4, 2, 3>(a, tiles, stream);
       down<4, 2, 2, 2, 2>(a, tiles, stream);
-    } else if (big) {
-      const unsigned pieces = (unsigned)tiles + 16;  // each kind's runs are rounded up to 8 pieces
-      hipLaunchKernelGGL(k_ex_up_mixed, dim3(pieces * (unsigned)a.ib), dim3(512), 0, stream, a);
-      hipLaunchKernelGGL(k_ex_down_mixed, dim3(pieces * (unsigned)((a.hidden + 255) / 256)), dim3(512), 0, stream, a);
     } else {
-      up<4, 4, 4, 2, 3>(a, tiles, stream);
-      down<4, 4, 4, 2, 3>(a, tiles, stream);
+      // each kind's runs are rounded up to 8 pieces: 16 tiles more hold them
+      up<4, 4, 4, 2, 3>(a, tiles + 16, stream);
+      hipLaunchKernelGGL(k_ex_down_mixed, dim3((unsigned)(tiles + 16) * (unsigned)((a.hidden + 255) / 256)), dim3(512), 0, stream, a);
     }
     const dim3 sum((unsigned)((a.tokens * a.hidden / 8 + 255) / 256));
     if (dtype == kBF16) hipLaunchKernelGGL((k_ex_sum<kBF16>), sum, dim3(256), 0, stream, a);

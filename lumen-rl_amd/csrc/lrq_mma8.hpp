@@ -15,8 +15,8 @@
 //   * EXACT: four bf16 instructions on the same codes, which are exact in bf16, as
 //     are their products; sums are float32.  Half the rate, and conversions: 48 tokens
 //     x [4096, 12288], the product and its join with weights from memory, 20.2 us
-//     instead of 17.0.  Taken for float32 results and for most of what experts
-//     quantize again; or
+//     instead of 17.0.  Taken for float32 results and for what experts quantize
+//     again; or
 //   * for up to four tokens, float32 multiply-adds.
 #pragma once
 

@@ -145,11 +145,9 @@ def fp8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_u
     e4m3 codes with float32 scales of 128x128 tiles, as ``quantize_fp8_blockwise``
     writes them; H and I are multiples of 16 up to 65536.  x and the hidden values are
     quantized in 1x128 blocks; all else is float32, but that beyond some 64 pairs the
-    second product's blocks of 128 are summed as ``fp8_matmul``'s for 16 bits, and the
-    first one's too for bf16 with 128 pairs an expert or more (1.2 to 1.6 times the
-    error of float32 sums, bf16's own rounding with it).  A pair whose id is not one of
-    0 .. E - 1 is left out (a shard's other experts, say).  No gradient: a backward
-    pass through the result raises.
+    second product's blocks of 128 are summed as ``fp8_matmul``'s for 16 bits.  A pair
+    whose id is not one of 0 .. E - 1 is left out (a shard's other experts, say).  No
+    gradient: a backward pass through the result raises.
     """
     what = "fp8_experts"
     _check_input(x, what)

@@ -388,3 +388,30 @@ def test_sizes_above_65536_are_refused_by_name(h, i):
     with pytest.raises(ValueError, match="fp8_experts: .*65536"):
         fp8_experts(torch.zeros(2, h, dtype=torch.bfloat16, device=DEV), torch.zeros(2, 1, dtype=torch.int32, device=DEV),
                     torch.ones(2, 1, device=DEV), gu, gus, dn, dns)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,e,h,i,k", [(2000, 3, 1040, 144, 2), (1111, 8, 400, 272, 4), (3000, 20, 256, 384, 8)])
+def test_a_tokens_result_does_not_depend_on_the_tokens_beside_it(t, e, h, i, k, dtype):
+    """Tiles of 16, 64, 128 and 256 rows sum in the same order and the same instructions: all tokens at once (128 pairs an expert and
+    more) and few of them at a time give the same bits."""
+    x, ids, weights, *w = make(t, e, h, i, k, dtype, t + k, whole=False)
+    want = fp8_experts(x, ids, weights, *w)
+    for some in (65, 400):  # more than 64 pairs, which do not go through tiles
+        for t0 in range(0, 800, some):
+            rows = slice(t0, t0 + some)
+            assert torch.equal(fp8_experts(x[rows], ids[rows], weights[rows], *w), want[rows])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,e,h,i,k", [(2000, 3, 1040, 144, 2), (1111, 8, 400, 272, 4), (3000, 20, 1024, 384, 8), (4096, 128, 2048, 768, 8)])
+def test_hidden_values_are_those_of_float32_sums_with_many_rows(t, e, h, i, k, dtype):
+    """As with few rows, and sharper, the three errors being independent: the result's rounding is a step / sqrt(12) in the mean, the
+    step eps at most relative to an element; the second product's sums and the codes that move as in the test of few rows."""
+    args = make(t, e, h, i, k, dtype, t + h + i, whole=False)
+    x, ids, weights, *w = args
+    y = fp8_experts(*args)[:1000]
+    want, _ = reference(x[:1000], ids[:1000], weights[:1000], *w)
+    off = (y.double() - want).norm() / want.norm()
+    rounding, sums, moved = torch.finfo(dtype).eps / 12 ** 0.5, 2.0 ** -13.5, 2.0 ** -8.5 * 2.0 ** -3
+    assert float(off) < (rounding ** 2 + sums ** 2 + moved ** 2) ** 0.5, float(off)
