@@ -2,8 +2,9 @@
 // one of its experts e,
 //   g, u = x_q Wgu[e]^T (two halves), h = g / (1 + exp(-g)) u, y = h_q Wd[e]^T,
 //   out[t] = sum over the token's pairs of weight y,
-// with x and h quantized to e4m3 in 1x128 blocks.  Everything between is float32;
-// out is rounded once.  lrq_mma8.hpp has the products' mathematics.
+// with x and h quantized to e4m3 in 1x128 blocks.  Everything between is float32, but
+// for the second product's sums within a block where it goes by tiles (f8f6f4); out is
+// rounded once.  lrq_mma8.hpp has the products' mathematics.
 //
 // Few pairs: two launches, a pair by itself (its expert's weights are all that
 // moves).  More: pairs are sorted by expert, and an expert's rows go through tiles
