@@ -253,6 +253,74 @@ int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, 
                     void* workspace, int64_t workspace_bytes, lrq_stream_t stream);
 
 /*
+ * The FP8 KV cache: pages of keys and values as e4m3 codes, with a power-of-two scale
+ * per page and KV head for each.
+ *   k : [layers, pages, kv_heads, page, dim], v : [layers, pages, kv_heads, dim, page];
+ *   k_scales, v_scales : [layers, pages, kv_heads] float32; refs : [pages] int32.
+ * `page` tokens a page: 16, 32, 64, 128 or 256; dim a multiple of 16 up to 256; kv_heads at
+ * most 256.  A page's heads are dense; k_layer .. vs_page are the steps from layer to
+ * layer and page to page, in codes (multiples of 16; k and v 16-byte aligned) and in scales.
+ * Sequences are rows of a page table [rows, width] int32 (row pitch ld) with their
+ * lengths [rows]: the first ceil(length / page) entries of a row are its pages.  What
+ * these hold is clamped to what there is: an entry that is no page of the pool is no
+ * page, a length ends at width x page (2^30 at most).
+ * No counterpart in the reference, whose engines (vLLM / ATOM) own their caches.
+ *
+ * lrq_kv_append writes new tokens, k and v [tokens, kv_heads, dim] (bf16, fp16 or
+ *   float32; element strides k_token .. v_head) into one layer.  Rows offsets[b] ..
+ *   offsets[b + 1] - 1 are sequence b's last tokens, which `lengths` counts in already;
+ *   offsets null: one token each.  A page's scale is the least power of two, from 2^-48
+ *   to 2^48, that takes the largest finite magnitude to 448 at most; where tokens join a
+ *   page it does not shrink, and where it grows, the codes there are rounded to it again.
+ *   Inf, NaN, and what a scale of 2^48 takes past 448 become NaN codes.
+ * lrq_kv_attend: out [tokens, heads, dim] = softmax(scale q k^T) v for the same rows, each
+ *   over its sequence's keys up to its own place, the last `window` of them if that is
+ *   above 0; query head i reads KV head i / (heads / kv_heads).  Scores and sums are
+ *   float32, probabilities are rounded to fp16.  A row that sees no key is 0; a NaN is
+ *   in the results of the rows that see it alone.  lse: [tokens, heads], the scores' log-sum-exp
+ *   (natural), or null.  Rows behind offsets[seqs] stay as they were, or become 0 with
+ *   zero_rest.  q is bf16 or fp16, out of its type, dense, 8-byte aligned.
+ *   `workspace`: lrq_kv_attend_workspace bytes, 256-byte aligned, overwritten.
+ * The three below write a new table (dense [rows, width], -1 behind a row's pages) and
+ *   new lengths beside the ones they read, and count in refs: how many rows hold a page,
+ *   one that none holds (0 or below) being free.
+ * lrq_kv_fork: row r becomes row parents[r] as it was; r, and what is no row, stays.
+ * lrq_kv_resize: row r gets pages for wanted[r] tokens, or gives back what is behind
+ *   them (all of them: 0).  Pages are taken lowest first in the rows' order; a row that
+ *   grows from inside a page which others hold too gets a copy of it.  Where free
+ *   pages run out (after what this call gives back), rows from there on that need any
+ *   keep their length, and short_ (one int32) is how many were missing; so does a row
+ *   that wants more than `width` pages.
+ * lrq_kv_compact: the n pages in use become pages 0 .. n - 1: the k-th in use at or behind
+ *   n moves to the k-th free one before n.  count (one int32) is n.
+ */
+typedef struct lrq_kv_cache {
+  void *k, *v;
+  float *k_scales, *v_scales;
+  int32_t* refs;
+  int64_t layers, pages, kv_heads, page, dim;
+  int64_t k_layer, v_layer, ks_layer, vs_layer;
+  int64_t k_page, v_page, ks_page, vs_page;
+} lrq_kv_cache;
+int lrq_kv_append(const lrq_kv_cache* cache, int64_t layer, const void* k, int64_t k_token, int64_t k_head, const void* v,
+                  int64_t v_token, int64_t v_head, int dtype, int64_t tokens, const int32_t* table, int64_t ld, int64_t width,
+                  const int32_t* lengths, const int32_t* offsets, int64_t seqs, lrq_stream_t stream);
+int64_t lrq_kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs);
+int lrq_kv_attend(const lrq_kv_cache* cache, int64_t layer, const void* q, int64_t q_token, int64_t q_head, int dtype,
+                  int64_t tokens, int64_t heads, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
+                  const int32_t* offsets, int64_t seqs, float scale, int64_t window, int zero_rest, void* out, float* lse,
+                  void* workspace, int64_t workspace_bytes, lrq_stream_t stream);
+int lrq_kv_fork(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
+                int64_t rows, const int32_t* parents, int32_t* out_table, int32_t* out_lengths, lrq_stream_t stream);
+int64_t lrq_kv_resize_workspace(int64_t rows, int64_t pages);
+int lrq_kv_resize(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
+                  int64_t rows, const int32_t* wanted, int32_t* out_table, int32_t* out_lengths, int32_t* short_,
+                  void* workspace, int64_t workspace_bytes, lrq_stream_t stream);
+int64_t lrq_kv_compact_workspace(int64_t pages);
+int lrq_kv_compact(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, int64_t rows,
+                   int32_t* out_table, int32_t* count, void* workspace, int64_t workspace_bytes, lrq_stream_t stream);
+
+/*
  * Unscaled cast of n contiguous elements to float8_e4m3fn, as torch's
  * `tensor.to(torch.float8_e4m3fn)`: round to nearest even, |x| rounding past
  * 448, +-inf and NaN -> NaN (0x7F | sign).  Replaces the FP8 path of

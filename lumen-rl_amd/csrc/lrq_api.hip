@@ -864,6 +864,183 @@ int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, 
   return check_hip(lrq::launch_experts(a, x_dtype, tokens, workspace, (hipStream_t)stream), "kernel launch");
 }
 
+namespace {
+constexpr int64_t kKvTokens = int64_t(1) << 30;  // of a sequence, a call's rows, a table's cells
+int page_shift(int64_t page) { return page >= 16 && page <= 256 && (page & (page - 1)) == 0 ? __builtin_ctzll((uint64_t)page) : -1; }
+
+// a step between pages or layers that is never taken is not looked at
+bool step_ok(int64_t step, int64_t most, int64_t unit) { return most <= 1 || (step >= 0 && step <= int64_t(1) << 46 && step % unit == 0); }
+
+int check_kv_cache(const char* what, const lrq_kv_cache* c) {
+  if (!c) return fail(LRQ_ERR_ARG, "%s: no cache", what);
+  if (page_shift(c->page) < 0) return fail(LRQ_ERR_ARG, "%s: pages of %lld tokens (16, 32, 64, 128 or 256)", what, (long long)c->page);
+  if (c->dim < 16 || c->dim > 256 || c->dim % 16) return fail(LRQ_ERR_ARG, "%s: heads of %lld (a multiple of 16 up to 256)", what, (long long)c->dim);
+  if (c->kv_heads < 1 || c->kv_heads > 256) return fail(LRQ_ERR_ARG, "%s: %lld KV heads (1 to 256)", what, (long long)c->kv_heads);
+  if (c->pages < 1 || c->pages > int64_t(1) << 28) return fail(LRQ_ERR_ARG, "%s: %lld pages (1 to 2^28)", what, (long long)c->pages);
+  if (c->layers < 0 || c->layers > 65536) return fail(LRQ_ERR_ARG, "%s: %lld layers", what, (long long)c->layers);
+  if (c->layers > 0) {
+    if (!c->k || !c->v || !c->k_scales || !c->v_scales) return fail(LRQ_ERR_ARG, "%s: null pointer in the cache", what);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scales, 4) || !aligned(c->v_scales, 4))
+      return fail(LRQ_ERR_ALIGN, "%s: codes must be 16-byte aligned, scales element-aligned", what);
+    if (!step_ok(c->k_layer, c->layers, 16) || !step_ok(c->v_layer, c->layers, 16) || !step_ok(c->ks_layer, c->layers, 1) ||
+        !step_ok(c->vs_layer, c->layers, 1) || !step_ok(c->k_page, c->pages, 16) || !step_ok(c->v_page, c->pages, 16) ||
+        !step_ok(c->ks_page, c->pages, 1) || !step_ok(c->vs_page, c->pages, 1))
+      return fail(LRQ_ERR_ALIGN, "%s: steps of the cache must not be negative, those of codes multiples of 16", what);
+  }
+  return 0;
+}
+lrq::KvCache kv_layer(const lrq_kv_cache& c, int64_t layer) {
+  lrq::KvCache o{};
+  o.k = static_cast<uint8_t*>(c.k) + layer * c.k_layer, o.v = static_cast<uint8_t*>(c.v) + layer * c.v_layer;
+  o.ks = c.k_scales + layer * c.ks_layer, o.vs = c.v_scales + layer * c.vs_layer;
+  o.k_page = c.k_page, o.v_page = c.v_page, o.ks_page = c.ks_page, o.vs_page = c.vs_page;
+  o.pages = (int)c.pages, o.heads = (int)c.kv_heads, o.dim = (int)c.dim;
+  return o;
+}
+lrq::KvPool kv_pool(const lrq_kv_cache& c) {
+  lrq::KvPool o{};
+  o.k = static_cast<uint8_t*>(c.k), o.v = static_cast<uint8_t*>(c.v), o.ks = c.k_scales, o.vs = c.v_scales, o.refs = c.refs;
+  o.k_layer = c.k_layer, o.v_layer = c.v_layer, o.ks_layer = c.ks_layer, o.vs_layer = c.vs_layer;
+  o.k_page = c.k_page, o.v_page = c.v_page, o.ks_page = c.ks_page, o.vs_page = c.vs_page;
+  o.layers = c.layers, o.pages = (int)c.pages, o.heads = (int)c.kv_heads, o.dim = (int)c.dim, o.shift = page_shift(c.page);
+  return o;
+}
+int check_kv_table(const char* what, const void* table, int64_t ld, int64_t width, int64_t rows, int64_t page, bool null_ok) {
+  if (rows < 0 || rows > 1 << 20 || width < 0 || width * page > kKvTokens || rows * width > kKvTokens)
+    return fail(LRQ_ERR_ARG, "%s: a table of %lld rows and %lld pages (at most 2^20 rows, 2^30 tokens a row, 2^30 entries)", what,
+                (long long)rows, (long long)width);
+  if (rows > 0 && width > 0 && !null_ok) {
+    if (!table) return fail(LRQ_ERR_ARG, "%s: null pointer", what);
+    if (!aligned(table, 4)) return fail(LRQ_ERR_ALIGN, "%s: the table must be element-aligned", what);
+    if (rows > 1 && (ld < width || ld > int64_t(1) << 40)) return fail(LRQ_ERR_ARG, "%s: the table's rows overlap, or are too far apart", what);
+  }
+  return 0;
+}
+// the sequences of a call; > 0: nothing to do
+int check_kv_seqs(const char* what, const lrq_kv_cache* c, int64_t layer, int64_t tokens, const int32_t* table, int64_t ld,
+                  int64_t width, const int32_t* lengths, const int32_t* offsets, int64_t seqs, lrq::KvSeqs* out) {
+  if (int rc = check_kv_cache(what, c)) return rc;
+  if (layer < 0 || layer >= c->layers) return fail(LRQ_ERR_ARG, "%s: layer %lld of %lld", what, (long long)layer, (long long)c->layers);
+  if (tokens < 0 || tokens > 1 << 22) return fail(LRQ_ERR_ARG, "%s: %lld tokens (at most 2^22)", what, (long long)tokens);
+  if (int rc = check_kv_table(what, table, ld, width, seqs, c->page, false)) return rc;
+  if (!offsets && tokens < seqs) return fail(LRQ_ERR_ARG, "%s: %lld tokens of %lld sequences without offsets", what, (long long)tokens, (long long)seqs);
+  if (tokens == 0) return 1;
+  if (seqs > 0 && !lengths) return fail(LRQ_ERR_ARG, "%s: null pointer", what);
+  if (!aligned(lengths, 4) || !aligned(offsets, 4)) return fail(LRQ_ERR_ALIGN, "%s: lengths and offsets must be element-aligned", what);
+  *out = lrq::KvSeqs{table, lengths, offsets, ld, tokens, (int)seqs, (int)width, page_shift(c->page)};
+  return 0;
+}
+bool strides_ok(int64_t token, int64_t head, int64_t dim, int64_t tokens, int64_t heads) {
+  const int64_t most = int64_t(1) << 40;
+  return (tokens <= 1 || (token >= 0 && token <= most)) && (heads <= 1 || (head >= 0 && head <= most)) && dim > 0;
+}
+int check_kv_tables(const char* what, const lrq_kv_cache* c, const int32_t* table, int64_t ld, int64_t width,
+                    const int32_t* lengths, int64_t rows, const int32_t* out_table, lrq::KvTable* out) {
+  if (int rc = check_kv_cache(what, c)) return rc;
+  if (!c->refs || !aligned(c->refs, 4)) return fail(LRQ_ERR_ARG, "%s: no counts of the pages' rows", what);
+  if (int rc = check_kv_table(what, table, ld, width, rows, c->page, false)) return rc;
+  if (rows > 0 && width > 0 && (!out_table || !aligned(out_table, 4))) return fail(LRQ_ERR_ARG, "%s: no table to write", what);
+  if (rows > 0 && width > 0 && out_table < table + ((rows - 1) * ld + width) && table < out_table + rows * width)
+    return fail(LRQ_ERR_ARG, "%s: the new table must not overlap the old one", what);
+  *out = lrq::KvTable{table, lengths, ld, (int)rows, (int)width, page_shift(c->page)};
+  return 0;
+}
+}  // namespace
+
+int lrq_kv_append(const lrq_kv_cache* cache, int64_t layer, const void* k, int64_t k_token, int64_t k_head, const void* v,
+                  int64_t v_token, int64_t v_head, int dtype, int64_t tokens, const int32_t* table, int64_t ld, int64_t width,
+                  const int32_t* lengths, const int32_t* offsets, int64_t seqs, lrq_stream_t stream) {
+  g_err.clear();
+  lrq::KvAppendArgs a{};
+  const int rc = check_kv_seqs("kv_append", cache, layer, tokens, table, ld, width, lengths, offsets, seqs, &a.seqs);
+  if (rc) return rc > 0 ? 0 : rc;
+  if (!valid_dtype(dtype)) return fail(LRQ_ERR_ARG, "kv_append: bad dtype %d", dtype);
+  if (seqs == 0 || width == 0) return 0;
+  if (!k || !v) return fail(LRQ_ERR_ARG, "kv_append: null pointer");
+  if (!aligned(k, (uintptr_t)esize(dtype)) || !aligned(v, (uintptr_t)esize(dtype)))
+    return fail(LRQ_ERR_ALIGN, "kv_append: keys and values must be element-aligned");
+  if (!strides_ok(k_token, k_head, cache->dim, tokens, cache->kv_heads) || !strides_ok(v_token, v_head, cache->dim, tokens, cache->kv_heads))
+    return fail(LRQ_ERR_ARG, "kv_append: strides are negative, or too large");
+  if (lrq::kv_append_tiles(a.seqs) * cache->kv_heads >= int64_t(1) << 24)
+    return fail(LRQ_ERR_ARG, "kv_append: %lld tokens of %lld sequences and %lld heads are more than one launch takes", (long long)tokens,
+                (long long)seqs, (long long)cache->kv_heads);
+  a.cache = kv_layer(*cache, layer);
+  a.k = k, a.v = v, a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
+  return check_hip(lrq::launch_kv_append(a, dtype, (hipStream_t)stream), "kernel launch");
+}
+
+int64_t lrq_kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs) {
+  if (tokens < 0 || heads < 1 || kv_heads < 1 || seqs < 0 || dim < 16 || dim > 256) return 0;
+  return lrq::kv_attend_workspace(dim);
+}
+
+int lrq_kv_attend(const lrq_kv_cache* cache, int64_t layer, const void* q, int64_t q_token, int64_t q_head, int dtype,
+                  int64_t tokens, int64_t heads, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
+                  const int32_t* offsets, int64_t seqs, float scale, int64_t window, int zero_rest, void* out, float* lse,
+                  void* workspace, int64_t workspace_bytes, lrq_stream_t stream) {
+  g_err.clear();
+  lrq::KvAttendArgs a{};
+  const int rc = check_kv_seqs("kv_attend", cache, layer, tokens, table, ld, width, lengths, offsets, seqs, &a.seqs);
+  if (rc < 0) return rc;
+  if (dtype != lrq::kBF16 && dtype != lrq::kF16) return fail(LRQ_ERR_ARG, "kv_attend: bad dtype %d (bf16 or fp16)", dtype);
+  if (heads < 1 || heads > 4096 || heads % cache->kv_heads)
+    return fail(LRQ_ERR_ARG, "kv_attend: %lld query heads on %lld KV heads", (long long)heads, (long long)cache->kv_heads);
+  if (window < 0) return fail(LRQ_ERR_ARG, "kv_attend: window %lld", (long long)window);
+  if (rc > 0) return 0;
+  if (!q || !out) return fail(LRQ_ERR_ARG, "kv_attend: null pointer");
+  if (!aligned(q, 2) || !aligned(out, 8) || !aligned(lse, 4))
+    return fail(LRQ_ERR_ALIGN, "kv_attend: queries must be element-aligned, the result 8-byte aligned");
+  if (!strides_ok(q_token, q_head, cache->dim, tokens, heads)) return fail(LRQ_ERR_ARG, "kv_attend: strides are negative, or too large");
+  if (int err = check_workspace("kv_attend", workspace, workspace_bytes, lrq::kv_attend_workspace(cache->dim))) return err;
+  a.cache = kv_layer(*cache, layer);
+  a.q = q, a.q_token = q_token, a.q_head = q_head, a.out = out, a.lse = lse;
+  a.scale = scale * 1.44269504089f, a.heads = (int)heads, a.group = (int)(heads / cache->kv_heads);
+  a.window = window > kKvTokens ? 0 : (int)window, a.zero_rest = zero_rest != 0;
+  return check_hip(lrq::launch_kv_attend(a, dtype, workspace, (hipStream_t)stream), "kernel launch");
+}
+
+int lrq_kv_fork(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
+                int64_t rows, const int32_t* parents, int32_t* out_table, int32_t* out_lengths, lrq_stream_t stream) {
+  g_err.clear();
+  lrq::KvTable t{};
+  if (int rc = check_kv_tables("kv_fork", cache, table, ld, width, lengths, rows, out_table, &t)) return rc;
+  if (rows == 0) return 0;
+  if (!lengths || !parents || !out_lengths) return fail(LRQ_ERR_ARG, "kv_fork: null pointer");
+  if (out_lengths < lengths + rows && lengths < out_lengths + rows) return fail(LRQ_ERR_ARG, "kv_fork: the new lengths must not overlap the old ones");
+  return check_hip(lrq::launch_kv_fork(t, parents, cache->refs, (int)cache->pages, out_table, out_lengths, (hipStream_t)stream),
+                   "kernel launch");
+}
+
+int64_t lrq_kv_resize_workspace(int64_t rows, int64_t pages) {
+  return rows < 0 || pages < 1 ? 0 : lrq::kv_resize_workspace(rows, pages);
+}
+
+int lrq_kv_resize(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
+                  int64_t rows, const int32_t* wanted, int32_t* out_table, int32_t* out_lengths, int32_t* short_,
+                  void* workspace, int64_t workspace_bytes, lrq_stream_t stream) {
+  g_err.clear();
+  lrq::KvTable t{};
+  if (int rc = check_kv_tables("kv_resize", cache, table, ld, width, lengths, rows, out_table, &t)) return rc;
+  if (!short_ || (rows > 0 && (!lengths || !wanted || !out_lengths))) return fail(LRQ_ERR_ARG, "kv_resize: null pointer");
+  if (rows > 0 && out_lengths < lengths + rows && lengths < out_lengths + rows)
+    return fail(LRQ_ERR_ARG, "kv_resize: the new lengths must not overlap the old ones");
+  if (int rc = check_workspace("kv_resize", workspace, workspace_bytes, lrq::kv_resize_workspace(rows, cache->pages))) return rc;
+  return check_hip(lrq::launch_kv_resize(t, kv_pool(*cache), wanted, out_table, out_lengths, short_, workspace, (hipStream_t)stream),
+                   "kernel launch");
+}
+
+int64_t lrq_kv_compact_workspace(int64_t pages) { return pages < 1 ? 0 : lrq::kv_compact_workspace(pages); }
+
+int lrq_kv_compact(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, int64_t rows,
+                   int32_t* out_table, int32_t* count, void* workspace, int64_t workspace_bytes, lrq_stream_t stream) {
+  g_err.clear();
+  lrq::KvTable t{};
+  if (int rc = check_kv_tables("kv_compact", cache, table, ld, width, nullptr, rows, out_table, &t)) return rc;
+  if (!count) return fail(LRQ_ERR_ARG, "kv_compact: null pointer");
+  if (int rc = check_workspace("kv_compact", workspace, workspace_bytes, lrq::kv_compact_workspace(cache->pages))) return rc;
+  return check_hip(lrq::launch_kv_compact(t, kv_pool(*cache), out_table, count, workspace, (hipStream_t)stream), "kernel launch");
+}
+
 int lrq_cast_e4m3(const void* in, int in_dtype, int64_t n, uint8_t* out, lrq_stream_t stream) {
   g_err.clear();
   lrq_tensor t{in, out, nullptr, 1, 1, n, n, n};

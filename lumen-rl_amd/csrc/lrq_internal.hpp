@@ -338,6 +338,77 @@ struct ExpertArgs {
 int64_t experts_workspace(int64_t tokens, ExpertArgs a);
 hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspace, hipStream_t stream);
 
+// The FP8 KV cache (lrq_kv.hpp, lrq_kv_*.hip).
+struct KvCache {  // one layer: K [pages, heads, page, dim], V [pages, heads, dim, page]
+  uint8_t *k, *v;
+  float *ks, *vs;  // [pages, heads]
+  int64_t k_page, v_page, ks_page, vs_page;  // from page to page: bytes, and scales
+  int pages, heads, dim;
+};
+struct KvSeqs {
+  const int32_t* table;    // [seqs, width], row pitch ld
+  const int32_t* lengths;  // [seqs], with the new tokens
+  const int32_t* offsets;  // [seqs + 1], or null: one new token each
+  int64_t ld, tokens;
+  int seqs, width, shift;  // 2^shift tokens a page
+};
+struct KvAppendArgs {
+  KvCache cache;
+  KvSeqs seqs;
+  const void *k, *v;  // [tokens, heads, dim]
+  int64_t k_token, k_head, v_token, v_head;  // strides
+};
+int64_t kv_append_tiles(const KvSeqs& s);  // work-groups a head, at most
+hipError_t launch_kv_append(const KvAppendArgs& a, int dtype, hipStream_t stream);
+
+struct KvAttendArgs {
+  KvCache cache;
+  KvSeqs seqs;
+  const void* q;  // [tokens, heads, dim]
+  int64_t q_token, q_head;
+  void* out;   // the same, dense
+  float* lse;  // [tokens, heads], or null
+  float scale;  // times log2(e)
+  int heads, group, window;
+  bool zero_rest;  // rows behind the last sequence become 0
+  // workspace
+  uint8_t* heads_at;
+  float* sums;
+  int parts, least;
+};
+int64_t kv_attend_workspace(int64_t dim);
+hipError_t launch_kv_attend(KvAttendArgs a, int dtype, void* workspace, hipStream_t stream);
+
+struct KvTable {
+  const int32_t *table, *lengths;  // [rows, width], row pitch ld; [rows]
+  int64_t ld;
+  int rows, width, shift;
+};
+struct KvPool {  // all layers
+  uint8_t *k, *v;
+  float *ks, *vs;
+  int32_t* refs;  // [pages]
+  int64_t k_layer, v_layer, ks_layer, vs_layer, k_page, v_page, ks_page, vs_page;
+  int64_t layers;
+  int pages, heads, dim, shift;
+};
+struct KvPlan {  // of a resize or a compaction, in the workspace
+  int64_t* after;   // rows' needs, summed up to each
+  int32_t* need;    // negative: a copy among them
+  int32_t* pairs;   // pages to copy, from and to
+  int32_t* free;    // free pages; compact: pages' new numbers
+  int32_t* count;   // pairs; compact: pages in use, too
+  int64_t capacity;  // of `free`
+};
+int64_t kv_resize_workspace(int64_t rows, int64_t pages);
+int64_t kv_compact_workspace(int64_t pages);
+hipError_t launch_kv_fork(const KvTable& t, const int32_t* parents, int32_t* refs, int pages, int32_t* out, int32_t* out_len,
+                          hipStream_t stream);
+hipError_t launch_kv_resize(const KvTable& t, const KvPool& c, const int32_t* wanted, int32_t* out, int32_t* out_len,
+                            int32_t* out_short, void* workspace, hipStream_t stream);
+hipError_t launch_kv_compact(const KvTable& t, const KvPool& c, int32_t* out, int32_t* out_count, void* workspace,
+                             hipStream_t stream);
+
 // Diagnostics: element encoders applied to raw inputs.
 hipError_t launch_diag_e4m3_bits(uint32_t start, int64_t n, uint8_t* out, hipStream_t stream);
 hipError_t launch_diag_bf16_bits(uint32_t start, int64_t n, uint16_t* out, hipStream_t stream);

@@ -42,6 +42,14 @@ class LrqTensor(ctypes.Structure):
     ]
 
 
+class LrqKvCache(ctypes.Structure):
+    """Mirror of ``lrq_kv_cache`` in include/lrq.h."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scales", "v_scales", "refs")] + [
+        (n, ctypes.c_int64) for n in ("layers", "pages", "kv_heads", "page", "dim", "k_layer", "v_layer", "ks_layer", "vs_layer",
+                                      "k_page", "v_page", "ks_page", "vs_page")]
+
+
 # name -> (restype, argtypes); every symbol of include/lrq.h
 _VP, _I64, _CI, _CU = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_uint
 SIGNATURES = {
@@ -59,6 +67,15 @@ SIGNATURES = {
     "lrq_route_grad": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _CI, _CI, _CI, ctypes.c_float, _VP, _VP]),
     "lrq_fp8_experts_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "lrq_fp8_experts": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _VP, _VP, _VP, _I64, _I64, _VP, _VP, _I64, _VP]),
+    "lrq_kv_append": (_CI, [_VP, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _CI, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _VP]),
+    "lrq_kv_attend_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64]),
+    "lrq_kv_attend": (_CI, [_VP, _I64, _VP, _I64, _I64, _CI, _I64, _I64, _VP, _I64, _I64, _VP, _VP, _I64, ctypes.c_float, _I64, _CI,
+                            _VP, _VP, _VP, _I64, _VP]),
+    "lrq_kv_fork": (_CI, [_VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _VP]),
+    "lrq_kv_resize_workspace": (_I64, [_I64, _I64]),
+    "lrq_kv_resize": (_CI, [_VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _I64, _VP]),
+    "lrq_kv_compact_workspace": (_I64, [_I64]),
+    "lrq_kv_compact": (_CI, [_VP, _VP, _I64, _I64, _I64, _VP, _VP, _VP, _I64, _VP]),
     "lrq_cast_e4m3": (_CI, [_VP, _CI, _I64, _VP, _VP]),
     "lrq_mx_dequant": (_CI, [_CI, _VP, _VP, _I64, _I64, _VP, _CI, _VP]),
     "lrq_group_table_bytes": (_I64, [_CI, ctypes.POINTER(LrqTensor), _I64, _CI, _I64, _I64, _CU]),

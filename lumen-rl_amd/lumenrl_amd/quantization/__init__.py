@@ -11,6 +11,7 @@ from lumenrl_amd.quantization.fp8_config import (
 from lumenrl_amd.quantization.fp8_kv_cache import FP8KVCacheQuantizer
 from lumenrl_amd.quantization.fp8_product import fp8_block_linear, fp8_matmul
 from lumenrl_amd.quantization.fp8_rollout import FP8RolloutQuantizer
+from lumenrl_amd.quantization.kv_cache import FP8KVCache
 from lumenrl_amd.quantization.ops import (
     CopyPlan,
     DequantPlan,
@@ -27,6 +28,7 @@ __all__ = [
     "CopyPlan",
     "DequantPlan",
     "FP8Config",
+    "FP8KVCache",
     "FP8KVCacheQuantizer",
     "FP8RolloutQuantizer",
     "QuantizationConfig",

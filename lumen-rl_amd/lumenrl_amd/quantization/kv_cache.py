@@ -1,0 +1,318 @@
+"""The FP8 KV cache: paged keys and values in e4m3, attention over them, and their pages' upkeep.
+
+``FP8KVCache`` holds a model's pages.  Sequences are rows of a page table that the
+caller keeps: ``table`` int32 [rows, width] with a row's page numbers in order and
+``lengths`` int32 [rows].  A step of a rollout is
+
+    table, lengths, short = cache.resize(table, lengths, lengths + new)   # once
+    cache.append(layer, k, v, table, lengths, offsets)                    # in each layer
+    out = cache.attend(layer, q, table, lengths, offsets)
+
+and ``fork`` makes samples of a prompt share its pages, ``resize`` to 0 ends a sequence,
+``compact`` moves what is left together.  Everything runs on the current stream of the
+cache's device, reads lengths and tables there, and returns without synchronizing, so a
+step can be captured into a graph.  What tables, lengths and offsets hold is clamped to
+what there is: an entry that is no page of the pool is no page.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+from typing import Optional
+
+import torch
+from torch import Tensor
+from torch.autograd import forward_ad
+
+from lumenrl_amd import _lib
+from lumenrl_amd.quantization.fp8_product import NoGradient
+from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _dense, _on, _stream, require_device
+
+_STRIDE_MAX = 1 << 40
+
+
+@functools.lru_cache(maxsize=4096)
+def _attend_workspace(tokens: int, heads: int, kv_heads: int, dim: int, seqs: int) -> int:
+    return _lib.lib().lrq_kv_attend_workspace(tokens, heads, kv_heads, dim, seqs)
+
+
+@functools.lru_cache(maxsize=4096)
+def _resize_workspace(rows: int, pages: int) -> int:
+    return _lib.lib().lrq_kv_resize_workspace(rows, pages)
+
+
+@functools.lru_cache(maxsize=4096)
+def _compact_workspace(pages: int) -> int:
+    return _lib.lib().lrq_kv_compact_workspace(pages)
+
+
+def _steps(name: str, x: Tensor, inner: int) -> tuple[int, int]:
+    """Strides from layer to layer and page to page of a tensor whose other ``inner`` dims are dense."""
+    if x.numel() == 0:
+        return 0, 0
+    step = 1
+    for d in range(x.dim() - 1, x.dim() - 1 - inner, -1):
+        if x.shape[d] > 1 and x.stride(d) != step:
+            raise ValueError(f"FP8KVCache: a page of {name} must be dense, got strides {x.stride()}")
+        step *= x.shape[d]
+    if x.shape[1] > 1 and x.stride(1) < step:
+        raise ValueError(f"FP8KVCache: pages of {name} overlap (strides {x.stride()})")
+    return x.stride(0), x.stride(1)
+
+
+class FP8KVCache:
+    """Pages of keys and values in e4m3, with one power-of-two scale per page and KV head for each.
+
+    ``k`` [layers, pages, kv_heads, page, dim] and ``v`` [layers, pages, kv_heads, dim,
+    page] are float8_e4m3fn codes, ``k_scales`` and ``v_scales`` [layers, pages,
+    kv_heads] float32, ``refs`` [pages] int32: how many rows of the caller's table hold
+    each page; it is free where none does.  ``page`` is 16, 32, 64, 128 or 256, ``dim`` a multiple
+    of 16 up to 256.  The tensors are kept and written in place; layers and pages may be
+    views of larger ones, what a page holds is dense.
+    """
+
+    def __init__(self, k: Tensor, v: Tensor, k_scales: Tensor, v_scales: Tensor, refs: Tensor) -> None:
+        parts = {"k": (k, torch.float8_e4m3fn), "v": (v, torch.float8_e4m3fn), "k_scales": (k_scales, torch.float32),
+                 "v_scales": (v_scales, torch.float32), "refs": (refs, torch.int32)}
+        for name, (x, dtype) in parts.items():
+            if not isinstance(x, Tensor) or x.dtype != dtype:
+                raise TypeError(f"FP8KVCache: {name} must be a {dtype} tensor, got {x.dtype if isinstance(x, Tensor) else type(x)!r}")
+        for name, (x, _) in parts.items():
+            if not x.is_cuda or x.device != k.device:
+                raise ValueError(f"FP8KVCache: expected {name} on one HIP device, got {x.device}")
+        if k.dim() != 5:
+            raise ValueError(f"FP8KVCache: k must be [layers, pages, kv_heads, page, dim], got {tuple(k.shape)}")
+        self.layers, self.pages, self.kv_heads, self.page, self.dim = k.shape
+        if v.shape != (*k.shape[:3], self.dim, self.page):
+            raise ValueError(f"FP8KVCache: v must be {(*k.shape[:3], self.dim, self.page)}, got {tuple(v.shape)}")
+        if k_scales.shape != k.shape[:3] or v_scales.shape != k.shape[:3]:
+            raise ValueError(f"FP8KVCache: scales must be {tuple(k.shape[:3])}, got {tuple(k_scales.shape)} and {tuple(v_scales.shape)}")
+        if refs.shape != (self.pages,) or not refs.is_contiguous():
+            raise ValueError(f"FP8KVCache: refs must be a contiguous [{self.pages}], got {tuple(refs.shape)}")
+        if self.page not in (16, 32, 64, 128, 256) or self.dim % 16 or not 16 <= self.dim <= 256:
+            raise ValueError(f"FP8KVCache: pages of {self.page} tokens (16, 32, 64, 128 or 256) and heads of {self.dim} (a multiple of "
+                             "16 up to 256)")
+        if not 1 <= self.kv_heads <= 256 or not 1 <= self.pages <= 1 << 28 or self.layers > 65536:
+            raise ValueError(f"FP8KVCache: {self.layers} layers (at most 65536), {self.pages} pages (1 to 2^28), {self.kv_heads} KV heads "
+                             "(1 to 256)")
+        if k.numel() and (k.data_ptr() % 16 or v.data_ptr() % 16):
+            raise ValueError("FP8KVCache: k and v must be 16-byte aligned")
+        (kl, kp), (vl, vp) = _steps("k", k, 3), _steps("v", v, 3)
+        (ksl, ksp), (vsl, vsp) = _steps("k_scales", k_scales, 1), _steps("v_scales", v_scales, 1)
+        if any(s % 16 for s in (kl, kp, vl, vp)):
+            raise ValueError(f"FP8KVCache: strides of layers and pages must be multiples of 16, got {k.stride()} and {v.stride()}")
+        self.k, self.v, self.k_scales, self.v_scales, self.refs = k, v, k_scales, v_scales, refs
+        self.device = k.device
+        self._desc = _lib.LrqKvCache(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), refs.data_ptr(),
+                                     self.layers, self.pages, self.kv_heads, self.page, self.dim, kl, vl, ksl, vsl, kp, vp, ksp, vsp)
+        self._ref = ctypes.byref(self._desc)
+
+    @classmethod
+    def empty(cls, layers: int, pages: int, kv_heads: int, dim: int, *, page: int = 64,
+              device: Optional[torch.device] = None) -> "FP8KVCache":
+        """A cache with all pages free, on ``device`` (the current one by default)."""
+        device = require_device() if device is None else torch.device(device)
+        with torch.cuda.device(device):
+            k = torch.empty((layers, pages, kv_heads, page, dim), dtype=torch.float8_e4m3fn, device=device)
+            v = torch.empty((layers, pages, kv_heads, dim, page), dtype=torch.float8_e4m3fn, device=device)
+            ks, vs = (torch.ones((layers, pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2))
+            return cls(k, v, ks, vs, torch.zeros(pages, dtype=torch.int32, device=device))
+
+    # -- arguments ---------------------------------------------------------------
+    def _ints(self, what: str, name: str, x: Tensor, shape: tuple) -> Tensor:
+        if not isinstance(x, Tensor) or x.dtype != torch.int32:
+            raise TypeError(f"{what}: {name} must be an int32 tensor, got {x.dtype if isinstance(x, Tensor) else type(x)!r}")
+        if x.shape != shape or x.device != self.device:
+            raise ValueError(f"{what}: {name} must be {tuple(shape)} on {self.device}, got {tuple(x.shape)} on {x.device}")
+        return x if x.is_contiguous() else x.contiguous()
+
+    def _table(self, what: str, table: Tensor) -> tuple[Tensor, int, int, int]:
+        """(table, rows, width, row pitch); a copy only where its rows are not of unit stride."""
+        if not isinstance(table, Tensor) or table.dtype != torch.int32:
+            raise TypeError(f"{what}: table must be an int32 tensor, got {table.dtype if isinstance(table, Tensor) else type(table)!r}")
+        if table.dim() != 2 or table.device != self.device:
+            raise ValueError(f"{what}: table must be [rows, width] on {self.device}, got {tuple(table.shape)} on {table.device}")
+        rows, width = table.shape
+        ld = table.stride(0) if rows > 1 else width
+        if (width > 1 and table.stride(1) != 1) or not width <= ld <= _STRIDE_MAX:
+            table, ld = table.contiguous(), width
+        return table, rows, width, ld
+
+    def _layer(self, what: str, layer: int) -> int:
+        if not isinstance(layer, int) or not 0 <= layer < self.layers:
+            raise ValueError(f"{what}: layer {layer!r} of {self.layers}")
+        return layer
+
+    def _offsets(self, what: str, offsets: Optional[Tensor], rows: int, tokens: int) -> Optional[Tensor]:
+        if offsets is None:
+            if tokens < rows:
+                raise ValueError(f"{what}: {tokens} tokens of {rows} sequences need offsets")
+            return None
+        return self._ints(what, "offsets", offsets, (rows + 1,))
+
+    def _vectors(self, what: str, name: str, x: Tensor, heads: Optional[int]) -> Tensor:
+        """``x`` [tokens, heads, dim] with channels of unit stride."""
+        if x.dim() != 3 or x.shape[2] != self.dim or (heads is not None and x.shape[1] != heads) or x.device != self.device:
+            raise ValueError(f"{what}: {name} must be [tokens, {'heads' if heads is None else heads}, {self.dim}] on {self.device}, got "
+                             f"{tuple(x.shape)} on {x.device}")
+        return x if x.stride(2) == 1 and x.stride(0) <= _STRIDE_MAX and x.stride(1) <= _STRIDE_MAX else x.contiguous()
+
+    # -- tokens ------------------------------------------------------------------
+    def append(self, layer: int, k: Tensor, v: Tensor, table: Tensor, lengths: Tensor, offsets: Optional[Tensor] = None) -> None:
+        """Write new tokens' keys and values, ``k`` and ``v`` [tokens, kv_heads, dim] (bf16, fp16 or fp32).
+
+        Rows ``offsets[b]`` .. ``offsets[b + 1] - 1`` (int32 [rows + 1]) are the last
+        tokens of sequence b, whose ``lengths[b]`` counts them in already; without
+        ``offsets`` each sequence has one, and rows behind the last belong to none.  A
+        page's scale is the least power of two, from 2^-48 to 2^48, that takes the
+        largest finite magnitude to 448 at most.  Tokens that join a page never make its
+        scale smaller; where they make it larger, the codes that are there are rounded to
+        it again.  Infinities and NaN become NaN codes.  Tokens whose place has no page in
+        the table are not written.  No gradient: keys or values that want one are refused.
+        """
+        what = "FP8KVCache.append"
+        _check_input(k, what)
+        _check_input(v, what)
+        self._layer(what, layer)
+        k, v = self._vectors(what, "k", k, self.kv_heads), self._vectors(what, "v", v, self.kv_heads)
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError(f"{what}: k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} do not fit")
+        if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+            raise RuntimeError(f"{what} has no gradient; pass detached keys and values")
+        tokens = k.shape[0]
+        table, rows, width, ld = self._table(what, table)
+        lengths = self._ints(what, "lengths", lengths, (rows,))
+        offsets = self._offsets(what, offsets, rows, tokens)
+        dev = self.device
+        with _on(dev):
+            rc = _lib.lib().lrq_kv_append(self._ref, layer, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                          v.stride(1), _IN_DTYPES[k.dtype], tokens, table.data_ptr(), ld, width,
+                                          lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), rows, _stream(dev))
+        if rc:
+            _lib.check(rc, "lrq_kv_append")
+
+    def attend(self, layer: int, q: Tensor, table: Tensor, lengths: Tensor, offsets: Optional[Tensor] = None, *,
+               scale: Optional[float] = None, window: Optional[int] = None, out: Optional[Tensor] = None, return_lse: bool = False):
+        """Causal attention of new tokens over their sequences' keys: ``q`` [tokens, heads, dim] (bf16 or fp16) -> the same.
+
+        Tokens, ``lengths`` and ``offsets`` are as in ``append``, which goes before: a token
+        sees its sequence's keys up to its own, the last ``window`` of them if that is
+        given.  Query head i reads KV head ``i // (heads // kv_heads)``; ``scale`` is
+        ``dim ** -0.5`` by default.  Scores and sums are float32, probabilities are rounded
+        to fp16.  A token that sees no key gets 0; a NaN reaches the tokens that see it.
+        Rows of no sequence (behind the last one) are 0, in a given ``out`` (dense, of q's shape
+        and type) they stay as they are.  ``return_lse`` adds the scores' log-sum-exp,
+        float32 [tokens, heads] (-inf where nothing is seen).  No gradient: a backward
+        pass through the result raises.
+        """
+        what = "FP8KVCache.attend"
+        _check_input(q, what)
+        if q.dtype == torch.float32:
+            raise TypeError(f"{what}: q must be bf16 or fp16")
+        self._layer(what, layer)
+        q = self._vectors(what, "q", q, None)
+        tokens, heads = q.shape[:2]
+        if heads % self.kv_heads or not 1 <= heads <= 4096:
+            raise ValueError(f"{what}: {heads} query heads (at most 4096) on {self.kv_heads} KV heads")
+        if window is not None and window < 1:
+            raise ValueError(f"{what}: window must be at least 1, got {window}")
+        table, rows, width, ld = self._table(what, table)
+        lengths = self._ints(what, "lengths", lengths, (rows,))
+        offsets = self._offsets(what, offsets, rows, tokens)
+        if out is not None and (not isinstance(out, Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != self.device
+                                or not out.is_contiguous() or out.data_ptr() % 8):
+            raise ValueError(f"{what}: out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {self.device}, 8-byte aligned")
+        args = (layer, q, table, ld, lengths, offsets, self.dim ** -0.5 if scale is None else float(scale), window or 0, out, return_lse)
+        if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (q.requires_grad or out is not None and out.requires_grad):
+            if out is not None:
+                raise RuntimeError(f"{what} has no gradient; pass no out, or a detached q")
+            return NoGradient.apply(what, self._attend, *args)
+        return self._attend(*args)
+
+    def _attend(self, layer, q, table, ld, lengths, offsets, scale, window, out, return_lse):
+        dev = self.device
+        tokens, heads, dim = q.shape
+        rows, width = table.shape
+        given = out is not None
+        if not given:
+            out = _dense((tokens, heads, dim), q.dtype, dev)
+        lse = _dense((tokens, heads), torch.float32, dev) if return_lse else None
+        need = _attend_workspace(tokens, heads, self.kv_heads, dim, rows)
+        work = _dense((need,), torch.uint8, dev)
+        with _on(dev):
+            rc = _lib.lib().lrq_kv_attend(self._ref, layer, q.data_ptr(), q.stride(0), q.stride(1), _IN_DTYPES[q.dtype], tokens, heads,
+                                          table.data_ptr(), ld, width, lengths.data_ptr(),
+                                          None if offsets is None else offsets.data_ptr(), rows, scale, window, not given,
+                                          out.data_ptr(), None if lse is None else lse.data_ptr(), work.data_ptr(), need, _stream(dev))
+        if rc:
+            _lib.check(rc, "lrq_kv_attend")
+        return (out, lse) if return_lse else out
+
+    # -- pages -------------------------------------------------------------------
+    def fork(self, table: Tensor, lengths: Tensor, parents: Tensor) -> tuple[Tensor, Tensor]:
+        """Row r becomes row ``parents[r]`` (int32 [rows]) as it was: (new table, new lengths).
+
+        The two rows share their pages, which ``refs`` counts; what row r held before is
+        given back.  A row whose parent is itself, or no row, stays.  Entries behind a row's
+        pages are -1.  The page that a sequence ends in stays shared until ``resize`` lets
+        a row grow: resize before appending.
+        """
+        what = "FP8KVCache.fork"
+        table, rows, width, ld = self._table(what, table)
+        lengths = self._ints(what, "lengths", lengths, (rows,))
+        parents = self._ints(what, "parents", parents, (rows,))
+        dev = self.device
+        out, out_lengths = _dense((rows, width), torch.int32, dev), _dense((rows,), torch.int32, dev)
+        with _on(dev):
+            rc = _lib.lib().lrq_kv_fork(self._ref, table.data_ptr(), ld, width, lengths.data_ptr(), rows, parents.data_ptr(),
+                                        out.data_ptr(), out_lengths.data_ptr(), _stream(dev))
+        if rc:
+            _lib.check(rc, "lrq_kv_fork")
+        return out, out_lengths
+
+    def resize(self, table: Tensor, lengths: Tensor, wanted: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+        """Pages for ``wanted`` tokens (int32 [rows]) in each row: (new table, new lengths, short).
+
+        A row that shrinks gives back the pages behind its new end (all of them for 0).
+        Rows that grow take the lowest free pages, in the rows' order; one that grows from
+        inside a page which other rows hold too gets a copy of that page, in every layer.
+        Where free pages run out, counting what this call gives back, rows from there on that
+        need any keep their length, and ``short`` (int32, no dimension) says how many pages
+        were missing; a row that wants more than the table is wide keeps its length as well.
+        Entries behind a row's pages are -1.
+        """
+        what = "FP8KVCache.resize"
+        table, rows, width, ld = self._table(what, table)
+        lengths = self._ints(what, "lengths", lengths, (rows,))
+        wanted = self._ints(what, "wanted", wanted, (rows,))
+        dev = self.device
+        out, out_lengths = _dense((rows, width), torch.int32, dev), _dense((rows,), torch.int32, dev)
+        short = _dense((), torch.int32, dev)
+        need = _resize_workspace(rows, self.pages)
+        work = _dense((need,), torch.uint8, dev)
+        with _on(dev):
+            rc = _lib.lib().lrq_kv_resize(self._ref, table.data_ptr(), ld, width, lengths.data_ptr(), rows, wanted.data_ptr(),
+                                          out.data_ptr(), out_lengths.data_ptr(), short.data_ptr(), work.data_ptr(), need, _stream(dev))
+        if rc:
+            _lib.check(rc, "lrq_kv_resize")
+        return out, out_lengths, short
+
+    def compact(self, table: Tensor) -> tuple[Tensor, Tensor]:
+        """Move the pages in use together: (new table, their number n as an int32 without dimensions).
+
+        Afterwards pages 0 .. n - 1 are in use.  The k-th page in use at or behind n moves,
+        in every layer, to the k-th free one before n; ``refs`` follows.
+        """
+        what = "FP8KVCache.compact"
+        table, rows, width, ld = self._table(what, table)
+        dev = self.device
+        out, count = _dense((rows, width), torch.int32, dev), _dense((), torch.int32, dev)
+        need = _compact_workspace(self.pages)
+        work = _dense((need,), torch.uint8, dev)
+        with _on(dev):
+            rc = _lib.lib().lrq_kv_compact(self._ref, table.data_ptr(), ld, width, rows, out.data_ptr(), count.data_ptr(),
+                                           work.data_ptr(), need, _stream(dev))
+        if rc:
+            _lib.check(rc, "lrq_kv_compact")
+        return out, count

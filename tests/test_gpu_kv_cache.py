@@ -1,0 +1,744 @@
+"""``FP8KVCache``: appends, attention and pages against the rules in float64 (kv_rules)."""
+
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+import torch
+
+import kv_rules as R
+from lumenrl_amd.quantization import FP8KVCache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def make(layers, pages, heads, dim, page, seed=0, spread=6):
+    """A cache of random codes, each page and head with a scale of its own."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    c = FP8KVCache.empty(layers, pages, heads, dim, page=page)
+    for x in (c.k, c.v):
+        x.copy_((torch.randn(x.shape, generator=g, device=DEV) * 60).clamp(-448, 448))
+    for s in (c.k_scales, c.v_scales):
+        s.copy_((torch.randint(-spread, 1, s.shape, generator=g, device=DEV) - 4 + 127 << 23).int().view(torch.float32))
+    return c
+
+
+def batch(new, prior, page, extra=2):
+    lengths = [a + b for a, b in zip(new, prior)]
+    offsets = [0]
+    for n in new:
+        offsets.append(offsets[-1] + n)
+    width = max([R.pages_of(n, page) for n in lengths] + [0]) + extra
+    return lengths, offsets, width
+
+
+def queries(tokens, heads, dim, dtype, seed=1, size=2.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(tokens, heads, dim, generator=g, device=DEV) * size).to(dtype)
+
+
+def close(got, want, bound, name=""):
+    err = (got.double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bool(bad.any()), (name, int(bad.sum()), float((err / bound.clamp_min(1e-300))[bad].max()), bad.nonzero()[:4].tolist())
+
+
+# ---------------------------------------------------------------------------
+# attend
+# ---------------------------------------------------------------------------
+ATTEND = [
+    # dtype, heads, kv heads, dim, page, new, prior, window
+    (torch.bfloat16, 32, 8, 128, 64, [1], [0], 0),
+    (torch.bfloat16, 32, 8, 128, 64, [1, 1, 1, 1], [63, 64, 65, 1000], 0),
+    (torch.float16, 8, 8, 64, 16, [1, 1, 1], [0, 15, 300], 0),
+    (torch.bfloat16, 10, 2, 128, 32, [1, 0, 3, 5], [700, 12, 0, 31], 0),
+    (torch.float16, 7, 1, 80, 128, [4, 1, 2], [127, 128, 500], 0),
+    (torch.bfloat16, 24, 1, 48, 256, [1, 2], [900, 255], 0),
+    (torch.bfloat16, 4, 4, 256, 64, [1, 2, 1], [200, 63, 0], 0),
+    (torch.float16, 6, 2, 192, 32, [1, 9], [77, 40], 0),
+    (torch.bfloat16, 2, 1, 16, 16, [1, 3], [100, 14], 0),
+    (torch.bfloat16, 8, 2, 112, 64, [17, 1, 40], [5, 0, 100], 0),
+    (torch.bfloat16, 8, 2, 128, 64, [1, 1, 3, 70], [400, 63, 200, 90], 64),
+    (torch.float16, 14, 2, 64, 32, [5, 0, 1, 2], [1200, 7, 33, 0], 1),
+    (torch.bfloat16, 4, 2, 128, 64, [130, 3], [0, 777], 100),
+    (torch.float16, 8, 1, 128, 64, [200, 33], [130, 0], 0),
+    (torch.bfloat16, 16, 2, 64, 16, [150, 1, 64, 0, 129], [37, 300, 0, 5, 64], 0),
+    (torch.bfloat16, 5, 1, 96, 64, [260], [1], 0),
+    (torch.float16, 4, 1, 256, 128, [140, 70], [60, 300], 50),
+    (torch.bfloat16, 40, 1, 128, 64, [1, 50], [500, 3], 0),
+]
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,page,new,prior,window", ATTEND)
+def test_attend_is_the_definition(dtype, heads, kv, dim, page, new, prior, window):
+    lengths, offsets, width = batch(new, prior, page)
+    pool = sum(R.pages_of(n, page) for n in lengths) + 3
+    c = make(2, pool, kv, dim, page)
+    table = R.spread_table(lengths, page, width, pool, 3)
+    q = queries(offsets[-1], heads, dim, dtype)
+    out, lse = c.attend(1, q, ints(table), ints(lengths), ints(offsets), window=window or None, return_lse=True)
+    want, bound, wl = R.attend(c, 1, q, table, lengths, offsets, dim ** -0.5, window)
+    close(out, want, bound)
+    # the log-sum-exp: the scores' error, and float32's own
+    assert bool(((lse.double() - wl).abs() <= 1e-4 + 2e-6 * wl.abs()).logical_or(lse.double() == wl).all())
+    if all(n == 1 for n in new):
+        assert torch.equal(c.attend(1, q, ints(table), ints(lengths), window=window or None), out)
+
+
+def test_attend_of_many_sequences_and_long_ones():
+    """More sequences than a work-group has threads, one of them a hundred times as long as the others."""
+    page, kv, dim = 64, 2, 128
+    new, prior = [1] * 700, [(37 * i) % 150 for i in range(700)]
+    prior[411] = 20000
+    lengths, offsets, width = batch(new, prior, page)
+    pool = sum(R.pages_of(n, page) for n in lengths)
+    c = make(1, pool, kv, dim, page)
+    table = R.spread_table(lengths, page, width, pool, 4)
+    q = queries(700, 8, dim, torch.bfloat16)
+    out = c.attend(0, q, ints(table), ints(lengths), ints(offsets))
+    assert torch.equal(out, c.attend(0, q, ints(table), ints(lengths)))
+    some = [0, 1, 255, 256, 257, 410, 411, 412, 699]
+    want, bound, _ = R.attend(c, 0, q[some], [table[i] for i in some], [lengths[i] for i in some], None, dim ** -0.5, 0)
+    close(out[some], want, bound)
+
+
+def test_attend_flat_and_peaked_probabilities():
+    """All keys alike: p is 1 / n for 30000 keys; then one key 60 above all others."""
+    page, dim, n = 64, 64, 30000
+    pool = R.pages_of(n, page)
+    c = make(1, pool, 1, dim, page, spread=0)
+    table = [list(range(pool))]
+    q = torch.zeros(1, 1, dim, dtype=torch.bfloat16, device=DEV)
+    out = c.attend(0, q, ints(table), ints([n]))
+    want, bound, _ = R.attend(c, 0, q, table, [n], None, dim ** -0.5, 0)
+    close(out, want, bound)
+    q = queries(1, 1, dim, torch.bfloat16, size=40.0)
+    out = c.attend(0, q, ints(table), ints([n]))
+    want, bound, _ = R.attend(c, 0, q, table, [n], None, dim ** -0.5, 0)
+    close(out, want, bound)
+
+
+def test_attend_scales_far_apart():
+    """Pages whose V is 2^30 times that of others, or all 0, and K of many sizes: nothing overflows, nothing small gets lost in the sum of p."""
+    page, dim = 16, 64
+    c = make(1, 40, 1, dim, page, spread=0)
+    for i in range(40):
+        c.v_scales[0, i] = 2.0 ** (-48 if i % 4 == 0 else -10 if i % 4 == 1 else 20 if i == 38 else -5)
+        c.k_scales[0, i] = 2.0 ** (-40 if i % 3 == 0 else -9)
+    c.v[0, 5].zero_()
+    c.v_scales[0, 5] = 2.0 ** -48
+    table, lengths = [list(range(40))], [633]
+    for dtype in (torch.bfloat16, torch.float16):
+        q = queries(1, 4, dim, dtype, size=0.5)
+        for n in (633, 600):  # with and without the page of 2^20
+            out = c.attend(0, q, ints(table), ints([n]))
+            want, bound, _ = R.attend(c, 0, q, table, [n], None, dim ** -0.5, 0)
+            if dtype == torch.float16 and n == 633:
+                assert float(want.abs().max()) < 6e6
+                keep = want.abs() < 60000
+                close(out[keep], want[keep], bound[keep])
+            else:
+                close(out, want, bound)
+
+
+def test_attend_strided_queries_out_lse_and_scale():
+    page, dim, heads = 64, 128, 8
+    new, prior = [3, 1, 20], [100, 64, 11]
+    lengths, offsets, width = batch(new, prior, page)
+    c = make(1, 12, 2, dim, page)
+    table = R.spread_table(lengths, page, width, 12, 5)
+    wide = queries(offsets[-1] + 2, heads + 3, dim + 16, torch.bfloat16)
+    q = wide[1: offsets[-1] + 1, 2: 2 + heads, 5: 5 + dim]  # an odd start
+    want, bound, _ = R.attend(c, 0, q, table, lengths, offsets, 0.3, 0)
+    close(c.attend(0, q, ints(table), ints(lengths), ints(offsets), scale=0.3), want, bound)
+    turned = q.transpose(0, 1).contiguous().transpose(0, 1)
+    close(c.attend(0, turned, ints(table), ints(lengths), ints(offsets), scale=0.3), want, bound)
+    # a table that is a view, of rows further apart
+    big = torch.full((3, 2 * width), 7, dtype=torch.int32, device=DEV)
+    big[:, :width] = ints(table)
+    close(c.attend(0, q, big[:, :width], ints(lengths), ints(offsets), scale=0.3), want, bound)
+    close(c.attend(0, q, ints(table).t().contiguous().t(), ints(lengths), ints(offsets), scale=0.3), want, bound)
+
+
+def test_attend_rows_behind_the_last_sequence():
+    page, dim = 64, 64
+    c = make(1, 8, 1, dim, page)
+    table, lengths, offsets = [[3, 1], [2, -1]], [100, 5], [0, 2, 3]
+    q = queries(9, 4, dim, torch.bfloat16)
+    want, bound, wl = R.attend(c, 0, q, table, lengths, offsets, dim ** -0.5, 0)
+    out, lse = c.attend(0, q, ints(table), ints(lengths), ints(offsets), return_lse=True)
+    close(out, want, bound)
+    assert bool((out[3:] == 0).all()) and bool((lse[3:] == -math.inf).all())
+    mine = torch.full_like(q, 7.0)
+    assert c.attend(0, q, ints(table), ints(lengths), ints(offsets), out=mine) is mine
+    assert torch.equal(mine[:3], out[:3]) and bool((mine[3:] == 7.0).all())
+    # without offsets, too, and with no sequence at all
+    out = c.attend(0, q, ints(table), ints(lengths))
+    assert bool((out[2:] == 0).all()) and not bool((out[:2] == 0).any())
+    out = c.attend(0, q, ints(table)[:0], ints([]), ints([0]))
+    assert bool((out == 0).all())
+    assert c.attend(0, q[:0], ints(table), ints(lengths), ints([0, 0, 0])).shape == (0, 4, dim)
+
+
+def test_attend_rows_that_see_nothing():
+    """A length of 0, more new tokens than the length, and pages that are none."""
+    page, dim = 16, 64
+    c = make(1, 8, 2, dim, page)
+    table = [[3, 1, 2], [4, 5, 6], [0, 99, -7], [-1, -1, -1]]
+    lengths, offsets = [0, 2, 48, 40], [0, 1, 6, 9, 10]
+    q = queries(10, 4, dim, torch.bfloat16)
+    out, lse = c.attend(0, q, ints(table), ints(lengths), ints(offsets), return_lse=True)
+    want, bound, wl = R.attend(c, 0, q, table, lengths, offsets, dim ** -0.5, 0)
+    close(out, want, bound)
+    nothing = wl == -math.inf
+    assert int(nothing.sum()) == 4 * (1 + 3 + 1)
+    assert bool((out[nothing] == 0).all()) and bool((lse[nothing] == -math.inf).all())
+    # lengths and offsets that are out of range are clamped
+    got = c.attend(0, q, ints(table), ints([-5, 2, 2 ** 31 - 1, 40]), ints([0, 1, 6, 9, 2 ** 31 - 1]))
+    want, bound, _ = R.attend(c, 0, q, table, [0, 2, 48, 40], offsets, dim ** -0.5, 0)
+    close(got, want, bound)
+
+
+@pytest.mark.parametrize("new,window", [([1], 0), ([1], 20), ([6], 0), ([6], 20), ([150], 0), ([150], 33)])
+def test_nan_reaches_only_those_who_see_it(new, window):
+    page, dim, kv, heads = 32, 64, 1, 4
+    lengths, offsets, width = batch(new, [200], page)
+    pool = 16
+    c = make(1, pool, kv, dim, page, spread=0)
+    table = R.spread_table(lengths, page, width, pool, 6)
+    n = lengths[0]
+    # everything that is not the sequence's is NaN, in codes and in scales
+    used = set(table[0])
+    for p in range(pool):
+        if p not in used:
+            c.k.view(torch.uint8)[0, p] = 0x7F
+            c.v.view(torch.uint8)[0, p] = 0xFF
+            c.k_scales[0, p] = c.v_scales[0, p] = math.nan
+    last = table[0][(n - 1) // page]
+    if n % page:
+        c.k.view(torch.uint8)[0, last, :, n % page:] = 0x7F
+        c.v.view(torch.uint8)[0, last, :, :, n % page:] = 0x7F
+    q = queries(new[0], heads, dim, torch.bfloat16)
+    want, bound, _ = R.attend(c, 0, q, table, lengths, offsets, dim ** -0.5, window)
+    out = c.attend(0, q, ints(table), ints(lengths), ints(offsets), window=window or None)
+    close(out, want, bound)
+
+    def place(j):
+        return table[0][j // page], j % page
+
+    # a NaN of V at the last key, and at one that a window leaves behind: only that channel, only for those who see it
+    for j, value in ((n - 1, 0xFF), (n - 1 - max(1, new[0] // 2), 0x7F), (150, 0x7F)):
+        p, slot = place(j)
+        keep = c.v.view(torch.uint8)[0, p, 0, 5, slot].clone()
+        c.v.view(torch.uint8)[0, p, 0, 5, slot] = value
+        out = c.attend(0, q, ints(table), ints(lengths), ints(offsets), window=window or None)
+        for i in range(new[0]):
+            pos = n - new[0] + i
+            sees = j <= pos and (not window or j > pos - window)
+            assert bool(out[i, :, 5].isnan().all()) == sees and bool(out[i, :, 5].isnan().any()) == sees, (j, i)
+        rest = torch.ones(dim, dtype=torch.bool, device=DEV)
+        rest[5] = False
+        close(out[:, :, rest], want[:, :, rest], bound[:, :, rest])
+        c.v.view(torch.uint8)[0, p, 0, 5, slot] = keep
+    # a NaN of K: the whole row of those who see it
+    for j in (n - 1, n - 1 - new[0] // 2, 150):
+        p, slot = place(j)
+        keep = c.k.view(torch.uint8)[0, p, 0, slot, 9].clone()
+        c.k.view(torch.uint8)[0, p, 0, slot, 9] = 0x7F
+        out = c.attend(0, q, ints(table), ints(lengths), ints(offsets), window=window or None)
+        for i in range(new[0]):
+            pos = n - new[0] + i
+            sees = j <= pos and (not window or j > pos - window)
+            assert bool(out[i].isnan().all()) == sees and bool(out[i].isnan().any()) == sees, (j, i)
+            if not sees:
+                close(out[i], want[i], bound[i])
+        c.k.view(torch.uint8)[0, p, 0, slot, 9] = keep
+    # and one of a query: its own row
+    q[0, 2, 3] = math.nan
+    out = c.attend(0, q, ints(table), ints(lengths), ints(offsets), window=window or None)
+    assert bool(out[0, 2].isnan().all())
+    out[0, 2] = want[0, 2]
+    close(out, want, bound)
+
+
+def test_cache_beyond_four_gigabytes():
+    """Pages whose codes lie behind 2^32 bytes, in K and in V; and views of a larger pool with steps of their own."""
+    page, dim, kv = 64, 128, 8
+    pool = (1 << 32) // (page * dim * kv) + 40
+    k = torch.zeros((1, pool, kv, page, dim), dtype=torch.uint8, device=DEV).view(R.E4M3)
+    v = torch.zeros((1, pool, kv, dim, page), dtype=torch.uint8, device=DEV).view(R.E4M3)
+    c = FP8KVCache(k, v, torch.ones(1, pool, kv, device=DEV), torch.ones(1, pool, kv, device=DEV), torch.zeros(pool, dtype=torch.int32, device=DEV))
+    table = [[pool - 1, pool - 3, 2], [pool - 8, 0, -1]]
+    lengths, offsets = [150, 70], [0, 150, 220]
+    g = torch.Generator(device=DEV).manual_seed(0)
+    kn, vn = (torch.randn(220, kv, dim, generator=g, device=DEV).bfloat16() for _ in range(2))
+    c.append(0, kn, vn, ints(table), ints(lengths), ints(offsets))
+    idx = [pool - 1, pool - 3, 2, pool - 8, 0]
+    small = FP8KVCache(c.k[:, idx].contiguous(), c.v[:, idx].contiguous(), c.k_scales[:, idx].contiguous(), c.v_scales[:, idx].contiguous(),
+                       torch.zeros(5, dtype=torch.int32, device=DEV))
+    back = [[0, 1, 2], [3, 4, -1]]
+    lone = FP8KVCache.empty(1, 5, kv, dim, page=page)
+    lone.k.view(torch.uint8).zero_(), lone.v.view(torch.uint8).zero_()
+    lone.append(0, kn, vn, ints(back), ints(lengths), ints(offsets))
+    assert torch.equal(lone.k.view(torch.uint8), small.k.view(torch.uint8)) and torch.equal(lone.v.view(torch.uint8), small.v.view(torch.uint8))
+    q = queries(2, 16, dim, torch.bfloat16)
+    assert torch.equal(c.attend(0, q, ints(table), ints(lengths)), small.attend(0, q, ints(back), ints(lengths)))
+    # upkeep there: two rows grow from a shared page, and everything moves down
+    c.refs[[pool - 1, pool - 3, 2, pool - 8, 0]] = 1
+    t, n = c.fork(ints(table + [[-1] * 3]), ints(lengths + [0]), ints([0, 1, 1]))
+    t, n, short = c.resize(t, n, ints([150, 70, 100]))
+    assert t.tolist() == [[pool - 1, pool - 3, 2], [pool - 8, 0, -1], [pool - 8, 1, -1]] and int(short) == 0
+    t, count = c.compact(t)
+    assert int(count) == 6
+    out = c.attend(0, torch.cat([q, q[1:]]), t, ints([150, 70, 70]))
+    want = small.attend(0, q, ints(back), ints(lengths))
+    assert torch.equal(out[:2], want) and torch.equal(out[2], want[1])
+
+
+def test_views_of_a_larger_pool():
+    """K, V and scales of a layer side by side: steps from page to page are larger than a page."""
+    page, dim, kv, pool = 32, 48, 3, 9
+    raw = torch.zeros(2, pool, 3, kv * page * dim, dtype=torch.uint8, device=DEV)
+    k = raw[:, :, 0].view(2, pool, kv, page, dim).view(R.E4M3)
+    v = raw[:, :, 2].view(2, pool, kv, dim, page).view(R.E4M3)
+    scales = torch.ones(2, pool, 4, kv, device=DEV)
+    c = FP8KVCache(k, v, scales[:, :, 1], scales[:, :, 3], torch.zeros(pool, dtype=torch.int32, device=DEV))
+    d = FP8KVCache.empty(2, pool, kv, dim, page=page)
+    for x in (d.k, d.v):
+        x.view(torch.uint8).zero_()
+    lengths, offsets = [50, 33], [0, 50, 83]
+    table = [[4, 7], [0, 2]]
+    kn, vn = queries(83, kv, dim, torch.bfloat16, 1), queries(83, kv, dim, torch.bfloat16, 2)
+    q = queries(2, 6, dim, torch.bfloat16, 3)
+    outs = []
+    for cache in (c, d):
+        cache.refs[[4, 7, 0, 2]] = 1
+        cache.append(1, kn, vn, ints(table), ints(lengths), ints(offsets))
+        t, n = cache.fork(ints(table), ints(lengths), ints([0, 0]))
+        t, n, _ = cache.resize(t, n, ints([60, 51]))
+        t, count = cache.compact(t)
+        outs.append((cache.attend(1, q, t, ints([50, 50])), t, n, count))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert torch.equal(c.k_scales, d.k_scales) and torch.equal(c.v.view(torch.uint8), d.v.view(torch.uint8))
+    assert bool((raw[:, :, 1] == 0).all()) and bool((scales[:, :, [0, 2]] == 1).all())
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+APPEND = [
+    (torch.bfloat16, 2, 128, 64, [1, 1, 1], [0, 5, 64]),
+    (torch.bfloat16, 3, 64, 16, [40, 0, 7, 1], [3, 9, 16, 15]),
+    (torch.float16, 1, 80, 32, [100, 31, 33], [0, 1, 31]),
+    (torch.float32, 2, 16, 128, [129, 1, 5], [100, 127, 0]),
+    (torch.bfloat16, 1, 256, 256, [300, 2], [17, 255]),
+    (torch.float16, 8, 48, 64, [64, 65, 63, 128], [64, 0, 1, 10]),
+]
+
+
+@pytest.mark.parametrize("dtype,kv,dim,page,new,prior", APPEND)
+def test_append_is_the_rule(dtype, kv, dim, page, new, prior):
+    lengths, offsets, width = batch(new, prior, page)
+    pool = sum(R.pages_of(n, page) for n in lengths) + 2
+    c = make(2, pool, kv, dim, page)
+    table = R.spread_table(lengths, page, width, pool, 7)
+    want = R.Cache(c)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    # sizes from far below to far above what the pages hold
+    k, v = ((torch.randn(offsets[-1], kv, dim, generator=g, device=DEV)
+             * torch.randint(-12, 9, (offsets[-1], kv, 1), generator=g, device=DEV).float().exp2()).to(dtype) for _ in range(2))
+    c.append(1, k, v, ints(table), ints(lengths), ints(offsets))
+    want.append(1, k, v, table, lengths, offsets)
+    want.same(c)
+    # once more with the same tokens: nothing changes, as scales already take them
+    c.append(1, k, v, ints(table), ints(lengths), ints(offsets))
+    want.append(1, k, v, table, lengths, offsets)
+    want.same(c)
+    if new == [1] * len(new):
+        c.append(1, v, k, ints(table), ints(lengths))
+        want.append(1, v, k, table, lengths, None)
+        want.same(c)
+
+
+def test_append_values_at_the_borders():
+    """Zeros, subnormals, the largest values, infinities and NaN; amax on either side of 448 x 2^e."""
+    page, dim = 16, 16
+    tops = [0.0, 448.0, 449.0, 1e-45, 2.0 ** -126, 448.0 * 2.0 ** -48, 449.0 * 2.0 ** -48, 448.0 * 2.0 ** 48, 3.0e38, 1.75 * 2.0 ** -40, math.inf, math.nan]
+    c = make(1, len(tops), 1, dim, page)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    k = torch.rand(page * len(tops), 1, dim, generator=g, device=DEV) * 2 - 1
+    for i, t in enumerate(tops):
+        part = k[page * i: page * (i + 1)]
+        if math.isfinite(t):
+            part *= t
+        part[3, 0, 2] = t
+        part[4, 0, 5] = -t
+    table = [[i] for i in range(len(tops))]
+    lengths, offsets = [page] * len(tops), [page * i for i in range(len(tops) + 1)]
+    want = R.Cache(c)
+    c.append(0, k, k.flip(0), ints(table), ints(lengths), ints(offsets))
+    want.append(0, k, k.flip(0), table, lengths, offsets)
+    want.same(c)
+    assert bool(c.k[0, 10, 0, 3, 2].float().isnan()) and bool(c.k_scales[0, 10, 0] == 2.0 ** -8)
+    # a page's codes through ever larger scales, one token at a time
+    d = make(1, 1, 1, dim, page)
+    rule = R.Cache(d)
+    for i in range(page):
+        x = torch.randn(1, 1, dim, generator=g, device=DEV) * 3.0 ** (i - 4)
+        d.append(0, x, -x, ints([[0]]), ints([i + 1]))
+        rule.append(0, x, -x, [[0]], [i + 1], None)
+        rule.same(d)
+
+
+def test_append_strided_and_out_of_range():
+    page, dim, kv = 32, 64, 2
+    c = make(1, 6, kv, dim, page)
+    wide = queries(40, 3 * kv + 1, dim + 8, torch.bfloat16)
+    k, v = wide[2:32, 1: 1 + kv, 3: 3 + dim], wide[2:32].transpose(0, 1)[kv + 1: 2 * kv + 1].transpose(0, 1)[..., 8:]
+    table = [[1, 99], [-1, 3], [4, 5], [0, 2]]
+    lengths, offsets = [40, 36, 3, 2 ** 31 - 1], [0, 10, 20, 26, 30]  # the third has three places for six tokens, the fourth ends at 64
+    want = R.Cache(c)
+    c.append(0, k, v, ints(table), ints(lengths), ints(offsets))
+    want.append(0, k, v, table, lengths, offsets)
+    want.same(c)
+    c.append(0, k[:0], v[:0], ints(table), ints(lengths), ints([0, 0, 0, 0, 0]))
+    c.append(0, k, v, ints(table)[:0], ints([]), ints([0]))
+    want.same(c)
+    # tokens behind the last sequence, with and without offsets
+    c.append(0, k, v, ints(table)[:2], ints([4, 36]), ints([0, 2, 3]))
+    want.append(0, k, v, table[:2], [4, 36], [0, 2, 3])
+    want.same(c)
+    c.append(0, k, v, ints(table)[:2], ints([5, 37]))
+    want.append(0, k, v, table[:2], [5, 37], None)
+    want.same(c)
+
+
+def test_append_of_many_sequences():
+    page, dim, kv = 16, 32, 1
+    new = [(5 * i) % 4 for i in range(900)]
+    lengths, offsets, width = batch(new, [(7 * i) % 30 for i in range(900)], page)
+    pool = sum(R.pages_of(n, page) for n in lengths)
+    c = make(1, pool, kv, dim, page)
+    table = R.spread_table(lengths, page, width, pool, 11)
+    want = R.Cache(c)
+    k, v = queries(offsets[-1], kv, dim, torch.float16, 1), queries(offsets[-1], kv, dim, torch.float16, 2)
+    c.append(0, k, v, ints(table), ints(lengths), ints(offsets))
+    want.append(0, k, v, table, lengths, offsets)
+    want.same(c)
+
+
+# ---------------------------------------------------------------------------
+# pages
+# ---------------------------------------------------------------------------
+def held(c, table, lengths):
+    refs = [0] * c.pages
+    for row, n in zip(table, lengths):
+        for p in row[: R.pages_of(n, c.page)]:
+            refs[p] += 1
+    c.refs.copy_(ints(refs))
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_pages_through_random_steps(seed):
+    """Forks, growth, ends and compactions in turn, each against the rule, with pools that run out."""
+    rnd = random.Random(seed)
+    page, rows, width = rnd.choice([16, 32, 64]), rnd.choice([1, 7, 40]), 6
+    pool = rnd.choice([3, rows, 3 * rows, 5000])
+    c = make(rnd.choice([1, 3]), min(pool, 200) if pool == 5000 and seed % 2 else min(pool, 300), 2, rnd.choice([16, 48]), page, seed)
+    want = R.Cache(c)
+    table, lengths = [[-1] * width] * rows, [0] * rows
+    dt, dl = ints(table), ints(lengths)
+    for step in range(14):
+        do = rnd.choice(["fork", "resize", "resize", "grow", "compact"])
+        if do == "fork":
+            parents = [rnd.choice([r, r, rnd.randrange(rows), -3, rows + 5]) for r in range(rows)]
+            dt, dl = c.fork(dt, dl, ints(parents))
+            table, lengths = want.fork(table, lengths, parents)
+        elif do == "compact":
+            dt, count = c.compact(dt)
+            table, n = want.compact(table)
+            assert int(count) == n
+        else:
+            wanted = [rnd.choice([0, lengths[r], rnd.randrange(width * page + 1), width * page + 1, -4]) if do == "resize"
+                      else lengths[r] + rnd.randrange(page) for r in range(rows)]
+            dt, dl, short = c.resize(dt, dl, ints(wanted))
+            table, lengths, n = want.resize(table, lengths, wanted)
+            assert int(short) == n
+        assert dt.tolist() == table and dl.tolist() == lengths, (step, do)
+        want.same(c)
+
+
+def test_pages_of_large_pools():
+    """Pools beyond a work-group's first rounds, free pages far behind; counts below 0 are free."""
+    page, pool = 16, 40000
+    c = FP8KVCache.empty(1, pool, 1, 16, page=page)
+    c.k.view(torch.uint8).copy_(torch.randint(0, 127, c.k.shape, device=DEV, dtype=torch.uint8))
+    c.v.view(torch.uint8).copy_(torch.randint(0, 127, c.v.shape, device=DEV, dtype=torch.uint8))
+    refs = [2] * 30000 + [1, 0, 3, -2] * 2500
+    c.refs.copy_(ints(refs))
+    want = R.Cache(c)
+    rows, width = 2100, 3
+    table, lengths = [[-1] * width] * rows, [0] * rows
+    dt, dl, short = c.resize(ints(table), ints(lengths), ints([33 if r % 3 else 5 for r in range(rows)]))
+    table, lengths, n = want.resize(table, lengths, [33 if r % 3 else 5 for r in range(rows)])
+    assert n == 0 and int(short) == n and dt.tolist() == table and dl.tolist() == lengths
+    want.same(c)
+    # 700 rows want two pages more than they have, and 100 are left
+    dt, dl, short = c.resize(dt, dl, ints([33] * rows))
+    table, lengths, n = want.resize(table, lengths, [33] * rows)
+    assert n == 1300 and int(short) == n and dt.tolist() == table and dl.tolist() == lengths
+    want.same(c)
+    c.refs[:25000] = 0
+    want.refs[:25000] = [0] * 25000
+    dt, count = c.compact(dt)
+    table, n = want.compact(table)
+    assert int(count) == n and dt.tolist() == table
+    want.same(c)
+
+
+def test_entries_that_are_no_pages_stay_without_effect():
+    c = make(1, 5, 1, 16, 16)
+    c.refs.copy_(ints([1, 2, 0, 1, 0]))
+    want = R.Cache(c)
+    table, lengths = [[1, 77, -9], [1, 3, 0], [2 ** 31 - 1, -1, -1]], [40, 33, 10]
+    dt, dl = c.fork(ints(table), ints(lengths), ints([1, 0, 2]))
+    t, n = want.fork(table, lengths, [1, 0, 2])
+    assert dt.tolist() == t and dl.tolist() == n
+    want.same(c)
+    dt, dl, short = c.resize(dt, dl, ints([1, 41, 12]))
+    t, n, s = want.resize(t, n, [1, 41, 12])
+    assert dt.tolist() == t and dl.tolist() == n and int(short) == s
+    want.same(c)
+    dt, count = c.compact(dt)
+    t, k = want.compact(t)
+    assert dt.tolist() == t and int(count) == k
+    want.same(c)
+
+
+def test_upkeep_without_rows_or_width():
+    c = make(1, 4, 1, 16, 16)
+    c.refs.copy_(ints([0, 1, 0, 2]))
+    none = torch.empty((0, 3), dtype=torch.int32, device=DEV)
+    t, n = c.fork(none, ints([]), ints([]))
+    assert t.shape == (0, 3) and n.shape == (0,)
+    t, n, short = c.resize(none, ints([]), ints([]))
+    assert int(short) == 0
+    t, n, short = c.resize(torch.empty((2, 0), dtype=torch.int32, device=DEV), ints([0, 5]), ints([1, 0]))
+    assert n.tolist() == [0, 0] and int(short) == 0
+    t, count = c.compact(none)
+    assert int(count) == 2 and c.refs.tolist() == [2, 1, 0, 0]
+
+
+# ---------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------
+def test_a_rollout():
+    """Prompts are cached and forked into samples, which decode and end; every step's attention against the tokens' own keys and values."""
+    page, layers, kv, heads, dim, width, samples = 16, 2, 2, 6, 64, 8, 3
+    prompts = [21, 48, 5]
+    rows = len(prompts) * samples
+    c = FP8KVCache.empty(layers, 60, kv, dim, page=page)
+    c.k.view(torch.uint8).fill_(0x7F), c.v.view(torch.uint8).fill_(0x7F)
+    table, lengths = ints([[-1] * width] * rows), ints([0] * rows)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    kept = [[(torch.empty(0, kv, dim, device=DEV), torch.empty(0, kv, dim, device=DEV)) for _ in range(layers)] for _ in range(rows)]
+
+    def step(new):
+        nonlocal table, lengths
+        table, lengths, short = c.resize(table, lengths, lengths + ints(new))
+        assert int(short) == 0
+        offsets = [0]
+        for n in new:
+            offsets.append(offsets[-1] + n)
+        for layer in range(layers):
+            k, v = ((torch.randn(offsets[-1], kv, dim, generator=g, device=DEV) * 2).bfloat16() for _ in range(2))
+            for r in range(rows):
+                part = slice(offsets[r], offsets[r + 1])
+                a, b = kept[r][layer]
+                kept[r][layer] = torch.cat([a, k[part].float()]), torch.cat([b, v[part].float()])
+            q = (torch.randn(offsets[-1], heads, dim, generator=g, device=DEV)).bfloat16()
+            c.append(layer, k, v, table, lengths, ints(offsets))
+            out = c.attend(layer, q, table, lengths, ints(offsets))
+            want, bound, _ = R.attend(c, layer, q, table.tolist(), lengths.tolist(), offsets, dim ** -0.5, 0)
+            close(out, want, bound)
+            # what is cached is what was given, to e4m3's half step (twice, where it was rounded to a larger scale), and half a step of
+            # the smallest codes
+            for r in range(rows):
+                n = int(lengths[r])
+                assert n == kept[r][layer][0].shape[0]
+                idx = table[r, : R.pages_of(n, page)].long()
+                for codes, scales, x, turned in ((c.k, c.k_scales, kept[r][layer][0], False), (c.v, c.v_scales, kept[r][layer][1], True)):
+                    got = codes[layer].view(torch.uint8)[idx].view(R.E4M3).float() * scales[layer][idx][..., None, None]
+                    got = (got.transpose(2, 3) if turned else got).transpose(1, 2).reshape(-1, kv, dim)[:n]
+                    top = scales[layer][idx][:, None].expand(-1, page, -1).reshape(-1, kv, 1)[:n]
+                    assert bool(((got - x).abs() <= 2.0 ** -4 * 2.1 * x.abs() + 2.0 ** -9 * top).all())
+
+    step([prompts[r // samples] if r % samples == 0 else 0 for r in range(rows)])
+    table, lengths = c.fork(table, lengths, ints([r - r % samples for r in range(rows)]))
+    kept[:] = [[pair for pair in kept[r - r % samples]] for r in range(rows)]
+    assert int(c.refs.max()) == samples
+    for i in range(4):
+        step([1 if (r + i) % 4 else 2 for r in range(rows)])
+    # some end, the pool is packed, the others go on
+    table, lengths, _ = c.resize(table, lengths, lengths * ints([r % 2 for r in range(rows)]))
+    for r in range(0, rows, 2):
+        kept[r] = [(a[:0], b[:0]) for a, b in kept[r]]
+    table, count = c.compact(table)
+    assert int(count) == int((c.refs > 0).sum()) and bool((c.refs[: int(count)] > 0).all())
+    step([r % 2 for r in range(rows)])
+    table, lengths, _ = c.resize(table, lengths, lengths * 0)
+    assert int(c.refs.abs().max()) == 0 and bool((table == -1).all())
+
+
+def test_a_captured_step_replays():
+    """resize, append and attend in one graph, replayed over a growing batch with eager work and synchronizations between."""
+    page, kv, heads, dim, rows, width = 16, 2, 4, 64, 5, 9
+    g = torch.Generator(device=DEV).manual_seed(3)
+
+    def fresh():
+        c = FP8KVCache.empty(1, 40, kv, dim, page=page)
+        c.k.view(torch.uint8).zero_(), c.v.view(torch.uint8).zero_()
+        return c
+
+    eager, caught = fresh(), fresh()
+    k, v, q = (torch.empty(rows, n, dim, dtype=torch.bfloat16, device=DEV) for n in (kv, kv, heads))
+    table, lengths = ints([[-1] * width] * rows), ints([0, 0, 0, 0, 0])
+
+    def step(c, table, lengths):
+        table, lengths, _ = c.resize(table, lengths, lengths + 1)
+        c.append(0, k, v, table, lengths)
+        return table, lengths, c.attend(0, q, table, lengths)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    gt, gl = table.clone(), lengths.clone()
+    warm = fresh()
+    with torch.cuda.stream(s):
+        step(warm, gt, gl)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        nt, nl, out = step(caught, gt, gl)
+        gt.copy_(nt), gl.copy_(nl)
+    caught.refs.zero_()
+    gt.copy_(table), gl.copy_(lengths)
+    for i in range(40):
+        for x in (k, v, q):
+            x.copy_(torch.randn(x.shape, generator=g, device=DEV))
+        table, lengths, want = step(eager, table, lengths)
+        graph.replay()
+        if i % 7 == 0:
+            torch.cuda.synchronize()
+        assert torch.equal(gt, table) and torch.equal(gl, lengths) and torch.equal(out, want), i
+        assert torch.equal(caught.refs, eager.refs)
+
+
+def test_two_streams_at_once():
+    page, kv, heads, dim = 64, 2, 8, 128
+    c = make(1, 70, kv, dim, page)
+    lengths = [4000, 300]
+    table = R.spread_table(lengths, page, 63, 70, 1)
+    q = [queries(2, heads, dim, torch.bfloat16, i) for i in range(8)]
+    want = [c.attend(0, x, ints(table), ints(lengths)) for x in q]
+    t, n = ints(table), ints(lengths)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i, x in enumerate(q):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(c.attend(0, x, t, n))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_results_do_not_depend_on_the_run():
+    c = make(1, 200, 2, 128, 64)
+    lengths = [5000, 17, 900]
+    table = R.spread_table(lengths, 64, 80, 200, 2)
+    q = queries(3, 8, 128, torch.float16)
+    first = c.attend(0, q, ints(table), ints(lengths))
+    for _ in range(5):
+        assert torch.equal(c.attend(0, q, ints(table), ints(lengths)), first)
+
+
+def test_gradients_are_refused_not_lost():
+    c = make(1, 4, 1, 64, 16)
+    table, lengths = ints([[0, 1]]), ints([20])
+    q = queries(1, 2, 64, torch.bfloat16).requires_grad_()
+    out, lse = c.attend(0, q, table, lengths, return_lse=True)
+    assert out.requires_grad
+    with pytest.raises(RuntimeError, match="no gradient"):
+        out.sum().backward()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        c.attend(0, q, table, lengths, out=torch.empty_like(q).detach())
+    with torch.no_grad():
+        assert torch.equal(c.attend(0, q, table, lengths), out)
+    k = queries(1, 1, 64, torch.bfloat16).requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        c.append(0, k, k, table, lengths)
+    c.append(0, k.detach(), k.detach(), table, lengths)
+
+
+def test_refusals():
+    c = make(1, 4, 2, 64, 16)
+    table, lengths = ints([[0, 1]]), ints([20])
+    q, k = queries(1, 4, 64, torch.bfloat16), queries(1, 2, 64, torch.bfloat16)
+
+    def bad(error, call, *args, **kw):
+        with pytest.raises(error):
+            call(*args, **kw)
+
+    for layer in (-1, 1, 0.0, None):
+        bad(ValueError, c.attend, layer, q, table, lengths)
+        bad(ValueError, c.append, layer, k, k, table, lengths)
+    bad(TypeError, c.attend, 0, q.float(), table, lengths)
+    bad(TypeError, c.attend, 0, q.double(), table, lengths)
+    bad(TypeError, c.attend, 0, None, table, lengths)
+    bad(ValueError, c.attend, 0, q.cpu(), table, lengths)
+    bad(ValueError, c.attend, 0, q[:, :3], table, lengths)
+    bad(ValueError, c.attend, 0, q[:, :0], table, lengths)
+    bad(ValueError, c.attend, 0, q[..., :48], table, lengths)
+    bad(ValueError, c.attend, 0, q[0], table, lengths)
+    bad(ValueError, c.attend, 0, q, table, lengths, window=0)
+    bad(ValueError, c.attend, 0, q, table, lengths, out=q.float())
+    bad(ValueError, c.attend, 0, q, table, lengths, out=q[:, :2])
+    bad(TypeError, c.attend, 0, q, table.long(), lengths)
+    bad(TypeError, c.attend, 0, q, table, lengths.long())
+    bad(TypeError, c.attend, 0, q, table, [20])
+    bad(ValueError, c.attend, 0, q, table[0], lengths)
+    bad(ValueError, c.attend, 0, q, table.cpu(), lengths)
+    bad(ValueError, c.attend, 0, q, table, ints([1, 2]))
+    bad(ValueError, c.attend, 0, q, table, lengths, ints([0]))
+    bad(TypeError, c.attend, 0, q, table, lengths, torch.tensor([0, 1], device=DEV))
+    bad(ValueError, c.attend, 0, q, ints([[0], [1]]), ints([3, 4]))  # two sequences, one token
+    bad(ValueError, c.append, 0, k, k[:, :1], table, lengths)
+    bad(ValueError, c.append, 0, k, k.half(), table, lengths)
+    bad(ValueError, c.append, 0, q, q, table, lengths)
+    bad(TypeError, c.append, 0, k.double(), k.double(), table, lengths)
+    bad(ValueError, c.fork, table, lengths, ints([0, 1]))
+    bad(TypeError, c.fork, table, lengths, torch.zeros(1, device=DEV))
+    bad(ValueError, c.resize, table, lengths, ints([[3]]))
+    bad(TypeError, c.compact, None)
+    ok = (c.k, c.v, c.k_scales, c.v_scales, c.refs)
+
+    def made(**kw):
+        names = ("k", "v", "k_scales", "v_scales", "refs")
+        FP8KVCache(*[kw.get(n, x) for n, x in zip(names, ok)])
+
+    made()
+    for kw in ({"k": c.k.float()}, {"refs": c.refs.long()}, {"k_scales": c.k_scales.half()}, {"v": None}):
+        bad(TypeError, made, **kw)
+    for kw in ({"k": c.k[0]}, {"v": c.v.transpose(3, 4)}, {"v": c.k}, {"k_scales": c.k_scales[:, :3]}, {"refs": c.refs[:3]}, {"refs": c.refs.cpu()},
+               {"k": c.k.cpu()}, {"v": c.v[:, :1].expand(-1, 4, -1, -1, -1)}, {"k_scales": c.k_scales[:, :1].expand(-1, 4, -1)}):
+        bad(ValueError, made, **kw)
+    for shape in ((1, 4, 2, 24, 64), (1, 4, 2, 16, 72), (1, 4, 2, 16, 272), (1, 4, 2, 512, 64), (1, 4, 0, 16, 64), (1, 0, 2, 16, 64), (1, 4, 257, 16, 16)):
+        bad(ValueError, FP8KVCache.empty, shape[0], shape[1], shape[2], shape[4], page=shape[3])
