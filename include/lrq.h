@@ -280,7 +280,8 @@ int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, 
  *   in the results of the rows that see it alone.  lse: [tokens, heads], the scores' log-sum-exp
  *   (natural), or null.  Rows behind offsets[seqs] stay as they were, or become 0 with
  *   zero_rest.  q is bf16 or fp16, out of its type, dense, 8-byte aligned.
- *   `workspace`: lrq_kv_attend_workspace bytes, 256-byte aligned, overwritten.
+ *   `workspace`: lrq_kv_attend_workspace bytes (one_each: no offsets), 256-byte aligned,
+ *   overwritten.
  * The three below write a new table (dense [rows, width], -1 behind a row's pages) and
  *   new lengths beside the ones they read, and count in refs: how many rows hold a page,
  *   one that none holds (0 or below) being free.
@@ -305,7 +306,7 @@ typedef struct lrq_kv_cache {
 int lrq_kv_append(const lrq_kv_cache* cache, int64_t layer, const void* k, int64_t k_token, int64_t k_head, const void* v,
                   int64_t v_token, int64_t v_head, int dtype, int64_t tokens, const int32_t* table, int64_t ld, int64_t width,
                   const int32_t* lengths, const int32_t* offsets, int64_t seqs, lrq_stream_t stream);
-int64_t lrq_kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs);
+int64_t lrq_kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int one_each);
 int lrq_kv_attend(const lrq_kv_cache* cache, int64_t layer, const void* q, int64_t q_token, int64_t q_head, int dtype,
                   int64_t tokens, int64_t heads, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
                   const int32_t* offsets, int64_t seqs, float scale, int64_t window, int zero_rest, void* out, float* lse,

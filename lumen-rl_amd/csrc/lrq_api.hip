@@ -969,9 +969,11 @@ int lrq_kv_append(const lrq_kv_cache* cache, int64_t layer, const void* k, int64
   return check_hip(lrq::launch_kv_append(a, dtype, (hipStream_t)stream), "kernel launch");
 }
 
-int64_t lrq_kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs) {
-  if (tokens < 0 || heads < 1 || kv_heads < 1 || seqs < 0 || dim < 16 || dim > 256) return 0;
-  return lrq::kv_attend_workspace(dim);
+int64_t lrq_kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int one_each) {
+  if (tokens < 1 || tokens > 1 << 22 || heads < 1 || heads > 4096 || kv_heads < 1 || kv_heads > 256 || heads % kv_heads || seqs < 0 ||
+      seqs > 1 << 20 || dim < 16 || dim > 256)
+    return 0;
+  return lrq::kv_attend_workspace(tokens, heads, kv_heads, dim, seqs, one_each != 0);
 }
 
 int lrq_kv_attend(const lrq_kv_cache* cache, int64_t layer, const void* q, int64_t q_token, int64_t q_head, int dtype,
@@ -991,7 +993,11 @@ int lrq_kv_attend(const lrq_kv_cache* cache, int64_t layer, const void* q, int64
   if (!aligned(q, 2) || !aligned(out, 8) || !aligned(lse, 4))
     return fail(LRQ_ERR_ALIGN, "kv_attend: queries must be element-aligned, the result 8-byte aligned");
   if (!strides_ok(q_token, q_head, cache->dim, tokens, heads)) return fail(LRQ_ERR_ARG, "kv_attend: strides are negative, or too large");
-  if (int err = check_workspace("kv_attend", workspace, workspace_bytes, lrq::kv_attend_workspace(cache->dim))) return err;
+  if ((tokens * (heads / cache->kv_heads) / 128 + seqs + 1024) * cache->kv_heads >= int64_t(1) << 24)
+    return fail(LRQ_ERR_ARG, "kv_attend: %lld tokens of %lld heads are more than one launch takes", (long long)tokens, (long long)heads);
+  if (int err = check_workspace("kv_attend", workspace, workspace_bytes,
+                                lrq::kv_attend_workspace(tokens, heads, cache->kv_heads, cache->dim, seqs, !offsets)))
+    return err;
   a.cache = kv_layer(*cache, layer);
   a.q = q, a.q_token = q_token, a.q_head = q_head, a.out = out, a.lse = lse;
   a.scale = scale * 1.44269504089f, a.heads = (int)heads, a.group = (int)(heads / cache->kv_heads);

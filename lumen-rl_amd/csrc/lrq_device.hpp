@@ -260,6 +260,7 @@ __device__ __forceinline__ float mx_mult(uint32_t e8m0) { return u2f((254u - e8m
 // ---------------------------------------------------------------------------
 typedef unsigned int v4u __attribute__((ext_vector_type(4)));
 typedef unsigned int v2u __attribute__((ext_vector_type(2)));
+typedef int v4i __attribute__((ext_vector_type(4)));
 
 // Every tensor is device memory, but the kernels take their pointers from
 // descriptors, so the compiler sees generic pointers and would emit flat_*

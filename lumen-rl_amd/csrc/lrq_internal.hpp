@@ -361,6 +361,12 @@ struct KvAppendArgs {
 int64_t kv_append_tiles(const KvSeqs& s);  // work-groups a head, at most
 hipError_t launch_kv_append(const KvAppendArgs& a, int dtype, hipStream_t stream);
 
+struct KvTiles {  // lrq_kv_prefill.hip's plan, in the workspace
+  int32_t *count, *upto;  // pieces, and tiles that were cut; tiles up to each sequence
+  v4i* piece;             // two each: sequence, tile, first unit, last + 1; place of its sums or -1
+  v4i* cut;               // sequence, tile, place of its first piece's sums, pieces
+  float* sums;
+};
 struct KvAttendArgs {
   KvCache cache;
   KvSeqs seqs;
@@ -371,12 +377,18 @@ struct KvAttendArgs {
   float scale;  // times log2(e)
   int heads, group, window;
   bool zero_rest;  // rows behind the last sequence become 0
+  int few;  // rows of a sequence that k_kv_attend takes; those of more are k_kv_prefill's
   // workspace
   uint8_t* heads_at;
   float* sums;
   int parts, least;
+  KvTiles tiles;
 };
-int64_t kv_attend_workspace(int64_t dim);
+// one_each: one new token a sequence
+int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, bool one_each);
+int64_t kv_prefill_tiles(int64_t tokens, int64_t group, int64_t seqs);
+int64_t kv_prefill_workspace(int64_t tiles, int64_t seqs, int64_t heads, int64_t dim);
+hipError_t launch_kv_prefill(KvAttendArgs a, int dtype, int64_t tiles, void* workspace, hipStream_t stream);
 hipError_t launch_kv_attend(KvAttendArgs a, int dtype, void* workspace, hipStream_t stream);
 
 struct KvTable {

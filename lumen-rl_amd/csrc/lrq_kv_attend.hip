@@ -21,32 +21,15 @@
 // keys whose V codes it loads with one 16-byte load, in its order, and P never leaves the
 // registers.
 #include "lrq_kv.hpp"
+#include "lrq_kv_attend.hpp"
 
 namespace lrq {
 
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kRows = 16;    // rows of a work-group
-constexpr int kUnit = 64;    // keys that a wave takes at a time
 constexpr int kWaves = 4;
 constexpr int kJoinTiles = 8;  // tiles of 16 channels that the waves' sums go through LDS with
-constexpr float kLow = -3.0e38f;  // a maximum before the first key
-constexpr float kLift = 10.0f;    // log2 of what p is multiplied with
-
-// Two e4m3 codes of a word, exactly, in the type of the queries (bf16 or fp16).
-template <int DT, bool HI>
-__device__ __forceinline__ uint32_t widen2(uint32_t w) {
-  if constexpr (DT == kBF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
-  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
-}
-template <int DT>
-__device__ __forceinline__ v4u widen8(uint32_t a, uint32_t b) {
-  return v4u{widen2<DT, false>(a), widen2<DT, true>(a), widen2<DT, false>(b), widen2<DT, true>(b)};
-}
 template <int DT>
 __device__ __forceinline__ f32x4 mma(v4u a, v4u b, f32x4 d) {
   if constexpr (DT == kBF16)
@@ -54,10 +37,6 @@ __device__ __forceinline__ f32x4 mma(v4u a, v4u b, f32x4 d) {
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), d, 0, 0, 0);
 }
-__device__ __forceinline__ uint32_t f16_pair(float a, float b) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
-}
-
 // The largest of the lanes l, l ^ 16, l ^ 32 and l ^ 48.
 __device__ __forceinline__ float column_max(float v) {
   auto a = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
@@ -71,11 +50,6 @@ __device__ __forceinline__ float column_sum(float v) {
   auto b = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
   return u2f(b[0]) + u2f(b[1]);
 }
-
-// Bytes of `w` that are NaN codes, as 0x80 in each.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
-// The first `n` bytes of a word (n any number).
-__device__ __forceinline__ uint32_t low_bytes(int n) { return n <= 0 ? 0u : n >= 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u; }
 
 // The units of keys that a sequence's rows see: [first, first + count), one at least.
 struct Span {
@@ -91,7 +65,11 @@ __device__ __forceinline__ Span span_of(const KvSeq& q, int window) {
   if (s.count < 1) s.count = 1;
   return s;
 }
-__device__ __forceinline__ int64_t row_tiles(const KvSeq& q, int group) { return ((int64_t)q.n * group + kRows - 1) / kRows; }
+// Tiles of a sequence's rows; none where it has so many that k_kv_prefill takes them.
+__device__ __forceinline__ int64_t row_tiles(const KvSeq& q, int group, int few) {
+  const int64_t rows = (int64_t)q.n * group;
+  return rows > few ? 0 : (rows + kRows - 1) / kRows;
+}
 
 // ---------------------------------------------------------------------------
 // Work: the units of all items (sequence, KV head, 16 rows) stand in one line, which is
@@ -113,18 +91,6 @@ struct PartHead {
   int parts;      // parts that hold pieces of it, the first included
 };
 static_assert(sizeof(PartHead) <= 32, "the join's heads are 32 bytes apart");
-
-template <int DT>
-__device__ __forceinline__ void store4(void* out, int64_t at, f32x4 v) {
-  uint16_t* const p = static_cast<uint16_t*>(out) + at;
-  v2u w;
-  if constexpr (DT == kBF16) {
-    w = v2u{bf16x2_bits(v.x, v.y), bf16x2_bits(v.z, v.w)};
-  } else {
-    w = v2u{f16_pair(v.x, v.y), f16_pair(v.z, v.w)};
-  }
-  gst<v2u>(p, w);
-}
 
 template <int DT, int NC>
 __global__ __launch_bounds__(64 * kWaves) void k_kv_attend(KvAttendArgs a) {
@@ -152,7 +118,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_kv_attend(KvAttendArgs a) {
 
   auto work_of = [&](int b) -> int64_t {
     const KvSeq q = kv_seq(a.seqs, b);
-    return q.n == 0 ? 0 : row_tiles(q, group) * a.cache.heads * span_of(q, a.window).count;
+    return row_tiles(q, group, a.few) * a.cache.heads * span_of(q, a.window).count;
   };
   // all work, then the sequence in which this part begins
   int64_t total = 0;
@@ -190,8 +156,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_kv_attend(KvAttendArgs a) {
   for (int64_t at = begin; at < end && b < a.seqs.seqs;) {
     const KvSeq q = kv_seq(a.seqs, b);
     const Span span = span_of(q, a.window);
-    const int64_t tiles = row_tiles(q, group);
-    if (q.n == 0 || inside >= tiles * a.cache.heads * span.count) {  // the next sequence
+    const int64_t tiles = row_tiles(q, group, a.few);
+    if (inside >= tiles * a.cache.heads * span.count) {  // the next sequence
       ++b, inside = 0;
       continue;
     }
@@ -404,7 +370,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_kv_attend(KvAttendArgs a) {
         gst<float>(out + r, all), gst<float>(out + kRows + r, sum);
       } else if (a.lse != nullptr && r < rows) {
         gst<float>(a.lse + (q.first + tok) * a.heads + qh,
-                   sum != 0.0f ? (all - kLift + __builtin_amdgcn_logf(sum)) * 0.69314718056f : -INFINITY);
+                   sum != 0.0f ? (all - kLift + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY);
       }
     }
     if (tid == 0 && starts && !whole) {
@@ -447,7 +413,7 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttendArgs a) {
     const int64_t at = (head.first + tok) * a.heads + head.h * a.group + (row - tok * a.group);
     store4<DT>(a.out, at * dim + 4 * c, v * (sum != 0.0f ? 1.0f / sum : 0.0f));
     if (a.lse != nullptr && c == 0)
-      gst<float>(a.lse + at, sum != 0.0f ? (top - kLift + __builtin_amdgcn_logf(sum)) * 0.69314718056f : -INFINITY);
+      gst<float>(a.lse + at, sum != 0.0f ? (top - kLift + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY);
   }
 }
 
@@ -466,19 +432,37 @@ void launch_of(const KvAttendArgs& a, hipStream_t stream) {
 
 constexpr unsigned kParts = 512;  // two work-groups a compute unit
 
+// Sequences of more rows than this are k_kv_prefill's, if the call has as many.
+constexpr int kFew = 64;
+
+int64_t few_workspace(int64_t dim) { return kParts * 32 + 2 * kParts * 4 * (kPlaceWords + kRows * dim); }
+
 }  // namespace
 
-int64_t kv_attend_workspace(int64_t dim) {
-  return kParts * 32 + 2 * kParts * 4 * (kPlaceWords + kRows * dim);
+int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, bool one_each) {
+  const int64_t group = heads / kv_heads, rows = (one_each ? 1 : tokens) * group;
+  int64_t need = few_workspace(dim);
+  if (rows > kFew) {
+    const int64_t many = kv_prefill_workspace(kv_prefill_tiles(tokens, group, seqs), seqs, kv_heads, dim);
+    if (many > need) need = many;
+  }
+  return need;
 }
 
 hipError_t launch_kv_attend(KvAttendArgs a, int dtype, void* workspace, hipStream_t stream) {
+  // no sequence has more rows than the call
+  const int64_t most = a.seqs.offsets == nullptr ? a.group : a.seqs.tokens * a.group;
+  a.few = most > kFew ? kFew : INT32_MAX;
   a.heads_at = static_cast<uint8_t*>(workspace);
   a.sums = reinterpret_cast<float*>(a.heads_at + kParts * 32);
   a.parts = kParts;
   a.least = kWaves;
   if (dtype == kBF16) launch_of<kBF16>(a, stream);
   else launch_of<kF16>(a, stream);
+  if (most > kFew) {
+    // the workspace is used again: the stream keeps the two in order
+    if (hipError_t e = launch_kv_prefill(a, dtype, kv_prefill_tiles(a.seqs.tokens, a.group, a.seqs.seqs), workspace, stream)) return e;
+  }
   return hipGetLastError();
 }
 

@@ -1,0 +1,480 @@
+// Attention of many new tokens a sequence on an FP8 KV cache (lrq_kv_attend.hip has the
+// formulas, and the kernel for few).
+//
+// A work-group takes 128 rows (tokens times the query heads of one KV head), 32 a wave,
+// and 64 keys at a time.  Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, on
+// 32x32x16 instructions, so that lane l holds the column l % 32 of every result: one row
+// of queries, of which l and l + 32 have half the keys each.  P goes from the first product's
+// result into the second's operand within its lane.
+//
+// The codes are widened once for all four waves, on their way into LDS: there they lie as the
+// instructions' operands, 1 KiB each, 16 bytes a lane in its order.  K, a piece of 16 channels
+// of a token: channels 0-7 go to the lower half of an operand, 8-15 to the upper.  V, 16 keys
+// of a channel: the lower half takes keys 0-3 and 8-11, the upper 4-7 and 12-15, the keys that
+// the halves of a lane pair hold of P.  A row's place in an operand is moved by twice the piece's
+// number modulo 4, so that eight lanes that write four pieces of two rows meet eight places.
+// While a tile is worked on, the next one's codes are on their way into registers.
+#include "lrq_kv.hpp"
+#include "lrq_kv_attend.hpp"
+
+namespace lrq {
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kTileRows = 128;
+constexpr int kSlots = 512;     // shares that the work is cut into: two work-groups a compute unit
+constexpr int kLeastUnits = 8;  // below it a tile is not cut: its pieces' sums cost as much
+constexpr float kSlack = 5.0f;  // what a row's maximum may grow by before its sums are scaled (p stays below 2^15)
+
+template <int DT>
+__device__ __forceinline__ f32x16 mma32(v4u a, v4u b, f32x16 d) {
+  if constexpr (DT == kBF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), d, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), d, 0, 0, 0);
+}
+__device__ __forceinline__ float pair_max(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+  return fmaxf(u2f(a[0]), u2f(a[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+  return u2f(a[0]) + u2f(a[1]);
+}
+
+// The rows of a tile of a sequence: how many, and the units of keys that some of them see.
+struct TileSpan {
+  int rows, hi, lo, first, end;  // keys [lo, hi), units [first, end)
+};
+__device__ __forceinline__ TileSpan tile_span(const KvSeq& q, int group, int window, int64_t tile) {
+  TileSpan s;
+  const int64_t row0 = tile * kTileRows, all = (int64_t)q.n * group;
+  s.rows = (int)(all - row0 < kTileRows ? all - row0 : kTileRows);
+  const int a = (int)(row0 / group), b = (int)((row0 + s.rows - 1) / group);
+  const int base = q.len - q.n + 1;
+  s.hi = base + b < 0 ? 0 : base + b;
+  s.lo = window > 0 && base + a > window ? base + a - window : 0;
+  s.first = s.lo / kUnit;
+  s.end = (s.hi + kUnit - 1) / kUnit;
+  if (s.end < s.first) s.end = s.first;
+  return s;
+}
+__device__ __forceinline__ int64_t tiles_of(const KvAttendArgs& a, int b) {
+  const KvSeq q = kv_seq(a.seqs, b);
+  const int64_t rows = (int64_t)q.n * a.group;
+  return rows <= a.few ? 0 : (rows + kTileRows - 1) / kTileRows;
+}
+
+// ---------------------------------------------------------------------------
+// The plan, by one work-group: all tiles of the sequences that have many rows, those with
+// more units than a work-group's share cut into pieces, the longest pieces first.
+// ---------------------------------------------------------------------------
+constexpr int kBuckets = 1024;  // of pieces' lengths; the last one takes all longer ones
+__global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
+  __shared__ int64_t scan[16];
+  __shared__ int64_t carry;
+  __shared__ uint32_t bucket[kBuckets];
+  __shared__ uint32_t counts[2];  // places of pieces, and tiles that were cut
+  const KvTiles& p = a.tiles;
+  const int tid = threadIdx.x, seqs = a.seqs.seqs;
+  // upto[b]: tiles of the sequences 0 .. b
+  if (tid == 0) carry = 0, counts[0] = counts[1] = 0;
+  bucket[tid] = 0;
+  __syncthreads();
+  for (int b0 = 0; b0 < seqs; b0 += 1024) {
+    const int64_t base = carry;
+    const int64_t upto = base + block_scan<1024, int64_t>(b0 + tid < seqs ? tiles_of(a, b0 + tid) : 0, scan);
+    if (b0 + tid < seqs) gst<int32_t>(p.upto + b0 + tid, (int32_t)upto);
+    if (tid == 1023) carry = upto;
+    __syncthreads();
+  }
+  const int tiles = (int)carry;
+  __syncthreads();
+  auto find = [&](int i, int& tile) {  // the sequence of tile i
+    int lo = 0, hi = seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (gld<int32_t>(p.upto + mid) > i) hi = mid;
+      else lo = mid + 1;
+    }
+    tile = i - (lo > 0 ? gld<int32_t>(p.upto + lo - 1) : 0);
+    return lo;
+  };
+  int64_t units = 0;
+  for (int i = tid; i < tiles; i += 1024) {
+    int tile;
+    const int b = find(i, tile);
+    const TileSpan s = tile_span(kv_seq(a.seqs, b), a.group, a.window, tile);
+    units += s.end - s.first;
+  }
+  const int64_t sum = block_scan<1024, int64_t>(units, scan);
+  if (tid == 1023) carry = sum;
+  __syncthreads();
+  int64_t most = (carry * a.cache.heads + kSlots - 1) / kSlots;
+  if (most < kLeastUnits) most = kLeastUnits;
+  auto cuts_of = [&](int n) { return n <= most ? 1 : (int)((n + most - 1) / most); };
+  auto bucket_of = [&](int n) { return n >= kBuckets ? 0 : kBuckets - 1 - n; };
+  for (int i = tid; i < tiles; i += 1024) {
+    int tile;
+    const int b = find(i, tile);
+    const TileSpan s = tile_span(kv_seq(a.seqs, b), a.group, a.window, tile);
+    const int n = s.end - s.first, cuts = cuts_of(n);
+    atomicAdd(&bucket[bucket_of(n / cuts)], (uint32_t)cuts);
+  }
+  __syncthreads();
+  const uint32_t mine = bucket[tid];
+  const int64_t before = block_scan<1024, int64_t>(mine, scan) - mine;
+  bucket[tid] = (uint32_t)before;
+  if (tid == 1023) gst<int32_t>(p.count, (int32_t)(before + mine));
+  __syncthreads();
+  for (int i = tid; i < tiles; i += 1024) {
+    int tile;
+    const int b = find(i, tile);
+    const TileSpan s = tile_span(kv_seq(a.seqs, b), a.group, a.window, tile);
+    const int n = s.end - s.first, cuts = cuts_of(n);
+    const uint32_t at = atomicAdd(&bucket[bucket_of(n / cuts)], (uint32_t)cuts);
+    int slot = -1;
+    if (cuts > 1) {
+      slot = (int)atomicAdd(&counts[0], (uint32_t)cuts);
+      const uint32_t cut = atomicAdd(&counts[1], 1u);
+      gst<v4i>(p.cut + cut, v4i{b, tile, slot, cuts});
+    }
+    for (int j = 0; j < cuts; ++j) {
+      const int u0 = s.first + (int)((int64_t)n * j / cuts), u1 = s.first + (int)((int64_t)n * (j + 1) / cuts);
+      gst<v4i>(p.piece + 2 * (at + j), v4i{b, tile, u0, u1});
+      gst<v4i>(p.piece + 2 * (at + j) + 1, v4i{slot < 0 ? -1 : slot + j, 0, 0, 0});
+    }
+  }
+  __syncthreads();
+  if (tid == 0) gst<int32_t>(p.count + 1, (int32_t)counts[1]);
+}
+
+template <int DT, int NC>
+__global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs a) {
+  constexpr int KS = 4 * NC, VT = 2 * NC;       // steps of 16 channels, tiles of 32
+  constexpr int kStage = (2 * KS + 4 * VT) * 64;  // 16-byte places of a tile: K's operands, then V's
+  __shared__ __attribute__((aligned(16))) v4u stage[2][kStage];
+  __shared__ __attribute__((aligned(16))) float page_of[2][12];  // per 16 keys: factor, exponent, its inverse
+  __shared__ int has_nan[2];  // a stage's unit + 1, if it has NaN codes that some rows may not see
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, half = lane >> 5;
+  const int heads = a.cache.heads, dim = a.cache.dim, shift = a.seqs.shift, S = 1 << shift, group = a.group;
+  const int count = gld<int32_t>(a.tiles.count);
+  const int h = blockIdx.x % heads, idx = blockIdx.x / heads;
+  if (idx >= count) return;
+  const v4i piece = gld<v4i>(a.tiles.piece + 2 * idx);
+  const int slot = gld<int32_t>(a.tiles.piece + 2 * idx + 1);
+  const int b = __builtin_amdgcn_readfirstlane(piece.x), tile = __builtin_amdgcn_readfirstlane(piece.y);
+  const int u0 = __builtin_amdgcn_readfirstlane(piece.z), u1 = __builtin_amdgcn_readfirstlane(piece.w);
+  const KvSeq q = kv_seq(a.seqs, b);
+  const TileSpan span = tile_span(q, group, a.window, tile);
+
+  // this lane's row, and the keys [lo, hi) that it sees
+  const int mine = wave * 32 + r;
+  const int64_t row = (int64_t)tile * kTileRows + (mine < span.rows ? mine : 0);
+  const int tok = (int)(row / group), qh = h * group + (int)(row - (int64_t)tok * group);
+  const int pos1 = q.len - q.n + tok + 1;
+  const int hi = pos1 < 0 ? 0 : pos1, lo = a.window > 0 && pos1 > a.window ? pos1 - a.window : 0;
+  // what the first and the last row of the tile see
+  const int first_hi = q.len - q.n + (int)((int64_t)tile * kTileRows / group) + 1;
+  const int last_hi = q.len - q.n + (int)(((int64_t)tile * kTileRows + span.rows - 1) / group) + 1;
+  const int last_lo = a.window > 0 && last_hi > a.window ? last_hi - a.window : 0;
+
+  v4u qf[KS];
+  {
+    const uint16_t* const src = static_cast<const uint16_t*>(a.q) + (q.first + tok) * a.q_token + qh * a.q_head;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;  // the keys' factor is to be positive
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      qf[k] = v4u{0, 0, 0, 0};
+      if (16 * k < dim && mine < span.rows) {
+        const v4u w = load_live(src + 16 * k + 8 * half);
+        qf[k] = v4u{w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip};
+      }
+    }
+  }
+  const float scale = __builtin_fabsf(a.scale);
+
+  // what this thread brings of a tile: of K token tid / 4, of V keys 16 (tid % 4) .., a piece of each 64 channels
+  const int k_tok = tid >> 2, c4 = tid & 3;
+  v4u kr[NC], vr[NC];
+  int kp = -1, vp = -1;  // pages
+  float ks = 0.0f, vs = 0.0f;
+  auto look_up = [&](int u) {
+    const int kk = (u * kUnit + k_tok) >> shift, vk = (u * kUnit + 16 * c4) >> shift;
+    kp = kk < a.seqs.width ? kv_page(a.seqs, a.cache.pages, b, kk) : -1;
+    vp = vk < a.seqs.width ? kv_page(a.seqs, a.cache.pages, b, vk) : -1;
+  };
+  bool k_ok = false, v_ok = false;
+  auto load = [&](int u) {
+    const int key = u * kUnit + k_tok, vkey = u * kUnit + 16 * c4;
+    k_ok = kp >= 0, v_ok = vp >= 0;
+    const uint8_t* const kb = a.cache.k + (int64_t)(k_ok ? kp : 0) * a.cache.k_page + ((int64_t)h * S + (key & (S - 1))) * dim + 16 * c4;
+    const uint8_t* const vb = a.cache.v + (int64_t)(v_ok ? vp : 0) * a.cache.v_page + ((int64_t)h * dim + k_tok) * S + (vkey & (S - 1));
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      kr[i] = vr[i] = v4u{0, 0, 0, 0};
+      if (64 * i + 16 * c4 < dim) kr[i] = gld<v4u>(kb + 64 * i);
+      if (64 * i + k_tok < dim) vr[i] = gld<v4u>(vb + (int64_t)64 * i * S);
+    }
+    if (tid < 4) {
+      ks = gld<float>(a.cache.ks + (int64_t)(v_ok ? vp : 0) * a.cache.ks_page + h);
+      vs = gld<float>(a.cache.vs + (int64_t)(v_ok ? vp : 0) * a.cache.vs_page + h);
+    }
+  };
+  auto cut_at = [&](int u) { return u * kUnit + kUnit > first_hi || u * kUnit < last_lo; };
+  auto put = [&](int u, int at) {  // the tile's operands into stage `at`
+    v4u* const st = stage[at];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const v4u w = k_ok ? kr[i] : v4u{0, 0, 0, 0};
+      v4u* const to = st + ((k_tok >> 5) * KS + 4 * i + c4) * 64 + ((k_tok & 31) ^ (2 * c4));
+      to[0] = widen8<DT>(w.x, w.y);
+      to[32] = widen8<DT>(w.z, w.w);
+    }
+    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+    const bool cut = cut_at(u);
+    if (cut) {
+      const int v_key = u * kUnit + 16 * c4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) keep[i] = low_bytes(span.hi - v_key - 4 * i) & ~low_bytes(span.lo - v_key - 4 * i);
+    }
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      v4u w = v_ok ? vr[i] : v4u{0, 0, 0, 0};
+      if (cut) {
+        w = v4u{w.x & keep[0], w.y & keep[1], w.z & keep[2], w.w & keep[3]};
+        bad |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
+      }
+      const int d = 64 * i + k_tok;
+      v4u* const to = st + 2 * KS * 64 + ((d >> 5) * 4 + c4) * 64 + ((d & 31) ^ (2 * c4));
+      const v4u x = widen8<kF16>(w.x, w.y), y = widen8<kF16>(w.z, w.w);  // keys 0-7, 8-15
+      to[0] = v4u{x.x, x.y, y.x, y.y};
+      to[32] = v4u{x.z, x.w, y.z, y.w};
+    }
+    if (bad != 0) has_nan[at] = u + 1;
+    if (tid < 4) {
+      const float ev = __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(vs, 0x1p-48f, 0x1p48f));
+      page_of[at][tid] = fmaxf(ks * scale, 0x1p-120f);  // above 0, so that no key stays no key
+      page_of[at][4 + tid] = v_ok ? ev : -INFINITY;
+      page_of[at][8 + tid] = v_ok ? __builtin_amdgcn_exp2f(-ev) : 0.0f;
+    }
+  };
+
+  float m = kLow, l = 0.0f;
+  f32x16 acc[VT];
+#pragma unroll
+  for (int n = 0; n < VT; ++n) acc[n] = f32x16{};
+  if (tid < 2) has_nan[tid] = 0;
+  __syncthreads();
+  if (u0 < u1) {
+    look_up(u0);
+    load(u0);
+    if (u0 + 1 < u1) look_up(u0 + 1);
+    put(u0, 0);
+  }
+  __syncthreads();
+  for (int u = u0; u < u1; ++u) {
+    const int at = (u - u0) & 1;
+    const bool more = u + 1 < u1;
+    if (more) {
+      load(u + 1);
+      if (u + 2 < u1) look_up(u + 2);
+    }
+    const v4u* const kst = stage[at];
+    const v4u* const vst = stage[at] + 2 * KS * 64;
+    f32x16 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = f32x16{};
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        if (16 * k < dim) s[t] = mma32<DT>(kst[(t * KS + k) * 64 + (lane ^ (2 * (k & 3)))], qf[k], s[t]);
+    }
+    const f32x4 factor = *reinterpret_cast<const f32x4*>(page_of[at]), ev = *reinterpret_cast<const f32x4*>(page_of[at] + 4);
+    const f32x4 back = *reinterpret_cast<const f32x4*>(page_of[at] + 8);
+    const bool cut = cut_at(u) || ev.x == -INFINITY || ev.y == -INFINITY || ev.z == -INFINITY || ev.w == -INFINITY;
+    if (__builtin_amdgcn_readfirstlane(cut)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = u * kUnit + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3);
+          s[t][i] = key < hi && key >= lo && ev[2 * t + (i >> 3)] != -INFINITY ? s[t][i] : -INFINITY;
+        }
+    }
+    float top = m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = s[e >> 1][8 * (e & 1)];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) x = fmaxf(x, s[e >> 1][8 * (e & 1) + i]);
+      // no key of the 16: 0 x -inf and -inf + -inf are kept out of it
+      top = x == -INFINITY ? top : fmaxf(top, __builtin_fmaf(x, factor[e], ev[e]));
+    }
+    top = pair_max(top);
+    if (__ballot(top > m + kSlack) != 0) {
+      const float fade = __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= fade;
+#pragma unroll
+      for (int n = 0; n < VT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[n][i] *= fade;
+    }
+    v4u p[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float shift_by = ev[e] - m + kLift;
+      float x[8], sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 1][8 * (e & 1) + i], factor[e], shift_by));
+        sum += x[i];
+      }
+      l = __builtin_fmaf(sum, back[e], l);
+      p[e] = v4u{f16_pair(x[0], x[1]), f16_pair(x[2], x[3]), f16_pair(x[4], x[5]), f16_pair(x[6], x[7])};
+    }
+    if (__builtin_amdgcn_readfirstlane(has_nan[at]) != u + 1) {
+#pragma unroll
+      for (int n = 0; n < VT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (32 * n < dim) acc[n] = mma32<kF16>(vst[(n * 4 + e) * 64 + (lane ^ (2 * e))], p[e], acc[n]);
+    } else {
+      // NaN codes that some rows see and others do not are counted by a product of their own
+      for (int n = 0; n < VT; ++n) {
+        if (32 * n >= dim) continue;
+        f32x16 hits = f32x16{};
+        f32x16 sums = acc[0];
+#pragma unroll
+        for (int k = 1; k < VT; ++k)
+          if (n == k) sums = acc[k];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const v4u w = vst[(n * 4 + e) * 64 + (lane ^ (2 * e))];
+          uint32_t in[4] = {w.x, w.y, w.z, w.w}, is[4], no[4], see[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool a0 = (in[i] & 0x7FFFu) > 0x7C00u, a1 = (in[i] & 0x7FFF0000u) > 0x7C000000u;
+            is[i] = (a0 ? 0x3C00u : 0u) | (a1 ? 0x3C000000u : 0u);
+            no[i] = in[i] & ((a0 ? 0u : 0xFFFFu) | (a1 ? 0u : 0xFFFF0000u));
+            const int key = u * kUnit + 16 * e + 8 * (i >> 1) + 4 * half + 2 * (i & 1);
+            see[i] = (key < hi && key >= lo ? 0x3C00u : 0u) | (key + 1 < hi && key + 1 >= lo ? 0x3C000000u : 0u);
+          }
+          hits = mma32<kF16>(v4u{is[0], is[1], is[2], is[3]}, v4u{see[0], see[1], see[2], see[3]}, hits);
+          sums = mma32<kF16>(v4u{no[0], no[1], no[2], no[3]}, p[e], sums);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[i] = hits[i] > 0.0f ? __builtin_nanf("") : sums[i];
+#pragma unroll
+        for (int k = 0; k < VT; ++k)
+          if (n == k) acc[k] = sums;
+      }
+    }
+    if (more) put(u + 1, at ^ 1);  // read last before the barrier of the round before
+    __syncthreads();
+  }
+  l = pair_sum(l);
+
+  if (slot < 0) {
+    if (mine >= span.rows) return;
+    const float over = l != 0.0f ? 1.0f / l : 0.0f;  // a row that sees nothing is 0
+    const int64_t at = (q.first + tok) * a.heads + qh;
+#pragma unroll
+    for (int n = 0; n < VT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * n + 8 * i + 4 * half;
+        if (d < dim) store4<DT>(a.out, at * dim + d, f32x4{acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]} * over);
+      }
+    if (a.lse != nullptr && half == 0) gst<float>(a.lse + at, l != 0.0f ? (m - kLift + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY);
+    return;
+  }
+  float* const out = a.tiles.sums + ((int64_t)slot * heads + h) * (kTileRows * (2 + (int64_t)dim));
+  if (half == 0) gst<float>(out + mine, m), gst<float>(out + kTileRows + mine, l);
+#pragma unroll
+  for (int n = 0; n < VT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = 32 * n + 8 * i + 4 * half;
+      if (d < dim)
+        gst<f32x4>(out + 2 * kTileRows + ((int64_t)(d / 4) * kTileRows + mine) * 4,
+                   f32x4{acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]});
+    }
+}
+
+// Tiles that were cut: their pieces' sums, brought to one maximum.
+template <int DT>
+__global__ __launch_bounds__(256) void k_kv_join_tiles(KvAttendArgs a) {
+  const int heads = a.cache.heads, dim = a.cache.dim;
+  const int h = blockIdx.x % heads, idx = blockIdx.x / heads;
+  if (idx >= gld<int32_t>(a.tiles.count + 1)) return;
+  const v4i cut = gld<v4i>(a.tiles.cut + idx);
+  const int b = cut.x, tile = cut.y, slot = cut.z, pieces = cut.w;
+  const KvSeq q = kv_seq(a.seqs, b);
+  const int64_t all = (int64_t)q.n * a.group, row0 = (int64_t)tile * kTileRows;
+  const int64_t step = (int64_t)heads * kTileRows * (2 + dim);
+  const float* const first = a.tiles.sums + ((int64_t)slot * heads + h) * (kTileRows * (2 + (int64_t)dim));
+  const int r = threadIdx.x % kTileRows;
+  if (row0 + r >= all) return;
+  float top = gld<float>(first + r);
+  for (int p = 1; p < pieces; ++p) top = fmaxf(top, gld<float>(first + p * step + r));
+  float sum = 0.0f;
+  for (int p = 0; p < pieces; ++p) sum += __builtin_amdgcn_exp2f(gld<float>(first + p * step + r) - top) * gld<float>(first + p * step + kTileRows + r);
+  const float over = sum != 0.0f ? 1.0f / sum : 0.0f;
+  const int64_t tok = (row0 + r) / a.group;
+  const int64_t at = (q.first + tok) * a.heads + h * a.group + (row0 + r - tok * a.group);
+  for (int c = blockIdx.y * 2 + threadIdx.x / kTileRows; c < dim / 4; c += 2 * gridDim.y) {
+    f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < pieces; ++p)
+      v += __builtin_amdgcn_exp2f(gld<float>(first + p * step + r) - top) * gld<f32x4>(first + p * step + 2 * kTileRows + ((int64_t)c * kTileRows + r) * 4);
+    store4<DT>(a.out, at * dim + 4 * c, v * over);
+    if (a.lse != nullptr && c == 0) gst<float>(a.lse + at, sum != 0.0f ? (top - kLift + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY);
+  }
+}
+
+template <int DT, int NC>
+void launch(const KvAttendArgs& a, int64_t tiles, hipStream_t stream) {
+  const int64_t heads = a.cache.heads;
+  hipLaunchKernelGGL(k_kv_tiles, dim3(1), dim3(1024), 0, stream, a);
+  hipLaunchKernelGGL((k_kv_prefill<DT, NC>), dim3((unsigned)((tiles + 2 * kSlots / heads + 1) * heads)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((k_kv_join_tiles<DT>), dim3((unsigned)((kSlots / heads + 1) * heads), 4), dim3(256), 0, stream, a);
+}
+template <int DT>
+void launch_of(const KvAttendArgs& a, int64_t tiles, hipStream_t stream) {
+  if (a.cache.dim <= 64) launch<DT, 1>(a, tiles, stream);
+  else if (a.cache.dim <= 128) launch<DT, 2>(a, tiles, stream);
+  else launch<DT, 4>(a, tiles, stream);
+}
+
+int64_t pad256(int64_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+// Tiles that the call's rows can come to; one that is cut is at most twice its share in pieces.
+int64_t kv_prefill_tiles(int64_t tokens, int64_t group, int64_t seqs) {
+  return tokens * group / kTileRows + (seqs < tokens ? seqs : tokens);
+}
+static int64_t most_pieces(int64_t tiles, int64_t heads) { return tiles + 2 * kSlots / heads + 1; }
+int64_t kv_prefill_workspace(int64_t tiles, int64_t seqs, int64_t heads, int64_t dim) {
+  return 256 + pad256(4 * seqs) + pad256(32 * most_pieces(tiles, heads)) + pad256(16 * (kSlots / heads + 1)) +
+         4 * (2 * kSlots / heads + 1) * heads * kTileRows * (2 + dim);
+}
+hipError_t launch_kv_prefill(KvAttendArgs a, int dtype, int64_t tiles, void* workspace, hipStream_t stream) {
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  const int64_t heads = a.cache.heads;
+  a.tiles.count = reinterpret_cast<int32_t*>(w), w += 256;
+  a.tiles.upto = reinterpret_cast<int32_t*>(w), w += pad256(4 * (int64_t)a.seqs.seqs);
+  a.tiles.piece = reinterpret_cast<v4i*>(w), w += pad256(32 * most_pieces(tiles, heads));
+  a.tiles.cut = reinterpret_cast<v4i*>(w), w += pad256(16 * (kSlots / heads + 1));
+  a.tiles.sums = reinterpret_cast<float*>(w);
+  if (dtype == kBF16) launch_of<kBF16>(a, tiles, stream);
+  else launch_of<kF16>(a, tiles, stream);
+  return hipGetLastError();
+}
+
+}  // namespace lrq

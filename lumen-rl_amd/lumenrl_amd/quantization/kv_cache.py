@@ -33,8 +33,8 @@ _STRIDE_MAX = 1 << 40
 
 
 @functools.lru_cache(maxsize=4096)
-def _attend_workspace(tokens: int, heads: int, kv_heads: int, dim: int, seqs: int) -> int:
-    return _lib.lib().lrq_kv_attend_workspace(tokens, heads, kv_heads, dim, seqs)
+def _attend_workspace(tokens: int, heads: int, kv_heads: int, dim: int, seqs: int, one_each: bool) -> int:
+    return _lib.lib().lrq_kv_attend_workspace(tokens, heads, kv_heads, dim, seqs, one_each)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -238,7 +238,7 @@ class FP8KVCache:
         if not given:
             out = _dense((tokens, heads, dim), q.dtype, dev)
         lse = _dense((tokens, heads), torch.float32, dev) if return_lse else None
-        need = _attend_workspace(tokens, heads, self.kv_heads, dim, rows)
+        need = _attend_workspace(tokens, heads, self.kv_heads, dim, rows, offsets is None)
         work = _dense((need,), torch.uint8, dev)
         with _on(dev):
             rc = _lib.lib().lrq_kv_attend(self._ref, layer, q.data_ptr(), q.stride(0), q.stride(1), _IN_DTYPES[q.dtype], tokens, heads,

@@ -66,9 +66,9 @@ def test_attend():
         assert attend(**bad) == _lib.ERR_ARG, bad
     for bad in ({"q": ODD}, {"out": OFF4}, {"lse": ODD}, {"table": ODD}, {"ws": OFF4}):
         assert attend(**bad) == _lib.ERR_ALIGN, bad
-    need = L().lrq_kv_attend_workspace(5, 8, 2, 128, 3)
+    need = L().lrq_kv_attend_workspace(5, 8, 2, 128, 3, 0)
     assert need > 0 and attend(ws=None) == _lib.ERR_CAPACITY and attend(wb=need - 1) == _lib.ERR_CAPACITY
-    assert L().lrq_kv_attend_workspace(5, 8, 2, 300, 3) == 0 and L().lrq_kv_attend_workspace(-1, 8, 2, 128, 3) == 0
+    assert L().lrq_kv_attend_workspace(5, 8, 2, 300, 3, 0) == 0 and L().lrq_kv_attend_workspace(-1, 8, 2, 128, 3, 0) == 0
     for bad in BAD_CACHES:
         assert attend(c=cache(**bad)) == _lib.ERR_ARG, bad
     for bad in FAR_CACHES:
