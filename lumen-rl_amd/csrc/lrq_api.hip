@@ -993,7 +993,7 @@ int lrq_kv_attend(const lrq_kv_cache* cache, int64_t layer, const void* q, int64
   if (!aligned(q, 2) || !aligned(out, 8) || !aligned(lse, 4))
     return fail(LRQ_ERR_ALIGN, "kv_attend: queries must be element-aligned, the result 8-byte aligned");
   if (!strides_ok(q_token, q_head, cache->dim, tokens, heads)) return fail(LRQ_ERR_ARG, "kv_attend: strides are negative, or too large");
-  if ((tokens * (heads / cache->kv_heads) / 128 + seqs + 1024) * cache->kv_heads >= int64_t(1) << 24)
+  if ((tokens * (heads / cache->kv_heads) / 128 + seqs + 4096) * cache->kv_heads >= int64_t(1) << 24)
     return fail(LRQ_ERR_ARG, "kv_attend: %lld tokens of %lld heads are more than one launch takes", (long long)tokens, (long long)heads);
   if (int err = check_workspace("kv_attend", workspace, workspace_bytes,
                                 lrq::kv_attend_workspace(tokens, heads, cache->kv_heads, cache->dim, seqs, !offsets)))

@@ -379,9 +379,9 @@ struct KvAttendArgs {
   bool zero_rest;  // rows behind the last sequence become 0
   int few;  // rows of a sequence that k_kv_attend takes; those of more are k_kv_prefill's
   // workspace
+  int32_t* cut_count;
   uint8_t* heads_at;
   float* sums;
-  int parts, least;
   KvTiles tiles;
 };
 // one_each: one new token a sequence

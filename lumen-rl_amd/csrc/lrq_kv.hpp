@@ -21,6 +21,14 @@ namespace lrq {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// A load for the whole wave through the scalar cache, of data that no one writes meanwhile;
+// `p` is the same in all lanes.  It does not stand in the line of the vector loads: a page
+// number that a lane had to wait for would first wait for all codes asked for before it.
+template <class T>
+__device__ __forceinline__ T sld(const T* p) {
+  return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
+
 // A sequence: its new tokens are rows [first, first + n) of the call's; len counts them in.
 struct KvSeq {
   int64_t first;
@@ -48,6 +56,29 @@ __device__ __forceinline__ int kv_page(const KvSeqs& s, int pages, int b, int j)
   return (uint32_t)p < (uint32_t)pages ? p : -1;
 }
 
+// The same for one b and j in all lanes.
+__device__ __forceinline__ KvSeq kv_seq_uniform(const KvSeqs& s, int b) {
+  KvSeq q;
+  const int64_t most = (int64_t)s.width << s.shift;
+  const int64_t len = sld(s.lengths + b);
+  q.len = (int)(len < 0 ? 0 : len > most ? most : len);
+  if (s.offsets == nullptr) {
+    q.first = b;
+    q.n = b < s.tokens ? 1 : 0;
+    return q;
+  }
+  const int64_t lo = sld(s.offsets + b), hi = sld(s.offsets + b + 1);
+  q.first = lo < 0 ? 0 : lo > s.tokens ? s.tokens : lo;
+  const int64_t end = hi < q.first ? q.first : hi > s.tokens ? s.tokens : hi;
+  q.n = (int)(end - q.first);
+  return q;
+}
+__device__ __forceinline__ int kv_page_uniform(const KvSeqs& s, int pages, int b, int j) {
+  if (j >= s.width) return -1;
+  const int p = sld(s.table + (int64_t)b * s.ld + j);
+  return (uint32_t)p < (uint32_t)pages ? p : -1;
+}
+
 // Inclusive sum over the work-group's threads (256 or 1024); `waves` is LDS, one word a wave.
 template <int THREADS, class T>
 __device__ __forceinline__ T block_scan(T v, T* waves) {
@@ -64,6 +95,20 @@ __device__ __forceinline__ T block_scan(T v, T* waves) {
   for (int w = 0; w < THREADS / 64; ++w) before += w < wave ? waves[w] : T(0);
   __syncthreads();
   return v + before;
+}
+
+// The sum over the work-group's threads, for each of them.
+template <int WAVES, class T>
+__device__ __forceinline__ T block_sum(T v, T* waves) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+  __syncthreads();
+  T sum = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) sum += waves[w];
+  __syncthreads();
+  return sum;
 }
 
 // The least e in -48 .. 48 whose 448 x 2^e is not below amax (a finite value's bits).

@@ -20,6 +20,10 @@
 // result i of tile t in lane l, so that a lane's 16 probabilities are those of the 16
 // keys whose V codes it loads with one 16-byte load, in its order, and P never leaves the
 // registers.
+//
+// This kernel is for few rows a sequence, where the codes' bytes are all there is.  Its
+// waves work each for itself, with no LDS and no barrier: a wave's next 64 keys are on
+// their way into registers while it works on the present ones.
 #include "lrq_kv.hpp"
 #include "lrq_kv_attend.hpp"
 
@@ -27,9 +31,8 @@ namespace lrq {
 
 namespace {
 
-constexpr int kRows = 16;    // rows of a work-group
-constexpr int kWaves = 4;
-constexpr int kJoinTiles = 8;  // tiles of 16 channels that the waves' sums go through LDS with
+constexpr int kWaves = 4;  // of a work-group, which share the search for where they begin
+
 template <int DT>
 __device__ __forceinline__ f32x4 mma(v4u a, v4u b, f32x4 d) {
   if constexpr (DT == kBF16)
@@ -66,42 +69,74 @@ __device__ __forceinline__ Span span_of(const KvSeq& q, int window) {
   return s;
 }
 // Tiles of a sequence's rows; none where it has so many that k_kv_prefill takes them.
-__device__ __forceinline__ int64_t row_tiles(const KvSeq& q, int group, int few) {
+template <int ROWS>
+__device__ __forceinline__ int row_tiles(const KvSeq& q, int group, int few) {
   const int64_t rows = (int64_t)q.n * group;
-  return rows > few ? 0 : (rows + kRows - 1) / kRows;
+  return rows > few ? 0 : (int)((rows + ROWS - 1) / ROWS);
 }
 
 // ---------------------------------------------------------------------------
-// Work: the units of all items (sequence, KV head, 16 rows) stand in one line, which is
-// cut into equal parts, one a work-group, whatever lengths the sequences have.  Where a
-// cut falls inside an item, its parts leave unnormalized sums, which k_kv_join puts
-// together.  Part w has two places for them: 2 w for an item that an earlier part
-// began, 2 w + 1 for one that it begins and a later part ends.
+// Work: an item is a sequence, a KV head and a tile of rows; its units are cut into pieces
+// of about the same number, so that all items together make a few pieces for each wave
+// that the chip holds.  A wave takes one piece.  Pieces are numbered sequence by sequence,
+// then piece by piece, heads and tiles last: waves that run side by side read the heads
+// of the same pages.  The pieces of an item that was cut leave unnormalized sums, which
+// k_kv_join puts together.
 // ---------------------------------------------------------------------------
-constexpr int kPlaceWords = kRows * 2;  // maxima and sums; then kRows x dim
-struct Item {
-  int b, h, tile, unit;  // unit: where in the item
-  int64_t left;          // units of the item from `unit` on
+struct Work {
+  int lines, count;  // items, units of each
 };
-
+template <int ROWS>
+__device__ __forceinline__ Work work_of(const KvAttendArgs& a, const KvSeq& q) {
+  Work w;
+  w.lines = row_tiles<ROWS>(q, a.group, a.few) * a.cache.heads;
+  w.count = span_of(q, a.window).count;
+  return w;
+}
+// For k_kv_join, from the wave that has an item's first piece.
 struct PartHead {
-  int64_t first;  // the item's first row's token
-  int rows;       // rows of the tile, 0: no such item
+  int64_t first;    // the item's first row's token
+  int slot, rows;   // its place, rows of the tile
   int tile, h;
-  int parts;      // parts that hold pieces of it, the first included
+  int parts, step;  // its pieces, and from each one's place to the next one's
 };
-static_assert(sizeof(PartHead) <= 32, "the join's heads are 32 bytes apart");
+static_assert(sizeof(PartHead) == 32, "the join's heads are 32 bytes apart");
 
-template <int DT, int NC>
-__global__ __launch_bounds__(64 * kWaves) void k_kv_attend(KvAttendArgs a) {
-  constexpr int NT = 4 * NC;  // tiles of 16 channels
-  extern __shared__ float lds[];  // waves' maxima and sums, then their sums of values
+// Waves of a SIMD, by the registers they need.
+template <int NC, int MT, bool FAST>
+constexpr int kPerSimd = MT * NC > 2 ? 1 : MT * NC == 1 || (FAST && MT == 1) ? 3 : 2;
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
+}
+// Where piece i of n begins in a line of `count`: pieces differ by one at most.
+__device__ __forceinline__ int piece_at(int count, int i, int n) {
+  const int each = (int)((uint32_t)count / (uint32_t)n), rest = count - each * n;
+  return i * each + (i < rest ? i : rest);
+}
+constexpr int kParts = 256 * 4 * 4;  // pieces that all work is cut into: four for each SIMD of the chip
+
+// An address that is the same in all lanes, kept in scalar registers: loads add a lane's
+// 32-bit offset and a constant to it by themselves, up to 4095.
+__device__ __forceinline__ const uint8_t* in_scalars(const uint8_t* p) {
+  asm("" : "+s"(p));
+  return p;
+}
+
+// FAST: heads of 64 NC channels and pages of 64 keys, which are the constants of the
+// addresses then, and a page is one for the whole wave.
+template <int DT, int NC, int MT, bool FAST>
+__global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_attend(KvAttendArgs a) {
+  constexpr int NT = 4 * NC;       // tiles of 16 channels
+  constexpr int ROWS = 16 * MT;
   __shared__ int64_t scan[kWaves];
-  __shared__ int64_t found[4];
+  __shared__ uint32_t scan32[kWaves];
+  __shared__ int found[kWaves][4];
+  __shared__ uint32_t carry[2];
+  __shared__ f32x4 aside[kWaves * MT * NT * 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int shift = a.seqs.shift, S = 1 << shift, dim = a.cache.dim, group = a.group;
-  const int64_t part = blockIdx.x;
+  const int shift = FAST ? 6 : a.seqs.shift, S = 1 << shift, dim = FAST ? 64 * NC : a.cache.dim, group = a.group;
 
   // rows of the result that are no sequence's
   if (a.zero_rest) {
@@ -109,340 +144,451 @@ __global__ __launch_bounds__(64 * kWaves) void k_kv_attend(KvAttendArgs a) {
     if (a.seqs.offsets != nullptr) lo = gld<int32_t>(a.seqs.offsets + a.seqs.seqs);
     lo = lo < 0 ? 0 : lo;
     const int64_t words = (int64_t)a.heads * dim / 2;
-    for (int64_t t = lo + part; t < hi; t += gridDim.x) {
+    for (int64_t t = lo + blockIdx.x; t < hi; t += gridDim.x) {
       for (int64_t i = tid; i < words; i += 64 * kWaves) gst<uint32_t>(static_cast<uint32_t*>(a.out) + t * words + i, 0u);
       if (a.lse != nullptr)
         for (int i = tid; i < a.heads; i += 64 * kWaves) gst<float>(a.lse + t * a.heads + i, -INFINITY);
     }
   }
 
-  auto work_of = [&](int b) -> int64_t {
-    const KvSeq q = kv_seq(a.seqs, b);
-    return row_tiles(q, group, a.few) * a.cache.heads * span_of(q, a.window).count;
-  };
-  // all work, then the sequence in which this part begins
+  // all work, and the sequences that the four waves' pieces are of
+  const bool one = a.seqs.seqs <= 64 * kWaves;  // a round of the search sees all of them
+  Work mine{};
   int64_t total = 0;
   for (int b0 = 0; b0 < a.seqs.seqs; b0 += 64 * kWaves) {
-    const int64_t upto = block_scan<64 * kWaves, int64_t>(b0 + tid < a.seqs.seqs ? work_of(b0 + tid) : 0, scan);
-    if (tid == 64 * kWaves - 1) found[3] = upto;
-    __syncthreads();
-    total += found[3];
-    __syncthreads();
+    if (b0 + tid < a.seqs.seqs) mine = work_of<ROWS>(a, kv_seq(a.seqs, b0 + tid));
+    else mine = Work{};
+    total += block_sum<kWaves>((int64_t)mine.lines * mine.count, scan);
   }
-  int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  if (per < a.least) per = a.least;
-  const int64_t begin = part * per;
-  int64_t end = begin + per < total ? begin + per : total;
-  PartHead* const head = reinterpret_cast<PartHead*>(a.heads_at + 32 * part);
-  if (tid == 0) head->rows = 0;
-  if (begin >= end) return;
-  {
-    int64_t before = 0;
-    for (int b0 = 0; b0 < a.seqs.seqs; b0 += 64 * kWaves) {
-      const int64_t mine = b0 + tid < a.seqs.seqs ? work_of(b0 + tid) : 0;
-      const int64_t upto = before + block_scan<64 * kWaves, int64_t>(mine, scan);
-      if (begin >= upto - mine && begin < upto) found[0] = b0 + tid, found[1] = begin - (upto - mine);
-      if (tid == 64 * kWaves - 1) found[3] = upto;
-      __syncthreads();
-      before = found[3];
-      __syncthreads();
-      if (begin < before) break;
-    }
-  }
-  int b = __builtin_amdgcn_readfirstlane((int)found[0]);
-  int64_t inside = found[1];
+  total = uniform(total);
+  // units of a piece: below 2^31, as the items are at most a.parts times as many as that
+  const uint32_t per = total <= kParts ? 1 : (uint32_t)((total + kParts - 1) / kParts);
+  if (tid < kWaves) found[tid][0] = -1;
   __syncthreads();
-
-  for (int64_t at = begin; at < end && b < a.seqs.seqs;) {
-    const KvSeq q = kv_seq(a.seqs, b);
-    const Span span = span_of(q, a.window);
-    const int64_t tiles = row_tiles(q, group, a.few);
-    if (inside >= tiles * a.cache.heads * span.count) {  // the next sequence
-      ++b, inside = 0;
-      continue;
+  // pieces so far; and those of items that are cut, with (times 2^16) these items: at most 2 kParts of each
+  uint32_t before = 0, before_cut = 0;
+  for (int b0 = 0; b0 < a.seqs.seqs; b0 += 64 * kWaves) {
+    if (!one) {
+      if (b0 + tid < a.seqs.seqs) mine = work_of<ROWS>(a, kv_seq(a.seqs, b0 + tid));
+      else mine = Work{};
     }
-    const int64_t item = inside / span.count;
-    const int from = (int)(inside - item * span.count);
-    const int64_t most = end - at;
-    const int to = span.count - from < most ? span.count : from + (int)most;
-    const int h = (int)(item / tiles);
-    const int64_t tile = item - h * tiles;
-    const int64_t row0 = tile * kRows;
-    const int rows = (int)((int64_t)q.n * group - row0 < kRows ? (int64_t)q.n * group - row0 : kRows);
-
-    // this lane's row: token and head, and the keys [lo, hi) that it sees
-    const int64_t mine = row0 + (r < rows ? r : 0);
-    const int tok = (int)(mine / group), qh = h * group + (int)(mine - (int64_t)tok * group);
-    const int pos = q.len - q.n + tok;  // below 0: it sees none
-    const int hi = pos + 1 < 0 ? 0 : pos + 1;
-    const int lo = a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0;
-    // what the first and the last row see (rows are in the order of their tokens)
-    const int tok_a = (int)(row0 / group), tok_b = (int)((row0 + rows - 1) / group);
-    const int hi_a = q.len - q.n + tok_a + 1, hi_b = q.len - q.n + tok_b + 1;
-    const int lo_a = a.window > 0 && hi_a > a.window ? hi_a - a.window : 0;
-    const int lo_b = a.window > 0 && hi_b > a.window ? hi_b - a.window : 0;
-
-    v4u qf[NC][2];
-    {
-      const uint16_t* const src = static_cast<const uint16_t*>(a.q) + (q.first + tok) * a.q_token + qh * a.q_head;
+    const uint32_t cuts = ((uint32_t)mine.count + per - 1) / per, pieces = cuts * (uint32_t)mine.lines;
+    const uint32_t cut = cuts > 1 ? pieces + ((uint32_t)mine.lines << 16) : 0;
+    const uint32_t upto = before + block_scan<64 * kWaves, uint32_t>(pieces, scan32);
+    const uint32_t upto_cut = before_cut + block_scan<64 * kWaves, uint32_t>(cut, scan32);
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int d = 64 * c + 16 * g + 8 * k;
-          qf[c][k] = v4u{0, 0, 0, 0};
-          if (d < dim && r < rows) qf[c][k] = load_live(src + d);
-        }
+    for (int w = 0; w < kWaves; ++w) {
+      const uint32_t at = blockIdx.x * kWaves + w - (upto - pieces);  // wraps below 0
+      if (at < pieces) {
+        const uint32_t first = upto_cut - cut;
+        found[w][0] = b0 + tid, found[w][1] = (int)at, found[w][2] = (int)((first & 0xFFFF) + at), found[w][3] = (int)(first >> 16);
+      }
     }
-    float m = kLow, l = 0.0f;
-    f32x4 acc[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (tid == 64 * kWaves - 1) carry[0] = upto, carry[1] = upto_cut;
+    __syncthreads();
+    before = carry[0], before_cut = carry[1];
+    if (blockIdx.x > 0 && before > blockIdx.x * kWaves + kWaves - 1) break;
+  }
+  if (blockIdx.x == 0 && tid == 0) gst<int32_t>(a.cut_count, (int32_t)(before_cut >> 16));
+  __syncthreads();
+  const int b = uniform(found[wave][0]), place = uniform(found[wave][1]), slot = uniform(found[wave][2]);
+  if (b < 0) return;
+  const KvSeq q = kv_seq_uniform(a.seqs, b);
+  const Work work = work_of<ROWS>(a, q);
+  const int cuts = (int)(((uint32_t)work.count + per - 1) / per);
+  const int piece = place / work.lines, line = place - piece * work.lines;
+  const int tiles = work.lines / a.cache.heads;
+  const int h = line / tiles, tile = line - h * tiles;
+  const int u0 = span_of(q, a.window).first + piece_at(work.count, piece, cuts);
+  const int u1 = span_of(q, a.window).first + piece_at(work.count, piece + 1, cuts);
 
-    for (int u = from + wave; u < to; u += kWaves) {
-      const int key0 = (span.first + u) * kUnit;
-      if (key0 >= hi_b || key0 + kUnit <= lo_a) continue;  // none of the rows sees any
-      // K: this lane's row of a tile is key 16 (r / 4) + 4 t + r % 4; V: keys 16 g ..
-      const int k_key = key0 + 16 * (r >> 2), v_key = key0 + 16 * g;
-      const int k_place = k_key >> shift, v_place = v_key >> shift;
-      const int kp = k_place < a.seqs.width ? kv_page(a.seqs, a.cache.pages, b, k_place) : -1;
-      const int vp = v_place < a.seqs.width ? kv_page(a.seqs, a.cache.pages, b, v_place) : -1;
-      const uint8_t* const kb = a.cache.k + (int64_t)(kp < 0 ? 0 : kp) * a.cache.k_page +
-                                ((int64_t)h * S + (k_key & (S - 1)) + (r & 3)) * dim + 16 * g;
-      const uint8_t* const vb = a.cache.v + (int64_t)(vp < 0 ? 0 : vp) * a.cache.v_page + (int64_t)h * S * dim + r * S + (v_key & (S - 1));
-      const float ks = gld<float>(a.cache.ks + (int64_t)(vp < 0 ? 0 : vp) * a.cache.ks_page + h);
-      const float vs = gld<float>(a.cache.vs + (int64_t)(vp < 0 ? 0 : vp) * a.cache.vs_page + h);
-      v4u kr[4][NC], vr[NT];
+  // What a lane loads of a unit: K, a row of each of four tiles of 16 keys, key 16 (r / 4) +
+  // 4 t + r % 4; V, keys 16 g .. of every 16th channel.  V's codes are asked for before K's
+  // are worked on, the next unit's K before V's.
+  v4u kc[4][NC], vc[NT];
+  int kp, vp;  // the page of this lane's key of K, and of its keys of V (16 keys are of one page)
+  auto pages_at = [&](int u, int& kpage, int& vpage) {
+    if constexpr (FAST) {
+      kpage = vpage = kv_page_uniform(a.seqs, a.cache.pages, b, u);
+    } else {
+      int p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = kv_page_uniform(a.seqs, a.cache.pages, b, (u * kUnit + 16 * i) >> shift);
+      kpage = (r & 8) ? ((r & 4) ? p[3] : p[2]) : ((r & 4) ? p[1] : p[0]);
+      vpage = (g & 2) ? ((g & 1) ? p[3] : p[2]) : ((g & 1) ? p[1] : p[0]);
+    }
+  };
+  const uint32_t k_lane = (FAST ? 16 * (r >> 2) + (r & 3) : r & 3) * dim + 16 * g;
+  const uint32_t v_lane = FAST ? r * S + 16 * g : r * S;
+  auto load_k = [&](int u, int page) {
+    const uint8_t* kb = a.cache.k + (int64_t)(page < 0 ? 0 : page) * a.cache.k_page + (int64_t)h * S * dim;
+    if constexpr (FAST) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if (t % 2 == 0) kb = in_scalars(a.cache.k + (int64_t)(page < 0 ? 0 : page) * a.cache.k_page + (int64_t)h * S * dim + 4 * t * dim);
+#pragma unroll
+        for (int k = 0; k < NC; ++k) kc[t][k] = gld<v4u>(kb + k_lane + (4 * (t % 2) * dim + 64 * k));
+      }
+    } else {
+      kb += ((u * kUnit + 16 * (r >> 2)) & (S - 1)) * dim;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          kr[t][c] = v4u{0, 0, 0, 0};
-          if (64 * c + 16 * g < dim) kr[t][c] = gld<v4u>(kb + 4 * t * dim + 64 * c);
+        for (int k = 0; k < NC; ++k) {
+          kc[t][k] = v4u{0, 0, 0, 0};
+          if (64 * k + 16 * g < dim) kc[t][k] = gld<v4u>(kb + k_lane + (4 * t * dim + 64 * k));
         }
+    }
+  };
+  auto load_v = [&](int u, int page) {
+    const uint8_t* vb = a.cache.v + (int64_t)(page < 0 ? 0 : page) * a.cache.v_page + (int64_t)h * S * dim;
+    if constexpr (FAST) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        vr[n] = v4u{0, 0, 0, 0};
-        if (16 * n < dim) vr[n] = gld<v4u>(vb + (int64_t)16 * n * S);
+        if (n % 4 == 0) vb = in_scalars(a.cache.v + (int64_t)(page < 0 ? 0 : page) * a.cache.v_page + (int64_t)h * S * dim + 16 * n * S);
+        vc[n] = gld<v4u>(vb + v_lane + 16 * (n % 4) * S);
       }
+    } else {
+      vb += (u * kUnit + 16 * g) & (S - 1);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        vc[n] = v4u{0, 0, 0, 0};
+        if (16 * n < dim) vc[n] = gld<v4u>(vb + v_lane + 16 * n * S);
+      }
+    }
+  };
 
-      f32x4 s[4];
+  // this lane's rows, and the keys below hi that they see
+  int hi[MT];
+  v4u qf[MT][NC][2];
+  float m[MT], l[MT];
+  f32x4 acc[MT][NT];
+  const int64_t row0 = (int64_t)tile * ROWS, all = (int64_t)q.n * group;
+  const int rows = (int)(all - row0 < ROWS ? all - row0 : ROWS);
+  const int base = q.len - q.n + 1;  // below 1: the first tokens see nothing
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = 0; t < MT; ++t) {
+    const int64_t row = row0 + (16 * t + r < rows ? 16 * t + r : 0);
+    const int tok = (int)(row / group), qh = h * group + (int)(row - (int64_t)tok * group);
+    hi[t] = base + tok < 0 ? 0 : base + tok;
+    const uint16_t* const src = static_cast<const uint16_t*>(a.q) + (q.first + tok) * a.q_token + qh * a.q_head;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          if (64 * c >= dim) continue;
-          s[t] = mma<DT>(widen8<DT>(kr[t][c].x, kr[t][c].y), qf[c][0], s[t]);
-          s[t] = mma<DT>(widen8<DT>(kr[t][c].z, kr[t][c].w), qf[c][1], s[t]);
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int d = 64 * c + 16 * g + 8 * k;
+        qf[t][c][k] = v4u{0, 0, 0, 0};
+        if (d < dim && 16 * t + r < rows) qf[t][c][k] = load_live(src + d);
+      }
+    m[t] = kLow, l[t] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  // what the first and the last row see (rows are in the order of their tokens)
+  const int hi_a = base + (int)(row0 / group), hi_b = base + (int)((row0 + rows - 1) / group);
+  const int lo_a = a.window > 0 && hi_a > a.window ? hi_a - a.window : 0;
+  const int lo_b = a.window > 0 && hi_b > a.window ? hi_b - a.window : 0;
+  float factor, ev, back;  // of this lane's 16 keys: the scores' factor, V's exponent, its inverse
+  auto scales_of = [&](int page) {
+    const int64_t at = page < 0 ? 0 : page;
+    const float* const ksp = a.cache.ks + at * a.cache.ks_page + h;
+    const float* const vsp = a.cache.vs + at * a.cache.vs_page + h;
+    factor = (FAST ? sld(ksp) : gld<float>(ksp)) * a.scale;
+    ev = __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(FAST ? sld(vsp) : gld<float>(vsp), 0x1p-48f, 0x1p48f));
+    back = __builtin_amdgcn_exp2f(-ev);
+  };
+  auto scores = [&](f32x4 (&s)[MT][4]) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        if (64 * k >= dim) continue;
+        const v4u x = widen8<DT>(kc[j][k].x, kc[j][k].y), y = widen8<DT>(kc[j][k].z, kc[j][k].w);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          s[t][j] = mma<DT>(x, qf[t][k][0], s[t][j]);
+          s[t][j] = mma<DT>(y, qf[t][k][1], s[t][j]);
         }
       }
-      const float factor = ks * a.scale;
-      const float ev = __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(vs, 0x1p-48f, 0x1p48f));
-      const float back = __builtin_amdgcn_exp2f(-ev);
-      const bool cut = key0 + kUnit > hi_a || key0 < lo_b || __ballot(vp < 0 || kp < 0) != 0;
-      float x[16];
+  };
+  v4u p[MT][2];
+  auto soften = [&](float (&x)[16], int t) {  // from scores and exponents to p; the sums so far fade as the maximum grows
+    float top = m[t];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(s[i >> 2][i & 3], factor, ev);
-      uint32_t bad = 0;
-      if (cut) {
-        // keys before the first or behind the last that some row sees have no value
-        const int keep_hi = vp < 0 ? 0 : hi_b - v_key, keep_lo = lo_a - v_key;
-        uint32_t keep[4];
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
+    top = column_max(top);
+    const float fade = __builtin_amdgcn_exp2f(m[t] - top);
+    m[t] = top;
+    float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) keep[i] = low_bytes(keep_hi - 4 * i) & ~low_bytes(keep_lo - 4 * i);
+    for (int i = 0; i < 16; ++i) {
+      x[i] = __builtin_amdgcn_exp2f(x[i] - top + kLift);
+      sum += x[i];
+    }
+    l[t] = l[t] * fade + sum * back;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          vr[n] = v4u{vr[n].x & keep[0], vr[n].y & keep[1], vr[n].z & keep[2], vr[n].w & keep[3]};
-          bad |= nan_bytes(vr[n].x) | nan_bytes(vr[n].y) | nan_bytes(vr[n].z) | nan_bytes(vr[n].w);
-        }
+    for (int k = 0; k < 2; ++k)
+      p[t][k] = v4u{f16_pair(x[8 * k], x[8 * k + 1]), f16_pair(x[8 * k + 2], x[8 * k + 3]), f16_pair(x[8 * k + 4], x[8 * k + 5]),
+                    f16_pair(x[8 * k + 6], x[8 * k + 7])};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[t][n] *= fade;
+  };
+  auto values = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (16 * n >= dim) continue;
+      const v4u x = widen8<kF16>(vc[n].x, vc[n].y), y = widen8<kF16>(vc[n].z, vc[n].w);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        acc[t][n] = mma<kF16>(x, p[t][0], acc[t][n]);
+        acc[t][n] = mma<kF16>(y, p[t][1], acc[t][n]);
+      }
+    }
+  };
+  // units that some row sees a part of, or whose pages are not all there
+  auto is_cut = [&](int u) {
+    const bool gone = FAST ? vp < 0 : __ballot(vp < 0) != 0;
+    return u * kUnit + kUnit > hi_a || u * kUnit < lo_b || gone;
+  };
+
+  int u = u0;
+  pages_at(u, kp, vp);
+  while (u < u1) {
+    if (is_cut(u)) {
+      const int v_key = u * kUnit + 16 * g, v_now = vp;
+      const bool ok = vp >= 0;
+      load_k(u, kp);
+      load_v(u, vp);
+      scales_of(vp);
+      f32x4 s[MT][4];
+      scores(s);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        float x[16];
+        const int lo = a.window > 0 && hi[t] > a.window ? hi[t] - a.window : 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int key = v_key + i;
-          x[i] = key < hi && key >= lo && vp >= 0 ? x[i] : -INFINITY;
+          x[i] = key < hi[t] && key >= lo && ok ? __builtin_fmaf(s[t][i >> 2][i & 3], factor, ev) : -INFINITY;
         }
+        soften(x, t);
       }
-      float top = m;
+      // keys before the first or behind the last that some row sees have no value
+      const int keep_hi = ok ? hi_b - v_key : 0, keep_lo = lo_a - v_key;
+      uint32_t keep[4], bad = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
-      top = column_max(top);
-      const float fade = __builtin_amdgcn_exp2f(m - top);
-      m = top;
-      float sum = 0.0f;
+      for (int i = 0; i < 4; ++i) keep[i] = low_bytes(keep_hi - 4 * i) & ~low_bytes(keep_lo - 4 * i);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(x[i] - top + kLift);
-        sum += x[i];
+      for (int n = 0; n < NT; ++n) {
+        vc[n] = v4u{vc[n].x & keep[0], vc[n].y & keep[1], vc[n].z & keep[2], vc[n].w & keep[3]};
+        bad |= nan_bytes(vc[n].x) | nan_bytes(vc[n].y) | nan_bytes(vc[n].z) | nan_bytes(vc[n].w);
       }
-      l = l * fade + sum * back;
-      v4u p[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        p[k] = v4u{f16_pair(x[8 * k], x[8 * k + 1]), f16_pair(x[8 * k + 2], x[8 * k + 3]), f16_pair(x[8 * k + 4], x[8 * k + 5]),
-                   f16_pair(x[8 * k + 6], x[8 * k + 7])};
-#pragma unroll
-      for (int n = 0; n < NT; ++n) acc[n] *= fade;
-      if (__ballot(bad != 0) != 0) {
-        // NaN codes that some rows see and others do not: 0 x NaN must not reach the
-        // others, so they are counted by a product of their own
-        v4u see[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = v_key + 8 * k + 2 * i;
-            w[i] = (key < hi && key >= lo ? 0x3C00u : 0u) | (key + 1 < hi && key + 1 >= lo ? 0x3C000000u : 0u);
-          }
-          see[k] = v4u{w[0], w[1], w[2], w[3]};
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (16 * n >= dim) continue;
-          f32x4 hits = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          const uint32_t w[4] = {vr[n].x, vr[n].y, vr[n].z, vr[n].w};
-          uint32_t is[4], no[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t b80 = nan_bytes(w[i]);
-            is[i] = (b80 >> 7) * 0x38u;                       // the code of 1
-            no[i] = w[i] & ~((b80 >> 7) * 0xFFu);
-          }
-          hits = mma<kF16>(widen8<kF16>(is[0], is[1]), see[0], hits);
-          hits = mma<kF16>(widen8<kF16>(is[2], is[3]), see[1], hits);
-          acc[n] = mma<kF16>(widen8<kF16>(no[0], no[1]), p[0], acc[n]);
-          acc[n] = mma<kF16>(widen8<kF16>(no[2], no[3]), p[1], acc[n]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[n][i] = hits[i] > 0.0f ? __builtin_nanf("") : acc[n][i];
-        }
+      if (__ballot(bad != 0) == 0) {
+        values();
       } else {
+        // NaN codes that some rows see and others do not: 0 x NaN must not reach the
+        // others.  So each token's rows get sums of their own, over what that token sees.
+        // (By way of LDS, so that this rare path needs few registers of the others'.)
+        f32x4* const mine = aside + wave * (MT * NT * 64) + lane;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (16 * n >= dim) continue;
-          acc[n] = mma<kF16>(widen8<kF16>(vr[n].x, vr[n].y), p[0], acc[n]);
-          acc[n] = mma<kF16>(widen8<kF16>(vr[n].z, vr[n].w), p[1], acc[n]);
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mine[(t * NT + n) * 64] = acc[t][n];
+        const uint8_t* const vb = a.cache.v + (int64_t)(v_now < 0 ? 0 : v_now) * a.cache.v_page + (int64_t)h * S * dim + r * S + (v_key & (S - 1));
+#pragma unroll 1
+        for (int n = 0; 16 * n < dim; ++n) {
+          const v4u w = gld<v4u>(vb + (int64_t)16 * n * S);
+#pragma unroll 1
+          for (int see = hi_a < 1 ? 1 : hi_a; see <= hi_b; ++see) {
+            const int see_hi = ok ? see - v_key : 0, see_lo = (a.window > 0 && see > a.window ? see - a.window : 0) - v_key;
+            uint32_t some[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) some[i] = low_bytes(see_hi - 4 * i) & ~low_bytes(see_lo - 4 * i);
+            const v4u x = widen8<kF16>(w.x & some[0], w.y & some[1]), y = widen8<kF16>(w.z & some[2], w.w & some[3]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              const f32x4 was = mine[(t * NT + n) * 64];
+              const f32x4 sums = mma<kF16>(y, p[t][1], mma<kF16>(x, p[t][0], was));
+              if (hi[t] == see) mine[(t * NT + n) * 64] = sums;
+            }
+          }
         }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) acc[t][n] = mine[(t * NT + n) * 64];
       }
+      if (++u < u1) pages_at(u, kp, vp);
+      continue;
     }
-    l = column_sum(l);
-
-    // the waves' sums together, 128 channels at a time: wave w adds up tiles w, w + 4, ..
-    float* const tops = lds;                       // [wave][row] maxima, then sums
-    float* const vals = lds + 2 * kWaves * kRows;  // [wave][channel / 4][row][4]
-    if (g == 0) tops[wave * kRows + r] = m, tops[(kWaves + wave) * kRows + r] = l;
-    const bool whole = from == 0 && to == span.count, starts = from == 0;
-    const int64_t place = 2 * part + (starts ? 1 : 0);
-    float* const out = a.sums + place * (kPlaceWords + (int64_t)kRows * dim);
-    float all = kLow, sum = 0.0f;
+    // a run of units that all rows see the whole of
+    load_k(u, kp);
+    bool more = true;
+    while (more) {
+      load_v(u, vp);
+      scales_of(vp);
+      more = ++u < u1;
+      if (more) pages_at(u, kp, vp), more = !is_cut(u);
+      __builtin_amdgcn_sched_barrier(0);
+      f32x4 s[MT][4];
+      scores(s);
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) load_k(u, kp);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int n0 = 0; n0 < NT; n0 += kJoinTiles) {
-      if (16 * n0 >= dim) continue;
-      if (n0 > 0) __syncthreads();
+      for (int t = 0; t < MT; ++t) {
+        float x[16];
 #pragma unroll
-      for (int n = n0; n < n0 + kJoinTiles && n < NT; ++n)
-        if (16 * n < dim) *reinterpret_cast<f32x4*>(vals + ((wave * 4 * kJoinTiles + 4 * (n - n0) + g) * kRows + r) * 4) = acc[n];
-      __syncthreads();
-      all = tops[r];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) all = fmaxf(all, tops[w * kRows + r]);
-      float part_of[kWaves];
-      sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        part_of[w] = __builtin_amdgcn_exp2f(tops[w * kRows + r] - all);
-        sum += part_of[w] * tops[(kWaves + w) * kRows + r];
+        for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(s[t][i >> 2][i & 3], factor, ev);
+        soften(x, t);
       }
+      values();
+    }
+  }
+
+  const bool whole = cuts == 1;
+  float* const out = a.sums + slot * ((2 + (int64_t)dim) * ROWS);
+  if (lane == 0 && piece == 0 && !whole)
+    reinterpret_cast<PartHead*>(a.heads_at)[found[wave][3] + line] = PartHead{q.first, slot, rows, tile, h, cuts, work.lines};
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const float sum = column_sum(l[t]);
+    if (16 * t + r >= rows) continue;
+    const int64_t row = row0 + 16 * t + r, tok = row / group;
+    const int64_t at_row = (q.first + tok) * a.heads + h * group + (row - tok * group);
+    if (whole) {
       const float over = sum != 0.0f ? 1.0f / sum : 0.0f;  // a row that sees nothing is 0
 #pragma unroll
-      for (int n = 0; n < kJoinTiles / kWaves; ++n) {
-        const int t = wave + kWaves * n, ch = 16 * (n0 + t) + 4 * g;
-        if (16 * (n0 + t) >= dim) continue;
-        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int n = 0; n < NT; ++n)
+        if (16 * n < dim) store4<DT>(a.out, at_row * dim + 16 * n + 4 * g, acc[t][n] * over);
+      if (a.lse != nullptr && g == 0)
+        gst<float>(a.lse + at_row, sum != 0.0f ? (m[t] - kLift + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY);
+    } else {
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w)
-          v += part_of[w] * *reinterpret_cast<const f32x4*>(vals + ((w * 4 * kJoinTiles + 4 * t + g) * kRows + r) * 4);
-        if (!whole) gst<f32x4>(out + kPlaceWords + (ch / 4 * kRows + r) * 4, v);
-        else if (r < rows) store4<DT>(a.out, ((q.first + tok) * a.heads + qh) * dim + ch, v * over);
-      }
+      for (int n = 0; n < NT; ++n)
+        if (16 * n < dim) gst<f32x4>(out + 2 * ROWS + ((4 * n + g) * ROWS + 16 * t + r) * 4, acc[t][n]);
+      if (g == 0) gst<float>(out + 16 * t + r, m[t]), gst<float>(out + ROWS + 16 * t + r, sum);
     }
-    if (wave == 0 && g == 0) {
-      if (!whole) {
-        gst<float>(out + r, all), gst<float>(out + kRows + r, sum);
-      } else if (a.lse != nullptr && r < rows) {
-        gst<float>(a.lse + (q.first + tok) * a.heads + qh,
-                   sum != 0.0f ? (all - kLift + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY);
-      }
-    }
-    if (tid == 0 && starts && !whole) {
-      head->first = q.first, head->tile = (int)tile, head->h = h;
-      // the units behind this part's, over the parts that follow
-      head->parts = 1 + (int)((span.count - to + per - 1) / per);
-      head->rows = rows;
-    }
-    __syncthreads();  // before LDS is written again
-    at += to - from;
-    inside += to - from;
   }
 }
 
-// Items that were cut: their parts' sums, brought to one maximum.  Work-group w looks
-// after the item that part w began.
-template <int DT>
+// Items that were cut: their pieces' sums, brought to one maximum.  A thread has four
+// channels of a row, and where there are fewer of these than threads, a share of the pieces.
+template <int DT, int MT>
 __global__ __launch_bounds__(256) void k_kv_join(KvAttendArgs a) {
-  const PartHead head = *reinterpret_cast<const PartHead*>(a.heads_at + 32 * (int64_t)blockIdx.x);
-  if (head.rows == 0) return;
-  const int dim = a.cache.dim;
-  const int64_t step = kPlaceWords + (int64_t)kRows * dim;
-  const float* const first = a.sums + (2 * (int64_t)blockIdx.x + 1) * step;
-  const float* const rest = a.sums + 2 * (int64_t)blockIdx.x * step;  // part i at 2 i steps
-  for (int i = threadIdx.x; i < dim / 4 * kRows; i += 256) {
-    const int r = i % kRows, c = i / kRows;
-    float top = gld<float>(first + r);
-    for (int p = 1; p < head.parts; ++p) top = fmaxf(top, gld<float>(rest + 2 * p * step + r));
-    float sum = 0.0f;
-    f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = 0; p < head.parts; ++p) {
-      const float* const at = p == 0 ? first : rest + 2 * p * step;
-      const float f = __builtin_amdgcn_exp2f(gld<float>(at + r) - top);
-      sum += f * gld<float>(at + kRows + r);
-      v += f * gld<f32x4>(at + kPlaceWords + i * 4);
+  constexpr int ROWS = 16 * MT;
+  __shared__ f32x4 vals[256];
+  __shared__ float tops[256], sums[256];
+  const int tid = threadIdx.x, dim = a.cache.dim;
+  const int64_t size = (2 + (int64_t)dim) * ROWS;
+  const int quads = dim / 4 / gridDim.y;  // of channels, from c0 on
+  const int c0 = blockIdx.y * quads;
+  const int count = gld<int32_t>(a.cut_count);
+  for (int i = blockIdx.x; i < count; i += gridDim.x) {
+    const PartHead head = reinterpret_cast<const PartHead*>(a.heads_at)[i];
+    const int all = head.rows * quads, shares = all < 256 ? 256 / all : 1;
+    const float* const first = a.sums + head.slot * size;
+    const int64_t step = head.step * size;
+    for (int o0 = 0; o0 < all; o0 += 256) {
+      const int o = all < 256 ? tid % all : o0 + tid, share = all < 256 ? tid / all : 0;
+      const int r = o / quads, c = c0 + o - r * quads;
+      const bool mine = o < all && share < shares;
+      float top = kLow, sum = 0.0f;
+      f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (mine) {
+#pragma unroll 4
+        for (int p = share; p < head.parts; p += shares) {
+          const float* const at = first + p * step;
+          const float m = gld<float>(at + r), l = gld<float>(at + ROWS + r);
+          const f32x4 x = gld<f32x4>(at + 2 * ROWS + (c * ROWS + r) * 4);
+          const float more = fmaxf(top, m);
+          const float f = __builtin_amdgcn_exp2f(top - more), e = __builtin_amdgcn_exp2f(m - more);
+          sum = sum * f + l * e, v = v * f + x * e;
+          top = more;
+        }
+      }
+      if (shares > 1) {
+        __syncthreads();
+        vals[tid] = v, tops[tid] = top, sums[tid] = sum;
+        __syncthreads();
+        if (share == 0) {
+          float more = top;
+          for (int k = 1; k < shares; ++k) more = fmaxf(more, tops[tid + k * all]);
+          const float f = __builtin_amdgcn_exp2f(top - more);
+          sum *= f, v *= f;
+          for (int k = 1; k < shares; ++k) {
+            const float e = __builtin_amdgcn_exp2f(tops[tid + k * all] - more);
+            sum += sums[tid + k * all] * e, v += vals[tid + k * all] * e;
+          }
+          top = more;
+        }
+      }
+      if (mine && share == 0) {
+        const int64_t row = (int64_t)head.tile * ROWS + r, tok = row / a.group;
+        const int64_t at = (head.first + tok) * a.heads + head.h * a.group + (row - tok * a.group);
+        store4<DT>(a.out, at * dim + 4 * c, v * (sum != 0.0f ? 1.0f / sum : 0.0f));
+        if (a.lse != nullptr && c == 0) gst<float>(a.lse + at, sum != 0.0f ? (top - kLift + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY);
+      }
     }
-    if (r >= head.rows) continue;
-    const int64_t row = (int64_t)head.tile * kRows + r;
-    const int64_t tok = row / a.group;
-    const int64_t at = (head.first + tok) * a.heads + head.h * a.group + (row - tok * a.group);
-    store4<DT>(a.out, at * dim + 4 * c, v * (sum != 0.0f ? 1.0f / sum : 0.0f));
-    if (a.lse != nullptr && c == 0)
-      gst<float>(a.lse + at, sum != 0.0f ? (top - kLift + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY);
   }
 }
 
-template <int DT, int NC>
-void launch(const KvAttendArgs& a, hipStream_t stream) {
-  const unsigned lds = 4 * (2 * kWaves * kRows + kWaves * kRows * 16 * kJoinTiles);
-  hipLaunchKernelGGL((k_kv_attend<DT, NC>), dim3(a.parts), dim3(64 * kWaves), lds, stream, a);
-  hipLaunchKernelGGL((k_kv_join<DT>), dim3(a.parts), dim3(256), 0, stream, a);
+constexpr int kMostRows = 64;  // of a sequence, that k_kv_attend takes if k_kv_prefill is there
+
+// Items of a call at most, and its pieces: an item of n units is cut into less than n / per + 1.
+int64_t most_items(int64_t tokens, int64_t group, int64_t heads, int64_t seqs) {
+  const int64_t some = seqs < tokens ? seqs : tokens;
+  int64_t tiles = tokens * group / 16 + some;
+  if (tiles > some * (kMostRows / 16)) tiles = some * (kMostRows / 16);
+  return tiles * heads;
+}
+int64_t most_pieces(int64_t items, int64_t width, int shift) {
+  const int64_t units = items * ((width << shift) / kUnit + 1);
+  return units < items + kParts ? units : items + kParts;
+}
+// Those that leave sums are of items of more than per units, twice their share at most.
+constexpr int64_t kPlaces = 2 * kParts;
+
+template <int DT, int NC, int MT>
+void launch(KvAttendArgs a, hipStream_t stream) {
+  const int64_t pieces = most_pieces(most_items(a.seqs.tokens, a.group, a.cache.heads, a.seqs.seqs), a.seqs.width, a.seqs.shift);
+  const int64_t groups = pieces > 0 ? (pieces + kWaves - 1) / kWaves : 1;
+  // few items: a work-group for 32 channels of each
+  const int64_t items = most_items(a.seqs.tokens, a.group, a.cache.heads, a.seqs.seqs);
+  const int64_t joins = items < 2048 ? items : 2048;
+  const int split = items <= 256 && a.cache.dim % 32 == 0 ? a.cache.dim / 32 : 1;
+  if (a.cache.dim == 64 * NC && a.seqs.shift == 6)
+    hipLaunchKernelGGL((k_kv_attend<DT, NC, MT, true>), dim3((unsigned)groups), dim3(64 * kWaves), 0, stream, a);
+  else
+    hipLaunchKernelGGL((k_kv_attend<DT, NC, MT, false>), dim3((unsigned)groups), dim3(64 * kWaves), 0, stream, a);
+  if (joins > 0) hipLaunchKernelGGL((k_kv_join<DT, MT>), dim3((unsigned)joins, split), dim3(256), 0, stream, a);
+}
+template <int DT, int MT>
+void launch_dim(const KvAttendArgs& a, hipStream_t stream) {
+  if (a.cache.dim <= 64) launch<DT, 1, MT>(a, stream);
+  else if (a.cache.dim <= 128) launch<DT, 2, MT>(a, stream);
+  else launch<DT, 4, 1>(a, stream);  // the registers of two tiles are not there
 }
 template <int DT>
 void launch_of(const KvAttendArgs& a, hipStream_t stream) {
-  if (a.cache.dim <= 64) launch<DT, 1>(a, stream);
-  else if (a.cache.dim <= 128) launch<DT, 2>(a, stream);
-  else launch<DT, 4>(a, stream);
+  // two tiles of 16 rows a wave where a sequence has more than one
+  const int64_t rows = a.seqs.offsets == nullptr ? a.group : a.seqs.tokens * a.group / (a.seqs.seqs > 0 ? a.seqs.seqs : 1);
+  if (rows > 16) launch_dim<DT, 2>(a, stream);
+  else launch_dim<DT, 1>(a, stream);
 }
 
-constexpr unsigned kParts = 512;  // two work-groups a compute unit
-
-// Sequences of more rows than this are k_kv_prefill's, if the call has as many.
-constexpr int kFew = 64;
-
-int64_t few_workspace(int64_t dim) { return kParts * 32 + 2 * kParts * 4 * (kPlaceWords + kRows * dim); }
+int64_t few_workspace(int64_t dim) { return 256 + kPlaces * 32 + 4 * kPlaces * (dim <= 128 ? 32 : 16) * (2 + dim); }
 
 }  // namespace
 
 int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, bool one_each) {
   const int64_t group = heads / kv_heads, rows = (one_each ? 1 : tokens) * group;
   int64_t need = few_workspace(dim);
-  if (rows > kFew) {
+  if (rows > kMostRows) {
     const int64_t many = kv_prefill_workspace(kv_prefill_tiles(tokens, group, seqs), seqs, kv_heads, dim);
     if (many > need) need = many;
   }
@@ -452,14 +598,13 @@ int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int
 hipError_t launch_kv_attend(KvAttendArgs a, int dtype, void* workspace, hipStream_t stream) {
   // no sequence has more rows than the call
   const int64_t most = a.seqs.offsets == nullptr ? a.group : a.seqs.tokens * a.group;
-  a.few = most > kFew ? kFew : INT32_MAX;
-  a.heads_at = static_cast<uint8_t*>(workspace);
-  a.sums = reinterpret_cast<float*>(a.heads_at + kParts * 32);
-  a.parts = kParts;
-  a.least = kWaves;
+  a.few = kMostRows;
+  a.cut_count = static_cast<int32_t*>(workspace);
+  a.heads_at = static_cast<uint8_t*>(workspace) + 256;
+  a.sums = reinterpret_cast<float*>(a.heads_at + kPlaces * 32);
   if (dtype == kBF16) launch_of<kBF16>(a, stream);
   else launch_of<kF16>(a, stream);
-  if (most > kFew) {
+  if (most > kMostRows) {
     // the workspace is used again: the stream keeps the two in order
     if (hipError_t e = launch_kv_prefill(a, dtype, kv_prefill_tiles(a.seqs.tokens, a.group, a.seqs.seqs), workspace, stream)) return e;
   }
