@@ -104,7 +104,7 @@ static_assert(sizeof(PartHead) == 32, "the join's heads are 32 bytes apart");
 
 // Waves of a SIMD, by the registers they need.
 template <int NC, int MT, bool FAST>
-constexpr int kPerSimd = MT * NC > 2 ? 1 : MT * NC == 1 || (FAST && MT == 1) ? 3 : 2;
+constexpr int kPerSimd = MT * NC > 2 ? 1 : MT * NC == 1 || (FAST && MT == 1) ? 2 : 2;
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
@@ -114,13 +114,24 @@ __device__ __forceinline__ int piece_at(int count, int i, int n) {
   const int each = (int)((uint32_t)count / (uint32_t)n), rest = count - each * n;
   return i * each + (i < rest ? i : rest);
 }
-constexpr int kParts = 256 * 4 * 4;  // pieces that all work is cut into: four for each SIMD of the chip
+// Pieces that all work is cut into: three for each SIMD of the chip, of which two run at a
+// time (256 sequences of up to 8100 keys: 2, 3, 4, 6 and 8 a SIMD take 428, 403, 408, 411 and
+// 423 us; one wave a SIMD 411, three 461).
+constexpr int kParts = 256 * 4 * 3;
+constexpr uint32_t kLeast = 2;  // units of a piece, if the item has as many
 
 // An address that is the same in all lanes, kept in scalar registers: loads add a lane's
 // 32-bit offset and a constant to it by themselves, up to 4095.
 __device__ __forceinline__ const uint8_t* in_scalars(const uint8_t* p) {
   asm("" : "+s"(p));
   return p;
+}
+
+// One tile of rows a sequence: each code is read once, past the caches (256 sequences of up to
+// 8100 keys 416 -> 408 us).  More tiles find them in the caches.
+template <int MT>
+__device__ __forceinline__ v4u codes_at(const uint8_t* p) {
+  return MT == 1 ? gld_nt<v4u>(p) : gld<v4u>(p);
 }
 
 // FAST: heads of 64 NC channels and pages of 64 keys, which are the constants of the
@@ -162,7 +173,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
   }
   total = uniform(total);
   // units of a piece: below 2^31, as the items are at most a.parts times as many as that
-  const uint32_t per = total <= kParts ? 1 : (uint32_t)((total + kParts - 1) / kParts);
+  const uint32_t per = total <= kLeast * kParts ? kLeast : (uint32_t)((total + kParts - 1) / kParts);
   if (tid < kWaves) found[tid][0] = -1;
   __syncthreads();
   // pieces so far; and those of items that are cut, with (times 2^16) these items: at most 2 kParts of each
@@ -227,7 +238,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
       for (int t = 0; t < 4; ++t) {
         if (t % 2 == 0) kb = in_scalars(a.cache.k + (int64_t)(page < 0 ? 0 : page) * a.cache.k_page + (int64_t)h * S * dim + 4 * t * dim);
 #pragma unroll
-        for (int k = 0; k < NC; ++k) kc[t][k] = gld<v4u>(kb + k_lane + (4 * (t % 2) * dim + 64 * k));
+        for (int k = 0; k < NC; ++k) kc[t][k] = codes_at<MT>(kb + k_lane + (4 * (t % 2) * dim + 64 * k));
       }
     } else {
       kb += ((u * kUnit + 16 * (r >> 2)) & (S - 1)) * dim;
@@ -236,7 +247,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
           kc[t][k] = v4u{0, 0, 0, 0};
-          if (64 * k + 16 * g < dim) kc[t][k] = gld<v4u>(kb + k_lane + (4 * t * dim + 64 * k));
+          if (64 * k + 16 * g < dim) kc[t][k] = codes_at<MT>(kb + k_lane + (4 * t * dim + 64 * k));
         }
     }
   };
@@ -246,14 +257,14 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if (n % 4 == 0) vb = in_scalars(a.cache.v + (int64_t)(page < 0 ? 0 : page) * a.cache.v_page + (int64_t)h * S * dim + 16 * n * S);
-        vc[n] = gld<v4u>(vb + v_lane + 16 * (n % 4) * S);
+        vc[n] = codes_at<MT>(vb + v_lane + 16 * (n % 4) * S);
       }
     } else {
       vb += (u * kUnit + 16 * g) & (S - 1);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         vc[n] = v4u{0, 0, 0, 0};
-        if (16 * n < dim) vc[n] = gld<v4u>(vb + v_lane + 16 * n * S);
+        if (16 * n < dim) vc[n] = codes_at<MT>(vb + v_lane + 16 * n * S);
       }
     }
   };
@@ -537,13 +548,17 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttendArgs a) {
   }
 }
 
-constexpr int kMostRows = 64;  // of a sequence, that k_kv_attend takes if k_kv_prefill is there
+// Sequences of more rows than kMostRows are k_kv_prefill's, but not in a call whose rows
+// are kAllRows together at most: three launches less.
+constexpr int kMostRows = 64, kAllRows = 1024;
+// Rows of a call; one_each: one token a sequence.
+int64_t all_rows(int64_t tokens, int64_t seqs, bool one_each, int64_t group) { return (one_each && seqs < tokens ? seqs : tokens) * group; }
+bool all_few(int64_t rows, bool one_each, int64_t group) { return one_each ? group <= kMostRows : rows <= kAllRows; }
 
 // Items of a call at most, and its pieces: an item of n units is cut into less than n / per + 1.
-int64_t most_items(int64_t tokens, int64_t group, int64_t heads, int64_t seqs) {
-  const int64_t some = seqs < tokens ? seqs : tokens;
-  int64_t tiles = tokens * group / 16 + some;
-  if (tiles > some * (kMostRows / 16)) tiles = some * (kMostRows / 16);
+int64_t most_items(int64_t rows, int64_t heads, int64_t seqs, bool all) {
+  int64_t tiles = rows / 16 + seqs;
+  if (!all && tiles > seqs * (kMostRows / 16)) tiles = seqs * (kMostRows / 16);
   return tiles * heads;
 }
 int64_t most_pieces(int64_t items, int64_t width, int shift) {
@@ -555,10 +570,13 @@ constexpr int64_t kPlaces = 2 * kParts;
 
 template <int DT, int NC, int MT>
 void launch(KvAttendArgs a, hipStream_t stream) {
-  const int64_t pieces = most_pieces(most_items(a.seqs.tokens, a.group, a.cache.heads, a.seqs.seqs), a.seqs.width, a.seqs.shift);
+  const int64_t seqs = a.seqs.seqs < a.seqs.tokens ? a.seqs.seqs : a.seqs.tokens;  // others have no new token
+  const bool one_each = a.seqs.offsets == nullptr;
+  const int64_t rows = all_rows(a.seqs.tokens, a.seqs.seqs, one_each, a.group);
+  const int64_t items = most_items(rows, a.cache.heads, seqs, a.few == INT32_MAX);
+  const int64_t pieces = most_pieces(items, a.seqs.width, a.seqs.shift);
   const int64_t groups = pieces > 0 ? (pieces + kWaves - 1) / kWaves : 1;
   // few items: a work-group for 32 channels of each
-  const int64_t items = most_items(a.seqs.tokens, a.group, a.cache.heads, a.seqs.seqs);
   const int64_t joins = items < 2048 ? items : 2048;
   const int split = items <= 256 && a.cache.dim % 32 == 0 ? a.cache.dim / 32 : 1;
   if (a.cache.dim == 64 * NC && a.seqs.shift == 6)
@@ -586,9 +604,9 @@ int64_t few_workspace(int64_t dim) { return 256 + kPlaces * 32 + 4 * kPlaces * (
 }  // namespace
 
 int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, bool one_each) {
-  const int64_t group = heads / kv_heads, rows = (one_each ? 1 : tokens) * group;
+  const int64_t group = heads / kv_heads;
   int64_t need = few_workspace(dim);
-  if (rows > kMostRows) {
+  if (!all_few(all_rows(tokens, seqs, one_each, group), one_each, group)) {
     const int64_t many = kv_prefill_workspace(kv_prefill_tiles(tokens, group, seqs), seqs, kv_heads, dim);
     if (many > need) need = many;
   }
@@ -596,15 +614,15 @@ int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int
 }
 
 hipError_t launch_kv_attend(KvAttendArgs a, int dtype, void* workspace, hipStream_t stream) {
-  // no sequence has more rows than the call
-  const int64_t most = a.seqs.offsets == nullptr ? a.group : a.seqs.tokens * a.group;
-  a.few = kMostRows;
+  const bool one_each = a.seqs.offsets == nullptr;
+  const bool all = all_few(all_rows(a.seqs.tokens, a.seqs.seqs, one_each, a.group), one_each, a.group);
+  a.few = all ? INT32_MAX : kMostRows;
   a.cut_count = static_cast<int32_t*>(workspace);
   a.heads_at = static_cast<uint8_t*>(workspace) + 256;
   a.sums = reinterpret_cast<float*>(a.heads_at + kPlaces * 32);
   if (dtype == kBF16) launch_of<kBF16>(a, stream);
   else launch_of<kF16>(a, stream);
-  if (most > kMostRows) {
+  if (!all) {
     // the workspace is used again: the stream keeps the two in order
     if (hipError_t e = launch_kv_prefill(a, dtype, kv_prefill_tiles(a.seqs.tokens, a.group, a.seqs.seqs), workspace, stream)) return e;
   }
