@@ -14,6 +14,10 @@
 // the halves of a lane pair hold of P.  A row's place in an operand is moved by twice the piece's
 // number modulo 4, so that eight lanes that write four pieces of two rows meet eight places.
 // While a tile is worked on, the next one's codes are on their way into registers.
+//
+// In units that some rows see only a part of, NaN codes of V are taken as 0 and a flag is
+// left: 0 x NaN must not reach rows that do not see it.  The last launch, k_kv_nan, then looks
+// for them again and writes NaN to the rows that do.
 #include "lrq_kv.hpp"
 #include "lrq_kv_attend.hpp"
 
@@ -80,7 +84,7 @@ __global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
   const KvTiles& p = a.tiles;
   const int tid = threadIdx.x, seqs = a.seqs.seqs;
   // upto[b]: tiles of the sequences 0 .. b
-  if (tid == 0) carry = 0, counts[0] = counts[1] = 0;
+  if (tid == 0) carry = 0, counts[0] = counts[1] = 0, gst<int32_t>(p.count + 2, 0);
   bucket[tid] = 0;
   __syncthreads();
   for (int b0 = 0; b0 < seqs; b0 += 1024) {
@@ -151,16 +155,16 @@ __global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
   if (tid == 0) gst<int32_t>(p.count + 1, (int32_t)counts[1]);
 }
 
-template <int DT, int NC>
+// FULL: heads of 64 NC channels.
+template <int DT, int NC, bool FULL>
 __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs a) {
   constexpr int KS = 4 * NC, VT = 2 * NC;       // steps of 16 channels, tiles of 32
   constexpr int kStage = (2 * KS + 4 * VT) * 64;  // 16-byte places of a tile: K's operands, then V's
   __shared__ __attribute__((aligned(16))) v4u stage[2][kStage];
   __shared__ __attribute__((aligned(16))) float page_of[2][12];  // per 16 keys: factor, exponent, its inverse
-  __shared__ int has_nan[2];  // a stage's unit + 1, if it has NaN codes that some rows may not see
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, half = lane >> 5;
-  const int heads = a.cache.heads, dim = a.cache.dim, shift = a.seqs.shift, S = 1 << shift, group = a.group;
+  const int heads = a.cache.heads, dim = FULL ? 64 * NC : a.cache.dim, shift = a.seqs.shift, S = 1 << shift, group = a.group;
   const int count = gld<int32_t>(a.tiles.count);
   const int h = blockIdx.x % heads, idx = blockIdx.x / heads;
   if (idx >= count) return;
@@ -247,7 +251,9 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
       v4u w = v_ok ? vr[i] : v4u{0, 0, 0, 0};
       if (cut) {
         w = v4u{w.x & keep[0], w.y & keep[1], w.z & keep[2], w.w & keep[3]};
-        bad |= nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
+        const v4u nan = v4u{nan_bytes(w.x), nan_bytes(w.y), nan_bytes(w.z), nan_bytes(w.w)} >> 7;
+        bad |= nan.x | nan.y | nan.z | nan.w;
+        w &= ~(nan * 0xFF);
       }
       const int d = 64 * i + k_tok;
       v4u* const to = st + 2 * KS * 64 + ((d >> 5) * 4 + c4) * 64 + ((d & 31) ^ (2 * c4));
@@ -255,7 +261,7 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
       to[0] = v4u{x.x, x.y, y.x, y.y};
       to[32] = v4u{x.z, x.w, y.z, y.w};
     }
-    if (bad != 0) has_nan[at] = u + 1;
+    if (bad != 0) gst<int32_t>(a.tiles.count + 2, 1);
     if (tid < 4) {
       const float ev = __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(vs, 0x1p-48f, 0x1p48f));
       page_of[at][tid] = fmaxf(ks * scale, 0x1p-120f);  // above 0, so that no key stays no key
@@ -268,8 +274,6 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
   f32x16 acc[VT];
 #pragma unroll
   for (int n = 0; n < VT; ++n) acc[n] = f32x16{};
-  if (tid < 2) has_nan[tid] = 0;
-  __syncthreads();
   if (u0 < u1) {
     look_up(u0);
     load(u0);
@@ -338,43 +342,11 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
       l = __builtin_fmaf(sum, back[e], l);
       p[e] = v4u{f16_pair(x[0], x[1]), f16_pair(x[2], x[3]), f16_pair(x[4], x[5]), f16_pair(x[6], x[7])};
     }
-    if (__builtin_amdgcn_readfirstlane(has_nan[at]) != u + 1) {
 #pragma unroll
-      for (int n = 0; n < VT; ++n)
+    for (int n = 0; n < VT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (32 * n < dim) acc[n] = mma32<kF16>(vst[(n * 4 + e) * 64 + (lane ^ (2 * e))], p[e], acc[n]);
-    } else {
-      // NaN codes that some rows see and others do not are counted by a product of their own
-      for (int n = 0; n < VT; ++n) {
-        if (32 * n >= dim) continue;
-        f32x16 hits = f32x16{};
-        f32x16 sums = acc[0];
-#pragma unroll
-        for (int k = 1; k < VT; ++k)
-          if (n == k) sums = acc[k];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const v4u w = vst[(n * 4 + e) * 64 + (lane ^ (2 * e))];
-          uint32_t in[4] = {w.x, w.y, w.z, w.w}, is[4], no[4], see[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool a0 = (in[i] & 0x7FFFu) > 0x7C00u, a1 = (in[i] & 0x7FFF0000u) > 0x7C000000u;
-            is[i] = (a0 ? 0x3C00u : 0u) | (a1 ? 0x3C000000u : 0u);
-            no[i] = in[i] & ((a0 ? 0u : 0xFFFFu) | (a1 ? 0u : 0xFFFF0000u));
-            const int key = u * kUnit + 16 * e + 8 * (i >> 1) + 4 * half + 2 * (i & 1);
-            see[i] = (key < hi && key >= lo ? 0x3C00u : 0u) | (key + 1 < hi && key + 1 >= lo ? 0x3C000000u : 0u);
-          }
-          hits = mma32<kF16>(v4u{is[0], is[1], is[2], is[3]}, v4u{see[0], see[1], see[2], see[3]}, hits);
-          sums = mma32<kF16>(v4u{no[0], no[1], no[2], no[3]}, p[e], sums);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sums[i] = hits[i] > 0.0f ? __builtin_nanf("") : sums[i];
-#pragma unroll
-        for (int k = 0; k < VT; ++k)
-          if (n == k) acc[k] = sums;
-      }
-    }
+      for (int e = 0; e < 4; ++e)
+        if (32 * n < dim) acc[n] = mma32<kF16>(vst[(n * 4 + e) * 64 + (lane ^ (2 * e))], p[e], acc[n]);
     if (more) put(u + 1, at ^ 1);  // read last before the barrier of the round before
     __syncthreads();
   }
@@ -407,33 +379,81 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
     }
 }
 
+// NaN for the channels of rows of a tile that see a NaN code of V in a unit that others of
+// the tile see only a part of.  A thread looks through one channel's keys after the other.
+template <int DT>
+__device__ void spread_nan(const KvAttendArgs& a, int b, int tile, int h) {
+  const int dim = a.cache.dim, S = 1 << a.seqs.shift, group = a.group;
+  const KvSeq q = kv_seq(a.seqs, b);
+  const TileSpan span = tile_span(q, group, a.window, tile);
+  const int64_t row0 = (int64_t)tile * kTileRows;
+  const int base = q.len - q.n + 1, first_hi = base + (int)(row0 / group), last_hi = base + (int)((row0 + span.rows - 1) / group);
+  const int last_lo = a.window > 0 && last_hi > a.window ? last_hi - a.window : 0;
+  for (int u = span.first; u < span.end; ++u) {
+    if (u * kUnit + kUnit <= first_hi && u * kUnit >= last_lo) continue;
+    for (int i = threadIdx.x; i < kUnit * dim; i += 256) {
+      const int key = u * kUnit + i % kUnit, d = i / kUnit, j = key >> a.seqs.shift;
+      if (key < span.lo || key >= span.hi) continue;
+      const int page = kv_page(a.seqs, a.cache.pages, b, j);
+      if (page < 0) continue;
+      const uint8_t code = gld<uint8_t>(a.cache.v + (int64_t)page * a.cache.v_page + ((int64_t)h * dim + d) * S + (key & (S - 1)));
+      if ((code & 0x7F) != 0x7F) continue;
+      for (int r = 0; r < span.rows; ++r) {
+        const int64_t tok = (row0 + r) / group;
+        const int hi = base + (int)tok;
+        if (key >= hi || (a.window > 0 && key < hi - a.window)) continue;
+        const int64_t at = (q.first + tok) * a.heads + h * group + (row0 + r - tok * group);
+        gst<uint16_t>(static_cast<uint16_t*>(a.out) + at * dim + d, DT == kBF16 ? 0x7FC0 : 0x7E00);
+      }
+    }
+  }
+}
+
 // Tiles that were cut: their pieces' sums, brought to one maximum.
 template <int DT>
 __global__ __launch_bounds__(256) void k_kv_join_tiles(KvAttendArgs a) {
   const int heads = a.cache.heads, dim = a.cache.dim;
   const int h = blockIdx.x % heads, idx = blockIdx.x / heads;
-  if (idx >= gld<int32_t>(a.tiles.count + 1)) return;
-  const v4i cut = gld<v4i>(a.tiles.cut + idx);
-  const int b = cut.x, tile = cut.y, slot = cut.z, pieces = cut.w;
-  const KvSeq q = kv_seq(a.seqs, b);
-  const int64_t all = (int64_t)q.n * a.group, row0 = (int64_t)tile * kTileRows;
-  const int64_t step = (int64_t)heads * kTileRows * (2 + dim);
-  const float* const first = a.tiles.sums + ((int64_t)slot * heads + h) * (kTileRows * (2 + (int64_t)dim));
-  const int r = threadIdx.x % kTileRows;
-  if (row0 + r >= all) return;
-  float top = gld<float>(first + r);
-  for (int p = 1; p < pieces; ++p) top = fmaxf(top, gld<float>(first + p * step + r));
-  float sum = 0.0f;
-  for (int p = 0; p < pieces; ++p) sum += __builtin_amdgcn_exp2f(gld<float>(first + p * step + r) - top) * gld<float>(first + p * step + kTileRows + r);
-  const float over = sum != 0.0f ? 1.0f / sum : 0.0f;
-  const int64_t tok = (row0 + r) / a.group;
-  const int64_t at = (q.first + tok) * a.heads + h * a.group + (row0 + r - tok * a.group);
-  for (int c = blockIdx.y * 2 + threadIdx.x / kTileRows; c < dim / 4; c += 2 * gridDim.y) {
-    f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = 0; p < pieces; ++p)
-      v += __builtin_amdgcn_exp2f(gld<float>(first + p * step + r) - top) * gld<f32x4>(first + p * step + 2 * kTileRows + ((int64_t)c * kTileRows + r) * 4);
-    store4<DT>(a.out, at * dim + 4 * c, v * over);
-    if (a.lse != nullptr && c == 0) gst<float>(a.lse + at, sum != 0.0f ? (top - kLift + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY);
+  if (idx < gld<int32_t>(a.tiles.count + 1)) {
+    const v4i cut = gld<v4i>(a.tiles.cut + idx);
+    const int b = cut.x, tile = cut.y, slot = cut.z, pieces = cut.w;
+    const KvSeq q = kv_seq(a.seqs, b);
+    const int64_t all = (int64_t)q.n * a.group, row0 = (int64_t)tile * kTileRows;
+    const int64_t step = (int64_t)heads * kTileRows * (2 + dim);
+    const float* const first = a.tiles.sums + ((int64_t)slot * heads + h) * (kTileRows * (2 + (int64_t)dim));
+    const int r = threadIdx.x % kTileRows;
+    if (row0 + r < all) {
+      float top = gld<float>(first + r);
+      for (int p = 1; p < pieces; ++p) top = fmaxf(top, gld<float>(first + p * step + r));
+      float sum = 0.0f;
+      for (int p = 0; p < pieces; ++p) sum += __builtin_amdgcn_exp2f(gld<float>(first + p * step + r) - top) * gld<float>(first + p * step + kTileRows + r);
+      const float over = sum != 0.0f ? 1.0f / sum : 0.0f;
+      const int64_t tok = (row0 + r) / a.group;
+      const int64_t at = (q.first + tok) * a.heads + h * a.group + (row0 + r - tok * a.group);
+      for (int c = blockIdx.y * 2 + threadIdx.x / kTileRows; c < dim / 4; c += 2 * gridDim.y) {
+        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int p = 0; p < pieces; ++p)
+          v += __builtin_amdgcn_exp2f(gld<float>(first + p * step + r) - top) * gld<f32x4>(first + p * step + 2 * kTileRows + ((int64_t)c * kTileRows + r) * 4);
+        store4<DT>(a.out, at * dim + 4 * c, v * over);
+        if (a.lse != nullptr && c == 0) gst<float>(a.lse + at, sum != 0.0f ? (top - kLift + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY);
+      }
+    }
+  }
+}
+
+// Every tile's NaN codes that k_kv_prefill took as 0, where it met any.
+template <int DT>
+__global__ __launch_bounds__(256) void k_kv_nan(KvAttendArgs a) {
+  const int heads = a.cache.heads, h = blockIdx.x % heads, step = gridDim.x / heads;
+  if (gld<int32_t>(a.tiles.count + 2) == 0) return;
+  const int pieces = gld<int32_t>(a.tiles.count), cuts = gld<int32_t>(a.tiles.count + 1);
+  for (int i = blockIdx.x / heads; i < pieces; i += step) {
+    const v4i piece = gld<v4i>(a.tiles.piece + 2 * i);
+    if (gld<int32_t>(a.tiles.piece + 2 * i + 1) < 0) spread_nan<DT>(a, piece.x, piece.y, h);
+  }
+  for (int i = blockIdx.x / heads; i < cuts; i += step) {
+    const v4i cut = gld<v4i>(a.tiles.cut + i);
+    spread_nan<DT>(a, cut.x, cut.y, h);
   }
 }
 
@@ -441,8 +461,11 @@ template <int DT, int NC>
 void launch(const KvAttendArgs& a, int64_t tiles, hipStream_t stream) {
   const int64_t heads = a.cache.heads;
   hipLaunchKernelGGL(k_kv_tiles, dim3(1), dim3(1024), 0, stream, a);
-  hipLaunchKernelGGL((k_kv_prefill<DT, NC>), dim3((unsigned)((tiles + 2 * kSlots / heads + 1) * heads)), dim3(256), 0, stream, a);
+  const dim3 grid((unsigned)((tiles + 2 * kSlots / heads + 1) * heads));
+  if (a.cache.dim == 64 * NC) hipLaunchKernelGGL((k_kv_prefill<DT, NC, true>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((k_kv_prefill<DT, NC, false>), grid, dim3(256), 0, stream, a);
   hipLaunchKernelGGL((k_kv_join_tiles<DT>), dim3((unsigned)((kSlots / heads + 1) * heads), 4), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((k_kv_nan<DT>), dim3((unsigned)((256 / heads + 1) * heads)), dim3(256), 0, stream, a);
 }
 template <int DT>
 void launch_of(const KvAttendArgs& a, int64_t tiles, hipStream_t stream) {
