@@ -155,8 +155,8 @@ __global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
   if (tid == 0) gst<int32_t>(p.count + 1, (int32_t)counts[1]);
 }
 
-// FULL: heads of 64 NC channels.
-template <int DT, int NC, bool FULL>
+// FAST: heads of 64 NC channels and pages of 64 keys or more, so that a unit is of one page.
+template <int DT, int NC, bool FAST>
 __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs a) {
   constexpr int KS = 4 * NC, VT = 2 * NC;       // steps of 16 channels, tiles of 32
   constexpr int kStage = (2 * KS + 4 * VT) * 64;  // 16-byte places of a tile: K's operands, then V's
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
   __shared__ __attribute__((aligned(16))) float page_of[2][12];  // per 16 keys: factor, exponent, its inverse
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, half = lane >> 5;
-  const int heads = a.cache.heads, dim = FULL ? 64 * NC : a.cache.dim, shift = a.seqs.shift, S = 1 << shift, group = a.group;
+  const int heads = a.cache.heads, dim = FAST ? 64 * NC : a.cache.dim, shift = a.seqs.shift, S = 1 << shift, group = a.group;
   const int count = gld<int32_t>(a.tiles.count);
   const int h = blockIdx.x % heads, idx = blockIdx.x / heads;
   if (idx >= count) return;
@@ -204,28 +204,42 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
   // what this thread brings of a tile: of K token tid / 4, of V keys 16 (tid % 4) .., a piece of each 64 channels
   const int k_tok = tid >> 2, c4 = tid & 3;
   v4u kr[NC], vr[NC];
-  int kp = -1, vp = -1;  // pages
-  float ks = 0.0f, vs = 0.0f;
+  int kp = -1, vp = -1;  // the pages of the next load
   auto look_up = [&](int u) {
-    const int kk = (u * kUnit + k_tok) >> shift, vk = (u * kUnit + 16 * c4) >> shift;
-    kp = kk < a.seqs.width ? kv_page(a.seqs, a.cache.pages, b, kk) : -1;
-    vp = vk < a.seqs.width ? kv_page(a.seqs, a.cache.pages, b, vk) : -1;
+    if constexpr (FAST) {
+      kp = vp = kv_page_uniform(a.seqs, a.cache.pages, b, (u * kUnit) >> shift);
+    } else {  // 16 keys are of one page
+      int p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = kv_page_uniform(a.seqs, a.cache.pages, b, (u * kUnit + 16 * i) >> shift);
+      const int g = k_tok >> 4;
+      kp = (g & 2) ? ((g & 1) ? p[3] : p[2]) : ((g & 1) ? p[1] : p[0]);
+      vp = (c4 & 2) ? ((c4 & 1) ? p[3] : p[2]) : ((c4 & 1) ? p[1] : p[0]);
+    }
   };
   bool k_ok = false, v_ok = false;
+  float ks = 0.0f, vs = 0.0f;  // of the keys 16 (tid % 4) ..; FAST: of the unit
   auto load = [&](int u) {
     const int key = u * kUnit + k_tok, vkey = u * kUnit + 16 * c4;
     k_ok = kp >= 0, v_ok = vp >= 0;
-    const uint8_t* const kb = a.cache.k + (int64_t)(k_ok ? kp : 0) * a.cache.k_page + ((int64_t)h * S + (key & (S - 1))) * dim + 16 * c4;
-    const uint8_t* const vb = a.cache.v + (int64_t)(v_ok ? vp : 0) * a.cache.v_page + ((int64_t)h * dim + k_tok) * S + (vkey & (S - 1));
+    const int64_t kpage = k_ok ? kp : 0, vpage = v_ok ? vp : 0;
+    const uint8_t* const kb = a.cache.k + kpage * a.cache.k_page + ((int64_t)h * S + (key & (S - 1))) * dim + 16 * c4;
+    const uint8_t* const vb = a.cache.v + vpage * a.cache.v_page + ((int64_t)h * dim + k_tok) * S + (vkey & (S - 1));
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      kr[i] = vr[i] = v4u{0, 0, 0, 0};
-      if (64 * i + 16 * c4 < dim) kr[i] = gld<v4u>(kb + 64 * i);
-      if (64 * i + k_tok < dim) vr[i] = gld<v4u>(vb + (int64_t)64 * i * S);
+      if constexpr (FAST) {
+        kr[i] = gld<v4u>(kb + 64 * i);
+        vr[i] = gld<v4u>(vb + (int64_t)64 * i * S);
+      } else {
+        kr[i] = vr[i] = v4u{0, 0, 0, 0};
+        if (64 * i + 16 * c4 < dim) kr[i] = gld<v4u>(kb + 64 * i);
+        if (64 * i + k_tok < dim) vr[i] = gld<v4u>(vb + (int64_t)64 * i * S);
+      }
     }
-    if (tid < 4) {
-      ks = gld<float>(a.cache.ks + (int64_t)(v_ok ? vp : 0) * a.cache.ks_page + h);
-      vs = gld<float>(a.cache.vs + (int64_t)(v_ok ? vp : 0) * a.cache.vs_page + h);
+    if constexpr (FAST) {
+      ks = sld(a.cache.ks + vpage * a.cache.ks_page + h), vs = sld(a.cache.vs + vpage * a.cache.vs_page + h);
+    } else if (tid < 4) {
+      ks = gld<float>(a.cache.ks + vpage * a.cache.ks_page + h), vs = gld<float>(a.cache.vs + vpage * a.cache.vs_page + h);
     }
   };
   auto cut_at = [&](int u) { return u * kUnit + kUnit > first_hi || u * kUnit < last_lo; };
@@ -262,7 +276,7 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
       to[32] = v4u{x.z, x.w, y.z, y.w};
     }
     if (bad != 0) gst<int32_t>(a.tiles.count + 2, 1);
-    if (tid < 4) {
+    if (FAST ? tid == 0 : tid < 4) {
       const float ev = __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(vs, 0x1p-48f, 0x1p48f));
       page_of[at][tid] = fmaxf(ks * scale, 0x1p-120f);  // above 0, so that no key stays no key
       page_of[at][4 + tid] = v_ok ? ev : -INFINITY;
@@ -290,33 +304,38 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
     }
     const v4u* const kst = stage[at];
     const v4u* const vst = stage[at] + 2 * KS * 64;
-    f32x16 s[2];
+    f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = f32x16{};
+    for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
-        if (16 * k < dim) s[t] = mma32<DT>(kst[(t * KS + k) * 64 + (lane ^ (2 * (k & 3)))], qf[k], s[t]);
+      for (int t = 0; t < 2; ++t)
+        if (FAST || 16 * k < dim) s[t] = mma32<DT>(kst[(t * KS + k) * 64 + (lane ^ (2 * (k & 3)))], qf[k], s[t]);
+    // the scores' factor, V's exponent and its inverse: of every 16 keys, or of them all
+    constexpr int E = FAST ? 1 : 4;
+    float factor[E], ev[E], back[E];
+    bool gone = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      factor[e] = page_of[at][e], ev[e] = page_of[at][4 + e], back[e] = page_of[at][8 + e];
+      gone |= ev[e] == -INFINITY;
     }
-    const f32x4 factor = *reinterpret_cast<const f32x4*>(page_of[at]), ev = *reinterpret_cast<const f32x4*>(page_of[at] + 4);
-    const f32x4 back = *reinterpret_cast<const f32x4*>(page_of[at] + 8);
-    const bool cut = cut_at(u) || ev.x == -INFINITY || ev.y == -INFINITY || ev.z == -INFINITY || ev.w == -INFINITY;
-    if (__builtin_amdgcn_readfirstlane(cut)) {
+    if (__builtin_amdgcn_readfirstlane(cut_at(u) || gone)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int key = u * kUnit + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3);
-          s[t][i] = key < hi && key >= lo && ev[2 * t + (i >> 3)] != -INFINITY ? s[t][i] : -INFINITY;
+          s[t][i] = key < hi && key >= lo && ev[(2 * t + (i >> 3)) % E] != -INFINITY ? s[t][i] : -INFINITY;
         }
     }
     float top = m;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < E; ++e) {
+      constexpr int N = 32 / E;
       float x = s[e >> 1][8 * (e & 1)];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) x = fmaxf(x, s[e >> 1][8 * (e & 1) + i]);
-      // no key of the 16: 0 x -inf and -inf + -inf are kept out of it
+      for (int i = 1; i < N; ++i) x = fmaxf(x, s[(e >> 1) + (i >> 4)][(8 * (e & 1) + i) & 15]);
+      // no key of them: 0 x -inf and -inf + -inf are kept out of it
       top = x == -INFINITY ? top : fmaxf(top, __builtin_fmaf(x, factor[e], ev[e]));
     }
     top = pair_max(top);
@@ -332,21 +351,21 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
     v4u p[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float shift_by = ev[e] - m + kLift;
+      const float shift_by = ev[e % E] - m + kLift;
       float x[8], sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 1][8 * (e & 1) + i], factor[e], shift_by));
+        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 1][8 * (e & 1) + i], factor[e % E], shift_by));
         sum += x[i];
       }
-      l = __builtin_fmaf(sum, back[e], l);
+      l = __builtin_fmaf(sum, back[e % E], l);
       p[e] = v4u{f16_pair(x[0], x[1]), f16_pair(x[2], x[3]), f16_pair(x[4], x[5]), f16_pair(x[6], x[7])};
     }
 #pragma unroll
-    for (int n = 0; n < VT; ++n)
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (32 * n < dim) acc[n] = mma32<kF16>(vst[(n * 4 + e) * 64 + (lane ^ (2 * e))], p[e], acc[n]);
+      for (int n = 0; n < VT; ++n)
+        if (FAST || 32 * n < dim) acc[n] = mma32<kF16>(vst[(n * 4 + e) * 64 + (lane ^ (2 * e))], p[e], acc[n]);
     if (more) put(u + 1, at ^ 1);  // read last before the barrier of the round before
     __syncthreads();
   }
@@ -462,7 +481,7 @@ void launch(const KvAttendArgs& a, int64_t tiles, hipStream_t stream) {
   const int64_t heads = a.cache.heads;
   hipLaunchKernelGGL(k_kv_tiles, dim3(1), dim3(1024), 0, stream, a);
   const dim3 grid((unsigned)((tiles + 2 * kSlots / heads + 1) * heads));
-  if (a.cache.dim == 64 * NC) hipLaunchKernelGGL((k_kv_prefill<DT, NC, true>), grid, dim3(256), 0, stream, a);
+  if (a.cache.dim == 64 * NC && a.seqs.shift >= 6) hipLaunchKernelGGL((k_kv_prefill<DT, NC, true>), grid, dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((k_kv_prefill<DT, NC, false>), grid, dim3(256), 0, stream, a);
   hipLaunchKernelGGL((k_kv_join_tiles<DT>), dim3((unsigned)((kSlots / heads + 1) * heads), 4), dim3(256), 0, stream, a);
   hipLaunchKernelGGL((k_kv_nan<DT>), dim3((unsigned)((256 / heads + 1) * heads)), dim3(256), 0, stream, a);
