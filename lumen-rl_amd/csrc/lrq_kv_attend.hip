@@ -172,6 +172,10 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
     total += block_sum<kWaves>((int64_t)mine.lines * mine.count, scan);
   }
   total = uniform(total);
+  if (total == 0) {  // all sequences are k_kv_prefill's
+    if (blockIdx.x == 0 && tid == 0) gst<int32_t>(a.cut_count, 0);
+    return;
+  }
   // units of a piece: below 2^31, as the items are at most a.parts times as many as that
   const uint32_t per = total <= kLeast * kParts ? kLeast : (uint32_t)((total + kParts - 1) / kParts);
   if (tid < kWaves) found[tid][0] = -1;

@@ -16,8 +16,8 @@
 // While a tile is worked on, the next one's codes are on their way into registers.
 //
 // In units that some rows see only a part of, NaN codes of V are taken as 0 and a flag is
-// left: 0 x NaN must not reach rows that do not see it.  The last launch, k_kv_nan, then looks
-// for them again and writes NaN to the rows that do.
+// left: 0 x NaN must not reach rows that do not see it.  k_kv_join_tiles, the last launch,
+// then looks for them again and writes NaN to the rows that do.
 #include "lrq_kv.hpp"
 #include "lrq_kv_attend.hpp"
 
@@ -79,6 +79,8 @@ constexpr int kBuckets = 1024;  // of pieces' lengths; the last one takes all lo
 __global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
   __shared__ int64_t scan[16];
   __shared__ int64_t carry;
+  __shared__ uint32_t scan32[16];
+  __shared__ int ends[1024];  // upto, where it is no longer than that
   __shared__ uint32_t bucket[kBuckets];
   __shared__ uint32_t counts[2];  // places of pieces, and tiles that were cut
   const KvTiles& p = a.tiles;
@@ -91,26 +93,42 @@ __global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
     const int64_t base = carry;
     const int64_t upto = base + block_scan<1024, int64_t>(b0 + tid < seqs ? tiles_of(a, b0 + tid) : 0, scan);
     if (b0 + tid < seqs) gst<int32_t>(p.upto + b0 + tid, (int32_t)upto);
+    ends[tid] = (int)upto;
     if (tid == 1023) carry = upto;
     __syncthreads();
   }
   const int tiles = (int)carry;
   __syncthreads();
+  auto end_of = [&](int b) { return seqs <= 1024 ? ends[b] : gld<int32_t>(p.upto + b); };
   auto find = [&](int i, int& tile) {  // the sequence of tile i
     int lo = 0, hi = seqs - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (gld<int32_t>(p.upto + mid) > i) hi = mid;
+      if (end_of(mid) > i) hi = mid;
       else lo = mid + 1;
     }
-    tile = i - (lo > 0 ? gld<int32_t>(p.upto + lo - 1) : 0);
+    tile = i - (lo > 0 ? end_of(lo - 1) : 0);
     return lo;
+  };
+  // a thread's first tile is looked at once, others (in calls of more tiles than threads) three times
+  int my_tile = 0;
+  const int my_b = tid < tiles ? find(tid, my_tile) : 0;
+  TileSpan my_span{};
+  if (tid < tiles) my_span = tile_span(kv_seq(a.seqs, my_b), a.group, a.window, my_tile);
+  auto look = [&](int i, int& tile, TileSpan& span) {
+    if (i == tid) {
+      tile = my_tile, span = my_span;
+      return my_b;
+    }
+    const int b = find(i, tile);
+    span = tile_span(kv_seq(a.seqs, b), a.group, a.window, tile);
+    return b;
   };
   int64_t units = 0;
   for (int i = tid; i < tiles; i += 1024) {
     int tile;
-    const int b = find(i, tile);
-    const TileSpan s = tile_span(kv_seq(a.seqs, b), a.group, a.window, tile);
+    TileSpan s;
+    look(i, tile, s);
     units += s.end - s.first;
   }
   const int64_t sum = block_scan<1024, int64_t>(units, scan);
@@ -122,21 +140,21 @@ __global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
   auto bucket_of = [&](int n) { return n >= kBuckets ? 0 : kBuckets - 1 - n; };
   for (int i = tid; i < tiles; i += 1024) {
     int tile;
-    const int b = find(i, tile);
-    const TileSpan s = tile_span(kv_seq(a.seqs, b), a.group, a.window, tile);
+    TileSpan s;
+    look(i, tile, s);
     const int n = s.end - s.first, cuts = cuts_of(n);
     atomicAdd(&bucket[bucket_of(n / cuts)], (uint32_t)cuts);
   }
   __syncthreads();
   const uint32_t mine = bucket[tid];
-  const int64_t before = block_scan<1024, int64_t>(mine, scan) - mine;
-  bucket[tid] = (uint32_t)before;
+  const uint32_t before = block_scan<1024, uint32_t>(mine, scan32) - mine;
+  bucket[tid] = before;
   if (tid == 1023) gst<int32_t>(p.count, (int32_t)(before + mine));
   __syncthreads();
   for (int i = tid; i < tiles; i += 1024) {
     int tile;
-    const int b = find(i, tile);
-    const TileSpan s = tile_span(kv_seq(a.seqs, b), a.group, a.window, tile);
+    TileSpan s;
+    const int b = look(i, tile, s);
     const int n = s.end - s.first, cuts = cuts_of(n);
     const uint32_t at = atomicAdd(&bucket[bucket_of(n / cuts)], (uint32_t)cuts);
     int slot = -1;
@@ -218,10 +236,11 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
     }
   };
   bool k_ok = false, v_ok = false;
+  int vp_now = -1;
   float ks = 0.0f, vs = 0.0f;  // of the keys 16 (tid % 4) ..; FAST: of the unit
   auto load = [&](int u) {
     const int key = u * kUnit + k_tok, vkey = u * kUnit + 16 * c4;
-    k_ok = kp >= 0, v_ok = vp >= 0;
+    k_ok = kp >= 0, v_ok = vp >= 0, vp_now = vp;
     const int64_t kpage = k_ok ? kp : 0, vpage = v_ok ? vp : 0;
     const uint8_t* const kb = a.cache.k + kpage * a.cache.k_page + ((int64_t)h * S + (key & (S - 1))) * dim + 16 * c4;
     const uint8_t* const vb = a.cache.v + vpage * a.cache.v_page + ((int64_t)h * dim + k_tok) * S + (vkey & (S - 1));
@@ -242,40 +261,40 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
       ks = gld<float>(a.cache.ks + vpage * a.cache.ks_page + h), vs = gld<float>(a.cache.vs + vpage * a.cache.vs_page + h);
     }
   };
+  // units that some row sees a part of
   auto cut_at = [&](int u) { return u * kUnit + kUnit > first_hi || u * kUnit < last_lo; };
-  auto put = [&](int u, int at) {  // the tile's operands into stage `at`
-    v4u* const st = stage[at];
+  // What was loaded of unit u: nothing where there is no page; where rows see a part of it,
+  // keys that none sees are 0, and so are NaN codes of V.
+  auto clean = [&](int u) {
+    uint32_t keep[4], bad = 0;
+    const int v_key = u * kUnit + 16 * c4;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const v4u w = k_ok ? kr[i] : v4u{0, 0, 0, 0};
-      v4u* const to = st + ((k_tok >> 5) * KS + 4 * i + c4) * 64 + ((k_tok & 31) ^ (2 * c4));
-      to[0] = widen8<DT>(w.x, w.y);
-      to[32] = widen8<DT>(w.z, w.w);
-    }
-    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+    for (int i = 0; i < 4; ++i) keep[i] = v_ok ? low_bytes(span.hi - v_key - 4 * i) & ~low_bytes(span.lo - v_key - 4 * i) : 0u;
     const bool cut = cut_at(u);
-    if (cut) {
-      const int v_key = u * kUnit + 16 * c4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) keep[i] = low_bytes(span.hi - v_key - 4 * i) & ~low_bytes(span.lo - v_key - 4 * i);
-    }
-    uint32_t bad = 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      v4u w = v_ok ? vr[i] : v4u{0, 0, 0, 0};
-      if (cut) {
-        w = v4u{w.x & keep[0], w.y & keep[1], w.z & keep[2], w.w & keep[3]};
-        const v4u nan = v4u{nan_bytes(w.x), nan_bytes(w.y), nan_bytes(w.z), nan_bytes(w.w)} >> 7;
-        bad |= nan.x | nan.y | nan.z | nan.w;
-        w &= ~(nan * 0xFF);
-      }
-      const int d = 64 * i + k_tok;
-      v4u* const to = st + 2 * KS * 64 + ((d >> 5) * 4 + c4) * 64 + ((d & 31) ^ (2 * c4));
-      const v4u x = widen8<kF16>(w.x, w.y), y = widen8<kF16>(w.z, w.w);  // keys 0-7, 8-15
-      to[0] = v4u{x.x, x.y, y.x, y.y};
-      to[32] = v4u{x.z, x.w, y.z, y.w};
+      kr[i] = k_ok ? kr[i] : v4u{0, 0, 0, 0};
+      const v4u w = v4u{vr[i].x & keep[0], vr[i].y & keep[1], vr[i].z & keep[2], vr[i].w & keep[3]};
+      const v4u nan = v4u{nan_bytes(w.x), nan_bytes(w.y), nan_bytes(w.z), nan_bytes(w.w)} >> 7;
+      if (cut) bad |= nan.x | nan.y | nan.z | nan.w;
+      vr[i] = cut ? w & ~(nan * 0xFF) : w;
     }
     if (bad != 0) gst<int32_t>(a.tiles.count + 2, 1);
+  };
+  auto is_odd = [&](int u) { return cut_at(u) || (FAST ? vp_now < 0 : __ballot(!k_ok || !v_ok) != 0); };
+  auto put_k = [&](int at, int i) {  // a piece's operands into stage `at`
+    v4u* const to = stage[at] + ((k_tok >> 5) * KS + 4 * i + c4) * 64 + ((k_tok & 31) ^ (2 * c4));
+    to[0] = widen8<DT>(kr[i].x, kr[i].y);
+    to[32] = widen8<DT>(kr[i].z, kr[i].w);
+  };
+  auto put_v = [&](int at, int i) {
+    const int d = 64 * i + k_tok;
+    v4u* const to = stage[at] + 2 * KS * 64 + ((d >> 5) * 4 + c4) * 64 + ((d & 31) ^ (2 * c4));
+    const v4u x = widen8<kF16>(vr[i].x, vr[i].y), y = widen8<kF16>(vr[i].z, vr[i].w);  // keys 0-7, 8-15
+    to[0] = v4u{x.x, x.y, y.x, y.y};
+    to[32] = v4u{x.z, x.w, y.z, y.w};
+  };
+  auto put_page = [&](int at) {
     if (FAST ? tid == 0 : tid < 4) {
       const float ev = __builtin_amdgcn_logf(__builtin_amdgcn_fmed3f(vs, 0x1p-48f, 0x1p48f));
       page_of[at][tid] = fmaxf(ks * scale, 0x1p-120f);  // above 0, so that no key stays no key
@@ -288,28 +307,39 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
   f32x16 acc[VT];
 #pragma unroll
   for (int n = 0; n < VT; ++n) acc[n] = f32x16{};
+  // Unit u's operands are in LDS, the next one's codes on their way into registers.  They are
+  // widened and put there while the matrix units take the scores; then the loads of the one
+  // after go out.  The second product's instructions run while the next exponentials are taken.
+  const int last = u1 - 1;
   if (u0 < u1) {
     look_up(u0);
     load(u0);
-    if (u0 + 1 < u1) look_up(u0 + 1);
-    put(u0, 0);
+    look_up(u0 < last ? u0 + 1 : last);
+    clean(u0);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) put_k(0, i), put_v(0, i);
+    put_page(0);
+    load(u0 < last ? u0 + 1 : last);
   }
   __syncthreads();
   for (int u = u0; u < u1; ++u) {
     const int at = (u - u0) & 1;
-    const bool more = u + 1 < u1;
-    if (more) {
-      load(u + 1);
-      if (u + 2 < u1) look_up(u + 2);
-    }
+    const int coming = u + 1 < last ? u + 1 : last;  // (once more the last one, into the stage that no one reads)
+    look_up(u + 2 < last ? u + 2 : last);
+    if (is_odd(coming)) clean(coming);
     const v4u* const kst = stage[at];
     const v4u* const vst = stage[at] + 2 * KS * 64;
     f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
-    for (int k = 0; k < KS; ++k)
+    for (int k = 0; k < KS; ++k) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         if (FAST || 16 * k < dim) s[t] = mma32<DT>(kst[(t * KS + k) * 64 + (lane ^ (2 * (k & 3)))], qf[k], s[t]);
+      if (k % 4 == 1) put_k(at ^ 1, k / 4);
+      if (k % 4 == 3) put_v(at ^ 1, k / 4);
+    }
+    put_page(at ^ 1);
+    load(u + 2 < last ? u + 2 : last);
     // the scores' factor, V's exponent and its inverse: of every 16 keys, or of them all
     constexpr int E = FAST ? 1 : 4;
     float factor[E], ev[E], back[E];
@@ -348,7 +378,6 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[n][i] *= fade;
     }
-    v4u p[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float shift_by = ev[e % E] - m + kLift;
@@ -359,14 +388,12 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
         sum += x[i];
       }
       l = __builtin_fmaf(sum, back[e % E], l);
-      p[e] = v4u{f16_pair(x[0], x[1]), f16_pair(x[2], x[3]), f16_pair(x[4], x[5]), f16_pair(x[6], x[7])};
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
+      const v4u p = v4u{f16_pair(x[0], x[1]), f16_pair(x[2], x[3]), f16_pair(x[4], x[5]), f16_pair(x[6], x[7])};
 #pragma unroll
       for (int n = 0; n < VT; ++n)
-        if (FAST || 32 * n < dim) acc[n] = mma32<kF16>(vst[(n * 4 + e) * 64 + (lane ^ (2 * e))], p[e], acc[n]);
-    if (more) put(u + 1, at ^ 1);  // read last before the barrier of the round before
+        if (FAST || 32 * n < dim) acc[n] = mma32<kF16>(vst[(n * 4 + e) * 64 + (lane ^ (2 * e))], p, acc[n]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     __syncthreads();
   }
   l = pair_sum(l);
@@ -399,9 +426,9 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
 }
 
 // NaN for the channels of rows of a tile that see a NaN code of V in a unit that others of
-// the tile see only a part of.  A thread looks through one channel's keys after the other.
+// the tile see only a part of.  Work-group y of `of` has every of-th eight channels.
 template <int DT>
-__device__ void spread_nan(const KvAttendArgs& a, int b, int tile, int h) {
+__device__ void spread_nan(const KvAttendArgs& a, int b, int tile, int h, int y, int of) {
   const int dim = a.cache.dim, S = 1 << a.seqs.shift, group = a.group;
   const KvSeq q = kv_seq(a.seqs, b);
   const TileSpan span = tile_span(q, group, a.window, tile);
@@ -411,9 +438,9 @@ __device__ void spread_nan(const KvAttendArgs& a, int b, int tile, int h) {
   for (int u = span.first; u < span.end; ++u) {
     if (u * kUnit + kUnit <= first_hi && u * kUnit >= last_lo) continue;
     for (int i = threadIdx.x; i < kUnit * dim; i += 256) {
-      const int key = u * kUnit + i % kUnit, d = i / kUnit, j = key >> a.seqs.shift;
-      if (key < span.lo || key >= span.hi) continue;
-      const int page = kv_page(a.seqs, a.cache.pages, b, j);
+      const int key = u * kUnit + i % kUnit, d = i / kUnit;
+      if (key < span.lo || key >= span.hi || d / 8 % of != y) continue;
+      const int page = kv_page(a.seqs, a.cache.pages, b, key >> a.seqs.shift);
       if (page < 0) continue;
       const uint8_t code = gld<uint8_t>(a.cache.v + (int64_t)page * a.cache.v_page + ((int64_t)h * dim + d) * S + (key & (S - 1)));
       if ((code & 0x7F) != 0x7F) continue;
@@ -428,12 +455,15 @@ __device__ void spread_nan(const KvAttendArgs& a, int b, int tile, int h) {
   }
 }
 
-// Tiles that were cut: their pieces' sums, brought to one maximum.
+// Last: tiles that were cut get their pieces' sums, brought to one maximum; and if there were
+// NaN codes that k_kv_prefill took as 0, every tile gets those.  blockIdx.y has every fourth
+// eight channels of a cut tile, in both.
 template <int DT>
 __global__ __launch_bounds__(256) void k_kv_join_tiles(KvAttendArgs a) {
-  const int heads = a.cache.heads, dim = a.cache.dim;
+  const int heads = a.cache.heads, dim = a.cache.dim, step_all = gridDim.x / heads;
   const int h = blockIdx.x % heads, idx = blockIdx.x / heads;
-  if (idx < gld<int32_t>(a.tiles.count + 1)) {
+  const v4i count = gld<v4i>(a.tiles.count);  // pieces, cut tiles, NaN codes
+  if (idx < count.y) {  // (the grid has a work-group for each)
     const v4i cut = gld<v4i>(a.tiles.cut + idx);
     const int b = cut.x, tile = cut.y, slot = cut.z, pieces = cut.w;
     const KvSeq q = kv_seq(a.seqs, b);
@@ -457,22 +487,15 @@ __global__ __launch_bounds__(256) void k_kv_join_tiles(KvAttendArgs a) {
         if (a.lse != nullptr && c == 0) gst<float>(a.lse + at, sum != 0.0f ? (top - kLift + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY);
       }
     }
+    if (count.z != 0) {
+      __syncthreads();  // the results above are written before
+      spread_nan<DT>(a, b, tile, h, blockIdx.y, gridDim.y);
+    }
   }
-}
-
-// Every tile's NaN codes that k_kv_prefill took as 0, where it met any.
-template <int DT>
-__global__ __launch_bounds__(256) void k_kv_nan(KvAttendArgs a) {
-  const int heads = a.cache.heads, h = blockIdx.x % heads, step = gridDim.x / heads;
-  if (gld<int32_t>(a.tiles.count + 2) == 0) return;
-  const int pieces = gld<int32_t>(a.tiles.count), cuts = gld<int32_t>(a.tiles.count + 1);
-  for (int i = blockIdx.x / heads; i < pieces; i += step) {
+  if (count.z == 0 || blockIdx.y != 0) return;
+  for (int i = idx; i < count.x; i += step_all) {
     const v4i piece = gld<v4i>(a.tiles.piece + 2 * i);
-    if (gld<int32_t>(a.tiles.piece + 2 * i + 1) < 0) spread_nan<DT>(a, piece.x, piece.y, h);
-  }
-  for (int i = blockIdx.x / heads; i < cuts; i += step) {
-    const v4i cut = gld<v4i>(a.tiles.cut + i);
-    spread_nan<DT>(a, cut.x, cut.y, h);
+    if (gld<int32_t>(a.tiles.piece + 2 * i + 1) < 0) spread_nan<DT>(a, piece.x, piece.y, h, 0, 1);
   }
 }
 
@@ -484,7 +507,6 @@ void launch(const KvAttendArgs& a, int64_t tiles, hipStream_t stream) {
   if (a.cache.dim == 64 * NC && a.seqs.shift >= 6) hipLaunchKernelGGL((k_kv_prefill<DT, NC, true>), grid, dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((k_kv_prefill<DT, NC, false>), grid, dim3(256), 0, stream, a);
   hipLaunchKernelGGL((k_kv_join_tiles<DT>), dim3((unsigned)((kSlots / heads + 1) * heads), 4), dim3(256), 0, stream, a);
-  hipLaunchKernelGGL((k_kv_nan<DT>), dim3((unsigned)((256 / heads + 1) * heads)), dim3(256), 0, stream, a);
 }
 template <int DT>
 void launch_of(const KvAttendArgs& a, int64_t tiles, hipStream_t stream) {

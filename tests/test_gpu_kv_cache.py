@@ -73,6 +73,13 @@ ATTEND = [
     (torch.bfloat16, 5, 1, 96, 64, [260], [1], 0),
     (torch.float16, 4, 1, 256, 128, [140, 70], [60, 300], 50),
     (torch.bfloat16, 40, 1, 128, 64, [1, 50], [500, 3], 0),
+    # calls of more than 1024 rows: tiles of 128, some of them cut
+    (torch.bfloat16, 8, 2, 128, 64, [300, 5, 33], [900, 0, 64], 0),
+    (torch.float16, 4, 1, 256, 128, [400], [700], 0),
+    (torch.bfloat16, 14, 2, 80, 16, [100, 90], [600, 30], 200),
+    (torch.float16, 8, 1, 64, 32, [128, 1, 200], [1000, 5, 0], 0),
+    (torch.bfloat16, 8, 1, 128, 256, [140, 17], [2000, 3], 600),
+    (torch.float16, 16, 1, 208, 64, [77], [130], 0),
 ]
 
 
@@ -206,11 +213,12 @@ def test_attend_rows_that_see_nothing():
     close(got, want, bound)
 
 
-@pytest.mark.parametrize("new,window", [([1], 0), ([1], 20), ([6], 0), ([6], 20), ([150], 0), ([150], 33)])
-def test_nan_reaches_only_those_who_see_it(new, window):
+@pytest.mark.parametrize("new,window,prior", [([1], 0, 200), ([1], 20, 200), ([6], 0, 200), ([6], 20, 200), ([150], 0, 200), ([150], 33, 200),
+                                              ([300], 0, 200), ([300], 33, 200), ([300], 0, 1100)])
+def test_nan_reaches_only_those_who_see_it(new, window, prior):
     page, dim, kv, heads = 32, 64, 1, 4
-    lengths, offsets, width = batch(new, [200], page)
-    pool = 16
+    lengths, offsets, width = batch(new, [prior], page)
+    pool = 50
     c = make(1, pool, kv, dim, page, spread=0)
     table = R.spread_table(lengths, page, width, pool, 6)
     n = lengths[0]
