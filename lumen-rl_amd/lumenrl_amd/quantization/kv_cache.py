@@ -104,6 +104,7 @@ class FP8KVCache:
             raise ValueError(f"FP8KVCache: strides of layers and pages must be multiples of 16, got {k.stride()} and {v.stride()}")
         self.k, self.v, self.k_scales, self.v_scales, self.refs = k, v, k_scales, v_scales, refs
         self.device = k.device
+        self._index = k.get_device()
         self._desc = _lib.LrqKvCache(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), refs.data_ptr(),
                                      self.layers, self.pages, self.kv_heads, self.page, self.dim, kl, vl, ksl, vsl, kp, vp, ksp, vsp)
         self._ref = ctypes.byref(self._desc)
@@ -121,28 +122,29 @@ class FP8KVCache:
 
     # -- arguments ---------------------------------------------------------------
     def _ints(self, what: str, name: str, x: Tensor, shape: tuple) -> Tensor:
-        if not isinstance(x, Tensor) or x.dtype != torch.int32:
+        if not isinstance(x, Tensor) or x.dtype is not torch.int32:
             raise TypeError(f"{what}: {name} must be an int32 tensor, got {x.dtype if isinstance(x, Tensor) else type(x)!r}")
-        if x.shape != shape or x.device != self.device:
+        if x.shape != shape or x.get_device() != self._index:
             raise ValueError(f"{what}: {name} must be {tuple(shape)} on {self.device}, got {tuple(x.shape)} on {x.device}")
         return x if x.is_contiguous() else x.contiguous()
 
     def _table(self, what: str, table: Tensor) -> tuple[Tensor, int, int, int]:
         """(table, rows, width, row pitch); a copy only where its rows are not of unit stride."""
-        if not isinstance(table, Tensor) or table.dtype != torch.int32:
+        if not isinstance(table, Tensor) or table.dtype is not torch.int32:
             raise TypeError(f"{what}: table must be an int32 tensor, got {table.dtype if isinstance(table, Tensor) else type(table)!r}")
-        if table.dim() != 2 or table.device != self.device:
+        if table.dim() != 2 or table.get_device() != self._index:
             raise ValueError(f"{what}: table must be [rows, width] on {self.device}, got {tuple(table.shape)} on {table.device}")
         rows, width = table.shape
+        if table.is_contiguous():
+            return table, rows, width, width
         ld = table.stride(0) if rows > 1 else width
         if (width > 1 and table.stride(1) != 1) or not width <= ld <= _STRIDE_MAX:
             table, ld = table.contiguous(), width
         return table, rows, width, ld
 
-    def _layer(self, what: str, layer: int) -> int:
+    def _layer(self, what: str, layer: int) -> None:
         if not isinstance(layer, int) or not 0 <= layer < self.layers:
             raise ValueError(f"{what}: layer {layer!r} of {self.layers}")
-        return layer
 
     def _offsets(self, what: str, offsets: Optional[Tensor], rows: int, tokens: int) -> Optional[Tensor]:
         if offsets is None:
@@ -153,9 +155,13 @@ class FP8KVCache:
 
     def _vectors(self, what: str, name: str, x: Tensor, heads: Optional[int]) -> Tensor:
         """``x`` [tokens, heads, dim] with channels of unit stride."""
-        if x.dim() != 3 or x.shape[2] != self.dim or (heads is not None and x.shape[1] != heads) or x.device != self.device:
+        _check_input(x, what)
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.dim or (heads is not None and shape[1] != heads) or x.get_device() != self._index:
             raise ValueError(f"{what}: {name} must be [tokens, {'heads' if heads is None else heads}, {self.dim}] on {self.device}, got "
-                             f"{tuple(x.shape)} on {x.device}")
+                             f"{tuple(shape)} on {x.device}")
+        if x.is_contiguous():
+            return x
         return x if x.stride(2) == 1 and x.stride(0) <= _STRIDE_MAX and x.stride(1) <= _STRIDE_MAX else x.contiguous()
 
     # -- tokens ------------------------------------------------------------------
@@ -172,8 +178,6 @@ class FP8KVCache:
         the table are not written.  No gradient: keys or values that want one are refused.
         """
         what = "FP8KVCache.append"
-        _check_input(k, what)
-        _check_input(v, what)
         self._layer(what, layer)
         k, v = self._vectors(what, "k", k, self.kv_heads), self._vectors(what, "v", v, self.kv_heads)
         if k.shape != v.shape or k.dtype != v.dtype:
@@ -207,11 +211,10 @@ class FP8KVCache:
         pass through the result raises.
         """
         what = "FP8KVCache.attend"
-        _check_input(q, what)
-        if q.dtype == torch.float32:
+        q = self._vectors(what, "q", q, None)
+        if q.dtype is torch.float32:
             raise TypeError(f"{what}: q must be bf16 or fp16")
         self._layer(what, layer)
-        q = self._vectors(what, "q", q, None)
         tokens, heads = q.shape[:2]
         if heads % self.kv_heads or not 1 <= heads <= 4096:
             raise ValueError(f"{what}: {heads} query heads (at most 4096) on {self.kv_heads} KV heads")
