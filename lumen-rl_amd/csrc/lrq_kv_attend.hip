@@ -555,9 +555,10 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttendArgs a) {
 // Sequences of more rows than kMostRows are k_kv_prefill's, but not in a call whose rows
 // are kAllRows together at most: three launches less.
 constexpr int kMostRows = 64, kAllRows = 1024;
+int most_rows(int64_t dim) { return dim <= 128 ? kMostRows : kMostRows / 2; }  // (tiles of 16 rows there, not 32)
 // Rows of a call; one_each: one token a sequence.
 int64_t all_rows(int64_t tokens, int64_t seqs, bool one_each, int64_t group) { return (one_each && seqs < tokens ? seqs : tokens) * group; }
-bool all_few(int64_t rows, bool one_each, int64_t group) { return one_each ? group <= kMostRows : rows <= kAllRows; }
+bool all_few(int64_t rows, bool one_each, int64_t group, int64_t dim) { return one_each ? group <= most_rows(dim) : rows <= kAllRows; }
 
 // Items of a call at most, and its pieces: an item of n units is cut into less than n / per + 1.
 int64_t most_items(int64_t rows, int64_t heads, int64_t seqs, bool all) {
@@ -593,7 +594,8 @@ template <int DT, int MT>
 void launch_dim(const KvAttendArgs& a, hipStream_t stream) {
   if (a.cache.dim <= 64) launch<DT, 1, MT>(a, stream);
   else if (a.cache.dim <= 128) launch<DT, 2, MT>(a, stream);
-  else launch<DT, 4, 1>(a, stream);  // the registers of two tiles are not there
+  else if (a.cache.dim <= 192) launch<DT, 3, 1>(a, stream);  // the registers of two tiles are not there
+  else launch<DT, 4, 1>(a, stream);
 }
 template <int DT>
 void launch_of(const KvAttendArgs& a, hipStream_t stream) {
@@ -610,7 +612,7 @@ int64_t few_workspace(int64_t dim) { return 256 + kPlaces * 32 + 4 * kPlaces * (
 int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, bool one_each) {
   const int64_t group = heads / kv_heads;
   int64_t need = few_workspace(dim);
-  if (!all_few(all_rows(tokens, seqs, one_each, group), one_each, group)) {
+  if (!all_few(all_rows(tokens, seqs, one_each, group), one_each, group, dim)) {
     const int64_t many = kv_prefill_workspace(kv_prefill_tiles(tokens, group, seqs), seqs, kv_heads, dim);
     if (many > need) need = many;
   }
@@ -619,8 +621,8 @@ int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int
 
 hipError_t launch_kv_attend(KvAttendArgs a, int dtype, void* workspace, hipStream_t stream) {
   const bool one_each = a.seqs.offsets == nullptr;
-  const bool all = all_few(all_rows(a.seqs.tokens, a.seqs.seqs, one_each, a.group), one_each, a.group);
-  a.few = all ? INT32_MAX : kMostRows;
+  const bool all = all_few(all_rows(a.seqs.tokens, a.seqs.seqs, one_each, a.group), one_each, a.group, a.cache.dim);
+  a.few = all ? INT32_MAX : most_rows(a.cache.dim);
   a.cut_count = static_cast<int32_t*>(workspace);
   a.heads_at = static_cast<uint8_t*>(workspace) + 256;
   a.sums = reinterpret_cast<float*>(a.heads_at + kPlaces * 32);

@@ -173,7 +173,8 @@ __global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
   if (tid == 0) gst<int32_t>(p.count + 1, (int32_t)counts[1]);
 }
 
-// FAST: heads of 64 NC channels and pages of 64 keys or more, so that a unit is of one page.
+// Heads of more than 64 (NC - 1) channels, 64 NC at most: those that are not there are zeros.
+// FAST: pages of 64 keys or more, so that a unit is of one page.
 template <int DT, int NC, bool FAST>
 __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs a) {
   constexpr int KS = 4 * NC, VT = 2 * NC;       // steps of 16 channels, tiles of 32
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
   __shared__ __attribute__((aligned(16))) float page_of[2][12];  // per 16 keys: factor, exponent, its inverse
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, half = lane >> 5;
-  const int heads = a.cache.heads, dim = FAST ? 64 * NC : a.cache.dim, shift = a.seqs.shift, S = 1 << shift, group = a.group;
+  const int heads = a.cache.heads, dim = a.cache.dim, shift = a.seqs.shift, S = 1 << shift, group = a.group;
   const int count = gld<int32_t>(a.tiles.count);
   const int h = blockIdx.x % heads, idx = blockIdx.x / heads;
   if (idx >= count) return;
@@ -246,14 +247,9 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
     const uint8_t* const vb = a.cache.v + vpage * a.cache.v_page + ((int64_t)h * dim + k_tok) * S + (vkey & (S - 1));
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      if constexpr (FAST) {
-        kr[i] = gld<v4u>(kb + 64 * i);
-        vr[i] = gld<v4u>(vb + (int64_t)64 * i * S);
-      } else {
-        kr[i] = vr[i] = v4u{0, 0, 0, 0};
-        if (64 * i + 16 * c4 < dim) kr[i] = gld<v4u>(kb + 64 * i);
-        if (64 * i + k_tok < dim) vr[i] = gld<v4u>(vb + (int64_t)64 * i * S);
-      }
+      if (i == NC - 1) kr[i] = vr[i] = v4u{0, 0, 0, 0};
+      if (i < NC - 1 || 64 * i + 16 * c4 < dim) kr[i] = gld<v4u>(kb + 64 * i);
+      if (i < NC - 1 || 64 * i + k_tok < dim) vr[i] = gld<v4u>(vb + (int64_t)64 * i * S);
     }
     if constexpr (FAST) {
       ks = sld(a.cache.ks + vpage * a.cache.ks_page + h), vs = sld(a.cache.vs + vpage * a.cache.vs_page + h);
@@ -334,7 +330,7 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
     for (int k = 0; k < KS; ++k) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        if (FAST || 16 * k < dim) s[t] = mma32<DT>(kst[(t * KS + k) * 64 + (lane ^ (2 * (k & 3)))], qf[k], s[t]);
+        s[t] = mma32<DT>(kst[(t * KS + k) * 64 + (lane ^ (2 * (k & 3)))], qf[k], s[t]);
       if (k % 4 == 1) put_k(at ^ 1, k / 4);
       if (k % 4 == 3) put_v(at ^ 1, k / 4);
     }
@@ -391,7 +387,7 @@ __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs
       const v4u p = v4u{f16_pair(x[0], x[1]), f16_pair(x[2], x[3]), f16_pair(x[4], x[5]), f16_pair(x[6], x[7])};
 #pragma unroll
       for (int n = 0; n < VT; ++n)
-        if (FAST || 32 * n < dim) acc[n] = mma32<kF16>(vst[(n * 4 + e) * 64 + (lane ^ (2 * e))], p, acc[n]);
+        acc[n] = mma32<kF16>(vst[(n * 4 + e) * 64 + (lane ^ (2 * e))], p, acc[n]);
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
@@ -504,7 +500,7 @@ void launch(const KvAttendArgs& a, int64_t tiles, hipStream_t stream) {
   const int64_t heads = a.cache.heads;
   hipLaunchKernelGGL(k_kv_tiles, dim3(1), dim3(1024), 0, stream, a);
   const dim3 grid((unsigned)((tiles + 2 * kSlots / heads + 1) * heads));
-  if (a.cache.dim == 64 * NC && a.seqs.shift >= 6) hipLaunchKernelGGL((k_kv_prefill<DT, NC, true>), grid, dim3(256), 0, stream, a);
+  if (a.seqs.shift >= 6) hipLaunchKernelGGL((k_kv_prefill<DT, NC, true>), grid, dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((k_kv_prefill<DT, NC, false>), grid, dim3(256), 0, stream, a);
   hipLaunchKernelGGL((k_kv_join_tiles<DT>), dim3((unsigned)((kSlots / heads + 1) * heads), 4), dim3(256), 0, stream, a);
 }
@@ -512,6 +508,7 @@ template <int DT>
 void launch_of(const KvAttendArgs& a, int64_t tiles, hipStream_t stream) {
   if (a.cache.dim <= 64) launch<DT, 1>(a, tiles, stream);
   else if (a.cache.dim <= 128) launch<DT, 2>(a, tiles, stream);
+  else if (a.cache.dim <= 192) launch<DT, 3>(a, tiles, stream);
   else launch<DT, 4>(a, tiles, stream);
 }
 
