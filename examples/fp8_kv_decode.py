@@ -1,0 +1,114 @@
+"""Samples of a prompt, decoded by an attention block on FP8 weights over an FP8 KV cache.
+
+    python examples/fp8_kv_decode.py [prompt tokens] [samples] [steps]
+
+The layer's linears run on 128x128-tile FP8 weights (``fp8_matmul``, ``fp8_block_linear``),
+keys and values live in an ``FP8KVCache``.  The prompt is appended and attended to once;
+``fork`` gives its pages to every sample; then each step makes room for a token
+(``resize``, which copies the page that the prompt ends in for each sample that writes to
+it), appends and attends.  In the end one sample goes on alone: the others' pages are given
+back and ``compact`` moves what is left together.
+"""
+
+from __future__ import annotations
+
+import os
+import sys
+
+import torch
+import torch.nn.functional as F
+
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "lumen-rl_amd"))
+from lumenrl_amd.quantization import (  # noqa: E402
+    FP8KVCache,
+    fp8_block_linear,
+    fp8_block_quant,
+    fp8_matmul,
+    quantize_fp8_blockwise,
+)
+
+
+class Attention:
+    """A layer's attention: q, k and v of x, the cache, o_proj."""
+
+    def __init__(self, cache, layer, hidden, heads, generator):
+        def weight(*shape):
+            return (torch.randn(shape, generator=generator, device=cache.device) * shape[-1] ** -0.5).bfloat16()
+
+        self.cache, self.layer, self.heads = cache, layer, heads
+        self.dense = {"q": weight(heads * cache.dim, hidden), "k": weight(cache.kv_heads * cache.dim, hidden),
+                      "v": weight(cache.kv_heads * cache.dim, hidden), "o": weight(hidden, heads * cache.dim)}
+        self.fp8 = {name: quantize_fp8_blockwise(w) for name, w in self.dense.items()}
+
+    def __call__(self, x, table, lengths, offsets=None):
+        """x [tokens, hidden] of sequences whose ``lengths`` count them in."""
+        codes, scales = fp8_block_quant(x, (1, 128))
+        q, k, v = (fp8_matmul(codes, scales, *self.fp8[name]).view(x.shape[0], -1, self.cache.dim) for name in "qkv")
+        self.cache.append(self.layer, k, v, table, lengths, offsets)
+        out = self.cache.attend(self.layer, q, table, lengths, offsets)
+        return fp8_block_linear(out.flatten(1), *self.fp8["o"])
+
+    def reference(self, x):
+        """The same of one whole sequence x [tokens, hidden] on the bf16 weights, in float32, with nothing cached."""
+        q, k, v = (F.linear(x.float(), self.dense[name].float()).view(x.shape[0], -1, self.cache.dim).transpose(0, 1) for name in "qkv")
+        k, v = (t.repeat_interleave(self.heads // self.cache.kv_heads, 0) for t in (k, v))
+        s = torch.matmul(q, k.transpose(1, 2).contiguous()) * self.cache.dim ** -0.5
+        s = s.masked_fill(torch.ones_like(s[0]).triu(1).bool(), -torch.inf)
+        return F.linear(torch.matmul(torch.softmax(s, -1), v).transpose(0, 1).flatten(1), self.dense["o"].float())
+
+
+def main(prompt: int = 300, samples: int = 4, steps: int = 40, layers: int = 2) -> dict:
+    hidden, heads = 1024, 8
+    width = (prompt + steps + 63) // 64
+    cache = FP8KVCache.empty(layers, (samples + 1) * width, 2, 128)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    blocks = [Attention(cache, i, hidden, heads, g) for i in range(layers)]
+    x = torch.randn(prompt, hidden, generator=g, device="cuda").bfloat16()
+    inputs = torch.randn(steps, samples, hidden, generator=g, device="cuda").bfloat16()
+
+    def run(x, *where):
+        for block in blocks:
+            x = x + block(x, *where)
+        return x
+
+    # the prompt, as row 0
+    table = torch.full((samples, width), -1, dtype=torch.int32, device="cuda")
+    lengths = torch.zeros(samples, dtype=torch.int32, device="cuda")
+    wanted = lengths.clone()
+    wanted[0] = prompt
+    table, lengths, _ = cache.resize(table, lengths, wanted)
+    offsets = torch.full((samples + 1,), prompt, dtype=torch.int32, device="cuda")
+    offsets[0] = 0
+    first = run(x, table, lengths, offsets)
+
+    # its samples
+    table, lengths = cache.fork(table, lengths, torch.zeros_like(lengths))
+    shared = int((cache.refs > 0).sum())
+    outs = []
+    for step in range(steps):
+        table, lengths, short = cache.resize(table, lengths, lengths + 1)
+        outs.append(run(inputs[step], table, lengths))
+    used = int((cache.refs > 0).sum())
+
+    # the last one goes on alone, in pages moved together
+    wanted = torch.zeros_like(lengths)
+    wanted[-1] = lengths[-1]
+    table, lengths, _ = cache.resize(table, lengths, wanted)
+    table, kept = cache.compact(table)
+    again = cache.attend(0, torch.zeros(samples, heads, 128, dtype=torch.bfloat16, device="cuda"), table, lengths)
+
+    errors = {"pages of the prompt": shared, "pages of all samples": used, "pages of the last one": int(kept), "pages short": int(short)}
+    whole = torch.stack(outs, 1)  # [samples, steps, hidden]
+    for s in (0, samples - 1):
+        want = torch.cat([x, inputs[:, s]])
+        for block in blocks:
+            want = want + block.reference(want)
+        got = torch.cat([first, whole[s]]).float()
+        errors[f"sample {s}"] = float((got - want).norm() / want.norm())
+    errors["ended samples see nothing"] = bool((again[:-1] == 0).all()) and bool((again[-1] != 0).any())
+    return errors
+
+
+if __name__ == "__main__":
+    for name, value in main(*(int(v) for v in sys.argv[1:])).items():
+        print(f"{name}: {value if not isinstance(value, float) else f'{value:.4f} of the bf16 weights result without a cache'}")

@@ -2,7 +2,9 @@
 
 from __future__ import annotations
 
+import importlib.util
 import math
+import os
 import random
 
 import pytest
@@ -604,6 +606,21 @@ def test_a_rollout():
     step([r % 2 for r in range(rows)])
     table, lengths, _ = c.resize(table, lengths, lengths * 0)
     assert int(c.refs.abs().max()) == 0 and bool((table == -1).all())
+
+
+def test_the_example_runs():
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples", "fp8_kv_decode.py")
+    spec = importlib.util.spec_from_file_location("fp8_kv_decode", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    got = mod.main(prompt=150, samples=3, steps=50, layers=2)
+    # 150 tokens are 3 pages, 2 of them full; each sample has 200, so 2 pages of its own more
+    assert (got["pages of the prompt"], got["pages of all samples"], got["pages of the last one"], got["pages short"]) == (3, 8, 4, 0)
+    assert got["ended samples see nothing"]
+    # A rounding to e4m3 is 2^-4 / sqrt(3) = 0.036 of a value in the mean square at most.  x, a weight, the code, o_proj's
+    # input and weight are five on the way through v: 0.081 of a block's result; x, two weights and K's code move the
+    # scores, which are about 1, by 0.08 more: 0.12 in all, of what a block adds to the stream.
+    assert 0.0 < got["sample 0"] < 0.15 and 0.0 < got["sample 2"] < 0.15
 
 
 def test_a_captured_step_replays():
