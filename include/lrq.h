@@ -269,17 +269,18 @@ int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, 
  * lrq_kv_append writes new tokens, k and v [tokens, kv_heads, dim] (bf16, fp16 or
  *   float32; element strides k_token .. v_head) into one layer.  Rows offsets[b] ..
  *   offsets[b + 1] - 1 are sequence b's last tokens, which `lengths` counts in already;
- *   offsets null: one token each.  A page's scale is the least power of two, from 2^-48
- *   to 2^48, that takes the largest finite magnitude to 448 at most; where tokens join a
- *   page it does not shrink, and where it grows, the codes there are rounded to it again.
- *   Inf, NaN, and what a scale of 2^48 takes past 448 become NaN codes.
+ *   offsets do not go back; null: one token each.  A page's scale is the least power of
+ *   two, from 2^-48 to 2^48, that takes the largest finite magnitude to 448 at most; where
+ *   tokens join a page it does not shrink, and where it grows, the codes there are rounded
+ *   to it again.  Inf, NaN, and what a scale of 2^48 takes past 448 become NaN codes.
  * lrq_kv_attend: out [tokens, heads, dim] = softmax(scale q k^T) v for the same rows, each
  *   over its sequence's keys up to its own place, the last `window` of them if that is
  *   above 0; query head i reads KV head i / (heads / kv_heads).  Scores and sums are
  *   float32, probabilities are rounded to fp16.  A row that sees no key is 0; a NaN is
  *   in the results of the rows that see it alone.  lse: [tokens, heads], the scores' log-sum-exp
- *   (natural), or null.  Rows behind offsets[seqs] stay as they were, or become 0 with
- *   zero_rest.  q is bf16 or fp16, out of its type, dense, 8-byte aligned.
+ *   (natural), or null.  Rows of no sequence (before offsets[0], behind offsets[seqs]) stay
+ *   as they were, or become 0 (lse: -inf) with zero_rest.  q is bf16 or fp16, out of its
+ *   type, dense, 8-byte aligned, and q itself or apart from it.
  *   `workspace`: lrq_kv_attend_workspace bytes (one_each: no offsets), 256-byte aligned,
  *   overwritten.
  * The three below write a new table (dense [rows, width], -1 behind a row's pages) and

@@ -366,6 +366,7 @@ struct KvTiles {  // lrq_kv_prefill.hip's plan, in the workspace
   v4i* piece;             // two each: sequence, tile, first unit, last + 1; place of its sums or -1
   v4i* cut;               // sequence, tile, place of its first piece's sums, pieces
   float* sums;
+  int most, shares;       // tiles; work-groups that work at a time
 };
 struct KvAttendArgs {
   KvCache cache;

@@ -103,8 +103,8 @@ struct PartHead {
 static_assert(sizeof(PartHead) == 32, "the join's heads are 32 bytes apart");
 
 // Waves of a SIMD, by the registers they need.
-template <int NC, int MT, bool FAST>
-constexpr int kPerSimd = MT * NC > 2 ? 1 : MT * NC == 1 || (FAST && MT == 1) ? 2 : 2;
+template <int NC, int MT>
+constexpr int kPerSimd = MT * NC > 2 ? 1 : 2;
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
@@ -118,7 +118,11 @@ __device__ __forceinline__ int piece_at(int count, int i, int n) {
 // time (256 sequences of up to 8100 keys: 2, 3, 4, 6 and 8 a SIMD take 428, 403, 408, 411 and
 // 423 us; one wave a SIMD 411, three 461).
 constexpr int kParts = 256 * 4 * 3;
-constexpr uint32_t kLeast = 2;  // units of a piece, if the item has as many
+// Units of a piece at least, if the item has as many; a piece of two tiles leaves twice the sums
+// (8000 keys, one row of 16 on each head: 1, 2 and 4 units 15.4, 15.9 and 17.4 us; 128 tokens of
+// 4 rows on 2000 keys: 2 units 48.8, 4 units 39.3 us, 48 of up to 5 tokens 23.0 and 21.9).
+template <int MT>
+constexpr uint32_t kLeast = 2 * MT;
 
 // An address that is the same in all lanes, kept in scalar registers: loads add a lane's
 // 32-bit offset and a constant to it by themselves, up to 4095.
@@ -128,16 +132,19 @@ __device__ __forceinline__ const uint8_t* in_scalars(const uint8_t* p) {
 }
 
 // One tile of rows a sequence: each code is read once, past the caches (256 sequences of up to
-// 8100 keys 416 -> 408 us).  More tiles find them in the caches.
-template <int MT>
+// 8100 keys 410 -> 393 us).  More tiles find them in the caches, which heads of more than 128
+// channels have with 17 rows already (32 sequences of 32 rows and 4000 keys of 192 channels:
+// past the caches 152, else 108 us).
+template <int NC, int MT>
 __device__ __forceinline__ v4u codes_at(const uint8_t* p) {
-  return MT == 1 ? gld_nt<v4u>(p) : gld<v4u>(p);
+  return MT == 1 && NC <= 2 ? gld_nt<v4u>(p) : gld<v4u>(p);
 }
 
 // FAST: heads of 64 NC channels and pages of 64 keys, which are the constants of the
-// addresses then, and a page is one for the whole wave.
+// addresses then, and a page is one for the whole wave (16, 32 and 64 rows on 4000 keys, 32
+// times, 66, 82 and 104 us; without it 78, 102 and 152).
 template <int DT, int NC, int MT, bool FAST>
-__global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_attend(KvAttendArgs a) {
+__global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT>)) void k_kv_attend(KvAttendArgs a) {
   constexpr int NT = 4 * NC;       // tiles of 16 channels
   constexpr int ROWS = 16 * MT;
   __shared__ int64_t scan[kWaves];
@@ -151,14 +158,16 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
 
   // rows of the result that are no sequence's
   if (a.zero_rest) {
-    int64_t lo = a.seqs.seqs, hi = a.seqs.tokens;
-    if (a.seqs.offsets != nullptr) lo = gld<int32_t>(a.seqs.offsets + a.seqs.seqs);
-    lo = lo < 0 ? 0 : lo;
+    int64_t lead = 0, lo = a.seqs.seqs;  // rows before the first sequence, and where those behind the last begin
+    if (a.seqs.offsets != nullptr) lead = gld<int32_t>(a.seqs.offsets), lo = gld<int32_t>(a.seqs.offsets + a.seqs.seqs);
+    lead = lead < 0 ? 0 : lead < a.seqs.tokens ? lead : a.seqs.tokens, lo = lo < lead ? lead : lo;
     const int64_t words = (int64_t)a.heads * dim / 2;
-    for (int64_t t = lo + blockIdx.x; t < hi; t += gridDim.x) {
-      for (int64_t i = tid; i < words; i += 64 * kWaves) gst<uint32_t>(static_cast<uint32_t*>(a.out) + t * words + i, 0u);
+    for (int64_t i = blockIdx.x;; i += gridDim.x) {
+      const int64_t t = i < lead ? i : lo + (i - lead);
+      if (t >= a.seqs.tokens) break;
+      for (int64_t w = tid; w < words; w += 64 * kWaves) gst<uint32_t>(static_cast<uint32_t*>(a.out) + t * words + w, 0u);
       if (a.lse != nullptr)
-        for (int i = tid; i < a.heads; i += 64 * kWaves) gst<float>(a.lse + t * a.heads + i, -INFINITY);
+        for (int w = tid; w < a.heads; w += 64 * kWaves) gst<float>(a.lse + t * a.heads + w, -INFINITY);
     }
   }
 
@@ -176,8 +185,12 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
     if (blockIdx.x == 0 && tid == 0) gst<int32_t>(a.cut_count, 0);
     return;
   }
-  // units of a piece: below 2^31, as the items are at most a.parts times as many as that
-  const uint32_t per = total <= kLeast * kParts ? kLeast : (uint32_t)((total + kParts - 1) / kParts);
+  // units of a piece, where a line has less than 2^25
+  const int64_t share = (total + kParts - 1) / kParts;
+  const uint32_t per = share < kLeast<MT> ? kLeast<MT> : share < 1 << 25 ? (uint32_t)share : 1u << 25;
+  // Offsets that go back would make rows of several sequences', and more pieces than there are
+  // waves: sequences whose pieces have not all one are left out.
+  const uint32_t limit = gridDim.x * kWaves;
   if (tid < kWaves) found[tid][0] = -1;
   __syncthreads();
   // pieces so far; and those of items that are cut, with (times 2^16) these items: at most 2 kParts of each
@@ -188,13 +201,14 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
       else mine = Work{};
     }
     const uint32_t cuts = ((uint32_t)mine.count + per - 1) / per, pieces = cuts * (uint32_t)mine.lines;
-    const uint32_t cut = cuts > 1 ? pieces + ((uint32_t)mine.lines << 16) : 0;
     const uint32_t upto = before + block_scan<64 * kWaves, uint32_t>(pieces, scan32);
+    const bool in = upto <= limit;
+    const uint32_t cut = cuts > 1 && in ? pieces + ((uint32_t)mine.lines << 16) : 0;
     const uint32_t upto_cut = before_cut + block_scan<64 * kWaves, uint32_t>(cut, scan32);
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const uint32_t at = blockIdx.x * kWaves + w - (upto - pieces);  // wraps below 0
-      if (at < pieces) {
+      if (at < pieces && in) {
         const uint32_t first = upto_cut - cut;
         found[w][0] = b0 + tid, found[w][1] = (int)at, found[w][2] = (int)((first & 0xFFFF) + at), found[w][3] = (int)(first >> 16);
       }
@@ -202,7 +216,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
     if (tid == 64 * kWaves - 1) carry[0] = upto, carry[1] = upto_cut;
     __syncthreads();
     before = carry[0], before_cut = carry[1];
-    if (blockIdx.x > 0 && before > blockIdx.x * kWaves + kWaves - 1) break;
+    if (before > limit || (blockIdx.x > 0 && before > blockIdx.x * kWaves + kWaves - 1)) break;
   }
   if (blockIdx.x == 0 && tid == 0) gst<int32_t>(a.cut_count, (int32_t)(before_cut >> 16));
   __syncthreads();
@@ -242,7 +256,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
       for (int t = 0; t < 4; ++t) {
         if (t % 2 == 0) kb = in_scalars(a.cache.k + (int64_t)(page < 0 ? 0 : page) * a.cache.k_page + (int64_t)h * S * dim + 4 * t * dim);
 #pragma unroll
-        for (int k = 0; k < NC; ++k) kc[t][k] = codes_at<MT>(kb + k_lane + (4 * (t % 2) * dim + 64 * k));
+        for (int k = 0; k < NC; ++k) kc[t][k] = codes_at<NC, MT>(kb + k_lane + (4 * (t % 2) * dim + 64 * k));
       }
     } else {
       kb += ((u * kUnit + 16 * (r >> 2)) & (S - 1)) * dim;
@@ -251,7 +265,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
           kc[t][k] = v4u{0, 0, 0, 0};
-          if (64 * k + 16 * g < dim) kc[t][k] = codes_at<MT>(kb + k_lane + (4 * t * dim + 64 * k));
+          if (64 * k + 16 * g < dim) kc[t][k] = codes_at<NC, MT>(kb + k_lane + (4 * t * dim + 64 * k));
         }
     }
   };
@@ -261,14 +275,14 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT, FAST>)) void k_kv_at
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if (n % 4 == 0) vb = in_scalars(a.cache.v + (int64_t)(page < 0 ? 0 : page) * a.cache.v_page + (int64_t)h * S * dim + 16 * n * S);
-        vc[n] = codes_at<MT>(vb + v_lane + 16 * (n % 4) * S);
+        vc[n] = codes_at<NC, MT>(vb + v_lane + 16 * (n % 4) * S);
       }
     } else {
       vb += (u * kUnit + 16 * g) & (S - 1);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         vc[n] = v4u{0, 0, 0, 0};
-        if (16 * n < dim) vc[n] = codes_at<MT>(vb + v_lane + 16 * n * S);
+        if (16 * n < dim) vc[n] = codes_at<NC, MT>(vb + v_lane + 16 * n * S);
       }
     }
   };
@@ -552,10 +566,13 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttendArgs a) {
   }
 }
 
-// Sequences of more rows than kMostRows are k_kv_prefill's, but not in a call whose rows
-// are kAllRows together at most: three launches less.
+// Sequences of more rows than kMostRows are k_kv_prefill's (32 of 4000 keys: with 64 rows each
+// 103 us here and 110 there, with 96 rows 126 and 114), of more than half as many where tiles
+// are of 16 rows and not of 32 (192 channels, 64 rows: 216 and 188).  But not in a call whose
+// rows are kAllRows together at most: three launches less (one of 2000 keys: 1024 rows 50.6
+// and 54.4 us, 4096 rows 124 and 102).
 constexpr int kMostRows = 64, kAllRows = 1024;
-int most_rows(int64_t dim) { return dim <= 128 ? kMostRows : kMostRows / 2; }  // (tiles of 16 rows there, not 32)
+int most_rows(int64_t dim) { return dim <= 128 ? kMostRows : kMostRows / 2; }
 // Rows of a call; one_each: one token a sequence.
 int64_t all_rows(int64_t tokens, int64_t seqs, bool one_each, int64_t group) { return (one_each && seqs < tokens ? seqs : tokens) * group; }
 bool all_few(int64_t rows, bool one_each, int64_t group, int64_t dim) { return one_each ? group <= most_rows(dim) : rows <= kAllRows; }
@@ -581,7 +598,8 @@ void launch(KvAttendArgs a, hipStream_t stream) {
   const int64_t items = most_items(rows, a.cache.heads, seqs, a.few == INT32_MAX);
   const int64_t pieces = most_pieces(items, a.seqs.width, a.seqs.shift);
   const int64_t groups = pieces > 0 ? (pieces + kWaves - 1) / kWaves : 1;
-  // few items: a work-group for 32 channels of each
+  // few items: a work-group for 32 channels of each (8000, 120000 and 500000 keys of one token
+  // 16, 61 and 182 us; 25, 83 and 204 with one for all channels; 8 channels 17, 58 and 180)
   const int64_t joins = items < 2048 ? items : 2048;
   const int split = items <= 256 && a.cache.dim % 32 == 0 ? a.cache.dim / 32 : 1;
   if (a.cache.dim == 64 * NC && a.seqs.shift == 6)
@@ -599,7 +617,8 @@ void launch_dim(const KvAttendArgs& a, hipStream_t stream) {
 }
 template <int DT>
 void launch_of(const KvAttendArgs& a, hipStream_t stream) {
-  // two tiles of 16 rows a wave where a sequence has more than one
+  // Two tiles of 16 rows a wave where a sequence has more than one: 32 rows on 4000 keys, 32 times,
+  // 82 us, 97 by single tiles; 4 rows on up to 8100, 256 times, 400 us, 393 by single tiles.
   const int64_t rows = a.seqs.offsets == nullptr ? a.group : a.seqs.tokens * a.group / (a.seqs.seqs > 0 ? a.seqs.seqs : 1);
   if (rows > 16) launch_dim<DT, 2>(a, stream);
   else launch_dim<DT, 1>(a, stream);

@@ -28,8 +28,15 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTileRows = 128;
-constexpr int kSlots = 512;     // shares that the work is cut into: two work-groups a compute unit
-constexpr int kLeastUnits = 8;  // below it a tile is not cut: its pieces' sums cost as much
+// Shares that the work is cut into, at most: a work-group that a compute unit holds each, two of
+// them, or one with heads of more than 128 channels (32 prompts of 24 tokens on 4000 keys: 128
+// channels, 512 shares 114, 256 shares 129 us; 192 channels, 192 and 166).
+constexpr int kSlots = 512;
+template <int NC>
+constexpr int kShares = NC > 2 ? kSlots / 2 : kSlots;
+// Below it a tile is not cut: its pieces' sums cost as much (42 prompts of 40 to 68 tokens on up
+// to 1138 keys, 8 units 62 us, 4 units 72; one of 912 tokens on 21, 36 and 33).
+constexpr int kLeastUnits = 8;
 constexpr float kSlack = 5.0f;  // what a row's maximum may grow by before its sums are scaled (p stays below 2^15)
 
 template <int DT>
@@ -92,12 +99,14 @@ __global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
   for (int b0 = 0; b0 < seqs; b0 += 1024) {
     const int64_t base = carry;
     const int64_t upto = base + block_scan<1024, int64_t>(b0 + tid < seqs ? tiles_of(a, b0 + tid) : 0, scan);
-    if (b0 + tid < seqs) gst<int32_t>(p.upto + b0 + tid, (int32_t)upto);
-    ends[tid] = (int)upto;
+    // offsets that go back would make rows of several sequences', and more tiles than there is room for
+    const int end = upto < p.most ? (int)upto : p.most;
+    if (b0 + tid < seqs) gst<int32_t>(p.upto + b0 + tid, end);
+    ends[tid] = end;
     if (tid == 1023) carry = upto;
     __syncthreads();
   }
-  const int tiles = (int)carry;
+  const int tiles = carry < p.most ? (int)carry : p.most;
   __syncthreads();
   auto end_of = [&](int b) { return seqs <= 1024 ? ends[b] : gld<int32_t>(p.upto + b); };
   auto find = [&](int i, int& tile) {  // the sequence of tile i
@@ -134,7 +143,7 @@ __global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
   const int64_t sum = block_scan<1024, int64_t>(units, scan);
   if (tid == 1023) carry = sum;
   __syncthreads();
-  int64_t most = (carry * a.cache.heads + kSlots - 1) / kSlots;
+  int64_t most = (carry * a.cache.heads + p.shares - 1) / p.shares;
   if (most < kLeastUnits) most = kLeastUnits;
   auto cuts_of = [&](int n) { return n <= most ? 1 : (int)((n + most - 1) / most); };
   auto bucket_of = [&](int n) { return n >= kBuckets ? 0 : kBuckets - 1 - n; };
@@ -174,7 +183,8 @@ __global__ __launch_bounds__(1024) void k_kv_tiles(KvAttendArgs a) {
 }
 
 // Heads of more than 64 (NC - 1) channels, 64 NC at most: those that are not there are zeros.
-// FAST: pages of 64 keys or more, so that a unit is of one page.
+// FAST: pages of 64 keys or more, so that a unit is of one page (4 prompts of up to 4000 tokens
+// 591 us; 626 without it).
 template <int DT, int NC, bool FAST>
 __global__ __launch_bounds__(256, NC > 2 ? 1 : 2) void k_kv_prefill(KvAttendArgs a) {
   constexpr int KS = 4 * NC, VT = 2 * NC;       // steps of 16 channels, tiles of 32
@@ -496,8 +506,9 @@ __global__ __launch_bounds__(256) void k_kv_join_tiles(KvAttendArgs a) {
 }
 
 template <int DT, int NC>
-void launch(const KvAttendArgs& a, int64_t tiles, hipStream_t stream) {
+void launch(KvAttendArgs a, int64_t tiles, hipStream_t stream) {
   const int64_t heads = a.cache.heads;
+  a.tiles.shares = kShares<NC>;
   hipLaunchKernelGGL(k_kv_tiles, dim3(1), dim3(1024), 0, stream, a);
   const dim3 grid((unsigned)((tiles + 2 * kSlots / heads + 1) * heads));
   if (a.seqs.shift >= 6) hipLaunchKernelGGL((k_kv_prefill<DT, NC, true>), grid, dim3(256), 0, stream, a);
@@ -533,6 +544,7 @@ hipError_t launch_kv_prefill(KvAttendArgs a, int dtype, int64_t tiles, void* wor
   a.tiles.piece = reinterpret_cast<v4i*>(w), w += pad256(32 * most_pieces(tiles, heads));
   a.tiles.cut = reinterpret_cast<v4i*>(w), w += pad256(16 * (kSlots / heads + 1));
   a.tiles.sums = reinterpret_cast<float*>(w);
+  a.tiles.most = (int)tiles;
   if (dtype == kBF16) launch_of<kBF16>(a, tiles, stream);
   else launch_of<kF16>(a, tiles, stream);
   return hipGetLastError();

@@ -11,8 +11,10 @@ caller keeps: ``table`` int32 [rows, width] with a row's page numbers in order a
 and ``fork`` makes samples of a prompt share its pages, ``resize`` to 0 ends a sequence,
 ``compact`` moves what is left together.  Everything runs on the current stream of the
 cache's device, reads lengths and tables there, and returns without synchronizing, so a
-step can be captured into a graph.  What tables, lengths and offsets hold is clamped to
-what there is: an entry that is no page of the pool is no page.
+step can be captured into a graph.  Calls that write a page are the caller's to keep in order
+with others on that page, ``fork``, ``resize`` and ``compact`` with each other.  What tables,
+lengths and offsets hold is clamped to what there is: an entry that is no page of the pool is
+no page.  Offsets do not go back; what becomes of rows that two sequences claim is open.
 """
 
 from __future__ import annotations
@@ -205,8 +207,9 @@ class FP8KVCache:
         given.  Query head i reads KV head ``i // (heads // kv_heads)``; ``scale`` is
         ``dim ** -0.5`` by default.  Scores and sums are float32, probabilities are rounded
         to fp16.  A token that sees no key gets 0; a NaN reaches the tokens that see it.
-        Rows of no sequence (behind the last one) are 0, in a given ``out`` (dense, of q's shape
-        and type) they stay as they are.  ``return_lse`` adds the scores' log-sum-exp,
+        Rows of no sequence (before the first one or behind the last) are 0, in a given ``out``
+        (dense, of q's shape and type, q itself or apart from it) they stay as they are.
+        ``return_lse`` adds the scores' log-sum-exp,
         float32 [tokens, heads] (-inf where nothing is seen).  No gradient: a backward
         pass through the result raises.
         """

@@ -82,6 +82,15 @@ ATTEND = [
     (torch.float16, 8, 1, 64, 32, [128, 1, 200], [1000, 5, 0], 0),
     (torch.bfloat16, 8, 1, 128, 256, [140, 17], [2000, 3], 600),
     (torch.float16, 16, 1, 208, 64, [77], [130], 0),
+    # heads of up to three and four times 64 channels, few rows and many, pages of more than a unit and of less
+    (torch.bfloat16, 8, 2, 192, 64, [1, 3, 9], [700, 64, 0], 0),
+    (torch.float16, 8, 2, 192, 128, [200, 1, 40], [700, 64, 0], 0),
+    (torch.bfloat16, 8, 2, 144, 64, [300, 9], [70, 300], 100),
+    (torch.float16, 8, 2, 256, 64, [1, 300, 8], [129, 70, 10], 0),
+    (torch.bfloat16, 8, 2, 240, 128, [300, 9], [70, 300], 0),
+    (torch.float16, 8, 2, 176, 16, [300, 9], [70, 300], 0),
+    (torch.bfloat16, 8, 2, 112, 64, [300, 9], [70, 300], 0),
+    (torch.float16, 8, 2, 48, 256, [300, 9], [70, 300], 0),
 ]
 
 
@@ -194,6 +203,54 @@ def test_attend_rows_behind_the_last_sequence():
     out = c.attend(0, q, ints(table)[:0], ints([]), ints([0]))
     assert bool((out == 0).all())
     assert c.attend(0, q[:0], ints(table), ints(lengths), ints([0, 0, 0])).shape == (0, 4, dim)
+
+
+@pytest.mark.parametrize("tokens", [9, 700])  # 700: by tiles of many rows
+def test_attend_rows_before_the_first_sequence(tokens):
+    c = make(1, 40, 1, 64, 64)
+    table, lengths = ints([list(range(20)), list(range(20, 40))]), ints([1100, 900])
+    q = queries(tokens, 4, 64, torch.bfloat16)
+    # (against the definition: a call of fewer rows may take its sums in another order, and so differ in their last bits)
+    want, bound, _ = R.attend(c, 0, q[3:], table.tolist(), [1100, 900], [0, tokens - 5, tokens - 4], 64 ** -0.5, 0)
+    out, lse = c.attend(0, q, table, lengths, ints([3, tokens - 2, tokens - 1]), return_lse=True)
+    close(out[3:], want, bound)
+    assert bool((out[3:-1] != 0).any(-1).all())
+    assert bool((out[:3] == 0).all()) and bool((lse[:3] == -math.inf).all()) and bool((out[-1] == 0).all())
+    mine = torch.full_like(q, 7.0)
+    c.attend(0, q, table, lengths, ints([3, tokens - 2, tokens - 1]), out=mine)
+    assert torch.equal(mine[3:-1], out[3:-1]) and bool((mine[:3] == 7.0).all()) and bool((mine[-1] == 7.0).all())
+    # the result in the queries' place
+    there = q.clone()
+    assert c.attend(0, there, table, lengths, ints([3, tokens - 2, tokens - 1]), out=there) is there
+    assert torch.equal(there[3:-1], out[3:-1]) and torch.equal(there[:3], q[:3])
+
+
+@pytest.mark.parametrize("tokens,heads,seqs", [(100, 4, 8), (250, 4, 41), (250, 4, 600), (600, 4, 8), (600, 4, 41), (600, 4, 2050)])
+def test_offsets_that_go_back_stay_within_the_call(tokens, heads, seqs):
+    """Every second sequence claims all rows: more work than there is room for.  What those rows become is
+    open; nothing else is written, and calls after it are right."""
+    c = make(1, 600, 2, 64, 64)
+    kept = [x.clone() for x in (c.k.view(torch.uint8), c.v.view(torch.uint8), c.k_scales, c.v_scales)]
+    table, lengths = (torch.arange(seqs * 6, device=DEV, dtype=torch.int32) % 600).view(seqs, 6), torch.full((seqs,), 380, device=DEV, dtype=torch.int32)
+    offsets = ints([tokens * (i % 2) for i in range(seqs + 1)])
+    q = queries(tokens, heads, 64, torch.bfloat16)
+    around = torch.full((tokens + 8, heads, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    c.attend(0, q, table, lengths, offsets, out=around[4:-4])
+    torch.cuda.synchronize()
+    assert bool((around[:4] == 7.0).all()) and bool((around[-4:] == 7.0).all())
+    for x, y in zip(kept, (c.k.view(torch.uint8), c.v.view(torch.uint8), c.k_scales, c.v_scales)):
+        assert torch.equal(x, y)
+    k = queries(tokens, 2, 64, torch.bfloat16)
+    used = table[:, 380 // 64 - tokens // 64 - 1:].unique() if tokens < 300 else table.unique()
+    c.append(0, k, k, table, lengths, offsets)
+    rest = torch.ones(600, dtype=torch.bool, device=DEV)
+    rest[used.long()] = False
+    assert torch.equal(kept[0][:, rest], c.k.view(torch.uint8)[:, rest]) and torch.equal(kept[1][:, rest], c.v.view(torch.uint8)[:, rest])
+    good = [0, tokens // 2, tokens]
+    rows = [[j for j in range(6)], [j + 6 for j in range(6)]]
+    c = make(1, 600, 2, 64, 64)
+    want, bound, _ = R.attend(c, 0, q, rows, [380, 380], good, 64 ** -0.5, 0)
+    close(c.attend(0, q, ints(rows), ints([380, 380]), ints(good)), want, bound)
 
 
 def test_attend_rows_that_see_nothing():
@@ -664,6 +721,42 @@ def test_a_captured_step_replays():
             torch.cuda.synchronize()
         assert torch.equal(gt, table) and torch.equal(gl, lengths) and torch.equal(out, want), i
         assert torch.equal(caught.refs, eager.refs)
+
+
+def test_a_captured_call_of_prompts_and_single_tokens_replays():
+    """Prompts, single tokens and NaN codes in one graph, whose batch changes from replay to replay."""
+    page, kv, heads, dim, rows, width, tokens = 16, 2, 8, 64, 6, 40, 900
+    g = torch.Generator(device=DEV).manual_seed(5)
+    c = make(1, 260, kv, dim, page)
+    q = torch.empty(tokens, heads, dim, dtype=torch.float16, device=DEV)
+    table, lengths, offsets = ints([[-1] * width] * rows), ints([0] * rows), ints([0] * (rows + 1))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        c.attend(0, q, table, lengths, offsets, return_lse=True)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = c.attend(0, q, table, lengths, offsets, return_lse=True)
+    rng = random.Random(4)
+    for i in range(12):
+        new = [rng.choice([0, 1, 1, 7, 130, 400]) for _ in range(rows)]
+        while sum(new) > tokens:
+            new[rng.randrange(rows)] = 1
+        n = [a + rng.randrange(0, 200) for a in new]
+        table.copy_(ints(R.spread_table(n, page, width, 260, i)))
+        lengths.copy_(ints(n)), offsets.copy_(ints([sum(new[:j]) for j in range(rows + 1)]))
+        q.copy_(torch.randn(q.shape, generator=g, device=DEV))
+        if i % 3 == 2:  # a NaN code where some rows see it and others do not
+            row = max(range(rows), key=lambda r: n[r])
+            c.v.view(torch.uint8)[0, table[row, (n[row] - 1) // page].long(), 0, 3, (n[row] - 1) % page] = 0x7F
+        want, wl = c.attend(0, q, table, lengths, offsets, return_lse=True)
+        graph.replay()
+        if i % 4 == 0:
+            torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16)) and torch.equal(lse, wl), i
+        assert bool(want.isnan().any()) == (i % 3 == 2), i
+        c.v.copy_(make(1, 260, kv, dim, page).v)
 
 
 def test_two_streams_at_once():
