@@ -6,7 +6,8 @@
 // rounded to it again; where they are the page's first, its scale starts anew.  Infinities
 // and NaN become NaN codes and leave the scale alone.
 //
-// Bound by its bytes: a page and head of 64 tokens reads 32 KiB (bf16) and writes 16.  Its
+// Bound by its bytes: a page and head of 64 tokens reads 32 KiB (bf16) and writes 16.  32 prompts
+// of 33 to 1500 tokens on 8 heads of 128 (154 MB) take 35 us, 4.4 TB/s (a copy: 4.7).  A page's
 // values are read once, into registers, where both passes (the maximum, the codes) find them.
 // V is turned round on its way: codes go through LDS as words of four channels, and come out
 // as eight tokens of four channels, whose bytes are exchanged in registers.

@@ -3,7 +3,9 @@
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c (q . k_j) - m),   c = scale log2(e),
 // with m the running maximum of a row, in one pass over the keys.  A row is a new token
 // and one of its query heads; the rows that share a KV head are taken together, 16 a
-// work-group, so that each code is read once for all of them.
+// work-group, so that each code is read once for all of them.  Bound by the codes' bytes:
+// 256 sequences of up to 8100 keys on 8 heads of 128 (2.1 GB) take 392 us, 5.4 TB/s, where a
+// read of as much and nothing else reaches 6.2; one of 1500 keys 13 us, two launches' latency.
 //
 // Both products run on bf16 or fp16 matrix instructions (float32 sums): e4m3 codes are
 // exact in both types, and the keys' scale is applied to the sums.  The first product
