@@ -273,6 +273,8 @@ int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, 
  *   two, from 2^-48 to 2^48, that takes the largest finite magnitude to 448 at most; where
  *   tokens join a page it does not shrink, and where it grows, the codes there are rounded
  *   to it again.  Inf, NaN, and what a scale of 2^48 takes past 448 become NaN codes.
+ *   `workspace`: lrq_kv_append_workspace bytes (one_each: no offsets), 256-byte aligned,
+ *   overwritten; 0 for up to 256 sequences.
  * lrq_kv_attend: out [tokens, heads, dim] = softmax(scale q k^T) v for the same rows, each
  *   over its sequence's keys up to its own place, the last `window` of them if that is
  *   above 0; query head i reads KV head i / (heads / kv_heads).  Scores and sums are
@@ -304,9 +306,11 @@ typedef struct lrq_kv_cache {
   int64_t k_layer, v_layer, ks_layer, vs_layer;
   int64_t k_page, v_page, ks_page, vs_page;
 } lrq_kv_cache;
+int64_t lrq_kv_append_workspace(int64_t seqs, int one_each);
 int lrq_kv_append(const lrq_kv_cache* cache, int64_t layer, const void* k, int64_t k_token, int64_t k_head, const void* v,
                   int64_t v_token, int64_t v_head, int dtype, int64_t tokens, const int32_t* table, int64_t ld, int64_t width,
-                  const int32_t* lengths, const int32_t* offsets, int64_t seqs, lrq_stream_t stream);
+                  const int32_t* lengths, const int32_t* offsets, int64_t seqs, void* workspace, int64_t workspace_bytes,
+                  lrq_stream_t stream);
 int64_t lrq_kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int one_each);
 int lrq_kv_attend(const lrq_kv_cache* cache, int64_t layer, const void* q, int64_t q_token, int64_t q_head, int dtype,
                   int64_t tokens, int64_t heads, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,

@@ -947,9 +947,14 @@ int check_kv_tables(const char* what, const lrq_kv_cache* c, const int32_t* tabl
 }
 }  // namespace
 
+int64_t lrq_kv_append_workspace(int64_t seqs, int one_each) {
+  return seqs < 0 || seqs > 1 << 20 ? 0 : lrq::kv_append_workspace(seqs, one_each != 0);
+}
+
 int lrq_kv_append(const lrq_kv_cache* cache, int64_t layer, const void* k, int64_t k_token, int64_t k_head, const void* v,
                   int64_t v_token, int64_t v_head, int dtype, int64_t tokens, const int32_t* table, int64_t ld, int64_t width,
-                  const int32_t* lengths, const int32_t* offsets, int64_t seqs, lrq_stream_t stream) {
+                  const int32_t* lengths, const int32_t* offsets, int64_t seqs, void* workspace, int64_t workspace_bytes,
+                  lrq_stream_t stream) {
   g_err.clear();
   lrq::KvAppendArgs a{};
   const int rc = check_kv_seqs("kv_append", cache, layer, tokens, table, ld, width, lengths, offsets, seqs, &a.seqs);
@@ -964,9 +969,10 @@ int lrq_kv_append(const lrq_kv_cache* cache, int64_t layer, const void* k, int64
   if (lrq::kv_append_tiles(a.seqs) * cache->kv_heads >= int64_t(1) << 24)
     return fail(LRQ_ERR_ARG, "kv_append: %lld tokens of %lld sequences and %lld heads are more than one launch takes", (long long)tokens,
                 (long long)seqs, (long long)cache->kv_heads);
+  if (int err = check_workspace("kv_append", workspace, workspace_bytes, lrq::kv_append_workspace(seqs, !offsets))) return err;
   a.cache = kv_layer(*cache, layer);
   a.k = k, a.v = v, a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
-  return check_hip(lrq::launch_kv_append(a, dtype, (hipStream_t)stream), "kernel launch");
+  return check_hip(lrq::launch_kv_append(a, dtype, workspace, (hipStream_t)stream), "kernel launch");
 }
 
 int64_t lrq_kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, int one_each) {

@@ -357,9 +357,11 @@ struct KvAppendArgs {
   KvSeqs seqs;
   const void *k, *v;  // [tokens, heads, dim]
   int64_t k_token, k_head, v_token, v_head;  // strides
+  int32_t* upto;  // workspace: work-groups up to each sequence, or null
 };
+int64_t kv_append_workspace(int64_t seqs, bool one_each);
 int64_t kv_append_tiles(const KvSeqs& s);  // work-groups a head, at most
-hipError_t launch_kv_append(const KvAppendArgs& a, int dtype, hipStream_t stream);
+hipError_t launch_kv_append(KvAppendArgs a, int dtype, void* workspace, hipStream_t stream);
 
 struct KvTiles {  // lrq_kv_prefill.hip's plan, in the workspace
   int32_t *count, *upto;  // pieces, and tiles that were cut; tiles up to each sequence
@@ -381,6 +383,7 @@ struct KvAttendArgs {
   int few;  // rows of a sequence that k_kv_attend takes; those of more are k_kv_prefill's
   // workspace
   int32_t* cut_count;
+  int32_t *counts, *upto, *upto_cut;  // of k_kv_count, or null: units of a piece, pieces; up to each sequence
   uint8_t* heads_at;
   float* sums;
   KvTiles tiles;

@@ -182,6 +182,29 @@ __global__ __launch_bounds__(256) void k_kv_append_one(KvAppendArgs a) {
 // ---------------------------------------------------------------------------
 // Any number: a work-group for each page that a sequence's new tokens fall into, and head.
 // ---------------------------------------------------------------------------
+static_assert(kOwnSearch == 256, "a thread looks at one sequence");
+__device__ __forceinline__ int pages_written(const KvSeqs& s, int b) {
+  const KvSeq q = kv_seq(s, b);
+  const int start = q.len - q.n < 0 ? 0 : q.len - q.n;
+  return q.n > 0 && q.len > start ? ((q.len - 1) >> s.shift) - (start >> s.shift) + 1 : 0;
+}
+// With more than kOwnSearch sequences, one work-group before: pages up to each of them, and above
+// `limit` no higher.
+__global__ __launch_bounds__(1024) void k_kv_append_count(KvSeqs s, int32_t* upto, int limit) {
+  __shared__ int scan[16], carry;
+  const int tid = threadIdx.x;
+  int before = 0;
+  for (int b0 = 0; b0 < s.seqs; b0 += 1024) {
+    const int b = b0 + tid;
+    int end = before + block_scan<1024, int>(b < s.seqs ? pages_written(s, b) : 0, scan);
+    end = end > limit ? limit + 1 : end;
+    if (b < s.seqs) gst<int32_t>(upto + b, end);
+    if (tid == 1023) carry = end;
+    __syncthreads();
+    before = carry;
+    __syncthreads();
+  }
+}
 constexpr int kHeld = 4;                    // pieces of eight values of K, and of V, that a thread holds
 constexpr int kSlab = kHeld * 256 * 8;      // values of a work-group: a page of 64 tokens of 128 channels
 template <int DT>
@@ -192,28 +215,21 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
   extern __shared__ uint8_t turn[];  // codes of V, [token][dim + 4]
   const int tid = threadIdx.x, h = blockIdx.y, S = 1 << a.seqs.shift, dim = a.cache.dim;
   // which sequence, and which of the pages that its new tokens fall into
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  int64_t before = 0;
-  for (int b0 = 0; b0 < a.seqs.seqs; b0 += 256) {
-    int tiles = 0;
-    if (b0 + tid < a.seqs.seqs) {
-      const KvSeq q = kv_seq(a.seqs, b0 + tid);
-      const int start = q.len - q.n < 0 ? 0 : q.len - q.n;
-      if (q.n > 0 && q.len > start) tiles = ((q.len - 1) >> a.seqs.shift) - (start >> a.seqs.shift) + 1;
-    }
-    const int upto = block_scan<256>(tiles, lds_scan);
-    const int64_t mine = (int64_t)blockIdx.x - before - (upto - tiles);
-    if (mine >= 0 && mine < tiles) found[0] = b0 + tid, found[1] = (int)mine;
-    if (tid == 255) lds_scan[0] = upto;
+  int b, tile;
+  if (a.upto != nullptr) {
+    if (blockIdx.x >= (uint32_t)sld(a.upto + a.seqs.seqs - 1)) return;
+    b = kv_find(a.upto, a.seqs.seqs, blockIdx.x);
+    tile = (int)blockIdx.x - (b > 0 ? sld(a.upto + b - 1) : 0);
+  } else {
+    if (tid == 0) found[0] = -1;
     __syncthreads();
-    before += lds_scan[0];
-    const bool done = found[0] >= 0 || before > (int64_t)blockIdx.x;
+    const int tiles = tid < a.seqs.seqs ? pages_written(a.seqs, tid) : 0;
+    const int mine = (int)blockIdx.x - (block_scan<256>(tiles, lds_scan) - tiles);
+    if (mine >= 0 && mine < tiles) found[0] = tid, found[1] = mine;
     __syncthreads();
-    if (done) break;
+    b = __builtin_amdgcn_readfirstlane(found[0]), tile = __builtin_amdgcn_readfirstlane(found[1]);
+    if (b < 0) return;
   }
-  const int b = __builtin_amdgcn_readfirstlane(found[0]), tile = __builtin_amdgcn_readfirstlane(found[1]);
-  if (b < 0) return;
   const KvSeq q = kv_seq_uniform(a.seqs, b);
   // tokens whose place would be before the sequence's start have none
   const int skip = q.len - q.n < 0 ? q.n - q.len : 0, start = q.len - q.n + skip;
@@ -336,6 +352,7 @@ void launch(const KvAppendArgs& a, hipStream_t stream) {
     return;
   }
   const dim3 grid((unsigned)kv_append_tiles(a.seqs), (unsigned)a.cache.heads);
+  if (a.upto != nullptr) hipLaunchKernelGGL(k_kv_append_count, dim3(1), dim3(1024), 0, stream, a.seqs, a.upto, (int)grid.x);
   const int most = kSlab / a.cache.dim < 1 << a.seqs.shift ? kSlab / a.cache.dim : 1 << a.seqs.shift;
   hipLaunchKernelGGL((k_kv_append<DT>), grid, dim3(256), most * (a.cache.dim + 4), stream, a);
 }
@@ -348,7 +365,9 @@ int64_t kv_append_tiles(const KvSeqs& s) {
   const int64_t tiles = s.offsets == nullptr ? B : (T >> s.shift) + 2 * B;
   return tiles < T ? tiles : T;
 }
-hipError_t launch_kv_append(const KvAppendArgs& a, int dtype, hipStream_t stream) {
+int64_t kv_append_workspace(int64_t seqs, bool one_each) { return one_each || seqs <= kOwnSearch ? 0 : (4 * seqs + 255) / 256 * 256; }
+hipError_t launch_kv_append(KvAppendArgs a, int dtype, void* workspace, hipStream_t stream) {
+  a.upto = kv_append_workspace(a.seqs.seqs, a.seqs.offsets == nullptr) > 0 ? static_cast<int32_t*>(workspace) : nullptr;
   if (dtype == kBF16) launch<kBF16>(a, stream);
   else if (dtype == kF16) launch<kF16>(a, stream);
   else launch<kF32>(a, stream);

@@ -34,6 +34,7 @@ namespace lrq {
 namespace {
 
 constexpr int kWaves = 4;  // of a work-group, which share the search for where they begin
+static_assert(64 * kWaves == kOwnSearch, "a thread looks at one sequence");
 
 template <int DT>
 __device__ __forceinline__ f32x4 mma(v4u a, v4u b, f32x4 d) {
@@ -125,6 +126,22 @@ constexpr int kParts = 256 * 4 * 3;
 // 4 rows on 2000 keys: 2 units 48.8, 4 units 39.3 us, 48 of up to 5 tokens 23.0 and 21.9).
 template <int MT>
 constexpr uint32_t kLeast = 2 * MT;
+// Units of a piece, where a line has less than 2^25.
+template <int MT>
+__device__ __forceinline__ uint32_t units_of_piece(int64_t total) {
+  const int64_t share = (total + kParts - 1) / kParts;
+  return share < kLeast<MT> ? kLeast<MT> : share < 1 << 25 ? (uint32_t)share : 1u << 25;
+}
+// A sequence's pieces; and those of items that are cut, with (times 2^16) these items: at most
+// 2 kParts of each in a call.  Offsets that go back would make rows of several sequences', and
+// more pieces than there are waves: sequences whose pieces have not all one are left out.
+struct Pieces {
+  uint32_t pieces, cut;
+};
+__device__ __forceinline__ Pieces pieces_of(const Work& w, uint32_t per) {
+  const uint32_t cuts = ((uint32_t)w.count + per - 1) / per, pieces = cuts * (uint32_t)w.lines;
+  return Pieces{pieces, cuts > 1 ? pieces + ((uint32_t)w.lines << 16) : 0};
+}
 
 // An address that is the same in all lanes, kept in scalar registers: loads add a lane's
 // 32-bit offset and a constant to it by themselves, up to 4095.
@@ -142,6 +159,38 @@ __device__ __forceinline__ v4u codes_at(const uint8_t* p) {
   return MT == 1 && NC <= 2 ? gld_nt<v4u>(p) : gld<v4u>(p);
 }
 
+// With more than kOwnSearch sequences, one work-group before: pieces up to each of them.
+template <int MT>
+__global__ __launch_bounds__(1024) void k_kv_count(KvAttendArgs a, uint32_t limit) {
+  __shared__ int64_t scan[16];
+  __shared__ uint32_t scan32[16], carry[2], most;
+  const int tid = threadIdx.x, seqs = a.seqs.seqs;
+  if (tid == 0) most = 0;
+  int64_t units = 0;
+  for (int b = tid; b < seqs; b += 1024) {
+    const Work w = work_of<16 * MT>(a, kv_seq(a.seqs, b));
+    units += (int64_t)w.lines * w.count;
+  }
+  const uint32_t per = units_of_piece<MT>(block_sum<16>(units, scan));
+  uint32_t before = 0, before_cut = 0;
+  for (int b0 = 0; b0 < seqs; b0 += 1024) {
+    const int b = b0 + tid;
+    Work w{};
+    if (b < seqs) w = work_of<16 * MT>(a, kv_seq(a.seqs, b));
+    const Pieces p = pieces_of(w, per);
+    const uint32_t upto = before + block_scan<1024, uint32_t>(p.pieces, scan32);
+    const bool in = upto <= limit;
+    const uint32_t upto_cut = before_cut + block_scan<1024, uint32_t>(in ? p.cut : 0, scan32);
+    if (b < seqs) gst<int32_t>(a.upto + b, (int32_t)(in ? upto : limit + 1)), gst<int32_t>(a.upto_cut + b, (int32_t)upto_cut);
+    if (in) atomicMax(&most, upto);
+    if (tid == 1023) carry[0] = in ? upto : limit + 1, carry[1] = upto_cut;
+    __syncthreads();
+    before = carry[0], before_cut = carry[1];
+    __syncthreads();
+  }
+  if (tid == 0) gst<int32_t>(a.counts, (int32_t)per), gst<int32_t>(a.counts + 1, (int32_t)most), gst<int32_t>(a.cut_count, (int32_t)(before_cut >> 16));
+}
+
 // FAST: heads of 64 NC channels and pages of 64 keys, which are the constants of the
 // addresses then, and a page is one for the whole wave (16, 32 and 64 rows on 4000 keys, 32
 // times, 66, 82 and 104 us; without it 78, 102 and 152).
@@ -152,7 +201,6 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT>)) void k_kv_attend(K
   __shared__ int64_t scan[kWaves];
   __shared__ uint32_t scan32[kWaves];
   __shared__ int found[kWaves][4];
-  __shared__ uint32_t carry[2];
   __shared__ f32x4 aside[kWaves * MT * NT * 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
@@ -173,57 +221,46 @@ __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT>)) void k_kv_attend(K
     }
   }
 
-  // all work, and the sequences that the four waves' pieces are of
-  const bool one = a.seqs.seqs <= 64 * kWaves;  // a round of the search sees all of them
-  Work mine{};
-  int64_t total = 0;
-  for (int b0 = 0; b0 < a.seqs.seqs; b0 += 64 * kWaves) {
-    if (b0 + tid < a.seqs.seqs) mine = work_of<ROWS>(a, kv_seq(a.seqs, b0 + tid));
-    else mine = Work{};
-    total += block_sum<kWaves>((int64_t)mine.lines * mine.count, scan);
-  }
-  total = uniform(total);
-  if (total == 0) {  // all sequences are k_kv_prefill's
-    if (blockIdx.x == 0 && tid == 0) gst<int32_t>(a.cut_count, 0);
-    return;
-  }
-  // units of a piece, where a line has less than 2^25
-  const int64_t share = (total + kParts - 1) / kParts;
-  const uint32_t per = share < kLeast<MT> ? kLeast<MT> : share < 1 << 25 ? (uint32_t)share : 1u << 25;
-  // Offsets that go back would make rows of several sequences', and more pieces than there are
-  // waves: sequences whose pieces have not all one are left out.
-  const uint32_t limit = gridDim.x * kWaves;
-  if (tid < kWaves) found[tid][0] = -1;
-  __syncthreads();
-  // pieces so far; and those of items that are cut, with (times 2^16) these items: at most 2 kParts of each
-  uint32_t before = 0, before_cut = 0;
-  for (int b0 = 0; b0 < a.seqs.seqs; b0 += 64 * kWaves) {
-    if (!one) {
-      if (b0 + tid < a.seqs.seqs) mine = work_of<ROWS>(a, kv_seq(a.seqs, b0 + tid));
-      else mine = Work{};
+  // the sequences that the four waves' pieces are of
+  int b, place, slot;
+  uint32_t per;
+  if (a.counts != nullptr) {
+    const uint32_t at = blockIdx.x * kWaves + wave;
+    per = (uint32_t)sld(a.counts);
+    if (at >= (uint32_t)sld(a.counts + 1)) return;
+    b = kv_find(a.upto, a.seqs.seqs, at);
+    const uint32_t first = b > 0 ? (uint32_t)sld(a.upto_cut + b - 1) : 0;
+    place = (int)at - (b > 0 ? sld(a.upto + b - 1) : 0);
+    slot = (int)(first & 0xFFFF) + place;
+    if (lane == 0) found[wave][3] = (int)(first >> 16);
+  } else {
+    Work mine{};
+    if (tid < a.seqs.seqs) mine = work_of<ROWS>(a, kv_seq(a.seqs, tid));
+    const int64_t total = uniform(block_sum<kWaves>((int64_t)mine.lines * mine.count, scan));
+    if (total == 0) {  // all sequences are k_kv_prefill's
+      if (blockIdx.x == 0 && tid == 0) gst<int32_t>(a.cut_count, 0);
+      return;
     }
-    const uint32_t cuts = ((uint32_t)mine.count + per - 1) / per, pieces = cuts * (uint32_t)mine.lines;
-    const uint32_t upto = before + block_scan<64 * kWaves, uint32_t>(pieces, scan32);
-    const bool in = upto <= limit;
-    const uint32_t cut = cuts > 1 && in ? pieces + ((uint32_t)mine.lines << 16) : 0;
-    const uint32_t upto_cut = before_cut + block_scan<64 * kWaves, uint32_t>(cut, scan32);
+    per = units_of_piece<MT>(total);
+    if (tid < kWaves) found[tid][0] = -1;
+    __syncthreads();
+    const Pieces p = pieces_of(mine, per);
+    const uint32_t upto = block_scan<64 * kWaves, uint32_t>(p.pieces, scan32);
+    const bool in = upto <= gridDim.x * kWaves;
+    const uint32_t cut = in ? p.cut : 0, upto_cut = block_scan<64 * kWaves, uint32_t>(cut, scan32);
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const uint32_t at = blockIdx.x * kWaves + w - (upto - pieces);  // wraps below 0
-      if (at < pieces && in) {
+      const uint32_t at = blockIdx.x * kWaves + w - (upto - p.pieces);  // wraps below 0
+      if (at < p.pieces && in) {
         const uint32_t first = upto_cut - cut;
-        found[w][0] = b0 + tid, found[w][1] = (int)at, found[w][2] = (int)((first & 0xFFFF) + at), found[w][3] = (int)(first >> 16);
+        found[w][0] = tid, found[w][1] = (int)at, found[w][2] = (int)((first & 0xFFFF) + at), found[w][3] = (int)(first >> 16);
       }
     }
-    if (tid == 64 * kWaves - 1) carry[0] = upto, carry[1] = upto_cut;
+    if (blockIdx.x == 0 && tid == 64 * kWaves - 1) gst<int32_t>(a.cut_count, (int32_t)(upto_cut >> 16));
     __syncthreads();
-    before = carry[0], before_cut = carry[1];
-    if (before > limit || (blockIdx.x > 0 && before > blockIdx.x * kWaves + kWaves - 1)) break;
+    b = uniform(found[wave][0]), place = uniform(found[wave][1]), slot = uniform(found[wave][2]);
+    if (b < 0) return;
   }
-  if (blockIdx.x == 0 && tid == 0) gst<int32_t>(a.cut_count, (int32_t)(before_cut >> 16));
-  __syncthreads();
-  const int b = uniform(found[wave][0]), place = uniform(found[wave][1]), slot = uniform(found[wave][2]);
-  if (b < 0) return;
   const KvSeq q = kv_seq_uniform(a.seqs, b);
   const Work work = work_of<ROWS>(a, q);
   const int cuts = (int)(((uint32_t)work.count + per - 1) / per);
@@ -604,6 +641,7 @@ void launch(KvAttendArgs a, hipStream_t stream) {
   // 16, 61 and 182 us; 25, 83 and 204 with one for all channels; 8 channels 17, 58 and 180)
   const int64_t joins = items < 2048 ? items : 2048;
   const int split = items <= 256 && a.cache.dim % 32 == 0 ? a.cache.dim / 32 : 1;
+  if (a.counts != nullptr) hipLaunchKernelGGL((k_kv_count<MT>), dim3(1), dim3(1024), 0, stream, a, (uint32_t)groups * kWaves);
   if (a.cache.dim == 64 * NC && a.seqs.shift == 6)
     hipLaunchKernelGGL((k_kv_attend<DT, NC, MT, true>), dim3((unsigned)groups), dim3(64 * kWaves), 0, stream, a);
   else
@@ -626,13 +664,14 @@ void launch_of(const KvAttendArgs& a, hipStream_t stream) {
   else launch_dim<DT, 1>(a, stream);
 }
 
+int64_t counts_bytes(int64_t seqs) { return (4 * seqs + 255) / 256 * 256; }
 int64_t few_workspace(int64_t dim) { return 256 + kPlaces * 32 + 4 * kPlaces * (dim <= 128 ? 32 : 16) * (2 + dim); }
 
 }  // namespace
 
 int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, bool one_each) {
   const int64_t group = heads / kv_heads;
-  int64_t need = few_workspace(dim);
+  int64_t need = few_workspace(dim) + (seqs > kOwnSearch ? 2 * counts_bytes(seqs) : 0);
   if (!all_few(all_rows(tokens, seqs, one_each, group), one_each, group, dim)) {
     const int64_t many = kv_prefill_workspace(kv_prefill_tiles(tokens, group, seqs), seqs, kv_heads, dim);
     if (many > need) need = many;
@@ -647,6 +686,12 @@ hipError_t launch_kv_attend(KvAttendArgs a, int dtype, void* workspace, hipStrea
   a.cut_count = static_cast<int32_t*>(workspace);
   a.heads_at = static_cast<uint8_t*>(workspace) + 256;
   a.sums = reinterpret_cast<float*>(a.heads_at + kPlaces * 32);
+  a.counts = a.upto = a.upto_cut = nullptr;
+  if (a.seqs.seqs > kOwnSearch) {
+    a.counts = a.cut_count + 1;
+    a.upto = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + few_workspace(a.cache.dim));
+    a.upto_cut = a.upto + counts_bytes(a.seqs.seqs) / 4;
+  }
   if (dtype == kBF16) launch_of<kBF16>(a, stream);
   else launch_of<kF16>(a, stream);
   if (!all) {

@@ -67,7 +67,8 @@ SIGNATURES = {
     "lrq_route_grad": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _CI, _CI, _CI, ctypes.c_float, _VP, _VP]),
     "lrq_fp8_experts_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "lrq_fp8_experts": (_CI, [_VP, _CI, _I64, _I64, _I64, _VP, _VP, _I64, _VP, _VP, _VP, _VP, _I64, _I64, _VP, _VP, _I64, _VP]),
-    "lrq_kv_append": (_CI, [_VP, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _CI, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _VP]),
+    "lrq_kv_append_workspace": (_I64, [_I64, _CI]),
+    "lrq_kv_append": (_CI, [_VP, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _CI, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _VP, _I64, _VP]),
     "lrq_kv_attend_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64, _CI]),
     "lrq_kv_attend": (_CI, [_VP, _I64, _VP, _I64, _I64, _CI, _I64, _I64, _VP, _I64, _I64, _VP, _VP, _I64, ctypes.c_float, _I64, _CI,
                             _VP, _VP, _VP, _I64, _VP]),

@@ -35,6 +35,11 @@ _STRIDE_MAX = 1 << 40
 
 
 @functools.lru_cache(maxsize=4096)
+def _append_workspace(seqs: int) -> int:
+    return _lib.lib().lrq_kv_append_workspace(seqs, False)
+
+
+@functools.lru_cache(maxsize=4096)
 def _attend_workspace(tokens: int, heads: int, kv_heads: int, dim: int, seqs: int, one_each: bool) -> int:
     return _lib.lib().lrq_kv_attend_workspace(tokens, heads, kv_heads, dim, seqs, one_each)
 
@@ -191,10 +196,13 @@ class FP8KVCache:
         lengths = self._ints(what, "lengths", lengths, (rows,))
         offsets = self._offsets(what, offsets, rows, tokens)
         dev = self.device
+        need = 0 if offsets is None else _append_workspace(rows)
+        work = _dense((need,), torch.uint8, dev) if need else None
         with _on(dev):
             rc = _lib.lib().lrq_kv_append(self._ref, layer, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
                                           v.stride(1), _IN_DTYPES[k.dtype], tokens, table.data_ptr(), ld, width,
-                                          lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), rows, _stream(dev))
+                                          lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), rows,
+                                          None if work is None else work.data_ptr(), need, _stream(dev))
         if rc:
             _lib.check(rc, "lrq_kv_append")
 

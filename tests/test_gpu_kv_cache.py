@@ -127,6 +127,31 @@ def test_attend_of_many_sequences_and_long_ones():
     close(out[some], want, bound)
 
 
+@pytest.mark.parametrize("seqs", [256, 257, 1100, 4500])
+@pytest.mark.parametrize("most", [2, 90])  # 90: some by tiles of many rows
+def test_attend_finds_its_sequences(seqs, most):
+    """Around the number up to which work-groups look for their own, and far beyond it."""
+    page, kv, dim = 16, 1, 16
+    new = [(7 * i + i // 97) % (most + 1) if i % 50 == 0 else (i + i // 13) % 3 for i in range(seqs)]
+    prior = [(11 * i) % 40 + (900 if i % 333 == 5 else 0) for i in range(seqs)]
+    lengths, offsets, width = batch(new, prior, page)
+    pool = sum(R.pages_of(n, page) for n in lengths)
+    c = make(1, pool, kv, dim, page)
+    table = R.spread_table(lengths, page, width, pool, 4)
+    q = queries(offsets[-1] + 3, 4, dim, torch.float16)
+    out, lse = c.attend(0, q, ints(table), ints(lengths), ints(offsets), return_lse=True)
+    some = sorted({0, 1, 5, 50, 255, 256 % seqs, seqs // 2, seqs - 2, seqs - 1, *range(0, seqs, 61)})
+    some = [i for i in some if new[i] > 0]
+    at = [t for i in some for t in range(offsets[i], offsets[i + 1])]
+    few = [0]
+    for i in some:
+        few.append(few[-1] + new[i])
+    want, bound, wl = R.attend(c, 0, q[at], [table[i] for i in some], [lengths[i] for i in some], few, dim ** -0.5, 0)
+    close(out[at], want, bound)
+    assert bool((out[offsets[-1]:] == 0).all()) and not bool(out[: offsets[-1]].isnan().any())
+    assert bool((lse[: offsets[-1]] > -math.inf).all()) and bool((out[: offsets[-1]] != 0).any(-1).all())
+
+
 def test_attend_flat_and_peaked_probabilities():
     """All keys alike: p is 1 / n for 30000 keys; then one key 60 above all others."""
     page, dim, n = 64, 64, 30000
@@ -488,10 +513,11 @@ def test_append_strided_and_out_of_range():
     want.same(c)
 
 
-def test_append_of_many_sequences():
+@pytest.mark.parametrize("seqs", [256, 257, 900, 2500])
+def test_append_of_many_sequences(seqs):
     page, dim, kv = 16, 32, 1
-    new = [(5 * i) % 4 for i in range(900)]
-    lengths, offsets, width = batch(new, [(7 * i) % 30 for i in range(900)], page)
+    new = [(5 * i) % 4 + (100 if i % 300 == 7 else 0) for i in range(seqs)]
+    lengths, offsets, width = batch(new, [(7 * i) % 30 for i in range(seqs)], page)
     pool = sum(R.pages_of(n, page) for n in lengths)
     c = make(1, pool, kv, dim, page)
     table = R.spread_table(lengths, page, width, pool, 11)

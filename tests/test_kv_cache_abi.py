@@ -26,8 +26,9 @@ def cache(**kw):
 
 
 def append(c=None, layer=0, k=FAKE, kt=256, kh=128, v=FAKE, vt=256, vh=128, dt=0, tokens=5, table=FAKE, ld=4, width=4, lengths=FAKE,
-           offsets=FAKE, seqs=3):
-    return L().lrq_kv_append(cache() if c is None else c, layer, k, kt, kh, v, vt, vh, dt, tokens, table, ld, width, lengths, offsets, seqs, None)
+           offsets=FAKE, seqs=3, ws=None, wb=0):
+    return L().lrq_kv_append(cache() if c is None else c, layer, k, kt, kh, v, vt, vh, dt, tokens, table, ld, width, lengths, offsets, seqs, ws, wb,
+                             None)
 
 
 def attend(c=None, layer=0, q=FAKE, qt=1024, qh=128, dt=0, tokens=5, heads=8, table=FAKE, ld=4, width=4, lengths=FAKE, offsets=FAKE,
@@ -52,6 +53,10 @@ def test_append():
         assert append(**bad) == _lib.ERR_ARG, bad
     for bad in ({"k": ODD}, {"v": ODD}, {"table": ODD}, {"lengths": ODD}, {"offsets": ODD}, {"dt": 2, "k": ctypes.c_void_p(0x10002)}):
         assert append(**bad) == _lib.ERR_ALIGN, bad
+    need = L().lrq_kv_append_workspace(257, 0)
+    assert need > 0 and append(seqs=257, ws=FAKE, wb=need - 1) == _lib.ERR_CAPACITY and append(seqs=257) == _lib.ERR_CAPACITY
+    assert append(seqs=257, ws=OFF4, wb=need) == _lib.ERR_ALIGN
+    assert L().lrq_kv_append_workspace(256, 0) == 0 and L().lrq_kv_append_workspace(1000, 1) == 0 and L().lrq_kv_append_workspace(-1, 0) == 0
     for bad in BAD_CACHES:
         assert append(c=cache(**bad)) == _lib.ERR_ARG, bad
     for bad in FAR_CACHES:
