@@ -606,15 +606,17 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttendArgs a) {
 }
 
 // Sequences of more rows than kMostRows are k_kv_prefill's (32 of 4000 keys: with 64 rows each
-// 103 us here and 110 there, with 96 rows 126 and 114), of more than half as many where tiles
-// are of 16 rows and not of 32 (192 channels, 64 rows: 216 and 188).  But not in a call whose
+// 103 us here and 110 there, with 96 rows 126 and 114; 64 channels, pages of 32: 75 and 87), of more
+// than half as many where this kernel holds its registers worst: more than 64 channels, without
+// FAST (128 in pages of 16, 48 rows 156 and 124 us; 80 channels 122 and 101) or in tiles of 16 rows
+// and not of 32 (192 channels, 64 rows: 216 and 188).  But not in a call whose
 // rows are kAllRows together at most: three launches less (one of 2000 keys: 1024 rows 50.6
 // and 54.4 us, 4096 rows 124 and 102).
 constexpr int kMostRows = 64, kAllRows = 1024;
-int most_rows(int64_t dim) { return dim <= 128 ? kMostRows : kMostRows / 2; }
+int most_rows(int64_t dim, int shift) { return dim <= 64 || (dim == 128 && shift == 6) ? kMostRows : kMostRows / 2; }
 // Rows of a call; one_each: one token a sequence.
 int64_t all_rows(int64_t tokens, int64_t seqs, bool one_each, int64_t group) { return (one_each && seqs < tokens ? seqs : tokens) * group; }
-bool all_few(int64_t rows, bool one_each, int64_t group, int64_t dim) { return one_each ? group <= most_rows(dim) : rows <= kAllRows; }
+bool all_few(int64_t rows, bool one_each, int64_t group, int most) { return one_each ? group <= most : rows <= kAllRows; }
 
 // Items of a call at most, and its pieces: an item of n units is cut into less than n / per + 1.
 int64_t most_items(int64_t rows, int64_t heads, int64_t seqs, bool all) {
@@ -672,7 +674,7 @@ int64_t few_workspace(int64_t dim) { return 256 + kPlaces * 32 + 4 * kPlaces * (
 int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, bool one_each) {
   const int64_t group = heads / kv_heads;
   int64_t need = few_workspace(dim) + (seqs > kOwnSearch ? 2 * counts_bytes(seqs) : 0);
-  if (!all_few(all_rows(tokens, seqs, one_each, group), one_each, group, dim)) {
+  if (!all_few(all_rows(tokens, seqs, one_each, group), one_each, group, kMostRows / 2)) {  // whatever the pages
     const int64_t many = kv_prefill_workspace(kv_prefill_tiles(tokens, group, seqs), seqs, kv_heads, dim);
     if (many > need) need = many;
   }
@@ -681,8 +683,9 @@ int64_t kv_attend_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int
 
 hipError_t launch_kv_attend(KvAttendArgs a, int dtype, void* workspace, hipStream_t stream) {
   const bool one_each = a.seqs.offsets == nullptr;
-  const bool all = all_few(all_rows(a.seqs.tokens, a.seqs.seqs, one_each, a.group), one_each, a.group, a.cache.dim);
-  a.few = all ? INT32_MAX : most_rows(a.cache.dim);
+  const int most = most_rows(a.cache.dim, a.seqs.shift);
+  const bool all = all_few(all_rows(a.seqs.tokens, a.seqs.seqs, one_each, a.group), one_each, a.group, most);
+  a.few = all ? INT32_MAX : most;
   a.cut_count = static_cast<int32_t*>(workspace);
   a.heads_at = static_cast<uint8_t*>(workspace) + 256;
   a.sums = reinterpret_cast<float*>(a.heads_at + kPlaces * 32);

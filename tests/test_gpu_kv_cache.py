@@ -82,6 +82,10 @@ ATTEND = [
     (torch.float16, 8, 1, 64, 32, [128, 1, 200], [1000, 5, 0], 0),
     (torch.bfloat16, 8, 1, 128, 256, [140, 17], [2000, 3], 600),
     (torch.float16, 16, 1, 208, 64, [77], [130], 0),
+    # 40 query heads a KV head, one token each: few rows with one page, many with another
+    (torch.bfloat16, 40, 1, 128, 64, [1] * 30, [50 * i for i in range(30)], 0),
+    (torch.bfloat16, 40, 1, 128, 16, [1] * 30, [50 * i for i in range(30)], 0),
+    (torch.float16, 66, 1, 64, 128, [1] * 17, [50 * i for i in range(17)], 0),
     # heads of up to three and four times 64 channels, few rows and many, pages of more than a unit and of less
     (torch.bfloat16, 8, 2, 192, 64, [1, 3, 9], [700, 64, 0], 0),
     (torch.float16, 8, 2, 192, 128, [200, 1, 40], [700, 64, 0], 0),
