@@ -273,6 +273,8 @@ int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, 
  *   two, from 2^-48 to 2^48, that takes the largest finite magnitude to 448 at most; where
  *   tokens join a page it does not shrink, and where it grows, the codes there are rounded
  *   to it again.  Inf, NaN, and what a scale of 2^48 takes past 448 become NaN codes.
+ *   Tokens whose place has no page, or one that refs (may be null: not looked at) counts for
+ *   more than one row, are not written.
  *   `workspace`: lrq_kv_append_workspace bytes (one_each: no offsets), 256-byte aligned,
  *   overwritten; 0 for up to 256 sequences.
  * lrq_kv_attend: out [tokens, heads, dim] = softmax(scale q k^T) v for the same rows, each

@@ -892,7 +892,7 @@ int check_kv_cache(const char* what, const lrq_kv_cache* c) {
 lrq::KvCache kv_layer(const lrq_kv_cache& c, int64_t layer) {
   lrq::KvCache o{};
   o.k = static_cast<uint8_t*>(c.k) + layer * c.k_layer, o.v = static_cast<uint8_t*>(c.v) + layer * c.v_layer;
-  o.ks = c.k_scales + layer * c.ks_layer, o.vs = c.v_scales + layer * c.vs_layer;
+  o.ks = c.k_scales + layer * c.ks_layer, o.vs = c.v_scales + layer * c.vs_layer, o.refs = c.refs;
   o.k_page = c.k_page, o.v_page = c.v_page, o.ks_page = c.ks_page, o.vs_page = c.vs_page;
   o.pages = (int)c.pages, o.heads = (int)c.kv_heads, o.dim = (int)c.dim;
   return o;
@@ -962,6 +962,7 @@ int lrq_kv_append(const lrq_kv_cache* cache, int64_t layer, const void* k, int64
   if (!valid_dtype(dtype)) return fail(LRQ_ERR_ARG, "kv_append: bad dtype %d", dtype);
   if (seqs == 0 || width == 0) return 0;
   if (!k || !v) return fail(LRQ_ERR_ARG, "kv_append: null pointer");
+  if (!aligned(cache->refs, 4)) return fail(LRQ_ERR_ALIGN, "kv_append: counts of the pages' rows must be element-aligned");
   if (!aligned(k, (uintptr_t)esize(dtype)) || !aligned(v, (uintptr_t)esize(dtype)))
     return fail(LRQ_ERR_ALIGN, "kv_append: keys and values must be element-aligned");
   if (!strides_ok(k_token, k_head, cache->dim, tokens, cache->kv_heads) || !strides_ok(v_token, v_head, cache->dim, tokens, cache->kv_heads))

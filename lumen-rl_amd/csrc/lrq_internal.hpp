@@ -342,6 +342,7 @@ hipError_t launch_experts(ExpertArgs a, int dtype, int64_t tokens, void* workspa
 struct KvCache {  // one layer: K [pages, heads, page, dim], V [pages, heads, dim, page]
   uint8_t *k, *v;
   float *ks, *vs;  // [pages, heads]
+  const int32_t* refs;  // [pages]: rows that hold each, or null
   int64_t k_page, v_page, ks_page, vs_page;  // from page to page: bytes, and scales
   int pages, heads, dim;
 };

@@ -6,6 +6,10 @@
 // rounded to it again; where they are the page's first, its scale starts anew.  Infinities
 // and NaN become NaN codes and leave the scale alone.
 //
+// A page that more than one row holds is not written.  Its tokens are the other rows' as well, and
+// two of them that write to it would round its codes again side by side: a row that could not
+// have a page of its own (a full pool) is to lose its new tokens and no one's old ones.
+//
 // Bound by its bytes: a page and head of 64 tokens reads 32 KiB (bf16) and writes 16.  32 prompts
 // of 33 to 1500 tokens on 8 heads of 128 (154 MB) take 35 us, 4.4 TB/s (a copy: 4.7).  A page's
 // values are read once, into registers, where both passes (the maximum, the codes) find them.
@@ -131,6 +135,9 @@ __device__ __forceinline__ void recode_v(uint8_t* vc, int slots, int page, int d
   }
 }
 
+// How many rows hold a page, the same one in all lanes; it is not waited for before it is looked at.
+__device__ __forceinline__ int holders(const KvCache& c, int page) { return c.refs != nullptr ? sld(c.refs + page) : 0; }
+
 // ---------------------------------------------------------------------------
 // One new token a sequence: a wave for each token and head, K in its lower half, V in the
 // upper, eight channels a lane.  Its values do not wait for where they go.
@@ -158,8 +165,10 @@ __global__ __launch_bounds__(256) void k_kv_append_one(KvAppendArgs a) {
   float* const ks = a.cache.ks + (int64_t)page * a.cache.ks_page + h;
   float* const vs = a.cache.vs + (int64_t)page * a.cache.vs_page + h;
   const float was = is_v ? gld<float>(vs) : gld<float>(ks);
+  const int held = holders(a.cache, page);
   uint32_t m = group_max<32>(amax_word<DT>(amax_raw<DT>(x, 0)));
   if (__ballot(m >= kNotFinite<DT>) != 0) m = group_max<32>(amax_finite<DT>(x, 0));
+  if (held > 1) return;
   float scale = kv_scale(amax_f32<DT>(m));
   if (slot > 0) scale = fmaxf(scale, was);
   uint8_t* const kc = a.cache.k + (int64_t)page * a.cache.k_page + (int64_t)h * S * dim;
@@ -246,6 +255,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
   float* const ks = a.cache.ks + (int64_t)page * a.cache.ks_page + h;
   float* const vs = a.cache.vs + (int64_t)page * a.cache.vs_page + h;
   const float k_old = gld<float>(ks), v_old = gld<float>(vs);
+  const int held = holders(a.cache, page);
 
   // slabs of tokens whose values the threads hold: one, but for pages of more than kSlab values
   const int per = kSlab / dim, slabs = (n + per - 1) / per;
@@ -290,6 +300,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
   }
   float k_new = kv_scale(amax_f32<DT>(km)), v_new = kv_scale(amax_f32<DT>(vm));
   if (s0 > 0) k_new = fmaxf(k_new, k_old), v_new = fmaxf(v_new, v_old);
+  if (held > 1) return;  // the same in all threads
   // every thread has the old scales (the barrier above) before one writes the new
   if (tid == 0) gst<float>(ks, k_new), gst<float>(vs, v_new);
 

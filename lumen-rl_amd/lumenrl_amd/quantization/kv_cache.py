@@ -182,7 +182,8 @@ class FP8KVCache:
         largest finite magnitude to 448 at most.  Tokens that join a page never make its
         scale smaller; where they make it larger, the codes that are there are rounded to
         it again.  Infinities and NaN become NaN codes.  Tokens whose place has no page in
-        the table are not written.  No gradient: keys or values that want one are refused.
+        the table, or one that ``refs`` counts for more than one row, are not written: what
+        other rows see is not changed.  No gradient: keys or values that want one are refused.
         """
         what = "FP8KVCache.append"
         self._layer(what, layer)
