@@ -6,7 +6,8 @@ The layer's linears run on 128x128-tile FP8 weights (``fp8_matmul``, ``fp8_block
 keys and values live in an ``FP8KVCache``.  The prompt is appended and attended to once;
 ``fork`` gives its pages to every sample; then each step makes room for a token
 (``resize``, which copies the page that the prompt ends in for each sample that writes to
-it), appends and attends.  In the end one sample goes on alone: the others' pages are given
+it), appends and attends, with the lengths that ``resize`` has ready: 0 for a sample that
+there was no page for.  In the end one sample goes on alone: the others' pages are given
 back and ``compact`` moves what is left together.
 """
 
@@ -76,18 +77,18 @@ def main(prompt: int = 300, samples: int = 4, steps: int = 40, layers: int = 2) 
     lengths = torch.zeros(samples, dtype=torch.int32, device="cuda")
     wanted = lengths.clone()
     wanted[0] = prompt
-    table, lengths, _ = cache.resize(table, lengths, wanted)
+    table, lengths, _, ready = cache.resize(table, lengths, wanted, return_ready=True)
     offsets = torch.full((samples + 1,), prompt, dtype=torch.int32, device="cuda")
     offsets[0] = 0
-    first = run(x, table, lengths, offsets)
+    first = run(x, table, ready, offsets)
 
     # its samples
     table, lengths = cache.fork(table, lengths, torch.zeros_like(lengths))
     shared = int((cache.refs > 0).sum())
     outs = []
     for step in range(steps):
-        table, lengths, short = cache.resize(table, lengths, lengths + 1)
-        outs.append(run(inputs[step], table, lengths))
+        table, lengths, short, ready = cache.resize(table, lengths, lengths + 1, return_ready=True)
+        outs.append(run(inputs[step], table, ready))
     used = int((cache.refs > 0).sum())
 
     # the last one goes on alone, in pages moved together

@@ -296,7 +296,11 @@ int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, 
  *   grows from inside a page which others hold too gets a copy of it.  Where free
  *   pages run out (after what this call gives back), rows from there on that need any
  *   keep their length, and short_ (one int32) is how many were missing; so does a row
- *   that wants more than `width` pages.
+ *   that wants more than `width` pages (which short_ does not count).
+ * lrq_kv_resize_ready leaves one thing more, in ready [rows]: the new length of a row that has
+ *   what it wanted, 0 of one that was refused.  These are the lengths for the append and the
+ *   attention of the tokens that `wanted` counts in: a refused row's have no place, and with
+ *   its own length the row's last tokens would be taken for them.
  * lrq_kv_compact: the n pages in use become pages 0 .. n - 1: the k-th in use at or behind
  *   n moves to the k-th free one before n.  count (one int32) is n.
  */
@@ -324,6 +328,9 @@ int64_t lrq_kv_resize_workspace(int64_t rows, int64_t pages);
 int lrq_kv_resize(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
                   int64_t rows, const int32_t* wanted, int32_t* out_table, int32_t* out_lengths, int32_t* short_,
                   void* workspace, int64_t workspace_bytes, lrq_stream_t stream);
+int lrq_kv_resize_ready(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
+                        int64_t rows, const int32_t* wanted, int32_t* out_table, int32_t* out_lengths, int32_t* ready,
+                        int32_t* short_, void* workspace, int64_t workspace_bytes, lrq_stream_t stream);
 int64_t lrq_kv_compact_workspace(int64_t pages);
 int lrq_kv_compact(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, int64_t rows,
                    int32_t* out_table, int32_t* count, void* workspace, int64_t workspace_bytes, lrq_stream_t stream);

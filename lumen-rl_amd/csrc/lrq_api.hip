@@ -1031,14 +1031,26 @@ int64_t lrq_kv_resize_workspace(int64_t rows, int64_t pages) {
 int lrq_kv_resize(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
                   int64_t rows, const int32_t* wanted, int32_t* out_table, int32_t* out_lengths, int32_t* short_,
                   void* workspace, int64_t workspace_bytes, lrq_stream_t stream) {
+  return lrq_kv_resize_ready(cache, table, ld, width, lengths, rows, wanted, out_table, out_lengths, nullptr, short_, workspace,
+                             workspace_bytes, stream);
+}
+
+int lrq_kv_resize_ready(const lrq_kv_cache* cache, const int32_t* table, int64_t ld, int64_t width, const int32_t* lengths,
+                        int64_t rows, const int32_t* wanted, int32_t* out_table, int32_t* out_lengths, int32_t* ready,
+                        int32_t* short_, void* workspace, int64_t workspace_bytes, lrq_stream_t stream) {
   g_err.clear();
   lrq::KvTable t{};
   if (int rc = check_kv_tables("kv_resize", cache, table, ld, width, lengths, rows, out_table, &t)) return rc;
   if (!short_ || (rows > 0 && (!lengths || !wanted || !out_lengths))) return fail(LRQ_ERR_ARG, "kv_resize: null pointer");
   if (rows > 0 && out_lengths < lengths + rows && lengths < out_lengths + rows)
     return fail(LRQ_ERR_ARG, "kv_resize: the new lengths must not overlap the old ones");
+  for (const int32_t* other : {lengths, wanted, (const int32_t*)out_lengths})
+    if (ready && ready < other + rows && other < ready + rows)
+      return fail(LRQ_ERR_ARG, "kv_resize: the ready lengths must not overlap the old, the wanted or the new ones");
+  if (!aligned(ready, 4)) return fail(LRQ_ERR_ALIGN, "kv_resize: the ready lengths must be element-aligned");
   if (int rc = check_workspace("kv_resize", workspace, workspace_bytes, lrq::kv_resize_workspace(rows, cache->pages))) return rc;
-  return check_hip(lrq::launch_kv_resize(t, kv_pool(*cache), wanted, out_table, out_lengths, short_, workspace, (hipStream_t)stream),
+  return check_hip(lrq::launch_kv_resize(t, kv_pool(*cache), wanted, out_table, out_lengths, ready, short_, workspace,
+                                          (hipStream_t)stream),
                    "kernel launch");
 }
 

@@ -422,7 +422,7 @@ int64_t kv_compact_workspace(int64_t pages);
 hipError_t launch_kv_fork(const KvTable& t, const int32_t* parents, int32_t* refs, int pages, int32_t* out, int32_t* out_len,
                           hipStream_t stream);
 hipError_t launch_kv_resize(const KvTable& t, const KvPool& c, const int32_t* wanted, int32_t* out, int32_t* out_len,
-                            int32_t* out_short, void* workspace, hipStream_t stream);
+                            int32_t* out_ready, int32_t* out_short, void* workspace, hipStream_t stream);
 hipError_t launch_kv_compact(const KvTable& t, const KvPool& c, int32_t* out, int32_t* out_count, void* workspace,
                              hipStream_t stream);
 

@@ -121,9 +121,9 @@ __device__ __forceinline__ v4i counts4(const int32_t* refs, int64_t p, int pages
 }
 
 // Second, one work-group: how many pages each row takes, which are free, who gets any.
-//   begin[r]: the first of row r's places in the list of free pages, or -1: none.
+// out_ready (or null): the new length of a row that has what it wants, 0 of one that was refused.
 __global__ __launch_bounds__(1024) void k_kv_plan(KvTable t, const int32_t* wanted, const int32_t* refs, int pages, KvPlan plan,
-                                                  int32_t* out_len, int32_t* out_short) {
+                                                  int32_t* out_len, int32_t* out_ready, int32_t* out_short) {
   __shared__ int64_t scan64[16];
   __shared__ int scan[16];
   __shared__ int64_t carry;
@@ -180,7 +180,9 @@ __global__ __launch_bounds__(1024) void k_kv_plan(KvTable t, const int32_t* want
     const int64_t after = gld<int64_t>(plan.after + r);
     const int signed_need = gld<int32_t>(plan.need + r), need = signed_need < 0 ? -signed_need : signed_need;
     const bool granted = need == 0 || after <= found;
-    gst<int32_t>(out_len + r, (int32_t)(granted || c.want <= c.len ? c.want : c.len));
+    const int32_t now = (int32_t)(granted || c.want <= c.len ? c.want : c.len);
+    gst<int32_t>(out_len + r, now);
+    if (out_ready != nullptr) gst<int32_t>(out_ready + r, now == gld<int32_t>(wanted + r) ? now : 0);
     if (!granted) gst<int32_t>(plan.need + r, 0);
     if (granted && signed_need < 0) {
       const int at = atomicAdd(&pairs, 1);
@@ -327,7 +329,7 @@ int64_t kv_resize_workspace(int64_t rows, int64_t pages) {
 int64_t kv_compact_workspace(int64_t pages) { return pad256(8 * pages) + pad256(4 * pages) + 256; }
 
 hipError_t launch_kv_resize(const KvTable& t, const KvPool& c, const int32_t* wanted, int32_t* out, int32_t* out_len,
-                            int32_t* out_short, void* workspace, hipStream_t stream) {
+                            int32_t* out_ready, int32_t* out_short, void* workspace, hipStream_t stream) {
   uint8_t* w = static_cast<uint8_t*>(workspace);
   KvPlan plan{};
   plan.after = reinterpret_cast<int64_t*>(w), w += pad256(8 * (int64_t)t.rows);
@@ -337,7 +339,8 @@ hipError_t launch_kv_resize(const KvTable& t, const KvPool& c, const int32_t* wa
   plan.count = reinterpret_cast<int32_t*>(w);
   plan.capacity = c.pages;
   if (t.rows > 0) hipLaunchKernelGGL(k_kv_release, dim3((unsigned)t.rows), dim3(256), 0, stream, t, wanted, c.refs, c.pages, out);
-  hipLaunchKernelGGL(k_kv_plan, dim3(1), dim3(1024), 0, stream, t, wanted, c.refs, c.pages, plan, out_len, out_short);
+  hipLaunchKernelGGL(k_kv_plan, dim3(1), dim3(1024), 0, stream, t, wanted, c.refs, c.pages, plan, out_len, out_ready,
+                     out_short);
   hipLaunchKernelGGL(k_kv_take, dim3(kCopyGroups), dim3(256), 0, stream, t, c, plan, out);
   return hipGetLastError();
 }

@@ -75,6 +75,7 @@ SIGNATURES = {
     "lrq_kv_fork": (_CI, [_VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _VP]),
     "lrq_kv_resize_workspace": (_I64, [_I64, _I64]),
     "lrq_kv_resize": (_CI, [_VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _I64, _VP]),
+    "lrq_kv_resize_ready": (_CI, [_VP, _VP, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _VP]),
     "lrq_kv_compact_workspace": (_I64, [_I64]),
     "lrq_kv_compact": (_CI, [_VP, _VP, _I64, _I64, _I64, _VP, _VP, _VP, _I64, _VP]),
     "lrq_cast_e4m3": (_CI, [_VP, _CI, _I64, _VP, _VP]),

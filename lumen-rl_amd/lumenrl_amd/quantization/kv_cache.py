@@ -4,12 +4,15 @@
 caller keeps: ``table`` int32 [rows, width] with a row's page numbers in order and
 ``lengths`` int32 [rows].  A step of a rollout is
 
-    table, lengths, short = cache.resize(table, lengths, lengths + new)   # once
-    cache.append(layer, k, v, table, lengths, offsets)                    # in each layer
-    out = cache.attend(layer, q, table, lengths, offsets)
+    table, lengths, short, ready = cache.resize(table, lengths, lengths + new, return_ready=True)   # once
+    cache.append(layer, k, v, table, ready, offsets)                                                # in each layer
+    out = cache.attend(layer, q, table, ready, offsets)
 
-and ``fork`` makes samples of a prompt share its pages, ``resize`` to 0 ends a sequence,
-``compact`` moves what is left together.  Everything runs on the current stream of the
+``ready`` is 0 for a row that there was no room for: its new tokens are written nowhere, see
+nothing and get 0, and ``lengths`` still says what it has.  (With ``lengths`` in its place
+the row's last tokens would be taken for the new ones, and overwritten.)  ``fork`` makes
+samples of a prompt share its pages, ``resize`` to 0 ends a sequence, ``compact`` moves what
+is left together.  Everything runs on the current stream of the
 cache's device, reads lengths and tables there, and returns without synchronizing, so a
 step can be captured into a graph.  Calls that write a page are the caller's to keep in order
 with others on that page, ``fork``, ``resize`` and ``compact`` with each other.  What tables,
@@ -176,8 +179,8 @@ class FP8KVCache:
         """Write new tokens' keys and values, ``k`` and ``v`` [tokens, kv_heads, dim] (bf16, fp16 or fp32).
 
         Rows ``offsets[b]`` .. ``offsets[b + 1] - 1`` (int32 [rows + 1]) are the last
-        tokens of sequence b, whose ``lengths[b]`` counts them in already; without
-        ``offsets`` each sequence has one, and rows behind the last belong to none.  A
+        tokens of sequence b, whose ``lengths[b]`` counts them in already (``resize``'s ``ready``,
+        where rows may have been refused); without ``offsets`` each sequence has one, and rows behind the last belong to none.  A
         page's scale is the least power of two, from 2^-48 to 2^48, that takes the
         largest finite magnitude to 448 at most.  Tokens that join a page never make its
         scale smaller; where they make it larger, the codes that are there are rounded to
@@ -286,16 +289,22 @@ class FP8KVCache:
             _lib.check(rc, "lrq_kv_fork")
         return out, out_lengths
 
-    def resize(self, table: Tensor, lengths: Tensor, wanted: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    def resize(self, table: Tensor, lengths: Tensor, wanted: Tensor, *, return_ready: bool = False) -> tuple[Tensor, ...]:
         """Pages for ``wanted`` tokens (int32 [rows]) in each row: (new table, new lengths, short).
 
         A row that shrinks gives back the pages behind its new end (all of them for 0).
         Rows that grow take the lowest free pages, in the rows' order; one that grows from
-        inside a page which other rows hold too gets a copy of that page, in every layer.
+        inside a page which other rows hold too gets a copy of that page, in every layer (where
+        all of its rows do, the last as well; the page itself is free after the call).
         Where free pages run out, counting what this call gives back, rows from there on that
         need any keep their length, and ``short`` (int32, no dimension) says how many pages
-        were missing; a row that wants more than the table is wide keeps its length as well.
-        Entries behind a row's pages are -1.
+        were missing; a row that wants more than the table is wide keeps its length as well, and
+        counts nothing there.  Entries behind a row's pages are -1.
+
+        ``return_ready`` adds the lengths for this step's ``append`` and ``attend`` (int32
+        [rows]): the new length of a row that has what it wanted, 0 of one that was refused.
+        A row that gives tokens back and takes new ones in their place, in a page that others
+        hold, is resized to what it keeps first.
         """
         what = "FP8KVCache.resize"
         table, rows, width, ld = self._table(what, table)
@@ -304,14 +313,16 @@ class FP8KVCache:
         dev = self.device
         out, out_lengths = _dense((rows, width), torch.int32, dev), _dense((rows,), torch.int32, dev)
         short = _dense((), torch.int32, dev)
+        ready = _dense((rows,), torch.int32, dev) if return_ready else None
         need = _resize_workspace(rows, self.pages)
         work = _dense((need,), torch.uint8, dev)
         with _on(dev):
-            rc = _lib.lib().lrq_kv_resize(self._ref, table.data_ptr(), ld, width, lengths.data_ptr(), rows, wanted.data_ptr(),
-                                          out.data_ptr(), out_lengths.data_ptr(), short.data_ptr(), work.data_ptr(), need, _stream(dev))
+            rc = _lib.lib().lrq_kv_resize_ready(self._ref, table.data_ptr(), ld, width, lengths.data_ptr(), rows, wanted.data_ptr(),
+                                                out.data_ptr(), out_lengths.data_ptr(), None if ready is None else ready.data_ptr(),
+                                                short.data_ptr(), work.data_ptr(), need, _stream(dev))
         if rc:
-            _lib.check(rc, "lrq_kv_resize")
-        return out, out_lengths, short
+            _lib.check(rc, "lrq_kv_resize_ready")
+        return (out, out_lengths, short) if ready is None else (out, out_lengths, short, ready)
 
     def compact(self, table: Tensor) -> tuple[Tensor, Tensor]:
         """Move the pages in use together: (new table, their number n as an int32 without dimensions).
