@@ -71,6 +71,13 @@ def _steps(name: str, x: Tensor, inner: int) -> tuple[int, int]:
     return x.stride(0), x.stride(1)
 
 
+def _wants_derivative(*tensors: Tensor) -> bool:
+    """Whether one of them is to be differentiated, backward or forward."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        return True
+    return torch.is_grad_enabled() and any(x.requires_grad for x in tensors)
+
+
 class FP8KVCache:
     """Pages of keys and values in e4m3, with one power-of-two scale per page and KV head for each.
 
@@ -186,15 +193,16 @@ class FP8KVCache:
         scale smaller; where they make it larger, the codes that are there are rounded to
         it again.  Infinities and NaN become NaN codes.  Tokens whose place has no page in
         the table, or one that ``refs`` counts for more than one row, are not written: what
-        other rows see is not changed.  No gradient: keys or values that want one are refused.
+        other rows see is not changed.  No gradient: keys or values that want one, backward
+        or forward, are refused.
         """
         what = "FP8KVCache.append"
         self._layer(what, layer)
         k, v = self._vectors(what, "k", k, self.kv_heads), self._vectors(what, "v", v, self.kv_heads)
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError(f"{what}: k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} do not fit")
-        if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
-            raise RuntimeError(f"{what} has no gradient; pass detached keys and values")
+        if _wants_derivative(k, v):
+            raise RuntimeError(f"{what} has no gradient, backward or forward; pass detached keys and values")
         tokens = k.shape[0]
         table, rows, width, ld = self._table(what, table)
         lengths = self._ints(what, "lengths", lengths, (rows,))
@@ -223,7 +231,7 @@ class FP8KVCache:
         (dense, of q's shape and type, q itself or apart from it) they stay as they are.
         ``return_lse`` adds the scores' log-sum-exp,
         float32 [tokens, heads] (-inf where nothing is seen).  No gradient: a backward
-        pass through the result raises.
+        pass through the result raises, and so does a ``q`` with a tangent.
         """
         what = "FP8KVCache.attend"
         q = self._vectors(what, "q", q, None)
@@ -242,9 +250,9 @@ class FP8KVCache:
                                 or not out.is_contiguous() or out.data_ptr() % 8):
             raise ValueError(f"{what}: out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {self.device}, 8-byte aligned")
         args = (layer, q, table, ld, lengths, offsets, self.dim ** -0.5 if scale is None else float(scale), window or 0, out, return_lse)
-        if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (q.requires_grad or out is not None and out.requires_grad):
+        if _wants_derivative(q) if out is None else _wants_derivative(q, out):
             if out is not None:
-                raise RuntimeError(f"{what} has no gradient; pass no out, or a detached q")
+                raise RuntimeError(f"{what} has no gradient, backward or forward; pass no out, or a detached q")
             return NoGradient.apply(what, self._attend, *args)
         return self._attend(*args)
 
