@@ -27,7 +27,7 @@ import functools
 from typing import Optional
 
 import torch
-from torch import Tensor
+from torch import Tensor, UntypedStorage
 from torch.autograd import forward_ad
 
 from lumenrl_amd import _lib
@@ -71,6 +71,11 @@ def _steps(name: str, x: Tensor, inner: int) -> tuple[int, int]:
     return x.stride(0), x.stride(1)
 
 
+def _places(parts: tuple) -> list:
+    """Where tensors are, and how long the memory is that they are in."""
+    return [*map(Tensor.data_ptr, parts), *map(UntypedStorage.nbytes, map(Tensor.untyped_storage, parts))]
+
+
 def _wants_derivative(*tensors: Tensor) -> bool:
     """Whether one of them is to be differentiated, backward or forward."""
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in tensors):
@@ -86,10 +91,26 @@ class FP8KVCache:
     kv_heads] float32, ``refs`` [pages] int32: how many rows of the caller's table hold
     each page; it is free where none does.  ``page`` is 16, 32, 64, 128 or 256, ``dim`` a multiple
     of 16 up to 256.  The tensors are kept and written in place; layers and pages may be
-    views of larger ones, what a page holds is dense.
+    views of larger ones, what a page holds is dense.  Their memory may be freed and put
+    back between calls (``untyped_storage().resize_``, ``.data =``), shapes and strides staying as
+    they are: each call looks where the tensors are, and raises where one has no memory, or too
+    little; a captured graph keeps the places of its capture.
     """
 
     def __init__(self, k: Tensor, v: Tensor, k_scales: Tensor, v_scales: Tensor, refs: Tensor) -> None:
+        self._parts = (k, v, k_scales, v_scales, refs)
+        self._describe()
+
+    k = property(lambda self: self._parts[0])
+    v = property(lambda self: self._parts[1])
+    k_scales = property(lambda self: self._parts[2])
+    v_scales = property(lambda self: self._parts[3])
+    refs = property(lambda self: self._parts[4])
+
+    def _describe(self) -> None:
+        """Checks the tensors, and notes where they are for the kernels."""
+        k, v, k_scales, v_scales, refs = self._parts
+        self._where = None  # until all is well
         parts = {"k": (k, torch.float8_e4m3fn), "v": (v, torch.float8_e4m3fn), "k_scales": (k_scales, torch.float32),
                  "v_scales": (v_scales, torch.float32), "refs": (refs, torch.int32)}
         for name, (x, dtype) in parts.items():
@@ -113,18 +134,27 @@ class FP8KVCache:
         if not 1 <= self.kv_heads <= 256 or not 1 <= self.pages <= 1 << 28 or self.layers > 65536:
             raise ValueError(f"FP8KVCache: {self.layers} layers (at most 65536), {self.pages} pages (1 to 2^28), {self.kv_heads} KV heads "
                              "(1 to 256)")
+        for name, (x, _) in parts.items():
+            last = x.storage_offset() + sum((n - 1) * step for n, step in zip(x.shape, x.stride()))
+            if x.numel() and (last + 1) * x.element_size() > x.untyped_storage().nbytes():
+                raise RuntimeError(f"FP8KVCache: the memory of {name} has been freed, or is too small for {tuple(x.shape)}")
         if k.numel() and (k.data_ptr() % 16 or v.data_ptr() % 16):
             raise ValueError("FP8KVCache: k and v must be 16-byte aligned")
         (kl, kp), (vl, vp) = _steps("k", k, 3), _steps("v", v, 3)
         (ksl, ksp), (vsl, vsp) = _steps("k_scales", k_scales, 1), _steps("v_scales", v_scales, 1)
         if any(s % 16 for s in (kl, kp, vl, vp)):
             raise ValueError(f"FP8KVCache: strides of layers and pages must be multiples of 16, got {k.stride()} and {v.stride()}")
-        self.k, self.v, self.k_scales, self.v_scales, self.refs = k, v, k_scales, v_scales, refs
         self.device = k.device
         self._index = k.get_device()
         self._desc = _lib.LrqKvCache(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), refs.data_ptr(),
                                      self.layers, self.pages, self.kv_heads, self.page, self.dim, kl, vl, ksl, vsl, kp, vp, ksp, vsp)
         self._ref = ctypes.byref(self._desc)
+        self._where = _places(self._parts)
+
+    def _look(self) -> None:
+        """First in every call: a caller may have moved the tensors' memory since the last one, or freed it (0.65 us of a call's 7)."""
+        if _places(self._parts) != self._where:
+            self._describe()
 
     @classmethod
     def empty(cls, layers: int, pages: int, kv_heads: int, dim: int, *, page: int = 64,
@@ -197,6 +227,7 @@ class FP8KVCache:
         or forward, are refused.
         """
         what = "FP8KVCache.append"
+        self._look()
         self._layer(what, layer)
         k, v = self._vectors(what, "k", k, self.kv_heads), self._vectors(what, "v", v, self.kv_heads)
         if k.shape != v.shape or k.dtype != v.dtype:
@@ -234,6 +265,7 @@ class FP8KVCache:
         pass through the result raises, and so does a ``q`` with a tangent.
         """
         what = "FP8KVCache.attend"
+        self._look()
         q = self._vectors(what, "q", q, None)
         if q.dtype is torch.float32:
             raise TypeError(f"{what}: q must be bf16 or fp16")
@@ -285,6 +317,7 @@ class FP8KVCache:
         a row grow: resize before appending.
         """
         what = "FP8KVCache.fork"
+        self._look()
         table, rows, width, ld = self._table(what, table)
         lengths = self._ints(what, "lengths", lengths, (rows,))
         parents = self._ints(what, "parents", parents, (rows,))
@@ -315,6 +348,7 @@ class FP8KVCache:
         hold, is resized to what it keeps first.
         """
         what = "FP8KVCache.resize"
+        self._look()
         table, rows, width, ld = self._table(what, table)
         lengths = self._ints(what, "lengths", lengths, (rows,))
         wanted = self._ints(what, "wanted", wanted, (rows,))
@@ -339,6 +373,7 @@ class FP8KVCache:
         in every layer, to the k-th free one before n; ``refs`` follows.
         """
         what = "FP8KVCache.compact"
+        self._look()
         table, rows, width, ld = self._table(what, table)
         dev = self.device
         out, count = _dense((rows, width), torch.int32, dev), _dense((), torch.int32, dev)

@@ -6,6 +6,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import kv_rules as R
 from test_gpu_kv_cache import ints, make, queries
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +42,54 @@ def test_tangents_are_refused_not_lost():
         torch.func.jvp(lambda x: c.append(0, x, x, table, lengths) or x, (k,), (torch.ones_like(k),))
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: c.attend(0, x, table, lengths), (q,), (torch.ones_like(q),))
+
+
+def test_memory_that_is_freed_and_put_back():
+    c = make(1, 6, 2, 64, 16)
+    table, lengths, wanted = ints([[0, 1, -1], [3, -1, -1]]), ints([20, 7]), ints([33, 8])
+    c.refs.copy_(ints([1, 1, 0, 1, 0, 0]))
+    k, q = queries(2, 2, 64, torch.bfloat16), queries(2, 4, 64, torch.bfloat16)
+
+    def calls():
+        return [lambda: c.append(0, k, k, table, lengths), lambda: c.attend(0, q, table, lengths), lambda: c.fork(table, lengths, lengths),
+                lambda: c.resize(table, lengths, wanted), lambda: c.compact(table)]
+
+    want = c.attend(0, q, table, lengths)
+    for name in ("k", "v", "k_scales", "v_scales", "refs"):
+        x = getattr(c, name)
+        saved, size = x.view(torch.uint8).clone(), x.untyped_storage().nbytes()
+        for left in (0, size // 2):
+            x.untyped_storage().resize_(left)
+            for call in calls():
+                with pytest.raises(RuntimeError, match=f"memory of {name} has been freed"):
+                    call()
+        held = torch.empty(size, dtype=torch.uint8, device=x.device)  # what was freed is someone else's now
+        x.untyped_storage().resize_(size)
+        x.view(torch.uint8).copy_(saved)
+        assert torch.equal(c.attend(0, q, table, lengths), want)
+        # and memory of another tensor
+        x.data = saved.clone().view(x.dtype)
+        assert torch.equal(c.attend(0, q, table, lengths), want)
+        assert torch.equal(saved, getattr(c, name).view(torch.uint8))
+        del held
+    # what is written goes where the tensors are
+    old = c.k.data
+    c.k.data = c.k.view(torch.uint8).clone().view(c.k.dtype)
+    rules = R.Cache(c)
+    c.append(0, k, k, table, lengths)
+    rules.append(0, k, k, table.tolist(), lengths.tolist(), None)
+    rules.same(c)
+    assert not torch.equal(old.view(torch.uint8), c.k.view(torch.uint8))
+    c.refs.data = ints([0, 1, 0, 1, 0, 0])
+    t, n, short = c.resize(table, lengths, wanted)
+    assert t.tolist() == [[0, 1, 0], [3, -1, -1]] and c.refs.tolist() == [1, 1, 0, 1, 0, 0]
+    # tensors that do not fit any more are refused as they would be at first, until they do
+    good = c.v.data
+    c.v.data = good[:, :5].clone()
+    for _ in range(2):
+        with pytest.raises(ValueError, match="v must be"):
+            c.attend(0, q, table, lengths)
+    c.v.data = good
+    c.attend(0, q, table, lengths)
+    with pytest.raises(AttributeError):
+        c.k = good
