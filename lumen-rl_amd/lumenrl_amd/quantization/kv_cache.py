@@ -32,7 +32,7 @@ from torch.autograd import forward_ad
 
 from lumenrl_amd import _lib
 from lumenrl_amd.quantization.fp8_product import NoGradient
-from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _dense, _on, _stream, require_device
+from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _current_device, _dense, _on, _stream, require_device
 
 _STRIDE_MAX = 1 << 40
 
@@ -76,11 +76,11 @@ def _places(parts: tuple) -> list:
     return [*map(Tensor.data_ptr, parts), *map(UntypedStorage.nbytes, map(Tensor.untyped_storage, parts))]
 
 
-def _wants_derivative(*tensors: Tensor) -> bool:
+def _wants_derivative(x: Tensor, y: Tensor) -> bool:
     """Whether one of them is to be differentiated, backward or forward."""
-    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, y)):
         return True
-    return torch.is_grad_enabled() and any(x.requires_grad for x in tensors)
+    return (x.requires_grad or y.requires_grad) and torch.is_grad_enabled()
 
 
 class FP8KVCache:
@@ -202,7 +202,8 @@ class FP8KVCache:
 
     def _vectors(self, what: str, name: str, x: Tensor, heads: Optional[int]) -> Tensor:
         """``x`` [tokens, heads, dim] with channels of unit stride."""
-        _check_input(x, what)
+        if not isinstance(x, Tensor) or x.get_device() != self._index or x.dtype not in _IN_DTYPES:
+            _check_input(x, what)
         shape = x.shape
         if len(shape) != 3 or shape[2] != self.dim or (heads is not None and shape[1] != heads) or x.get_device() != self._index:
             raise ValueError(f"{what}: {name} must be [tokens, {'heads' if heads is None else heads}, {self.dim}] on {self.device}, got "
@@ -235,17 +236,21 @@ class FP8KVCache:
         if _wants_derivative(k, v):
             raise RuntimeError(f"{what} has no gradient, backward or forward; pass detached keys and values")
         tokens = k.shape[0]
+        (k_token, k_head, _), (v_token, v_head, _) = k.stride(), v.stride()
         table, rows, width, ld = self._table(what, table)
         lengths = self._ints(what, "lengths", lengths, (rows,))
         offsets = self._offsets(what, offsets, rows, tokens)
         dev = self.device
         need = 0 if offsets is None else _append_workspace(rows)
         work = _dense((need,), torch.uint8, dev) if need else None
-        with _on(dev):
-            rc = _lib.lib().lrq_kv_append(self._ref, layer, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                          v.stride(1), _IN_DTYPES[k.dtype], tokens, table.data_ptr(), ld, width,
-                                          lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), rows,
-                                          None if work is None else work.data_ptr(), need, _stream(dev))
+        args = (self._ref, layer, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, _IN_DTYPES[k.dtype], tokens,
+                table.data_ptr(), ld, width, lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), rows,
+                None if work is None else work.data_ptr(), need, _stream(dev))
+        if self._index == _current_device():  # without a context, 0.2 us
+            rc = _lib.lib().lrq_kv_append(*args)
+        else:
+            with _on(dev):
+                rc = _lib.lib().lrq_kv_append(*args)
         if rc:
             _lib.check(rc, "lrq_kv_append")
 
@@ -282,7 +287,7 @@ class FP8KVCache:
                                 or not out.is_contiguous() or out.data_ptr() % 8):
             raise ValueError(f"{what}: out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {self.device}, 8-byte aligned")
         args = (layer, q, table, ld, lengths, offsets, self.dim ** -0.5 if scale is None else float(scale), window or 0, out, return_lse)
-        if _wants_derivative(q) if out is None else _wants_derivative(q, out):
+        if _wants_derivative(q, q if out is None else out):
             if out is not None:
                 raise RuntimeError(f"{what} has no gradient, backward or forward; pass no out, or a detached q")
             return NoGradient.apply(what, self._attend, *args)
