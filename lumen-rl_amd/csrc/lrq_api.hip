@@ -995,6 +995,7 @@ int lrq_kv_attend(const lrq_kv_cache* cache, int64_t layer, const void* q, int64
   if (heads < 1 || heads > 4096 || heads % cache->kv_heads)
     return fail(LRQ_ERR_ARG, "kv_attend: %lld query heads on %lld KV heads", (long long)heads, (long long)cache->kv_heads);
   if (window < 0) return fail(LRQ_ERR_ARG, "kv_attend: window %lld", (long long)window);
+  if (!(scale >= -0x1p127f && scale <= 0x1p127f)) return fail(LRQ_ERR_ARG, "kv_attend: scale %g (at most 2^127 in size)", (double)scale);
   if (rc > 0) return 0;
   if (!q || !out) return fail(LRQ_ERR_ARG, "kv_attend: null pointer");
   if (!aligned(q, 2) || !aligned(out, 8) || !aligned(lse, 4))

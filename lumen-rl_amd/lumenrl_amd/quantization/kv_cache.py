@@ -35,6 +35,8 @@ from lumenrl_amd.quantization.fp8_product import NoGradient
 from lumenrl_amd.quantization.ops import _IN_DTYPES, _check_input, _current_device, _dense, _on, _stream, require_device
 
 _STRIDE_MAX = 1 << 40
+_WINDOW_MAX = 1 << 31  # more than a sequence can have
+_SCALE_MAX = 2.0 ** 127  # that of float32, in base 2, has an exponent of one more
 
 
 @functools.lru_cache(maxsize=4096)
@@ -278,15 +280,18 @@ class FP8KVCache:
         tokens, heads = q.shape[:2]
         if heads % self.kv_heads or not 1 <= heads <= 4096:
             raise ValueError(f"{what}: {heads} query heads (at most 4096) on {self.kv_heads} KV heads")
-        if window is not None and window < 1:
-            raise ValueError(f"{what}: window must be at least 1, got {window}")
+        if window is not None and (not isinstance(window, int) or window < 1):
+            raise ValueError(f"{what}: window must be a whole number of at least 1, got {window!r}")
+        scale = self.dim ** -0.5 if scale is None else float(scale)
+        if not abs(scale) <= _SCALE_MAX:
+            raise ValueError(f"{what}: scale {scale!r} (at most {_SCALE_MAX:.1e} in size)")
         table, rows, width, ld = self._table(what, table)
         lengths = self._ints(what, "lengths", lengths, (rows,))
         offsets = self._offsets(what, offsets, rows, tokens)
         if out is not None and (not isinstance(out, Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != self.device
                                 or not out.is_contiguous() or out.data_ptr() % 8):
             raise ValueError(f"{what}: out must be a contiguous {tuple(q.shape)} {q.dtype} tensor on {self.device}, 8-byte aligned")
-        args = (layer, q, table, ld, lengths, offsets, self.dim ** -0.5 if scale is None else float(scale), window or 0, out, return_lse)
+        args = (layer, q, table, ld, lengths, offsets, scale, min(window or 0, _WINDOW_MAX), out, return_lse)
         if _wants_derivative(q, q if out is None else out):
             if out is not None:
                 raise RuntimeError(f"{what} has no gradient, backward or forward; pass no out, or a detached q")

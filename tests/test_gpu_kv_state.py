@@ -7,7 +7,7 @@ import torch
 from torch.autograd import forward_ad
 
 import kv_rules as R
-from test_gpu_kv_cache import ints, make, queries
+from test_gpu_kv_cache import close, ints, make, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +93,25 @@ def test_memory_that_is_freed_and_put_back():
     c.attend(0, q, table, lengths)
     with pytest.raises(AttributeError):
         c.k = good
+
+
+@pytest.mark.parametrize("tokens", [1, 400])  # 400: by tiles of many rows
+def test_windows_and_scales_of_any_size(tokens):
+    c = make(1, 40, 1, 64, 16)
+    table, lengths, offsets = ints([list(range(40))]), ints([640]), ints([0, tokens])
+    q = queries(tokens, 4, 64, torch.bfloat16)
+    plain = c.attend(0, q, table, lengths, offsets)
+    for window in (640, 1 << 30, (1 << 31) - 1, 1 << 32, (1 << 32) + 3, 1 << 63, (1 << 64) + 3, 1 << 90):
+        assert torch.equal(c.attend(0, q, table, lengths, offsets, window=window), plain), window
+    for window in (0, -1, -(1 << 64) + 3, 2.5, 64.0, "3"):
+        with pytest.raises(ValueError, match="window"):
+            c.attend(0, q, table, lengths, offsets, window=window)
+    for scale in (float("nan"), float("inf"), -float("inf"), 1e300, -3e38):
+        with pytest.raises(ValueError, match="scale"):
+            c.attend(0, q, table, lengths, offsets, scale=scale)
+    # the sign is the queries', and 0 takes the mean of what is seen
+    want, bound, _ = R.attend(c, 0, -q, table.tolist(), [640], [0, tokens], 0.125, 0)
+    got = c.attend(0, q, table, lengths, offsets, scale=-0.125)
+    close(got, want, bound)
+    want, bound, _ = R.attend(c, 0, q, table.tolist(), [640], [0, tokens], 0.0, 0)
+    close(c.attend(0, q, table, lengths, offsets, scale=0.0), want, bound)

@@ -5,7 +5,7 @@ from __future__ import annotations
 import ctypes
 
 from lumenrl_amd import _lib
-from test_kv_cache_abi import FAKE, append, cache
+from test_kv_cache_abi import FAKE, append, attend, cache
 
 
 def test_append_looks_at_counts_that_are_aligned():
@@ -25,3 +25,9 @@ def test_resize_ready():
     assert resize(ready=ctypes.c_void_p(0xD00002)) == _lib.ERR_ALIGN
     need = _lib.lib().lrq_kv_resize_workspace(3, 10)
     assert resize(ready=ctypes.c_void_p(0xD00000), wb=need - 1) == _lib.ERR_CAPACITY and resize(ws=None) == _lib.ERR_CAPACITY
+
+
+def test_attend_takes_finite_scales():
+    for scale in (float("nan"), float("inf"), -float("inf"), 3e38, -3e38):
+        assert attend(scale=scale) == _lib.ERR_ARG, scale
+    assert attend(tokens=0, scale=2.0 ** 127) == 0 and attend(tokens=0, scale=0.0) == 0
