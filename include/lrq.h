@@ -280,7 +280,8 @@ int lrq_fp8_experts(const void* x, int x_dtype, int64_t tokens, int64_t hidden, 
  * lrq_kv_attend: out [tokens, heads, dim] = softmax(scale q k^T) v for the same rows, each
  *   over its sequence's keys up to its own place, the last `window` of them if that is
  *   above 0; scale is at most 2^127 in size; query head i reads KV head i / (heads / kv_heads).  Scores and sums are
- *   float32, probabilities are rounded to fp16.  A row that sees no key is 0; a NaN is
+ *   float32, probabilities are rounded to fp16.  Scales of the cache are finite, not negative,
+ *   V's are taken within 2^-48 .. 2^48.  A row that sees no key is 0; a NaN is
  *   in the results of the rows that see it alone.  lse: [tokens, heads], the scores' log-sum-exp
  *   (natural), or null.  Rows of no sequence (before offsets[0], behind offsets[seqs]) stay
  *   as they were, or become 0 (lse: -inf) with zero_rest.  q is bf16 or fp16, out of its

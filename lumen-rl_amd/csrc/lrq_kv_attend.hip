@@ -14,7 +14,10 @@
 //   o 2^M = sum_j 2^(s_j + e_j - M) code_j,   l 2^M = sum_j 2^(s_j + e_j - M) 2^-e_j,
 // M the running maximum of s + e.  So p has 11 bits and a range of 2^-34 below the
 // largest term (it is taken 2^10 times as large, and fp16's subnormals count), where bf16
-// would have 8 bits: its rounding is then far below that of a 16-bit result.
+// would have 8 bits: its rounding is then far below that of a 16-bit result.  l takes p before
+// that rounding: a key of a page whose V is far smaller than others' has a p far below fp16's
+// range, and yet its part of l.  That part is in float32's range as long as V's scales are no
+// further than 2^96 apart: they are taken within 2^-48 .. 2^48.
 //
 // Layout: both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, on 16x16x32
 // instructions.  Lane l holds of every result the column l % 16, a row of queries, and so

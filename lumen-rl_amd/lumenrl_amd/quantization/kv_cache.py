@@ -93,10 +93,15 @@ class FP8KVCache:
     kv_heads] float32, ``refs`` [pages] int32: how many rows of the caller's table hold
     each page; it is free where none does.  ``page`` is 16, 32, 64, 128 or 256, ``dim`` a multiple
     of 16 up to 256.  The tensors are kept and written in place; layers and pages may be
-    views of larger ones, what a page holds is dense.  Their memory may be freed and put
-    back between calls (``untyped_storage().resize_``, ``.data =``), shapes and strides staying as
-    they are: each call looks where the tensors are, and raises where one has no memory, or too
-    little; a captured graph keeps the places of its capture.
+    views of larger ones, what a page holds is dense.
+
+    A caller's own scales may be any finite numbers that are not negative; ``attend`` takes V's
+    within 2^-48 to 2^48, which ``append`` does not leave, and others as the nearest of these.
+
+    The tensors' memory may be freed and put back between calls (``untyped_storage().resize_``,
+    ``.data =``), shapes and strides staying as they are: each call looks where the tensors
+    are, and raises where one has no memory, or too little; a captured graph keeps the
+    places of its capture.
     """
 
     def __init__(self, k: Tensor, v: Tensor, k_scales: Tensor, v_scales: Tensor, refs: Tensor) -> None:

@@ -115,3 +115,40 @@ def test_windows_and_scales_of_any_size(tokens):
     close(got, want, bound)
     want, bound, _ = R.attend(c, 0, q, table.tolist(), [640], [0, tokens], 0.0, 0)
     close(c.attend(0, q, table, lengths, offsets, scale=0.0), want, bound)
+
+
+@pytest.mark.parametrize("page,dim,tokens", [(64, 128, 3), (16, 80, 3), (64, 128, 300), (32, 80, 300)])  # few rows and tiles, a page or less a unit
+@pytest.mark.parametrize("kind", ["any", "large", "small", "range"])
+def test_scales_of_a_callers_own(page, dim, tokens, kind):
+    """Scales that are no powers of two, V's over all of the range in which they are taken; beyond it they are the nearest in it.
+
+    Beside what the bound holds already, log2 of a scale and 2^ of it are approximate: 2^-22 of an exponent of up to 64, 2^-16 ln 2."""
+    keys = 700
+    pool = R.pages_of(keys, page) + 1
+    c = make(1, pool, 1, dim, page, spread=0)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    c.k_scales.copy_(0.004 + 0.006 * torch.rand(c.k_scales.shape, generator=g, device="cuda"))
+    spread = torch.rand(c.v_scales.shape, generator=g, device="cuda", dtype=torch.float64)
+    c.v_scales.copy_({"any": 0.01 + spread, "large": 2.0 ** (40 + 8 * spread), "small": 2.0 ** (-48 + 8 * spread),
+                       "range": 2.0 ** (-48 + 96 * spread)}[kind])
+    table = R.spread_table([keys], page, pool, pool, 2)
+    q = queries(tokens, 4, dim, torch.bfloat16)
+    out, lse = c.attend(0, q, ints(table), ints([keys]), ints([0, tokens]), return_lse=True)
+    want, bound, wl = R.attend(c, 0, q, table, [keys], [0, tokens], dim ** -0.5, 0)
+    size, _, _ = R.attend(_sizes(c), 0, q, table, [keys], [0, tokens], dim ** -0.5, 0)
+    close(out, want, bound - 2.0 ** -32 + 2.0 ** -134 + 2.0 ** -16 * size)  # (half a step of the smallest number is fp16's there, bf16's here)
+    assert bool(((lse.double() - wl).abs() <= 1e-4 + 2e-6 * wl.abs()).all())
+    p = table[0]
+    for inside, beyond in ((2.0 ** 48, 2.0 ** 90), (2.0 ** -48, 2.0 ** -100), (2.0 ** -48, 0.0)):
+        c.v_scales[0, p[1]] = c.v_scales[0, p[2]] = inside
+        want = c.attend(0, q, ints(table), ints([keys]), ints([0, tokens]))
+        c.v_scales[0, p[1]] = c.v_scales[0, p[2]] = beyond
+        assert torch.equal(c.attend(0, q, ints(table), ints([keys]), ints([0, tokens])), want), beyond
+
+
+class _sizes:
+    """A cache whose values are their sizes."""
+
+    def __init__(self, c):
+        self.__dict__.update({n: getattr(c, n) for n in ("k", "k_scales", "v_scales", "kv_heads", "page", "pages")})
+        self.v = c.v.float().abs()
