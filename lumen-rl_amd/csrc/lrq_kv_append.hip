@@ -11,7 +11,7 @@
 // have a page of its own (a full pool) is to lose its new tokens and no one's old ones.
 //
 // Bound by its bytes: a page and head of 64 tokens reads 32 KiB (bf16) and writes 16.  32 prompts
-// of 33 to 1500 tokens on 8 heads of 128 (154 MB) take 35 us, 4.4 TB/s (a copy: 4.7).  A page's
+// of 33 to 1500 tokens on 8 heads of 128 (154 MB) take 35 us, 4.4 TB/s (moved pages: 5.2).  A page's
 // values are read once, into registers, where both passes (the maximum, the codes) find them.
 // V is turned round on its way: codes go through LDS as words of four channels, and come out
 // as eight tokens of four channels, whose bytes are exchanged in registers.

@@ -2,8 +2,8 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c (q . k_j) - m),   c = scale log2(e),
 // with m the running maximum of a row, in one pass over the keys.  A row is a new token
-// and one of its query heads; the rows that share a KV head are taken together, 16 a
-// work-group, so that each code is read once for all of them.  Bound by the codes' bytes:
+// and one of its query heads; the rows that share a KV head are taken together, 16 or 32 a
+// wave, so that each code is read once for all of them.  Bound by the codes' bytes:
 // 256 sequences of up to 8100 keys on 8 heads of 128 (2.1 GB) take 392 us, 5.4 TB/s, where a
 // read of as much and nothing else reaches 6.2; one of 1500 keys 13 us, two launches' latency.
 //
@@ -26,9 +26,12 @@
 // keys whose V codes it loads with one 16-byte load, in its order, and P never leaves the
 // registers.
 //
-// This kernel is for few rows a sequence, where the codes' bytes are all there is.  Its
-// waves work each for itself, with no LDS and no barrier: a wave's next 64 keys are on
-// their way into registers while it works on the present ones.
+// This kernel is for few rows a sequence, where the codes' bytes are all there is.  The four
+// waves of a work-group look for their pieces of work together, by sums over the work-group; then
+// each works for itself: its loop over the keys has no barrier and no LDS, the next 64 keys
+// are on their way into registers while it works on the present ones.  LDS (16 KiB for each 64
+// channels of 16 rows, up to 64 KiB a work-group) holds the sums where NaN codes that only
+// some rows see are worked on; registers, not it, bound the waves of a compute unit.
 #include "lrq_kv.hpp"
 #include "lrq_kv_attend.hpp"
 
@@ -196,7 +199,8 @@ __global__ __launch_bounds__(1024) void k_kv_count(KvAttendArgs a, uint32_t limi
 
 // FAST: heads of 64 NC channels and pages of 64 keys, which are the constants of the
 // addresses then, and a page is one for the whole wave (16, 32 and 64 rows on 4000 keys, 32
-// times, 66, 82 and 104 us; without it 78, 102 and 152).
+// times, 66, 82 and 104 us; without it 78, 102 and 152, and spills of 26 to 117 scalar registers and
+// up to 4 vector ones).
 template <int DT, int NC, int MT, bool FAST>
 __global__ __launch_bounds__(64 * kWaves, (kPerSimd<NC, MT>)) void k_kv_attend(KvAttendArgs a) {
   constexpr int NT = 4 * NC;       // tiles of 16 channels

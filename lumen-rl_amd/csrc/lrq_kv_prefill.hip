@@ -1,6 +1,7 @@
 // Attention of many new tokens a sequence on an FP8 KV cache (lrq_kv_attend.hip has the
 // formulas, and the kernel for few).  Bound by instructions: 4 prompts of 3500 to 4096 tokens, 32
-// heads on 4 of 128 channels, take 570 us (850 TFLOP/s), the matrix units busy for 39 % of the
+// heads on 4 of 128 channels, take 560 to 575 us (850 TFLOP/s) once the clock has settled (650 us in
+// the first twenty calls, 562 from the eightieth on), the matrix units busy for 39 % of the
 // cycles and the other vector instructions (exponentials, widening) for 50 %.
 //
 // A work-group takes 128 rows (tokens times the query heads of one KV head), 32 a wave,
