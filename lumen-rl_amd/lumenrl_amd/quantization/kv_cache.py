@@ -78,6 +78,16 @@ def _places(parts: tuple) -> list:
     return [*map(Tensor.data_ptr, parts), *map(UntypedStorage.nbytes, map(Tensor.untyped_storage, parts))]
 
 
+def _part(i: int) -> property:
+    """One of a cache's tensors: to be written to (``cache.refs += 1`` too), not to be replaced."""
+
+    def keep(self, x: Tensor) -> None:
+        if x is not self._parts[i]:
+            raise AttributeError("FP8KVCache: its tensors cannot be replaced; make another cache of the new ones")
+
+    return property(lambda self: self._parts[i], keep)
+
+
 def _wants_derivative(x: Tensor, y: Tensor) -> bool:
     """Whether one of them is to be differentiated, backward or forward."""
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, y)):
@@ -108,11 +118,7 @@ class FP8KVCache:
         self._parts = (k, v, k_scales, v_scales, refs)
         self._describe()
 
-    k = property(lambda self: self._parts[0])
-    v = property(lambda self: self._parts[1])
-    k_scales = property(lambda self: self._parts[2])
-    v_scales = property(lambda self: self._parts[3])
-    refs = property(lambda self: self._parts[4])
+    k, v, k_scales, v_scales, refs = (_part(i) for i in range(5))
 
     def _describe(self) -> None:
         """Checks the tensors, and notes where they are for the kernels."""
@@ -225,14 +231,14 @@ class FP8KVCache:
 
         Rows ``offsets[b]`` .. ``offsets[b + 1] - 1`` (int32 [rows + 1]) are the last
         tokens of sequence b, whose ``lengths[b]`` counts them in already (``resize``'s ``ready``,
-        where rows may have been refused); without ``offsets`` each sequence has one, and rows behind the last belong to none.  A
-        page's scale is the least power of two, from 2^-48 to 2^48, that takes the
-        largest finite magnitude to 448 at most.  Tokens that join a page never make its
-        scale smaller; where they make it larger, the codes that are there are rounded to
-        it again.  Infinities and NaN become NaN codes.  Tokens whose place has no page in
-        the table, or one that ``refs`` counts for more than one row, are not written: what
-        other rows see is not changed.  No gradient: keys or values that want one, backward
-        or forward, are refused.
+        where rows may have been refused); without ``offsets`` each sequence has one, and rows
+        behind the last belong to none.  A page's scale is the least power of two, from 2^-48
+        to 2^48, that takes the largest finite magnitude to 448 at most.  Tokens that join a
+        page never make its scale smaller; where they make it larger, the codes that are there
+        are rounded to it again.  Infinities and NaN become NaN codes.  Tokens whose place has
+        no page in the table, or one that ``refs`` counts for more than one row, are not
+        written: what other rows see is not changed.  No gradient: keys or values that want
+        one, backward or forward, are refused.
         """
         what = "FP8KVCache.append"
         self._look()

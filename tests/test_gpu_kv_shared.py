@@ -2,12 +2,14 @@
 
 from __future__ import annotations
 
+import ctypes
 import random
 
 import pytest
 import torch
 
 import kv_rules as R
+from lumenrl_amd import _lib
 from test_gpu_kv_cache import DEV, close, ints, make, queries
 
 pytestmark = pytest.mark.gpu
@@ -62,6 +64,23 @@ def test_a_shared_page_is_not_written(dtype, page, kv, dim):
     want.append(1, k[:1], v[:1], table[:1], [12], None)
     want.same(c)
     assert not torch.equal(was[0], c.k.view(torch.uint8)[:, 4])
+
+
+def test_a_cache_without_counts():
+    """The C entry without refs has no shared pages."""
+    c = make(1, 3, 1, 64, 16)
+    c.refs.fill_(2)
+    want = R.Cache(c)
+    k = tokens(3, 1, 64, torch.bfloat16, 1)
+    t, n, offsets = ints([[1], [2]]), ints([4, 9]), ints([0, 1, 3])
+    desc = _lib.LrqKvCache.from_buffer_copy(c._desc)
+    desc.refs = None
+    for where in (offsets, None):
+        rc = _lib.lib().lrq_kv_append(ctypes.byref(desc), 0, k.data_ptr(), 64, 64, k.data_ptr(), 64, 64, 0, 3, t.data_ptr(), 1, 1, n.data_ptr(),
+                                      None if where is None else where.data_ptr(), 2, None, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        want.append(0, k, k, t.tolist(), n.tolist(), None if where is None else where.tolist())
+        want.same(c)
 
 
 def test_a_shared_page_is_not_written_among_many_sequences():

@@ -152,3 +152,15 @@ class _sizes:
     def __init__(self, c):
         self.__dict__.update({n: getattr(c, n) for n in ("k", "k_scales", "v_scales", "kv_heads", "page", "pages")})
         self.v = c.v.float().abs()
+
+
+def test_a_caches_tensors_are_written_in_place():
+    c = make(1, 4, 1, 64, 16)
+    refs, scales = c.refs, c.k_scales.clone()
+    c.refs += 1
+    c.k_scales *= 2
+    assert c.refs is refs and c.refs.tolist() == [1] * 4 and torch.equal(c.k_scales, scales * 2)
+    for name in ("k", "v", "k_scales", "v_scales", "refs"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name).clone())
+    assert c.refs is refs
